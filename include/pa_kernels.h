@@ -144,6 +144,87 @@ int pa_attn_bwd_noalloc(const pa_attn_desc* desc, const void* q, const void* k, 
 int pa_attn_delta(const pa_attn_desc* desc, const void* dO, const void* o, float* delta,
                   pa_stream_t stream);
 
+/* ---------------------------------------------------------------- rotary positions
+ * Not in the reference, whose attention has no positions. Pair i of a head
+ * (i < P = sum of the sections, 2 P <= head_dim) turns by the angle
+ * position[axis(i)] * base^-f(i): the first sections[0] pairs follow axis 0, the
+ * next sections[1] axis 1, and so on (one axis: a token's index in a text;
+ * several: time, height and width of an image or video token). Values from
+ * 2 P on are copied. Angles are taken in 64 bits, so far positions keep fp32
+ * accuracy. */
+#define PA_ROPE_MAX_AXES 4
+typedef enum pa_rope_layout {
+  PA_ROPE_HALVES = 0, /* pair i = values i and P + i */
+  PA_ROPE_PAIRS = 1   /* pair i = values 2 i and 2 i + 1 */
+} pa_rope_layout;
+typedef enum pa_rope_freqs {
+  PA_ROPE_SHARED = 0,  /* f(i) = i / P: one range of frequencies over all axes */
+  PA_ROPE_PER_AXIS = 1 /* f = (index within its section) / section: each axis its own range */
+} pa_rope_freqs;
+typedef struct pa_rope_desc {
+  int32_t batch;        /* B */
+  int32_t seq_len;      /* L */
+  int32_t num_heads;    /* heads of q */
+  int32_t num_kv_heads; /* heads of k; 0: there is no k */
+  int32_t head_dim;     /* at most 256 */
+  int32_t dtype;        /* pa_dtype of q and k */
+  int32_t layout;       /* pa_rope_layout */
+  int32_t freqs;        /* pa_rope_freqs */
+  int32_t axes;         /* 1 .. PA_ROPE_MAX_AXES */
+  int32_t sections[PA_ROPE_MAX_AXES]; /* pairs of each axis, at least 1 for each of `axes` */
+  double base;          /* > 1, e.g. 10000 */
+} pa_rope_desc;
+
+/* q_out = turn(q) [B, L, num_heads, D], k_out = turn(k) [B, L, num_kv_heads, D];
+ * positions is a device array [axes, B, L] of any int32 values. q_out may be q
+ * and k_out k (in place); other overlaps are not allowed. */
+int pa_rope_fwd(const pa_rope_desc* desc, const void* q, const void* k, const int32_t* positions,
+                void* q_out, void* k_out, pa_stream_t stream);
+/* Its adjoint, the turn by the negative angles: dq (overwritten, or added to
+ * when accumulate != 0) from the gradient dq_out of q_out, dk from dk_out. In
+ * place only when accumulate is 0. */
+int pa_rope_bwd(const pa_rope_desc* desc, const void* dq_out, const void* dk_out,
+                const int32_t* positions, void* dq, void* dk, int accumulate, pa_stream_t stream);
+
+/* ---------------------------------------------------------------- linear attention
+ * Causal linear attention with a decay per head; not in the reference. With
+ * l = exp(log_decay[h]) and S a [D, D] state per sequence and head,
+ *   S_t = l S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t,
+ * i.e. o_t = scale (sum_{s <= t} l^(t-s) (q_t . k_s) v_s + l^(t+1) q_t S_0).
+ * The cost grows with the tokens, not with their square, and one [D, D] state
+ * replaces a cache of keys and values. desc as for pa_attn_fwd (softmax_scale is
+ * the scale; bf16 with head_dim 64 or 128, fp32 with 32 or 64, fp32 products under
+ * the calling thread's f32 math mode); log_decay: device [H], usually <= 0 (-inf: each
+ * token sees itself alone), a constant without a gradient. seq_lens: device [B], valid
+ * tokens of each sequence, clamped to 0 .. seq_len; NULL: all. What q, k, v, dO hold past
+ * them is not used (NaN allowed) and o, dq, dk, dv are zero there (left as they
+ * were by accumulate). States are [B, H, D, D] fp32 in every dtype: state_in
+ * NULL starts from zero; state_out (NULL: not wanted) is the state after the
+ * last valid token and may be state_in. Results do not depend on the run: no
+ * atomics. */
+size_t pa_linear_attn_fwd_workspace_size(const pa_attn_desc* desc);
+int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const float* log_decay, const int32_t* seq_lens, const float* state_in,
+                       void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                       pa_stream_t stream);
+
+/* Gradients from dO and d_state_out (the gradient of state_out; NULL: zero):
+ * dq, dk, dv (overwritten, or added to when accumulate != 0) and d_state_in
+ * (overwritten; NULL: not wanted; may be d_state_out). state_in: as in the forward. */
+size_t pa_linear_attn_bwd_workspace_size(const pa_attn_desc* desc);
+int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const void* dO, const float* log_decay, const int32_t* seq_lens,
+                       const float* state_in, const float* d_state_out, void* dq, void* dk,
+                       void* dv, float* d_state_in, int accumulate, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream);
+
+/* One new token per sequence (desc->seq_len is 1; q, k, v, o [B, 1, H, D]):
+ * state_out = l state_in + k v^T, o = scale q state_out. state_out may be
+ * state_in (the usual in-place update); neither may be NULL. */
+int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                        const float* log_decay, const float* state_in, void* o, float* state_out,
+                        pa_stream_t stream);
+
 /* ---------------------------------------------------------------- layer norm */
 
 /* y = gamma * (x - mean) * rstd + beta over rows of length N; saves mean, rstd.

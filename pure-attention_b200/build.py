@@ -30,6 +30,8 @@ KERNEL_SOURCES = [
     "elementwise.cu",
     "gemm.cu",
     "training.cu",
+    "rope.cu",
+    "linear_attn.cu",
     "capi.cu",
     "attn_bwd_noalloc.cu",
 ]

@@ -214,6 +214,165 @@ int pa_attn_delta(const pa_attn_desc* desc, const void* dO, const void* o, float
 
 }  // extern "C"
 
+// ------------------------------------------------------------------ rotary positions, linear attention
+namespace {
+// Validates a rope descriptor and the pointers of one call; fills `sh`.
+int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_t* positions,
+               const void* qo, const void* ko, pa::RopeShape* sh) {
+  if (!d) return PA_ERR_NULL;
+  if (d->batch <= 0 || d->seq_len <= 0 || d->num_heads <= 0 || d->num_kv_heads < 0 ||
+      d->head_dim <= 0 || d->axes < 1 || d->axes > PA_ROPE_MAX_AXES)
+    return PA_ERR_SHAPE;
+  if (d->dtype != PA_BF16 && d->dtype != PA_F32) return PA_ERR_DTYPE;
+  if (d->head_dim > 256) return PA_ERR_UNSUPPORTED;
+  if ((d->layout != PA_ROPE_HALVES && d->layout != PA_ROPE_PAIRS) ||
+      (d->freqs != PA_ROPE_SHARED && d->freqs != PA_ROPE_PER_AXIS))
+    return PA_ERR_UNSUPPORTED;
+  if (!(d->base > 1.0) || !std::isfinite(d->base)) return PA_ERR_SHAPE;
+  int pairs = 0;
+  for (int a = 0; a < d->axes; ++a) {
+    if (d->sections[a] < 1 || d->sections[a] > 128) return PA_ERR_SHAPE;
+    pairs += d->sections[a];
+    sh->sections[a] = d->sections[a];
+  }
+  if (2 * pairs > d->head_dim) return PA_ERR_SHAPE;
+  const long long tokens = static_cast<long long>(d->batch) * d->seq_len;
+  // the kernel's items of one token block and its grid are ints
+  if (tokens > 0x7fffffffLL ||
+      (static_cast<long long>(d->num_heads) + d->num_kv_heads) * d->head_dim * 8 > 0x7fffffffLL)
+    return PA_ERR_SHAPE;
+  if (!q || !qo || !positions || (d->num_kv_heads > 0 && (!k || !ko))) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(qo) || (d->num_kv_heads > 0 && (!aligned16(k) || !aligned16(ko))))
+    return PA_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0) return PA_ERR_ALIGN;
+  sh->B = d->batch;
+  sh->L = d->seq_len;
+  sh->Hq = d->num_heads;
+  sh->Hk = d->num_kv_heads;
+  sh->D = d->head_dim;
+  sh->axes = d->axes;
+  sh->pairs = pairs;
+  sh->f32 = d->dtype == PA_F32;
+  sh->halves = d->layout == PA_ROPE_HALVES;
+  sh->per_axis = d->freqs == PA_ROPE_PER_AXIS;
+  sh->base = d->base;
+  return PA_OK;
+}
+
+bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
+
+size_t linear_attn_workspace(const pa_attn_desc* desc, bool backward) {
+  pa::AttnShape sh;
+  if (check_attn(desc, &sh) != PA_OK) return 0;
+  return pa::linear_attn_workspace_bytes(sh, desc->dtype == PA_F32, backward);
+}
+
+int check_linear_attn_ws(const pa_attn_desc* desc, bool backward, const void* ws, size_t bytes) {
+  const size_t need = linear_attn_workspace(desc, backward);
+  if (need == 0) return PA_OK;
+  if (!ws || bytes < need) return PA_ERR_WORKSPACE;
+  return (reinterpret_cast<uintptr_t>(ws) & 255u) == 0 ? PA_OK : PA_ERR_ALIGN;
+}
+}  // namespace
+
+extern "C" {
+
+int pa_rope_fwd(const pa_rope_desc* desc, const void* q, const void* k, const int32_t* positions,
+                void* q_out, void* k_out, pa_stream_t stream) {
+  pa::RopeShape sh;
+  const int st = check_rope(desc, q, k, positions, q_out, k_out, &sh);
+  if (st != PA_OK) return st;
+  return pa::launch_rope(sh, q, k, q_out, k_out, positions, false, false,
+                         static_cast<cudaStream_t>(stream));
+}
+
+int pa_rope_bwd(const pa_rope_desc* desc, const void* dq_out, const void* dk_out,
+                const int32_t* positions, void* dq, void* dk, int accumulate, pa_stream_t stream) {
+  pa::RopeShape sh;
+  const int st = check_rope(desc, dq_out, dk_out, positions, dq, dk, &sh);
+  if (st != PA_OK) return st;
+  if (accumulate && (dq_out == dq || (desc->num_kv_heads > 0 && dk_out == dk))) return PA_ERR_SHAPE;
+  return pa::launch_rope(sh, dq_out, dk_out, dq, dk, positions, true, accumulate != 0,
+                         static_cast<cudaStream_t>(stream));
+}
+
+size_t pa_linear_attn_fwd_workspace_size(const pa_attn_desc* desc) {
+  return linear_attn_workspace(desc, false);
+}
+
+int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const float* log_decay, const int32_t* seq_lens, const float* state_in,
+                       void* o, float* state_out, void* workspace, size_t workspace_bytes,
+                       pa_stream_t stream) {
+  pa::AttnShape sh;
+  int st = check_attn(desc, &sh);
+  if (st != PA_OK) return st;
+  if (!q || !k || !v || !log_decay || !o) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(log_decay) ||
+      !aligned4(seq_lens) || !aligned16(state_in) || !aligned16(state_out))
+    return PA_ERR_ALIGN;
+  if (o == q || o == k || o == v) return PA_ERR_SHAPE;
+  st = check_linear_attn_ws(desc, false, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  uint32_t* status = status_word();
+  if (!status) return PA_ERR_DEVICE;
+  return pa::launch_linear_attn_fwd(sh, desc->dtype == PA_F32, q, k, v, log_decay, seq_lens, state_in,
+                                    o, state_out, workspace, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t pa_linear_attn_bwd_workspace_size(const pa_attn_desc* desc) {
+  return linear_attn_workspace(desc, true);
+}
+
+int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const void* dO, const float* log_decay, const int32_t* seq_lens,
+                       const float* state_in, const float* d_state_out, void* dq, void* dk,
+                       void* dv, float* d_state_in, int accumulate, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream) {
+  pa::AttnShape sh;
+  int st = check_attn(desc, &sh);
+  if (st != PA_OK) return st;
+  if (!q || !k || !v || !dO || !log_decay || !dq || !dk || !dv) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(dO) || !aligned16(dq) ||
+      !aligned16(dk) || !aligned16(dv) || !aligned4(log_decay) || !aligned4(seq_lens) ||
+      !aligned16(state_in) || !aligned16(d_state_out) || !aligned16(d_state_in))
+    return PA_ERR_ALIGN;
+  // the three gradients are written while the inputs are still read
+  const void* in[4] = {q, k, v, dO};
+  const void* out[3] = {dq, dk, dv};
+  for (int i = 0; i < 3; ++i) {
+    for (const void* p : in)
+      if (out[i] == p) return PA_ERR_SHAPE;
+    if (out[i] == out[(i + 1) % 3]) return PA_ERR_SHAPE;
+  }
+  if (d_state_in && d_state_in == state_in) return PA_ERR_SHAPE;
+  st = check_linear_attn_ws(desc, true, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  uint32_t* status = status_word();
+  if (!status) return PA_ERR_DEVICE;
+  return pa::launch_linear_attn_bwd(sh, desc->dtype == PA_F32, q, k, v, dO, log_decay, seq_lens,
+                                    state_in, d_state_out, dq, dk, dv, d_state_in, accumulate != 0,
+                                    workspace, status, static_cast<cudaStream_t>(stream));
+}
+
+int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
+                        const float* log_decay, const float* state_in, void* o, float* state_out,
+                        pa_stream_t stream) {
+  pa::AttnShape sh;
+  const int st = check_attn(desc, &sh);
+  if (st != PA_OK) return st;
+  if (sh.L != 1) return PA_ERR_SHAPE;
+  if (!q || !k || !v || !log_decay || !state_in || !o || !state_out) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(log_decay) ||
+      !aligned16(state_in) || !aligned16(state_out))
+    return PA_ERR_ALIGN;
+  if (o == q || o == k || o == v) return PA_ERR_SHAPE;
+  return pa::launch_linear_attn_step(sh, desc->dtype == PA_F32, q, k, v, log_decay, state_in, o,
+                                     state_out, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
 // ------------------------------------------------------------------ layer norm, matmul, elementwise
 namespace {
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

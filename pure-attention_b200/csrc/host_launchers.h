@@ -129,3 +129,41 @@ int launch_fill_normal(float* x, size_t n, float std_dev, uint64_t seed, cudaStr
 int launch_fill(float* x, size_t n, float value, cudaStream_t s);
 
 }  // namespace pa
+
+namespace pa {
+
+// rope.cu
+struct RopeShape {
+  int B, L, Hq, Hk, D;       // Hk = 0: no k tensor
+  int axes, sections[4], pairs;  // pairs = sum of the sections
+  bool f32, halves, per_axis;
+  double base;
+};
+// positions [axes, B, L]; inverse: turn by the negative angle; accumulate: add
+// to the outputs.
+int launch_rope(const RopeShape& sh, const void* q, const void* k, void* qo, void* ko,
+                const int32_t* positions, bool inverse, bool accumulate, cudaStream_t s);
+
+// linear_attn.cu. How one direction of the recurrence walks the tokens and
+// takes and gives its state.
+struct MixDir {
+  bool reverse = false;     // last valid token first
+  bool transposed = false;  // the caller's state is the transpose
+  bool accumulate = false;  // add to the output
+  int lead = 0;             // 1: the carried state enters the first token undecayed
+                            // and leaves with one more decay (gradients of a state)
+  float in_mult = 1.f, out_mult = 1.f;  // factors of the state taken and given
+};
+size_t linear_attn_workspace_bytes(const AttnShape& sh, bool f32, bool backward);
+int launch_linear_attn_fwd(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,
+                           const float* log_decay, const int32_t* lens, const float* s_in, void* o,
+                           float* s_out, void* ws, uint32_t* status, cudaStream_t s);
+int launch_linear_attn_bwd(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,
+                           const void* dO, const float* log_decay, const int32_t* lens,
+                           const float* s_in, const float* ds_out, void* dq, void* dk, void* dv,
+                           float* ds_in, bool accumulate, void* ws, uint32_t* status, cudaStream_t s);
+int launch_linear_attn_step(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,
+                            const float* log_decay, const float* s_in, void* o, float* s_out,
+                            cudaStream_t s);
+
+}  // namespace pa

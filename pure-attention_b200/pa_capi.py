@@ -25,6 +25,8 @@ EXPORTS = [
     "pa_get_f32_math",
     "pa_attn_fwd_workspace_size", "pa_attn_fwd", "pa_attn_bwd_workspace_size", "pa_attn_bwd", "pa_attn_bwd_kept", "pa_attn_bwd_noalloc",
     "pa_attn_delta",
+    "pa_rope_fwd", "pa_rope_bwd", "pa_linear_attn_fwd_workspace_size", "pa_linear_attn_fwd",
+    "pa_linear_attn_bwd_workspace_size", "pa_linear_attn_bwd", "pa_linear_attn_step",
     "pa_layer_norm_fwd", "pa_add_layer_norm_fwd", "pa_layer_norm_fwd_planes", "pa_layer_norm_bwd_workspace_size", "pa_layer_norm_bwd",
     "pa_layer_norm_bwd_accumulate", "pa_add_layer_norm_bwd",
     "pa_matmul_workspace_size", "pa_matmul", "pa_matmul_grad_x", "pa_matmul_grad_w",
@@ -49,6 +51,14 @@ class AttnDesc(ctypes.Structure):
                 ("dtype", ctypes.c_int32), ("softmax_scale", ctypes.c_float)]
 
 
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int32), ("seq_len", ctypes.c_int32),
+                ("num_heads", ctypes.c_int32), ("num_kv_heads", ctypes.c_int32),
+                ("head_dim", ctypes.c_int32), ("dtype", ctypes.c_int32),
+                ("layout", ctypes.c_int32), ("freqs", ctypes.c_int32), ("axes", ctypes.c_int32),
+                ("sections", ctypes.c_int32 * 4), ("base", ctypes.c_double)]
+
+
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _u32 = ctypes.c_uint32
@@ -69,6 +79,13 @@ _SIGS = {
     "pa_attn_bwd_kept": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 9 + [_int, _vp, _sz, _int, _vp, _sz, _vp]),
     "pa_attn_bwd_noalloc": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 9 + [_int, _vp]),
     "pa_attn_delta": (_int, [ctypes.POINTER(AttnDesc), _vp, _vp, _vp, _vp]),
+    "pa_rope_fwd": (_int, [ctypes.POINTER(RopeDesc)] + [_vp] * 6),
+    "pa_rope_bwd": (_int, [ctypes.POINTER(RopeDesc)] + [_vp] * 5 + [_int, _vp]),
+    "pa_linear_attn_fwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
+    "pa_linear_attn_fwd": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 9 + [_sz, _vp]),
+    "pa_linear_attn_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
+    "pa_linear_attn_bwd": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 12 + [_int, _vp, _sz, _vp]),
+    "pa_linear_attn_step": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 8),
     "pa_layer_norm_fwd": (_int, [_vp] * 6 + [_u32, _u32, _flt, _vp]),
     "pa_add_layer_norm_fwd": (_int, [_vp] * 8 + [_u32, _u32, _flt, _vp]),
     "pa_layer_norm_fwd_planes": (_int, [_vp] * 8 + [_u32, _u32, _flt, _vp, _sz, _vp]),
@@ -245,6 +262,137 @@ def attn_delta(dO, o, delta, desc=None, stream=None):
     st = load().pa_attn_delta(ctypes.byref(d), _ptr(dO), _ptr(o), _ptr(delta),
                               _stream() if stream is None else stream)
     _check("pa_attn_delta", st)
+
+
+def _check_tensors(fn, dev, dtype, shape, names, *tensors):
+    """Each tensor (None: skipped) has this type and shape, is contiguous and on CUDA device `dev`:
+    a call with any other would read past its memory."""
+    for name, t in zip(names, tensors):
+        if t is None:
+            continue
+        if t.dtype is not dtype or t.shape != shape:
+            raise ValueError(f"{fn}: {name} must be {dtype} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+        if not t.is_contiguous():
+            raise ValueError(f"{fn}: {name} must be contiguous")
+        if t.get_device() != dev:
+            raise ValueError(f"{fn}: {name} must be on the first tensor's device, not {t.device}")
+
+
+def _check_device(fn, t):
+    """The kernels run on the current device's stream."""
+    import torch
+    if t.get_device() < 0 or t.get_device() != torch.cuda.current_device():
+        raise ValueError(f"{fn}: tensors must be on the current CUDA device, not {t.device}")
+
+
+ROPE_LAYOUT = {"halves": 0, "pairs": 1}
+ROPE_FREQS = {"shared": 0, "per_axis": 1}
+
+
+def rope_desc(q, k=None, sections=None, base=10000.0, layout="halves", freqs="shared"):
+    """Descriptor of the rotary positions of q [B, L, H, D] and k [B, L, Hk, D] (or None).
+    sections: pairs turned by each position axis (None: one axis over the whole head);
+    layout: "halves" or "pairs"; freqs: "shared" or "per_axis" (include/pa_kernels.h)."""
+    B, L, H, D = q.shape
+    sections = [D // 2] if sections is None else list(sections)
+    if len(sections) > 4:
+        raise ValueError("rope_desc: at most 4 position axes")
+    return RopeDesc(B, L, H, 0 if k is None else k.shape[2], D, _dtype_code(q), ROPE_LAYOUT[layout],
+                    ROPE_FREQS[freqs], len(sections), (ctypes.c_int32 * 4)(*sections), float(base))
+
+
+def _rope(name, q, k, positions, q_out, k_out, desc, *accumulate, stream=None):
+    import torch
+    d = desc
+    t, dev = torch.float32 if d.dtype == PA_F32 else torch.bfloat16, q.get_device()
+    if (k is None) != (d.num_kv_heads == 0) or (k is None) != (k_out is None):
+        raise ValueError(f"{name}: k and its output go with the descriptor's kv heads")
+    _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_heads, d.head_dim), ("q", "q_out"), q, q_out)
+    _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_kv_heads, d.head_dim), ("k", "k_out"), k, k_out)
+    _check_tensors(name, dev, torch.int32, (d.axes, d.batch, d.seq_len), ("positions",), positions)
+    _check_device(name, q)
+    _check(name, getattr(load(), name)(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(positions), _ptr(q_out),
+                                       _ptr(k_out), *accumulate, _stream() if stream is None else stream))
+
+
+def rope_fwd(q, k, positions, q_out, k_out, desc, stream=None):
+    """q_out = turn(q), k_out = turn(k) by positions (int32 [axes, B, L]); k and k_out may be
+    None, and the outputs may be the inputs."""
+    _rope("pa_rope_fwd", q, k, positions, q_out, k_out, desc, stream=stream)
+
+
+def rope_bwd(dq_out, dk_out, positions, dq, dk, desc, accumulate=False, stream=None):
+    """Gradients of rope_fwd's inputs from those of its outputs (overwritten, or added to)."""
+    _rope("pa_rope_bwd", dq_out, dk_out, positions, dq, dk, desc, int(bool(accumulate)), stream=stream)
+
+
+def _check_linear_attn(fn, q, log_decay, seq_lens, names, tensors, states):
+    import torch
+    if q.dim() != 4:
+        raise ValueError(f"{fn}: q must be [B, L, H, D]")
+    B, L, H, D = q.shape
+    dev = q.get_device()
+    _check_tensors(fn, dev, q.dtype, q.shape, names, *tensors)
+    _check_tensors(fn, dev, torch.float32, (B, H, D, D),
+                   ("state_in", "state_out") if len(states) == 2 else ("state_in", "d_state_out", "d_state_in"), *states)
+    _check_tensors(fn, dev, torch.float32, (H,), ("log_decay",), log_decay)
+    _check_tensors(fn, dev, torch.int32, (B,), ("seq_lens",), seq_lens)
+    _check_device(fn, q)
+
+
+def _linear_attn_ws(need, workspace, device):
+    if workspace is None and need:
+        import torch
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace, 0 if workspace is None else workspace.numel() * workspace.element_size()
+
+
+def linear_attn_fwd_workspace_size(desc):
+    return load().pa_linear_attn_fwd_workspace_size(ctypes.byref(desc))
+
+
+def linear_attn_fwd(q, k, v, log_decay, o, seq_lens=None, state_in=None, state_out=None, desc=None,
+                    workspace=None, stream=None):
+    """o = causal linear attention of q, k, v [B, L, H, D] with decay exp(log_decay[h]), from
+    state_in to state_out ([B, H, D, D] fp32, either may be None) over seq_lens (int32 [B])
+    tokens of each sequence. A workspace is allocated with torch unless given."""
+    d = desc or attn_desc(q)
+    _check_linear_attn("linear_attn_fwd", q, log_decay, seq_lens, ("q", "k", "v", "o"), (q, k, v, o),
+                       (state_in, state_out))
+    ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size(d), workspace, q.device)
+    _check("pa_linear_attn_fwd", load().pa_linear_attn_fwd(
+        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(seq_lens), _ptr(state_in),
+        _ptr(o), _ptr(state_out), _ptr(ws), nb, _stream() if stream is None else stream))
+
+
+def linear_attn_bwd_workspace_size(desc):
+    return load().pa_linear_attn_bwd_workspace_size(ctypes.byref(desc))
+
+
+def linear_attn_bwd(q, k, v, dO, log_decay, dq, dk, dv, seq_lens=None, state_in=None,
+                    d_state_out=None, d_state_in=None, accumulate=False, desc=None, workspace=None,
+                    stream=None):
+    """Gradients dq, dk, dv (overwritten, or added to) and d_state_in of linear_attn_fwd from dO
+    and d_state_out (None: zero)."""
+    d = desc or attn_desc(q)
+    _check_linear_attn("linear_attn_bwd", q, log_decay, seq_lens, ("q", "k", "v", "dO", "dq", "dk", "dv"),
+                       (q, k, v, dO, dq, dk, dv), (state_in, d_state_out, d_state_in))
+    ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size(d), workspace, q.device)
+    _check("pa_linear_attn_bwd", load().pa_linear_attn_bwd(
+        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(log_decay), _ptr(seq_lens),
+        _ptr(state_in), _ptr(d_state_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d_state_in),
+        int(bool(accumulate)), _ptr(ws), nb, _stream() if stream is None else stream))
+
+
+def linear_attn_step(q, k, v, log_decay, state_in, o, state_out, desc=None, stream=None):
+    """One new token of each sequence (q, k, v, o [B, 1, H, D]): state_out = decay * state_in +
+    k v^T, o = scale q state_out; state_out may be state_in."""
+    d = desc or attn_desc(q)
+    _check_linear_attn("linear_attn_step", q, log_decay, None, ("q", "k", "v", "o"), (q, k, v, o),
+                       (state_in, state_out))
+    _check("pa_linear_attn_step", load().pa_linear_attn_step(
+        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state_in), _ptr(o),
+        _ptr(state_out), _stream() if stream is None else stream))
 
 
 def device_status(clear=True, stream=None):

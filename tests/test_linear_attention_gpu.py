@@ -1,0 +1,315 @@
+"""Linear attention with a decay per head through the C ABI against its 64-bit
+quadratic form: forward, backward, carried states and the single-token step.
+
+Tolerances, per value, from the roundings of the kernels. `mag` is the same sum
+with every factor's magnitude, so an error of r in every factor moves a value by
+at most r * mag.
+  bf16 operands: the intermediate products rounded to bf16 (2^-8 of `mag`), the output's rounding
+      (2^-8 of the value); the carried states as two bf16 parts (2^-16) and fp32
+      sums (2^-20 for the lengths here) are inside the same 2^-8 mag: 2^-8 (|value| + 1.02 mag).
+  fp32 operands (split products): an operand in two bf16 parts is off by 2^-16,
+      the product drops the low parts' product, 2^-16: 3 x 2^-16 a product, two
+      products in a row and two splits of the state: 12 x 2^-16 < 2^-12 of mag.
+  states from bf16 operands: values times decay in two parts 2^-16 and fp32 sums:
+      2^-15 of mag; from fp32 operands 2^-12.
+Norm-wise, roundings of random sign: bf16 2^-8 x 2 (the output's own rounding and one more), fp32 2^-15."""
+import pytest
+
+torch = pytest.importorskip("torch")
+from conftest import rel_err  # noqa: E402
+from seq_ref import mix, mix_grads, mix_grads_absolute  # noqa: E402
+
+REL = {torch.bfloat16: 2.0 ** -8, torch.float32: 2.0 ** -12}
+NORM = {torch.bfloat16: 2.0 ** -7, torch.float32: 2.0 ** -15}
+STATE = {torch.bfloat16: 2.0 ** -15, torch.float32: 2.0 ** -12}
+
+
+def _close(got, want, mag, r, step):
+    err = (got.double() - want).abs()
+    tol = step * want.abs() + 1.02 * r * mag + 1e-30
+    worst = (err / tol).max().item() if err.numel() else 0.0
+    assert worst <= 1.0, f"{worst} of the tolerance"
+
+
+def _inputs(B, L, H, D, dtype, seed, decays=None, states=False):
+    g = torch.Generator().manual_seed(seed)
+    q, k, v, dO = ((0.5 * torch.randn(B, L, H, D, generator=g)).to(dtype).cuda() for _ in range(4))
+    if decays is None:
+        decays = [-(2.0 ** -(8.0 * (h + 1) / H)) for h in range(H)]
+    ld = torch.tensor(decays, dtype=torch.float32).cuda()
+    s, ds = ((torch.randn(B, H, D, D, generator=g).cuda() if states else None) for _ in range(2))
+    return q, k, v, dO, ld, s, ds
+
+
+def _forward(q, k, v, ld, **kw):
+    import pa_capi
+    B, L, H, D = q.shape
+    o = torch.full_like(q, float("nan"))
+    so = torch.full((B, H, D, D), float("nan"), device="cuda")
+    pa_capi.linear_attn_fwd(q, k, v, ld, o, state_out=so, **kw)
+    assert pa_capi.device_status() == 0
+    return o, so
+
+
+def _check_forward(q, k, v, ld, lens=None, s=None, scale=None):
+    import pa_capi
+    desc = pa_capi.attn_desc(q, scale=scale or 0.0)
+    o, so = _forward(q, k, v, ld, seq_lens=lens, state_in=s, desc=desc)
+    want, ws = mix(q, k, v, ld, lens, s, scale)
+    mag, ms = mix(q, k, v, ld, lens, s, scale, absolute=True)
+    t = q.dtype
+    _close(o, want, mag, REL[t], 2.0 ** -8 if t == torch.bfloat16 else 2.0 ** -24)
+    _close(so, ws, ms, STATE[t], 2.0 ** -24)
+    if want.norm() > 0:
+        assert rel_err(o.double().cpu(), want.cpu()) < NORM[t]
+    return o, so
+
+
+TYPES = [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.float32, 32), (torch.float32, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("L", [1, 2, 63, 64, 65, 127, 128, 129, 257, 500])
+def test_forward_lengths(dtype, D, L):
+    q, k, v, _, ld, _, _ = _inputs(2, L, 3, D, dtype, L)
+    _check_forward(q, k, v, ld)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_forward_state_and_ragged(dtype, D):
+    """Padded batch: lengths of zero, one, a tile's border, full, and beyond the range; the padding
+    holds NaN and infinities, which must reach neither outputs nor states."""
+    q, k, v, _, ld, s, _ = _inputs(7, 300, 2, D, dtype, 5, states=True)
+    lens = torch.tensor([0, 1, 128, 129, 300, 999, -4], dtype=torch.int32)
+    for b in range(7):
+        n = max(0, min(300, int(lens[b])))
+        for x in (q, k, v):
+            x[b, n:] = float("nan")
+            x[b, n::2] = float("inf")
+    o, so = _check_forward(q, k, v, ld, lens.cuda(), s)
+    for b in range(7):
+        assert (o[b, max(0, min(300, int(lens[b]))):] == 0).all()
+    assert torch.equal(so[0], s[0]) and torch.equal(so[6], s[6])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_forward_decays(dtype, D):
+    """No decay, a fast one, one that underflows within a tile, zero (each token alone), a growing one."""
+    decays = [0.0, -0.7, -9.0, -1e3, float("-inf"), 0.01]
+    q, k, v, _, ld, s, _ = _inputs(1, 280, 6, D, dtype, 6, decays, states=True)
+    _check_forward(q, k, v, ld, None, s)
+
+
+@pytest.mark.gpu
+def test_forward_scale_and_values_of_all_sizes():
+    q, k, v, _, ld, s, _ = _inputs(2, 200, 2, 64, torch.bfloat16, 7, states=True)
+    _check_forward(q, k, v, ld, None, s, scale=1.0)
+    _check_forward(q * 2.0 ** 40, k * 2.0 ** -30, v * 2.0 ** 20, ld, None, s * 2.0 ** -10)
+    z = torch.zeros_like(q)
+    o, so = _forward(z, z, z, ld)
+    assert (o == 0).all() and (so == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("B,H,L", [(1, 1, 4100), (2, 8, 1500), (1, 3, 9000)])
+def test_long_sequences_of_few_heads(dtype, D, B, H, L):
+    """Few (sequence, head) pairs: the work of one is split over the GPU and joined."""
+    q, k, v, dO, ld, s, ds = _inputs(B, L, H, D, dtype, 8, states=True)
+    lens = torch.tensor([L - 77 * b for b in range(B)], dtype=torch.int32).cuda()
+    _check_forward(q, k, v, ld, lens, s)
+    _check_backward(q, k, v, dO, ld, lens, s, ds)
+
+
+def _check_backward(q, k, v, dO, ld, lens=None, s=None, ds=None, accumulate=False):
+    import pa_capi
+    t = q.dtype
+    base = [torch.randn_like(q) if accumulate else torch.full_like(q, float("nan")) for _ in range(3)]
+    g = [x.clone() for x in base]
+    dsi = torch.full((*q.shape[:1], q.shape[2], q.shape[3], q.shape[3]), float("nan"), device="cuda")
+    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, seq_lens=lens, state_in=s, d_state_out=ds,
+                            d_state_in=dsi, accumulate=accumulate)
+    assert pa_capi.device_status() == 0
+    want = mix_grads(q, k, v, ld, dO, lens, s, ds)
+    mag = mix_grads_absolute(q, k, v, ld, dO, lens, s, ds)
+    step = 2.0 ** -8 if t == torch.bfloat16 else 2.0 ** -24
+    for got, w, m, b0 in zip(g, want, mag, base):
+        w = w + b0.double() if accumulate else w
+        _close(got, w, m, REL[t], step * 1.01)
+        if w.norm() > 0:
+            assert rel_err(got.double().cpu(), w.cpu()) < NORM[t]
+    _close(dsi, want[3], mag[3], STATE[t], 2.0 ** -24)
+    return g, dsi
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("L", [1, 2, 64, 127, 129, 300])
+def test_backward_lengths(dtype, D, L):
+    q, k, v, dO, ld, s, ds = _inputs(2, L, 3, D, dtype, 20 + L, states=True)
+    _check_backward(q, k, v, dO, ld)
+    _check_backward(q, k, v, dO, ld, None, s, ds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_backward_ragged_and_accumulating(dtype, D):
+    q, k, v, dO, ld, s, ds = _inputs(5, 260, 2, D, dtype, 30, [-0.3, float("-inf")], states=True)
+    lens = torch.tensor([0, 1, 128, 131, 260], dtype=torch.int32)
+    for b in range(5):
+        for x in (q, k, v, dO):
+            x[b, int(lens[b]):] = float("nan")
+    lens = lens.cuda()
+    g, dsi = _check_backward(q, k, v, dO, ld, lens, s, ds)
+    for b in range(5):
+        for x in g:
+            assert (x[b, int(lens[b]):] == 0).all()
+    assert rel_err(dsi[0].cpu(), ds[0].cpu()) < 2.0 ** -22  # no token: the gradient passes through
+    q, k, v, dO, ld, s, ds = _inputs(3, 150, 2, D, dtype, 31, states=True)
+    _check_backward(q, k, v, dO, ld, torch.tensor([150, 0, 9], dtype=torch.int32).cuda(), s, ds, accumulate=True)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences():
+    """o is linear in each of q, k, v and the state, so a difference of the forward over any step is
+    the gradient along it: <dO, o(q + d) - o(q)> = <dq, d>, with the state's part for k, v, S_0."""
+    import pa_capi
+    q, k, v, dO, ld, s, ds = _inputs(2, 190, 3, 64, torch.float32, 40, states=True)
+    g = [torch.empty_like(q) for _ in range(3)]
+    dsi = torch.empty_like(s)
+    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, state_in=s, d_state_out=ds, d_state_in=dsi)
+
+    def value(q, k, v, s):
+        o, so = _forward(q, k, v, ld, state_in=s)
+        return (o.double() * dO).sum() + (so.double() * ds).sum()
+
+    x = [q, k, v, s]
+    for i, grad in enumerate([*g, dsi]):
+        d = torch.randn_like(x[i])
+        hi, lo = list(x), list(x)
+        hi[i], lo[i] = x[i] + d, x[i] - d
+        diff = (value(*hi) - value(*lo)) / 2
+        want = (grad.double() * d).sum()
+        scale = grad.double().norm() * d.double().norm()
+        assert abs(diff - want) <= 2.0 ** -12 * scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("B,H", [(1, 1), (5, 3), (64, 4)])
+def test_step_matches_formula(dtype, D, B, H):
+    import pa_capi
+    q, k, v, _, ld, s, _ = _inputs(B, 1, H, D, dtype, 50 + B, states=True)
+    o, so = torch.empty_like(q), torch.empty_like(s)
+    pa_capi.linear_attn_step(q, k, v, ld, s, o, so)
+    want, ws = mix(q, k, v, ld, None, s)
+    mag, ms = mix(q, k, v, ld, None, s, absolute=True)
+    step = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24
+    _close(o, want, mag, 2.0 ** -20, step)
+    _close(so, ws, ms, 2.0 ** -22, 2.0 ** -24)
+    inplace = s.clone()
+    pa_capi.linear_attn_step(q, k, v, ld, inplace, o, inplace)
+    assert torch.equal(inplace, so)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_prompt_in_pieces_then_tokens_equals_one_pass(dtype, D):
+    """A prompt in two pieces with the state carried (in place), then single tokens: the same outputs
+    as one pass over all of it."""
+    import pa_capi
+    B, L, H = 2, 220, 3
+    q, k, v, _, ld, s, _ = _inputs(B, L, H, D, dtype, 60, states=True)
+    want, ws = mix(q, k, v, ld, None, s)
+    mag, ms = mix(q, k, v, ld, None, s, absolute=True)
+    state, outs = s.clone(), []
+    for a, b in ((0, 130), (130, 213)):
+        part = [x[:, a:b].contiguous() for x in (q, k, v)]
+        o = torch.empty_like(part[0])
+        pa_capi.linear_attn_fwd(*part, ld, o, state_in=state, state_out=state)
+        outs.append(o)
+    for t in range(213, L):
+        part = [x[:, t:t + 1].contiguous() for x in (q, k, v)]
+        o = torch.empty_like(part[0])
+        pa_capi.linear_attn_step(*part, ld, state, o, state)
+        outs.append(o)
+    _close(torch.cat(outs, 1), want, mag, REL[dtype], 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -24)
+    _close(state, ws, ms, STATE[dtype], 2.0 ** -22)
+
+
+@pytest.mark.gpu
+def test_same_bits_every_time_on_streams_and_in_graphs():
+    """Two calls at once on two streams with a workspace each, and a captured call replayed with new
+    inputs, give the bits of a call alone."""
+    import pa_capi
+    a = _inputs(1, 2100, 4, 64, torch.bfloat16, 70, states=True)
+    b = _inputs(1, 2100, 4, 64, torch.bfloat16, 71, states=True)
+
+    def call(x, out, ws):
+        q, k, v, dO, ld, s, ds = x
+        pa_capi.linear_attn_fwd(q, k, v, ld, out[0], state_in=s, state_out=out[1], workspace=ws[0])
+        pa_capi.linear_attn_bwd(q, k, v, dO, ld, *out[2:5], state_in=s, d_state_out=ds, d_state_in=out[5],
+                                workspace=ws[1])
+
+    def buffers(x):
+        d = pa_capi.attn_desc(x[0])
+        n = (pa_capi.linear_attn_fwd_workspace_size(d), pa_capi.linear_attn_bwd_workspace_size(d))
+        q, s = x[0], x[5]
+        return ([torch.zeros_like(q), torch.zeros_like(s), *(torch.zeros_like(q) for _ in range(3)), torch.zeros_like(s)],
+                [torch.empty(max(m, 256), dtype=torch.uint8, device="cuda") for m in n])
+
+    alone = []
+    for x in (a, b):
+        out, ws = buffers(x)
+        call(x, out, ws)
+        alone.append(out)
+    torch.cuda.synchronize()
+    both = [buffers(x) for x in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(3):
+        for x, (out, ws), st in zip((a, b), both, streams):
+            with torch.cuda.stream(st):
+                call(x, out, ws)
+    torch.cuda.synchronize()
+    for (out, _), want in zip(both, alone):
+        assert all(torch.equal(m, n) for m, n in zip(out, want))
+    out, ws = buffers(a)
+    x = [t.clone() for t in a]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call(x, out, ws)
+    for src, want in ((a, alone[0]), (b, alone[1])):
+        for t, n in zip(x, src):
+            t.copy_(n)
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(m, n) for m, n in zip(out, want))
+    assert pa_capi.device_status() == 0
+
+
+@pytest.mark.gpu
+def test_rotary_then_linear_attention_trains_as_in_64_bits():
+    """The two together as a layer uses them: turn q and k, mix, and the gradients back through both."""
+    import pa_capi
+    from seq_ref import turn
+    B, L, H, D = 2, 333, 4, 64
+    q, k, v, dO, ld, _, _ = _inputs(B, L, H, D, torch.float32, 80)
+    pos = torch.stack([torch.arange(L) // 49, torch.arange(L) // 7 % 7, torch.arange(L) % 7]).int()
+    pos = pos[:, None].expand(3, B, L).contiguous().cuda()
+    sections = [8, 12, 12]
+    desc = pa_capi.rope_desc(q, k, sections)
+    qr, kr, o = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)
+    pa_capi.rope_fwd(q, k, pos, qr, kr, desc)
+    pa_capi.linear_attn_fwd(qr, kr, v, ld, o)
+    g = [torch.empty_like(q) for _ in range(3)]
+    pa_capi.linear_attn_bwd(qr, kr, v, dO, ld, *g)
+    pa_capi.rope_bwd(g[0], g[1], pos, g[0], g[1], desc)
+    x = [t.double().requires_grad_() for t in (q, k, v)]
+    want, _ = mix(turn(x[0], pos, sections), turn(x[1], pos, sections), x[2], ld)
+    assert rel_err(o.double().cpu(), want.detach().cpu()) < NORM[torch.float32]
+    for got, w in zip(g, torch.autograd.grad((want * dO.double()).sum(), x)):
+        assert rel_err(got.double().cpu(), w.cpu()) < NORM[torch.float32]

@@ -1,0 +1,127 @@
+"""Argument checks of the rotary positions and of linear attention: the C ABI's
+status codes before any device work, and the Python binding's refusals (no GPU)."""
+import ctypes
+
+import pytest
+
+NULL, SHAPE, DTYPE, ALIGN, UNSUPPORTED, WORKSPACE = 8, 1, 2, 3, 4, 7
+
+
+def _rope(**kw):
+    import pa_capi
+    f = dict(batch=1, seq_len=8, num_heads=2, num_kv_heads=1, head_dim=64, dtype=pa_capi.PA_BF16, layout=0,
+             freqs=0, axes=2, sections=(ctypes.c_int32 * 4)(8, 8, 0, 0), base=10000.0)
+    f.update(kw)
+    if isinstance(f["sections"], tuple):
+        f["sections"] = (ctypes.c_int32 * 4)(*f["sections"])
+    return ctypes.byref(pa_capi.RopeDesc(**f))
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(batch=0), SHAPE), (dict(seq_len=0), SHAPE), (dict(num_heads=0), SHAPE), (dict(num_kv_heads=-1), SHAPE),
+    (dict(head_dim=0), SHAPE), (dict(head_dim=258), UNSUPPORTED), (dict(dtype=5), DTYPE), (dict(layout=2), UNSUPPORTED),
+    (dict(freqs=-1), UNSUPPORTED), (dict(axes=0), SHAPE), (dict(axes=5), SHAPE), (dict(sections=(8, 0, 0, 0)), SHAPE),
+    (dict(sections=(30, 3, 0, 0)), SHAPE), (dict(sections=(2 ** 31 - 1, 2 ** 31 - 1, 0, 0)), SHAPE),
+    (dict(base=1.0), SHAPE), (dict(base=float("nan")), SHAPE), (dict(base=float("inf")), SHAPE),
+    (dict(batch=1 << 16, seq_len=1 << 16), SHAPE), (dict(num_heads=1 << 25), SHAPE),
+])
+def test_rope_descriptor_refusals(kw, status):
+    import pa_capi
+    lib = pa_capi.load()
+    assert lib.pa_rope_fwd(_rope(**kw), 16, 32, 64, 128, 256, None) == status
+    assert lib.pa_rope_bwd(_rope(**kw), 16, 32, 64, 128, 256, 0, None) == status
+
+
+def test_rope_pointer_refusals():
+    import pa_capi
+    lib = pa_capi.load()
+    assert lib.pa_rope_fwd(None, 16, 32, 64, 128, 256, None) == NULL
+    for i in range(5):
+        a = [16, 32, 64, 128, 256]
+        a[i] = None
+        assert lib.pa_rope_fwd(_rope(), *a, None) == NULL
+        a[i] = 18  # misaligned for values, and for positions
+        assert lib.pa_rope_fwd(_rope(), *a, None) == ALIGN
+    # adding in place would read what it has written
+    assert lib.pa_rope_bwd(_rope(), 16, 32, 64, 16, 256, 1, None) == SHAPE
+    assert lib.pa_rope_bwd(_rope(), 16, 32, 64, 128, 32, 1, None) == SHAPE
+
+
+def _desc(B=2, L=128, H=2, D=64, dtype=1, scale=0.0):
+    import pa_capi
+    return ctypes.byref(pa_capi.AttnDesc(B, L, H, D, dtype, scale))
+
+
+@pytest.mark.parametrize("kw,status", [
+    (dict(B=0), SHAPE), (dict(L=0), SHAPE), (dict(L=-3), SHAPE), (dict(H=0), SHAPE), (dict(D=96), UNSUPPORTED),
+    (dict(D=32), UNSUPPORTED), (dict(dtype=0, D=128), UNSUPPORTED), (dict(dtype=9), DTYPE),
+    (dict(B=1 << 16, H=1 << 10), SHAPE),
+])
+def test_linear_attention_descriptor_refusals(kw, status):
+    import pa_capi
+    lib = pa_capi.load()
+    big = 1 << 40
+    assert lib.pa_linear_attn_fwd(_desc(**kw), 16, 32, 48, 64, None, None, 80, None, 256, big, None) == status
+    assert lib.pa_linear_attn_bwd(_desc(**kw), 16, 32, 48, 64, 80, None, None, None, 96, 112, 128, None, 0, 256,
+                                  big, None) == status
+    assert lib.pa_linear_attn_step(_desc(**dict(kw, L=kw.get("L", 1))), 16, 32, 48, 64, 80, 96, 112, None) == status
+    assert lib.pa_linear_attn_fwd_workspace_size(_desc(**kw)) == 0
+    assert lib.pa_linear_attn_bwd_workspace_size(_desc(**kw)) == 0
+
+
+def test_linear_attention_pointer_refusals():
+    import pa_capi
+    lib = pa_capi.load()
+    big = 1 << 40
+    fwd = lambda q=16, k=32, v=48, ld=64, n=None, s=None, o=80, so=None, ws=256, nb=big: lib.pa_linear_attn_fwd(
+        _desc(), q, k, v, ld, n, s, o, so, ws, nb, None)
+    assert lib.pa_linear_attn_fwd(None, 16, 32, 48, 64, None, None, 80, None, 256, big, None) == NULL
+    for name in ("q", "k", "v", "ld", "o"):
+        assert fwd(**{name: None}) == NULL
+    for name in ("q", "k", "v", "o", "s", "so"):
+        assert fwd(**{name: 8}) == ALIGN
+    assert fwd(ld=66) == ALIGN and fwd(n=66) == ALIGN
+    for name in ("q", "k", "v"):
+        assert fwd(**{name: 80}) == SHAPE  # an input as the output
+    bwd = lambda q=16, k=32, v=48, dO=64, ld=80, n=None, s=None, ds=None, dq=96, dk=112, dv=128, dsi=None, ws=256, \
+        nb=big: lib.pa_linear_attn_bwd(_desc(), q, k, v, dO, ld, n, s, ds, dq, dk, dv, dsi, 0, ws, nb, None)
+    for name in ("q", "k", "v", "dO", "ld", "dq", "dk", "dv"):
+        assert bwd(**{name: None}) == NULL
+    for name in ("q", "k", "v", "dO", "dq", "dk", "dv", "s", "ds", "dsi"):
+        assert bwd(**{name: 8}) == ALIGN
+    assert bwd(dq=16) == SHAPE and bwd(dk=64) == SHAPE and bwd(dv=96) == SHAPE
+    assert bwd(s=160, dsi=160) == SHAPE
+    step = lambda L=1, q=16, k=32, v=48, ld=64, s=80, o=96, so=112: lib.pa_linear_attn_step(
+        _desc(L=L), q, k, v, ld, s, o, so, None)
+    assert step(L=2) == SHAPE and step(o=16) == SHAPE
+    for name in ("q", "k", "v", "ld", "s", "o", "so"):
+        assert step(**{name: None}) == NULL
+        if name != "ld":
+            assert step(**{name: 8}) == ALIGN
+
+
+def test_binding_refusals():
+    """Types, shapes, layouts and devices that the kernels would misread are refused by name."""
+    torch = pytest.importorskip("torch")
+    import pa_capi
+    q = torch.zeros(2, 8, 4, 64)
+    ld = torch.zeros(4)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        pa_capi.linear_attn_fwd(q, q, q, ld, q)
+    with pytest.raises(ValueError, match="k must be"):
+        pa_capi.linear_attn_fwd(q, q[:, :4], q, ld, q, workspace=q)
+    with pytest.raises(TypeError):
+        pa_capi.linear_attn_fwd(q.double(), q, q, ld, q)
+    with pytest.raises(ValueError, match="sections|axes"):
+        pa_capi.rope_desc(q, q, [1] * 5)
+    with pytest.raises(KeyError):
+        pa_capi.rope_desc(q, q, layout="both")
+    d = pa_capi.rope_desc(q, q)
+    with pytest.raises(ValueError, match="kv heads"):
+        pa_capi.rope_fwd(q, None, torch.zeros(1, 2, 8, dtype=torch.int32), q, None, d)
+    with pytest.raises(ValueError):
+        pa_capi.rope_fwd(q, q, torch.zeros(1, 2, 8, dtype=torch.int64), q, q, d)
+    with pytest.raises(ValueError, match="v must be contiguous"):
+        pa_capi.linear_attn_fwd(q, q, q.transpose(1, 2).contiguous().transpose(1, 2), ld, q)
+    with pytest.raises(ValueError, match="state_in must be"):
+        pa_capi.linear_attn_step(q, q, q, ld, torch.zeros(2, 4, 64, 32), q, q)
