@@ -210,7 +210,7 @@ int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, c
 
 /* Gradients from dO and d_state_out (the gradient of state_out; NULL: zero):
  * dq, dk, dv (overwritten, or added to when accumulate != 0) and d_state_in
- * (overwritten; NULL: not wanted; may be d_state_out). state_in: as in the forward. */
+ * (overwritten; NULL: not wanted; neither state_in nor d_state_out). state_in: as in the forward. */
 size_t pa_linear_attn_bwd_workspace_size(const pa_attn_desc* desc);
 int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
                        const void* dO, const float* log_decay, const int32_t* seq_lens,

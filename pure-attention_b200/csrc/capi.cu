@@ -345,7 +345,7 @@ int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, c
       if (out[i] == p) return PA_ERR_SHAPE;
     if (out[i] == out[(i + 1) % 3]) return PA_ERR_SHAPE;
   }
-  if (d_state_in && d_state_in == state_in) return PA_ERR_SHAPE;
+  if (d_state_in && (d_state_in == state_in || d_state_in == d_state_out)) return PA_ERR_SHAPE;
   st = check_linear_attn_ws(desc, true, workspace, workspace_bytes);
   if (st != PA_OK) return st;
   uint32_t* status = status_word();

@@ -34,45 +34,655 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
   return n < 0 ? 0 : (n > L ? L : n);
 }
 
-// Thread e holds column e of the state (D values) and walks the tokens.
-template <typename T, int D>
-__global__ void __launch_bounds__(D)
-    mix_scan_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v, T* o,
-                    const float* __restrict__ log_decay, const int32_t* __restrict__ lens,
-                    const float* s_in, float* s_out, int L, int H, float scale, MixDir dir) {
-  __shared__ float sq[D], sk[D];
-  const int h = blockIdx.x % H, b = blockIdx.x / H, e = threadIdx.x;
-  const int n = valid_tokens(lens, b, L);
-  const float lam = exp2f(log2_decay(log_decay, h));
-  const size_t st0 = static_cast<size_t>(blockIdx.x) * D * D;
-  float S[D];
-#pragma unroll
-  for (int d = 0; d < D; ++d)
-    S[d] = s_in ? dir.in_mult * s_in[st0 + (dir.transposed ? e * D + d : d * D + e)] : 0.f;
-  for (int p = 0; p < n; ++p) {
-    const int t = dir.reverse ? n - 1 - p : p;
-    const size_t at = ((static_cast<size_t>(b) * L + t) * H + h) * D + e;
-    __syncthreads();
-    sq[e] = ld_f(q + at);
-    sk[e] = ld_f(k + at);
-    const float ve = ld_f(v + at);
-    __syncthreads();
-    const float w = p == 0 && dir.lead ? 1.f : lam;
-    float acc = 0.f;
-#pragma unroll
-    for (int d = 0; d < D; ++d) {
-      S[d] = fmaf(w, S[d], sk[d] * ve);
-      acc = fmaf(sq[d], S[d], acc);
-    }
-    st_f(o + at, (dir.accumulate ? ld_f(o + at) : 0.f) + scale * acc);
+// ---------------------------------------------------------------- chunked kernel
+// A sequence in chunks of C = 128 tokens. With S the state entering a chunk of n
+// valid tokens (rows i, j of the chunk; l the decay):
+//   O   = scale (P V + diag(l^(i+1)) Q S),   P = (Q K^T) o l^(i-j) for j <= i, else 0
+//   S' = l^n S + K^T V',                      V' = diag(l^(n-1-j)) V
+// All four products run on the tensor cores; every power of l has a whole,
+// non-negative exponent, so nothing overflows where l is small.
+//
+// One CTA per SM walks units (sequence, head, 64 columns of V, segment of the
+// sequence); a unit's chunks follow one another through the state, and the
+// rings below run on across units.
+//   warps 0-3   P: load Q K^T from TMEM, times l^(i-j), bf16 back to TMEM
+//   warps 4-7   the state in fp32 registers (thread = row of the state), its bf16
+//               parts to shared memory for Q S; then O out
+//   warp 8      tcgen05.mma issue
+//   warps 9-16  loads: global memory -> registers (pieces of 128 x 64 values, some
+//               always in flight) -> 128-byte swizzled tiles. Rows past the
+//               sequence are zeros, rows may run backwards in time, and fp32 is
+//               split here: none of these fits a plain TMA box.
+// Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
+// MN-major A of K^T V'.
+//
+// Roundings: fp32 sums and state throughout. V' and the state are two bf16
+// parts (off by 2^-16), so states keep fp32-like accuracy; P is one bf16 (2^-8),
+// as in the softmax kernels. NT = 3 (fp32 operands): every operand is a
+// hi/lo pair and every product hi*hi + hi*lo + lo*hi.
+//
+// TMEM columns: Q K^T and P 2 x 128 (P over its own scores: hi 0-63, lo 64-127),
+// Q S 64, P V 64, K^T V' 2 x 64.
+constexpr int kMixThreads = 17 * 32;
+constexpr int kTile = 128 * 128;  // bytes of 128 rows x 64 bf16
+
+template <int DK, int NT>
+struct MixCfg {
+  static constexpr int NP = NT == 3 ? 2 : 1;       // planes (hi, lo) of q, k, v
+  static constexpr int KT = DK / 64;               // 64-column tiles of q and k
+  static constexpr int OPER = NP * KT * kTile;     // bytes of q (or k) of a stage
+  static constexpr int V_STAGE = (NP + 2) * kTile; // v, and V' hi and lo
+  static constexpr int ST_PLANE = DK * 128;        // [DK, 64] bf16
+  static constexpr bool SMALL = NP == 1 && DK == 64;
+  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 2 : 1, STB = DK == 64 ? 2 : 1;
+  static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + STB * 2 * ST_PLANE + 1024;
+  static constexpr int NC = DK == 64 ? 32 : 64;    // state columns of a thread
+};
+static_assert(MixCfg<64, 1>::SMEM <= 226 * 1024 && MixCfg<64, 3>::SMEM <= 226 * 1024 &&
+              MixCfg<128, 1>::SMEM <= 226 * 1024, "shared memory of one CTA");
+
+struct MixOne {  // one direction of the recurrence
+  const void *q, *k, *v;
+  void* o;
+  const float* s_in;
+  float* s_out;
+  MixDir dir;
+};
+struct MixArgs {
+  MixOne one[3];
+  int n_dir;
+  const float* log_decay;
+  const int32_t* lens;
+  float* ws;  // segment states, see seg_slot
+  int B, L, H, D;
+  int n_seg, seg_tokens, n_units;
+  float scale;
+};
+
+struct MixUnit {
+  int dir, b, h, half, seg;
+  int n;          // valid tokens of the sequence
+  int p0, count;  // first position and tokens of this segment
+  int chunks;
+};
+
+// unit -> (segment, sequence, head, direction, column half), halves and
+// directions of one head next to one another: they read the same rows, from L2
+template <int DK>
+__device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
+  MixUnit x;
+  constexpr int halves = DK / 64;
+  x.half = u % halves;
+  u /= halves;
+  x.dir = u % a.n_dir;
+  u /= a.n_dir;
+  x.h = u % a.H;
+  u /= a.H;
+  x.b = u % a.B;
+  x.seg = u / a.B;
+  x.n = valid_tokens(a.lens, x.b, a.L);
+  x.p0 = x.seg * a.seg_tokens;
+  const int left = x.n - x.p0;
+  x.count = left < 0 ? 0 : (left < a.seg_tokens ? left : a.seg_tokens);
+  x.chunks = (x.count + 127) >> 7;
+  return x;
+}
+
+// Workspace of a sequence cut in segments: per (sequence, head, direction, half)
+// n_seg slots of [DK, 64] fp32. Slot s < n_seg - 1 holds the state of segment s
+// alone (from zero), slot n_seg - 1 a copy of the carried state (state_out may
+// overwrite state_in while other segments still need it).
+template <int DK>
+__device__ __forceinline__ float* seg_slot(const MixArgs& a, const MixUnit& x, int slot) {
+  const size_t w = ((static_cast<size_t>(x.b) * a.H + x.h) * a.n_dir + x.dir) * (DK / 64) + x.half;
+  return a.ws + (w * a.n_seg + slot) * (DK * 64);
+}
+
+// A piece is 128 rows x 64 values of one operand; thread t of 256 holds the
+// 16-byte vectors t, t + 256, ...
+template <typename T>
+struct Piece {
+  static constexpr int VECS = sizeof(T) == 2 ? 4 : 8;
+  static constexpr int PER_ROW = 64 * static_cast<int>(sizeof(T)) / 16;
+  uint4 r[VECS];
+};
+
+__device__ __forceinline__ uint32_t lo_pair(float a, float b, uint32_t hi) {
+  return pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
+}
+
+// The loads in order: per chunk the k pieces, the q pieces (not for segment
+// states), the v piece.
+template <int DK, bool STATES>
+struct PieceIter {
+  MixUnit x;
+  int u, chunk, piece, g;  // g: chunks of this CTA so far
+  static constexpr int KT = DK / 64;
+  static constexpr int PER = STATES ? KT + 1 : 2 * KT + 1;
+  __device__ __forceinline__ bool first(const MixArgs& a) {
+    u = blockIdx.x;
+    chunk = piece = g = 0;
+    return settle(a);
   }
-  if (!dir.accumulate)
-    for (int t = n; t < L; ++t) st_f(o + ((static_cast<size_t>(b) * L + t) * H + h) * D + e, 0.f);
-  if (s_out) {
-    const float w = dir.out_mult * (dir.lead && n > 0 ? lam : 1.f);
+  __device__ __forceinline__ bool settle(const MixArgs& a) {  // to a unit that has chunks
+    for (; u < a.n_units; u += gridDim.x) {
+      x = mix_unit<DK>(a, u);
+      if (x.chunks > 0) return true;
+    }
+    return false;
+  }
+  __device__ __forceinline__ bool next(const MixArgs& a) {
+    if (++piece < PER) return true;
+    piece = 0;
+    ++g;
+    if (++chunk < x.chunks) return true;
+    chunk = 0;
+    u += gridDim.x;
+    return settle(a);
+  }
+  __device__ __forceinline__ bool is_v() const { return piece == PER - 1; }
+  __device__ __forceinline__ bool is_q() const { return !STATES && piece >= KT && piece < 2 * KT; }
+  __device__ __forceinline__ int valid() const {  // valid rows of the chunk
+    const int left = x.count - chunk * 128;
+    return left < 128 ? left : 128;
+  }
+};
+
+template <typename T, int DK, bool STATES>
+__device__ __forceinline__ void load_piece(const MixArgs& a, const PieceIter<DK, STATES>& it, int t, Piece<T>& p) {
+  using P = Piece<T>;
+  const MixOne& one = a.one[it.x.dir];
+  const void* base = it.is_v() ? one.v : (it.is_q() ? one.q : one.k);
+  const int tile = it.is_v() ? it.x.half : it.piece % (DK / 64);
+  const int row0 = t / P::PER_ROW, col = (t % P::PER_ROW) * (16 / static_cast<int>(sizeof(T)));
+  const int valid = it.valid();
+  const bool in_cols = tile * 64 + col < a.D;  // head dim 32 fills half a tile
+  const int pos = it.x.p0 + it.chunk * 128 + row0;
+  const bool rev = one.dir.reverse;
+  const long long tok0 = static_cast<long long>(it.x.b) * a.L + (rev ? it.x.n - 1 - pos : pos);
+  const long long step = static_cast<long long>(a.H) * a.D * (256 / P::PER_ROW) * (rev ? -1 : 1);
+  const T* src = static_cast<const T*>(base) + (tok0 * a.H + it.x.h) * a.D + tile * 64 + col;
 #pragma unroll
-    for (int d = 0; d < D; ++d)
-      s_out[st0 + (dir.transposed ? e * D + d : d * D + e)] = w * S[d];
+  for (int i = 0; i < P::VECS; ++i) {
+    const bool ok = in_cols && row0 + i * (256 / P::PER_ROW) < valid;
+    p.r[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src + i * step)) : make_uint4(0, 0, 0, 0);
+  }
+}
+
+// Four (fp32) or eight (bf16) values of row `row` from byte column `cb` on, as
+// bf16 hi and, where `lo` is not 0, lo.
+__device__ __forceinline__ void put4(uint32_t hi, uint32_t lo, uint32_t off, float a, float b, float c, float d) {
+  const uint32_t h0 = pack_bf16x2(a, b), h1 = pack_bf16x2(c, d);
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(hi + off), "r"(h0), "r"(h1) : "memory");
+  if (lo)
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(lo + off), "r"(lo_pair(a, b, h0)),
+                 "r"(lo_pair(c, d, h1)) : "memory");
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
+// A piece as an operand tile (hi, and lo where NP = 2).
+template <typename T, int NP>
+__device__ __forceinline__ void store_operand(const Piece<T>& p, int t, uint32_t hi, uint32_t lo) {
+  using P = Piece<T>;
+#pragma unroll
+  for (int i = 0; i < P::VECS; ++i) {
+    const int row = t / P::PER_ROW + i * (256 / P::PER_ROW);
+    if constexpr (sizeof(T) == 2) {
+      st_shared_v4(hi + sw128_offset(row, (t % 8) * 16), p.r[i].x, p.r[i].y, p.r[i].z, p.r[i].w);
+    } else {
+      put4(hi, NP == 2 ? lo : 0, sw128_offset(row, (t % 16) * 8), __uint_as_float(p.r[i].x),
+           __uint_as_float(p.r[i].y), __uint_as_float(p.r[i].z), __uint_as_float(p.r[i].w));
+    }
+  }
+}
+
+// A v piece as V' = diag(l^(valid - 1 - row)) V in two parts.
+template <typename T>
+__device__ __forceinline__ void store_decayed(const Piece<T>& p, int t, uint32_t hi, uint32_t lo, float l2, int valid) {
+  using P = Piece<T>;
+#pragma unroll
+  for (int i = 0; i < P::VECS; ++i) {
+    const int row = t / P::PER_ROW + i * (256 / P::PER_ROW);
+    const float w = row < valid ? exp2f(l2 * static_cast<float>(valid - 1 - row)) : 0.f;
+    if constexpr (sizeof(T) == 2) {
+      const uint32_t x[4] = {p.r[i].x, p.r[i].y, p.r[i].z, p.r[i].w};
+      uint32_t h[4], l[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float a = w * __uint_as_float(x[j] << 16), b = w * __uint_as_float(x[j] & 0xffff0000u);
+        h[j] = pack_bf16x2(a, b);
+        l[j] = lo_pair(a, b, h[j]);
+      }
+      const uint32_t off = sw128_offset(row, (t % 8) * 16);
+      st_shared_v4(hi + off, h[0], h[1], h[2], h[3]);
+      st_shared_v4(lo + off, l[0], l[1], l[2], l[3]);
+    } else {
+      put4(hi, lo, sw128_offset(row, (t % 16) * 8), w * __uint_as_float(p.r[i].x), w * __uint_as_float(p.r[i].y),
+           w * __uint_as_float(p.r[i].z), w * __uint_as_float(p.r[i].w));
+    }
+  }
+}
+
+// 16 values of an output row.
+__device__ __forceinline__ void store16(float* dst, const float* v, bool acc) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float4 f = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    if (acc) {
+      const float4 o = reinterpret_cast<const float4*>(dst)[i];
+      f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
+    }
+    reinterpret_cast<float4*>(dst)[i] = f;
+  }
+}
+__device__ __forceinline__ void store16(__nv_bfloat16* dst, const float* v, bool acc) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    uint32_t w[4];
+    uint4 o = make_uint4(0, 0, 0, 0);
+    if (acc) o = reinterpret_cast<const uint4*>(dst)[i];
+    const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = v[8 * i + 2 * j], b = v[8 * i + 2 * j + 1];
+      if (acc) {
+        a += __uint_as_float(ow[j] << 16);
+        b += __uint_as_float(ow[j] & 0xffff0000u);
+      }
+      w[j] = pack_bf16x2(a, b);
+    }
+    reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+__device__ __forceinline__ void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if (lane_id() == 0) mbar_arrive(bar);
+}
+
+// STATES: only the segments' own states, into the workspace.
+template <typename T, int DK, int NT, bool STATES>
+__global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_constant__ MixArgs a, uint32_t* status) {
+  using C = MixCfg<DK, NT>;
+  constexpr int NP = C::NP, KT = C::KT;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[26];
+  __shared__ float wtab[32 + 64 + 96 + 128];  // powers of the decay, a table for each P warp
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  if (cta_aborted(status, &abort_flag)) return;
+  const uint32_t sm0 = smem_u32(align1024(smem_raw));
+  const uint32_t sv0 = sm0 + C::QKS * 2 * C::OPER, ss0 = sv0 + C::VS * C::V_STAGE;
+  auto bar = [&](int i) { return smem_u32(&bars[i]); };
+  // ring slot s: K planes, then Q planes; V, V' hi, V' lo; state hi, lo
+  auto sK = [&](int s) { return sm0 + s * 2 * C::OPER; };
+  auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
+  auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
+  auto sS = [&](int s) { return ss0 + s * 2 * C::ST_PLANE; };
+  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 8, S_FULL = 10, P_FULL = 12, KV_FULL = 14,
+         KV_FREE = 16, ST_FULL = 18, ST_EMPTY = 20, O_FULL = 22, O_FREE = 23 };
+  constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
+
+  const int warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 3; ++i) {
+      mbar_init(bar(QK_FULL + i), 8);
+      mbar_init(bar(QK_EMPTY + i), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(V_FULL + i), 8);
+      mbar_init(bar(V_EMPTY + i), 1);
+      mbar_init(bar(S_FULL + i), 1);
+      mbar_init(bar(P_FULL + i), 4);
+      mbar_init(bar(KV_FULL + i), 1);
+      mbar_init(bar(KV_FREE + i), 4);
+      mbar_init(bar(ST_FULL + i), 4);
+      mbar_init(bar(ST_EMPTY + i), 1);
+    }
+    mbar_init(bar(O_FULL), 1);
+    mbar_init(bar(O_FREE), 4);
+    fence_mbar_init();
+  }
+  if (warp == 8) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+
+  if (warp >= 9) {
+    // ------------------------------------------------------------ loads
+    const int t = threadIdx.x - 9 * 32;
+    constexpr int DEPTH = sizeof(T) == 2 ? 3 : 2;  // pieces in flight
+    PieceIter<DK, STATES> ld, st;
+    Piece<T> buf[DEPTH];
+    bool more_ld = ld.first(a), more = st.first(a), ok = true;
+#pragma unroll
+    for (int i = 0; i < DEPTH; ++i)
+      if (more_ld) {
+        load_piece(a, ld, t, buf[i]);
+        more_ld = ld.next(a);
+      }
+    while (more && ok) {
+      const int g = st.g, qs = g % C::QKS, vs = g % C::VS;
+      if (st.piece == 0 && g >= C::QKS) ok = mbar_wait_warp(bar(QK_EMPTY + qs), (g / C::QKS - 1) & 1, status);
+      if (st.is_v() && g >= C::VS) ok = ok && mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status);
+      if (!ok) break;
+      if (st.is_v()) {
+        if (!STATES) store_operand<T, NP>(buf[0], t, sV(vs), sV(vs) + kTile);
+        store_decayed<T>(buf[0], t, sV(vs) + NP * kTile, sV(vs) + (NP + 1) * kTile,
+                         log2_decay(a.log_decay, st.x.h), st.valid());
+      } else {
+        const uint32_t at = (st.is_q() ? sQ(qs) : sK(qs)) + (st.piece % KT) * kTile;
+        store_operand<T, NP>(buf[0], t, at, at + KT * kTile);
+      }
+#pragma unroll
+      for (int i = 0; i + 1 < DEPTH; ++i) buf[i] = buf[i + 1];
+      if (more_ld) {
+        load_piece(a, ld, t, buf[DEPTH - 1]);
+        more_ld = ld.next(a);
+      }
+      if (st.is_v()) {
+        fence_proxy_async_smem();
+        warp_arrive(bar(V_FULL + vs));
+      } else if (st.piece == decltype(st)::PER - 2) {
+        fence_proxy_async_smem();
+        warp_arrive(bar(QK_FULL + qs));
+      }
+      more = st.next(a);
+    }
+  } else if (warp == 8) {
+    // ------------------------------------------------------------ MMA issue
+    if (elect_one()) {
+      int total = 0;
+      for (int u = blockIdx.x; u < a.n_units; u += gridDim.x) total += mix_unit<DK>(a, u).chunks;
+      constexpr uint32_t idS = make_idesc(128, 128, 1, false, false), idV = make_idesc(128, 64, 1, false, true),
+                         idKV = make_idesc(128, 64, 1, true, true);
+      auto wait = [&](int i, int phase) { return mbar_wait(bar(i), phase & 1, status); };
+      auto issue_S = [&](int g) {
+        const int s = g % C::QKS;
+        if (!wait(QK_FULL + s, g / C::QKS)) return false;
+        tc_fence_after();
+#pragma unroll
+        for (int term = 0; term < NT; ++term) {
+          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
+          const uint64_t kd = make_sdesc(sK(s) + (term == 1 ? KT * kTile : 0), 16, 1024);
+#pragma unroll
+          for (int k = 0; k < DK / 16; ++k) {
+            const uint32_t off = ((k / 4) * kTile + (k % 4) * 32) >> 4;
+            umma_f16_ss(tmem + T_S + (g & 1) * 128, qd + off, kd + off, idS, (term > 0 || k > 0) ? 1u : 0u);
+          }
+        }
+        umma_commit(bar(S_FULL + (g & 1)));
+        return true;
+      };
+      bool ok = true;
+      for (int g = 0; ok && g < total; ++g) {
+        const int s = g % C::QKS, vs = g % C::VS, b = g & 1;
+        if (STATES) ok = wait(QK_FULL + s, g / C::QKS);
+        else if (g == 0) ok = issue_S(0);
+        // K^T V' (DK = 64: both halves of the 128 rows are the same 64 rows of the
+        // state, so every warp of the state finds its columns in its own lanes)
+        ok = ok && wait(V_FULL + vs, g / C::VS) && (g < 2 || wait(KV_FREE + b, (g >> 1) - 1));
+        if (!ok) break;
+        tc_fence_after();
+        constexpr int KV_TERMS = NT == 3 ? 3 : 2;
+#pragma unroll
+        for (int term = 0; term < KV_TERMS; ++term) {
+          const uint64_t kd = make_sdesc(sK(s) + (term == 2 ? KT * kTile : 0), DK == 64 ? 0 : kTile, 1024);
+          const uint64_t vd = make_sdesc(sV(vs) + (NP + (term == 1 ? 1 : 0)) * kTile, kTile, 1024);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ss(tmem + T_KV + b * 64, kd + (k * 2048 >> 4), vd + (k * 2048 >> 4), idKV,
+                        (term > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(bar(KV_FULL + b));
+        if (STATES) {
+          umma_commit(bar(QK_EMPTY + s));
+          umma_commit(bar(V_EMPTY + vs));
+          continue;
+        }
+        if (g + 1 < total && !(ok = issue_S(g + 1))) break;
+        // Q S from the state entering this chunk
+        const int sb = g % C::STB;
+        ok = wait(ST_FULL + sb, g / C::STB) && (g < 1 || wait(O_FREE, g - 1));
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int term = 0; term < KV_TERMS; ++term) {
+          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
+          const uint64_t sd = make_sdesc(sS(sb) + (term == 1 ? C::ST_PLANE : 0), kTile, 1024);
+#pragma unroll
+          for (int k = 0; k < DK / 16; ++k)
+            umma_f16_ss(tmem + T_QS, qd + (((k / 4) * kTile + (k % 4) * 32) >> 4), sd + (k * 2048 >> 4), idV,
+                        (term > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(bar(ST_EMPTY + sb));
+        umma_commit(bar(QK_EMPTY + s));
+        // P V
+        if (!(ok = wait(P_FULL + b, g >> 1))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int term = 0; term < NT; ++term) {
+          const uint64_t vd = make_sdesc(sV(vs) + (term == 1 ? kTile : 0), kTile, 1024);
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            umma_f16_ts(tmem + T_PV, tmem + T_S + b * 128 + (term == 2 ? 64 : 0) + k * 8, vd + (k * 2048 >> 4), idV,
+                        (term > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(bar(V_EMPTY + vs));
+        umma_commit(bar(O_FULL));
+      }
+    }
+  } else if (warp < 4) {
+    // ------------------------------------------------------------ P
+    if (!STATES) {
+      const int i = threadIdx.x;
+      float* w = wtab + 16 * warp * (warp + 1);
+      int g = 0;
+      bool ok = true;
+      for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+        const MixUnit x = mix_unit<DK>(a, u);
+        if (x.chunks == 0) continue;
+        // l^0 .. l^i for this warp's rows
+        const float l2 = log2_decay(a.log_decay, x.h);
+        __syncwarp();
+        for (int d = lane_id(); d < 32 * (warp + 1); d += 32) w[d] = exp2f(l2 * static_cast<float>(d));
+        __syncwarp();
+        for (int c = 0; c < x.chunks; ++c, ++g) {
+          if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
+          tc_fence_after();
+          const uint32_t ts = tmem + T_S + (g & 1) * 128 + lane_base;
+          uint32_t lo[3][16];  // lo parts wait until their columns' scores are loaded
+#pragma unroll
+          for (int cb = 0; cb < 4; ++cb) {
+            uint32_t hi[16];
+            if (cb <= (warp & 3)) {
+              uint32_t r[32];
+              tmem_ld32_sync(ts + cb * 32, r);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                const int d = i - cb * 32 - 2 * j;
+                const float p0 = d >= 0 ? __uint_as_float(r[2 * j]) * w[d] : 0.f;
+                const float p1 = d >= 1 ? __uint_as_float(r[2 * j + 1]) * w[d - 1] : 0.f;
+                hi[j] = pack_bf16x2(p0, p1);
+                if (NT == 3) lo[cb < 3 ? cb : 0][j] = lo_pair(p0, p1, hi[j]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) {
+                hi[j] = 0;
+                if (NT == 3) lo[cb < 3 ? cb : 0][j] = 0;
+              }
+            }
+            if (NT == 3) {
+              // hi 16 cb .., lo 64 + 16 cb ..: over columns loaded by now
+              if (cb == 2) {
+                // scores 64-95 are in registers: lo of blocks 0 and 1 go over them
+                tmem_st16(ts + 64, lo[0]);
+                tmem_st16(ts + 80, lo[1]);
+              }
+              if (cb == 3) {
+                tmem_st16(ts + 96, lo[2]);
+                tmem_st16(ts + 112, lo[0]);
+              }
+            }
+            tmem_st16(ts + cb * 16, hi);
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          warp_arrive(bar(P_FULL + (g & 1)));
+        }
+      }
+    }
+  } else {
+    // ------------------------------------------------------------ state and output
+    const int r = threadIdx.x - 128;
+    constexpr int NC = C::NC;
+    const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
+    int g = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+      const MixUnit x = mix_unit<DK>(a, u);
+      const MixOne& one = a.one[x.dir];
+      const float l2 = log2_decay(a.log_decay, x.h);
+      const bool in_state = row < a.D && x.half * 64 + col0 < a.D;  // head dim 32: a quarter of the tile
+      const size_t st0 = (static_cast<size_t>(x.b) * a.H + x.h) * a.D * a.D;
+      // element (row, col) of the caller's state
+      auto state_at = [&](int c) {
+        const int e = x.half * 64 + col0 + c;
+        return st0 + (one.dir.transposed ? static_cast<size_t>(e) * a.D + row : static_cast<size_t>(row) * a.D + e);
+      };
+      float S[NC];
+      if (a.n_seg == 1 || (STATES && x.seg == 0)) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c) S[c] = one.s_in && in_state ? one.dir.in_mult * one.s_in[state_at(c)] : 0.f;
+      }
+      if (STATES) {
+        if (x.seg == 0) {
+          float4* dst = reinterpret_cast<float4*>(seg_slot<DK>(a, x, a.n_seg - 1));
+#pragma unroll
+          for (int c = 0; c < NC / 4; ++c) dst[c * 128 + r] = make_float4(S[4 * c], S[4 * c + 1], S[4 * c + 2], S[4 * c + 3]);
+        }
+#pragma unroll
+        for (int c = 0; c < NC; ++c) S[c] = 0.f;
+      } else if (a.n_seg > 1) {
+        // the state entering this segment from the segments before it
+        auto add = [&](int slot, float w, bool first) {
+          const float4* src = reinterpret_cast<const float4*>(seg_slot<DK>(a, x, slot));
+#pragma unroll
+          for (int c = 0; c < NC / 4; ++c) {
+            const float4 f = src[c * 128 + r];
+            S[4 * c] = fmaf(w, f.x, first ? 0.f : S[4 * c]);
+            S[4 * c + 1] = fmaf(w, f.y, first ? 0.f : S[4 * c + 1]);
+            S[4 * c + 2] = fmaf(w, f.z, first ? 0.f : S[4 * c + 2]);
+            S[4 * c + 3] = fmaf(w, f.w, first ? 0.f : S[4 * c + 3]);
+          }
+        };
+        add(a.n_seg - 1, x.seg == 0 ? 1.f : exp2f(l2 * static_cast<float>(x.p0 - one.dir.lead)), true);
+        for (int f = 0; f < x.seg && x.count > 0; ++f)
+          add(f, exp2f(l2 * static_cast<float>(x.p0 - (f + 1) * a.seg_tokens)), false);
+      }
+      // the state's bf16 parts for chunk gg's Q S
+      auto put_state = [&](int gg) {
+        const int sb = gg % C::STB;
+        if (gg >= C::STB && !mbar_wait_warp(bar(ST_EMPTY + sb), (gg / C::STB - 1) & 1, status)) return false;
+#pragma unroll
+        for (int c = 0; c < NC / 8; ++c) {
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            h[j] = pack_bf16x2(S[8 * c + 2 * j], S[8 * c + 2 * j + 1]);
+            l[j] = lo_pair(S[8 * c + 2 * j], S[8 * c + 2 * j + 1], h[j]);
+          }
+          const uint32_t at = sS(sb) + sw128_offset(row, col0 * 2 + c * 16);
+          st_shared_v4(at, h[0], h[1], h[2], h[3]);
+          st_shared_v4(at + C::ST_PLANE, l[0], l[1], l[2], l[3]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(bar(ST_FULL + sb));
+        return true;
+      };
+      if (!STATES && x.chunks > 0 && !(ok = put_state(g))) break;
+      for (int c = 0; c < x.chunks; ++c, ++g) {
+        const int left = x.count - c * 128, valid = left < 128 ? left : 128;
+        // the carried state enters the very first token without a decay (lead)
+        const int lead = c == 0 && x.seg == 0 && !STATES ? one.dir.lead : 0;
+        if (!(ok = mbar_wait_warp(bar(KV_FULL + (g & 1)), (g >> 1) & 1, status))) break;
+        tc_fence_after();
+        const float dec = exp2f(l2 * static_cast<float>(valid - lead));
+#pragma unroll
+        for (int j = 0; j < NC / 16; ++j) {
+          uint32_t v[16];
+          tmem_ld16(tmem + T_KV + (g & 1) * 64 + col0 + j * 16 + lane_base, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) S[16 * j + e] = fmaf(dec, S[16 * j + e], __uint_as_float(v[e]));
+        }
+        tc_fence_before();
+        warp_arrive(bar(KV_FREE + (g & 1)));
+        if (STATES) continue;
+        if (c + 1 < x.chunks && !(ok = put_state(g + 1))) break;
+        if (!(ok = mbar_wait_warp(bar(O_FULL), g & 1, status))) break;
+        tc_fence_after();
+        const int pos = x.p0 + c * 128 + r;
+        const int tok = one.dir.reverse ? x.n - 1 - pos : pos;
+        const float wq = a.scale * exp2f(l2 * static_cast<float>(r + 1 - lead));
+        T* dst = static_cast<T*>(one.o) + ((static_cast<size_t>(x.b) * a.L + tok) * a.H + x.h) * a.D + x.half * 64;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          uint32_t o1[16], o2[16];
+          tmem_ld16x2_sync(tmem + T_QS + j * 16 + lane_base, tmem + T_PV + j * 16 + lane_base, o1, o2);
+          if (j == 3) {
+            tc_fence_before();
+            warp_arrive(bar(O_FREE));
+          }
+          float v[16];
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            v[e] = fmaf(wq, __uint_as_float(o1[e]), a.scale * __uint_as_float(o2[e]));
+          if (r < valid && x.half * 64 + j * 16 < a.D) store16(dst + j * 16, v, one.dir.accumulate);
+        }
+      }
+      if (!ok) break;
+      if (STATES) {
+        if (x.seg < a.n_seg - 1) {
+          float4* dst = reinterpret_cast<float4*>(seg_slot<DK>(a, x, x.seg));
+#pragma unroll
+          for (int c = 0; c < NC / 4; ++c) dst[c * 128 + r] = make_float4(S[4 * c], S[4 * c + 1], S[4 * c + 2], S[4 * c + 3]);
+        }
+        continue;
+      }
+      // after the last token's segment (the first one of an empty sequence)
+      if (one.s_out && in_state && x.seg == (x.n > 0 ? (x.n - 1) / a.seg_tokens : 0)) {
+        const float w = one.dir.out_mult * (one.dir.lead && x.n > 0 ? exp2f(l2) : 1.f);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) one.s_out[state_at(c)] = w * S[c];
+      }
+      if (!one.dir.accumulate) {  // zeros past the sequence
+        const int p1 = a.L - x.p0 < a.seg_tokens ? a.L : x.p0 + a.seg_tokens;
+        const int pz = x.n > x.p0 ? x.n : x.p0;
+        const int vecs = (a.D < 64 ? a.D : 64) * static_cast<int>(sizeof(T)) / 16;
+        const long long zeros = static_cast<long long>(p1 - pz) * vecs;
+        for (long long i = r; i < zeros; i += 128) {
+          const size_t tok = static_cast<size_t>(x.b) * a.L + pz + i / vecs;
+          reinterpret_cast<uint4*>(static_cast<T*>(one.o) + (tok * a.H + x.h) * a.D + x.half * 64)[i % vecs] =
+              make_uint4(0, 0, 0, 0);
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -122,23 +732,63 @@ __global__ void __launch_bounds__(256)
   }
 }
 
-template <typename T, int D>
-int mix(const AttnShape& sh, const void* q, const void* k, const void* v, void* o, const float* log_decay,
-        const int32_t* lens, const float* s_in, float* s_out, const MixDir& dir, cudaStream_t s) {
-  mix_scan_kernel<T, D><<<sh.B * sh.H, D, 0, s>>>(
-      static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), static_cast<T*>(o),
-      log_decay, lens, s_in, s_out, sh.L, sh.H, sh.scale, dir);
+// Segments of one sequence. A sequence's chunks follow one another, so with few
+// (sequence, head) pairs most of the GPU would idle: the sequence is cut, the
+// segments' own states are computed first (k and v are read a second time) and
+// each segment starts from their sum.
+struct MixPlan {
+  int n_seg, seg_tokens, units;
+};
+MixPlan mix_plan(const AttnShape& sh, int n_dir) {
+  MixPlan p;
+  const int chunks = (sh.L + 127) / 128;
+  const long long pairs = static_cast<long long>(sh.B) * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
+  long long seg = device_sm_count() / pairs;
+  if (seg > chunks / 4) seg = chunks / 4;
+  if (seg < 1) seg = 1;
+  const int seg_chunks = static_cast<int>((chunks + seg - 1) / seg);
+  p.n_seg = (chunks + seg_chunks - 1) / seg_chunks;
+  p.seg_tokens = seg_chunks * 128;
+  p.units = static_cast<int>(pairs) * p.n_seg;
+  return p;
+}
+
+template <typename T, int DK, int NT>
+int mix_launch(MixArgs a, uint32_t* status, cudaStream_t s) {
+  using C = MixCfg<DK, NT>;
+  static std::atomic<uint64_t> attr_s{0}, attr{0};
+  const int sms = device_sm_count();
+  if (a.n_seg > 1) {
+    if (!ensure_smem_attr(mix_kernel<T, DK, NT, true>, C::SMEM, attr_s)) return PA_ERR_LAUNCH;
+    MixArgs f = a;
+    f.n_units = a.n_units / a.n_seg * (a.n_seg - 1);
+    mix_kernel<T, DK, NT, true><<<f.n_units < sms ? f.n_units : sms, kMixThreads, C::SMEM, s>>>(f, status);
+    if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
+  }
+  if (!ensure_smem_attr(mix_kernel<T, DK, NT, false>, C::SMEM, attr)) return PA_ERR_LAUNCH;
+  mix_kernel<T, DK, NT, false><<<a.n_units < sms ? a.n_units : sms, kMixThreads, C::SMEM, s>>>(a, status);
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
-int mix_any(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v, void* o,
-            const float* log_decay, const int32_t* lens, const float* s_in, float* s_out,
-            const MixDir& dir, cudaStream_t s) {
-  if (f32)
-    return sh.D == 32 ? mix<float, 32>(sh, q, k, v, o, log_decay, lens, s_in, s_out, dir, s)
-                      : mix<float, 64>(sh, q, k, v, o, log_decay, lens, s_in, s_out, dir, s);
-  return sh.D == 64 ? mix<__nv_bfloat16, 64>(sh, q, k, v, o, log_decay, lens, s_in, s_out, dir, s)
-                    : mix<__nv_bfloat16, 128>(sh, q, k, v, o, log_decay, lens, s_in, s_out, dir, s);
+int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const int32_t* lens, void* ws,
+        uint32_t* status, cudaStream_t s) {
+  const MixPlan p = mix_plan(sh, a.n_dir);
+  a.log_decay = log_decay;
+  a.lens = lens;
+  a.ws = static_cast<float*>(ws);
+  a.B = sh.B;
+  a.L = sh.L;
+  a.H = sh.H;
+  a.D = sh.D;
+  a.n_seg = p.n_seg;
+  a.seg_tokens = p.seg_tokens;
+  a.n_units = p.units;
+  a.scale = sh.scale;
+  if (!f32)
+    return sh.D == 64 ? mix_launch<__nv_bfloat16, 64, 1>(a, status, s)
+                      : mix_launch<__nv_bfloat16, 128, 1>(a, status, s);
+  return f32_math() == PA_F32_MATH_BF16 ? mix_launch<float, 64, 1>(a, status, s)
+                                        : mix_launch<float, 64, 3>(a, status, s);
 }
 
 template <typename T, int D>
@@ -152,31 +802,43 @@ int step(const AttnShape& sh, const void* q, const void* k, const void* v, const
 
 }  // namespace
 
-size_t linear_attn_workspace_bytes(const AttnShape&, bool, bool) { return 0; }
+size_t linear_attn_workspace_bytes(const AttnShape& sh, bool, bool backward) {
+  const MixPlan p = mix_plan(sh, backward ? 3 : 1);
+  return p.n_seg == 1 ? 0 : static_cast<size_t>(p.units) * (sh.D == 128 ? 128 : 64) * 64 * sizeof(float);
+}
 
 int launch_linear_attn_fwd(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,
                            const float* log_decay, const int32_t* lens, const float* s_in, void* o,
-                           float* s_out, void*, uint32_t*, cudaStream_t s) {
-  return mix_any(sh, f32, q, k, v, o, log_decay, lens, s_in, s_out, MixDir{}, s);
+                           float* s_out, void* ws, uint32_t* status, cudaStream_t s) {
+  MixArgs a{};
+  a.n_dir = 1;
+  a.one[0] = MixOne{q, k, v, o, s_in, s_out, MixDir{}};
+  return mix(sh, f32, a, log_decay, lens, ws, status, s);
 }
 
 int launch_linear_attn_bwd(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,
                            const void* dO, const float* log_decay, const int32_t* lens,
                            const float* s_in, const float* ds_out, void* dq, void* dk, void* dv,
-                           float* ds_in, bool accumulate, void*, uint32_t*, cudaStream_t s) {
+                           float* ds_in, bool accumulate, void* ws, uint32_t* status, cudaStream_t s) {
+  // The backward recurrence keeps U / scale, so one product with scale gives
+  // dk and dv: the gradient of the state enters divided by it and leaves
+  // multiplied.
   MixDir d;
   d.accumulate = accumulate;
   d.transposed = true;
-  int st = mix_any(sh, f32, dO, v, k, dq, log_decay, lens, s_in, nullptr, d, s);
-  if (st != PA_OK) return st;
-  d.reverse = true;
-  d.lead = 1;
-  d.in_mult = 1.f / sh.scale;
-  d.out_mult = sh.scale;
-  st = mix_any(sh, f32, v, dO, q, dk, log_decay, lens, ds_out, nullptr, d, s);
-  if (st != PA_OK) return st;
-  d.transposed = false;
-  return mix_any(sh, f32, k, q, dO, dv, log_decay, lens, ds_out, ds_in, d, s);
+  MixDir dk_dir = d;
+  dk_dir.reverse = true;
+  dk_dir.lead = 1;
+  dk_dir.in_mult = 1.f / sh.scale;
+  dk_dir.out_mult = sh.scale;
+  MixDir dv_dir = dk_dir;
+  dv_dir.transposed = false;
+  MixArgs a{};
+  a.n_dir = 3;
+  a.one[0] = MixOne{k, q, dO, dv, ds_out, ds_in, dv_dir};
+  a.one[1] = MixOne{v, dO, q, dk, ds_out, nullptr, dk_dir};
+  a.one[2] = MixOne{dO, v, k, dq, s_in, nullptr, d};
+  return mix(sh, f32, a, log_decay, lens, ws, status, s);
 }
 
 int launch_linear_attn_step(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,

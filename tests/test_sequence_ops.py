@@ -90,7 +90,7 @@ def test_linear_attention_pointer_refusals():
     for name in ("q", "k", "v", "dO", "dq", "dk", "dv", "s", "ds", "dsi"):
         assert bwd(**{name: 8}) == ALIGN
     assert bwd(dq=16) == SHAPE and bwd(dk=64) == SHAPE and bwd(dv=96) == SHAPE
-    assert bwd(s=160, dsi=160) == SHAPE
+    assert bwd(s=160, dsi=160) == SHAPE and bwd(ds=160, dsi=160) == SHAPE
     step = lambda L=1, q=16, k=32, v=48, ld=64, s=80, o=96, so=112: lib.pa_linear_attn_step(
         _desc(L=L), q, k, v, ld, s, o, so, None)
     assert step(L=2) == SHAPE and step(o=16) == SHAPE
