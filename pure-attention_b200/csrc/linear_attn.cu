@@ -45,14 +45,16 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // One CTA per SM walks units (sequence, head, 64 columns of V, segment of the
 // sequence); a unit's chunks follow one another through the state, and the
 // rings below run on across units.
-//   warps 0-3   P: load Q K^T from TMEM, times l^(i-j), bf16 back to TMEM
+//   warps 0-3   P: load Q K^T from TMEM, times l^(i-j), bf16 back to TMEM; then the
+//               previous chunk's O out
 //   warps 4-7   the state in fp32 registers (thread = row of the state), its bf16
-//               parts to shared memory for Q S; then O out
+//               parts to shared memory for Q S
 //   warp 8      tcgen05.mma issue
-//   warps 9-16  loads: global memory -> registers (pieces of 128 x 64 values, some
-//               always in flight) -> 128-byte swizzled tiles. Rows past the
-//               sequence are zeros, rows may run backwards in time, and fp32 is
-//               split here: none of these fits a plain TMA box.
+//   warps 9-12  k and q into 128-byte swizzled tiles: bf16 by cp.async, fp32 through
+//               registers, split on the way
+//   warps 13-16 v through registers into V and V'
+//               (Rows past the sequence are zeros, rows may run backwards in
+//               time, and fp32 is split: none of these fits a plain TMA box.)
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
@@ -61,8 +63,12 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // as in the softmax kernels. NT = 3 (fp32 operands): every operand is a
 // hi/lo pair and every product hi*hi + hi*lo + lo*hi.
 //
-// TMEM columns: Q K^T and P 2 x 128 (P over its own scores: hi 0-63, lo 64-127),
-// Q S 64, P V 64, K^T V' 2 x 64.
+// TMEM columns: Q K^T and P 2 x 128 (P of 32 tokens over their 32 scores: hi in the
+// first 16 columns, lo in the others), Q S 64, P V 64, K^T V' 2 x 64.
+//
+// The loops below stay rolled where they can: six roles that each run a long
+// straight line once per chunk miss the instruction cache (measured: 38% of the
+// stall cycles, 5500 against XXXX clocks a chunk).
 constexpr int kMixThreads = 17 * 32;
 constexpr int kTile = 128 * 128;  // bytes of 128 rows x 64 bf16
 
@@ -138,30 +144,18 @@ __device__ __forceinline__ float* seg_slot(const MixArgs& a, const MixUnit& x, i
   return a.ws + (w * a.n_seg + slot) * (DK * 64);
 }
 
-// A piece is 128 rows x 64 values of one operand; thread t of 256 holds the
-// 16-byte vectors t, t + 256, ...
-template <typename T>
-struct Piece {
-  static constexpr int VECS = sizeof(T) == 2 ? 4 : 8;
-  static constexpr int PER_ROW = 64 * static_cast<int>(sizeof(T)) / 16;
-  uint4 r[VECS];
-};
-
 __device__ __forceinline__ uint32_t lo_pair(float a, float b, uint32_t hi) {
   return pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
 }
 
-// The loads in order: per chunk the k pieces, the q pieces (not for segment
-// states), the v piece.
-template <int DK, bool STATES>
-struct PieceIter {
+// The chunks of this CTA in order, for the loading warps.
+template <int DK>
+struct ChunkIter {
   MixUnit x;
-  int u, chunk, piece, g;  // g: chunks of this CTA so far
-  static constexpr int KT = DK / 64;
-  static constexpr int PER = STATES ? KT + 1 : 2 * KT + 1;
+  int u, chunk, g;  // g: chunks of this CTA so far
   __device__ __forceinline__ bool first(const MixArgs& a) {
     u = blockIdx.x;
-    chunk = piece = g = 0;
+    chunk = g = 0;
     return settle(a);
   }
   __device__ __forceinline__ bool settle(const MixArgs& a) {  // to a unit that has chunks
@@ -172,41 +166,52 @@ struct PieceIter {
     return false;
   }
   __device__ __forceinline__ bool next(const MixArgs& a) {
-    if (++piece < PER) return true;
-    piece = 0;
     ++g;
     if (++chunk < x.chunks) return true;
     chunk = 0;
     u += gridDim.x;
     return settle(a);
   }
-  __device__ __forceinline__ bool is_v() const { return piece == PER - 1; }
-  __device__ __forceinline__ bool is_q() const { return !STATES && piece >= KT && piece < 2 * KT; }
   __device__ __forceinline__ int valid() const {  // valid rows of the chunk
     const int left = x.count - chunk * 128;
     return left < 128 ? left : 128;
   }
 };
 
-template <typename T, int DK, bool STATES>
-__device__ __forceinline__ void load_piece(const MixArgs& a, const PieceIter<DK, STATES>& it, int t, Piece<T>& p) {
-  using P = Piece<T>;
-  const MixOne& one = a.one[it.x.dir];
-  const void* base = it.is_v() ? one.v : (it.is_q() ? one.q : one.k);
-  const int tile = it.is_v() ? it.x.half : it.piece % (DK / 64);
-  const int row0 = t / P::PER_ROW, col = (t % P::PER_ROW) * (16 / static_cast<int>(sizeof(T)));
-  const int valid = it.valid();
-  const bool in_cols = tile * 64 + col < a.D;  // head dim 32 fills half a tile
-  const int pos = it.x.p0 + it.chunk * 128 + row0;
-  const bool rev = one.dir.reverse;
-  const long long tok0 = static_cast<long long>(it.x.b) * a.L + (rev ? it.x.n - 1 - pos : pos);
-  const long long step = static_cast<long long>(a.H) * a.D * (256 / P::PER_ROW) * (rev ? -1 : 1);
-  const T* src = static_cast<const T*>(base) + (tok0 * a.H + it.x.h) * a.D + tile * 64 + col;
-#pragma unroll
-  for (int i = 0; i < P::VECS; ++i) {
-    const bool ok = in_cols && row0 + i * (256 / P::PER_ROW) < valid;
-    p.r[i] = ok ? __ldg(reinterpret_cast<const uint4*>(src + i * step)) : make_uint4(0, 0, 0, 0);
+// Rows of 64 values (one column tile) of a chunk, dealt to the 128 threads of a
+// loading group in 16-byte vectors: thread t has column vector t % PER_ROW of rows
+// t / PER_ROW + i * ROWS.
+template <typename T>
+struct Rows {
+  static constexpr int PER_ROW = 64 * static_cast<int>(sizeof(T)) / 16;  // 8 or 16
+  static constexpr int ROWS = 128 / PER_ROW;                             // rows a pass: 16 or 8
+  const T* src;
+  long long step;
+  int row0, valid;  // valid = 0 past the head's columns
+  template <int DK>
+  __device__ __forceinline__ Rows(const MixArgs& a, const ChunkIter<DK>& it, const void* base, int tile, int t) {
+    const bool rev = a.one[it.x.dir].dir.reverse;
+    const int col = (t % PER_ROW) * (16 / static_cast<int>(sizeof(T)));
+    row0 = t / PER_ROW;
+    valid = tile * 64 + col < a.D ? it.valid() : 0;  // head dim 32 fills half a tile
+    const int pos = it.x.p0 + it.chunk * 128 + row0;
+    const long long tok = static_cast<long long>(it.x.b) * a.L + (rev ? it.x.n - 1 - pos : pos);
+    step = static_cast<long long>(a.H) * a.D * ROWS * (rev ? -1 : 1);
+    src = static_cast<const T*>(base) + (tok * a.H + it.x.h) * a.D + tile * 64 + col;
   }
+  __device__ __forceinline__ int row(int i) const { return row0 + i * ROWS; }
+  __device__ __forceinline__ uint4 load(int i) const {
+    return row(i) < valid ? __ldg(reinterpret_cast<const uint4*>(src + i * step)) : make_uint4(0, 0, 0, 0);
+  }
+};
+
+// 16 bytes global -> shared, zeros where !ok (nothing is read then).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+// One arrival on `bar` once this thread's cp.asyncs so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // Four (fp32) or eight (bf16) values of row `row` from byte column `cb` on, as
@@ -222,78 +227,74 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
-// A piece as an operand tile (hi, and lo where NP = 2).
-template <typename T, int NP>
-__device__ __forceinline__ void store_operand(const Piece<T>& p, int t, uint32_t hi, uint32_t lo) {
-  using P = Piece<T>;
-#pragma unroll
-  for (int i = 0; i < P::VECS; ++i) {
-    const int row = t / P::PER_ROW + i * (256 / P::PER_ROW);
-    if constexpr (sizeof(T) == 2) {
-      st_shared_v4(hi + sw128_offset(row, (t % 8) * 16), p.r[i].x, p.r[i].y, p.r[i].z, p.r[i].w);
-    } else {
-      put4(hi, NP == 2 ? lo : 0, sw128_offset(row, (t % 16) * 8), __uint_as_float(p.r[i].x),
-           __uint_as_float(p.r[i].y), __uint_as_float(p.r[i].z), __uint_as_float(p.r[i].w));
-    }
-  }
-}
-
-// A v piece as V' = diag(l^(valid - 1 - row)) V in two parts.
-template <typename T>
-__device__ __forceinline__ void store_decayed(const Piece<T>& p, int t, uint32_t hi, uint32_t lo, float l2, int valid) {
-  using P = Piece<T>;
-#pragma unroll
-  for (int i = 0; i < P::VECS; ++i) {
-    const int row = t / P::PER_ROW + i * (256 / P::PER_ROW);
-    const float w = row < valid ? exp2f(l2 * static_cast<float>(valid - 1 - row)) : 0.f;
-    if constexpr (sizeof(T) == 2) {
-      const uint32_t x[4] = {p.r[i].x, p.r[i].y, p.r[i].z, p.r[i].w};
-      uint32_t h[4], l[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float a = w * __uint_as_float(x[j] << 16), b = w * __uint_as_float(x[j] & 0xffff0000u);
-        h[j] = pack_bf16x2(a, b);
-        l[j] = lo_pair(a, b, h[j]);
-      }
-      const uint32_t off = sw128_offset(row, (t % 8) * 16);
-      st_shared_v4(hi + off, h[0], h[1], h[2], h[3]);
-      st_shared_v4(lo + off, l[0], l[1], l[2], l[3]);
-    } else {
-      put4(hi, lo, sw128_offset(row, (t % 16) * 8), w * __uint_as_float(p.r[i].x), w * __uint_as_float(p.r[i].y),
-           w * __uint_as_float(p.r[i].z), w * __uint_as_float(p.r[i].w));
-    }
-  }
-}
-
-// 16 values of an output row.
-__device__ __forceinline__ void store16(float* dst, const float* v, bool acc) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    float4 f = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-    if (acc) {
-      const float4 o = reinterpret_cast<const float4*>(dst)[i];
-      f.x += o.x; f.y += o.y; f.z += o.z; f.w += o.w;
-    }
-    reinterpret_cast<float4*>(dst)[i] = f;
-  }
-}
-__device__ __forceinline__ void store16(__nv_bfloat16* dst, const float* v, bool acc) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    uint32_t w[4];
-    uint4 o = make_uint4(0, 0, 0, 0);
-    if (acc) o = reinterpret_cast<const uint4*>(dst)[i];
-    const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+// V (hi, and lo where NP = 2; not for segment states) and V' = diag(l^(valid - 1 - row)) V
+// in two parts, from one vector of V.
+template <typename T, int NP, bool STATES>
+__device__ __forceinline__ void store_v(uint4 r, int row, int t, uint32_t at, float w) {
+  const uint32_t x[4] = {r.x, r.y, r.z, r.w};
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t off = sw128_offset(row, (t % 8) * 16);
+    if (!STATES) st_shared_v4(at + off, x[0], x[1], x[2], x[3]);
+    uint32_t h[4], l[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      float a = v[8 * i + 2 * j], b = v[8 * i + 2 * j + 1];
-      if (acc) {
-        a += __uint_as_float(ow[j] << 16);
-        b += __uint_as_float(ow[j] & 0xffff0000u);
-      }
-      w[j] = pack_bf16x2(a, b);
+      const float a = w * __uint_as_float(x[j] << 16), b = w * __uint_as_float(x[j] & 0xffff0000u);
+      h[j] = pack_bf16x2(a, b);
+      l[j] = lo_pair(a, b, h[j]);
     }
-    reinterpret_cast<uint4*>(dst)[i] = make_uint4(w[0], w[1], w[2], w[3]);
+    st_shared_v4(at + kTile + off, h[0], h[1], h[2], h[3]);
+    st_shared_v4(at + 2 * kTile + off, l[0], l[1], l[2], l[3]);
+  } else {
+    const uint32_t off = sw128_offset(row, (t % 16) * 8);
+    const float f[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+    if (!STATES) put4(at, NP == 2 ? at + kTile : 0, off, f[0], f[1], f[2], f[3]);
+    put4(at + NP * kTile, at + (NP + 1) * kTile, off, w * f[0], w * f[1], w * f[2], w * f[3]);
+  }
+}
+
+// Lane l of each group of 4 holds 4 16-byte vectors of row l; afterwards lane a holds
+// vector a of rows 0 .. 3, so that 4 lanes store 64 contiguous bytes (one row per
+// lane would spread every store over 32 rows).
+__device__ __forceinline__ void transpose4(uint4 (&v)[4]) {
+#pragma unroll
+  for (int s = 1; s < 4; s *= 2) {
+    const bool up = (lane_id() & s) != 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i & s) continue;
+      const uint4 give = up ? v[i] : v[i + s];
+      uint4 got;
+      got.x = __shfl_xor_sync(0xffffffffu, give.x, s);
+      got.y = __shfl_xor_sync(0xffffffffu, give.y, s);
+      got.z = __shfl_xor_sync(0xffffffffu, give.z, s);
+      got.w = __shfl_xor_sync(0xffffffffu, give.w, s);
+      if (up) v[i] = got;
+      else v[i + s] = got;
+    }
+  }
+}
+
+// f[0..15] += 16 values of an output row.
+__device__ __forceinline__ void add16(const float* src, float* f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float4 o = reinterpret_cast<const float4*>(src)[i];
+    f[4 * i] += o.x;
+    f[4 * i + 1] += o.y;
+    f[4 * i + 2] += o.z;
+    f[4 * i + 3] += o.w;
+  }
+}
+__device__ __forceinline__ void add16(const __nv_bfloat16* src, float* f) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint4 o = reinterpret_cast<const uint4*>(src)[i];
+    const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      f[8 * i + 2 * j] += __uint_as_float(w[j] << 16);
+      f[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
+    }
   }
 }
 
@@ -309,7 +310,7 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
   constexpr int NP = C::NP, KT = C::KT;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[26];
-  __shared__ float wtab[32 + 64 + 96 + 128];  // powers of the decay, a table for each P warp
+  __shared__ __align__(16) float wtab[256];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   if (cta_aborted(status, &abort_flag)) return;
@@ -328,11 +329,11 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
   const int warp = warp_id();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) {
-      mbar_init(bar(QK_FULL + i), 8);
+      mbar_init(bar(QK_FULL + i), 128);
       mbar_init(bar(QK_EMPTY + i), 1);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(V_FULL + i), 8);
+      mbar_init(bar(V_FULL + i), 4);
       mbar_init(bar(V_EMPTY + i), 1);
       mbar_init(bar(S_FULL + i), 1);
       mbar_init(bar(P_FULL + i), 4);
@@ -355,46 +356,105 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
   const uint32_t tmem = tmem_slot;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
 
-  if (warp >= 9) {
-    // ------------------------------------------------------------ loads
+  if (warp >= 13) {
+    // ------------------------------------------------------------ v: one chunk ahead in registers
+    const int t = threadIdx.x - 13 * 32;
+    constexpr int VECS = 128 / Rows<T>::ROWS;
+    uint4 r[VECS];
+    ChunkIter<DK> it;
+    bool more = it.first(a);
+    if (more) {
+      const Rows<T> rows(a, it, a.one[it.x.dir].v, it.x.half, t);
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) r[i] = rows.load(i);
+    }
+    float w[VECS];  // the rows' powers of the decay, kept while they stay the same
+    int w_unit = -1, w_valid = 0;
+    while (more) {
+      const int g = it.g, vs = g % C::VS, valid = it.valid();
+      if (it.u != w_unit || valid != w_valid) {
+        const float l2 = log2_decay(a.log_decay, it.x.h);
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) {
+          const int row = t / Rows<T>::PER_ROW + i * Rows<T>::ROWS;
+          w[i] = row < valid ? exp2f(l2 * static_cast<float>(valid - 1 - row)) : 0.f;
+        }
+        w_unit = it.u;
+        w_valid = valid;
+      }
+      if (g >= C::VS && !mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
+#pragma unroll
+      for (int i = 0; i < VECS; ++i) {
+        const int row = t / Rows<T>::PER_ROW + i * Rows<T>::ROWS;
+        store_v<T, NP, STATES>(r[i], row, t, sV(vs), w[i]);
+      }
+      fence_proxy_async_smem();
+      warp_arrive(bar(V_FULL + vs));
+      more = it.next(a);
+      if (more) {
+        const Rows<T> rows(a, it, a.one[it.x.dir].v, it.x.half, t);
+#pragma unroll
+        for (int i = 0; i < VECS; ++i) r[i] = rows.load(i);
+      }
+    }
+  } else if (warp >= 9) {
+    // ------------------------------------------------------------ k and q
     const int t = threadIdx.x - 9 * 32;
-    constexpr int DEPTH = sizeof(T) == 2 ? 3 : 2;  // pieces in flight
-    PieceIter<DK, STATES> ld, st;
-    Piece<T> buf[DEPTH];
-    bool more_ld = ld.first(a), more = st.first(a), ok = true;
+    constexpr int TILES = STATES ? KT : 2 * KT;  // k tiles, then q tiles
+    ChunkIter<DK> it;
+    bool more = it.first(a);
+    auto rows_of = [&](int tile) {
+      const MixOne& one = a.one[it.x.dir];
+      return Rows<T>(a, it, tile < KT ? one.k : one.q, tile % KT, t);
+    };
+    auto tile_at = [&](int s, int tile) { return (tile < KT ? sK(s) : sQ(s)) + (tile % KT) * kTile; };
+    if constexpr (sizeof(T) == 2) {
+      // straight into the ring; the barrier completes as the copies land
+      for (; more; more = it.next(a)) {
+        const int g = it.g, s = g % C::QKS;
+        if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+#pragma unroll 1
+        for (int tile = 0; tile < TILES; ++tile) {
+          const Rows<T> rows = rows_of(tile);
+          const uint32_t at = tile_at(s, tile);
 #pragma unroll
-    for (int i = 0; i < DEPTH; ++i)
-      if (more_ld) {
-        load_piece(a, ld, t, buf[i]);
-        more_ld = ld.next(a);
+          for (int i = 0; i < 8; ++i) {
+            const bool ok = rows.row(i) < rows.valid;
+            cp_async16(at + sw128_offset(rows.row(i), (t % 8) * 16), ok ? rows.src + i * rows.step : rows.src, ok);
+          }
+        }
+        cp_async_arrive(bar(QK_FULL + s));
       }
-    while (more && ok) {
-      const int g = st.g, qs = g % C::QKS, vs = g % C::VS;
-      if (st.piece == 0 && g >= C::QKS) ok = mbar_wait_warp(bar(QK_EMPTY + qs), (g / C::QKS - 1) & 1, status);
-      if (st.is_v() && g >= C::VS) ok = ok && mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status);
-      if (!ok) break;
-      if (st.is_v()) {
-        if (!STATES) store_operand<T, NP>(buf[0], t, sV(vs), sV(vs) + kTile);
-        store_decayed<T>(buf[0], t, sV(vs) + NP * kTile, sV(vs) + (NP + 1) * kTile,
-                         log2_decay(a.log_decay, st.x.h), st.valid());
-      } else {
-        const uint32_t at = (st.is_q() ? sQ(qs) : sK(qs)) + (st.piece % KT) * kTile;
-        store_operand<T, NP>(buf[0], t, at, at + KT * kTile);
-      }
+    } else {
+      // through registers, half a tile at a time, the next half always in flight
+      uint4 r0[8], r1[8];
+      auto load_half = [&](uint4 (&r)[8], int tile, int half) {
+        const Rows<T> rows = rows_of(tile);
 #pragma unroll
-      for (int i = 0; i + 1 < DEPTH; ++i) buf[i] = buf[i + 1];
-      if (more_ld) {
-        load_piece(a, ld, t, buf[DEPTH - 1]);
-        more_ld = ld.next(a);
-      }
-      if (st.is_v()) {
+        for (int j = 0; j < 8; ++j) r[j] = rows.load(half * 8 + j);
+      };
+      auto put_half = [&](const uint4 (&r)[8], uint32_t at, int half) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          put4(at, NP == 2 ? at + KT * kTile : 0, sw128_offset(t / 16 + (half * 8 + j) * 8, (t % 16) * 8),
+               __uint_as_float(r[j].x), __uint_as_float(r[j].y), __uint_as_float(r[j].z), __uint_as_float(r[j].w));
+      };
+      if (more) load_half(r0, 0, 0);
+      while (more) {
+        const int g = it.g, s = g % C::QKS;
+        if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+#pragma unroll 1
+        for (int tile = 0; tile < TILES; ++tile) {
+          const uint32_t at = tile_at(s, tile);
+          load_half(r1, tile, 1);
+          put_half(r0, at, 0);
+          if (tile + 1 == TILES) more = it.next(a);
+          if (more) load_half(r0, tile + 1 == TILES ? 0 : tile + 1, 0);
+          put_half(r1, at, 1);
+        }
         fence_proxy_async_smem();
-        warp_arrive(bar(V_FULL + vs));
-      } else if (st.piece == decltype(st)::PER - 2) {
-        fence_proxy_async_smem();
-        warp_arrive(bar(QK_FULL + qs));
+        mbar_arrive(bar(QK_FULL + s));
       }
-      more = st.next(a);
     }
   } else if (warp == 8) {
     // ------------------------------------------------------------ MMA issue
@@ -407,8 +467,9 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
       auto issue_S = [&](int g) {
         const int s = g % C::QKS;
         if (!wait(QK_FULL + s, g / C::QKS)) return false;
+        fence_proxy_async_smem();  // bf16: the copies' writes, before the tensor core reads them
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int term = 0; term < NT; ++term) {
           const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
           const uint64_t kd = make_sdesc(sK(s) + (term == 1 ? KT * kTile : 0), 16, 1024);
@@ -430,9 +491,10 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
         // state, so every warp of the state finds its columns in its own lanes)
         ok = ok && wait(V_FULL + vs, g / C::VS) && (g < 2 || wait(KV_FREE + b, (g >> 1) - 1));
         if (!ok) break;
+        if (STATES) fence_proxy_async_smem();
         tc_fence_after();
         constexpr int KV_TERMS = NT == 3 ? 3 : 2;
-#pragma unroll
+#pragma unroll 1
         for (int term = 0; term < KV_TERMS; ++term) {
           const uint64_t kd = make_sdesc(sK(s) + (term == 2 ? KT * kTile : 0), DK == 64 ? 0 : kTile, 1024);
           const uint64_t vd = make_sdesc(sV(vs) + (NP + (term == 1 ? 1 : 0)) * kTile, kTile, 1024);
@@ -453,7 +515,7 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
         ok = wait(ST_FULL + sb, g / C::STB) && (g < 1 || wait(O_FREE, g - 1));
         if (!ok) break;
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int term = 0; term < KV_TERMS; ++term) {
           const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
           const uint64_t sd = make_sdesc(sS(sb) + (term == 1 ? C::ST_PLANE : 0), kTile, 1024);
@@ -467,12 +529,13 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
         // P V
         if (!(ok = wait(P_FULL + b, g >> 1))) break;
         tc_fence_after();
-#pragma unroll
+#pragma unroll 1
         for (int term = 0; term < NT; ++term) {
           const uint64_t vd = make_sdesc(sV(vs) + (term == 1 ? kTile : 0), kTile, 1024);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + T_PV, tmem + T_S + b * 128 + (term == 2 ? 64 : 0) + k * 8, vd + (k * 2048 >> 4), idV,
+            umma_f16_ts(tmem + T_PV, tmem + T_S + b * 128 + (k / 2) * 32 + (term == 2 ? 16 : 0) + (k % 2) * 8,
+                        vd + (k * 2048 >> 4), idV,
                         (term > 0 || k > 0) ? 1u : 0u);
         }
         umma_commit(bar(V_EMPTY + vs));
@@ -480,68 +543,140 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
       }
     }
   } else if (warp < 4) {
-    // ------------------------------------------------------------ P
+    // ------------------------------------------------------------ P, then the previous chunk's O
     if (!STATES) {
-      const int i = threadIdx.x;
-      float* w = wtab + 16 * warp * (warp + 1);
+      const int i = threadIdx.x, lane = lane_id();
+      float* tab = wtab + 64 * warp;  // tab[j] = l^(31 - j), this warp's own; past 31 not used
       int g = 0;
       bool ok = true;
+      // the chunk whose output is due
+      T* o_base = nullptr;     // its first row, this head and column half
+      long long o_step = 0;    // values from one row to the next
+      int o_valid = 0;
+      float o_scale = 0.f;     // of Q S
+      bool o_add = false;
+      auto write_out = [&]() {
+        if (!mbar_wait_warp(bar(O_FULL), (g - 1) & 1, status)) return false;
+        tc_fence_after();
+        constexpr int COLS = 64 / static_cast<int>(sizeof(T));  // columns of 64 bytes
+        const int cols = a.D < 64 ? a.D : 64;
+#pragma unroll 1
+        for (int c0 = 0; c0 < cols; c0 += COLS) {
+          uint4 v[4];
+#pragma unroll
+          for (int c = 0; c < COLS; c += 16) {
+            uint32_t o1[16], o2[16];
+            tmem_ld16x2_sync(tmem + T_QS + c0 + c + lane_base, tmem + T_PV + c0 + c + lane_base, o1, o2);
+            float f[16];
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              f[e] = fmaf(o_scale, __uint_as_float(o1[e]), a.scale * __uint_as_float(o2[e]));
+            if (o_add && i < o_valid) add16(o_base + i * o_step + c0 + c, f);
+            if constexpr (sizeof(T) == 2) {
+              v[c / 8] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                                    pack_bf16x2(f[6], f[7]));
+              v[c / 8 + 1] = make_uint4(pack_bf16x2(f[8], f[9]), pack_bf16x2(f[10], f[11]),
+                                        pack_bf16x2(f[12], f[13]), pack_bf16x2(f[14], f[15]));
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = make_uint4(__float_as_uint(f[4 * e]), __float_as_uint(f[4 * e + 1]),
+                                  __float_as_uint(f[4 * e + 2]), __float_as_uint(f[4 * e + 3]));
+            }
+          }
+          if (c0 + COLS >= cols) {
+            tc_fence_before();
+            warp_arrive(bar(O_FREE));
+          }
+          transpose4(v);
+          const int r0 = 32 * warp + (lane & ~3);
+          T* dst = o_base + r0 * o_step + c0 + (lane & 3) * (16 / static_cast<int>(sizeof(T)));
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (r0 + k < o_valid) *reinterpret_cast<uint4*>(dst + k * o_step) = v[k];
+        }
+        return true;
+      };
       for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
         const MixUnit x = mix_unit<DK>(a, u);
         if (x.chunks == 0) continue;
-        // l^0 .. l^i for this warp's rows
+        const MixOne& one = a.one[x.dir];
         const float l2 = log2_decay(a.log_decay, x.h);
         __syncwarp();
-        for (int d = lane_id(); d < 32 * (warp + 1); d += 32) w[d] = exp2f(l2 * static_cast<float>(d));
+        tab[lane] = exp2f(l2 * static_cast<float>(31 - lane));
+        tab[32 + lane] = 0.f;
         __syncwarp();
-        for (int c = 0; c < x.chunks; ++c, ++g) {
+        const float l32 = exp2f(l2 * 32.f), l_first = exp2f(l2 * static_cast<float>(lane + 1));
+        for (int c = 0; c < x.chunks; ++c) {
           if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
           tc_fence_after();
           const uint32_t ts = tmem + T_S + (g & 1) * 128 + lane_base;
-          uint32_t lo[3][16];  // lo parts wait until their columns' scores are loaded
+          // P of 32 columns goes over their scores: hi in the first 16 columns, lo (NT = 3)
+          // in the next
+          auto put = [&](int cb, const float (&p)[32]) {
+            uint32_t h[16];
 #pragma unroll
-          for (int cb = 0; cb < 4; ++cb) {
-            uint32_t hi[16];
-            if (cb <= (warp & 3)) {
-              uint32_t r[32];
-              tmem_ld32_sync(ts + cb * 32, r);
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                const int d = i - cb * 32 - 2 * j;
-                const float p0 = d >= 0 ? __uint_as_float(r[2 * j]) * w[d] : 0.f;
-                const float p1 = d >= 1 ? __uint_as_float(r[2 * j + 1]) * w[d - 1] : 0.f;
-                hi[j] = pack_bf16x2(p0, p1);
-                if (NT == 3) lo[cb < 3 ? cb : 0][j] = lo_pair(p0, p1, hi[j]);
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < 16; ++j) {
-                hi[j] = 0;
-                if (NT == 3) lo[cb < 3 ? cb : 0][j] = 0;
-              }
-            }
+            for (int j = 0; j < 16; ++j) h[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
+            tmem_st16(ts + cb * 32, h);
             if (NT == 3) {
-              // hi 16 cb .., lo 64 + 16 cb ..: over columns loaded by now
-              if (cb == 2) {
-                // scores 64-95 are in registers: lo of blocks 0 and 1 go over them
-                tmem_st16(ts + 64, lo[0]);
-                tmem_st16(ts + 80, lo[1]);
-              }
-              if (cb == 3) {
-                tmem_st16(ts + 96, lo[2]);
-                tmem_st16(ts + 112, lo[0]);
-              }
+              uint32_t l[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) l[j] = lo_pair(p[2 * j], p[2 * j + 1], h[j]);
+              tmem_st16(ts + cb * 32 + 16, l);
             }
-            tmem_st16(ts + cb * 16, hi);
+          };
+          uint32_t r[32];
+          float p[32];
+          // on the diagonal: column j of row `lane` has l^(lane - j) = tab[31 - lane + j]
+          tmem_ld32_sync(ts + warp * 32, r);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) {
+            const float w = tab[31 - lane + j];
+            p[j] = j <= lane ? __uint_as_float(r[j]) * w : 0.f;
+          }
+          put(warp, p);
+          // left of it, nearest first: l^(i - j) = l^(i - 32 cb - 31) l^(31 - j), no negative exponent
+          float rf = l_first;
+#pragma unroll 1
+          for (int cb = warp - 1; cb >= 0; --cb) {
+            tmem_ld32_sync(ts + cb * 32, r);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = reinterpret_cast<const float4*>(tab)[j];
+              p[4 * j] = __uint_as_float(r[4 * j]) * (rf * f.x);
+              p[4 * j + 1] = __uint_as_float(r[4 * j + 1]) * (rf * f.y);
+              p[4 * j + 2] = __uint_as_float(r[4 * j + 2]) * (rf * f.z);
+              p[4 * j + 3] = __uint_as_float(r[4 * j + 3]) * (rf * f.w);
+            }
+            put(cb, p);
+            rf *= l32;
+          }
+          // right of it: zero
+#pragma unroll
+          for (int j = 0; j < 16; ++j) r[j] = 0;
+#pragma unroll 1
+          for (int cb = warp + 1; cb < 4; ++cb) {
+            tmem_st16(ts + cb * 32, r);
+            if (NT == 3) tmem_st16(ts + cb * 32 + 16, r);
           }
           tmem_st_wait();
           tc_fence_before();
           warp_arrive(bar(P_FULL + (g & 1)));
+          if (g > 0 && !(ok = write_out())) break;
+          const int pos = x.p0 + c * 128, left = x.count - c * 128;
+          const long long tok = static_cast<long long>(x.b) * a.L + (one.dir.reverse ? x.n - 1 - pos : pos);
+          o_step = static_cast<long long>(a.H) * a.D * (one.dir.reverse ? -1 : 1);
+          o_base = static_cast<T*>(one.o) + (tok * a.H + x.h) * a.D + x.half * 64;
+          o_valid = left < 128 ? left : 128;
+          o_add = one.dir.accumulate;
+          o_scale = a.scale * exp2f(l2 * static_cast<float>(i + 1 - (pos == 0 ? one.dir.lead : 0)));
+          ++g;
         }
       }
+      if (ok && g > 0) write_out();
     }
   } else {
-    // ------------------------------------------------------------ state and output
+    // ------------------------------------------------------------ state
     const int r = threadIdx.x - 128;
     constexpr int NC = C::NC;
     const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
@@ -628,26 +763,6 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
         warp_arrive(bar(KV_FREE + (g & 1)));
         if (STATES) continue;
         if (c + 1 < x.chunks && !(ok = put_state(g + 1))) break;
-        if (!(ok = mbar_wait_warp(bar(O_FULL), g & 1, status))) break;
-        tc_fence_after();
-        const int pos = x.p0 + c * 128 + r;
-        const int tok = one.dir.reverse ? x.n - 1 - pos : pos;
-        const float wq = a.scale * exp2f(l2 * static_cast<float>(r + 1 - lead));
-        T* dst = static_cast<T*>(one.o) + ((static_cast<size_t>(x.b) * a.L + tok) * a.H + x.h) * a.D + x.half * 64;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          uint32_t o1[16], o2[16];
-          tmem_ld16x2_sync(tmem + T_QS + j * 16 + lane_base, tmem + T_PV + j * 16 + lane_base, o1, o2);
-          if (j == 3) {
-            tc_fence_before();
-            warp_arrive(bar(O_FREE));
-          }
-          float v[16];
-#pragma unroll
-          for (int e = 0; e < 16; ++e)
-            v[e] = fmaf(wq, __uint_as_float(o1[e]), a.scale * __uint_as_float(o2[e]));
-          if (r < valid && x.half * 64 + j * 16 < a.D) store16(dst + j * 16, v, one.dir.accumulate);
-        }
       }
       if (!ok) break;
       if (STATES) {
