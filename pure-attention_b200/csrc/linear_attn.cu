@@ -35,26 +35,26 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 }
 
 // ---------------------------------------------------------------- chunked kernel
-// A sequence in chunks of C = 128 tokens. With S the state entering a chunk of n
-// valid tokens (rows i, j of the chunk; l the decay):
+// A sequence in chunks of 128 tokens. With S the state entering a chunk of n
+// valid tokens (rows i, j of the chunk; l the decay), forward in time:
 //   O   = scale (P V + diag(l^(i+1)) Q S),   P = (Q K^T) o l^(i-j) for j <= i, else 0
-//   S' = l^n S + K^T V',                      V' = diag(l^(n-1-j)) V
-// All four products run on the tensor cores; every power of l has a whole,
-// non-negative exponent, so nothing overflows where l is small.
+//   S'  = l^n S + K^T V',                     V' = diag(l^(n-1-j)) V
+// and backward in time, the chunks from the last on: P with l^(j-i) for j >= i,
+// diag(l^(n-i)), V' = diag(l^j) V. All four products run on the tensor cores;
+// every power of l has a whole, non-negative exponent, so nothing overflows where
+// l is small.
 //
 // One CTA per SM walks units (sequence, head, 64 columns of V, segment of the
 // sequence); a unit's chunks follow one another through the state, and the
 // rings below run on across units.
-//   warps 0-3   P: load Q K^T from TMEM, times l^(i-j), bf16 back to TMEM; then the
-//               previous chunk's O out
-//   warps 4-7   the state in fp32 registers (thread = row of the state), its bf16
+//   warps 0-7   P: load Q K^T from TMEM, times l^|i-j|, bf16 back to TMEM; then the
+//               previous chunk's O out (two warps share 32 rows: some blocks of P
+//               and 32 columns of O each)
+//   warps 8-11  the state in fp32 registers (thread = row of the state), its bf16
 //               parts to shared memory for Q S
-//   warp 8      tcgen05.mma issue
-//   warps 9-12  k and q into 128-byte swizzled tiles: bf16 by cp.async, fp32 through
-//               registers, split on the way
-//   warps 13-16 v through registers into V and V'
-//               (Rows past the sequence are zeros, rows may run backwards in
-//               time, and fp32 is split: none of these fits a plain TMA box.)
+//   warps 12-15 V' from V (fp32: and q, v through registers, split on the way)
+//   warps 16-17 bf16: TMA loads of q, k, v; fp32: k through registers
+//   warp 18     tcgen05.mma issue
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
@@ -64,12 +64,8 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // hi/lo pair and every product hi*hi + hi*lo + lo*hi.
 //
 // TMEM columns: Q K^T and P 2 x 128 (P of 32 tokens over their 32 scores: hi in the
-// first 16 columns, lo in the others), Q S 64, P V 64, K^T V' 2 x 64.
-//
-// The loops below stay rolled where they can: six roles that each run a long
-// straight line once per chunk miss the instruction cache (measured: 38% of the
-// stall cycles, 5500 against XXXX clocks a chunk).
-constexpr int kMixThreads = 17 * 32;
+// first 16 columns, lo in the others), Q S 64, P V 64, K^T [V' hi, V' lo] 128.
+constexpr int kMixThreads = 20 * 32;
 constexpr int kTile = 128 * 128;  // bytes of 128 rows x 64 bf16
 
 template <int DK, int NT>
@@ -77,15 +73,16 @@ struct MixCfg {
   static constexpr int NP = NT == 3 ? 2 : 1;       // planes (hi, lo) of q, k, v
   static constexpr int KT = DK / 64;               // 64-column tiles of q and k
   static constexpr int OPER = NP * KT * kTile;     // bytes of q (or k) of a stage
-  static constexpr int V_STAGE = (NP + 2) * kTile; // v, and V' hi and lo
+  static constexpr int V_STAGE = NP * kTile;       // v
+  static constexpr int VP_BYTES = 2 * kTile;       // V' hi and lo
   static constexpr int ST_PLANE = DK * 128;        // [DK, 64] bf16
   static constexpr bool SMALL = NP == 1 && DK == 64;
-  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 2 : 1, STB = DK == 64 ? 2 : 1;
-  static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + STB * 2 * ST_PLANE + 1024;
+  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 3 : (NP == 1 ? 2 : 1), STB = DK == 64 ? 2 : 1;
+  static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + VP_BYTES + STB * 2 * ST_PLANE + 1024;
   static constexpr int NC = DK == 64 ? 32 : 64;    // state columns of a thread
 };
-static_assert(MixCfg<64, 1>::SMEM <= 226 * 1024 && MixCfg<64, 3>::SMEM <= 226 * 1024 &&
-              MixCfg<128, 1>::SMEM <= 226 * 1024, "shared memory of one CTA");
+static_assert(MixCfg<64, 1>::SMEM <= 225 * 1024 && MixCfg<64, 3>::SMEM <= 225 * 1024 &&
+              MixCfg<128, 1>::SMEM <= 225 * 1024, "shared memory of one CTA");
 
 struct MixOne {  // one direction of the recurrence
   const void *q, *k, *v;
@@ -93,6 +90,8 @@ struct MixOne {  // one direction of the recurrence
   const float* s_in;
   float* s_out;
   MixDir dir;
+  int mq, mk, mv;  // bf16: the tensor maps of q, k, v
+  int mo;          // and of o
 };
 struct MixArgs {
   MixOne one[3];
@@ -104,17 +103,34 @@ struct MixArgs {
   int n_seg, seg_tokens, n_units;
   float scale;
 };
+struct MixMaps {
+  CUtensorMap m[4];  // inputs: 64 columns x 128 tokens
+  CUtensorMap o[3];  // outputs: 32 columns x 32 tokens
+};
 
 struct MixUnit {
   int dir, b, h, half, seg;
   int n;          // valid tokens of the sequence
-  int p0, count;  // first position and tokens of this segment
+  int p0, count;  // first token and tokens of this segment
   int chunks;
+  bool rev;
+  // Chunk c in the order of the recurrence: its first token, its valid tokens.
+  __device__ __forceinline__ int index(int c) const { return rev ? chunks - 1 - c : c; }
+  __device__ __forceinline__ int token(int c) const { return p0 + index(c) * 128; }
+  __device__ __forceinline__ int valid(int c) const {
+    const int left = count - index(c) * 128;
+    return left < 128 ? left : 128;
+  }
+  // the chunk that the carried state of the sequence enters
+  __device__ __forceinline__ bool starts(int c) const {
+    return rev ? token(c) + 128 >= n : token(c) == 0;
+  }
 };
 
 // unit -> (segment, sequence, head, direction, column half), halves and
-// directions of one head next to one another: they read the same rows, from L2
-template <int DK>
+// directions of one head next to one another: they read the same rows, from L2.
+// Segment states are wanted of all but the segment that comes last in time order.
+template <int DK, bool STATES>
 __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
   MixUnit x;
   constexpr int halves = DK / 64;
@@ -125,7 +141,8 @@ __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
   x.h = u % a.H;
   u /= a.H;
   x.b = u % a.B;
-  x.seg = u / a.B;
+  x.rev = a.one[x.dir].dir.reverse;
+  x.seg = u / a.B + (STATES && x.rev ? 1 : 0);
   x.n = valid_tokens(a.lens, x.b, a.L);
   x.p0 = x.seg * a.seg_tokens;
   const int left = x.n - x.p0;
@@ -135,8 +152,8 @@ __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
 }
 
 // Workspace of a sequence cut in segments: per (sequence, head, direction, half)
-// n_seg slots of [DK, 64] fp32. Slot s < n_seg - 1 holds the state of segment s
-// alone (from zero), slot n_seg - 1 a copy of the carried state (state_out may
+// n_seg slots of [DK, 64] fp32. The first n_seg - 1 hold the states of single
+// segments (from zero), the last a copy of the carried state (state_out may
 // overwrite state_in while other segments still need it).
 template <int DK>
 __device__ __forceinline__ float* seg_slot(const MixArgs& a, const MixUnit& x, int slot) {
@@ -144,12 +161,8 @@ __device__ __forceinline__ float* seg_slot(const MixArgs& a, const MixUnit& x, i
   return a.ws + (w * a.n_seg + slot) * (DK * 64);
 }
 
-__device__ __forceinline__ uint32_t lo_pair(float a, float b, uint32_t hi) {
-  return pack_bf16x2(a - __uint_as_float(hi << 16), b - __uint_as_float(hi & 0xffff0000u));
-}
-
-// The chunks of this CTA in order, for the loading warps.
-template <int DK>
+// The chunks of this CTA in order.
+template <int DK, bool STATES>
 struct ChunkIter {
   MixUnit x;
   int u, chunk, g;  // g: chunks of this CTA so far
@@ -160,7 +173,7 @@ struct ChunkIter {
   }
   __device__ __forceinline__ bool settle(const MixArgs& a) {  // to a unit that has chunks
     for (; u < a.n_units; u += gridDim.x) {
-      x = mix_unit<DK>(a, u);
+      x = mix_unit<DK, STATES>(a, u);
       if (x.chunks > 0) return true;
     }
     return false;
@@ -172,129 +185,92 @@ struct ChunkIter {
     u += gridDim.x;
     return settle(a);
   }
-  __device__ __forceinline__ int valid() const {  // valid rows of the chunk
-    const int left = x.count - chunk * 128;
-    return left < 128 ? left : 128;
-  }
+  __device__ __forceinline__ int valid() const { return x.valid(chunk); }
 };
 
-// Rows of 64 values (one column tile) of a chunk, dealt to the 128 threads of a
-// loading group in 16-byte vectors: thread t has column vector t % PER_ROW of rows
-// t / PER_ROW + i * ROWS.
-template <typename T>
-struct Rows {
-  static constexpr int PER_ROW = 64 * static_cast<int>(sizeof(T)) / 16;  // 8 or 16
-  static constexpr int ROWS = 128 / PER_ROW;                             // rows a pass: 16 or 8
-  const T* src;
-  long long step;
-  int row0, valid;  // valid = 0 past the head's columns
-  template <int DK>
-  __device__ __forceinline__ Rows(const MixArgs& a, const ChunkIter<DK>& it, const void* base, int tile, int t) {
-    const bool rev = a.one[it.x.dir].dir.reverse;
-    const int col = (t % PER_ROW) * (16 / static_cast<int>(sizeof(T)));
-    row0 = t / PER_ROW;
-    valid = tile * 64 + col < a.D ? it.valid() : 0;  // head dim 32 fills half a tile
-    const int pos = it.x.p0 + it.chunk * 128 + row0;
-    const long long tok = static_cast<long long>(it.x.b) * a.L + (rev ? it.x.n - 1 - pos : pos);
-    step = static_cast<long long>(a.H) * a.D * ROWS * (rev ? -1 : 1);
-    src = static_cast<const T*>(base) + (tok * a.H + it.x.h) * a.D + tile * 64 + col;
-  }
-  __device__ __forceinline__ int row(int i) const { return row0 + i * ROWS; }
-  __device__ __forceinline__ uint4 load(int i) const {
-    return row(i) < valid ? __ldg(reinterpret_cast<const uint4*>(src + i * step)) : make_uint4(0, 0, 0, 0);
-  }
-};
-
-// 16 bytes global -> shared, zeros where !ok (nothing is read then).
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool ok) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(ok ? 16 : 0) : "memory");
+// Pairs of fp32 values.
+__device__ __forceinline__ float2 pair_of(uint32_t a, uint32_t b) {
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
 }
-// One arrival on `bar` once this thread's cp.asyncs so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-
-// Four (fp32) or eight (bf16) values of row `row` from byte column `cb` on, as
-// bf16 hi and, where `lo` is not 0, lo.
-__device__ __forceinline__ void put4(uint32_t hi, uint32_t lo, uint32_t off, float a, float b, float c, float d) {
-  const uint32_t h0 = pack_bf16x2(a, b), h1 = pack_bf16x2(c, d);
-  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(hi + off), "r"(h0), "r"(h1) : "memory");
-  if (lo)
-    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(lo + off), "r"(lo_pair(a, b, h0)),
-                 "r"(lo_pair(c, d, h1)) : "memory");
+__device__ __forceinline__ uint32_t hi_pair(float2 v) { return pack_bf16x2(v.x, v.y); }
+__device__ __forceinline__ uint32_t lo_pair(float2 v, uint32_t hi) {
+  const float2 d = __fadd2_rn(v, make_float2(-__uint_as_float(hi << 16), -__uint_as_float(hi & 0xffff0000u)));
+  return pack_bf16x2(d.x, d.y);
 }
 __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
-
-// V (hi, and lo where NP = 2; not for segment states) and V' = diag(l^(valid - 1 - row)) V
-// in two parts, from one vector of V.
-template <typename T, int NP, bool STATES>
-__device__ __forceinline__ void store_v(uint4 r, int row, int t, uint32_t at, float w) {
-  const uint32_t x[4] = {r.x, r.y, r.z, r.w};
-  if constexpr (sizeof(T) == 2) {
-    const uint32_t off = sw128_offset(row, (t % 8) * 16);
-    if (!STATES) st_shared_v4(at + off, x[0], x[1], x[2], x[3]);
-    uint32_t h[4], l[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float a = w * __uint_as_float(x[j] << 16), b = w * __uint_as_float(x[j] & 0xffff0000u);
-      h[j] = pack_bf16x2(a, b);
-      l[j] = lo_pair(a, b, h[j]);
-    }
-    st_shared_v4(at + kTile + off, h[0], h[1], h[2], h[3]);
-    st_shared_v4(at + 2 * kTile + off, l[0], l[1], l[2], l[3]);
-  } else {
-    const uint32_t off = sw128_offset(row, (t % 16) * 8);
-    const float f[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
-    if (!STATES) put4(at, NP == 2 ? at + kTile : 0, off, f[0], f[1], f[2], f[3]);
-    put4(at + NP * kTile, at + (NP + 1) * kTile, off, w * f[0], w * f[1], w * f[2], w * f[3]);
-  }
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
+// Four fp32 values as bf16 hi and, where `lo` is not 0, lo.
+__device__ __forceinline__ void put4(uint32_t hi, uint32_t lo, uint32_t off, float2 a, float2 b) {
+  const uint32_t h0 = hi_pair(a), h1 = hi_pair(b);
+  asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(hi + off), "r"(h0), "r"(h1) : "memory");
+  if (lo)
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(lo + off), "r"(lo_pair(a, h0)), "r"(lo_pair(b, h1))
+                 : "memory");
 }
 
-// Lane l of each group of 4 holds 4 16-byte vectors of row l; afterwards lane a holds
-// vector a of rows 0 .. 3, so that 4 lanes store 64 contiguous bytes (one row per
-// lane would spread every store over 32 rows).
-__device__ __forceinline__ void transpose4(uint4 (&v)[4]) {
-#pragma unroll
-  for (int s = 1; s < 4; s *= 2) {
-    const bool up = (lane_id() & s) != 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (i & s) continue;
-      const uint4 give = up ? v[i] : v[i + s];
-      uint4 got;
-      got.x = __shfl_xor_sync(0xffffffffu, give.x, s);
-      got.y = __shfl_xor_sync(0xffffffffu, give.y, s);
-      got.z = __shfl_xor_sync(0xffffffffu, give.z, s);
-      got.w = __shfl_xor_sync(0xffffffffu, give.w, s);
-      if (up) v[i] = got;
-      else v[i + s] = got;
-    }
+// fp32 loads: the 64 columns of a chunk's rows, dealt to the N threads of a loading
+// group in 16-byte vectors: thread t has column vector t % 16 of rows t / 16 + i * N / 16.
+template <int N>
+struct Rows {
+  static constexpr int ROWS = N / 16;         // rows a pass
+  static constexpr int VECS = 128 / ROWS;     // vectors of a thread
+  const float* src;
+  long long step;
+  int row0, valid;  // valid = 0 past the head's columns
+  template <typename It>
+  __device__ __forceinline__ Rows(const MixArgs& a, const It& it, const void* base, int t) {
+    const int col = (t % 16) * 4;
+    row0 = t / 16;
+    valid = col < a.D ? it.valid() : 0;  // head dim 32 fills half a tile
+    const long long tok = static_cast<long long>(it.x.b) * a.L + it.x.token(it.chunk) + row0;
+    step = static_cast<long long>(a.H) * a.D * ROWS;
+    src = static_cast<const float*>(base) + (tok * a.H + it.x.h) * a.D + col;
   }
+  __device__ __forceinline__ float4 load(int i) const {
+    return row0 + i * ROWS < valid ? __ldg(reinterpret_cast<const float4*>(src + i * step))
+                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+};
+
+// Two 8-column TMEM loads and their wait.
+__device__ __forceinline__ void tmem_ld8x2_sync(uint32_t ta, uint32_t tb, uint32_t (&a)[8], uint32_t (&b)[8]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(b[0]),
+        "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7])
+      : "r"(ta), "r"(tb)
+      : "memory");
 }
 
-// f[0..15] += 16 values of an output row.
-__device__ __forceinline__ void add16(const float* src, float* f) {
+// 32 values of an output row += f.
+__device__ __forceinline__ void add_row(float* dst, const float2 (&f)[16]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float4 o = reinterpret_cast<const float4*>(dst)[i];
+    o.x += f[2 * i].x;
+    o.y += f[2 * i].y;
+    o.z += f[2 * i + 1].x;
+    o.w += f[2 * i + 1].y;
+    reinterpret_cast<float4*>(dst)[i] = o;
+  }
+}
+__device__ __forceinline__ void add_row(__nv_bfloat16* dst, const float2 (&f)[16]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const float4 o = reinterpret_cast<const float4*>(src)[i];
-    f[4 * i] += o.x;
-    f[4 * i + 1] += o.y;
-    f[4 * i + 2] += o.z;
-    f[4 * i + 3] += o.w;
-  }
-}
-__device__ __forceinline__ void add16(const __nv_bfloat16* src, float* f) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint4 o = reinterpret_cast<const uint4*>(src)[i];
+    const uint4 o = reinterpret_cast<const uint4*>(dst)[i];
     const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+    uint32_t y[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[8 * i + 2 * j] += __uint_as_float(w[j] << 16);
-      f[8 * i + 2 * j + 1] += __uint_as_float(w[j] & 0xffff0000u);
-    }
+    for (int j = 0; j < 4; ++j) y[j] = hi_pair(__fadd2_rn(f[4 * i + j], pair_of(w[j] << 16, w[j] & 0xffff0000u)));
+    reinterpret_cast<uint4*>(dst)[i] = make_uint4(y[0], y[1], y[2], y[3]);
   }
 }
 
@@ -303,50 +279,60 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   if (lane_id() == 0) mbar_arrive(bar);
 }
 
+// A descriptor `bytes` further on (its address field is the low 14 bits, in 16 bytes).
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) {
+  const uint32_t lo = static_cast<uint32_t>(desc) + (bytes >> 4);
+  return (desc & 0xffffffff00000000ull) | lo;
+}
+
 // STATES: only the segments' own states, into the workspace.
 template <typename T, int DK, int NT, bool STATES>
-__global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_constant__ MixArgs a, uint32_t* status) {
+__global__ void __launch_bounds__(kMixThreads, 1)
+    mix_kernel(const __grid_constant__ MixArgs a, const __grid_constant__ MixMaps maps, uint32_t* status) {
   using C = MixCfg<DK, NT>;
   constexpr int NP = C::NP, KT = C::KT;
+  constexpr bool TMA = sizeof(T) == 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[26];
-  __shared__ __align__(16) float wtab[256];  // powers of the decay, a table for each P warp
+  __shared__ uint64_t bars[26];  // N_BARS
+  __shared__ __align__(16) float wtab[4 * 64 + 4 * 32];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   if (cta_aborted(status, &abort_flag)) return;
   const uint32_t sm0 = smem_u32(align1024(smem_raw));
-  const uint32_t sv0 = sm0 + C::QKS * 2 * C::OPER, ss0 = sv0 + C::VS * C::V_STAGE;
+  const uint32_t sv0 = sm0 + C::QKS * 2 * C::OPER, sVp = sv0 + C::VS * C::V_STAGE, ss0 = sVp + C::VP_BYTES;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  // ring slot s: K planes, then Q planes; V, V' hi, V' lo; state hi, lo
+  // ring slot s: K planes, then Q planes; V planes; state hi, lo. V' hi, lo at sVp.
   auto sK = [&](int s) { return sm0 + s * 2 * C::OPER; };
   auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
   auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
   auto sS = [&](int s) { return ss0 + s * 2 * C::ST_PLANE; };
-  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 8, S_FULL = 10, P_FULL = 12, KV_FULL = 14,
-         KV_FREE = 16, ST_FULL = 18, ST_EMPTY = 20, O_FULL = 22, O_FREE = 23 };
+  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 9, S_FULL = 12, P_FULL = 14, ST_FULL = 16, ST_EMPTY = 18,
+         VP_FULL = 20, VP_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, N_BARS };
   constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) {
-      mbar_init(bar(QK_FULL + i), 128);
+      mbar_init(bar(QK_FULL + i), TMA ? 1 : (STATES ? 2 : 6));  // fp32: the loading warps
       mbar_init(bar(QK_EMPTY + i), 1);
+      mbar_init(bar(V_FULL + i), TMA ? 1 : 4);
+      mbar_init(bar(V_EMPTY + i), STATES ? 1 : 8);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(bar(V_FULL + i), 4);
-      mbar_init(bar(V_EMPTY + i), 1);
       mbar_init(bar(S_FULL + i), 1);
-      mbar_init(bar(P_FULL + i), 4);
-      mbar_init(bar(KV_FULL + i), 1);
-      mbar_init(bar(KV_FREE + i), 4);
+      mbar_init(bar(P_FULL + i), 8);
       mbar_init(bar(ST_FULL + i), 4);
       mbar_init(bar(ST_EMPTY + i), 1);
     }
+    mbar_init(bar(VP_FULL), 4);
+    mbar_init(bar(VP_EMPTY), 1);
+    mbar_init(bar(KV_FULL), 1);
+    mbar_init(bar(KV_FREE), 4);
     mbar_init(bar(O_FULL), 1);
-    mbar_init(bar(O_FREE), 4);
+    mbar_init(bar(O_FREE), 8);
     fence_mbar_init();
   }
-  if (warp == 8) {
+  if (warp == 18) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
@@ -356,127 +342,531 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
   const uint32_t tmem = tmem_slot;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
 
-  if (warp >= 13) {
-    // ------------------------------------------------------------ v: one chunk ahead in registers
-    const int t = threadIdx.x - 13 * 32;
-    constexpr int VECS = 128 / Rows<T>::ROWS;
-    uint4 r[VECS];
-    ChunkIter<DK> it;
-    bool more = it.first(a);
-    if (more) {
-      const Rows<T> rows(a, it, a.one[it.x.dir].v, it.x.half, t);
-#pragma unroll
-      for (int i = 0; i < VECS; ++i) r[i] = rows.load(i);
-    }
-    float w[VECS];  // the rows' powers of the decay, kept while they stay the same
-    int w_unit = -1, w_valid = 0;
-    while (more) {
-      const int g = it.g, vs = g % C::VS, valid = it.valid();
-      if (it.u != w_unit || valid != w_valid) {
-        const float l2 = log2_decay(a.log_decay, it.x.h);
-#pragma unroll
-        for (int i = 0; i < VECS; ++i) {
-          const int row = t / Rows<T>::PER_ROW + i * Rows<T>::ROWS;
-          w[i] = row < valid ? exp2f(l2 * static_cast<float>(valid - 1 - row)) : 0.f;
+  // Head dim 128: a state thread holds 64 values. 2 x 96 + 152 + 88 + 48 = 5 x 96 registers.
+  constexpr bool MOVE_REGS = DK == 128 && !STATES;
+  if (MOVE_REGS) {
+    if (warp >= 16) regs_dec<48>();
+    else if (warp >= 12) regs_dec<88>();
+    else if (warp >= 8) regs_inc<152>();
+  }
+
+  if (warp < 8) {
+    // ------------------------------------------------------------ P, then the previous chunk's O
+    if (!STATES) {
+      const int w4 = warp & 3, part = warp >> 2;  // 32 rows, and which of their two warps
+      const int lane = lane_id(), i = 32 * w4 + lane;
+      float* tab = wtab + (part == 0 ? 64 * w4 : 256 + 32 * w4);  // this warp's own
+      int g = 0;
+      bool ok = true;
+      // the chunk whose output is due
+      int o_dir = 0, o_col = 0, o_h = 0, o_tok = 0, o_b = 0, o_valid = 0;
+      float o_scale = 0.f;   // of Q S
+      bool o_stored = false; // a store of this warp may still read the V slot of chunk g - 1
+      // The output goes through the V slot of its own chunk (P V was its last reader).
+      // 32 rows of 64 (bf16) or 128 bytes per warp, swizzled as the tensor map says.
+      auto release = [&]() {
+        if (o_stored && lane == 0) {
+          bulk_wait_read<0>();
+          mbar_arrive(bar(V_EMPTY + (g - 2) % C::VS));
         }
-        w_unit = it.u;
-        w_valid = valid;
-      }
-      if (g >= C::VS && !mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
+        o_stored = false;
+      };
+      auto write_out = [&]() {
+        if (!mbar_wait_warp(bar(O_FULL), (g - 1) & 1, status)) return false;
+        tc_fence_after();
+        const float2 w2 = make_float2(o_scale, o_scale);
+        uint32_t o1[32], o2[32];
+        const uint32_t at = tmem + lane_base + 32 * part;
+        tmem_ld32(at + T_QS, o1);
+        tmem_ld32_sync(at + T_PV, o2);
+        tc_fence_before();
+        warp_arrive(bar(O_FREE));
+        o_stored = true;
+        if (32 * part >= a.D) return true;  // head dim 32: no columns for part 1
+        float2 f[16];
 #pragma unroll
-      for (int i = 0; i < VECS; ++i) {
-        const int row = t / Rows<T>::PER_ROW + i * Rows<T>::ROWS;
-        store_v<T, NP, STATES>(r[i], row, t, sV(vs), w[i]);
-      }
-      fence_proxy_async_smem();
-      warp_arrive(bar(V_FULL + vs));
-      more = it.next(a);
-      if (more) {
-        const Rows<T> rows(a, it, a.one[it.x.dir].v, it.x.half, t);
+        for (int e = 0; e < 16; ++e)
+          f[e] = __ffma2_rn(w2, pair_of(o1[2 * e], o1[2 * e + 1]), pair_of(o2[2 * e], o2[2 * e + 1]));
+        const bool add = a.one[o_dir].dir.accumulate;
+        if (add && (sizeof(T) == 2 || o_valid < 128)) {
+          // added in fp32 and rounded once, and rows past the end left alone: each lane its row
+          if (i < o_valid)
+            add_row(static_cast<T*>(a.one[o_dir].o) +
+                        ((static_cast<size_t>(o_b) * a.L + o_tok + i) * a.H + o_h) * a.D + o_col,
+                    f);
+          return true;
+        }
+        const uint32_t stage = sV((g - 1) % C::VS) + warp * (32 * 32 * static_cast<int>(sizeof(T)));
+        if (i >= o_valid) {
 #pragma unroll
-        for (int i = 0; i < VECS; ++i) r[i] = rows.load(i);
+          for (int e = 0; e < 16; ++e) f[e] = make_float2(0.f, 0.f);
+        }
+        if constexpr (sizeof(T) == 2) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            st_shared_v4(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), hi_pair(f[4 * c]), hi_pair(f[4 * c + 1]),
+                         hi_pair(f[4 * c + 2]), hi_pair(f[4 * c + 3]));
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            st_shared_v4(stage + sw128_offset(lane, c * 16), __float_as_uint(f[2 * c].x), __float_as_uint(f[2 * c].y),
+                         __float_as_uint(f[2 * c + 1].x), __float_as_uint(f[2 * c + 1].y));
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0 && o_tok + 32 * w4 < a.L) {
+          const CUtensorMap* map = &maps.o[a.one[o_dir].mo];
+          if (add) tma_reduce_add_4d(map, stage, o_col, o_h, o_tok + 32 * w4, o_b);
+          else tma_store_4d(map, stage, o_col, o_h, o_tok + 32 * w4, o_b);
+          tma_store_commit();
+        }
+        return true;
+      };
+      for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+        const MixUnit x = mix_unit<DK, STATES>(a, u);
+        if (x.chunks == 0) continue;
+        const MixOne& one = a.one[x.dir];
+        const float l2 = log2_decay(a.log_decay, x.h);
+        // tab[e] with e = 31 - lane + j on the diagonal: forward l^(31-e) for e <= 31, backward
+        // l^(e-31) for e >= 31; the blocks beside it use its first / its last 32. Times scale.
+        __syncwarp();
+        const float near = a.scale * exp2f(l2 * static_cast<float>(x.rev ? lane + 1 : 31 - lane));
+        if (part == 0) {
+          tab[lane] = x.rev ? (lane == 31 ? a.scale : 0.f) : near;
+          tab[32 + lane] = x.rev ? near : 0.f;
+        } else {
+          tab[lane] = near;
+        }
+        __syncwarp();
+        const float *beside = part == 0 && x.rev ? tab + 32 : tab, *diag = tab + 31 - lane;
+        // Blocks beside the diagonal, at distance d = 1 .. nb: part 0 takes the nearer ones and the
+        // diagonal, part 1 the farther ones. l^|i-j| = l^(32 (d - 1)) l^(base) tab, no negative exponent.
+        const int nb = x.rev ? 3 - w4 : w4, cut = nb / 2;
+        const int d0 = part == 0 ? 1 : cut + 1, d1 = part == 0 ? cut : nb, dir = x.rev ? 1 : -1;
+        const float l32 = exp2f(l2 * 32.f);
+        const float l_first = exp2f(l2 * static_cast<float>((x.rev ? 31 - lane : lane + 1) + 32 * (d0 - 1)));
+        for (int c = 0; c < x.chunks; ++c) {
+          const int valid = x.valid(c);
+          release();  // before any wait: the loads may wait for this slot
+          if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
+          tc_fence_after();
+          const uint32_t ts = tmem + T_S + (g & 1) * 128 + lane_base;
+          uint32_t r[32];
+          float2 p[16];
+          // P of 32 columns goes over their scores: hi in the first 16 columns, lo (NT = 3) in the next
+          auto put = [&](int cb) {
+            uint32_t h[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) h[j] = hi_pair(p[j]);
+            tmem_st16(ts + cb * 32, h);
+            if (NT == 3) {
+              uint32_t l[16];
+#pragma unroll
+              for (int j = 0; j < 16; ++j) l[j] = lo_pair(p[j], h[j]);
+              tmem_st16(ts + cb * 32 + 16, l);
+            }
+          };
+          // columns of block cb to keep: tokens up to the end of the sequence
+          auto tokens = [&](int cb) {
+            const int left = valid - 32 * cb;
+            return left >= 32 ? 0xffffffffu : (left <= 0 ? 0u : (1u << left) - 1u);
+          };
+          // zeros where the mask has none (not by zero weights: a score there may be infinite)
+          auto keep = [&](uint32_t mask) {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              p[j].x = (mask >> (2 * j)) & 1u ? p[j].x : 0.f;
+              p[j].y = (mask >> (2 * j + 1)) & 1u ? p[j].y : 0.f;
+            }
+          };
+          if (part == 0) {
+            tmem_ld32_sync(ts + w4 * 32, r);
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              p[j] = __fmul2_rn(pair_of(r[2 * j], r[2 * j + 1]), make_float2(diag[2 * j], diag[2 * j + 1]));
+            keep(x.rev ? tokens(w4) & (0xffffffffu << lane) : 0xffffffffu >> (31 - lane));
+            put(w4);
+          }
+          float rf = l_first;
+#pragma unroll 1
+          for (int d = d0; d <= d1; ++d) {
+            const int cb = w4 + dir * d;
+            tmem_ld32_sync(ts + cb * 32, r);
+            const float2 rf2 = make_float2(rf, rf);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 f = reinterpret_cast<const float4*>(beside)[j];
+              p[2 * j] = __fmul2_rn(pair_of(r[4 * j], r[4 * j + 1]), __fmul2_rn(rf2, make_float2(f.x, f.y)));
+              p[2 * j + 1] = __fmul2_rn(pair_of(r[4 * j + 2], r[4 * j + 3]), __fmul2_rn(rf2, make_float2(f.z, f.w)));
+            }
+            if (x.rev && valid < 128) keep(tokens(cb));
+            put(cb);
+            rf *= l32;
+          }
+          if (part == 1) {  // the other side of the diagonal is zero
+            uint32_t z[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) z[j] = 0;
+#pragma unroll 1
+            for (int d = 1; d <= 3 - nb; ++d) {
+              tmem_st16(ts + (w4 - dir * d) * 32, z);
+              if (NT == 3) tmem_st16(ts + (w4 - dir * d) * 32 + 16, z);
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          warp_arrive(bar(P_FULL + (g & 1)));
+          if (g > 0 && !(ok = write_out())) break;
+          o_dir = x.dir;
+          o_col = x.half * 64 + 32 * part;
+          o_h = x.h;
+          o_tok = x.token(c);
+          o_b = x.b;
+          o_valid = valid;
+          const int lead = x.starts(c) ? one.dir.lead : 0;
+          o_scale = a.scale * exp2f(l2 * static_cast<float>((x.rev ? valid - i : i + 1) - lead));
+          ++g;
+        }
+      }
+      release();
+      if (ok && g > 0) write_out();
+      if (lane == 0) bulk_wait_all();
+    }
+  } else if (warp < 12) {
+    // ------------------------------------------------------------ state
+    const int r = threadIdx.x - 8 * 32;
+    constexpr int NC = C::NC;
+    const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
+    int g = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+      const MixUnit x = mix_unit<DK, STATES>(a, u);
+      const MixOne& one = a.one[x.dir];
+      const float l2 = log2_decay(a.log_decay, x.h);
+      const bool in_state = row < a.D && x.half * 64 + col0 < a.D;  // head dim 32: a quarter of the tile
+      // element (row, column 0) of the caller's state, and the step to the next column
+      const long long e0 = x.half * 64 + col0, st_step = one.dir.transposed ? a.D : 1;
+      const size_t st0 = (static_cast<size_t>(x.b) * a.H + x.h) * a.D * a.D +
+                         (one.dir.transposed ? e0 * a.D + row : static_cast<long long>(row) * a.D + e0);
+      float2 S[NC / 2];
+      auto save = [&](int slot) {
+        float4* dst = reinterpret_cast<float4*>(seg_slot<DK>(a, x, slot));
+#pragma unroll
+        for (int c = 0; c < NC / 4; ++c)
+          dst[c * 128 + r] = make_float4(S[2 * c].x, S[2 * c].y, S[2 * c + 1].x, S[2 * c + 1].y);
+      };
+      const bool carried = a.n_seg == 1 || (STATES && x.seg == (x.rev ? 1 : 0));
+#pragma unroll
+      for (int c = 0; c < NC / 2; ++c) S[c] = make_float2(0.f, 0.f);
+      if (carried && one.s_in && in_state) {
+        const float* src = one.s_in + st0;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c, src += 2 * st_step)
+          S[c] = make_float2(one.dir.in_mult * src[0], one.dir.in_mult * src[st_step]);
+      }
+      const int last = x.n > 0 ? (x.n - 1) / a.seg_tokens : 0;  // the segment of the last token
+      if (STATES) {
+        if (carried) save(a.n_seg - 1);
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c) S[c] = make_float2(0.f, 0.f);
+      } else if (a.n_seg > 1) {
+        // the state entering this segment, from the carried one and the segments in between
+        auto add = [&](int slot, int tokens) {
+          const float w = exp2f(l2 * static_cast<float>(tokens));
+          const float4* src = reinterpret_cast<const float4*>(seg_slot<DK>(a, x, slot));
+#pragma unroll
+          for (int c = 0; c < NC / 4; ++c) {
+            const float4 f = src[c * 128 + r];
+            S[2 * c] = __ffma2_rn(make_float2(w, w), make_float2(f.x, f.y), S[2 * c]);
+            S[2 * c + 1] = __ffma2_rn(make_float2(w, w), make_float2(f.z, f.w), S[2 * c + 1]);
+          }
+        };
+        const int end = x.p0 + a.seg_tokens;
+        const int before = x.rev ? (x.n > end ? x.n - end : 0) : x.p0;  // tokens before this segment
+        add(a.n_seg - 1, before > 0 ? before - one.dir.lead : 0);
+        if (x.count > 0) {
+          if (x.rev)
+            for (int f = x.seg + 1; f <= last; ++f) add(f - 1, (f - x.seg - 1) * a.seg_tokens);
+          else
+            for (int f = 0; f < x.seg; ++f) add(f, (x.seg - f - 1) * a.seg_tokens);
+        }
+      }
+      // the state's bf16 parts for chunk gg's Q S
+      auto put_state = [&](int gg) {
+        const int sb = gg % C::STB;
+        if (gg >= C::STB && !mbar_wait_warp(bar(ST_EMPTY + sb), (gg / C::STB - 1) & 1, status)) return false;
+#pragma unroll
+        for (int c = 0; c < NC / 8; ++c) {
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            h[j] = hi_pair(S[4 * c + j]);
+            l[j] = lo_pair(S[4 * c + j], h[j]);
+          }
+          const uint32_t at = sS(sb) + sw128_offset(row, col0 * 2 + c * 16);
+          st_shared_v4(at, h[0], h[1], h[2], h[3]);
+          st_shared_v4(at + C::ST_PLANE, l[0], l[1], l[2], l[3]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(bar(ST_FULL + sb));
+        return true;
+      };
+      if (!STATES && x.chunks > 0 && !(ok = put_state(g))) break;
+      for (int c = 0; c < x.chunks; ++c, ++g) {
+        // the carried state enters the very first token without a decay (lead)
+        const int lead = !STATES && x.starts(c) ? one.dir.lead : 0;
+        const float dec = exp2f(l2 * static_cast<float>(x.valid(c) - lead));
+        const float2 dec2 = make_float2(dec, dec);
+        if (!(ok = mbar_wait_warp(bar(KV_FULL), g & 1, status))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int j = 0; j < NC / 8; ++j) {
+          uint32_t vh[8], vl[8];  // K^T V' hi and K^T V' lo
+          const uint32_t at = tmem + T_KV + col0 + j * 8 + lane_base;
+          tmem_ld8x2_sync(at, at + 64, vh, vl);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            S[4 * j + e] = __ffma2_rn(dec2, S[4 * j + e], __fadd2_rn(pair_of(vh[2 * e], vh[2 * e + 1]),
+                                                                   pair_of(vl[2 * e], vl[2 * e + 1])));
+        }
+        tc_fence_before();
+        warp_arrive(bar(KV_FREE));
+        if (!STATES && c + 1 < x.chunks && !(ok = put_state(g + 1))) break;
+      }
+      if (!ok) break;
+      if (STATES) {
+        save(x.rev ? x.seg - 1 : x.seg);
+        continue;
+      }
+      // the state after the last token in time order
+      if (one.s_out && in_state && x.seg == (x.rev ? 0 : last)) {
+        const float w = one.dir.out_mult * (one.dir.lead && x.n > 0 ? exp2f(l2) : 1.f);
+        float* dst = one.s_out + st0;
+#pragma unroll
+        for (int c = 0; c < NC / 2; ++c, dst += 2 * st_step) {
+          dst[0] = w * S[c].x;
+          dst[st_step] = w * S[c].y;
+        }
+      }
+      if (!one.dir.accumulate) {  // zeros past the sequence
+        const int p1 = a.L - x.p0 < a.seg_tokens ? a.L : x.p0 + a.seg_tokens;
+        const int pz = x.n > x.p0 ? x.n : x.p0;
+        const int vecs = (a.D < 64 ? a.D : 64) * static_cast<int>(sizeof(T)) / 16;
+        const long long zeros = static_cast<long long>(p1 - pz) * vecs;
+        for (long long z = r; z < zeros; z += 128) {
+          const size_t tok = static_cast<size_t>(x.b) * a.L + pz + z / vecs;
+          reinterpret_cast<uint4*>(static_cast<T*>(one.o) + (tok * a.H + x.h) * a.D + x.half * 64)[z % vecs] =
+              make_uint4(0, 0, 0, 0);
+        }
       }
     }
-  } else if (warp >= 9) {
-    // ------------------------------------------------------------ k and q
-    const int t = threadIdx.x - 9 * 32;
-    constexpr int TILES = STATES ? KT : 2 * KT;  // k tiles, then q tiles
-    ChunkIter<DK> it;
+  } else if (warp < 16) {
+    // ------------------------------------------------------------ V'
+    const int t = threadIdx.x - 12 * 32;
+    ChunkIter<DK, STATES> it;
     bool more = it.first(a);
-    auto rows_of = [&](int tile) {
-      const MixOne& one = a.one[it.x.dir];
-      return Rows<T>(a, it, tile < KT ? one.k : one.q, tile % KT, t);
+    int w_unit = -1, w_valid = 0;
+    // l^(valid - 1 - row), backward l^row; zero past the end
+    auto weight = [&](int row, int valid) {
+      const float l2 = log2_decay(a.log_decay, it.x.h);
+      return row < valid ? exp2f(l2 * static_cast<float>(it.x.rev ? row : valid - 1 - row)) : 0.f;
     };
-    auto tile_at = [&](int s, int tile) { return (tile < KT ? sK(s) : sQ(s)) + (tile % KT) * kTile; };
-    if constexpr (sizeof(T) == 2) {
-      // straight into the ring; the barrier completes as the copies land
+    if constexpr (TMA) {
+      // Each thread has 16-byte column t % 8 of rows t / 8 + 16 i. A weight w is two bf16 parts;
+      // hi = bf16(v w_hi), and since v w_hi has 16 bits, v w_hi - hi is a bf16 too:
+      // lo = bf16(v w_lo + (v w_hi - hi)), off by 2^-17 of v w, in three packed instructions.
+      __nv_bfloat162 wh[8], wl[8];
       for (; more; more = it.next(a)) {
-        const int g = it.g, s = g % C::QKS;
-        if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
-#pragma unroll 1
-        for (int tile = 0; tile < TILES; ++tile) {
-          const Rows<T> rows = rows_of(tile);
-          const uint32_t at = tile_at(s, tile);
+        const int g = it.g, vs = g % C::VS, valid = it.valid();
+        if (it.u != w_unit || valid != w_valid) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const bool ok = rows.row(i) < rows.valid;
-            cp_async16(at + sw128_offset(rows.row(i), (t % 8) * 16), ok ? rows.src + i * rows.step : rows.src, ok);
+            const float w = weight(t / 8 + 16 * i, valid);
+            wh[i] = __float2bfloat162_rn(w);
+            wl[i] = __float2bfloat162_rn(w - __low2float(wh[i]));
+          }
+          w_unit = it.u;
+          w_valid = valid;
+        }
+        if (!mbar_wait_warp(bar(V_FULL + vs), (g / C::VS) & 1, status)) break;
+        if (it.x.token(it.chunk) + valid < a.L && valid < 128) {
+          // Tokens past this sequence lie in the tiles, and may hold anything: their rows of V meet
+          // zeros of P, and their rows of K zeros of V', which NaN or infinity would survive.
+          const int s = g % C::QKS;
+          if (!mbar_wait_warp(bar(QK_FULL + s), (g / C::QKS) & 1, status)) break;
+          for (int z = t + valid * 8; z < 128 * 8; z += 128) {
+            st_shared_v4(sV(vs) + z * 16, 0, 0, 0, 0);
+            for (int tile = 0; tile < KT; ++tile) st_shared_v4(sK(s) + tile * kTile + z * 16, 0, 0, 0, 0);
           }
         }
-        cp_async_arrive(bar(QK_FULL + s));
+        if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const int row = t / 8 + 16 * i;
+          const uint32_t off = sw128_offset(row, (t % 8) * 16);
+          const uint4 v = ld_shared_v4(sV(vs) + off);
+          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          uint32_t h[4], l[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 vv = *reinterpret_cast<const __nv_bfloat162*>(&x[j]);
+            const __nv_bfloat162 hh = __hmul2_rn(vv, wh[i]);
+            const __nv_bfloat162 ll = __hfma2(vv, wl[i], __hfma2(vv, wh[i], __hneg2(hh)));
+            h[j] = row < valid ? *reinterpret_cast<const uint32_t*>(&hh) : 0;
+            l[j] = row < valid ? *reinterpret_cast<const uint32_t*>(&ll) : 0;
+          }
+          st_shared_v4(sVp + off, h[0], h[1], h[2], h[3]);
+          st_shared_v4(sVp + kTile + off, l[0], l[1], l[2], l[3]);
+        }
+        fence_proxy_async_smem();
+        warp_arrive(bar(VP_FULL));
       }
     } else {
-      // through registers, half a tile at a time, the next half always in flight
-      uint4 r0[8], r1[8];
-      auto load_half = [&](uint4 (&r)[8], int tile, int half) {
-        const Rows<T> rows = rows_of(tile);
+      // fp32: q, then v, half a tile in each register buffer
+      using R = Rows<128>;
+      constexpr int HALF = R::VECS / 2;
+      float4 r0[HALF], r1[HALF];
+      float w0[HALF], w1[HALF];
+      auto load_half = [&](float4 (&r)[HALF], const void* base, int half) {
+        const R rows(a, it, base, t);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = rows.load(half * 8 + j);
+        for (int i = 0; i < HALF; ++i) r[i] = rows.load(half * HALF + i);
       };
-      auto put_half = [&](const uint4 (&r)[8], uint32_t at, int half) {
+      auto row_of = [&](int half, int i) { return t / 16 + (half * HALF + i) * R::ROWS; };
+      auto put_half = [&](const float4 (&r)[HALF], uint32_t at, int half) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i)
+          put4(at, NP == 2 ? at + kTile : 0, sw128_offset(row_of(half, i), (t % 16) * 8), make_float2(r[i].x, r[i].y),
+               make_float2(r[i].z, r[i].w));
+      };
+      auto put_times = [&](const float4 (&r)[HALF], const float (&w)[HALF], int half) {
+#pragma unroll
+        for (int i = 0; i < HALF; ++i)
+          put4(sVp, sVp + kTile, sw128_offset(row_of(half, i), (t % 16) * 8),
+               __fmul2_rn(make_float2(r[i].x, r[i].y), make_float2(w[i], w[i])),
+               __fmul2_rn(make_float2(r[i].z, r[i].w), make_float2(w[i], w[i])));
+      };
+      auto load_first = [&]() {
+        const MixOne& one = a.one[it.x.dir];
+        load_half(r0, STATES ? one.v : one.q, 0);
+        load_half(r1, STATES ? one.v : one.q, 1);
+      };
+      if (more) load_first();
+      while (more) {
+        const int g = it.g, vs = g % C::VS, valid = it.valid();
+        if (it.u != w_unit || valid != w_valid) {
+#pragma unroll
+          for (int i = 0; i < HALF; ++i) {
+            w0[i] = weight(row_of(0, i), valid);
+            w1[i] = weight(row_of(1, i), valid);
+          }
+          w_unit = it.u;
+          w_valid = valid;
+        }
+        if (!STATES) {
+          const int s = g % C::QKS;
+          if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+          put_half(r0, sQ(s), 0);
+          put_half(r1, sQ(s), 1);
+          fence_proxy_async_smem();  // before the next loads: the fence would wait for them
+          warp_arrive(bar(QK_FULL + s));
+          load_half(r0, a.one[it.x.dir].v, 0);
+          load_half(r1, a.one[it.x.dir].v, 1);
+        }
+        if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
+        put_times(r0, w0, 0);
+        put_times(r1, w1, 1);
+        fence_proxy_async_smem();
+        warp_arrive(bar(VP_FULL));
+        if (!STATES) {
+          if (g >= C::VS && !mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
+          put_half(r0, sV(vs), 0);
+          put_half(r1, sV(vs), 1);
+          fence_proxy_async_smem();
+          warp_arrive(bar(V_FULL + vs));
+        }
+        more = it.next(a);
+        if (more) load_first();
+      }
+    }
+  } else if (warp < 18) {
+    if constexpr (TMA) {
+      // ------------------------------------------------------------ TMA loads
+      if (warp == 16 && elect_one()) {
+        ChunkIter<DK, STATES> it;
+        for (bool more = it.first(a); more; more = it.next(a)) {
+          const int g = it.g, s = g % C::QKS, vs = g % C::VS;
+          const MixOne& one = a.one[it.x.dir];
+          const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
+          if (g >= C::QKS && !mbar_wait(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+          mbar_arrive_expect_tx(bar(QK_FULL + s), (STATES ? 1 : 2) * C::OPER);
+          for (int tile = 0; tile < KT; ++tile) {
+            tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], bar(QK_FULL + s), tile * 64, h, tok, b);
+            if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], bar(QK_FULL + s), tile * 64, h, tok, b);
+          }
+          if (g >= C::VS && !mbar_wait(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
+          mbar_arrive_expect_tx(bar(V_FULL + vs), C::V_STAGE);
+          tma_load_4d(sV(vs), &maps.m[one.mv], bar(V_FULL + vs), it.x.half * 64, h, tok, b);
+        }
+      }
+    } else {
+      // ------------------------------------------------------------ fp32 k, a quarter of the tile at a time
+      const int t = threadIdx.x - 16 * 32;
+      using R = Rows<64>;
+      constexpr int QUARTERS = R::VECS / 8;
+      ChunkIter<DK, STATES> it;
+      bool more = it.first(a);
+      float4 r0[8], r1[8];
+      auto load = [&](float4 (&r)[8], int quarter) {
+        const R rows(a, it, a.one[it.x.dir].k, t);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = rows.load(quarter * 8 + j);
+      };
+      auto put = [&](const float4 (&r)[8], uint32_t at, int quarter) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          put4(at, NP == 2 ? at + KT * kTile : 0, sw128_offset(t / 16 + (half * 8 + j) * 8, (t % 16) * 8),
-               __uint_as_float(r[j].x), __uint_as_float(r[j].y), __uint_as_float(r[j].z), __uint_as_float(r[j].w));
+          put4(at, NP == 2 ? at + kTile : 0, sw128_offset(t / 16 + (quarter * 8 + j) * R::ROWS, (t % 16) * 8),
+               make_float2(r[j].x, r[j].y), make_float2(r[j].z, r[j].w));
       };
-      if (more) load_half(r0, 0, 0);
+      if (more) load(r0, 0);
       while (more) {
         const int g = it.g, s = g % C::QKS;
         if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
 #pragma unroll 1
-        for (int tile = 0; tile < TILES; ++tile) {
-          const uint32_t at = tile_at(s, tile);
-          load_half(r1, tile, 1);
-          put_half(r0, at, 0);
-          if (tile + 1 == TILES) more = it.next(a);
-          if (more) load_half(r0, tile + 1 == TILES ? 0 : tile + 1, 0);
-          put_half(r1, at, 1);
+        for (int quarter = 0; quarter < QUARTERS; quarter += 2) {
+          load(r1, quarter + 1);
+          put(r0, sK(s), quarter);
+          if (quarter + 2 < QUARTERS) load(r0, quarter + 2);
+          put(r1, sK(s), quarter + 1);
         }
         fence_proxy_async_smem();
-        mbar_arrive(bar(QK_FULL + s));
+        warp_arrive(bar(QK_FULL + s));
+        more = it.next(a);
+        if (more) load(r0, 0);
       }
     }
-  } else if (warp == 8) {
+  } else if (warp == 18) {
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
       int total = 0;
-      for (int u = blockIdx.x; u < a.n_units; u += gridDim.x) total += mix_unit<DK>(a, u).chunks;
+      for (int u = blockIdx.x; u < a.n_units; u += gridDim.x) total += mix_unit<DK, STATES>(a, u).chunks;
       constexpr uint32_t idS = make_idesc(128, 128, 1, false, false), idV = make_idesc(128, 64, 1, false, true),
-                         idKV = make_idesc(128, 64, 1, true, true);
+                         idKV = make_idesc(128, 128, 1, true, true), idKV1 = make_idesc(128, 64, 1, true, true);
+      constexpr int LO = KT * kTile;  // from a hi plane of q or k to its lo plane
       auto wait = [&](int i, int phase) { return mbar_wait(bar(i), phase & 1, status); };
       auto issue_S = [&](int g) {
         const int s = g % C::QKS;
         if (!wait(QK_FULL + s, g / C::QKS)) return false;
-        fence_proxy_async_smem();  // bf16: the copies' writes, before the tensor core reads them
         tc_fence_after();
 #pragma unroll 1
         for (int term = 0; term < NT; ++term) {
-          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
-          const uint64_t kd = make_sdesc(sK(s) + (term == 1 ? KT * kTile : 0), 16, 1024);
+          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? LO : 0), 16, 1024);
+          const uint64_t kd = make_sdesc(sK(s) + (term == 1 ? LO : 0), 16, 1024);
 #pragma unroll
           for (int k = 0; k < DK / 16; ++k) {
-            const uint32_t off = ((k / 4) * kTile + (k % 4) * 32) >> 4;
-            umma_f16_ss(tmem + T_S + (g & 1) * 128, qd + off, kd + off, idS, (term > 0 || k > 0) ? 1u : 0u);
+            const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
+            umma_f16_ss(tmem + T_S + (g & 1) * 128, desc_at(qd, off), desc_at(kd, off), idS,
+                        (term > 0 || k > 0) ? 1u : 0u);
           }
         }
         umma_commit(bar(S_FULL + (g & 1)));
@@ -485,25 +875,26 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
       bool ok = true;
       for (int g = 0; ok && g < total; ++g) {
         const int s = g % C::QKS, vs = g % C::VS, b = g & 1;
-        if (STATES) ok = wait(QK_FULL + s, g / C::QKS);
-        else if (g == 0) ok = issue_S(0);
-        // K^T V' (DK = 64: both halves of the 128 rows are the same 64 rows of the
+        ok = wait(QK_FULL + s, g / C::QKS);
+        if (!STATES && g == 0) ok = ok && issue_S(0);
+        // K^T [V' hi, V' lo] (DK = 64: both halves of the 128 rows are the same 64 rows of the
         // state, so every warp of the state finds its columns in its own lanes)
-        ok = ok && wait(V_FULL + vs, g / C::VS) && (g < 2 || wait(KV_FREE + b, (g >> 1) - 1));
+        ok = ok && wait(VP_FULL, g) && (g < 1 || wait(KV_FREE, g - 1));
         if (!ok) break;
-        if (STATES) fence_proxy_async_smem();
         tc_fence_after();
-        constexpr int KV_TERMS = NT == 3 ? 3 : 2;
-#pragma unroll 1
-        for (int term = 0; term < KV_TERMS; ++term) {
-          const uint64_t kd = make_sdesc(sK(s) + (term == 2 ? KT * kTile : 0), DK == 64 ? 0 : kTile, 1024);
-          const uint64_t vd = make_sdesc(sV(vs) + (NP + (term == 1 ? 1 : 0)) * kTile, kTile, 1024);
+        {
+          const uint64_t kd = make_sdesc(sK(s), DK == 64 ? 0 : kTile, 1024), vd = make_sdesc(sVp, kTile, 1024);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ss(tmem + T_KV + b * 64, kd + (k * 2048 >> 4), vd + (k * 2048 >> 4), idKV,
-                        (term > 0 || k > 0) ? 1u : 0u);
+            umma_f16_ss(tmem + T_KV, desc_at(kd, k * 2048), desc_at(vd, k * 2048), idKV, k > 0 ? 1u : 0u);
+          if (NT == 3) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              umma_f16_ss(tmem + T_KV, desc_at(kd, LO + k * 2048), desc_at(vd, k * 2048), idKV1, 1u);
+          }
         }
-        umma_commit(bar(KV_FULL + b));
+        umma_commit(bar(KV_FULL));
+        umma_commit(bar(VP_EMPTY));
         if (STATES) {
           umma_commit(bar(QK_EMPTY + s));
           umma_commit(bar(V_EMPTY + vs));
@@ -516,286 +907,37 @@ __global__ void __launch_bounds__(kMixThreads, 1) mix_kernel(const __grid_consta
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
-        for (int term = 0; term < KV_TERMS; ++term) {
-          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? KT * kTile : 0), 16, 1024);
+        for (int term = 0; term < (NT == 3 ? 3 : 2); ++term) {
+          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? LO : 0), 16, 1024);
           const uint64_t sd = make_sdesc(sS(sb) + (term == 1 ? C::ST_PLANE : 0), kTile, 1024);
 #pragma unroll
           for (int k = 0; k < DK / 16; ++k)
-            umma_f16_ss(tmem + T_QS, qd + (((k / 4) * kTile + (k % 4) * 32) >> 4), sd + (k * 2048 >> 4), idV,
+            umma_f16_ss(tmem + T_QS, desc_at(qd, (k / 4) * kTile + (k % 4) * 32), desc_at(sd, k * 2048), idV,
                         (term > 0 || k > 0) ? 1u : 0u);
         }
         umma_commit(bar(ST_EMPTY + sb));
         umma_commit(bar(QK_EMPTY + s));
         // P V
-        if (!(ok = wait(P_FULL + b, g >> 1))) break;
+        ok = wait(V_FULL + vs, g / C::VS) && wait(P_FULL + b, g >> 1);
+        if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
         for (int term = 0; term < NT; ++term) {
           const uint64_t vd = make_sdesc(sV(vs) + (term == 1 ? kTile : 0), kTile, 1024);
+          const uint32_t p0 = tmem + T_S + b * 128 + (term == 2 ? 16 : 0);
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + T_PV, tmem + T_S + b * 128 + (k / 2) * 32 + (term == 2 ? 16 : 0) + (k % 2) * 8,
-                        vd + (k * 2048 >> 4), idV,
+            umma_f16_ts(tmem + T_PV, p0 + (k / 2) * 32 + (k % 2) * 8, desc_at(vd, k * 2048), idV,
                         (term > 0 || k > 0) ? 1u : 0u);
         }
-        umma_commit(bar(V_EMPTY + vs));
         umma_commit(bar(O_FULL));
-      }
-    }
-  } else if (warp < 4) {
-    // ------------------------------------------------------------ P, then the previous chunk's O
-    if (!STATES) {
-      const int i = threadIdx.x, lane = lane_id();
-      float* tab = wtab + 64 * warp;  // tab[j] = l^(31 - j), this warp's own; past 31 not used
-      int g = 0;
-      bool ok = true;
-      // the chunk whose output is due
-      T* o_base = nullptr;     // its first row, this head and column half
-      long long o_step = 0;    // values from one row to the next
-      int o_valid = 0;
-      float o_scale = 0.f;     // of Q S
-      bool o_add = false;
-      auto write_out = [&]() {
-        if (!mbar_wait_warp(bar(O_FULL), (g - 1) & 1, status)) return false;
-        tc_fence_after();
-        constexpr int COLS = 64 / static_cast<int>(sizeof(T));  // columns of 64 bytes
-        const int cols = a.D < 64 ? a.D : 64;
-#pragma unroll 1
-        for (int c0 = 0; c0 < cols; c0 += COLS) {
-          uint4 v[4];
-#pragma unroll
-          for (int c = 0; c < COLS; c += 16) {
-            uint32_t o1[16], o2[16];
-            tmem_ld16x2_sync(tmem + T_QS + c0 + c + lane_base, tmem + T_PV + c0 + c + lane_base, o1, o2);
-            float f[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e)
-              f[e] = fmaf(o_scale, __uint_as_float(o1[e]), a.scale * __uint_as_float(o2[e]));
-            if (o_add && i < o_valid) add16(o_base + i * o_step + c0 + c, f);
-            if constexpr (sizeof(T) == 2) {
-              v[c / 8] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                                    pack_bf16x2(f[6], f[7]));
-              v[c / 8 + 1] = make_uint4(pack_bf16x2(f[8], f[9]), pack_bf16x2(f[10], f[11]),
-                                        pack_bf16x2(f[12], f[13]), pack_bf16x2(f[14], f[15]));
-            } else {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                v[e] = make_uint4(__float_as_uint(f[4 * e]), __float_as_uint(f[4 * e + 1]),
-                                  __float_as_uint(f[4 * e + 2]), __float_as_uint(f[4 * e + 3]));
-            }
-          }
-          if (c0 + COLS >= cols) {
-            tc_fence_before();
-            warp_arrive(bar(O_FREE));
-          }
-          transpose4(v);
-          const int r0 = 32 * warp + (lane & ~3);
-          T* dst = o_base + r0 * o_step + c0 + (lane & 3) * (16 / static_cast<int>(sizeof(T)));
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            if (r0 + k < o_valid) *reinterpret_cast<uint4*>(dst + k * o_step) = v[k];
-        }
-        return true;
-      };
-      for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
-        const MixUnit x = mix_unit<DK>(a, u);
-        if (x.chunks == 0) continue;
-        const MixOne& one = a.one[x.dir];
-        const float l2 = log2_decay(a.log_decay, x.h);
-        __syncwarp();
-        tab[lane] = exp2f(l2 * static_cast<float>(31 - lane));
-        tab[32 + lane] = 0.f;
-        __syncwarp();
-        const float l32 = exp2f(l2 * 32.f), l_first = exp2f(l2 * static_cast<float>(lane + 1));
-        for (int c = 0; c < x.chunks; ++c) {
-          if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
-          tc_fence_after();
-          const uint32_t ts = tmem + T_S + (g & 1) * 128 + lane_base;
-          // P of 32 columns goes over their scores: hi in the first 16 columns, lo (NT = 3)
-          // in the next
-          auto put = [&](int cb, const float (&p)[32]) {
-            uint32_t h[16];
-#pragma unroll
-            for (int j = 0; j < 16; ++j) h[j] = pack_bf16x2(p[2 * j], p[2 * j + 1]);
-            tmem_st16(ts + cb * 32, h);
-            if (NT == 3) {
-              uint32_t l[16];
-#pragma unroll
-              for (int j = 0; j < 16; ++j) l[j] = lo_pair(p[2 * j], p[2 * j + 1], h[j]);
-              tmem_st16(ts + cb * 32 + 16, l);
-            }
-          };
-          uint32_t r[32];
-          float p[32];
-          // on the diagonal: column j of row `lane` has l^(lane - j) = tab[31 - lane + j]
-          tmem_ld32_sync(ts + warp * 32, r);
-#pragma unroll
-          for (int j = 0; j < 32; ++j) {
-            const float w = tab[31 - lane + j];
-            p[j] = j <= lane ? __uint_as_float(r[j]) * w : 0.f;
-          }
-          put(warp, p);
-          // left of it, nearest first: l^(i - j) = l^(i - 32 cb - 31) l^(31 - j), no negative exponent
-          float rf = l_first;
-#pragma unroll 1
-          for (int cb = warp - 1; cb >= 0; --cb) {
-            tmem_ld32_sync(ts + cb * 32, r);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 f = reinterpret_cast<const float4*>(tab)[j];
-              p[4 * j] = __uint_as_float(r[4 * j]) * (rf * f.x);
-              p[4 * j + 1] = __uint_as_float(r[4 * j + 1]) * (rf * f.y);
-              p[4 * j + 2] = __uint_as_float(r[4 * j + 2]) * (rf * f.z);
-              p[4 * j + 3] = __uint_as_float(r[4 * j + 3]) * (rf * f.w);
-            }
-            put(cb, p);
-            rf *= l32;
-          }
-          // right of it: zero
-#pragma unroll
-          for (int j = 0; j < 16; ++j) r[j] = 0;
-#pragma unroll 1
-          for (int cb = warp + 1; cb < 4; ++cb) {
-            tmem_st16(ts + cb * 32, r);
-            if (NT == 3) tmem_st16(ts + cb * 32 + 16, r);
-          }
-          tmem_st_wait();
-          tc_fence_before();
-          warp_arrive(bar(P_FULL + (g & 1)));
-          if (g > 0 && !(ok = write_out())) break;
-          const int pos = x.p0 + c * 128, left = x.count - c * 128;
-          const long long tok = static_cast<long long>(x.b) * a.L + (one.dir.reverse ? x.n - 1 - pos : pos);
-          o_step = static_cast<long long>(a.H) * a.D * (one.dir.reverse ? -1 : 1);
-          o_base = static_cast<T*>(one.o) + (tok * a.H + x.h) * a.D + x.half * 64;
-          o_valid = left < 128 ? left : 128;
-          o_add = one.dir.accumulate;
-          o_scale = a.scale * exp2f(l2 * static_cast<float>(i + 1 - (pos == 0 ? one.dir.lead : 0)));
-          ++g;
-        }
-      }
-      if (ok && g > 0) write_out();
-    }
-  } else {
-    // ------------------------------------------------------------ state
-    const int r = threadIdx.x - 128;
-    constexpr int NC = C::NC;
-    const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
-    int g = 0;
-    bool ok = true;
-    for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
-      const MixUnit x = mix_unit<DK>(a, u);
-      const MixOne& one = a.one[x.dir];
-      const float l2 = log2_decay(a.log_decay, x.h);
-      const bool in_state = row < a.D && x.half * 64 + col0 < a.D;  // head dim 32: a quarter of the tile
-      const size_t st0 = (static_cast<size_t>(x.b) * a.H + x.h) * a.D * a.D;
-      // element (row, col) of the caller's state
-      auto state_at = [&](int c) {
-        const int e = x.half * 64 + col0 + c;
-        return st0 + (one.dir.transposed ? static_cast<size_t>(e) * a.D + row : static_cast<size_t>(row) * a.D + e);
-      };
-      float S[NC];
-      if (a.n_seg == 1 || (STATES && x.seg == 0)) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) S[c] = one.s_in && in_state ? one.dir.in_mult * one.s_in[state_at(c)] : 0.f;
-      }
-      if (STATES) {
-        if (x.seg == 0) {
-          float4* dst = reinterpret_cast<float4*>(seg_slot<DK>(a, x, a.n_seg - 1));
-#pragma unroll
-          for (int c = 0; c < NC / 4; ++c) dst[c * 128 + r] = make_float4(S[4 * c], S[4 * c + 1], S[4 * c + 2], S[4 * c + 3]);
-        }
-#pragma unroll
-        for (int c = 0; c < NC; ++c) S[c] = 0.f;
-      } else if (a.n_seg > 1) {
-        // the state entering this segment from the segments before it
-        auto add = [&](int slot, float w, bool first) {
-          const float4* src = reinterpret_cast<const float4*>(seg_slot<DK>(a, x, slot));
-#pragma unroll
-          for (int c = 0; c < NC / 4; ++c) {
-            const float4 f = src[c * 128 + r];
-            S[4 * c] = fmaf(w, f.x, first ? 0.f : S[4 * c]);
-            S[4 * c + 1] = fmaf(w, f.y, first ? 0.f : S[4 * c + 1]);
-            S[4 * c + 2] = fmaf(w, f.z, first ? 0.f : S[4 * c + 2]);
-            S[4 * c + 3] = fmaf(w, f.w, first ? 0.f : S[4 * c + 3]);
-          }
-        };
-        add(a.n_seg - 1, x.seg == 0 ? 1.f : exp2f(l2 * static_cast<float>(x.p0 - one.dir.lead)), true);
-        for (int f = 0; f < x.seg && x.count > 0; ++f)
-          add(f, exp2f(l2 * static_cast<float>(x.p0 - (f + 1) * a.seg_tokens)), false);
-      }
-      // the state's bf16 parts for chunk gg's Q S
-      auto put_state = [&](int gg) {
-        const int sb = gg % C::STB;
-        if (gg >= C::STB && !mbar_wait_warp(bar(ST_EMPTY + sb), (gg / C::STB - 1) & 1, status)) return false;
-#pragma unroll
-        for (int c = 0; c < NC / 8; ++c) {
-          uint32_t h[4], l[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            h[j] = pack_bf16x2(S[8 * c + 2 * j], S[8 * c + 2 * j + 1]);
-            l[j] = lo_pair(S[8 * c + 2 * j], S[8 * c + 2 * j + 1], h[j]);
-          }
-          const uint32_t at = sS(sb) + sw128_offset(row, col0 * 2 + c * 16);
-          st_shared_v4(at, h[0], h[1], h[2], h[3]);
-          st_shared_v4(at + C::ST_PLANE, l[0], l[1], l[2], l[3]);
-        }
-        fence_proxy_async_smem();
-        warp_arrive(bar(ST_FULL + sb));
-        return true;
-      };
-      if (!STATES && x.chunks > 0 && !(ok = put_state(g))) break;
-      for (int c = 0; c < x.chunks; ++c, ++g) {
-        const int left = x.count - c * 128, valid = left < 128 ? left : 128;
-        // the carried state enters the very first token without a decay (lead)
-        const int lead = c == 0 && x.seg == 0 && !STATES ? one.dir.lead : 0;
-        if (!(ok = mbar_wait_warp(bar(KV_FULL + (g & 1)), (g >> 1) & 1, status))) break;
-        tc_fence_after();
-        const float dec = exp2f(l2 * static_cast<float>(valid - lead));
-#pragma unroll
-        for (int j = 0; j < NC / 16; ++j) {
-          uint32_t v[16];
-          tmem_ld16(tmem + T_KV + (g & 1) * 64 + col0 + j * 16 + lane_base, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) S[16 * j + e] = fmaf(dec, S[16 * j + e], __uint_as_float(v[e]));
-        }
-        tc_fence_before();
-        warp_arrive(bar(KV_FREE + (g & 1)));
-        if (STATES) continue;
-        if (c + 1 < x.chunks && !(ok = put_state(g + 1))) break;
-      }
-      if (!ok) break;
-      if (STATES) {
-        if (x.seg < a.n_seg - 1) {
-          float4* dst = reinterpret_cast<float4*>(seg_slot<DK>(a, x, x.seg));
-#pragma unroll
-          for (int c = 0; c < NC / 4; ++c) dst[c * 128 + r] = make_float4(S[4 * c], S[4 * c + 1], S[4 * c + 2], S[4 * c + 3]);
-        }
-        continue;
-      }
-      // after the last token's segment (the first one of an empty sequence)
-      if (one.s_out && in_state && x.seg == (x.n > 0 ? (x.n - 1) / a.seg_tokens : 0)) {
-        const float w = one.dir.out_mult * (one.dir.lead && x.n > 0 ? exp2f(l2) : 1.f);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) one.s_out[state_at(c)] = w * S[c];
-      }
-      if (!one.dir.accumulate) {  // zeros past the sequence
-        const int p1 = a.L - x.p0 < a.seg_tokens ? a.L : x.p0 + a.seg_tokens;
-        const int pz = x.n > x.p0 ? x.n : x.p0;
-        const int vecs = (a.D < 64 ? a.D : 64) * static_cast<int>(sizeof(T)) / 16;
-        const long long zeros = static_cast<long long>(p1 - pz) * vecs;
-        for (long long i = r; i < zeros; i += 128) {
-          const size_t tok = static_cast<size_t>(x.b) * a.L + pz + i / vecs;
-          reinterpret_cast<uint4*>(static_cast<T*>(one.o) + (tok * a.H + x.h) * a.D + x.half * 64)[i % vecs] =
-              make_uint4(0, 0, 0, 0);
-        }
       }
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == 18) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
@@ -869,7 +1011,7 @@ MixPlan mix_plan(const AttnShape& sh, int n_dir) {
 }
 
 template <typename T, int DK, int NT>
-int mix_launch(MixArgs a, uint32_t* status, cudaStream_t s) {
+int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s) {
   using C = MixCfg<DK, NT>;
   static std::atomic<uint64_t> attr_s{0}, attr{0};
   const int sms = device_sm_count();
@@ -877,12 +1019,22 @@ int mix_launch(MixArgs a, uint32_t* status, cudaStream_t s) {
     if (!ensure_smem_attr(mix_kernel<T, DK, NT, true>, C::SMEM, attr_s)) return PA_ERR_LAUNCH;
     MixArgs f = a;
     f.n_units = a.n_units / a.n_seg * (a.n_seg - 1);
-    mix_kernel<T, DK, NT, true><<<f.n_units < sms ? f.n_units : sms, kMixThreads, C::SMEM, s>>>(f, status);
+    mix_kernel<T, DK, NT, true><<<f.n_units < sms ? f.n_units : sms, kMixThreads, C::SMEM, s>>>(f, maps, status);
     if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
   }
   if (!ensure_smem_attr(mix_kernel<T, DK, NT, false>, C::SMEM, attr)) return PA_ERR_LAUNCH;
-  mix_kernel<T, DK, NT, false><<<a.n_units < sms ? a.n_units : sms, kMixThreads, C::SMEM, s>>>(a, status);
+  mix_kernel<T, DK, NT, false><<<a.n_units < sms ? a.n_units : sms, kMixThreads, C::SMEM, s>>>(a, maps, status);
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
+// An output [B, L, H, D] as boxes of 32 columns x 1 head x 32 tokens.
+bool make_out_map(CUtensorMap* m, const void* base, const AttnShape& sh, bool f32) {
+  const uint64_t e = f32 ? 4 : 2, D = sh.D, H = sh.H, L = sh.L;
+  const uint64_t dims[4] = {D, H, L, static_cast<uint64_t>(sh.B)};
+  const uint64_t strides[3] = {D * e, H * D * e, L * H * D * e};
+  const uint32_t box[4] = {32, 1, 32, 1};
+  return make_tmap(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
+                   box, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const int32_t* lens, void* ws,
@@ -899,11 +1051,32 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
   a.seg_tokens = p.seg_tokens;
   a.n_units = p.units;
   a.scale = sh.scale;
-  if (!f32)
-    return sh.D == 64 ? mix_launch<__nv_bfloat16, 64, 1>(a, status, s)
-                      : mix_launch<__nv_bfloat16, 128, 1>(a, status, s);
-  return f32_math() == PA_F32_MATH_BF16 ? mix_launch<float, 64, 1>(a, status, s)
-                                        : mix_launch<float, 64, 3>(a, status, s);
+  MixMaps maps{};
+  for (int d = 0; d < a.n_dir; ++d) {
+    if (!make_out_map(&maps.o[d], a.one[d].o, sh, f32)) return PA_ERR_ALIGN;
+    a.one[d].mo = d;
+  }
+  if (f32)
+    return f32_math() == PA_F32_MATH_BF16 ? mix_launch<float, 64, 1>(a, maps, status, s)
+                                          : mix_launch<float, 64, 3>(a, maps, status, s);
+  // tensor maps of the distinct inputs (at most q, k, v and dO)
+  const void* seen[4];
+  int n = 0;
+  for (int d = 0; d < a.n_dir; ++d) {
+    const void* in[3] = {a.one[d].q, a.one[d].k, a.one[d].v};
+    int* index[3] = {&a.one[d].mq, &a.one[d].mk, &a.one[d].mv};
+    for (int j = 0; j < 3; ++j) {
+      int m = 0;
+      while (m < n && seen[m] != in[j]) ++m;
+      if (m == n) {
+        if (!make_qkv_map(&maps.m[n], in[j], sh, 128)) return PA_ERR_ALIGN;
+        seen[n++] = in[j];
+      }
+      *index[j] = m;
+    }
+  }
+  return sh.D == 64 ? mix_launch<__nv_bfloat16, 64, 1>(a, maps, status, s)
+                    : mix_launch<__nv_bfloat16, 128, 1>(a, maps, status, s);
 }
 
 template <typename T, int D>
