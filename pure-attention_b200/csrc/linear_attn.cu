@@ -58,9 +58,9 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
-// Roundings: fp32 sums and state throughout. V' and the state are two bf16
-// parts (off by 2^-16), so states keep fp32-like accuracy; P is one bf16 (2^-8),
-// as in the softmax kernels. NT = 3 (fp32 operands): every operand is a
+// Roundings: fp32 sums and state throughout. V' is two bf16 parts (off by 2^-16), so
+// the states keep fp32-like accuracy; as operands of the output's two products, P and
+// the state entering the chunk are one bf16 each (2^-8), like P in the softmax kernels. NT = 3 (fp32 operands): every operand is a
 // hi/lo pair and every product hi*hi + hi*lo + lo*hi.
 //
 // TMEM columns: Q K^T and P 2 x 128 (P of 32 tokens over their 32 scores: hi in the
@@ -77,8 +77,9 @@ struct MixCfg {
   static constexpr int VP_BYTES = 2 * kTile;       // V' hi and lo
   static constexpr int ST_PLANE = DK * 128;        // [DK, 64] bf16
   static constexpr bool SMALL = NP == 1 && DK == 64;
-  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 3 : (NP == 1 ? 2 : 1), STB = DK == 64 ? 2 : 1;
-  static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + VP_BYTES + STB * 2 * ST_PLANE + 1024;
+  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 4 : (NP == 1 ? 2 : 1);
+  // V', state planes, and 2 KB a warp through which the output goes out
+  static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + VP_BYTES + NP * ST_PLANE + kTile + 1024;
   static constexpr int NC = DK == 64 ? 32 : 64;    // state columns of a thread
 };
 static_assert(MixCfg<64, 1>::SMEM <= 225 * 1024 && MixCfg<64, 3>::SMEM <= 225 * 1024 &&
@@ -105,7 +106,7 @@ struct MixArgs {
 };
 struct MixMaps {
   CUtensorMap m[4];  // inputs: 64 columns x 128 tokens
-  CUtensorMap o[3];  // outputs: 32 columns x 32 tokens
+  CUtensorMap o[3];  // outputs: 64 bytes of columns x 32 tokens
 };
 
 struct MixUnit {
@@ -166,13 +167,15 @@ template <int DK, bool STATES>
 struct ChunkIter {
   MixUnit x;
   int u, chunk, g;  // g: chunks of this CTA so far
-  __device__ __forceinline__ bool first(const MixArgs& a) {
+  int n_units;
+  __device__ __forceinline__ bool first(const MixArgs& a, int units) {
+    n_units = units;
     u = blockIdx.x;
     chunk = g = 0;
     return settle(a);
   }
   __device__ __forceinline__ bool settle(const MixArgs& a) {  // to a unit that has chunks
-    for (; u < a.n_units; u += gridDim.x) {
+    for (; u < n_units; u += gridDim.x) {
       x = mix_unit<DK, STATES>(a, u);
       if (x.chunks > 0) return true;
     }
@@ -238,18 +241,6 @@ struct Rows {
   }
 };
 
-// Two 8-column TMEM loads and their wait.
-__device__ __forceinline__ void tmem_ld8x2_sync(uint32_t ta, uint32_t tb, uint32_t (&a)[8], uint32_t (&b)[8]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%16];\n\t"
-      "tcgen05.ld.sync.aligned.32x32b.x8.b32 {%8,%9,%10,%11,%12,%13,%14,%15}, [%17];\n\t"
-      "tcgen05.wait::ld.sync.aligned;"
-      : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3]), "=r"(a[4]), "=r"(a[5]), "=r"(a[6]), "=r"(a[7]), "=r"(b[0]),
-        "=r"(b[1]), "=r"(b[2]), "=r"(b[3]), "=r"(b[4]), "=r"(b[5]), "=r"(b[6]), "=r"(b[7])
-      : "r"(ta), "r"(tb)
-      : "memory");
-}
-
 // 32 values of an output row += f.
 __device__ __forceinline__ void add_row(float* dst, const float2 (&f)[16]) {
 #pragma unroll
@@ -279,11 +270,13 @@ __device__ __forceinline__ void warp_arrive(uint32_t bar) {
   if (lane_id() == 0) mbar_arrive(bar);
 }
 
-// A descriptor `bytes` further on (its address field is the low 14 bits, in 16 bytes).
-__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t bytes) {
-  const uint32_t lo = static_cast<uint32_t>(desc) + (bytes >> 4);
-  return (desc & 0xffffffff00000000ull) | lo;
-}
+// A shared-memory descriptor and the one `bytes` further on (16-byte units in the low word).
+struct Desc {
+  uint64_t d;
+  __device__ __forceinline__ Desc at(uint32_t bytes) const {
+    return Desc{(d & 0xffffffff00000000ull) | (static_cast<uint32_t>(d) + (bytes >> 4))};
+  }
+};
 
 // STATES: only the segments' own states, into the workspace.
 template <typename T, int DK, int NT, bool STATES>
@@ -297,17 +290,15 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   __shared__ __align__(16) float wtab[4 * 64 + 4 * 32];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  if (cta_aborted(status, &abort_flag)) return;
   const uint32_t sm0 = smem_u32(align1024(smem_raw));
   const uint32_t sv0 = sm0 + C::QKS * 2 * C::OPER, sVp = sv0 + C::VS * C::V_STAGE, ss0 = sVp + C::VP_BYTES;
   auto bar = [&](int i) { return smem_u32(&bars[i]); };
-  // ring slot s: K planes, then Q planes; V planes; state hi, lo. V' hi, lo at sVp.
+  // ring slot s: K planes, then Q planes; V planes. V' hi, lo; the state's hi, lo (ss0); the stage
   auto sK = [&](int s) { return sm0 + s * 2 * C::OPER; };
   auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
   auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
-  auto sS = [&](int s) { return ss0 + s * 2 * C::ST_PLANE; };
-  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 9, S_FULL = 12, P_FULL = 14, ST_FULL = 16, ST_EMPTY = 18,
-         VP_FULL = 20, VP_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, N_BARS };
+  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 10, S_FULL = 14, P_FULL = 16, VP_FULL = 18, VP_EMPTY,
+         ST_FULL, ST_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, N_BARS };
   constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
 
   const int warp = warp_id();
@@ -315,17 +306,19 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     for (int i = 0; i < 3; ++i) {
       mbar_init(bar(QK_FULL + i), TMA ? 1 : (STATES ? 2 : 6));  // fp32: the loading warps
       mbar_init(bar(QK_EMPTY + i), 1);
+    }
+    for (int i = 0; i < 4; ++i) {
       mbar_init(bar(V_FULL + i), TMA ? 1 : 4);
-      mbar_init(bar(V_EMPTY + i), STATES ? 1 : 8);
+      mbar_init(bar(V_EMPTY + i), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(S_FULL + i), 1);
       mbar_init(bar(P_FULL + i), 8);
-      mbar_init(bar(ST_FULL + i), 4);
-      mbar_init(bar(ST_EMPTY + i), 1);
     }
     mbar_init(bar(VP_FULL), 4);
     mbar_init(bar(VP_EMPTY), 1);
+    mbar_init(bar(ST_FULL), 4);
+    mbar_init(bar(ST_EMPTY), 1);
     mbar_init(bar(KV_FULL), 1);
     mbar_init(bar(KV_FREE), 4);
     mbar_init(bar(O_FULL), 1);
@@ -336,10 +329,17 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
+  if (warp == 19 && lane_id() == 0) abort_flag = aborted(status);
+  if (TMA && warp == 16 && lane_id() < 3) {
+    const MixOne& one = a.one[mix_unit<DK, STATES>(a, blockIdx.x).dir];
+    tma_prefetch_desc(&maps.m[lane_id() == 0 ? one.mk : (lane_id() == 1 ? one.mq : one.mv)]);
+  }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // an earlier kernel's failure: no work
+  const int n_units = abort_flag ? 0 : a.n_units;
   const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
 
   // Head dim 128: a state thread holds 64 values. 2 x 96 + 152 + 88 + 48 = 5 x 96 registers.
@@ -361,16 +361,6 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       // the chunk whose output is due
       int o_dir = 0, o_col = 0, o_h = 0, o_tok = 0, o_b = 0, o_valid = 0;
       float o_scale = 0.f;   // of Q S
-      bool o_stored = false; // a store of this warp may still read the V slot of chunk g - 1
-      // The output goes through the V slot of its own chunk (P V was its last reader).
-      // 32 rows of 64 (bf16) or 128 bytes per warp, swizzled as the tensor map says.
-      auto release = [&]() {
-        if (o_stored && lane == 0) {
-          bulk_wait_read<0>();
-          mbar_arrive(bar(V_EMPTY + (g - 2) % C::VS));
-        }
-        o_stored = false;
-      };
       auto write_out = [&]() {
         if (!mbar_wait_warp(bar(O_FULL), (g - 1) & 1, status)) return false;
         tc_fence_after();
@@ -381,7 +371,6 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         tmem_ld32_sync(at + T_PV, o2);
         tc_fence_before();
         warp_arrive(bar(O_FREE));
-        o_stored = true;
         if (32 * part >= a.D) return true;  // head dim 32: no columns for part 1
         float2 f[16];
 #pragma unroll
@@ -396,33 +385,38 @@ __global__ void __launch_bounds__(kMixThreads, 1)
                     f);
           return true;
         }
-        const uint32_t stage = sV((g - 1) % C::VS) + warp * (32 * 32 * static_cast<int>(sizeof(T)));
         if (i >= o_valid) {
 #pragma unroll
           for (int e = 0; e < 16; ++e) f[e] = make_float2(0.f, 0.f);
         }
-        if constexpr (sizeof(T) == 2) {
+        // 32 rows of 64 bytes a store, 64-byte swizzled: a bf16 row's 32 columns, 16 of fp32
+        const uint32_t stage = ss0 + NP * C::ST_PLANE + warp * 2048;
+        constexpr int STORES = static_cast<int>(sizeof(T)) / 2;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            st_shared_v4(stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4), hi_pair(f[4 * c]), hi_pair(f[4 * c + 1]),
-                         hi_pair(f[4 * c + 2]), hi_pair(f[4 * c + 3]));
-        } else {
+        for (int half = 0; half < STORES; ++half) {
+          if (lane == 0) bulk_wait_read<0>();  // this warp's store before
+          __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 8; ++c)
-            st_shared_v4(stage + sw128_offset(lane, c * 16), __float_as_uint(f[2 * c].x), __float_as_uint(f[2 * c].y),
-                         __float_as_uint(f[2 * c + 1].x), __float_as_uint(f[2 * c + 1].y));
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0 && o_tok + 32 * w4 < a.L) {
-          const CUtensorMap* map = &maps.o[a.one[o_dir].mo];
-          if (add) tma_reduce_add_4d(map, stage, o_col, o_h, o_tok + 32 * w4, o_b);
-          else tma_store_4d(map, stage, o_col, o_h, o_tok + 32 * w4, o_b);
-          tma_store_commit();
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t to = stage + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4);
+            if constexpr (sizeof(T) == 2)
+              st_shared_v4(to, hi_pair(f[4 * c]), hi_pair(f[4 * c + 1]), hi_pair(f[4 * c + 2]), hi_pair(f[4 * c + 3]));
+            else
+              st_shared_v4(to, __float_as_uint(f[8 * half + 2 * c].x), __float_as_uint(f[8 * half + 2 * c].y),
+                           __float_as_uint(f[8 * half + 2 * c + 1].x), __float_as_uint(f[8 * half + 2 * c + 1].y));
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && o_tok + 32 * w4 < a.L) {
+            const CUtensorMap* map = &maps.o[a.one[o_dir].mo];
+            if (add) tma_reduce_add_4d(map, stage, o_col + 16 * half, o_h, o_tok + 32 * w4, o_b);
+            else tma_store_4d(map, stage, o_col + 16 * half, o_h, o_tok + 32 * w4, o_b);
+            tma_store_commit();
+          }
         }
         return true;
       };
-      for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+      for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
         const MixUnit x = mix_unit<DK, STATES>(a, u);
         if (x.chunks == 0) continue;
         const MixOne& one = a.one[x.dir];
@@ -447,7 +441,6 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         const float l_first = exp2f(l2 * static_cast<float>((x.rev ? 31 - lane : lane + 1) + 32 * (d0 - 1)));
         for (int c = 0; c < x.chunks; ++c) {
           const int valid = x.valid(c);
-          release();  // before any wait: the loads may wait for this slot
           if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
           tc_fence_after();
           const uint32_t ts = tmem + T_S + (g & 1) * 128 + lane_base;
@@ -528,7 +521,6 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           ++g;
         }
       }
-      release();
       if (ok && g > 0) write_out();
       if (lane == 0) bulk_wait_all();
     }
@@ -539,7 +531,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
     int g = 0;
     bool ok = true;
-    for (int u = blockIdx.x; ok && u < a.n_units; u += gridDim.x) {
+    for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
       const MixUnit x = mix_unit<DK, STATES>(a, u);
       const MixOne& one = a.one[x.dir];
       const float l2 = log2_decay(a.log_decay, x.h);
@@ -593,22 +585,20 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       }
       // the state's bf16 parts for chunk gg's Q S
       auto put_state = [&](int gg) {
-        const int sb = gg % C::STB;
-        if (gg >= C::STB && !mbar_wait_warp(bar(ST_EMPTY + sb), (gg / C::STB - 1) & 1, status)) return false;
+        if (gg > 0 && !mbar_wait_warp(bar(ST_EMPTY), (gg - 1) & 1, status)) return false;
 #pragma unroll
         for (int c = 0; c < NC / 8; ++c) {
-          uint32_t h[4], l[4];
+          uint32_t h[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            h[j] = hi_pair(S[4 * c + j]);
-            l[j] = lo_pair(S[4 * c + j], h[j]);
-          }
-          const uint32_t at = sS(sb) + sw128_offset(row, col0 * 2 + c * 16);
+          for (int j = 0; j < 4; ++j) h[j] = hi_pair(S[4 * c + j]);
+          const uint32_t at = ss0 + sw128_offset(row, col0 * 2 + c * 16);
           st_shared_v4(at, h[0], h[1], h[2], h[3]);
-          st_shared_v4(at + C::ST_PLANE, l[0], l[1], l[2], l[3]);
+          if (NT == 3)
+            st_shared_v4(at + C::ST_PLANE, lo_pair(S[4 * c], h[0]), lo_pair(S[4 * c + 1], h[1]),
+                         lo_pair(S[4 * c + 2], h[2]), lo_pair(S[4 * c + 3], h[3]));
         }
         fence_proxy_async_smem();
-        warp_arrive(bar(ST_FULL + sb));
+        warp_arrive(bar(ST_FULL));
         return true;
       };
       if (!STATES && x.chunks > 0 && !(ok = put_state(g))) break;
@@ -620,13 +610,13 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         if (!(ok = mbar_wait_warp(bar(KV_FULL), g & 1, status))) break;
         tc_fence_after();
 #pragma unroll
-        for (int j = 0; j < NC / 8; ++j) {
-          uint32_t vh[8], vl[8];  // K^T V' hi and K^T V' lo
-          const uint32_t at = tmem + T_KV + col0 + j * 8 + lane_base;
-          tmem_ld8x2_sync(at, at + 64, vh, vl);
+        for (int j = 0; j < NC / 16; ++j) {
+          uint32_t vh[16], vl[16];  // K^T V' hi and K^T V' lo
+          const uint32_t at = tmem + T_KV + col0 + j * 16 + lane_base;
+          tmem_ld16x2_sync(at, at + 64, vh, vl);
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            S[4 * j + e] = __ffma2_rn(dec2, S[4 * j + e], __fadd2_rn(pair_of(vh[2 * e], vh[2 * e + 1]),
+          for (int e = 0; e < 8; ++e)
+            S[8 * j + e] = __ffma2_rn(dec2, S[8 * j + e], __fadd2_rn(pair_of(vh[2 * e], vh[2 * e + 1]),
                                                                    pair_of(vl[2 * e], vl[2 * e + 1])));
         }
         tc_fence_before();
@@ -664,7 +654,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     // ------------------------------------------------------------ V'
     const int t = threadIdx.x - 12 * 32;
     ChunkIter<DK, STATES> it;
-    bool more = it.first(a);
+    bool more = it.first(a, n_units);
     int w_unit = -1, w_valid = 0;
     // l^(valid - 1 - row), backward l^row; zero past the end
     auto weight = [&](int row, int valid) {
@@ -689,7 +679,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           w_valid = valid;
         }
         if (!mbar_wait_warp(bar(V_FULL + vs), (g / C::VS) & 1, status)) break;
-        if (it.x.token(it.chunk) + valid < a.L && valid < 128) {
+        uint4 v[8];  // all loads before the first store: they may not pass it
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = ld_shared_v4(sV(vs) + sw128_offset(t / 8 + 16 * i, (t % 8) * 16));
+        if (valid < 128) {
           // Tokens past this sequence lie in the tiles, and may hold anything: their rows of V meet
           // zeros of P, and their rows of K zeros of V', which NaN or infinity would survive.
           const int s = g % C::QKS;
@@ -698,22 +691,23 @@ __global__ void __launch_bounds__(kMixThreads, 1)
             st_shared_v4(sV(vs) + z * 16, 0, 0, 0, 0);
             for (int tile = 0; tile < KT; ++tile) st_shared_v4(sK(s) + tile * kTile + z * 16, 0, 0, 0, 0);
           }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (t / 8 + 16 * i >= valid) v[i] = make_uint4(0, 0, 0, 0);
         }
         if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const int row = t / 8 + 16 * i;
-          const uint32_t off = sw128_offset(row, (t % 8) * 16);
-          const uint4 v = ld_shared_v4(sV(vs) + off);
-          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+          const uint32_t off = sw128_offset(t / 8 + 16 * i, (t % 8) * 16);
+          const uint32_t x[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
           uint32_t h[4], l[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const __nv_bfloat162 vv = *reinterpret_cast<const __nv_bfloat162*>(&x[j]);
             const __nv_bfloat162 hh = __hmul2_rn(vv, wh[i]);
             const __nv_bfloat162 ll = __hfma2(vv, wl[i], __hfma2(vv, wh[i], __hneg2(hh)));
-            h[j] = row < valid ? *reinterpret_cast<const uint32_t*>(&hh) : 0;
-            l[j] = row < valid ? *reinterpret_cast<const uint32_t*>(&ll) : 0;
+            h[j] = *reinterpret_cast<const uint32_t*>(&hh);
+            l[j] = *reinterpret_cast<const uint32_t*>(&ll);
           }
           st_shared_v4(sVp + off, h[0], h[1], h[2], h[3]);
           st_shared_v4(sVp + kTile + off, l[0], l[1], l[2], l[3]);
@@ -739,10 +733,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           put4(at, NP == 2 ? at + kTile : 0, sw128_offset(row_of(half, i), (t % 16) * 8), make_float2(r[i].x, r[i].y),
                make_float2(r[i].z, r[i].w));
       };
-      auto put_times = [&](const float4 (&r)[HALF], const float (&w)[HALF], int half) {
+      auto put_times = [&](const float4 (&r)[HALF], const float (&w)[HALF], uint32_t at, int half) {
 #pragma unroll
         for (int i = 0; i < HALF; ++i)
-          put4(sVp, sVp + kTile, sw128_offset(row_of(half, i), (t % 16) * 8),
+          put4(at, at + kTile, sw128_offset(row_of(half, i), (t % 16) * 8),
                __fmul2_rn(make_float2(r[i].x, r[i].y), make_float2(w[i], w[i])),
                __fmul2_rn(make_float2(r[i].z, r[i].w), make_float2(w[i], w[i])));
       };
@@ -774,8 +768,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           load_half(r1, a.one[it.x.dir].v, 1);
         }
         if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
-        put_times(r0, w0, 0);
-        put_times(r1, w1, 1);
+        put_times(r0, w0, sVp, 0);
+        put_times(r1, w1, sVp, 1);
         fence_proxy_async_smem();
         warp_arrive(bar(VP_FULL));
         if (!STATES) {
@@ -794,7 +788,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       // ------------------------------------------------------------ TMA loads
       if (warp == 16 && elect_one()) {
         ChunkIter<DK, STATES> it;
-        for (bool more = it.first(a); more; more = it.next(a)) {
+        for (bool more = it.first(a, n_units); more; more = it.next(a)) {
           const int g = it.g, s = g % C::QKS, vs = g % C::VS;
           const MixOne& one = a.one[it.x.dir];
           const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
@@ -815,7 +809,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       using R = Rows<64>;
       constexpr int QUARTERS = R::VECS / 8;
       ChunkIter<DK, STATES> it;
-      bool more = it.first(a);
+      bool more = it.first(a, n_units);
       float4 r0[8], r1[8];
       auto load = [&](float4 (&r)[8], int quarter) {
         const R rows(a, it, a.one[it.x.dir].k, t);
@@ -849,26 +843,28 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
       int total = 0;
-      for (int u = blockIdx.x; u < a.n_units; u += gridDim.x) total += mix_unit<DK, STATES>(a, u).chunks;
+      for (int u = blockIdx.x; u < n_units; u += gridDim.x) total += mix_unit<DK, STATES>(a, u).chunks;
       constexpr uint32_t idS = make_idesc(128, 128, 1, false, false), idV = make_idesc(128, 64, 1, false, true),
                          idKV = make_idesc(128, 128, 1, true, true), idKV1 = make_idesc(128, 64, 1, true, true);
       constexpr int LO = KT * kTile;  // from a hi plane of q or k to its lo plane
+      // K-step `k` of a K-major tile, of an MN-major one
+      auto kmaj = [](int k) { return static_cast<uint32_t>((k / 4) * kTile + (k % 4) * 32); };
+      auto mn = [](int k) { return static_cast<uint32_t>(k * 2048); };
+      const Desc dQ{make_sdesc(sQ(0), 16, 1024)}, dK{make_sdesc(sK(0), 16, 1024)},
+          dKt{make_sdesc(sK(0), DK == 64 ? 0 : kTile, 1024)}, dV{make_sdesc(sV(0), kTile, 1024)},
+          dVp{make_sdesc(sVp, kTile, 1024)}, dS{make_sdesc(ss0, kTile, 1024)};
       auto wait = [&](int i, int phase) { return mbar_wait(bar(i), phase & 1, status); };
       auto issue_S = [&](int g) {
         const int s = g % C::QKS;
         if (!wait(QK_FULL + s, g / C::QKS)) return false;
         tc_fence_after();
-#pragma unroll 1
-        for (int term = 0; term < NT; ++term) {
-          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? LO : 0), 16, 1024);
-          const uint64_t kd = make_sdesc(sK(s) + (term == 1 ? LO : 0), 16, 1024);
+        const Desc q = dQ.at(s * 2 * C::OPER), kk = dK.at(s * 2 * C::OPER);
 #pragma unroll
-          for (int k = 0; k < DK / 16; ++k) {
-            const uint32_t off = (k / 4) * kTile + (k % 4) * 32;
-            umma_f16_ss(tmem + T_S + (g & 1) * 128, desc_at(qd, off), desc_at(kd, off), idS,
-                        (term > 0 || k > 0) ? 1u : 0u);
-          }
-        }
+        for (int term = 0; term < NT; ++term)
+#pragma unroll
+          for (int k = 0; k < DK / 16; ++k)
+            umma_f16_ss(tmem + T_S + (g & 1) * 128, q.at((term == 2 ? LO : 0) + kmaj(k)).d,
+                        kk.at((term == 1 ? LO : 0) + kmaj(k)).d, idS, (term > 0 || k > 0) ? 1u : 0u);
         umma_commit(bar(S_FULL + (g & 1)));
         return true;
       };
@@ -882,16 +878,12 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         ok = ok && wait(VP_FULL, g) && (g < 1 || wait(KV_FREE, g - 1));
         if (!ok) break;
         tc_fence_after();
-        {
-          const uint64_t kd = make_sdesc(sK(s), DK == 64 ? 0 : kTile, 1024), vd = make_sdesc(sVp, kTile, 1024);
+        const Desc kt = dKt.at(s * 2 * C::OPER);
 #pragma unroll
-          for (int k = 0; k < 8; ++k)
-            umma_f16_ss(tmem + T_KV, desc_at(kd, k * 2048), desc_at(vd, k * 2048), idKV, k > 0 ? 1u : 0u);
-          if (NT == 3) {
+        for (int k = 0; k < 8; ++k) umma_f16_ss(tmem + T_KV, kt.at(mn(k)).d, dVp.at(mn(k)).d, idKV, k > 0 ? 1u : 0u);
+        if (NT == 3) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
-              umma_f16_ss(tmem + T_KV, desc_at(kd, LO + k * 2048), desc_at(vd, k * 2048), idKV1, 1u);
-          }
+          for (int k = 0; k < 8; ++k) umma_f16_ss(tmem + T_KV, kt.at(LO + mn(k)).d, dVp.at(mn(k)).d, idKV1, 1u);
         }
         umma_commit(bar(KV_FULL));
         umma_commit(bar(VP_EMPTY));
@@ -902,34 +894,30 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         }
         if (g + 1 < total && !(ok = issue_S(g + 1))) break;
         // Q S from the state entering this chunk
-        const int sb = g % C::STB;
-        ok = wait(ST_FULL + sb, g / C::STB) && (g < 1 || wait(O_FREE, g - 1));
+        ok = wait(ST_FULL, g) && (g < 1 || wait(O_FREE, g - 1));
         if (!ok) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int term = 0; term < (NT == 3 ? 3 : 2); ++term) {
-          const uint64_t qd = make_sdesc(sQ(s) + (term == 2 ? LO : 0), 16, 1024);
-          const uint64_t sd = make_sdesc(sS(sb) + (term == 1 ? C::ST_PLANE : 0), kTile, 1024);
+        const Desc q = dQ.at(s * 2 * C::OPER);
+#pragma unroll
+        for (int term = 0; term < NT; ++term)
 #pragma unroll
           for (int k = 0; k < DK / 16; ++k)
-            umma_f16_ss(tmem + T_QS, desc_at(qd, (k / 4) * kTile + (k % 4) * 32), desc_at(sd, k * 2048), idV,
-                        (term > 0 || k > 0) ? 1u : 0u);
-        }
-        umma_commit(bar(ST_EMPTY + sb));
+            umma_f16_ss(tmem + T_QS, q.at((term == 2 ? LO : 0) + kmaj(k)).d,
+                        dS.at((term == 1 ? C::ST_PLANE : 0) + mn(k)).d, idV, (term > 0 || k > 0) ? 1u : 0u);
+        umma_commit(bar(ST_EMPTY));
         umma_commit(bar(QK_EMPTY + s));
         // P V
         ok = wait(V_FULL + vs, g / C::VS) && wait(P_FULL + b, g >> 1);
         if (!ok) break;
         tc_fence_after();
-#pragma unroll 1
-        for (int term = 0; term < NT; ++term) {
-          const uint64_t vd = make_sdesc(sV(vs) + (term == 1 ? kTile : 0), kTile, 1024);
-          const uint32_t p0 = tmem + T_S + b * 128 + (term == 2 ? 16 : 0);
+        const Desc v = dV.at(vs * C::V_STAGE);
+#pragma unroll
+        for (int term = 0; term < NT; ++term)
 #pragma unroll
           for (int k = 0; k < 8; ++k)
-            umma_f16_ts(tmem + T_PV, p0 + (k / 2) * 32 + (k % 2) * 8, desc_at(vd, k * 2048), idV,
-                        (term > 0 || k > 0) ? 1u : 0u);
-        }
+            umma_f16_ts(tmem + T_PV, tmem + T_S + b * 128 + (term == 2 ? 16 : 0) + (k / 2) * 32 + (k % 2) * 8,
+                        v.at((term == 1 ? kTile : 0) + mn(k)).d, idV, (term > 0 || k > 0) ? 1u : 0u);
+        umma_commit(bar(V_EMPTY + vs));
         umma_commit(bar(O_FULL));
       }
     }
@@ -1027,14 +1015,14 @@ int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s)
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
-// An output [B, L, H, D] as boxes of 32 columns x 1 head x 32 tokens.
+// An output [B, L, H, D] as boxes of 64 bytes of columns x 1 head x 32 tokens.
 bool make_out_map(CUtensorMap* m, const void* base, const AttnShape& sh, bool f32) {
   const uint64_t e = f32 ? 4 : 2, D = sh.D, H = sh.H, L = sh.L;
   const uint64_t dims[4] = {D, H, L, static_cast<uint64_t>(sh.B)};
   const uint64_t strides[3] = {D * e, H * D * e, L * H * D * e};
-  const uint32_t box[4] = {32, 1, 32, 1};
+  const uint32_t box[4] = {static_cast<uint32_t>(64 / e), 1, 32, 1};
   return make_tmap(m, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, base, dims, strides,
-                   box, f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                   box, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const int32_t* lens, void* ws,
