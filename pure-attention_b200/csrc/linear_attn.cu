@@ -53,8 +53,8 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 //   warps 8-11  the state in fp32 registers (thread = row of the state), its bf16
 //               parts to shared memory for Q S
 //   warps 12-15 V' from V (fp32: and q, v through registers, split on the way)
-//   warps 16-17 bf16: TMA loads of q, k, v; fp32: k through registers
-//   warp 18     tcgen05.mma issue
+//   warps 16-19 tcgen05.mma issue (one warp); bf16: TMA loads of q, k, v (one thread);
+//               fp32: k through registers (two warps)
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
@@ -325,12 +325,17 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     mbar_init(bar(O_FREE), 8);
     fence_mbar_init();
   }
-  if (warp == 18) {
+  // Role of a warp of the last warpgroup: 0 MMA issue, 1 and 2 loads. The issuing warp slows the
+  // other warps of its sub-partition (an MMA that waits for the queue holds up their TMEM
+  // loads), so it sits with the 32 rows that have the fewest scores: the first forward in time,
+  // the last backward.
+  const int role = warp < 16 ? -1 : (warp - 16 + (a.n_dir == 1 ? 0 : 1)) & 3;
+  if (role == 0) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
-  if (warp == 19 && lane_id() == 0) abort_flag = aborted(status);
-  if (TMA && warp == 16 && lane_id() < 3) {
+  if (role == 3 && lane_id() == 0) abort_flag = aborted(status);
+  if (TMA && role == 1 && lane_id() < 3) {
     const MixOne& one = a.one[mix_unit<DK, STATES>(a, blockIdx.x).dir];
     tma_prefetch_desc(&maps.m[lane_id() == 0 ? one.mk : (lane_id() == 1 ? one.mq : one.mv)]);
   }
@@ -421,8 +426,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         if (x.chunks == 0) continue;
         const MixOne& one = a.one[x.dir];
         const float l2 = log2_decay(a.log_decay, x.h);
-        // tab[e] with e = 31 - lane + j on the diagonal: forward l^(31-e) for e <= 31, backward
-        // l^(e-31) for e >= 31; the blocks beside it use its first / its last 32. Times scale.
+        // Part 0: tab[e] with e = 31 - lane + j, forward l^(31-e) for e <= 31, backward l^(e-31) for
+        // e >= 31. Part 1: l^(31-j), backward l^(j+1). All times scale.
         __syncwarp();
         const float near = a.scale * exp2f(l2 * static_cast<float>(x.rev ? lane + 1 : 31 - lane));
         if (part == 0) {
@@ -432,13 +437,12 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           tab[lane] = near;
         }
         __syncwarp();
-        const float *beside = part == 0 && x.rev ? tab + 32 : tab, *diag = tab + 31 - lane;
-        // Blocks beside the diagonal, at distance d = 1 .. nb: part 0 takes the nearer ones and the
-        // diagonal, part 1 the farther ones. l^|i-j| = l^(32 (d - 1)) l^(base) tab, no negative exponent.
-        const int nb = x.rev ? 3 - w4 : w4, cut = nb / 2;
-        const int d0 = part == 0 ? 1 : cut + 1, d1 = part == 0 ? cut : nb, dir = x.rev ? 1 : -1;
+        const float* diag = tab + 31 - lane;
+        // Part 0 takes the block on the diagonal (as dear as two others), part 1 those beside it, at
+        // distance d = 1 .. nb: l^|i-j| = l^(32 (d - 1)) l_first tab, no negative exponent.
+        const int nb = x.rev ? 3 - w4 : w4, dir = x.rev ? 1 : -1;
         const float l32 = exp2f(l2 * 32.f);
-        const float l_first = exp2f(l2 * static_cast<float>((x.rev ? 31 - lane : lane + 1) + 32 * (d0 - 1)));
+        const float l_first = exp2f(l2 * static_cast<float>(x.rev ? 31 - lane : lane + 1));
         for (int c = 0; c < x.chunks; ++c) {
           const int valid = x.valid(c);
           if (!(ok = mbar_wait_warp(bar(S_FULL + (g & 1)), (g >> 1) & 1, status))) break;
@@ -480,24 +484,24 @@ __global__ void __launch_bounds__(kMixThreads, 1)
             keep(x.rev ? tokens(w4) & (0xffffffffu << lane) : 0xffffffffu >> (31 - lane));
             put(w4);
           }
-          float rf = l_first;
+          if (part == 1) {
+            float rf = l_first;
 #pragma unroll 1
-          for (int d = d0; d <= d1; ++d) {
-            const int cb = w4 + dir * d;
-            tmem_ld32_sync(ts + cb * 32, r);
-            const float2 rf2 = make_float2(rf, rf);
+            for (int d = 1; d <= nb; ++d) {
+              const int cb = w4 + dir * d;
+              tmem_ld32_sync(ts + cb * 32, r);
+              const float2 rf2 = make_float2(rf, rf);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float4 f = reinterpret_cast<const float4*>(beside)[j];
-              p[2 * j] = __fmul2_rn(pair_of(r[4 * j], r[4 * j + 1]), __fmul2_rn(rf2, make_float2(f.x, f.y)));
-              p[2 * j + 1] = __fmul2_rn(pair_of(r[4 * j + 2], r[4 * j + 3]), __fmul2_rn(rf2, make_float2(f.z, f.w)));
+              for (int j = 0; j < 8; ++j) {
+                const float4 f = reinterpret_cast<const float4*>(tab)[j];
+                p[2 * j] = __fmul2_rn(pair_of(r[4 * j], r[4 * j + 1]), __fmul2_rn(rf2, make_float2(f.x, f.y)));
+                p[2 * j + 1] = __fmul2_rn(pair_of(r[4 * j + 2], r[4 * j + 3]), __fmul2_rn(rf2, make_float2(f.z, f.w)));
+              }
+              if (x.rev && valid < 128) keep(tokens(cb));
+              put(cb);
+              rf *= l32;
             }
-            if (x.rev && valid < 128) keep(tokens(cb));
-            put(cb);
-            rf *= l32;
-          }
-          if (part == 1) {  // the other side of the diagonal is zero
-            uint32_t z[16];
+            uint32_t z[16];  // the other side of the diagonal is zero
 #pragma unroll
             for (int j = 0; j < 16; ++j) z[j] = 0;
 #pragma unroll 1
@@ -783,10 +787,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         if (more) load_first();
       }
     }
-  } else if (warp < 18) {
+  } else if (role == 1 || role == 2) {
     if constexpr (TMA) {
       // ------------------------------------------------------------ TMA loads
-      if (warp == 16 && elect_one()) {
+      if (role == 1 && elect_one()) {
         ChunkIter<DK, STATES> it;
         for (bool more = it.first(a, n_units); more; more = it.next(a)) {
           const int g = it.g, s = g % C::QKS, vs = g % C::VS;
@@ -805,7 +809,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       }
     } else {
       // ------------------------------------------------------------ fp32 k, a quarter of the tile at a time
-      const int t = threadIdx.x - 16 * 32;
+      const int t = (role - 1) * 32 + lane_id();
       using R = Rows<64>;
       constexpr int QUARTERS = R::VECS / 8;
       ChunkIter<DK, STATES> it;
@@ -839,7 +843,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         if (more) load(r0, 0);
       }
     }
-  } else if (warp == 18) {
+  } else if (role == 0) {
     // ------------------------------------------------------------ MMA issue
     if (elect_one()) {
       int total = 0;
@@ -925,7 +929,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 18) {
+  if (role == 0) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
