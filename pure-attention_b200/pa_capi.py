@@ -154,9 +154,20 @@ def _ptr(t):
     return t.data_ptr()
 
 
+_torch = None
+
+
 def _stream():
-    import torch
-    return torch.cuda.current_stream().cuda_stream
+    """The current CUDA stream's handle (the raw getter where torch has it: a Stream object
+    costs 3 us more, as much as a launch)."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
+    if raw is None:
+        return _torch.cuda.current_stream().cuda_stream
+    return raw(_torch.cuda.current_device())
 
 
 F32_MATH = {"split3": 0, "bf16": 1}
@@ -267,21 +278,21 @@ def attn_delta(dO, o, delta, desc=None, stream=None):
 def _check_tensors(fn, dev, dtype, shape, names, *tensors):
     """Each tensor (None: skipped) has this type and shape, is contiguous and on CUDA device `dev`:
     a call with any other would read past its memory."""
-    for name, t in zip(names, tensors):
-        if t is None:
-            continue
-        if t.dtype is not dtype or t.shape != shape:
-            raise ValueError(f"{fn}: {name} must be {dtype} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
-        if not t.is_contiguous():
-            raise ValueError(f"{fn}: {name} must be contiguous")
-        if t.get_device() != dev:
+    for t in tensors:
+        if t is not None and (t.dtype is not dtype or t.shape != shape or not t.is_contiguous()
+                              or t.get_device() != dev):
+            name = names[[t is x for x in tensors].index(True)]
+            if t.dtype is not dtype or t.shape != shape:
+                raise ValueError(f"{fn}: {name} must be {dtype} {tuple(shape)}, not {t.dtype} {tuple(t.shape)}")
+            if not t.is_contiguous():
+                raise ValueError(f"{fn}: {name} must be contiguous")
             raise ValueError(f"{fn}: {name} must be on the first tensor's device, not {t.device}")
 
 
-def _check_device(fn, t):
+def _check_device(fn, t, dev):
     """The kernels run on the current device's stream."""
     import torch
-    if t.get_device() < 0 or t.get_device() != torch.cuda.current_device():
+    if dev < 0 or dev != torch.cuda.current_device():
         raise ValueError(f"{fn}: tensors must be on the current CUDA device, not {t.device}")
 
 
@@ -310,7 +321,7 @@ def _rope(name, q, k, positions, q_out, k_out, desc, *accumulate, stream=None):
     _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_heads, d.head_dim), ("q", "q_out"), q, q_out)
     _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_kv_heads, d.head_dim), ("k", "k_out"), k, k_out)
     _check_tensors(name, dev, torch.int32, (d.axes, d.batch, d.seq_len), ("positions",), positions)
-    _check_device(name, q)
+    _check_device(name, q, dev)
     _check(name, getattr(load(), name)(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(positions), _ptr(q_out),
                                        _ptr(k_out), *accumulate, _stream() if stream is None else stream))
 
@@ -326,18 +337,22 @@ def rope_bwd(dq_out, dk_out, positions, dq, dk, desc, accumulate=False, stream=N
     _rope("pa_rope_bwd", dq_out, dk_out, positions, dq, dk, desc, int(bool(accumulate)), stream=stream)
 
 
+_STATES = {2: ("state_in", "state_out"), 3: ("state_in", "d_state_out", "d_state_in")}
+
+
 def _check_linear_attn(fn, q, log_decay, seq_lens, names, tensors, states):
     import torch
-    if q.dim() != 4:
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError(f"{fn}: q must be [B, L, H, D]")
-    B, L, H, D = q.shape
+    B, _, H, D = shape
     dev = q.get_device()
-    _check_tensors(fn, dev, q.dtype, q.shape, names, *tensors)
-    _check_tensors(fn, dev, torch.float32, (B, H, D, D),
-                   ("state_in", "state_out") if len(states) == 2 else ("state_in", "d_state_out", "d_state_in"), *states)
+    _check_tensors(fn, dev, q.dtype, shape, names, *tensors)
+    _check_tensors(fn, dev, torch.float32, (B, H, D, D), _STATES[len(states)], *states)
     _check_tensors(fn, dev, torch.float32, (H,), ("log_decay",), log_decay)
-    _check_tensors(fn, dev, torch.int32, (B,), ("seq_lens",), seq_lens)
-    _check_device(fn, q)
+    if seq_lens is not None:
+        _check_tensors(fn, dev, torch.int32, (B,), ("seq_lens",), seq_lens)
+    _check_device(fn, q, dev)
 
 
 def _linear_attn_ws(need, workspace, device):
