@@ -52,9 +52,9 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 //               and 32 columns of O each)
 //   warps 8-11  the state in fp32 registers (thread = row of the state), its bf16
 //               parts to shared memory for Q S
-//   warps 12-15 V' from V (fp32: and q, v through registers, split on the way)
-//   warps 16-19 tcgen05.mma issue (one warp); bf16: TMA loads of q, k, v (one thread);
-//               fp32: k through registers (two warps)
+//   warps 12-15 V' from V (fp32: and the splitting of q and v)
+//   warps 16-19 tcgen05.mma issue (one thread), TMA loads (one thread), the splitting of
+//               fp32 k (two warps)
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
@@ -68,22 +68,23 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 constexpr int kMixThreads = 20 * 32;
 constexpr int kTile = 128 * 128;  // bytes of 128 rows x 64 bf16
 
-template <int DK, int NT>
+template <typename T, int DK, int NT>
 struct MixCfg {
   static constexpr int NP = NT == 3 ? 2 : 1;       // planes (hi, lo) of q, k, v
   static constexpr int KT = DK / 64;               // 64-column tiles of q and k
-  static constexpr int OPER = NP * KT * kTile;     // bytes of q (or k) of a stage
+  // bytes of q (or k) of a stage; fp32 tiles land there whole before they are split
+  static constexpr int OPER = (sizeof(T) == 4 ? 2 : 1) * KT * kTile;
   static constexpr int V_STAGE = NP * kTile;       // v
   static constexpr int VP_BYTES = 2 * kTile;       // V' hi and lo
   static constexpr int ST_PLANE = DK * 128;        // [DK, 64] bf16
-  static constexpr bool SMALL = NP == 1 && DK == 64;
-  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 4 : (NP == 1 ? 2 : 1);
+  static constexpr bool SMALL = sizeof(T) == 2 && DK == 64;
+  static constexpr int QKS = SMALL ? 3 : 2, VS = SMALL ? 4 : (sizeof(T) == 2 ? 2 : 1);
   // V', state planes, and 2 KB a warp through which the output goes out
   static constexpr int SMEM = QKS * 2 * OPER + VS * V_STAGE + VP_BYTES + NP * ST_PLANE + kTile + 1024;
   static constexpr int NC = DK == 64 ? 32 : 64;    // state columns of a thread
 };
-static_assert(MixCfg<64, 1>::SMEM <= 225 * 1024 && MixCfg<64, 3>::SMEM <= 225 * 1024 &&
-              MixCfg<128, 1>::SMEM <= 225 * 1024, "shared memory of one CTA");
+static_assert(MixCfg<__nv_bfloat16, 64, 1>::SMEM <= 225 * 1024 && MixCfg<__nv_bfloat16, 128, 1>::SMEM <= 225 * 1024 &&
+              MixCfg<float, 64, 3>::SMEM <= 225 * 1024, "shared memory of one CTA");
 
 struct MixOne {  // one direction of the recurrence
   const void *q, *k, *v;
@@ -217,27 +218,37 @@ __device__ __forceinline__ void put4(uint32_t hi, uint32_t lo, uint32_t off, flo
                  : "memory");
 }
 
-// fp32 loads: the 64 columns of a chunk's rows, dealt to the N threads of a loading
-// group in 16-byte vectors: thread t has column vector t % 16 of rows t / 16 + i * N / 16.
+// An fp32 tile (128 rows x 64 values) as TMA leaves it: columns 0-31 as rows of 128 bytes
+// where the hi plane will be, 32-63 where the lo plane will be. Split in place it stays
+// within its rows: 16 lanes hold a row between reading and writing it. Thread t of N
+// has the 16-byte vectors t % 16 of rows t / 16 + i * N / 16.
 template <int N>
-struct Rows {
-  static constexpr int ROWS = N / 16;         // rows a pass
-  static constexpr int VECS = 128 / ROWS;     // vectors of a thread
-  const float* src;
-  long long step;
-  int row0, valid;  // valid = 0 past the head's columns
-  template <typename It>
-  __device__ __forceinline__ Rows(const MixArgs& a, const It& it, const void* base, int t) {
-    const int col = (t % 16) * 4;
-    row0 = t / 16;
-    valid = col < a.D ? it.valid() : 0;  // head dim 32 fills half a tile
-    const long long tok = static_cast<long long>(it.x.b) * a.L + it.x.token(it.chunk) + row0;
-    step = static_cast<long long>(a.H) * a.D * ROWS;
-    src = static_cast<const float*>(base) + (tok * a.H + it.x.h) * a.D + col;
+struct Split {
+  static constexpr int ROWS = N / 16, VECS = 128 / ROWS;
+  uint32_t at;  // of the tile
+  int row0, c;
+  __device__ __forceinline__ Split(uint32_t tile, int t) : at(tile), row0(t / 16), c(t % 16) {}
+  __device__ __forceinline__ int row(int i) const { return row0 + i * ROWS; }
+  // zero past the sequence, whatever is there
+  __device__ __forceinline__ float4 load(int i, int valid) const {
+    const uint4 v = ld_shared_v4(at + (c >> 3) * kTile + row(i) * 128 + (c & 7) * 16);
+    return row(i) < valid ? make_float4(__uint_as_float(v.x), __uint_as_float(v.y), __uint_as_float(v.z),
+                                        __uint_as_float(v.w))
+                          : make_float4(0.f, 0.f, 0.f, 0.f);
   }
-  __device__ __forceinline__ float4 load(int i) const {
-    return row0 + i * ROWS < valid ? __ldg(reinterpret_cast<const float4*>(src + i * step))
-                                   : make_float4(0.f, 0.f, 0.f, 0.f);
+  template <int NP>
+  __device__ __forceinline__ void store(uint32_t to, int i, float4 v) const {
+    put4(to, NP == 2 ? to + kTile : 0, sw128_offset(row(i), c * 8), make_float2(v.x, v.y), make_float2(v.z, v.w));
+  }
+  // vectors i0 .. i0 + 7 in place
+  template <int NP>
+  __device__ __forceinline__ void eight(int i0, int valid) const {
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = load(i0 + i, valid);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) store<NP>(at, i0 + i, v[i]);
   }
 };
 
@@ -282,11 +293,11 @@ struct Desc {
 template <typename T, int DK, int NT, bool STATES>
 __global__ void __launch_bounds__(kMixThreads, 1)
     mix_kernel(const __grid_constant__ MixArgs a, const __grid_constant__ MixMaps maps, uint32_t* status) {
-  using C = MixCfg<DK, NT>;
+  using C = MixCfg<T, DK, NT>;
   constexpr int NP = C::NP, KT = C::KT;
-  constexpr bool TMA = sizeof(T) == 2;
+  constexpr bool BF16 = sizeof(T) == 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[26];  // N_BARS
+  __shared__ uint64_t bars[29];  // N_BARS
   __shared__ __align__(16) float wtab[4 * 64 + 4 * 32];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -298,23 +309,25 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
   auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
   enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 10, S_FULL = 14, P_FULL = 16, VP_FULL = 18, VP_EMPTY,
-         ST_FULL, ST_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, N_BARS };
+         ST_FULL, ST_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, QK_RAW, V_RAW = QK_RAW + 2, N_BARS };
   constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
     for (int i = 0; i < 3; ++i) {
-      mbar_init(bar(QK_FULL + i), TMA ? 1 : (STATES ? 2 : 6));  // fp32: the loading warps
+      mbar_init(bar(QK_FULL + i), BF16 ? 1 : (STATES ? 2 : 6));  // fp32: the splitting warps
       mbar_init(bar(QK_EMPTY + i), 1);
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(bar(V_FULL + i), TMA ? 1 : 4);
+      mbar_init(bar(V_FULL + i), BF16 ? 1 : 4);
       mbar_init(bar(V_EMPTY + i), 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(bar(S_FULL + i), 1);
       mbar_init(bar(P_FULL + i), 8);
     }
+    for (int i = 0; i < 2; ++i) mbar_init(bar(QK_RAW + i), 1);
+    mbar_init(bar(V_RAW), 1);
     mbar_init(bar(VP_FULL), 4);
     mbar_init(bar(VP_EMPTY), 1);
     mbar_init(bar(ST_FULL), 4);
@@ -325,7 +338,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     mbar_init(bar(O_FREE), 8);
     fence_mbar_init();
   }
-  // Role of a warp of the last warpgroup: 0 MMA issue, 1 and 2 loads. The issuing warp slows the
+  // Role of a warp of the last warpgroup: 0 MMA issue, 1 loads, 2 and 3 splitting. The issuing warp slows the
   // other warps of its sub-partition (an MMA that waits for the queue holds up their TMEM
   // loads), so it sits with the 32 rows that have the fewest scores: the first forward in time,
   // the last backward.
@@ -335,7 +348,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     tmem_relinquish();
   }
   if (role == 3 && lane_id() == 0) abort_flag = aborted(status);
-  if (TMA && role == 1 && lane_id() < 3) {
+  if (role == 1 && lane_id() < 3) {
     const MixOne& one = a.one[mix_unit<DK, STATES>(a, blockIdx.x).dir];
     tma_prefetch_desc(&maps.m[lane_id() == 0 ? one.mk : (lane_id() == 1 ? one.mq : one.mv)]);
   }
@@ -665,7 +678,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       const float l2 = log2_decay(a.log_decay, it.x.h);
       return row < valid ? exp2f(l2 * static_cast<float>(it.x.rev ? row : valid - 1 - row)) : 0.f;
     };
-    if constexpr (TMA) {
+    if constexpr (BF16) {
       // Each thread has 16-byte column t % 8 of rows t / 8 + 16 i. A weight w is two bf16 parts;
       // hi = bf16(v w_hi), and since v w_hi has 16 bits, v w_hi - hi is a bf16 too:
       // lo = bf16(v w_lo + (v w_hi - hi)), off by 2^-17 of v w, in three packed instructions.
@@ -720,127 +733,87 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         warp_arrive(bar(VP_FULL));
       }
     } else {
-      // fp32: q, then v, half a tile in each register buffer
-      using R = Rows<128>;
-      constexpr int HALF = R::VECS / 2;
-      float4 r0[HALF], r1[HALF];
-      float w0[HALF], w1[HALF];
-      auto load_half = [&](float4 (&r)[HALF], const void* base, int half) {
-        const R rows(a, it, base, t);
-#pragma unroll
-        for (int i = 0; i < HALF; ++i) r[i] = rows.load(half * HALF + i);
-      };
-      auto row_of = [&](int half, int i) { return t / 16 + (half * HALF + i) * R::ROWS; };
-      auto put_half = [&](const float4 (&r)[HALF], uint32_t at, int half) {
-#pragma unroll
-        for (int i = 0; i < HALF; ++i)
-          put4(at, NP == 2 ? at + kTile : 0, sw128_offset(row_of(half, i), (t % 16) * 8), make_float2(r[i].x, r[i].y),
-               make_float2(r[i].z, r[i].w));
-      };
-      auto put_times = [&](const float4 (&r)[HALF], const float (&w)[HALF], uint32_t at, int half) {
-#pragma unroll
-        for (int i = 0; i < HALF; ++i)
-          put4(at, at + kTile, sw128_offset(row_of(half, i), (t % 16) * 8),
-               __fmul2_rn(make_float2(r[i].x, r[i].y), make_float2(w[i], w[i])),
-               __fmul2_rn(make_float2(r[i].z, r[i].w), make_float2(w[i], w[i])));
-      };
-      auto load_first = [&]() {
-        const MixOne& one = a.one[it.x.dir];
-        load_half(r0, STATES ? one.v : one.q, 0);
-        load_half(r1, STATES ? one.v : one.q, 1);
-      };
-      if (more) load_first();
-      while (more) {
-        const int g = it.g, vs = g % C::VS, valid = it.valid();
+      // fp32: split q in place, then v, which lands where its V' goes
+      using X = Split<128>;
+      float w[X::VECS];
+      for (; more; more = it.next(a)) {
+        const int g = it.g, s = g % C::QKS, valid = it.valid();
         if (it.u != w_unit || valid != w_valid) {
 #pragma unroll
-          for (int i = 0; i < HALF; ++i) {
-            w0[i] = weight(row_of(0, i), valid);
-            w1[i] = weight(row_of(1, i), valid);
-          }
+          for (int i = 0; i < X::VECS; ++i) w[i] = weight(t / 16 + i * X::ROWS, valid);
           w_unit = it.u;
           w_valid = valid;
         }
         if (!STATES) {
-          const int s = g % C::QKS;
-          if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
-          put_half(r0, sQ(s), 0);
-          put_half(r1, sQ(s), 1);
-          fence_proxy_async_smem();  // before the next loads: the fence would wait for them
+          if (!mbar_wait_warp(bar(QK_RAW + s), (g / C::QKS) & 1, status)) break;
+          const X q(sQ(s), t);
+#pragma unroll 1
+          for (int i = 0; i < X::VECS; i += 8) q.template eight<NP>(i, valid);
+          fence_proxy_async_smem();
           warp_arrive(bar(QK_FULL + s));
-          load_half(r0, a.one[it.x.dir].v, 0);
-          load_half(r1, a.one[it.x.dir].v, 1);
         }
-        if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
-        put_times(r0, w0, sVp, 0);
-        put_times(r1, w1, sVp, 1);
+        if (!mbar_wait_warp(bar(V_RAW), g & 1, status)) break;
+        const X v(sVp, t);
+        float4 r[X::VECS];
+#pragma unroll
+        for (int i = 0; i < X::VECS; ++i) r[i] = v.load(i, valid);
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < X::VECS; ++i)
+          v.template store<2>(sVp, i, make_float4(r[i].x * w[i], r[i].y * w[i], r[i].z * w[i], r[i].w * w[i]));
         fence_proxy_async_smem();
         warp_arrive(bar(VP_FULL));
         if (!STATES) {
-          if (g >= C::VS && !mbar_wait_warp(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
-          put_half(r0, sV(vs), 0);
-          put_half(r1, sV(vs), 1);
+          if (g > 0 && !mbar_wait_warp(bar(V_EMPTY), (g - 1) & 1, status)) break;
+#pragma unroll
+          for (int i = 0; i < X::VECS; ++i) v.template store<NP>(sV(0), i, r[i]);
           fence_proxy_async_smem();
-          warp_arrive(bar(V_FULL + vs));
+          warp_arrive(bar(V_FULL));
         }
-        more = it.next(a);
-        if (more) load_first();
       }
     }
-  } else if (role == 1 || role == 2) {
-    if constexpr (TMA) {
-      // ------------------------------------------------------------ TMA loads
-      if (role == 1 && elect_one()) {
-        ChunkIter<DK, STATES> it;
-        for (bool more = it.first(a, n_units); more; more = it.next(a)) {
-          const int g = it.g, s = g % C::QKS, vs = g % C::VS;
-          const MixOne& one = a.one[it.x.dir];
-          const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
-          if (g >= C::QKS && !mbar_wait(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
-          mbar_arrive_expect_tx(bar(QK_FULL + s), (STATES ? 1 : 2) * C::OPER);
-          for (int tile = 0; tile < KT; ++tile) {
-            tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], bar(QK_FULL + s), tile * 64, h, tok, b);
-            if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], bar(QK_FULL + s), tile * 64, h, tok, b);
-          }
+  } else if (role == 1) {
+    // ------------------------------------------------------------ TMA loads
+    if (elect_one()) {
+      ChunkIter<DK, STATES> it;
+      for (bool more = it.first(a, n_units); more; more = it.next(a)) {
+        const int g = it.g, s = g % C::QKS, vs = g % C::VS;
+        const MixOne& one = a.one[it.x.dir];
+        const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
+        const uint32_t qk = bar((BF16 ? QK_FULL : QK_RAW) + s);
+        if (g >= C::QKS && !mbar_wait(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+        mbar_arrive_expect_tx(qk, (STATES ? 1 : 2) * C::OPER);
+        constexpr int COLS = 128 / static_cast<int>(sizeof(T));  // 128 bytes a row
+#pragma unroll
+        for (int tile = 0; tile < C::OPER / kTile; ++tile) {
+          tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], qk, tile * COLS, h, tok, b);
+          if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], qk, tile * COLS, h, tok, b);
+        }
+        if (BF16) {
           if (g >= C::VS && !mbar_wait(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
-          mbar_arrive_expect_tx(bar(V_FULL + vs), C::V_STAGE);
+          mbar_arrive_expect_tx(bar(V_FULL + vs), kTile);
           tma_load_4d(sV(vs), &maps.m[one.mv], bar(V_FULL + vs), it.x.half * 64, h, tok, b);
+        } else {
+          if (g > 0 && !mbar_wait(bar(VP_EMPTY), (g - 1) & 1, status)) break;
+          mbar_arrive_expect_tx(bar(V_RAW), 2 * kTile);
+          tma_load_4d(sVp, &maps.m[one.mv], bar(V_RAW), 0, h, tok, b);
+          tma_load_4d(sVp + kTile, &maps.m[one.mv], bar(V_RAW), COLS, h, tok, b);
         }
       }
-    } else {
-      // ------------------------------------------------------------ fp32 k, a quarter of the tile at a time
-      const int t = (role - 1) * 32 + lane_id();
-      using R = Rows<64>;
-      constexpr int QUARTERS = R::VECS / 8;
+    }
+  } else if (role >= 2) {
+    // ------------------------------------------------------------ fp32: split k in place
+    if constexpr (!BF16) {
+      const int t = (role - 2) * 32 + lane_id();
       ChunkIter<DK, STATES> it;
-      bool more = it.first(a, n_units);
-      float4 r0[8], r1[8];
-      auto load = [&](float4 (&r)[8], int quarter) {
-        const R rows(a, it, a.one[it.x.dir].k, t);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) r[j] = rows.load(quarter * 8 + j);
-      };
-      auto put = [&](const float4 (&r)[8], uint32_t at, int quarter) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          put4(at, NP == 2 ? at + kTile : 0, sw128_offset(t / 16 + (quarter * 8 + j) * R::ROWS, (t % 16) * 8),
-               make_float2(r[j].x, r[j].y), make_float2(r[j].z, r[j].w));
-      };
-      if (more) load(r0, 0);
-      while (more) {
+      for (bool more = it.first(a, n_units); more; more = it.next(a)) {
         const int g = it.g, s = g % C::QKS;
-        if (g >= C::QKS && !mbar_wait_warp(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
+        if (!mbar_wait_warp(bar(QK_RAW + s), (g / C::QKS) & 1, status)) break;
+        const Split<64> k(sK(s), t);
 #pragma unroll 1
-        for (int quarter = 0; quarter < QUARTERS; quarter += 2) {
-          load(r1, quarter + 1);
-          put(r0, sK(s), quarter);
-          if (quarter + 2 < QUARTERS) load(r0, quarter + 2);
-          put(r1, sK(s), quarter + 1);
-        }
+        for (int i = 0; i < Split<64>::VECS; i += 8) k.template eight<NP>(i, it.valid());
         fence_proxy_async_smem();
         warp_arrive(bar(QK_FULL + s));
-        more = it.next(a);
-        if (more) load(r0, 0);
       }
     }
   } else if (role == 0) {
@@ -993,7 +966,7 @@ MixPlan mix_plan(const AttnShape& sh, int n_dir) {
   const int chunks = (sh.L + 127) / 128;
   const long long pairs = static_cast<long long>(sh.B) * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
   long long seg = device_sm_count() / pairs;
-  if (seg > chunks / 4) seg = chunks / 4;
+  if (seg > chunks / 8) seg = chunks / 8;
   if (seg < 1) seg = 1;
   const int seg_chunks = static_cast<int>((chunks + seg - 1) / seg);
   p.n_seg = (chunks + seg_chunks - 1) / seg_chunks;
@@ -1004,7 +977,7 @@ MixPlan mix_plan(const AttnShape& sh, int n_dir) {
 
 template <typename T, int DK, int NT>
 int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s) {
-  using C = MixCfg<DK, NT>;
+  using C = MixCfg<T, DK, NT>;
   static std::atomic<uint64_t> attr_s{0}, attr{0};
   const int sms = device_sm_count();
   if (a.n_seg > 1) {
@@ -1017,6 +990,17 @@ int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s)
   if (!ensure_smem_attr(mix_kernel<T, DK, NT, false>, C::SMEM, attr)) return PA_ERR_LAUNCH;
   mix_kernel<T, DK, NT, false><<<a.n_units < sms ? a.n_units : sms, kMixThreads, C::SMEM, s>>>(a, maps, status);
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
+// An input [B, L, H, D] as boxes of 128 bytes of columns x 1 head x 128 tokens, bf16 in
+// the MMA operands' swizzle.
+bool make_in_map(CUtensorMap* m, const void* base, const AttnShape& sh, bool f32) {
+  if (!f32) return make_qkv_map(m, base, sh, 128);
+  const uint64_t D = sh.D, H = sh.H, L = sh.L;
+  const uint64_t dims[4] = {D, H, L, static_cast<uint64_t>(sh.B)};
+  const uint64_t strides[3] = {D * 4, H * D * 4, L * H * D * 4};
+  const uint32_t box[4] = {32, 1, 128, 1};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
 // An output [B, L, H, D] as boxes of 64 bytes of columns x 1 head x 32 tokens.
@@ -1048,9 +1032,6 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
     if (!make_out_map(&maps.o[d], a.one[d].o, sh, f32)) return PA_ERR_ALIGN;
     a.one[d].mo = d;
   }
-  if (f32)
-    return f32_math() == PA_F32_MATH_BF16 ? mix_launch<float, 64, 1>(a, maps, status, s)
-                                          : mix_launch<float, 64, 3>(a, maps, status, s);
   // tensor maps of the distinct inputs (at most q, k, v and dO)
   const void* seen[4];
   int n = 0;
@@ -1061,12 +1042,15 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
       int m = 0;
       while (m < n && seen[m] != in[j]) ++m;
       if (m == n) {
-        if (!make_qkv_map(&maps.m[n], in[j], sh, 128)) return PA_ERR_ALIGN;
+        if (!make_in_map(&maps.m[n], in[j], sh, f32)) return PA_ERR_ALIGN;
         seen[n++] = in[j];
       }
       *index[j] = m;
     }
   }
+  if (f32)
+    return f32_math() == PA_F32_MATH_BF16 ? mix_launch<float, 64, 1>(a, maps, status, s)
+                                          : mix_launch<float, 64, 3>(a, maps, status, s);
   return sh.D == 64 ? mix_launch<__nv_bfloat16, 64, 1>(a, maps, status, s)
                     : mix_launch<__nv_bfloat16, 128, 1>(a, maps, status, s);
 }

@@ -4,9 +4,9 @@ quadratic form: forward, backward, carried states and the single-token step.
 Tolerances, per value, from the roundings of the kernels. `mag` is the same sum
 with every factor's magnitude, so an error of r in every factor moves a value by
 at most r * mag.
-  bf16 operands: the intermediate products rounded to bf16 (2^-8 of `mag`), the output's rounding
-      (2^-8 of the value); the carried states as two bf16 parts (2^-16) and fp32
-      sums (2^-20 for the lengths here) are inside the same 2^-8 mag: 2^-8 (|value| + 1.02 mag).
+  bf16 operands: each term of an output has one factor rounded to bf16 on the way, a score or
+      the state entering its chunk (2^-8 of `mag`), and the output's rounding (2^-8 of the
+      value); the states' own errors (next but one) are inside 2^-8 x 0.02: 2^-8 (|value| + 1.02 mag).
   fp32 operands (split products): an operand in two bf16 parts is off by 2^-16,
       the product drops the low parts' product, 2^-16: 3 x 2^-16 a product, two
       products in a row and two splits of the state: 12 x 2^-16 < 2^-12 of mag.
@@ -195,6 +195,33 @@ def test_gradients_against_differences():
         want = (grad.double() * d).sum()
         scale = grad.double().norm() * d.double().norm()
         assert abs(diff - want) <= 2.0 ** -12 * scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64])
+def test_bf16_math_of_fp32_tensors(D):
+    """set_f32_math("bf16"): as bf16 operands (v times its decay and the states excepted, which keep
+    two parts), so against inputs rounded to bf16 the bf16 tolerance holds with an fp32 output."""
+    import pa_capi
+    q, k, v, dO, ld, s, ds = _inputs(3, 290, 2, D, torch.float32, 90, states=True)
+    q, k, v, dO = (x.bfloat16().float() for x in (q, k, v, dO))
+    lens = torch.tensor([290, 130, 7], dtype=torch.int32).cuda()
+    pa_capi.set_f32_math("bf16")
+    try:
+        o, so = _forward(q, k, v, ld, seq_lens=lens, state_in=s)
+        g = [torch.empty_like(q) for _ in range(3)]
+        dsi = torch.empty_like(s)
+        pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, seq_lens=lens, state_in=s, d_state_out=ds, d_state_in=dsi)
+    finally:
+        pa_capi.set_f32_math("split3")
+    want, ws = mix(q, k, v, ld, lens, s)
+    mag, ms = mix(q, k, v, ld, lens, s, absolute=True)
+    _close(o, want, mag, 2.0 ** -8, 2.0 ** -24)
+    _close(so, ws, ms, 2.0 ** -15, 2.0 ** -24)
+    wg, mg = mix_grads(q, k, v, ld, dO, lens, s, ds), mix_grads_absolute(q, k, v, ld, dO, lens, s, ds)
+    for got, w, m in zip(g, wg, mg):
+        _close(got, w, m, 2.0 ** -8, 2.0 ** -24)
+    _close(dsi, wg[3], mg[3], 2.0 ** -15, 2.0 ** -24)
 
 
 @pytest.mark.gpu
