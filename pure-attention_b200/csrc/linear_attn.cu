@@ -103,6 +103,7 @@ struct MixArgs {
   float* ws;  // segment states, see seg_slot
   int B, L, H, D;
   int n_seg, seg_tokens, n_units;
+  int fine, state_tokens, n_slots;  // segment states: `fine` pieces a segment, their tokens; see seg_slot
   float scale;
 };
 struct MixMaps {
@@ -131,7 +132,8 @@ struct MixUnit {
 
 // unit -> (segment, sequence, head, direction, column half), halves and
 // directions of one head next to one another: they read the same rows, from L2.
-// Segment states are wanted of all but the segment that comes last in time order.
+// Segment states are wanted of all but the segment that comes last in time order; there
+// x.seg counts pieces.
 template <int DK, bool STATES>
 __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
   MixUnit x;
@@ -144,23 +146,24 @@ __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
   u /= a.H;
   x.b = u % a.B;
   x.rev = a.one[x.dir].dir.reverse;
-  x.seg = u / a.B + (STATES && x.rev ? 1 : 0);
+  x.seg = u / a.B + (STATES && x.rev ? a.fine : 0);
   x.n = valid_tokens(a.lens, x.b, a.L);
-  x.p0 = x.seg * a.seg_tokens;
+  const int tokens = STATES ? a.state_tokens : a.seg_tokens;
+  x.p0 = x.seg * tokens;
   const int left = x.n - x.p0;
-  x.count = left < 0 ? 0 : (left < a.seg_tokens ? left : a.seg_tokens);
+  x.count = left < 0 ? 0 : (left < tokens ? left : tokens);
   x.chunks = (x.count + 127) >> 7;
   return x;
 }
 
 // Workspace of a sequence cut in segments: per (sequence, head, direction, half)
-// n_seg slots of [DK, 64] fp32. The first n_seg - 1 hold the states of single
-// segments (from zero), the last a copy of the carried state (state_out may
-// overwrite state_in while other segments still need it).
+// n_slots = (n_seg - 1) * fine + 1 slots of [DK, 64] fp32. The last holds a copy of the
+// carried state (state_out may overwrite state_in while other segments still need
+// it), the others the states of single pieces of segments (from zero).
 template <int DK>
 __device__ __forceinline__ float* seg_slot(const MixArgs& a, const MixUnit& x, int slot) {
   const size_t w = ((static_cast<size_t>(x.b) * a.H + x.h) * a.n_dir + x.dir) * (DK / 64) + x.half;
-  return a.ws + (w * a.n_seg + slot) * (DK * 64);
+  return a.ws + (w * a.n_slots + slot) * (DK * 64);
 }
 
 // The chunks of this CTA in order.
@@ -564,7 +567,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         for (int c = 0; c < NC / 4; ++c)
           dst[c * 128 + r] = make_float4(S[2 * c].x, S[2 * c].y, S[2 * c + 1].x, S[2 * c + 1].y);
       };
-      const bool carried = a.n_seg == 1 || (STATES && x.seg == (x.rev ? 1 : 0));
+      const bool carried = a.n_seg == 1 || (STATES && x.seg == (x.rev ? a.fine : 0));
 #pragma unroll
       for (int c = 0; c < NC / 2; ++c) S[c] = make_float2(0.f, 0.f);
       if (carried && one.s_in && in_state) {
@@ -575,7 +578,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       }
       const int last = x.n > 0 ? (x.n - 1) / a.seg_tokens : 0;  // the segment of the last token
       if (STATES) {
-        if (carried) save(a.n_seg - 1);
+        if (carried) save(a.n_slots - 1);
 #pragma unroll
         for (int c = 0; c < NC / 2; ++c) S[c] = make_float2(0.f, 0.f);
       } else if (a.n_seg > 1) {
@@ -592,12 +595,12 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         };
         const int end = x.p0 + a.seg_tokens;
         const int before = x.rev ? (x.n > end ? x.n - end : 0) : x.p0;  // tokens before this segment
-        add(a.n_seg - 1, before > 0 ? before - one.dir.lead : 0);
+        add(a.n_slots - 1, before > 0 ? before - one.dir.lead : 0);
         if (x.count > 0) {
           if (x.rev)
-            for (int f = x.seg + 1; f <= last; ++f) add(f - 1, (f - x.seg - 1) * a.seg_tokens);
+            for (int f = (x.seg + 1) * a.fine; f * a.state_tokens < x.n; ++f) add(f - a.fine, f * a.state_tokens - end);
           else
-            for (int f = 0; f < x.seg; ++f) add(f, (x.seg - f - 1) * a.seg_tokens);
+            for (int f = 0; f < x.seg * a.fine; ++f) add(f, x.p0 - (f + 1) * a.state_tokens);
         }
       }
       // the state's bf16 parts for chunk gg's Q S
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       }
       if (!ok) break;
       if (STATES) {
-        save(x.rev ? x.seg - 1 : x.seg);
+        save(x.rev ? x.seg - a.fine : x.seg);
         continue;
       }
       // the state after the last token in time order
@@ -908,49 +911,52 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   }
 }
 
-// One new token: a block per (sequence, head); each warp takes rows of the
-// state, lanes take 16 bytes of columns.
+// One new token. A block takes 32 columns of a state (sequence, head): 8 lanes a row of
+// 128 bytes, 16 rows a pass, all passes' loads in flight at once. Bound by HBM: the
+// state is read once and written once.
+constexpr int kStepThreads = 128, kStepCols = 32;
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(kStepThreads)
     mix_step_kernel(const T* __restrict__ q, const T* __restrict__ k, const T* __restrict__ v,
                     const float* __restrict__ log_decay, const float* s_in, T* __restrict__ o, float* s_out,
                     int H, float scale) {
-  constexpr int CV = D / 4, RPI = 256 / CV, ROWS = D / RPI;  // vectors a row, rows a pass, passes
-  __shared__ float4 part[256];
-  const int bh = blockIdx.x, h = bh % H;
-  const int c = threadIdx.x % CV, r0 = threadIdx.x / CV;
-  const size_t st0 = static_cast<size_t>(bh) * D * D, at = static_cast<size_t>(bh) * D;
-  float4 s[ROWS];
+  constexpr int BLOCKS = D / kStepCols, ROWS = kStepThreads / 8, PASSES = D / ROWS;
+  __shared__ float part[ROWS][kStepCols];
+  const int bh = blockIdx.x / BLOCKS, col = (blockIdx.x % BLOCKS) * kStepCols + (threadIdx.x % 8) * 4;
+  const int r0 = threadIdx.x / 8;
+  const size_t st0 = static_cast<size_t>(bh) * D * D + col, at = static_cast<size_t>(bh) * D;
+  float4 s[PASSES];
+  float kd[PASSES], qd[PASSES], ve[4];
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i)
-    s[i] = reinterpret_cast<const float4*>(s_in + st0)[(r0 + i * RPI) * CV + c];
-  const float lam = exp2f(log2_decay(log_decay, h));
-  float ve[4];
+  for (int i = 0; i < PASSES; ++i) s[i] = *reinterpret_cast<const float4*>(s_in + st0 + (r0 + i * ROWS) * D);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) ve[j] = ld_f(v + at + 4 * c + j);
+  for (int i = 0; i < PASSES; ++i) {
+    kd[i] = ld_f(k + at + r0 + i * ROWS);
+    qd[i] = ld_f(q + at + r0 + i * ROWS);
+  }
+#pragma unroll
+  for (int j = 0; j < 4; ++j) ve[j] = ld_f(v + at + col + j);
+  const float lam = exp2f(log2_decay(log_decay, bh % H));
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    const int d = r0 + i * RPI;
-    const float kd = ld_f(k + at + d), qd = ld_f(q + at + d);
-    s[i].x = fmaf(lam, s[i].x, kd * ve[0]);
-    s[i].y = fmaf(lam, s[i].y, kd * ve[1]);
-    s[i].z = fmaf(lam, s[i].z, kd * ve[2]);
-    s[i].w = fmaf(lam, s[i].w, kd * ve[3]);
-    reinterpret_cast<float4*>(s_out + st0)[d * CV + c] = s[i];
-    acc.x = fmaf(qd, s[i].x, acc.x);
-    acc.y = fmaf(qd, s[i].y, acc.y);
-    acc.z = fmaf(qd, s[i].z, acc.z);
-    acc.w = fmaf(qd, s[i].w, acc.w);
+  for (int i = 0; i < PASSES; ++i) {
+    s[i].x = fmaf(lam, s[i].x, kd[i] * ve[0]);
+    s[i].y = fmaf(lam, s[i].y, kd[i] * ve[1]);
+    s[i].z = fmaf(lam, s[i].z, kd[i] * ve[2]);
+    s[i].w = fmaf(lam, s[i].w, kd[i] * ve[3]);
+    *reinterpret_cast<float4*>(s_out + st0 + (r0 + i * ROWS) * D) = s[i];
+    acc.x = fmaf(qd[i], s[i].x, acc.x);
+    acc.y = fmaf(qd[i], s[i].y, acc.y);
+    acc.z = fmaf(qd[i], s[i].z, acc.z);
+    acc.w = fmaf(qd[i], s[i].w, acc.w);
   }
-  part[threadIdx.x] = acc;
+  *reinterpret_cast<float4*>(&part[r0][(threadIdx.x % 8) * 4]) = acc;
   __syncthreads();
-  if (threadIdx.x < D) {  // fixed order: the same bits every time
-    const float* p = reinterpret_cast<const float*>(part);
+  if (threadIdx.x < kStepCols) {  // fixed order: the same bits every time
     float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < RPI; ++i) sum += p[i * D + threadIdx.x];
-    st_f(o + at + threadIdx.x, scale * sum);
+    for (int i = 0; i < ROWS; ++i) sum += part[i][threadIdx.x];
+    st_f(o + at + (blockIdx.x % BLOCKS) * kStepCols + threadIdx.x, scale * sum);
   }
 }
 
@@ -959,19 +965,29 @@ __global__ void __launch_bounds__(256)
 // segments' own states are computed first (k and v are read a second time) and
 // each segment starts from their sum.
 struct MixPlan {
-  int n_seg, seg_tokens, units;
+  int pairs;             // units of a segment: (sequence, head, direction, column half)
+  int n_seg, seg_tokens;
+  int fine;              // pieces of a segment whose states are computed on their own
+  int n_slots;
 };
 MixPlan mix_plan(const AttnShape& sh, int n_dir) {
   MixPlan p;
-  const int chunks = (sh.L + 127) / 128;
-  const long long pairs = static_cast<long long>(sh.B) * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
-  long long seg = device_sm_count() / pairs;
+  const int chunks = (sh.L + 127) / 128, sms = device_sm_count();
+  p.pairs = sh.B * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
+  // segments for the SMs there are, of 8 chunks at least: below that the second launch and the
+  // second reading of k and v cost more than they bring
+  int seg = sms / p.pairs;
   if (seg > chunks / 8) seg = chunks / 8;
   if (seg < 1) seg = 1;
-  const int seg_chunks = static_cast<int>((chunks + seg - 1) / seg);
+  int seg_chunks = (chunks + seg - 1) / seg;
+  // the states' launch has one segment less: cut finer it still fills the GPU
+  p.fine = seg > 1 ? sms / (p.pairs * (seg - 1)) : 1;
+  if (p.fine > seg_chunks / 4) p.fine = seg_chunks / 4;
+  if (p.fine < 1) p.fine = 1;
+  seg_chunks = (seg_chunks + p.fine - 1) / p.fine * p.fine;
   p.n_seg = (chunks + seg_chunks - 1) / seg_chunks;
   p.seg_tokens = seg_chunks * 128;
-  p.units = static_cast<int>(pairs) * p.n_seg;
+  p.n_slots = (p.n_seg - 1) * p.fine + 1;
   return p;
 }
 
@@ -983,7 +999,7 @@ int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s)
   if (a.n_seg > 1) {
     if (!ensure_smem_attr(mix_kernel<T, DK, NT, true>, C::SMEM, attr_s)) return PA_ERR_LAUNCH;
     MixArgs f = a;
-    f.n_units = a.n_units / a.n_seg * (a.n_seg - 1);
+    f.n_units = a.n_units / a.n_seg * (a.n_slots - 1);
     mix_kernel<T, DK, NT, true><<<f.n_units < sms ? f.n_units : sms, kMixThreads, C::SMEM, s>>>(f, maps, status);
     if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
   }
@@ -1025,7 +1041,10 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
   a.D = sh.D;
   a.n_seg = p.n_seg;
   a.seg_tokens = p.seg_tokens;
-  a.n_units = p.units;
+  a.n_units = p.pairs * p.n_seg;
+  a.fine = p.fine;
+  a.state_tokens = p.seg_tokens / p.fine;
+  a.n_slots = p.n_slots;
   a.scale = sh.scale;
   MixMaps maps{};
   for (int d = 0; d < a.n_dir; ++d) {
@@ -1058,7 +1077,7 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
 template <typename T, int D>
 int step(const AttnShape& sh, const void* q, const void* k, const void* v, const float* log_decay,
          const float* s_in, void* o, float* s_out, cudaStream_t s) {
-  mix_step_kernel<T, D><<<sh.B * sh.H, 256, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
+  mix_step_kernel<T, D><<<sh.B * sh.H * (D / kStepCols), kStepThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
                                                     static_cast<const T*>(v), log_decay, s_in,
                                                     static_cast<T*>(o), s_out, sh.H, sh.scale);
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
@@ -1068,7 +1087,7 @@ int step(const AttnShape& sh, const void* q, const void* k, const void* v, const
 
 size_t linear_attn_workspace_bytes(const AttnShape& sh, bool, bool backward) {
   const MixPlan p = mix_plan(sh, backward ? 3 : 1);
-  return p.n_seg == 1 ? 0 : static_cast<size_t>(p.units) * (sh.D == 128 ? 128 : 64) * 64 * sizeof(float);
+  return p.n_seg == 1 ? 0 : static_cast<size_t>(p.pairs) * p.n_slots * (sh.D == 128 ? 128 : 64) * 64 * sizeof(float);
 }
 
 int launch_linear_attn_fwd(const AttnShape& sh, bool f32, const void* q, const void* k, const void* v,

@@ -33,9 +33,29 @@ struct RopeTable {
 
 // V values as V * sizeof(T) bytes (16 for the vector paths).
 template <typename T, int V>
-struct alignas(sizeof(T) * V) Pack {
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
   T v[V];
 };
+
+// Values 2 j and 2 j + 1 of a vector (bf16 as one 32-bit word: unpacked and packed two at a time).
+template <int V>
+__device__ __forceinline__ float2 two_of(const Pack<float, V>& x, int j) {
+  return make_float2(x.v[2 * j], x.v[2 * j + 1]);
+}
+template <int V>
+__device__ __forceinline__ float2 two_of(const Pack<__nv_bfloat16, V>& x, int j) {
+  const uint32_t w = reinterpret_cast<const uint32_t*>(&x)[j];
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+template <int V>
+__device__ __forceinline__ void set_two(Pack<float, V>& x, int j, float2 y) {
+  x.v[2 * j] = y.x;
+  x.v[2 * j + 1] = y.y;
+}
+template <int V>
+__device__ __forceinline__ void set_two(Pack<__nv_bfloat16, V>& x, int j, float2 y) {
+  reinterpret_cast<uint32_t*>(&x)[j] = pack_bf16x2(y.x, y.y);
+}
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -46,106 +66,133 @@ __device__ __forceinline__ float from_f<float>(float x) { return x; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-// One tile of `tokens` tokens per block. V: values per load; the scalar form
-// (V = 1) takes head sizes and sections whose runs are not whole 16-byte
-// vectors. ACC: y += turn(x) (gradients added to what y holds).
+// How a block's threads share its tokens: thread = (token t of T, head slot of G, vector c
+// of a head). A head slot takes heads slot, slot + G, ... of q and then k, so a thread's
+// vector and cosines stay the same from head to head.
+struct RopeSplit {
+  int T, G;
+};
+
+// V: values per load; the scalar form (V = 1) takes head sizes and sections whose runs are
+// not whole 16-byte vectors. ACC: y += turn(x) (gradients added to what y holds).
+//
+// A vector is two runs of V values that turn together (halves: values i and P + i on),
+// or W values of pairs side by side, or V values that pass through. Each thread loads
+// the vectors of kRopeUnroll heads before it works on the first.
+constexpr int kRopeUnroll = 4;
 template <typename T, int V, bool HALVES, bool ACC>
 __global__ void __launch_bounds__(kRopeThreads)
     rope_kernel(const T* __restrict__ q, const T* __restrict__ k, T* qo, T* ko,
                 const int32_t* __restrict__ pos, const __grid_constant__ RopeTable tab, int P, int D,
-                int Hq, int Hk, long long n_tok, int tokens, float sign) {
-  extern __shared__ float2 cs[];  // [tokens][P] (cos, sin)
-  const long long t0 = static_cast<long long>(blockIdx.x) * tokens;
-  const int nt = static_cast<int>(n_tok - t0 < tokens ? n_tok - t0 : tokens);
-  for (int i = threadIdx.x; i < nt * P; i += kRopeThreads) {
-    const int t = i / P, p = i - t * P;
-    const double u = static_cast<double>(pos[tab.axis[p] * n_tok + t0 + t]) * tab.turns[p];
-    float s, c;
-    sincospif(2.f * static_cast<float>(u - rint(u)), &s, &c);
-    cs[i] = make_float2(c, sign * s);
-  }
-  __syncthreads();
-  // Work items of one head: `run` pairs of vectors (halves) or vectors (pairs)
-  // to turn, then `tail` vectors to pass through.
-  constexpr int W = HALVES ? V : (V == 1 ? 2 : V);  // values a pairs-layout item covers
-  const int turn = HALVES ? P / V : 2 * P / W;
-  const int tail = (D - 2 * P) / V;
-  const int per_head = turn + tail, per_tok = (Hq + Hk) * per_head;
-  for (int it = threadIdx.x; it < nt * per_tok; it += kRopeThreads) {
-    const int t = it / per_tok, r = it - t * per_tok;
-    const int h = r / per_head, c = r - h * per_head;
-    const bool is_k = h >= Hq;
-    const size_t at = (is_k ? (static_cast<size_t>(t0 + t) * Hk + (h - Hq))
-                            : (static_cast<size_t>(t0 + t) * Hq + h)) * D;
-    const T* src = (is_k ? k : q) + at;
-    T* dst = (is_k ? ko : qo) + at;
-    const float2* w = cs + t * P;
-    if (c >= turn) {  // pass through
-      using PV = Pack<T, V>;
-      const int e = 2 * P + (c - turn) * V;
-      PV x = *reinterpret_cast<const PV*>(src + e);
-      if (ACC) {
-        const PV o = *reinterpret_cast<const PV*>(dst + e);
+                int Hq, int Hk, long long n_tok, const RopeSplit split, float sign) {
+  // 2 x (cos [T][P], sin [T][P]): one sync a tile; apart, so that the lanes of a head read
+  // whole 16-byte vectors from different banks
+  extern __shared__ __align__(16) float tables[];
+  constexpr int W = V == 1 ? 2 : V;       // values of a pairs vector
+  constexpr bool TWO = HALVES || V == 1;  // a turning vector has a second run
+  constexpr int N = TWO ? V : V / 2;      // angles of a vector
+  using PV = Pack<T, V>;
+  using PN = Pack<float, N>;
+  const int n_turn = HALVES ? P / V : 2 * P / W, per_head = n_turn + (D - 2 * P) / V;
+  const int c = threadIdx.x % per_head, slot = threadIdx.x / per_head % split.G;
+  const int t = threadIdx.x / (per_head * split.G);
+  const bool works = t < split.T, turns = c < n_turn;
+  const int e = turns ? c * (HALVES ? V : W) : 2 * P + (c - n_turn) * V, second = HALVES ? P : 1;
+  const int angle = t * P + (HALVES ? e : e / 2);
+  // A thread's first entry of the table has the same pair in every tile: lanes that index the
+  // parameter differently are served one by one, so it is read once.
+  const int my_t = threadIdx.x / P, my_p = threadIdx.x - my_t * P;
+  const double my_turns = tab.turns[my_p];
+  const int32_t* my_pos = pos + tab.axis[my_p] * n_tok;
+  const long long n_tiles = (n_tok + split.T - 1) / split.T;
+#pragma unroll 1
+  for (long long tile = blockIdx.x; tile < n_tiles; tile += gridDim.x) {
+    float *cosines = tables + ((tile / gridDim.x) & 1) * 2 * split.T * P, *sines = cosines + split.T * P;
+    const long long t0 = tile * split.T, tok = t0 + t;
+    const bool live = works && tok < n_tok;
+    PN cv, sv;
+#pragma unroll 1
+    for (int h0 = slot; h0 - slot < Hq + Hk; h0 += kRopeUnroll * split.G) {
+      PV a[kRopeUnroll], b[kRopeUnroll], oa[kRopeUnroll], ob[kRopeUnroll];
+      T* dst[kRopeUnroll];
 #pragma unroll
-        for (int i = 0; i < V; ++i) x.v[i] = from_f<T>(to_f(o.v[i]) + to_f(x.v[i]));
-      }
-      *reinterpret_cast<PV*>(dst + e) = x;
-    } else if (HALVES) {
-      using PV = Pack<T, V>;
-      const int e = c * V;
-      PV a = *reinterpret_cast<const PV*>(src + e), b = *reinterpret_cast<const PV*>(src + P + e);
-      PV oa, ob;
-      if (ACC) {
-        oa = *reinterpret_cast<const PV*>(dst + e);
-        ob = *reinterpret_cast<const PV*>(dst + P + e);
-      }
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const float2 m = w[e + i];
-        const float fa = to_f(a.v[i]), fb = to_f(b.v[i]);
-        float ya = fa * m.x - fb * m.y, yb = fb * m.x + fa * m.y;
-        if (ACC) {
-          ya += to_f(oa.v[i]);
-          yb += to_f(ob.v[i]);
+      for (int n = 0; n < kRopeUnroll; ++n) {
+        const int h = h0 + n * split.G;
+        const bool is_k = h >= Hq;
+        const size_t at = (is_k ? static_cast<size_t>(tok) * Hk + (h - Hq) : static_cast<size_t>(tok) * Hq + h) * D + e;
+        dst[n] = live && h < Hq + Hk ? (is_k ? ko : qo) + at : nullptr;
+        if (dst[n]) {
+          const T* src = (is_k ? k : q) + at;
+          a[n] = *reinterpret_cast<const PV*>(src);
+          if (TWO && turns) b[n] = *reinterpret_cast<const PV*>(src + second);
+          if (ACC) {
+            oa[n] = *reinterpret_cast<const PV*>(dst[n]);
+            if (TWO && turns) ob[n] = *reinterpret_cast<const PV*>(dst[n] + second);
+          }
         }
-        a.v[i] = from_f<T>(ya);
-        b.v[i] = from_f<T>(yb);
       }
-      *reinterpret_cast<PV*>(dst + e) = a;
-      *reinterpret_cast<PV*>(dst + P + e) = b;
-    } else {
-      using PW = Pack<T, W>;
-      const int e = c * W;
-      PW x;
-      PW o;
-      if constexpr (V == 1) {  // a pair need not be aligned to its size
-        x.v[0] = src[e];
-        x.v[1] = src[e + 1];
-        if (ACC) {
-          o.v[0] = dst[e];
-          o.v[1] = dst[e + 1];
+      if (h0 == slot) {  // the table, while the first loads are on their way
+        const int nt = static_cast<int>(n_tok - t0 < split.T ? n_tok - t0 : split.T);
+        auto entry = [&](int i, double u) {
+          float s, co;
+          sincospif(2.f * static_cast<float>(u - rint(u)), &s, &co);
+          cosines[i] = co;
+          sines[i] = sign * s;
+        };
+        if (my_t < nt) entry(threadIdx.x, static_cast<double>(my_pos[t0 + my_t]) * my_turns);
+        for (int i = threadIdx.x + kRopeThreads; i < nt * P; i += kRopeThreads) {
+          const int ti = i / P, p = i - ti * P;
+          if (p == my_p) entry(i, static_cast<double>(my_pos[t0 + ti]) * my_turns);
+          else entry(i, static_cast<double>(pos[tab.axis[p] * n_tok + t0 + ti]) * tab.turns[p]);
         }
-      } else {
-        x = *reinterpret_cast<const PW*>(src + e);
-        if (ACC) o = *reinterpret_cast<const PW*>(dst + e);
+        __syncthreads();
+        if (live && turns) {
+          cv = *reinterpret_cast<const PN*>(cosines + angle);
+          sv = *reinterpret_cast<const PN*>(sines + angle);
+        }
       }
 #pragma unroll
-      for (int i = 0; i < W / 2; ++i) {
-        const float2 m = w[e / 2 + i];
-        const float fa = to_f(x.v[2 * i]), fb = to_f(x.v[2 * i + 1]);
-        float ya = fa * m.x - fb * m.y, yb = fb * m.x + fa * m.y;
-        if (ACC) {
-          ya += to_f(o.v[2 * i]);
-          yb += to_f(o.v[2 * i + 1]);
+      for (int n = 0; n < kRopeUnroll; ++n) {
+        if (!dst[n]) continue;
+        if (turns) {
+          if constexpr (V == 1) {
+            const float fa = to_f(a[n].v[0]), fb = to_f(b[n].v[0]);
+            a[n].v[0] = from_f<T>(fa * cv.v[0] - fb * sv.v[0] + (ACC ? to_f(oa[n].v[0]) : 0.f));
+            b[n].v[0] = from_f<T>(fb * cv.v[0] + fa * sv.v[0] + (ACC ? to_f(ob[n].v[0]) : 0.f));
+          } else if constexpr (HALVES) {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+              const float2 fa = two_of(a[n], j), fb = two_of(b[n], j);
+              const float2 co = two_of(cv, j), si = two_of(sv, j);
+              float2 ya = __ffma2_rn(fb, make_float2(-si.x, -si.y), __fmul2_rn(fa, co));
+              float2 yb = __ffma2_rn(fa, si, __fmul2_rn(fb, co));
+              if (ACC) {
+                ya = __fadd2_rn(ya, two_of(oa[n], j));
+                yb = __fadd2_rn(yb, two_of(ob[n], j));
+              }
+              set_two(a[n], j, ya);
+              set_two(b[n], j, yb);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) {
+              const float2 f = two_of(a[n], j);
+              float2 y = __ffma2_rn(make_float2(f.y, f.x), make_float2(-sv.v[j], sv.v[j]),
+                                    __fmul2_rn(f, make_float2(cv.v[j], cv.v[j])));
+              if (ACC) y = __fadd2_rn(y, two_of(oa[n], j));
+              set_two(a[n], j, y);
+            }
+          }
+          if (TWO) *reinterpret_cast<PV*>(dst[n] + second) = b[n];
+        } else if (ACC) {
+          if constexpr (V == 1) {
+            a[n].v[0] = from_f<T>(to_f(oa[n].v[0]) + to_f(a[n].v[0]));
+          } else {
+#pragma unroll
+            for (int j = 0; j < V / 2; ++j) set_two(a[n], j, __fadd2_rn(two_of(oa[n], j), two_of(a[n], j)));
+          }
         }
-        x.v[2 * i] = from_f<T>(ya);
-        x.v[2 * i + 1] = from_f<T>(yb);
-      }
-      if constexpr (V == 1) {
-        dst[e] = x.v[0];
-        dst[e + 1] = x.v[1];
-      } else {
-        *reinterpret_cast<PW*>(dst + e) = x;
+        *reinterpret_cast<PV*>(dst[n]) = a[n];
       }
     }
   }
@@ -153,15 +200,27 @@ __global__ void __launch_bounds__(kRopeThreads)
 
 template <typename T, int V>
 void rope_launch(const RopeShape& sh, const void* q, const void* k, void* qo, void* ko,
-                 const int32_t* pos, const RopeTable& tab, long long n_tok, int tokens, bool inverse,
-                 bool accumulate, cudaStream_t s) {
-  const unsigned grid = static_cast<unsigned>((n_tok + tokens - 1) / tokens);
-  const size_t smem = static_cast<size_t>(tokens) * sh.pairs * sizeof(float2);
+                 const int32_t* pos, const RopeTable& tab, bool inverse, bool accumulate, cudaStream_t s) {
+  const int run = sh.halves ? V : (V == 1 ? 2 : V), heads = sh.Hq + sh.Hk;
+  const int per_head = (sh.halves ? sh.pairs : 2 * sh.pairs) / run + (sh.D - 2 * sh.pairs) / V;  // <= 256
+  const long long n_tok = static_cast<long long>(sh.B) * sh.L;
+  // Head slots so that a thread has kRopeUnroll heads (all its loads in flight at once), the rest of
+  // the block for tokens; with few tokens one token a block, so that more blocks share them.
+  RopeSplit split;
+  const int fit = kRopeThreads / per_head;
+  split.G = (heads + kRopeUnroll - 1) / kRopeUnroll;
+  if (split.G > fit) split.G = fit;
+  split.T = fit / split.G;
+  const long long spread = n_tok / device_sm_count();
+  if (split.T > spread) split.T = spread < 1 ? 1 : static_cast<int>(spread);
+  const long long tiles = (n_tok + split.T - 1) / split.T, blocks = 8ll * device_sm_count();
+  const unsigned grid = static_cast<unsigned>(tiles < blocks ? tiles : blocks);
+  const size_t smem = 4 * static_cast<size_t>(split.T) * sh.pairs * sizeof(float);
   const float sign = inverse ? -1.f : 1.f;
   auto go = [&](auto kernel) {
     kernel<<<grid, kRopeThreads, smem, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
                                             static_cast<T*>(qo), static_cast<T*>(ko), pos, tab,
-                                            sh.pairs, sh.D, sh.Hq, sh.Hk, n_tok, tokens, sign);
+                                            sh.pairs, sh.D, sh.Hq, sh.Hk, n_tok, split, sign);
   };
   if (sh.halves) {
     if (accumulate) go(rope_kernel<T, V, true, true>);
@@ -186,20 +245,15 @@ int launch_rope(const RopeShape& sh, const void* q, const void* k, void* qo, voi
       tab.turns[i] = turn * std::exp2(-f * log2_base);
       tab.axis[i] = static_cast<uint8_t>(a);
     }
-  const long long n_tok = static_cast<long long>(sh.B) * sh.L;
-  // Tokens per block: one while that leaves blocks for the whole GPU, up to 8
-  // (the table of 8 tokens x 128 pairs is 8 KB).
-  const long long want = n_tok / (8ll * device_sm_count());
-  const int tokens = want < 1 ? 1 : (want > 8 ? 8 : static_cast<int>(want));
   const int V = sh.f32 ? 4 : 8;
   // whole 16-byte vectors in every run that is turned or passed through
   const bool vec = sh.D % V == 0 && (sh.halves ? sh.pairs : 2 * sh.pairs) % V == 0;
   if (sh.f32) {
-    if (vec) rope_launch<float, 4>(sh, q, k, qo, ko, positions, tab, n_tok, tokens, inverse, accumulate, s);
-    else rope_launch<float, 1>(sh, q, k, qo, ko, positions, tab, n_tok, tokens, inverse, accumulate, s);
+    if (vec) rope_launch<float, 4>(sh, q, k, qo, ko, positions, tab, inverse, accumulate, s);
+    else rope_launch<float, 1>(sh, q, k, qo, ko, positions, tab, inverse, accumulate, s);
   } else {
-    if (vec) rope_launch<__nv_bfloat16, 8>(sh, q, k, qo, ko, positions, tab, n_tok, tokens, inverse, accumulate, s);
-    else rope_launch<__nv_bfloat16, 1>(sh, q, k, qo, ko, positions, tab, n_tok, tokens, inverse, accumulate, s);
+    if (vec) rope_launch<__nv_bfloat16, 8>(sh, q, k, qo, ko, positions, tab, inverse, accumulate, s);
+    else rope_launch<__nv_bfloat16, 1>(sh, q, k, qo, ko, positions, tab, inverse, accumulate, s);
   }
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }

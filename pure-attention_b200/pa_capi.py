@@ -154,20 +154,14 @@ def _ptr(t):
     return t.data_ptr()
 
 
-_torch = None
-
-
 def _stream():
     """The current CUDA stream's handle (the raw getter where torch has it: a Stream object
     costs 3 us more, as much as a launch)."""
-    global _torch
-    if _torch is None:
-        import torch
-        _torch = torch
-    raw = getattr(_torch._C, "_cuda_getCurrentRawStream", None)
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
     if raw is None:
-        return _torch.cuda.current_stream().cuda_stream
-    return raw(_torch.cuda.current_device())
+        return torch.cuda.current_stream().cuda_stream
+    return raw(torch.cuda.current_device())
 
 
 F32_MATH = {"split3": 0, "bf16": 1}
@@ -199,10 +193,11 @@ def _dtype_code(t):
 
 def attn_desc(q, num_heads=None, scale=0.0):
     """Descriptor for q of shape [B, L, H, D] (or [B, L, E] with num_heads)."""
-    if q.dim() == 4:
-        B, L, H, D = q.shape
+    shape = q.shape
+    if len(shape) == 4:
+        B, L, H, D = shape
     else:
-        B, L, E = q.shape
+        B, L, E = shape
         H = num_heads
         D = E // H
     return AttnDesc(B, L, H, D, _dtype_code(q), float(scale))
@@ -298,6 +293,7 @@ def _check_device(fn, t, dev):
 
 ROPE_LAYOUT = {"halves": 0, "pairs": 1}
 ROPE_FREQS = {"shared": 0, "per_axis": 1}
+_Sections = ctypes.c_int32 * 4
 
 
 def rope_desc(q, k=None, sections=None, base=10000.0, layout="halves", freqs="shared"):
@@ -305,25 +301,29 @@ def rope_desc(q, k=None, sections=None, base=10000.0, layout="halves", freqs="sh
     sections: pairs turned by each position axis (None: one axis over the whole head);
     layout: "halves" or "pairs"; freqs: "shared" or "per_axis" (include/pa_kernels.h)."""
     B, L, H, D = q.shape
-    sections = [D // 2] if sections is None else list(sections)
+    if sections is None:
+        sections = (D // 2,)
     if len(sections) > 4:
         raise ValueError("rope_desc: at most 4 position axes")
     return RopeDesc(B, L, H, 0 if k is None else k.shape[2], D, _dtype_code(q), ROPE_LAYOUT[layout],
-                    ROPE_FREQS[freqs], len(sections), (ctypes.c_int32 * 4)(*sections), float(base))
+                    ROPE_FREQS[freqs], len(sections), _Sections(*sections), base)
 
 
-def _rope(name, q, k, positions, q_out, k_out, desc, *accumulate, stream=None):
+def _rope(name, q, k, positions, q_out, k_out, d, *accumulate, stream=None):
     import torch
-    d = desc
-    t, dev = torch.float32 if d.dtype == PA_F32 else torch.bfloat16, q.get_device()
-    if (k is None) != (d.num_kv_heads == 0) or (k is None) != (k_out is None):
+    dtype, dev = torch.float32 if d.dtype == PA_F32 else torch.bfloat16, q.get_device()
+    B, L, Hk, D = d.batch, d.seq_len, d.num_kv_heads, d.head_dim
+    if (k is None) != (Hk == 0) or (k is None) != (k_out is None):
         raise ValueError(f"{name}: k and its output go with the descriptor's kv heads")
-    _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_heads, d.head_dim), ("q", "q_out"), q, q_out)
-    _check_tensors(name, dev, t, (d.batch, d.seq_len, d.num_kv_heads, d.head_dim), ("k", "k_out"), k, k_out)
-    _check_tensors(name, dev, torch.int32, (d.axes, d.batch, d.seq_len), ("positions",), positions)
+    _check_tensors(name, dev, dtype, (B, L, d.num_heads, D), ("q", "q_out"), q, q_out)
+    if k is not None:
+        _check_tensors(name, dev, dtype, (B, L, Hk, D), ("k", "k_out"), k, k_out)
+        k, k_out = k.data_ptr(), k_out.data_ptr()
+    _check_tensors(name, dev, torch.int32, (d.axes, B, L), ("positions",), positions)
     _check_device(name, q, dev)
-    _check(name, getattr(load(), name)(ctypes.byref(d), _ptr(q), _ptr(k), _ptr(positions), _ptr(q_out),
-                                       _ptr(k_out), *accumulate, _stream() if stream is None else stream))
+    _check(name, getattr(load(), name)(ctypes.byref(d), q.data_ptr(), k, positions.data_ptr(),
+                                       q_out.data_ptr(), k_out, *accumulate,
+                                       _stream() if stream is None else stream))
 
 
 def rope_fwd(q, k, positions, q_out, k_out, desc, stream=None):
@@ -340,11 +340,11 @@ def rope_bwd(dq_out, dk_out, positions, dq, dk, desc, accumulate=False, stream=N
 _STATES = {2: ("state_in", "state_out"), 3: ("state_in", "d_state_out", "d_state_in")}
 
 
-def _check_linear_attn(fn, q, log_decay, seq_lens, names, tensors, states):
+def _check_linear_attn(fn, d, q, log_decay, seq_lens, names, tensors, states):
     import torch
     shape = q.shape
-    if len(shape) != 4:
-        raise ValueError(f"{fn}: q must be [B, L, H, D]")
+    if shape != (d.batch, d.seq_len, d.num_heads, d.head_dim) or d.dtype != _dtype_code(q):
+        raise ValueError(f"{fn}: q must be [B, L, H, D] and the descriptor its own")
     B, _, H, D = shape
     dev = q.get_device()
     _check_tensors(fn, dev, q.dtype, shape, names, *tensors)
@@ -355,11 +355,21 @@ def _check_linear_attn(fn, q, log_decay, seq_lens, names, tensors, states):
     _check_device(fn, q, dev)
 
 
-def _linear_attn_ws(need, workspace, device):
-    if workspace is None and need:
+# Workspace sizes by shape: a query costs a short call as much as a check of its arguments.
+_linear_attn_sizes = {}
+
+
+def _linear_attn_ws(size_of, d, workspace, q):
+    if workspace is None:
+        key = (size_of, d.batch, d.seq_len, d.num_heads, d.head_dim, d.dtype, q.get_device())
+        need = _linear_attn_sizes.get(key)
+        if need is None:
+            need = _linear_attn_sizes[key] = size_of(d)
+        if need == 0:
+            return None, 0
         import torch
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-    return workspace, 0 if workspace is None else workspace.numel() * workspace.element_size()
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    return workspace, workspace.numel() * workspace.element_size()
 
 
 def linear_attn_fwd_workspace_size(desc):
@@ -372,12 +382,12 @@ def linear_attn_fwd(q, k, v, log_decay, o, seq_lens=None, state_in=None, state_o
     state_in to state_out ([B, H, D, D] fp32, either may be None) over seq_lens (int32 [B])
     tokens of each sequence. A workspace is allocated with torch unless given."""
     d = desc or attn_desc(q)
-    _check_linear_attn("linear_attn_fwd", q, log_decay, seq_lens, ("q", "k", "v", "o"), (q, k, v, o),
+    _check_linear_attn("linear_attn_fwd", d, q, log_decay, seq_lens, ("q", "k", "v", "o"), (q, k, v, o),
                        (state_in, state_out))
-    ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size(d), workspace, q.device)
+    ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size, d, workspace, q)
     _check("pa_linear_attn_fwd", load().pa_linear_attn_fwd(
-        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(seq_lens), _ptr(state_in),
-        _ptr(o), _ptr(state_out), _ptr(ws), nb, _stream() if stream is None else stream))
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(seq_lens),
+        _ptr(state_in), o.data_ptr(), _ptr(state_out), _ptr(ws), nb, _stream() if stream is None else stream))
 
 
 def linear_attn_bwd_workspace_size(desc):
@@ -390,12 +400,13 @@ def linear_attn_bwd(q, k, v, dO, log_decay, dq, dk, dv, seq_lens=None, state_in=
     """Gradients dq, dk, dv (overwritten, or added to) and d_state_in of linear_attn_fwd from dO
     and d_state_out (None: zero)."""
     d = desc or attn_desc(q)
-    _check_linear_attn("linear_attn_bwd", q, log_decay, seq_lens, ("q", "k", "v", "dO", "dq", "dk", "dv"),
+    _check_linear_attn("linear_attn_bwd", d, q, log_decay, seq_lens, ("q", "k", "v", "dO", "dq", "dk", "dv"),
                        (q, k, v, dO, dq, dk, dv), (state_in, d_state_out, d_state_in))
-    ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size(d), workspace, q.device)
+    ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size, d, workspace, q)
     _check("pa_linear_attn_bwd", load().pa_linear_attn_bwd(
-        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(dO), _ptr(log_decay), _ptr(seq_lens),
-        _ptr(state_in), _ptr(d_state_out), _ptr(dq), _ptr(dk), _ptr(dv), _ptr(d_state_in),
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), dO.data_ptr(), log_decay.data_ptr(),
+        _ptr(seq_lens), _ptr(state_in), _ptr(d_state_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        _ptr(d_state_in),
         int(bool(accumulate)), _ptr(ws), nb, _stream() if stream is None else stream))
 
 
@@ -403,11 +414,11 @@ def linear_attn_step(q, k, v, log_decay, state_in, o, state_out, desc=None, stre
     """One new token of each sequence (q, k, v, o [B, 1, H, D]): state_out = decay * state_in +
     k v^T, o = scale q state_out; state_out may be state_in."""
     d = desc or attn_desc(q)
-    _check_linear_attn("linear_attn_step", q, log_decay, None, ("q", "k", "v", "o"), (q, k, v, o),
+    _check_linear_attn("linear_attn_step", d, q, log_decay, None, ("q", "k", "v", "o"), (q, k, v, o),
                        (state_in, state_out))
     _check("pa_linear_attn_step", load().pa_linear_attn_step(
-        ctypes.byref(d), _ptr(q), _ptr(k), _ptr(v), _ptr(log_decay), _ptr(state_in), _ptr(o),
-        _ptr(state_out), _stream() if stream is None else stream))
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state_in.data_ptr(),
+        o.data_ptr(), state_out.data_ptr(), _stream() if stream is None else stream))
 
 
 def device_status(clear=True, stream=None):
