@@ -80,7 +80,7 @@ def build_kernels(force=False):
 
 
 HOST = os.path.join(HERE, "host")
-HOST_SOURCES = ["src/Tensor.cpp", "src/Autograd.cpp", "src/Functional.cpp", "src/Adam.cpp",
+HOST_SOURCES = ["src/Tensor.cpp", "src/Autograd.cpp", "src/Functional.cpp", "src/Sequence.cpp", "src/Adam.cpp",
                 "src/layers.cpp", "bindings.cpp"]
 
 

@@ -14,8 +14,10 @@
 #include "core/Adam.h"
 #include "core/Context.h"
 #include "core/Functional.h"
+#include "core/Sequence.h"
 #include "core/Tensor.h"
 #include "layers/LayerNorm.h"
+#include "layers/LinearAttention.h"
 #include "layers/Linear.h"
 #include "layers/MHA.h"
 #include "layers/Module.h"
@@ -36,6 +38,20 @@ class PyModule : public layers::Module {
     PYBIND11_OVERRIDE(std::vector<std::shared_ptr<Tensor>>, layers::Module, parameters, );
   }
 };
+
+static core::RopeSpec rope_spec(const std::vector<int32_t>& sections, double base,
+                                const std::string& layout, const std::string& freqs) {
+  core::RopeSpec s;
+  s.sections = sections;
+  s.base = base;
+  if (layout != "halves" && layout != "pairs")
+    throw std::invalid_argument("rotary layout must be 'halves' or 'pairs'");
+  if (freqs != "shared" && freqs != "per_axis")
+    throw std::invalid_argument("rotary freqs must be 'shared' or 'per_axis'");
+  s.layout = layout == "halves" ? PA_ROPE_HALVES : PA_ROPE_PAIRS;
+  s.freqs = freqs == "shared" ? PA_ROPE_SHARED : PA_ROPE_PER_AXIS;
+  return s;
+}
 
 PYBIND11_MODULE(PureAttention, m) {
   m.doc() = "Pure-Attention operator surface over sm_100a kernels";
@@ -133,6 +149,34 @@ PYBIND11_MODULE(PureAttention, m) {
                              const std::shared_ptr<Tensor>&>(&layers::MultiheadAttention::forward))
       .def("parameters", &layers::MultiheadAttention::parameters);
 
+  py::class_<core::IntTensor, std::shared_ptr<core::IntTensor>>(m, "IntTensor",
+      "32-bit whole numbers on the device (positions [axes, N, L], lengths [N])")
+      .def(py::init<std::vector<uint32_t>, std::vector<int32_t>>(), py::arg("shape"), py::arg("values"))
+      .def("shape", &core::IntTensor::get_shape);
+
+  py::class_<layers::LinearAttention, layers::Module, std::shared_ptr<layers::LinearAttention>>(
+      m, "LinearAttention")
+      .def(py::init([](uint32_t e, uint32_t h, const std::vector<float>& log_decay,
+                       const std::vector<int32_t>& sections, double base, const std::string& layout,
+                       const std::string& freqs) {
+             return std::make_shared<layers::LinearAttention>(e, h, log_decay,
+                                                              rope_spec(sections, base, layout, freqs));
+           }),
+           py::arg("embed_dim"), py::arg("num_heads"), py::arg("log_decay") = std::vector<float>{},
+           py::arg("sections") = std::vector<int32_t>{}, py::arg("base") = 10000.0,
+           py::arg("layout") = "halves", py::arg("freqs") = "shared",
+           "Causal linear attention with a decay per head between MultiheadAttention's projections; "
+           "sections: rotary position pairs per axis (empty: none). Not in the reference.")
+      .def("forward", py::overload_cast<const std::shared_ptr<Tensor>&>(&layers::LinearAttention::forward))
+      .def("forward",
+           py::overload_cast<const std::shared_ptr<Tensor>&, const std::shared_ptr<core::IntTensor>&,
+                             const std::shared_ptr<core::IntTensor>&>(&layers::LinearAttention::forward),
+           py::arg("input"), py::arg("positions"), py::arg("lengths") = nullptr)
+      .def("forward_state", &layers::LinearAttention::forward_state, py::arg("input"),
+           py::arg("positions") = nullptr, py::arg("lengths") = nullptr, py::arg("state") = nullptr,
+           "(output, state after the last token) of a piece of a longer sequence")
+      .def("parameters", &layers::LinearAttention::parameters);
+
   py::class_<layers::LayerNorm, layers::Module, std::shared_ptr<layers::LayerNorm>>(m, "LayerNorm")
       .def(py::init<uint32_t, float>(), py::arg("normalized_shape"), py::arg("epsilon") = 1e-5f)
       .def("forward", &layers::LayerNorm::forward)
@@ -191,6 +235,26 @@ PYBIND11_MODULE(PureAttention, m) {
     return o;
   }, "core::flash_attention: softmax(q k^T / sqrt(d)) v per head of [N, L, E] fp32 tensors, with "
      "its graph node", py::arg("q"), py::arg("k"), py::arg("v"), py::arg("num_heads"));
+  m.def("rope", [](const std::shared_ptr<Tensor>& q, const std::shared_ptr<Tensor>& k, int head_dim,
+                   const std::shared_ptr<core::IntTensor>& positions, const std::vector<int32_t>& sections,
+                   double base, const std::string& layout, const std::string& freqs) {
+    return core::rope(q, k, head_dim, rope_spec(sections, base, layout, freqs), positions,
+                      CudaContext::getStream());
+  }, "core::rope: rotary positions of q and k [N, L, E] by positions [axes, N, L], with their graph "
+     "node. Not in the reference.", py::arg("q"), py::arg("k"), py::arg("head_dim"), py::arg("positions"),
+        py::arg("sections"), py::arg("base") = 10000.0, py::arg("layout") = "halves",
+        py::arg("freqs") = "shared");
+  m.def("linear_attention", [](const std::shared_ptr<Tensor>& q, const std::shared_ptr<Tensor>& k,
+                               const std::shared_ptr<Tensor>& v, int num_heads,
+                               const std::shared_ptr<Tensor>& log_decay,
+                               const std::shared_ptr<core::IntTensor>& lengths,
+                               const std::shared_ptr<Tensor>& state, bool want_state) {
+    return core::linear_attention(q, k, v, num_heads, log_decay, lengths, state, want_state,
+                                  CudaContext::getStream());
+  }, "core::linear_attention: (causal linear attention with decay exp(log_decay[h]) of [N, L, E] fp32 "
+     "tensors, state after the last token or None), with their graph node. Not in the reference.",
+        py::arg("q"), py::arg("k"), py::arg("v"), py::arg("num_heads"), py::arg("log_decay"),
+        py::arg("lengths") = nullptr, py::arg("state") = nullptr, py::arg("want_state") = false);
   m.def("set_stream", [](uintptr_t handle) {
     CudaContext::setStream(reinterpret_cast<cudaStream_t>(handle));
   }, "Stream every operator, allocation and gradient of this module runs on from now on "

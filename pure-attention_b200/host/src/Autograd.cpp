@@ -10,26 +10,6 @@ namespace core {
 namespace {
 cudaStream_t stream() { return CudaContext::getStream(); }
 size_t rows_of(const Tensor& t) { return t.numel() / last_dim(t); }
-
-// The gradient that reached an output, or null when none did (the tensor has
-// expired, has no gradient, or nothing has written its gradient: zero).
-const float* grad_in(const std::shared_ptr<Tensor>& t) {
-  if (!t || !t->requires_grad() || t->gradient_unwritten()) return nullptr;
-  return t->get_gradient_ptr();
-}
-
-// t.grad += src (n floats), as a copy when nothing has written t.grad yet.
-void add_into(const Tensor& t, const float* src, size_t n, const char* what) {
-  bool unwritten = false;
-  float* dst = t.gradient_for_write(&unwritten);
-  if (unwritten) {
-    if (cudaMemcpyAsync(dst, src, n * sizeof(float), cudaMemcpyDeviceToDevice, stream()) !=
-        cudaSuccess)
-      throw std::runtime_error(std::string(what) + ": cudaMemcpyAsync failed");
-    return;
-  }
-  check_status(pa_grad_accumulate(src, dst, n, ps(stream())), what);
-}
 }  // namespace
 
 MatMulFunction::MatMulFunction(std::shared_ptr<Tensor> x, std::shared_ptr<Tensor> w,

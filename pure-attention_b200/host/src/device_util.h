@@ -66,6 +66,26 @@ inline std::shared_ptr<void> device_buffer(size_t bytes, cudaStream_t s, const c
   return std::shared_ptr<void>(p, [](void* q) { cudaFreeAsync(q, CudaContext::getStream()); });
 }
 
+// The gradient that reached an output, or null when none did (the tensor has
+// expired, has no gradient, or nothing has written its gradient: zero).
+inline const float* grad_in(const std::shared_ptr<Tensor>& t) {
+  if (!t || !t->requires_grad() || t->gradient_unwritten()) return nullptr;
+  return t->get_gradient_ptr();
+}
+
+// t.grad += src (n floats), as a copy when nothing has written t.grad yet.
+inline void add_into(const Tensor& t, const float* src, size_t n, const char* what) {
+  const cudaStream_t s = CudaContext::getStream();
+  bool unwritten = false;
+  float* dst = t.gradient_for_write(&unwritten);
+  if (unwritten) {
+    if (cudaMemcpyAsync(dst, src, n * sizeof(float), cudaMemcpyDeviceToDevice, s) != cudaSuccess)
+      throw std::runtime_error(std::string(what) + ": cudaMemcpyAsync failed");
+    return;
+  }
+  check_status(pa_grad_accumulate(src, dst, n, ps(s)), what);
+}
+
 inline size_t last_dim(const Tensor& t) {
   const auto sh = t.get_shape();
   return sh.empty() ? 1 : sh.back();

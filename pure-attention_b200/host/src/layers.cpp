@@ -1,9 +1,12 @@
 // Layers and loss over core::Functional (reference: source/layers/*.cpp, source/loss/MSE.cpp).
 #include <cmath>
+#include <stdexcept>
+#include <tuple>
 
 #include "core/Functional.h"
 #include "device_util.h"
 #include "layers/LayerNorm.h"
+#include "layers/LinearAttention.h"
 #include "layers/Linear.h"
 #include "layers/MHA.h"
 #include "layers/ReLU.h"
@@ -103,6 +106,69 @@ std::shared_ptr<core::Tensor> MultiheadAttention::forward(const std::shared_ptr<
 }
 
 std::vector<std::shared_ptr<core::Tensor>> MultiheadAttention::parameters() {
+  return {in_proj_weight, in_proj_bias, out_proj_weight, out_proj_bias};
+}
+
+LinearAttention::LinearAttention(uint32_t e, uint32_t h, const std::vector<float>& decay,
+                                 const core::RopeSpec& rope)
+    : in_proj_weight(param({e, 3 * e})),
+      in_proj_bias(param({1, 3 * e})),
+      out_proj_weight(param({e, e})),
+      out_proj_bias(param({1, e})),
+      log_decay(std::make_shared<core::Tensor>(std::vector<uint32_t>{h}, false)),
+      embed_dim(e),
+      num_heads(h),
+      rope_spec(rope) {
+  if (!decay.empty() && decay.size() != h)
+    throw std::runtime_error("LinearAttention: one log decay per head");
+  std::vector<float> l(decay);
+  if (l.empty())
+    for (uint32_t i = 0; i < h; ++i)
+      l.push_back(-std::exp2(-8.0f * static_cast<float>(i + 1) / static_cast<float>(h)));
+  log_decay->to_device(l);
+  const float std_dev = std::sqrt(2.0f / static_cast<float>(e));
+  core::pop_data_normal(in_proj_weight, std_dev, stream());
+  core::pop_data_zeros(in_proj_bias, stream());
+  core::pop_data_normal(out_proj_weight, std_dev, stream());
+  core::pop_data_zeros(out_proj_bias, stream());
+}
+
+std::pair<std::shared_ptr<core::Tensor>, std::shared_ptr<core::Tensor>> LinearAttention::run(
+    const std::shared_ptr<core::Tensor>& x, const std::shared_ptr<core::IntTensor>& positions,
+    const std::shared_ptr<core::IntTensor>& lengths, const std::shared_ptr<core::Tensor>& state,
+    bool want_state) {
+  if (rope_spec.sections.empty() != (positions == nullptr))
+    throw std::runtime_error("LinearAttention: positions go with rotary sections");
+  std::vector<std::shared_ptr<core::Tensor>> qkv, out;
+  core::linear(x, in_proj_weight, in_proj_bias, 3, qkv, stream());
+  if (positions)
+    std::tie(qkv[0], qkv[1]) = core::rope(qkv[0], qkv[1], static_cast<int>(embed_dim / num_heads),
+                                          rope_spec, positions, stream());
+  auto [o, after] = core::linear_attention(qkv[0], qkv[1], qkv[2], static_cast<int>(num_heads),
+                                           log_decay, lengths, state, want_state, stream());
+  core::linear(o, out_proj_weight, out_proj_bias, 1, out, stream());
+  return {out[0], after};
+}
+
+std::shared_ptr<core::Tensor> LinearAttention::forward(const std::shared_ptr<core::Tensor>& x) {
+  return run(x, nullptr, nullptr, nullptr, false).first;
+}
+
+std::shared_ptr<core::Tensor> LinearAttention::forward(
+    const std::shared_ptr<core::Tensor>& x, const std::shared_ptr<core::IntTensor>& positions,
+    const std::shared_ptr<core::IntTensor>& lengths) {
+  return run(x, positions, lengths, nullptr, false).first;
+}
+
+std::pair<std::shared_ptr<core::Tensor>, std::shared_ptr<core::Tensor>>
+LinearAttention::forward_state(const std::shared_ptr<core::Tensor>& x,
+                               const std::shared_ptr<core::IntTensor>& positions,
+                               const std::shared_ptr<core::IntTensor>& lengths,
+                               const std::shared_ptr<core::Tensor>& state) {
+  return run(x, positions, lengths, state, true);
+}
+
+std::vector<std::shared_ptr<core::Tensor>> LinearAttention::parameters() {
   return {in_proj_weight, in_proj_bias, out_proj_weight, out_proj_bias};
 }
 
