@@ -316,7 +316,41 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
 
   const int warp = warp_id();
-  if (threadIdx.x == 0) {
+  // Role of a warp of the last warpgroup: 0 MMA issue, 1 loads, 2 and 3 splitting. The issuing warp slows the
+  // other warps of its sub-partition (an MMA that waits for the queue holds up their TMEM
+  // loads), so it sits with the 32 rows that have the fewest scores: the first forward in time,
+  // the last backward.
+  const int role = warp < 16 ? -1 : (warp - 16 + (a.n_dir == 1 ? 0 : 1)) & 3;
+  // One thread loads, all tiles by TMA.
+  const bool loads = role == 1 && lane_id() == 0;
+  auto load = [&](const ChunkIter<DK, STATES>& it) {
+    const int g = it.g, s = g % C::QKS, vs = g % C::VS;
+    const MixOne& one = a.one[it.x.dir];
+    const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
+    const uint32_t qk = bar((BF16 ? QK_FULL : QK_RAW) + s);
+    constexpr int COLS = 128 / static_cast<int>(sizeof(T));  // 128 bytes a row
+    if (g >= C::QKS && !mbar_wait(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) return false;
+    mbar_arrive_expect_tx(qk, (STATES ? 1 : 2) * C::OPER);
+#pragma unroll
+    for (int tile = 0; tile < C::OPER / kTile; ++tile) {
+      tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], qk, tile * COLS, h, tok, b);
+      if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], qk, tile * COLS, h, tok, b);
+    }
+    if (BF16) {
+      if (g >= C::VS && !mbar_wait(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) return false;
+      mbar_arrive_expect_tx(bar(V_FULL + vs), kTile);
+      tma_load_4d(sV(vs), &maps.m[one.mv], bar(V_FULL + vs), it.x.half * 64, h, tok, b);
+    } else {
+      if (g > 0 && !mbar_wait(bar(VP_EMPTY), (g - 1) & 1, status)) return false;
+      mbar_arrive_expect_tx(bar(V_RAW), 2 * kTile);
+      tma_load_4d(sVp, &maps.m[one.mv], bar(V_RAW), 0, h, tok, b);
+      tma_load_4d(sVp + kTile, &maps.m[one.mv], bar(V_RAW), COLS, h, tok, b);
+    }
+    return true;
+  };
+  ChunkIter<DK, STATES> load_it;
+  bool load_more = false;
+  if (loads) {  // the first chunk is on its way before the block has set itself up
     for (int i = 0; i < 3; ++i) {
       mbar_init(bar(QK_FULL + i), BF16 ? 1 : (STATES ? 2 : 6));  // fp32: the splitting warps
       mbar_init(bar(QK_EMPTY + i), 1);
@@ -340,20 +374,21 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     mbar_init(bar(O_FULL), 1);
     mbar_init(bar(O_FREE), 8);
     fence_mbar_init();
-  }
-  // Role of a warp of the last warpgroup: 0 MMA issue, 1 loads, 2 and 3 splitting. The issuing warp slows the
-  // other warps of its sub-partition (an MMA that waits for the queue holds up their TMEM
-  // loads), so it sits with the 32 rows that have the fewest scores: the first forward in time,
-  // the last backward.
-  const int role = warp < 16 ? -1 : (warp - 16 + (a.n_dir == 1 ? 0 : 1)) & 3;
-  if (role == 0) {
+    load_more = load_it.first(a, a.n_units);
+    if (load_more) {
+      load(load_it);
+      load_more = load_it.next(a);
+    }
+  } else if (role == 0) {
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
-  }
-  if (role == 3 && lane_id() == 0) abort_flag = aborted(status);
-  if (role == 1 && lane_id() < 3) {
-    const MixOne& one = a.one[mix_unit<DK, STATES>(a, blockIdx.x).dir];
-    tma_prefetch_desc(&maps.m[lane_id() == 0 ? one.mk : (lane_id() == 1 ? one.mq : one.mv)]);
+  } else if (role == 3) {
+    if (lane_id() == 0) abort_flag = aborted(status);
+    if (lane_id() < 4) {
+      const MixOne& one = a.one[mix_unit<DK, STATES>(a, blockIdx.x).dir];
+      tma_prefetch_desc(lane_id() == 3 ? &maps.o[one.mo]
+                                       : &maps.m[lane_id() == 0 ? one.mk : (lane_id() == 1 ? one.mq : one.mv)]);
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -777,31 +812,18 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     }
   } else if (role == 1) {
     // ------------------------------------------------------------ TMA loads
-    if (elect_one()) {
-      ChunkIter<DK, STATES> it;
-      for (bool more = it.first(a, n_units); more; more = it.next(a)) {
-        const int g = it.g, s = g % C::QKS, vs = g % C::VS;
-        const MixOne& one = a.one[it.x.dir];
-        const int tok = it.x.token(it.chunk), h = it.x.h, b = it.x.b;
-        const uint32_t qk = bar((BF16 ? QK_FULL : QK_RAW) + s);
-        if (g >= C::QKS && !mbar_wait(bar(QK_EMPTY + s), (g / C::QKS - 1) & 1, status)) break;
-        mbar_arrive_expect_tx(qk, (STATES ? 1 : 2) * C::OPER);
-        constexpr int COLS = 128 / static_cast<int>(sizeof(T));  // 128 bytes a row
-#pragma unroll
-        for (int tile = 0; tile < C::OPER / kTile; ++tile) {
-          tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], qk, tile * COLS, h, tok, b);
-          if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], qk, tile * COLS, h, tok, b);
-        }
-        if (BF16) {
-          if (g >= C::VS && !mbar_wait(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) break;
-          mbar_arrive_expect_tx(bar(V_FULL + vs), kTile);
-          tma_load_4d(sV(vs), &maps.m[one.mv], bar(V_FULL + vs), it.x.half * 64, h, tok, b);
-        } else {
-          if (g > 0 && !mbar_wait(bar(VP_EMPTY), (g - 1) & 1, status)) break;
-          mbar_arrive_expect_tx(bar(V_RAW), 2 * kTile);
-          tma_load_4d(sVp, &maps.m[one.mv], bar(V_RAW), 0, h, tok, b);
-          tma_load_4d(sVp + kTile, &maps.m[one.mv], bar(V_RAW), COLS, h, tok, b);
-        }
+    if (loads) {
+      if (abort_flag) load_more = false;
+      while (load_more && load(load_it)) load_more = load_it.next(a);
+      // After a failure nobody waits for what is still on its way: it must land before the block ends.
+      auto landed = [&](int first, int ring) {
+        for (int g = load_it.g < ring ? 0 : load_it.g - ring; g <= load_it.g; ++g)
+          mbar_drain(bar(first + g % ring), (g / ring) & 1);
+      };
+      if (aborted(status)) {
+        landed(BF16 ? QK_FULL : QK_RAW, C::QKS);
+        if (BF16) landed(V_FULL, C::VS);
+        else landed(V_RAW, 1);
       }
     }
   } else if (role >= 2) {
