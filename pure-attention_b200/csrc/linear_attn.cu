@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   constexpr int NP = C::NP, KT = C::KT;
   constexpr bool BF16 = sizeof(T) == 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[29];  // N_BARS
+  __shared__ uint64_t bars[34];  // N_BARS
   __shared__ __align__(16) float wtab[4 * 64 + 4 * 32];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -311,9 +311,15 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   auto sK = [&](int s) { return sm0 + s * 2 * C::OPER; };
   auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
   auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
-  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 10, S_FULL = 14, P_FULL = 16, VP_FULL = 18, VP_EMPTY,
-         ST_FULL, ST_EMPTY, KV_FULL, KV_FREE, O_FULL, O_FREE, QK_RAW, V_RAW = QK_RAW + 2, N_BARS };
-  constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320, T_KV = 384;
+  enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 10, S_FULL = 14, P_FULL = 16, VP_FULL = 18, VP_EMPTY = 20,
+         KV_FULL = 22, KV_FREE = 24, ST_FULL = 26, ST_EMPTY, O_FULL, O_FREE, QK_RAW = 30, V_RAW = 32, N_BARS = 34 };
+  // Segment states: V' and K^T V' twice, in what Q and its scores do not use there.
+  constexpr int VB = STATES ? 2 : 1;
+  constexpr uint32_t VP_LO2 = C::OPER >= 2 * kTile ? kTile : 2 * C::OPER;  // hi to lo in the second V'
+  auto vp_at = [&](int g) { return VB == 2 && (g & 1) ? sm0 + C::OPER : sVp; };
+  auto vp_lo = [&](int g) { return VB == 2 && (g & 1) ? VP_LO2 : static_cast<uint32_t>(kTile); };
+  auto kv_at = [&](int g) { return VB == 2 && (g & 1) ? 0u : 384u; };
+  constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320;  // and kv_at
 
   const int warp = warp_id();
   // Role of a warp of the last warpgroup: 0 MMA issue, 1 loads, 2 and 3 splitting. The issuing warp slows the
@@ -341,10 +347,11 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       mbar_arrive_expect_tx(bar(V_FULL + vs), kTile);
       tma_load_4d(sV(vs), &maps.m[one.mv], bar(V_FULL + vs), it.x.half * 64, h, tok, b);
     } else {
-      if (g > 0 && !mbar_wait(bar(VP_EMPTY), (g - 1) & 1, status)) return false;
-      mbar_arrive_expect_tx(bar(V_RAW), 2 * kTile);
-      tma_load_4d(sVp, &maps.m[one.mv], bar(V_RAW), 0, h, tok, b);
-      tma_load_4d(sVp + kTile, &maps.m[one.mv], bar(V_RAW), COLS, h, tok, b);
+      if (g >= VB && !mbar_wait(bar(VP_EMPTY + g % VB), (g / VB - 1) & 1, status)) return false;
+      const uint32_t raw = bar(V_RAW + g % VB);
+      mbar_arrive_expect_tx(raw, 2 * kTile);
+      tma_load_4d(vp_at(g), &maps.m[one.mv], raw, 0, h, tok, b);
+      tma_load_4d(vp_at(g) + vp_lo(g), &maps.m[one.mv], raw, COLS, h, tok, b);
     }
     return true;
   };
@@ -363,14 +370,16 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       mbar_init(bar(S_FULL + i), 1);
       mbar_init(bar(P_FULL + i), 8);
     }
-    for (int i = 0; i < 2; ++i) mbar_init(bar(QK_RAW + i), 1);
-    mbar_init(bar(V_RAW), 1);
-    mbar_init(bar(VP_FULL), 4);
-    mbar_init(bar(VP_EMPTY), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(bar(QK_RAW + i), 1);
+      mbar_init(bar(V_RAW + i), 1);
+      mbar_init(bar(VP_FULL + i), 4);
+      mbar_init(bar(VP_EMPTY + i), 1);
+      mbar_init(bar(KV_FULL + i), 1);
+      mbar_init(bar(KV_FREE + i), 4);
+    }
     mbar_init(bar(ST_FULL), 4);
     mbar_init(bar(ST_EMPTY), 1);
-    mbar_init(bar(KV_FULL), 1);
-    mbar_init(bar(KV_FREE), 4);
     mbar_init(bar(O_FULL), 1);
     mbar_init(bar(O_FREE), 8);
     fence_mbar_init();
@@ -662,12 +671,12 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         const int lead = !STATES && x.starts(c) ? one.dir.lead : 0;
         const float dec = exp2f(l2 * static_cast<float>(x.valid(c) - lead));
         const float2 dec2 = make_float2(dec, dec);
-        if (!(ok = mbar_wait_warp(bar(KV_FULL), g & 1, status))) break;
+        if (!(ok = mbar_wait_warp(bar(KV_FULL + g % VB), (g / VB) & 1, status))) break;
         tc_fence_after();
 #pragma unroll
         for (int j = 0; j < NC / 16; ++j) {
           uint32_t vh[16], vl[16];  // K^T V' hi and K^T V' lo
-          const uint32_t at = tmem + T_KV + col0 + j * 16 + lane_base;
+          const uint32_t at = tmem + kv_at(g) + col0 + j * 16 + lane_base;
           tmem_ld16x2_sync(at, at + 64, vh, vl);
 #pragma unroll
           for (int e = 0; e < 8; ++e)
@@ -675,7 +684,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
                                                                    pair_of(vl[2 * e], vl[2 * e + 1])));
         }
         tc_fence_before();
-        warp_arrive(bar(KV_FREE));
+        warp_arrive(bar(KV_FREE + g % VB));
         if (!STATES && c + 1 < x.chunks && !(ok = put_state(g + 1))) break;
       }
       if (!ok) break;
@@ -750,7 +759,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           for (int i = 0; i < 8; ++i)
             if (t / 8 + 16 * i >= valid) v[i] = make_uint4(0, 0, 0, 0);
         }
-        if (g > 0 && !mbar_wait_warp(bar(VP_EMPTY), (g - 1) & 1, status)) break;
+        if (g >= VB && !mbar_wait_warp(bar(VP_EMPTY + g % VB), (g / VB - 1) & 1, status)) break;
+        const uint32_t to = vp_at(g), to_lo = to + vp_lo(g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const uint32_t off = sw128_offset(t / 8 + 16 * i, (t % 8) * 16);
@@ -764,11 +774,11 @@ __global__ void __launch_bounds__(kMixThreads, 1)
             h[j] = *reinterpret_cast<const uint32_t*>(&hh);
             l[j] = *reinterpret_cast<const uint32_t*>(&ll);
           }
-          st_shared_v4(sVp + off, h[0], h[1], h[2], h[3]);
-          st_shared_v4(sVp + kTile + off, l[0], l[1], l[2], l[3]);
+          st_shared_v4(to + off, h[0], h[1], h[2], h[3]);
+          st_shared_v4(to_lo + off, l[0], l[1], l[2], l[3]);
         }
         fence_proxy_async_smem();
-        warp_arrive(bar(VP_FULL));
+        warp_arrive(bar(VP_FULL + g % VB));
       }
     } else {
       // fp32: split q in place, then v, which lands where its V' goes
@@ -790,17 +800,17 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           fence_proxy_async_smem();
           warp_arrive(bar(QK_FULL + s));
         }
-        if (!mbar_wait_warp(bar(V_RAW), g & 1, status)) break;
-        const X v(sVp, t);
+        if (!mbar_wait_warp(bar(V_RAW + g % VB), (g / VB) & 1, status)) break;
+        const X v(vp_at(g), t);  // (its planes are a tile apart there in either place)
         float4 r[X::VECS];
 #pragma unroll
         for (int i = 0; i < X::VECS; ++i) r[i] = v.load(i, valid);
         __syncwarp();
 #pragma unroll
         for (int i = 0; i < X::VECS; ++i)
-          v.template store<2>(sVp, i, make_float4(r[i].x * w[i], r[i].y * w[i], r[i].z * w[i], r[i].w * w[i]));
+          v.template store<2>(vp_at(g), i, make_float4(r[i].x * w[i], r[i].y * w[i], r[i].z * w[i], r[i].w * w[i]));
         fence_proxy_async_smem();
-        warp_arrive(bar(VP_FULL));
+        warp_arrive(bar(VP_FULL + g % VB));
         if (!STATES) {
           if (g > 0 && !mbar_wait_warp(bar(V_EMPTY), (g - 1) & 1, status)) break;
 #pragma unroll
@@ -823,7 +833,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       if (aborted(status)) {
         landed(BF16 ? QK_FULL : QK_RAW, C::QKS);
         if (BF16) landed(V_FULL, C::VS);
-        else landed(V_RAW, 1);
+        else landed(V_RAW, VB);
       }
     }
   } else if (role >= 2) {
@@ -854,7 +864,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       auto mn = [](int k) { return static_cast<uint32_t>(k * 2048); };
       const Desc dQ{make_sdesc(sQ(0), 16, 1024)}, dK{make_sdesc(sK(0), 16, 1024)},
           dKt{make_sdesc(sK(0), DK == 64 ? 0 : kTile, 1024)}, dV{make_sdesc(sV(0), kTile, 1024)},
-          dVp{make_sdesc(sVp, kTile, 1024)}, dS{make_sdesc(ss0, kTile, 1024)};
+          dS{make_sdesc(ss0, kTile, 1024)};
       auto wait = [&](int i, int phase) { return mbar_wait(bar(i), phase & 1, status); };
       auto issue_S = [&](int g) {
         const int s = g % C::QKS;
@@ -877,18 +887,19 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         if (!STATES && g == 0) ok = ok && issue_S(0);
         // K^T [V' hi, V' lo] (DK = 64: both halves of the 128 rows are the same 64 rows of the
         // state, so every warp of the state finds its columns in its own lanes)
-        ok = ok && wait(VP_FULL, g) && (g < 1 || wait(KV_FREE, g - 1));
+        ok = ok && wait(VP_FULL + g % VB, g / VB) && (g < VB || wait(KV_FREE + g % VB, g / VB - 1));
         if (!ok) break;
         tc_fence_after();
-        const Desc kt = dKt.at(s * 2 * C::OPER);
+        const Desc kt = dKt.at(s * 2 * C::OPER), vp{make_sdesc(vp_at(g), vp_lo(g), 1024)};
+        const uint32_t kv = tmem + kv_at(g);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) umma_f16_ss(tmem + T_KV, kt.at(mn(k)).d, dVp.at(mn(k)).d, idKV, k > 0 ? 1u : 0u);
+        for (int k = 0; k < 8; ++k) umma_f16_ss(kv, kt.at(mn(k)).d, vp.at(mn(k)).d, idKV, k > 0 ? 1u : 0u);
         if (NT == 3) {
 #pragma unroll
-          for (int k = 0; k < 8; ++k) umma_f16_ss(tmem + T_KV, kt.at(LO + mn(k)).d, dVp.at(mn(k)).d, idKV1, 1u);
+          for (int k = 0; k < 8; ++k) umma_f16_ss(kv, kt.at(LO + mn(k)).d, vp.at(mn(k)).d, idKV1, 1u);
         }
-        umma_commit(bar(KV_FULL));
-        umma_commit(bar(VP_EMPTY));
+        umma_commit(bar(KV_FULL + g % VB));
+        umma_commit(bar(VP_EMPTY + g % VB));
         if (STATES) {
           umma_commit(bar(QK_EMPTY + s));
           umma_commit(bar(V_EMPTY + vs));
