@@ -52,9 +52,10 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 //               and 32 columns of O each)
 //   warps 8-11  the state in fp32 registers (thread = row of the state), its bf16
 //               parts to shared memory for Q S
-//   warps 12-15 V' from V (fp32: and the splitting of q and v)
+//               (fp32: and the splitting of k)
+//   warps 12-15 V' from V (fp32: and the splitting of v)
 //   warps 16-19 tcgen05.mma issue (one thread), TMA loads (one thread), the splitting of
-//               fp32 k (two warps)
+//               fp32 q (two warps)
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
@@ -595,6 +596,24 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     const int row = DK == 64 ? (r & 63) : r, col0 = DK == 64 ? (r >> 6) * 32 : 0;
     int g = 0;
     bool ok = true;
+    // fp32: these warps have the time to split k, a chunk ahead of the state
+    ChunkIter<DK, STATES> k_it;
+    bool k_more = !BF16 && !STATES && k_it.first(a, n_units);
+    auto split_k = [&]() {
+      if constexpr (!BF16 && !STATES) {
+        if (!k_more) return true;
+        const int s = k_it.g % C::QKS;
+        if (!mbar_wait_warp(bar(QK_RAW + s), (k_it.g / C::QKS) & 1, status)) return false;
+        const Split<128> k(sK(s), r);
+#pragma unroll 1
+        for (int i = 0; i < Split<128>::VECS; i += 8) k.template eight<NP>(i, k_it.valid());
+        fence_proxy_async_smem();
+        warp_arrive(bar(QK_FULL + s));
+        k_more = k_it.next(a);
+      }
+      return true;
+    };
+    ok = split_k();
     for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
       const MixUnit x = mix_unit<DK, STATES>(a, u);
       const MixOne& one = a.one[x.dir];
@@ -671,6 +690,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         const int lead = !STATES && x.starts(c) ? one.dir.lead : 0;
         const float dec = exp2f(l2 * static_cast<float>(x.valid(c) - lead));
         const float2 dec2 = make_float2(dec, dec);
+        if (!(ok = split_k())) break;
         if (!(ok = mbar_wait_warp(bar(KV_FULL + g % VB), (g / VB) & 1, status))) break;
         tc_fence_after();
 #pragma unroll
@@ -781,24 +801,16 @@ __global__ void __launch_bounds__(kMixThreads, 1)
         warp_arrive(bar(VP_FULL + g % VB));
       }
     } else {
-      // fp32: split q in place, then v, which lands where its V' goes
+      // fp32: v lands where its V' goes
       using X = Split<128>;
       float w[X::VECS];
       for (; more; more = it.next(a)) {
-        const int g = it.g, s = g % C::QKS, valid = it.valid();
+        const int g = it.g, valid = it.valid();
         if (it.u != w_unit || valid != w_valid) {
 #pragma unroll
           for (int i = 0; i < X::VECS; ++i) w[i] = weight(t / 16 + i * X::ROWS, valid);
           w_unit = it.u;
           w_valid = valid;
-        }
-        if (!STATES) {
-          if (!mbar_wait_warp(bar(QK_RAW + s), (g / C::QKS) & 1, status)) break;
-          const X q(sQ(s), t);
-#pragma unroll 1
-          for (int i = 0; i < X::VECS; i += 8) q.template eight<NP>(i, valid);
-          fence_proxy_async_smem();
-          warp_arrive(bar(QK_FULL + s));
         }
         if (!mbar_wait_warp(bar(V_RAW + g % VB), (g / VB) & 1, status)) break;
         const X v(vp_at(g), t);  // (its planes are a tile apart there in either place)
@@ -837,16 +849,16 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       }
     }
   } else if (role >= 2) {
-    // ------------------------------------------------------------ fp32: split k in place
+    // ------------------------------------------------------------ fp32: split q in place (segment states: k)
     if constexpr (!BF16) {
       const int t = (role - 2) * 32 + lane_id();
       ChunkIter<DK, STATES> it;
       for (bool more = it.first(a, n_units); more; more = it.next(a)) {
         const int g = it.g, s = g % C::QKS;
         if (!mbar_wait_warp(bar(QK_RAW + s), (g / C::QKS) & 1, status)) break;
-        const Split<64> k(sK(s), t);
+        const Split<64> x(STATES ? sK(s) : sQ(s), t);
 #pragma unroll 1
-        for (int i = 0; i < Split<64>::VECS; i += 8) k.template eight<NP>(i, it.valid());
+        for (int i = 0; i < Split<64>::VECS; i += 8) x.template eight<NP>(i, it.valid());
         fence_proxy_async_smem();
         warp_arrive(bar(QK_FULL + s));
       }
@@ -905,7 +917,9 @@ __global__ void __launch_bounds__(kMixThreads, 1)
           umma_commit(bar(V_EMPTY + vs));
           continue;
         }
-        if (g + 1 < total && !(ok = issue_S(g + 1))) break;
+        // The next chunk's scores before this one's Q S, so that its P is ready in time; fp32 tiles, of
+        // which there are two, the other way round: Q S frees the tiles of the chunk after next.
+        if (BF16 && g + 1 < total && !(ok = issue_S(g + 1))) break;
         // Q S from the state entering this chunk
         ok = wait(ST_FULL, g) && (g < 1 || wait(O_FREE, g - 1));
         if (!ok) break;
@@ -919,6 +933,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
                         dS.at((term == 1 ? C::ST_PLANE : 0) + mn(k)).d, idV, (term > 0 || k > 0) ? 1u : 0u);
         umma_commit(bar(ST_EMPTY));
         umma_commit(bar(QK_EMPTY + s));
+        if (!BF16 && g + 1 < total && !(ok = issue_S(g + 1))) break;
         // P V
         ok = wait(V_FULL + vs, g / C::VS) && wait(P_FULL + b, g >> 1);
         if (!ok) break;
