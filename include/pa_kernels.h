@@ -177,7 +177,8 @@ typedef struct pa_rope_desc {
 
 /* q_out = turn(q) [B, L, num_heads, D], k_out = turn(k) [B, L, num_kv_heads, D];
  * positions is a device array [axes, B, L] of any int32 values. q_out may be q
- * and k_out k (in place); other overlaps are not allowed. */
+ * and k_out k (in place); other overlaps are not allowed (PA_ERR_SHAPE where the
+ * pointers show one). q and k may be the same tensor if neither is an output. */
 int pa_rope_fwd(const pa_rope_desc* desc, const void* q, const void* k, const int32_t* positions,
                 void* q_out, void* k_out, pa_stream_t stream);
 /* Its adjoint, the turn by the negative angles: dq (overwritten, or added to
@@ -200,8 +201,12 @@ int pa_rope_bwd(const pa_rope_desc* desc, const void* dq_out, const void* dk_out
  * them is not used (NaN allowed) and o, dq, dk, dv are zero there (left as they
  * were by accumulate). States are [B, H, D, D] fp32 in every dtype: state_in
  * NULL starts from zero; state_out (NULL: not wanted) is the state after the
- * last valid token and may be state_in. Results do not depend on the run: no
- * atomics. */
+ * last valid token and may be state_in. Results do not depend on the run: each
+ * sum has one order. The scale lies within 2^-64 .. 2^64 (PA_ERR_SHAPE otherwise).
+ * Values of valid tokens and states are finite: an infinity or NaN there may
+ * show in outputs of other tokens of its sequence and head, earlier ones too.
+ * A workspace belongs to one call at a time: calls that may overlap on the GPU,
+ * and graphs that may, need one each. */
 size_t pa_linear_attn_fwd_workspace_size(const pa_attn_desc* desc);
 int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
                        const float* log_decay, const int32_t* seq_lens, const float* state_in,

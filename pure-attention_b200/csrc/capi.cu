@@ -237,7 +237,7 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
   }
   if (2 * pairs > d->head_dim) return PA_ERR_SHAPE;
   const long long tokens = static_cast<long long>(d->batch) * d->seq_len;
-  // the kernel's items of one token block and its grid are ints
+  // the kernel counts heads and the tokens of one block in ints
   if (tokens > 0x7fffffffLL ||
       (static_cast<long long>(d->num_heads) + d->num_kv_heads) * d->head_dim * 8 > 0x7fffffffLL)
     return PA_ERR_SHAPE;
@@ -245,6 +245,8 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
   if (!aligned16(q) || !aligned16(qo) || (d->num_kv_heads > 0 && (!aligned16(k) || !aligned16(ko))))
     return PA_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0) return PA_ERR_ALIGN;
+  // in place is one tensor's turn over itself, not over the other's
+  if (d->num_kv_heads > 0 && (qo == ko || qo == k || ko == q)) return PA_ERR_SHAPE;
   sh->B = d->batch;
   sh->L = d->seq_len;
   sh->Hq = d->num_heads;
@@ -261,9 +263,16 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
+// The backward divides by the scale, so that has to stay far from fp32's limits.
+int check_linear_attn(const pa_attn_desc* desc, pa::AttnShape* sh) {
+  const int st = check_attn(desc, sh);
+  if (st != PA_OK) return st;
+  return sh->scale >= 0x1p-64f && sh->scale <= 0x1p64f ? PA_OK : PA_ERR_SHAPE;
+}
+
 size_t linear_attn_workspace(const pa_attn_desc* desc, bool backward) {
   pa::AttnShape sh;
-  if (check_attn(desc, &sh) != PA_OK) return 0;
+  if (check_linear_attn(desc, &sh) != PA_OK) return 0;
   return pa::linear_attn_workspace_bytes(sh, desc->dtype == PA_F32, backward);
 }
 
@@ -305,7 +314,7 @@ int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, c
                        void* o, float* state_out, void* workspace, size_t workspace_bytes,
                        pa_stream_t stream) {
   pa::AttnShape sh;
-  int st = check_attn(desc, &sh);
+  int st = check_linear_attn(desc, &sh);
   if (st != PA_OK) return st;
   if (!q || !k || !v || !log_decay || !o) return PA_ERR_NULL;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(log_decay) ||
@@ -330,7 +339,7 @@ int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, c
                        void* dv, float* d_state_in, int accumulate, void* workspace,
                        size_t workspace_bytes, pa_stream_t stream) {
   pa::AttnShape sh;
-  int st = check_attn(desc, &sh);
+  int st = check_linear_attn(desc, &sh);
   if (st != PA_OK) return st;
   if (!q || !k || !v || !dO || !log_decay || !dq || !dk || !dv) return PA_ERR_NULL;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(dO) || !aligned16(dq) ||
@@ -359,7 +368,7 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
                         const float* log_decay, const float* state_in, void* o, float* state_out,
                         pa_stream_t stream) {
   pa::AttnShape sh;
-  const int st = check_attn(desc, &sh);
+  const int st = check_linear_attn(desc, &sh);
   if (st != PA_OK) return st;
   if (sh.L != 1) return PA_ERR_SHAPE;
   if (!q || !k || !v || !log_decay || !state_in || !o || !state_out) return PA_ERR_NULL;

@@ -359,7 +359,7 @@ def _check_linear_attn(fn, d, q, log_decay, seq_lens, names, tensors, states):
 _linear_attn_sizes = {}
 
 
-def _linear_attn_ws(size_of, d, workspace, q):
+def _linear_attn_ws(size_of, d, workspace, q, stream):
     if workspace is None:
         key = (size_of, d.batch, d.seq_len, d.num_heads, d.head_dim, d.dtype, q.get_device())
         need = _linear_attn_sizes.get(key)
@@ -368,7 +368,9 @@ def _linear_attn_ws(size_of, d, workspace, q):
         if need == 0:
             return None, 0
         import torch
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        # memory of the stream that will use it: the allocator orders its reuse there
+        with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     return workspace, workspace.numel() * workspace.element_size()
 
 
@@ -384,7 +386,7 @@ def linear_attn_fwd(q, k, v, log_decay, o, seq_lens=None, state_in=None, state_o
     d = desc or attn_desc(q)
     _check_linear_attn("linear_attn_fwd", d, q, log_decay, seq_lens, ("q", "k", "v", "o"), (q, k, v, o),
                        (state_in, state_out))
-    ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size, d, workspace, q)
+    ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size, d, workspace, q, stream)
     _check("pa_linear_attn_fwd", load().pa_linear_attn_fwd(
         ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), _ptr(seq_lens),
         _ptr(state_in), o.data_ptr(), _ptr(state_out), _ptr(ws), nb, _stream() if stream is None else stream))
@@ -402,7 +404,7 @@ def linear_attn_bwd(q, k, v, dO, log_decay, dq, dk, dv, seq_lens=None, state_in=
     d = desc or attn_desc(q)
     _check_linear_attn("linear_attn_bwd", d, q, log_decay, seq_lens, ("q", "k", "v", "dO", "dq", "dk", "dv"),
                        (q, k, v, dO, dq, dk, dv), (state_in, d_state_out, d_state_in))
-    ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size, d, workspace, q)
+    ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size, d, workspace, q, stream)
     _check("pa_linear_attn_bwd", load().pa_linear_attn_bwd(
         ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), dO.data_ptr(), log_decay.data_ptr(),
         _ptr(seq_lens), _ptr(state_in), _ptr(d_state_out), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

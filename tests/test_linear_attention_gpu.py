@@ -340,3 +340,80 @@ def test_rotary_then_linear_attention_trains_as_in_64_bits():
     assert rel_err(o.double().cpu(), want.detach().cpu()) < NORM[torch.float32]
     for got, w in zip(g, torch.autograd.grad((want * dO.double()).sum(), x)):
         assert rel_err(got.double().cpu(), w.cpu()) < NORM[torch.float32]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_more_heads_than_sms_with_lengths_of_all_kinds(dtype, D):
+    """Each block takes several (sequence, head) pairs one after another, some of them empty."""
+    B, L, H = 61, 270, 5
+    q, k, v, dO, ld, s, ds = _inputs(B, L, H, D, dtype, 90, states=True)
+    g = torch.Generator().manual_seed(91)
+    lens = torch.randint(-3, L + 9, (B,), generator=g, dtype=torch.int32)
+    lens[::7] = 0
+    lens[1::9] = 1
+    lens[2::11] = 128
+    for b in range(B):
+        for x in (q, k, v, dO):
+            x[b, max(0, int(lens[b])):] = float("nan")
+    lens = lens.cuda()
+    _check_forward(*(torch.nan_to_num(x) for x in (q, k, v)), ld, lens, s)
+    o, _ = _forward(q, k, v, ld, seq_lens=lens, state_in=s)
+    assert torch.isfinite(o).all()
+    _check_backward(q, k, v, dO, ld, lens, s, ds)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_segments_with_short_and_empty_sequences(dtype, D):
+    """Long enough to be cut into segments, most of which the shorter sequences do not reach."""
+    q, k, v, dO, ld, s, ds = _inputs(4, 4500, 2, D, dtype, 92, states=True)
+    lens = torch.tensor([4500, 130, 0, 2049], dtype=torch.int32).cuda()
+    _check_forward(q, k, v, ld, lens, s)
+    _check_backward(q, k, v, dO, ld, lens, s, ds)
+    _check_backward(q, k, v, dO, ld, lens, None, None, accumulate=True)
+
+
+@pytest.mark.gpu
+def test_past_2_31_values():
+    """The last tokens of tensors of more than 2^31 values. With a decay of e^-0.7 what lies 400
+    tokens back counts e^-280: the last 600 tokens alone give them."""
+    import pa_capi
+    B, L, H, D, W, C = 1, (1 << 19) + 77, 64, 64, 600, 200
+    t, heads = torch.bfloat16, [0, 63]
+    q, k, v, dO = (torch.empty(B, L, H, D, dtype=t, device="cuda").normal_(std=0.5) for _ in range(4))
+    ld = torch.full((H,), -0.7, device="cuda")
+    o = torch.full_like(q, float("nan"))
+    so = torch.empty(B, H, D, D, device="cuda")
+    pa_capi.linear_attn_fwd(q, k, v, ld, o, state_out=so)
+    x = [y[:, -W:, heads].contiguous() for y in (q, k, v, dO)]
+    want, ws = mix(*x[:3], ld[heads])
+    mag, ms = mix(*x[:3], ld[heads], absolute=True)
+    _close(o[:, -C:, heads], want[:, -C:], mag[:, -C:], REL[t], 2.0 ** -8)
+    _close(so[:, heads], ws, ms, STATE[t], 2.0 ** -24)
+    g = [o] + [torch.empty_like(q) for _ in range(2)]
+    for y in g:
+        y.fill_(1.0)
+    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, accumulate=True)
+    assert pa_capi.device_status() == 0
+    want = mix_grads(*x[:3], ld[heads], x[3])
+    mag = mix_grads_absolute(*x[:3], ld[heads], x[3])
+    for got, w, m in zip(g, want, mag):
+        _close(got[:, -C:, heads], w[:, -C:] + 1.0, m[:, -C:], REL[t], 2.0 ** -8 * 1.01)
+
+
+@pytest.mark.gpu
+def test_workspace_of_a_call_on_a_stream_given_by_its_handle():
+    """The workspace that the binding allocates belongs to the stream that the kernels run on."""
+    import pa_capi
+    q, k, v, dO, ld, _, _ = _inputs(1, 4100, 2, 64, torch.bfloat16, 93)
+    want, _ = _forward(q, k, v, ld)
+    side = torch.cuda.Stream()
+    for handle, st in ((side.cuda_stream, side), (0, torch.cuda.default_stream())):
+        outs = [torch.zeros_like(q) for _ in range(4)]
+        torch.cuda.synchronize()
+        for o in outs:
+            pa_capi.linear_attn_fwd(q, k, v, ld, o, stream=handle)
+            torch.full((1 << 22,), float("nan"), device="cuda")  # would take a freed workspace of its own stream
+        st.synchronize()
+        assert all(torch.equal(o, want) for o in outs)

@@ -130,3 +130,18 @@ def test_rope_on_a_stream_and_in_a_graph():
     g.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_rope_past_2_31_values():
+    import pa_capi
+    B, L, H, D = 1, (1 << 19) + 77, 64, 64
+    q = torch.zeros(B, L, H, D, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(9)
+    tail = torch.randn(B, 90, H, D, generator=g).bfloat16().cuda()
+    q[:, -90:] = tail
+    pos = torch.arange(L, dtype=torch.int32, device="cuda").reshape(1, 1, L)
+    pa_capi.rope_fwd(q, None, pos, q, None, pa_capi.rope_desc(q))
+    want = turn(tail, pos[:, :, -90:], [32])
+    _check(q[:, -90:], tail, want, [32], "halves")
+    assert not q[:, :-90].any()

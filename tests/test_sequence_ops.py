@@ -125,3 +125,23 @@ def test_binding_refusals():
         pa_capi.linear_attn_fwd(q, q, q.transpose(1, 2).contiguous().transpose(1, 2), ld, q)
     with pytest.raises(ValueError, match="state_in must be"):
         pa_capi.linear_attn_step(q, q, q, ld, torch.zeros(2, 4, 64, 32), q, q)
+
+
+def test_rope_refuses_outputs_over_the_other_tensor():
+    import pa_capi
+    lib = pa_capi.load()
+    for a in ((16, 32, 64, 128, 128), (16, 32, 64, 32, 256), (16, 32, 64, 128, 16)):
+        assert lib.pa_rope_fwd(_rope(), *a, None) == SHAPE
+        assert lib.pa_rope_bwd(_rope(), *a, 0, None) == SHAPE
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-44, 1e30, float("inf")])
+def test_linear_attention_scale_refusals(scale):
+    import pa_capi
+    lib = pa_capi.load()
+    big = 1 << 40
+    assert lib.pa_linear_attn_fwd(_desc(scale=scale), 16, 32, 48, 64, None, None, 80, None, 256, big, None) == SHAPE
+    assert lib.pa_linear_attn_bwd(_desc(scale=scale), 16, 32, 48, 64, 80, None, None, None, 96, 112, 128, None, 0,
+                                  256, big, None) == SHAPE
+    assert lib.pa_linear_attn_step(_desc(L=1, scale=scale), 16, 32, 48, 64, 80, 96, 112, None) == SHAPE
+    assert lib.pa_linear_attn_fwd_workspace_size(_desc(L=9000, scale=scale)) == 0
