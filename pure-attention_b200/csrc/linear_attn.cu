@@ -96,9 +96,28 @@ struct MixOne {  // one direction of the recurrence
   int mq, mk, mv;  // bf16: the tensor maps of q, k, v
   int mo;          // and of o
 };
+// Division by a number that the host knows: n / d = (high word of n mul + n) >> shift for
+// n < 2^31, with shift = ceil(log2 d) and mul = floor(2^32 (2^shift - d) / d) + 1.
+struct Divisor {
+  uint32_t d, mul, shift;
+  static Divisor of(int d) {
+    Divisor x{static_cast<uint32_t>(d), 0, 0};
+    while ((1ull << x.shift) < x.d) ++x.shift;
+    x.mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << x.shift) - x.d)) / x.d + 1);
+    return x;
+  }
+  // n / d, and n becomes the remainder
+  __device__ __forceinline__ int split(int& n) const {
+    const uint32_t u = static_cast<uint32_t>(n), q = (__umulhi(u, mul) + u) >> shift;
+    n = static_cast<int>(u - q * d);
+    return static_cast<int>(q);
+  }
+};
+
 struct MixArgs {
   MixOne one[3];
   int n_dir;
+  Divisor by_dir, by_H, by_B;
   const float* log_decay;
   const int32_t* lens;
   float* ws;  // segment states, see seg_slot
@@ -141,13 +160,12 @@ __device__ __forceinline__ MixUnit mix_unit(const MixArgs& a, int u) {
   constexpr int halves = DK / 64;
   x.half = u % halves;
   u /= halves;
-  x.dir = u % a.n_dir;
-  u /= a.n_dir;
-  x.h = u % a.H;
-  u /= a.H;
-  x.b = u % a.B;
+  x.dir = u;
+  x.h = a.by_dir.split(x.dir);
+  x.b = a.by_H.split(x.h);
+  x.seg = a.by_B.split(x.b);
   x.rev = a.one[x.dir].dir.reverse;
-  x.seg = u / a.B + (STATES && x.rev ? a.fine : 0);
+  if (STATES && x.rev) x.seg += a.fine;
   x.n = valid_tokens(a.lens, x.b, a.L);
   const int tokens = STATES ? a.state_tokens : a.seg_tokens;
   x.p0 = x.seg * tokens;
@@ -1087,6 +1105,9 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
   a.L = sh.L;
   a.H = sh.H;
   a.D = sh.D;
+  a.by_dir = Divisor::of(a.n_dir);
+  a.by_H = Divisor::of(sh.H);
+  a.by_B = Divisor::of(sh.B);
   a.n_seg = p.n_seg;
   a.seg_tokens = p.seg_tokens;
   a.n_units = p.pairs * p.n_seg;
