@@ -759,8 +759,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     bool more = it.first(a, n_units);
     int w_unit = -1, w_valid = 0;
     // l^(valid - 1 - row), backward l^row; zero past the end
-    auto weight = [&](int row, int valid) {
-      const float l2 = log2_decay(a.log_decay, it.x.h);
+    auto weight = [&](float l2, int row, int valid) {
       return row < valid ? exp2f(l2 * static_cast<float>(it.x.rev ? row : valid - 1 - row)) : 0.f;
     };
     if constexpr (BF16) {
@@ -771,9 +770,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       for (; more; more = it.next(a)) {
         const int g = it.g, vs = g % C::VS, valid = it.valid();
         if (it.u != w_unit || valid != w_valid) {
+          const float l2 = log2_decay(a.log_decay, it.x.h);
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            const float w = weight(t / 8 + 16 * i, valid);
+            const float w = weight(l2, t / 8 + 16 * i, valid);
             wh[i] = __float2bfloat162_rn(w);
             wl[i] = __float2bfloat162_rn(w - __low2float(wh[i]));
           }
@@ -825,8 +825,9 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       for (; more; more = it.next(a)) {
         const int g = it.g, valid = it.valid();
         if (it.u != w_unit || valid != w_valid) {
+          const float l2 = log2_decay(a.log_decay, it.x.h);
 #pragma unroll
-          for (int i = 0; i < X::VECS; ++i) w[i] = weight(t / 16 + i * X::ROWS, valid);
+          for (int i = 0; i < X::VECS; ++i) w[i] = weight(l2, t / 16 + i * X::ROWS, valid);
           w_unit = it.u;
           w_valid = valid;
         }
