@@ -1040,14 +1040,21 @@ struct MixPlan {
   int fine;              // pieces of a segment whose states are computed on their own
   int n_slots;
 };
-MixPlan mix_plan(const AttnShape& sh, int n_dir) {
+MixPlan mix_plan(const AttnShape& sh, bool f32, int n_dir) {
   MixPlan p;
   const int chunks = (sh.L + 127) / 128, sms = device_sm_count();
   p.pairs = sh.B * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
-  // segments for the SMs there are, of 8 chunks at least: below that the second launch and the
-  // second reading of k and v cost more than they bring
+  // Segments for the SMs there are, of 2 chunks at least (fp32, 2 heads, 64 chunks: 36 us with 48
+  // segments, 43 with 64), and so few that adding up their states stays cheap (bf16, 2 heads, 64
+  // chunks: 25 us with 24, 28 with 37; 1024 chunks: 78 with 64, 82 with 74).
   int seg = sms / p.pairs;
-  if (seg > chunks / 8) seg = chunks / 8;
+  if (seg > chunks / 2) seg = chunks / 2;
+  while (seg > 1 && seg * seg > 8 * chunks) --seg;
+  // None where the second launch and the second reading of k and v cost more than the chunks that a
+  // sequence no longer waits for. bf16, 2 segments of 4 heads: 8 chunks 19 us whole and 24 cut, 32
+  // chunks 50 and 39; 4 segments of 32 heads: 8 chunks 19 and 22, 16 chunks 30 and 26. A chunk of fp32
+  // takes twice as long: gradients in 2 segments of 16 heads 12 chunks 50 and 54, 16 chunks 63 and 59.
+  if (seg > 1 && chunks - (chunks + seg - 1) / seg < (f32 ? 7 : 9)) seg = 1;
   if (seg < 1) seg = 1;
   int seg_chunks = (chunks + seg - 1) / seg;
   // the states' launch has one segment less: cut finer it still fills the GPU
@@ -1101,7 +1108,7 @@ bool make_out_map(CUtensorMap* m, const void* base, const AttnShape& sh, bool f3
 
 int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const int32_t* lens, void* ws,
         uint32_t* status, cudaStream_t s) {
-  const MixPlan p = mix_plan(sh, a.n_dir);
+  const MixPlan p = mix_plan(sh, f32, a.n_dir);
   a.log_decay = log_decay;
   a.lens = lens;
   a.ws = static_cast<float*>(ws);
@@ -1158,8 +1165,8 @@ int step(const AttnShape& sh, const void* q, const void* k, const void* v, const
 
 }  // namespace
 
-size_t linear_attn_workspace_bytes(const AttnShape& sh, bool, bool backward) {
-  const MixPlan p = mix_plan(sh, backward ? 3 : 1);
+size_t linear_attn_workspace_bytes(const AttnShape& sh, bool f32, bool backward) {
+  const MixPlan p = mix_plan(sh, f32, backward ? 3 : 1);
   return p.n_seg == 1 ? 0 : static_cast<size_t>(p.pairs) * p.n_slots * (sh.D == 128 ? 128 : 64) * 64 * sizeof(float);
 }
 
