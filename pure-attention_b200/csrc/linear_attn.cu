@@ -637,8 +637,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       const MixOne& one = a.one[x.dir];
       const float l2 = log2_decay(a.log_decay, x.h);
       const bool in_state = row < a.D && x.half * 64 + col0 < a.D;  // head dim 32: a quarter of the tile
-      // element (row, column 0) of the caller's state, and the step to the next column
-      const long long e0 = x.half * 64 + col0, st_step = one.dir.transposed ? a.D : 1;
+      // element (row, column 0) of the caller's state
+      const long long e0 = x.half * 64 + col0;
       const size_t st0 = (static_cast<size_t>(x.b) * a.H + x.h) * a.D * a.D +
                          (one.dir.transposed ? e0 * a.D + row : static_cast<long long>(row) * a.D + e0);
       float2 S[NC / 2];
@@ -653,9 +653,17 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       for (int c = 0; c < NC / 2; ++c) S[c] = make_float2(0.f, 0.f);
       if (carried && one.s_in && in_state) {
         const float* src = one.s_in + st0;
+        const float w = one.dir.in_mult;
 #pragma unroll
-        for (int c = 0; c < NC / 2; ++c, src += 2 * st_step)
-          S[c] = make_float2(one.dir.in_mult * src[0], one.dir.in_mult * src[st_step]);
+        for (int c = 0; c < NC / 4; ++c) {
+          float4 f;
+          if (one.dir.transposed)  // the lanes' values lie side by side
+            f = make_float4(src[4 * c * a.D], src[(4 * c + 1) * a.D], src[(4 * c + 2) * a.D], src[(4 * c + 3) * a.D]);
+          else
+            f = reinterpret_cast<const float4*>(src)[c];
+          S[2 * c] = make_float2(w * f.x, w * f.y);
+          S[2 * c + 1] = make_float2(w * f.z, w * f.w);
+        }
       }
       const int last = x.n > 0 ? (x.n - 1) / a.seg_tokens : 0;  // the segment of the last token
       if (STATES) {
@@ -733,12 +741,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       // the state after the last token in time order
       if (one.s_out && in_state && x.seg == (x.rev ? 0 : last)) {
         const float w = one.dir.out_mult * (one.dir.lead && x.n > 0 ? exp2f(l2) : 1.f);
-        float* dst = one.s_out + st0;
+        float4* dst = reinterpret_cast<float4*>(one.s_out + st0);  // (a transposed state has no output)
 #pragma unroll
-        for (int c = 0; c < NC / 2; ++c, dst += 2 * st_step) {
-          dst[0] = w * S[c].x;
-          dst[st_step] = w * S[c].y;
-        }
+        for (int c = 0; c < NC / 4; ++c)
+          dst[c] = make_float4(w * S[2 * c].x, w * S[2 * c].y, w * S[2 * c + 1].x, w * S[2 * c + 1].y);
       }
       if (!one.dir.accumulate) {  // zeros past the sequence
         const int p1 = a.L - x.p0 < a.seg_tokens ? a.L : x.p0 + a.seg_tokens;
