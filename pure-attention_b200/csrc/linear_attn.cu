@@ -340,6 +340,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   auto kv_at = [&](int g) { return VB == 2 && (g & 1) ? 0u : 384u; };
   constexpr uint32_t T_S = 0, T_QS = 256, T_PV = 320;  // and kv_at
 
+  // The launch that needs these states may set itself up on SMs that are free.
+  if (STATES && threadIdx.x == 0) launch_dependents();
   const int warp = warp_id();
   // Role of a warp of the last warpgroup: 0 MMA issue, 1 loads, 2 and 3 splitting. The issuing warp slows the
   // other warps of its sub-partition (an MMA that waits for the queue holds up their TMEM
@@ -632,6 +634,8 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       return true;
     };
     ok = split_k();
+    // the segments' states: also where there is nothing to do, so that this launch ends after theirs
+    if (!STATES && a.n_seg > 1) wait_prerequisites();
     for (int u = blockIdx.x; ok && u < n_units; u += gridDim.x) {
       const MixUnit x = mix_unit<DK, STATES>(a, u);
       const MixOne& one = a.one[x.dir];
@@ -1087,8 +1091,19 @@ int mix_launch(MixArgs a, const MixMaps& maps, uint32_t* status, cudaStream_t s)
     if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
   }
   if (!ensure_smem_attr(mix_kernel<T, DK, NT, false>, C::SMEM, attr)) return PA_ERR_LAUNCH;
-  mix_kernel<T, DK, NT, false><<<a.n_units < sms ? a.n_units : sms, kMixThreads, C::SMEM, s>>>(a, maps, status);
-  return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+  // After the states' launch this one starts while that one runs (all its blocks are on SMs by then,
+  // so these take none from them) and waits for it where a state is added up.
+  cudaLaunchAttribute early{};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.n_units < sms ? a.n_units : sms);
+  cfg.blockDim = dim3(kMixThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = a.n_seg > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, mix_kernel<T, DK, NT, false>, a, maps, status) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
 // An input [B, L, H, D] as boxes of 128 bytes of columns x 1 head x 128 tokens, bf16 in
