@@ -59,10 +59,21 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // Q and K feed two products each as they lie: K as the K-major B of Q K^T and as the
 // MN-major A of K^T V'.
 //
-// Roundings: fp32 sums and state throughout. V' is two bf16 parts (off by 2^-16), so
-// the states keep fp32-like accuracy; as operands of the output's two products, P and
-// the state entering the chunk are one bf16 each (2^-8), like P in the softmax kernels. NT = 3 (fp32 operands): every operand is a
-// hi/lo pair and every product hi*hi + hi*lo + lo*hi.
+// Roundings: fp32 sums and state throughout. V' is two bf16 parts (off by 2^-17), so a carried
+// state gains an error of 2^-17 of each token's part, not 2^-9 (one part would save a quarter of
+// the products, but a state is read by every later token). As operands of the output's two products,
+// P and the state entering the chunk are one bf16 each (2^-9), as P is in the softmax kernels: the
+// output is rounded to bf16 itself. NT = 3 (fp32 operands): every operand is a hi/lo pair and every
+// product hi*hi + hi*lo + lo*hi (2^-16 in all).
+//
+// What bounds it. 8 x 4096 tokens of 16 heads of 64 in bf16 (268 MB: 41 us at the copy rate) take 58
+// us alone, 4.6 TB/s, 66 us back to back under the power limit. A chunk takes 2900 clocks, and by
+// count 270 KB of it pass the 128 bytes a clock of the SM's shared memory, 2200 clocks: tiles of
+// q, k and v land there, V' is made there in two parts, and the four products read their operands
+// there (but P, from TMEM); 128 of 148 SMs are busy. At head dim 128 a unit is half of V's columns,
+// and each half forms P anew: a state of 128 x 128 would need 128 registers of each of 128 threads.
+// Chunks of fp32 move 700 KB (three products, and tiles split into parts in place), 5400 of 6000
+// clocks. Short calls wait for their own code: the first chunk of a cold launch takes 5 us.
 //
 // TMEM columns: Q K^T and P 2 x 128 (P of 32 tokens over their 32 scores: hi in the
 // first 16 columns, lo in the others), Q S 64, P V 64, K^T [V' hi, V' lo] 128.
@@ -228,7 +239,10 @@ __device__ __forceinline__ void st_shared_v4(uint32_t at, uint32_t a, uint32_t b
 }
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
   uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(at)
+               : "memory");
   return v;
 }
 // Four fp32 values as bf16 hi and, where `lo` is not 0, lo.
@@ -993,7 +1007,9 @@ __global__ void __launch_bounds__(kMixThreads, 1)
 
 // One new token. A block takes 32 columns of a state (sequence, head): 8 lanes a row of
 // 128 bytes, 16 rows a pass, all passes' loads in flight at once. Bound by HBM: the
-// state is read once and written once.
+// state is read once and written once. 64 sequences of 16 heads of 128 (134 MB) take 24.6 us, 5.5
+// TB/s, of 32 heads 39.4 us, 6.8 TB/s; one sequence of 8 heads of 64 2.3 us, less than its
+// launch on the host. Whole states a block (fewer, larger) left SMs idle where users are few.
 constexpr int kStepThreads = 128, kStepCols = 32;
 template <typename T, int D>
 __global__ void __launch_bounds__(kStepThreads)
@@ -1054,20 +1070,21 @@ MixPlan mix_plan(const AttnShape& sh, bool f32, int n_dir) {
   MixPlan p;
   const int chunks = (sh.L + 127) / 128, sms = device_sm_count();
   p.pairs = sh.B * sh.H * n_dir * (sh.D == 128 ? 2 : 1);
-  // Segments for the SMs there are, of 2 chunks at least (fp32, 2 heads, 64 chunks: 36 us with 48
-  // segments, 43 with 64), and so few that adding up their states stays cheap (bf16, 2 heads, 64
-  // chunks: 25 us with 24, 28 with 37; 1024 chunks: 78 with 64, 82 with 74).
+  // Segments for the SMs there are, of 2 chunks at least (2 heads, 64 chunks: fp32 33 us with 32
+  // segments, 40 with 64; bf16 25 and 34), and so few that adding up their states stays cheap (2 heads,
+  // bf16: 64 chunks 23 us with 22 segments, 25 with 32; 1024 chunks 72 with 64, 74 with 74).
   int seg = sms / p.pairs;
   if (seg > chunks / 2) seg = chunks / 2;
   while (seg > 1 && seg * seg > 8 * chunks) --seg;
   // None where the second launch and the second reading of k and v cost more than the chunks that a
-  // sequence no longer waits for. bf16, 2 segments of 4 heads: 8 chunks 19 us whole and 24 cut, 32
-  // chunks 50 and 39; 4 segments of 32 heads: 8 chunks 19 and 22, 16 chunks 30 and 26. A chunk of fp32
-  // takes twice as long: gradients in 2 segments of 16 heads 12 chunks 50 and 54, 16 chunks 63 and 59.
-  if (seg > 1 && chunks - (chunks + seg - 1) / seg < (f32 ? 7 : 9)) seg = 1;
+  // sequence no longer waits for. bf16: 8 heads in 2 segments 8 chunks 18.6 us whole and 19.3 cut, 12
+  // chunks 24.5 and 23.6; 32 heads in 4, 6 chunks 16.5 and 17.2, 8 chunks 18.5 and 17.4. A chunk of
+  // fp32 takes twice as long: 32 heads in 2 segments 6 chunks 30 and 29, 8 chunks 37 and 34.
+  if (seg > 1 && chunks - (chunks + seg - 1) / seg < (f32 ? 3 : 6)) seg = 1;
   if (seg < 1) seg = 1;
   int seg_chunks = (chunks + seg - 1) / seg;
-  // the states' launch has one segment less: cut finer it still fills the GPU
+  // The states' launch has one segment less: cut finer it still fills the GPU (2 x 16384 tokens of 16
+  // heads of 128: 191 us, 220 without).
   p.fine = seg > 1 ? sms / (p.pairs * (seg - 1)) : 1;
   if (p.fine > seg_chunks / 4) p.fine = seg_chunks / 4;
   if (p.fine < 1) p.fine = 1;
@@ -1178,9 +1195,9 @@ int mix(const AttnShape& sh, bool f32, MixArgs a, const float* log_decay, const 
 template <typename T, int D>
 int step(const AttnShape& sh, const void* q, const void* k, const void* v, const float* log_decay,
          const float* s_in, void* o, float* s_out, cudaStream_t s) {
-  mix_step_kernel<T, D><<<sh.B * sh.H * (D / kStepCols), kStepThreads, 0, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
-                                                    static_cast<const T*>(v), log_decay, s_in,
-                                                    static_cast<T*>(o), s_out, sh.H, sh.scale);
+  mix_step_kernel<T, D><<<sh.B * sh.H * (D / kStepCols), kStepThreads, 0, s>>>(
+      static_cast<const T*>(q), static_cast<const T*>(k), static_cast<const T*>(v), log_decay, s_in,
+      static_cast<T*>(o), s_out, sh.H, sh.scale);
   return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 

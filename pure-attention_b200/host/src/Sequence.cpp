@@ -146,7 +146,7 @@ std::pair<std::shared_ptr<Tensor>, std::shared_ptr<Tensor>> linear_attention(
   const pa_attn_desc d = attn_desc(*Q, num_heads);
   int st;
   if (sh[1] == 1 && !g && state && out && !lengths) {
-    // one new token (5.5 us as a chunk of one token against 2.5 us, 8 heads of 64)
+    // one new token (2.3 us; as a chunk of one token 9 us; 8 heads of 64 in fp32)
     st = pa_linear_attn_step(&d, Q->get_data_ptr(), K->get_data_ptr(), V->get_data_ptr(),
                              log_decay->get_data_ptr(), state->get_data_ptr(), O->get_data_ptr(),
                              out->get_data_ptr(), ps(s));
