@@ -174,7 +174,8 @@ PYBIND11_MODULE(PureAttention, m) {
            py::arg("input"), py::arg("positions"), py::arg("lengths") = nullptr)
       .def("forward_state", &layers::LinearAttention::forward_state, py::arg("input"),
            py::arg("positions") = nullptr, py::arg("lengths") = nullptr, py::arg("state") = nullptr,
-           "(output, state after the last token) of a piece of a longer sequence")
+           "(output, state after the last token) of a piece of a longer sequence; for generation with "
+           "set_grad_enabled(False), which also takes the single-token kernel")
       .def("parameters", &layers::LinearAttention::parameters);
 
   py::class_<layers::LayerNorm, layers::Module, std::shared_ptr<layers::LayerNorm>>(m, "LayerNorm")
@@ -213,6 +214,12 @@ PYBIND11_MODULE(PureAttention, m) {
     return c;
   }, "Element-wise addition (a [1, N] second operand is broadcast over rows)", py::arg("a"),
         py::arg("b"));
+
+  m.def("set_grad_enabled", &core::set_grad_enabled,
+        "Whether the calling thread's operators record graph nodes from now on (default True). Off for "
+        "inference: a carried state then holds nothing of the tokens before it. Not in the reference.",
+        py::arg("on"));
+  m.def("grad_enabled", &core::grad_enabled);
 
   m.def("set_float32_math", [](const std::string& mode) {
     int m_ = -1;

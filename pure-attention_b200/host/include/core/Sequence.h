@@ -45,7 +45,7 @@ std::pair<std::shared_ptr<Tensor>, std::shared_ptr<Tensor>> rope(
 // Causal linear attention of Q, K, V [N, L, E] with decay exp(log_decay[h]) (a constant [H]; no
 // gradient), over the first lengths[n] tokens of each sequence (null: all), from
 // state [N, H, D, D] (null: zero). Returns {O, the state after the last token};
-// the second is null unless want_state. One new token without gradients
+// the second is null unless want_state. One new token without gradients (set_grad_enabled)
 // takes the single-token kernel.
 std::pair<std::shared_ptr<Tensor>, std::shared_ptr<Tensor>> linear_attention(
     const std::shared_ptr<Tensor>& Q, const std::shared_ptr<Tensor>& K,

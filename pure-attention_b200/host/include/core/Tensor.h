@@ -87,6 +87,12 @@ class Tensor : public std::enable_shared_from_this<Tensor> {
   std::shared_ptr<Function> grad_function;
 };
 
+// Whether the calling thread's operators record graph nodes (at first they do). Off, their
+// outputs need no gradient and hold no inputs: a state carried from token to token would
+// otherwise hold the graph of all tokens before it. Not in the reference.
+void set_grad_enabled(bool on);
+bool grad_enabled();
+
 // Throws std::runtime_error("<what>: <status string>") for a non-zero pa_status.
 void check_status(int status, const char* what);
 }  // namespace core

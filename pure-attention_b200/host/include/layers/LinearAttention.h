@@ -20,7 +20,8 @@ class LinearAttention : public Module {
                                         const std::shared_ptr<core::IntTensor>& positions,
                                         const std::shared_ptr<core::IntTensor>& lengths);
   // A piece of a longer sequence (a prompt, a single new token): from state [N, H, D, D]
-  // (null: the start) to {output, state after it}.
+  // (null: the start) to {output, state after it}. Generation turns set_grad_enabled off: with it
+  // on, the state keeps the graph of every piece before it, to be trained through.
   std::pair<std::shared_ptr<core::Tensor>, std::shared_ptr<core::Tensor>> forward_state(
       const std::shared_ptr<core::Tensor>& input, const std::shared_ptr<core::IntTensor>& positions,
       const std::shared_ptr<core::IntTensor>& lengths, const std::shared_ptr<core::Tensor>& state);

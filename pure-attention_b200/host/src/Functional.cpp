@@ -104,7 +104,7 @@ void linear(const std::shared_ptr<Tensor>& A, const std::shared_ptr<Tensor>& W,
   if (num_parts < 1 || num_parts > 3 || N % num_parts || (relu && num_parts != 1))
     throw std::runtime_error("Linear: 1 to 3 parts, dividing the output dimension");
   const int M = static_cast<int>(A->numel() / K);
-  const bool g = A->requires_grad() || W->requires_grad() || bias->requires_grad();
+  const bool g = grad_enabled() && (A->requires_grad() || W->requires_grad() || bias->requires_grad());
   auto ps_ = a;
   ps_.back() = static_cast<uint32_t>(N / num_parts);
   std::vector<std::shared_ptr<Tensor>> mine;

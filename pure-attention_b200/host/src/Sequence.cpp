@@ -67,7 +67,7 @@ std::pair<std::shared_ptr<Tensor>, std::shared_ptr<Tensor>> rope(
   if (!positions || positions->get_shape() !=
                         std::vector<uint32_t>{static_cast<uint32_t>(spec.sections.size()), q[0], q[1]})
     throw std::runtime_error("Rope: positions must be [axes, N, L]");
-  const bool g = Q->requires_grad() || K->requires_grad();
+  const bool g = grad_enabled() && (Q->requires_grad() || K->requires_grad());
   auto Qo = std::make_shared<Tensor>(q, g, false);
   auto Ko = std::make_shared<Tensor>(k, g, false);
   const pa_rope_desc d = rope_desc(q, static_cast<int>(q[2]) / head_dim,
@@ -138,8 +138,8 @@ std::pair<std::shared_ptr<Tensor>, std::shared_ptr<Tensor>> linear_attention(
   const std::vector<uint32_t> state_shape{sh[0], H, D, D};
   if (state && state->get_shape() != state_shape)
     throw std::runtime_error("LinearAttention: the state must be [N, H, D, D]");
-  const bool g = Q->requires_grad() || K->requires_grad() || V->requires_grad() ||
-                 (state && state->requires_grad());
+  const bool g = grad_enabled() && (Q->requires_grad() || K->requires_grad() || V->requires_grad() ||
+                                    (state && state->requires_grad()));
   auto O = std::make_shared<Tensor>(sh, g, false);
   std::shared_ptr<Tensor> out;
   if (want_state) out = std::make_shared<Tensor>(state_shape, g, false);

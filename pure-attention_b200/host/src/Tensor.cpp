@@ -24,8 +24,14 @@ static float32_t* device_alloc(size_t n, cudaStream_t s) {
   return static_cast<float32_t*>(p);
 }
 
+namespace {
+thread_local bool recording = true;
+}
+void set_grad_enabled(bool on) { recording = on; }
+bool grad_enabled() { return recording; }
+
 Tensor::Tensor(const std::vector<uint32_t>& shape_, bool requires_gradient_, bool is_leaf_)
-    : shape(shape_), requires_gradient(requires_gradient_), is_leaf(is_leaf_) {
+    : shape(shape_), requires_gradient(requires_gradient_ && (is_leaf_ || recording)), is_leaf(is_leaf_) {
   size = 1;
   for (uint32_t s : shape) size *= s;
   const cudaStream_t s = CudaContext::getStream();
@@ -94,6 +100,7 @@ std::vector<float32_t> Tensor::grad_to_host() const {
 }
 
 void Tensor::set_grad_fn(std::shared_ptr<Function> fn) {
+  if (!recording) return;
   grad_function = std::move(fn);
   is_leaf = false;
 }

@@ -233,3 +233,50 @@ def test_host_refusals(pa):
         pa.LinearAttention(64, 1, sections=[8]).forward(x)
     with pytest.raises(RuntimeError, match="fill the shape"):
         pa.IntTensor([2, 2], [1, 2, 3])
+
+
+@pytest.fixture
+def no_graph(pa):
+    pa.set_grad_enabled(False)
+    yield
+    pa.set_grad_enabled(True)
+
+
+@pytest.mark.gpu
+def test_generation_without_a_graph(pa, no_graph):
+    """With the graph off a layer whose parameters have gradients generates token by token: the same values,
+    and neither the output nor the state has a graph behind it."""
+    N, E, H, sections = 1, 128, 2, [32]
+    layer = pa.LinearAttention(E, H, [-0.01, -0.3], sections)
+    x = seeded_normal(50, (N, 300, E))
+    pos = np.arange(300, dtype=np.int32).reshape(1, 1, 300)
+    w = [torch.from_numpy(_h(p)) for p in layer.parameters()]
+    want, ws = _layer_ref(torch.from_numpy(x).double(), w, H, torch.tensor([-0.01, -0.3]), torch.from_numpy(pos),
+                          sections)
+    out, state = [], None
+    for a, b in ((0, 200), *((i, i + 1) for i in range(200, 300))):
+        y, state = layer.forward_state(_t(pa, x[:, a:b]), _ints(pa, pos[:, :, a:b]), None, state)
+        out.append(_h(y))
+    assert rel_err(np.concatenate(out, 1), want) < TOL
+    assert rel_err(_h(state), ws) < TOL
+    for t in (y, state):
+        with pytest.raises(RuntimeError, match="does not require"):
+            t.backward()
+
+
+@pytest.mark.gpu
+def test_one_token_takes_the_single_token_kernel_without_a_graph(pa):
+    """Tensors that need gradients give the bits of tensors that need none once the graph is off."""
+    ld, s = _t(pa, np.array([-0.1, -0.4], np.float32)), seeded_normal(60, (2, 2, 64, 64))
+    qkv = [seeded_normal(61 + i, (2, 1, 128)) for i in range(3)]
+    plain = pa.linear_attention(*(_t(pa, x) for x in qkv), 2, ld, None, _t(pa, s), True)
+    assert pa.grad_enabled()
+    pa.set_grad_enabled(False)
+    try:
+        off = pa.linear_attention(*(_t(pa, x, True) for x in qkv), 2, ld, None, _t(pa, s, True), True)
+    finally:
+        pa.set_grad_enabled(True)
+    on = pa.linear_attention(*(_t(pa, x, True) for x in qkv), 2, ld, None, _t(pa, s, True), True)
+    for a, b, c in zip(plain, off, on):
+        assert np.array_equal(_h(a), _h(b))
+        assert rel_err(_h(c), _h(a)) < TOL
