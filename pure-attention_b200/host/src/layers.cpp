@@ -109,9 +109,17 @@ std::vector<std::shared_ptr<core::Tensor>> MultiheadAttention::parameters() {
   return {in_proj_weight, in_proj_bias, out_proj_weight, out_proj_bias};
 }
 
+namespace {
+uint32_t dividing(uint32_t e, uint32_t h) {
+  if (h == 0 || e == 0 || e % h)
+    throw std::runtime_error("LinearAttention: embedding dim not divisible by num_heads");
+  return e;
+}
+}  // namespace
+
 LinearAttention::LinearAttention(uint32_t e, uint32_t h, const std::vector<float>& decay,
                                  const core::RopeSpec& rope)
-    : in_proj_weight(param({e, 3 * e})),
+    : in_proj_weight(param({dividing(e, h), 3 * e})),
       in_proj_bias(param({1, 3 * e})),
       out_proj_weight(param({e, e})),
       out_proj_bias(param({1, e})),

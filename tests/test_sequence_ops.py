@@ -145,3 +145,10 @@ def test_linear_attention_scale_refusals(scale):
                                   256, big, None) == SHAPE
     assert lib.pa_linear_attn_step(_desc(L=1, scale=scale), 16, 32, 48, 64, 80, 96, 112, None) == SHAPE
     assert lib.pa_linear_attn_fwd_workspace_size(_desc(L=9000, scale=scale)) == 0
+
+
+@pytest.mark.parametrize("e,h", [(64, 0), (0, 1), (64, 3)])
+def test_layer_refuses_heads_that_do_not_divide(e, h):
+    import PureAttention
+    with pytest.raises(RuntimeError, match="not divisible"):
+        PureAttention.LinearAttention(e, h, sections=[4])
