@@ -339,15 +339,33 @@ def rope_bwd(dq_out, dk_out, positions, dq, dk, desc, accumulate=False, stream=N
 
 _STATES = {2: ("state_in", "state_out"), 3: ("state_in", "d_state_out", "d_state_in")}
 
+# Descriptors and workspace sizes by shape: making them costs a short call as much as a check of its
+# arguments.
+_linear_attn_descs, _linear_attn_sizes = {}, {}
+
+
+def _kept(cache, key, make):
+    got = cache.get(key)
+    if got is None:
+        if len(cache) >= 4096:
+            cache.clear()
+        got = cache[key] = make()
+    return got
+
+
+def _linear_attn_desc(fn, d, q):
+    """The descriptor of a call: its own, which has to be q's, or q's."""
+    if d is None:
+        return _kept(_linear_attn_descs, (q.shape, q.dtype), lambda: attn_desc(q))
+    if q.shape != (d.batch, d.seq_len, d.num_heads, d.head_dim) or d.dtype != _dtype_code(q):
+        raise ValueError(f"{fn}: q must be [B, L, H, D] and the descriptor its own")
+    return d
+
 
 def _check_linear_attn(fn, d, q, log_decay, seq_lens, names, tensors, states):
     import torch
-    shape = q.shape
-    if shape != (d.batch, d.seq_len, d.num_heads, d.head_dim) or d.dtype != _dtype_code(q):
-        raise ValueError(f"{fn}: q must be [B, L, H, D] and the descriptor its own")
-    B, _, H, D = shape
-    dev = q.get_device()
-    _check_tensors(fn, dev, q.dtype, shape, names, *tensors)
+    dtype, dev, B, H, D = q.dtype, q.get_device(), d.batch, d.num_heads, d.head_dim
+    _check_tensors(fn, dev, dtype, q.shape, names, *tensors)
     _check_tensors(fn, dev, torch.float32, (B, H, D, D), _STATES[len(states)], *states)
     _check_tensors(fn, dev, torch.float32, (H,), ("log_decay",), log_decay)
     if seq_lens is not None:
@@ -355,16 +373,11 @@ def _check_linear_attn(fn, d, q, log_decay, seq_lens, names, tensors, states):
     _check_device(fn, q, dev)
 
 
-# Workspace sizes by shape: a query costs a short call as much as a check of its arguments.
-_linear_attn_sizes = {}
-
-
 def _linear_attn_ws(size_of, d, workspace, q, stream):
     if workspace is None:
-        key = (size_of, d.batch, d.seq_len, d.num_heads, d.head_dim, d.dtype, q.get_device())
-        need = _linear_attn_sizes.get(key)
-        if need is None:
-            need = _linear_attn_sizes[key] = size_of(d)
+        # (the scale: a descriptor that the call refuses needs 0 bytes)
+        need = _kept(_linear_attn_sizes, (size_of, q.shape, q.dtype, q.get_device(), d.softmax_scale),
+                     lambda: size_of(d))
         if need == 0:
             return None, 0
         import torch
@@ -383,7 +396,7 @@ def linear_attn_fwd(q, k, v, log_decay, o, seq_lens=None, state_in=None, state_o
     """o = causal linear attention of q, k, v [B, L, H, D] with decay exp(log_decay[h]), from
     state_in to state_out ([B, H, D, D] fp32, either may be None) over seq_lens (int32 [B])
     tokens of each sequence. A workspace is allocated with torch unless given."""
-    d = desc or attn_desc(q)
+    d = _linear_attn_desc("linear_attn_fwd", desc, q)
     _check_linear_attn("linear_attn_fwd", d, q, log_decay, seq_lens, ("q", "k", "v", "o"), (q, k, v, o),
                        (state_in, state_out))
     ws, nb = _linear_attn_ws(linear_attn_fwd_workspace_size, d, workspace, q, stream)
@@ -401,7 +414,7 @@ def linear_attn_bwd(q, k, v, dO, log_decay, dq, dk, dv, seq_lens=None, state_in=
                     stream=None):
     """Gradients dq, dk, dv (overwritten, or added to) and d_state_in of linear_attn_fwd from dO
     and d_state_out (None: zero)."""
-    d = desc or attn_desc(q)
+    d = _linear_attn_desc("linear_attn_bwd", desc, q)
     _check_linear_attn("linear_attn_bwd", d, q, log_decay, seq_lens, ("q", "k", "v", "dO", "dq", "dk", "dv"),
                        (q, k, v, dO, dq, dk, dv), (state_in, d_state_out, d_state_in))
     ws, nb = _linear_attn_ws(linear_attn_bwd_workspace_size, d, workspace, q, stream)
@@ -415,7 +428,7 @@ def linear_attn_bwd(q, k, v, dO, log_decay, dq, dk, dv, seq_lens=None, state_in=
 def linear_attn_step(q, k, v, log_decay, state_in, o, state_out, desc=None, stream=None):
     """One new token of each sequence (q, k, v, o [B, 1, H, D]): state_out = decay * state_in +
     k v^T, o = scale q state_out; state_out may be state_in."""
-    d = desc or attn_desc(q)
+    d = _linear_attn_desc("linear_attn_step", desc, q)
     _check_linear_attn("linear_attn_step", d, q, log_decay, None, ("q", "k", "v", "o"), (q, k, v, o),
                        (state_in, state_out))
     _check("pa_linear_attn_step", load().pa_linear_attn_step(

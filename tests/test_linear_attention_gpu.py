@@ -417,3 +417,13 @@ def test_workspace_of_a_call_on_a_stream_given_by_its_handle():
             torch.full((1 << 22,), float("nan"), device="cuda")  # would take a freed workspace of its own stream
         st.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.gpu
+def test_a_refused_scale_does_not_change_the_workspace_of_later_calls():
+    import pa_capi
+    q, k, v, _, ld, _, _ = _inputs(1, 4100, 2, 64, torch.bfloat16, 94)
+    with pytest.raises(pa_capi.PaError):
+        _forward(q, k, v, ld, desc=pa_capi.attn_desc(q, scale=1e-30))
+    _check_forward(q, k, v, ld)
+    assert pa_capi.linear_attn_fwd_workspace_size(pa_capi.attn_desc(q)) > 0
