@@ -56,8 +56,8 @@ typedef struct pa_attn_desc {
 } pa_attn_desc;
 
 /* Arithmetic of the fp32 entry points (pa_matmul*, pa_linear_*, and
- * pa_attn_fwd / pa_attn_bwd with dtype PA_F32 and head_dim 64), set per
- * calling thread:
+ * pa_attn_fwd / pa_attn_bwd with dtype PA_F32 and head_dim 64, and
+ * pa_linear_attn_fwd / _bwd with dtype PA_F32), set per calling thread:
  *   PA_F32_MATH_SPLIT3 (default): operands split into bf16 hi/lo planes and
  *     every product taken as hi*hi + hi*lo + lo*hi (fp32-level accuracy,
  *     within 1e-3 of float64 where the reference computes in fp32);
