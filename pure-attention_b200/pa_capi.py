@@ -384,6 +384,10 @@ def _linear_attn_ws(size_of, d, workspace, q, stream):
         # memory of the stream that will use it: the allocator orders its reuse there
         with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif workspace.get_device() != q.get_device():
+        raise ValueError(f"linear attention: workspace must be on {q.device}, not {workspace.device}")
+    elif not workspace.is_contiguous():  # an expanded view counts bytes that its memory does not have
+        raise ValueError("linear attention: workspace must be contiguous")
     return workspace, workspace.numel() * workspace.element_size()
 
 

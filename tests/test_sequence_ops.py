@@ -152,3 +152,32 @@ def test_layer_refuses_heads_that_do_not_divide(e, h):
     import PureAttention
     with pytest.raises(RuntimeError, match="not divisible"):
         PureAttention.LinearAttention(e, h, sections=[4])
+
+
+def test_binding_refuses_workspaces_that_the_kernel_must_not_write():
+    """A workspace of another device, or a view that counts more bytes than its memory holds, is
+    refused like any other tensor of the call, before the library sees it."""
+    torch = pytest.importorskip("torch")
+    import pa_capi
+
+    class OnGpu:  # what the helper asks of q
+        shape, dtype, device = (1, 4100, 2, 64), torch.bfloat16, "cuda:0"
+
+        def __init__(self, index):
+            self.index = index
+
+        def get_device(self):
+            return self.index
+
+    d = pa_capi.AttnDesc(1, 4100, 2, 64, pa_capi.PA_BF16, 0.0)
+    plain = torch.empty(1 << 22, dtype=torch.uint8)
+    view = torch.empty(1, dtype=torch.uint8).expand(1 << 22)
+    strided = torch.empty(1 << 12, dtype=torch.uint8)[::2]
+    for size_of in (pa_capi.linear_attn_fwd_workspace_size, pa_capi.linear_attn_bwd_workspace_size):
+        for ws in (plain, torch.empty(1 << 22, dtype=torch.uint8, device="meta")):
+            with pytest.raises(ValueError, match="workspace must be on"):
+                pa_capi._linear_attn_ws(size_of, d, ws, OnGpu(0), None)
+        for ws in (view, strided):
+            with pytest.raises(ValueError, match="workspace must be contiguous"):
+                pa_capi._linear_attn_ws(size_of, d, ws, OnGpu(-1), None)
+        assert pa_capi._linear_attn_ws(size_of, d, plain, OnGpu(-1), None) == (plain, 1 << 22)
