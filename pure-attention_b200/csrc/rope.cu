@@ -85,10 +85,9 @@ struct RopeSplit {
 // heads in fp32 85, 63, 66 and 63 us, 2 x 1177 tokens of 32 + 8 heads in bf16 17, 15, 14 and 14 us.
 constexpr int kRopeUnroll = 4;
 template <typename T, int V, bool HALVES, bool ACC>
-__global__ void __launch_bounds__(kRopeThreads)
-    rope_kernel(const T* __restrict__ q, const T* __restrict__ k, T* qo, T* ko,
-                const int32_t* __restrict__ pos, const __grid_constant__ RopeTable tab, int P, int D,
-                int Hq, int Hk, long long n_tok, const RopeSplit split, float sign) {
+__device__ __forceinline__ void rope_tokens(const T* q, const T* k, T* qo, T* ko, const int32_t* __restrict__ pos,
+                                            const RopeTable& tab, int P, int D, int Hq, int Hk, long long n_tok,
+                                            const RopeSplit split, float sign) {
   // 2 x (cos [T][P], sin [T][P]): one sync a tile; apart, so that the lanes of a head read
   // whole 16-byte vectors from different banks
   extern __shared__ __align__(16) float tables[];
@@ -202,6 +201,25 @@ __global__ void __launch_bounds__(kRopeThreads)
   }
 }
 
+// Outputs apart from the inputs: loads and stores may pass one another (8 x 4096 tokens of 16 + 16
+// heads of 64 in bf16, pairs side by side: 45 us, 51 without __restrict__).
+template <typename T, int V, bool HALVES, bool ACC>
+__global__ void __launch_bounds__(kRopeThreads)
+    rope_kernel(const T* __restrict__ q, const T* __restrict__ k, T* __restrict__ qo, T* __restrict__ ko,
+                const int32_t* __restrict__ pos, const __grid_constant__ RopeTable tab, int P, int D,
+                int Hq, int Hk, long long n_tok, const RopeSplit split, float sign) {
+  rope_tokens<T, V, HALVES, ACC>(q, k, qo, ko, pos, tab, P, D, Hq, Hk, n_tok, split, sign);
+}
+
+// qo is q, or ko is k: a thread has loaded each value before it stores its turn.
+template <typename T, int V, bool HALVES>
+__global__ void __launch_bounds__(kRopeThreads)
+    rope_in_place_kernel(const T* q, const T* k, T* qo, T* ko, const int32_t* __restrict__ pos,
+                         const __grid_constant__ RopeTable tab, int P, int D, int Hq, int Hk, long long n_tok,
+                         const RopeSplit split, float sign) {
+  rope_tokens<T, V, HALVES, false>(q, k, qo, ko, pos, tab, P, D, Hq, Hk, n_tok, split, sign);
+}
+
 template <typename T, int V>
 void rope_launch(const RopeShape& sh, const void* q, const void* k, void* qo, void* ko,
                  const int32_t* pos, const RopeTable& tab, bool inverse, bool accumulate, cudaStream_t s) {
@@ -221,6 +239,7 @@ void rope_launch(const RopeShape& sh, const void* q, const void* k, void* qo, vo
   const unsigned grid = static_cast<unsigned>(tiles < blocks ? tiles : blocks);
   const size_t smem = 4 * static_cast<size_t>(split.T) * sh.pairs * sizeof(float);
   const float sign = inverse ? -1.f : 1.f;
+  const bool in_place = qo == q || (sh.Hk > 0 && ko == k);  // (never with accumulate)
   auto go = [&](auto kernel) {
     kernel<<<grid, kRopeThreads, smem, s>>>(static_cast<const T*>(q), static_cast<const T*>(k),
                                             static_cast<T*>(qo), static_cast<T*>(ko), pos, tab,
@@ -228,9 +247,11 @@ void rope_launch(const RopeShape& sh, const void* q, const void* k, void* qo, vo
   };
   if (sh.halves) {
     if (accumulate) go(rope_kernel<T, V, true, true>);
+    else if (in_place) go(rope_in_place_kernel<T, V, true>);
     else go(rope_kernel<T, V, true, false>);
   } else {
     if (accumulate) go(rope_kernel<T, V, false, true>);
+    else if (in_place) go(rope_in_place_kernel<T, V, false>);
     else go(rope_kernel<T, V, false, false>);
   }
 }

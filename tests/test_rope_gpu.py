@@ -145,3 +145,22 @@ def test_rope_past_2_31_values():
     want = turn(tail, pos[:, :, -90:], [32])
     _check(q[:, -90:], tail, want, [32], "halves")
     assert not q[:, :-90].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D,sections", [(64, [8, 16]), (128, [64]), (50, [3, 7]), (7, [2])])
+def test_rope_in_place_in_every_form(dtype, layout, D, sections):
+    """Whole vectors and single values, forward and gradient: an output over its own input gives the bits
+    of one beside it. 19 heads in all: a thread takes several groups of them, one after another."""
+    import pa_capi
+    q, pos = _data(2, 290, 16, D, dtype, len(sections), 3000, 10)
+    k, _ = _data(2, 290, 3, D, dtype, 1, 2, 11)
+    desc = pa_capi.rope_desc(q, k, sections, layout=layout)
+    for turn_by in (pa_capi.rope_fwd, pa_capi.rope_bwd):
+        qo, ko = torch.empty_like(q), torch.empty_like(k)
+        turn_by(q, k, pos, qo, ko, desc)
+        a, b = q.clone(), k.clone()
+        turn_by(a, b, pos, a, b, desc)
+        assert torch.equal(a, qo) and torch.equal(b, ko)
