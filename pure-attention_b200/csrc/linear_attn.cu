@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   constexpr int NP = C::NP, KT = C::KT;
   constexpr bool BF16 = sizeof(T) == 2;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[34];  // N_BARS
+  __shared__ uint64_t bars[35];  // N_BARS
   __shared__ __align__(16) float wtab[4 * 64 + 4 * 32];  // powers of the decay, a table for each P warp
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   auto sQ = [&](int s) { return sm0 + s * 2 * C::OPER + C::OPER; };
   auto sV = [&](int s) { return sv0 + s * C::V_STAGE; };
   enum { QK_FULL = 0, QK_EMPTY = 3, V_FULL = 6, V_EMPTY = 10, S_FULL = 14, P_FULL = 16, VP_FULL = 18, VP_EMPTY = 20,
-         KV_FULL = 22, KV_FREE = 24, ST_FULL = 26, ST_EMPTY, O_FULL, O_FREE, QK_RAW = 30, V_RAW = 32, N_BARS = 34 };
+         KV_FULL = 22, KV_FREE = 24, ST_FULL = 26, ST_EMPTY, O_FULL, O_FREE, QK_RAW = 30, V_RAW = 32, MMA_DONE = 34, N_BARS };
   // Segment states: V' and K^T V' twice, in what Q and its scores do not use there.
   constexpr int VB = STATES ? 2 : 1;
   constexpr uint32_t VP_LO2 = C::OPER >= 2 * kTile ? kTile : 2 * C::OPER;  // hi to lo in the second V'
@@ -364,6 +364,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
   const int role = warp < 16 ? -1 : (warp - 16 + (a.n_dir == 1 ? 0 : 1)) & 3;
   // One thread loads, all tiles by TMA.
   const bool loads = role == 1 && lane_id() == 0;
+  int n_qk = 0, n_v = 0;  // chunks whose tiles it has sent for
   auto load = [&](const ChunkIter<DK, STATES>& it) {
     const int g = it.g, s = g % C::QKS, vs = g % C::VS;
     const MixOne& one = a.one[it.x.dir];
@@ -377,6 +378,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       tma_load_4d(sK(s) + tile * kTile, &maps.m[one.mk], qk, tile * COLS, h, tok, b);
       if (!STATES) tma_load_4d(sQ(s) + tile * kTile, &maps.m[one.mq], qk, tile * COLS, h, tok, b);
     }
+    ++n_qk;
     if (BF16) {
       if (g >= C::VS && !mbar_wait(bar(V_EMPTY + vs), (g / C::VS - 1) & 1, status)) return false;
       mbar_arrive_expect_tx(bar(V_FULL + vs), kTile);
@@ -388,6 +390,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
       tma_load_4d(vp_at(g), &maps.m[one.mv], raw, 0, h, tok, b);
       tma_load_4d(vp_at(g) + vp_lo(g), &maps.m[one.mv], raw, COLS, h, tok, b);
     }
+    ++n_v;
     return true;
   };
   ChunkIter<DK, STATES> load_it;
@@ -417,6 +420,7 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     mbar_init(bar(ST_EMPTY), 1);
     mbar_init(bar(O_FULL), 1);
     mbar_init(bar(O_FREE), 8);
+    mbar_init(bar(MMA_DONE), 1);
     fence_mbar_init();
     load_more = load_it.first(a, a.n_units);
     if (load_more) {
@@ -880,16 +884,13 @@ __global__ void __launch_bounds__(kMixThreads, 1)
     if (loads) {
       if (abort_flag) load_more = false;
       while (load_more && load(load_it)) load_more = load_it.next(a);
-      // After a failure nobody waits for what is still on its way: it must land before the block ends.
-      auto landed = [&](int first, int ring) {
-        for (int g = load_it.g < ring ? 0 : load_it.g - ring; g <= load_it.g; ++g)
-          mbar_drain(bar(first + g % ring), (g / ring) & 1);
+      // What is still on its way must land before the block ends, also where a failure, here or in another
+      // block and at any moment, lets the other roles leave without waiting for it.
+      auto landed = [&](int first, int ring, int n) {
+        for (int g = n < ring ? 0 : n - ring; g < n; ++g) mbar_drain(bar(first + g % ring), (g / ring) & 1);
       };
-      if (aborted(status)) {
-        landed(BF16 ? QK_FULL : QK_RAW, C::QKS);
-        if (BF16) landed(V_FULL, C::VS);
-        else landed(V_RAW, VB);
-      }
+      landed(BF16 ? QK_FULL : QK_RAW, C::QKS, n_qk);
+      landed(BF16 ? V_FULL : V_RAW, BF16 ? C::VS : VB, n_v);
     }
   } else if (role >= 2) {
     // ------------------------------------------------------------ fp32: split q in place (segment states: k)
@@ -993,6 +994,10 @@ __global__ void __launch_bounds__(kMixThreads, 1)
                         v.at((term == 1 ? kTile : 0) + mn(k)).d, idV, (term > 0 || k > 0) ? 1u : 0u);
         umma_commit(bar(V_EMPTY + vs));
         umma_commit(bar(O_FULL));
+      }
+      if (total > 0) {  // as with the copies: no product reads tiles or writes TMEM that the block gives up
+        umma_commit(bar(MMA_DONE));
+        mbar_drain(bar(MMA_DONE), 0);
       }
     }
   }

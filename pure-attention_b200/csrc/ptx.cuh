@@ -102,9 +102,9 @@ __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, uint32_
   return mbar_wait_for(bar, parity, status, PA_WAIT_NS);
 }
 
-// Waits for a phase whether or not an error was recorded (copies in flight must
-// land before their shared memory is given up), for 20 ms at most: a phase that
-// nothing was issued for never completes.
+// Waits for a phase whether or not an error was recorded: copies and products in
+// flight must end before their memory is given up. They do by themselves, so this is for phases
+// that something was issued for; 20 ms at most all the same.
 __device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
   const uint64_t t0 = globaltimer();
   while (!mbar_try_wait(bar, parity) && globaltimer() - t0 < 20000000ull) {

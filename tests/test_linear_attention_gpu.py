@@ -427,3 +427,38 @@ def test_a_refused_scale_does_not_change_the_workspace_of_later_calls():
         _forward(q, k, v, ld, desc=pa_capi.attn_desc(q, scale=1e-30))
     _check_forward(q, k, v, ld)
     assert pa_capi.linear_attn_fwd_workspace_size(pa_capi.attn_desc(q)) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+@pytest.mark.parametrize("B,L,H", [(1, 100, 2), (2, 900, 3), (1, 4100, 2), (61, 270, 5)])
+def test_calls_after_a_recorded_error_end_at_once(dtype, D, B, L, H):
+    """While an error of an earlier wait is recorded, a call waits for the copies that its blocks have already sent
+    for and for nothing else: it ends within a few milliseconds (a wait for a copy that was never sent takes
+    20), leaves its outputs as they were, and the same call is right once the error is cleared."""
+    import pa_capi
+    q, k, v, dO, ld, s, ds = _inputs(B, L, H, D, dtype, 95, states=True)
+    want = (*_forward(q, k, v, ld, state_in=s), *(torch.empty_like(q) for _ in range(3)), torch.empty_like(s))
+
+    def call(o, so, dq, dk, dv, dsi):
+        pa_capi.linear_attn_fwd(q, k, v, ld, o, state_in=s, state_out=so)
+        pa_capi.linear_attn_bwd(q, k, v, dO, ld, dq, dk, dv, state_in=s, d_state_out=ds, d_state_in=dsi)
+
+    call(*want)
+    out = [torch.full_like(x, float("nan")) for x in want]
+    torch.cuda.synchronize()
+    pa_capi.wait_selftest(1_000_000, arrive=False)
+    try:
+        assert pa_capi.device_status(clear=False) == 6
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call(*out)
+        b.record()
+        torch.cuda.synchronize()
+        assert a.elapsed_time(b) < 10
+        assert all(torch.isnan(x).all() for x in out)
+    finally:
+        assert pa_capi.device_status(clear=True) == 6
+    call(*out)
+    assert pa_capi.device_status() == 0
+    assert all(torch.equal(x, w) for x, w in zip(out, want))
