@@ -177,8 +177,9 @@ typedef struct pa_rope_desc {
 
 /* q_out = turn(q) [B, L, num_heads, D], k_out = turn(k) [B, L, num_kv_heads, D];
  * positions is a device array [axes, B, L] of any int32 values. q_out may be q
- * and k_out k (in place); other overlaps are not allowed (PA_ERR_SHAPE where the
- * pointers show one). q and k may be the same tensor if neither is an output. */
+ * and k_out k (in place); an output that shares any other byte with an input or
+ * with the other output is refused (PA_ERR_SHAPE). q and k may be the same tensor if
+ * neither is an output. */
 int pa_rope_fwd(const pa_rope_desc* desc, const void* q, const void* k, const int32_t* positions,
                 void* q_out, void* k_out, pa_stream_t stream);
 /* Its adjoint, the turn by the negative angles: dq (overwritten, or added to
@@ -206,7 +207,9 @@ int pa_rope_bwd(const pa_rope_desc* desc, const void* dq_out, const void* dk_out
  * Values of valid tokens and states are finite: an infinity or NaN there may
  * show in outputs of other tokens of its sequence and head, earlier ones too.
  * A workspace belongs to one call at a time: calls that may overlap on the GPU,
- * and graphs that may, need one each. */
+ * and graphs that may, need one each. An output or a workspace that shares bytes
+ * with an input or with another of them is refused (PA_ERR_SHAPE), but for a
+ * state that is updated in place. */
 size_t pa_linear_attn_fwd_workspace_size(const pa_attn_desc* desc);
 int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, const void* v,
                        const float* log_decay, const int32_t* seq_lens, const float* state_in,

@@ -3,6 +3,7 @@
 // translation units.
 #include <cmath>
 #include <cstdio>
+#include <initializer_list>
 #include "attn_common.cuh"
 #include "host_launchers.h"
 
@@ -216,6 +217,25 @@ int pa_attn_delta(const pa_attn_desc* desc, const void* dO, const void* o, float
 
 // ------------------------------------------------------------------ rotary positions, linear attention
 namespace {
+// The bytes of one tensor of a call (none where it is NULL).
+struct Span {
+  uintptr_t at;
+  size_t n;
+  Span(const void* p, size_t bytes) : at(reinterpret_cast<uintptr_t>(p)), n(p ? bytes : 0) {}
+  bool meets(const Span& o) const { return n && o.n && at < o.at + o.n && o.at < at + n; }
+};
+// Whether no output shares a byte with an input or with another output: one that does would be
+// written while it is still read, by blocks in no order.
+bool apart(std::initializer_list<Span> out, std::initializer_list<Span> in) {
+  for (const Span* a = out.begin(); a != out.end(); ++a) {
+    for (const Span& b : in)
+      if (a->meets(b)) return false;
+    for (const Span* b = a + 1; b != out.end(); ++b)
+      if (a->meets(*b)) return false;
+  }
+  return true;
+}
+
 // Validates a rope descriptor and the pointers of one call; fills `sh`.
 int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_t* positions,
                const void* qo, const void* ko, pa::RopeShape* sh) {
@@ -245,8 +265,12 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
   if (!aligned16(q) || !aligned16(qo) || (d->num_kv_heads > 0 && (!aligned16(k) || !aligned16(ko))))
     return PA_ERR_ALIGN;
   if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0) return PA_ERR_ALIGN;
-  // in place is one tensor's turn over itself, not over the other's
-  if (d->num_kv_heads > 0 && (qo == ko || qo == k || ko == q)) return PA_ERR_SHAPE;
+  // in place is one tensor's turn over the whole of itself
+  const size_t head = static_cast<size_t>(tokens) * d->head_dim * (d->dtype == PA_F32 ? 4 : 2);
+  const size_t nq = d->num_heads * head, nk = d->num_kv_heads * head;
+  if (!apart({{qo, nq}, {ko, nk}}, {{q == qo ? nullptr : q, nq}, {k == ko ? nullptr : k, nk},
+                                    {positions, static_cast<size_t>(d->axes) * tokens * sizeof(int32_t)}}))
+    return PA_ERR_SHAPE;
   sh->B = d->batch;
   sh->L = d->seq_len;
   sh->Hq = d->num_heads;
@@ -276,12 +300,23 @@ size_t linear_attn_workspace(const pa_attn_desc* desc, bool backward) {
   return pa::linear_attn_workspace_bytes(sh, desc->dtype == PA_F32, backward);
 }
 
-int check_linear_attn_ws(const pa_attn_desc* desc, bool backward, const void* ws, size_t bytes) {
-  const size_t need = linear_attn_workspace(desc, backward);
+int check_linear_attn_ws(size_t need, const void* ws, size_t bytes) {
   if (need == 0) return PA_OK;
   if (!ws || bytes < need) return PA_ERR_WORKSPACE;
   return (reinterpret_cast<uintptr_t>(ws) & 255u) == 0 ? PA_OK : PA_ERR_ALIGN;
 }
+
+// Bytes of a call's tensors [B, L, H, D], of its states and of a value per head or sequence.
+struct LinearAttnBytes {
+  size_t x, state, heads, seqs;
+  LinearAttnBytes(const pa::AttnShape& sh, const pa_attn_desc* d) {
+    const size_t BH = static_cast<size_t>(sh.B) * sh.H;
+    x = BH * sh.L * sh.D * (d->dtype == PA_F32 ? 4 : 2);
+    state = BH * sh.D * sh.D * sizeof(float);
+    heads = sh.H * sizeof(float);
+    seqs = sh.B * sizeof(int32_t);
+  }
+};
 }  // namespace
 
 extern "C" {
@@ -320,8 +355,13 @@ int pa_linear_attn_fwd(const pa_attn_desc* desc, const void* q, const void* k, c
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(log_decay) ||
       !aligned4(seq_lens) || !aligned16(state_in) || !aligned16(state_out))
     return PA_ERR_ALIGN;
-  if (o == q || o == k || o == v) return PA_ERR_SHAPE;
-  st = check_linear_attn_ws(desc, false, workspace, workspace_bytes);
+  const LinearAttnBytes n(sh, desc);
+  const size_t need = pa_linear_attn_fwd_workspace_size(desc);
+  if (!apart({{o, n.x}, {state_out, n.state}, {workspace, need}},
+             {{q, n.x}, {k, n.x}, {v, n.x}, {log_decay, n.heads}, {seq_lens, n.seqs},
+              {state_in == state_out ? nullptr : state_in, n.state}}))
+    return PA_ERR_SHAPE;
+  st = check_linear_attn_ws(need, workspace, workspace_bytes);
   if (st != PA_OK) return st;
   uint32_t* status = status_word();
   if (!status) return PA_ERR_DEVICE;
@@ -346,16 +386,13 @@ int pa_linear_attn_bwd(const pa_attn_desc* desc, const void* q, const void* k, c
       !aligned16(dk) || !aligned16(dv) || !aligned4(log_decay) || !aligned4(seq_lens) ||
       !aligned16(state_in) || !aligned16(d_state_out) || !aligned16(d_state_in))
     return PA_ERR_ALIGN;
-  // the three gradients are written while the inputs are still read
-  const void* in[4] = {q, k, v, dO};
-  const void* out[3] = {dq, dk, dv};
-  for (int i = 0; i < 3; ++i) {
-    for (const void* p : in)
-      if (out[i] == p) return PA_ERR_SHAPE;
-    if (out[i] == out[(i + 1) % 3]) return PA_ERR_SHAPE;
-  }
-  if (d_state_in && (d_state_in == state_in || d_state_in == d_state_out)) return PA_ERR_SHAPE;
-  st = check_linear_attn_ws(desc, true, workspace, workspace_bytes);
+  const LinearAttnBytes n(sh, desc);
+  const size_t need = pa_linear_attn_bwd_workspace_size(desc);
+  if (!apart({{dq, n.x}, {dk, n.x}, {dv, n.x}, {d_state_in, n.state}, {workspace, need}},
+             {{q, n.x}, {k, n.x}, {v, n.x}, {dO, n.x}, {log_decay, n.heads}, {seq_lens, n.seqs},
+              {state_in, n.state}, {d_state_out, n.state}}))
+    return PA_ERR_SHAPE;
+  st = check_linear_attn_ws(need, workspace, workspace_bytes);
   if (st != PA_OK) return st;
   uint32_t* status = status_word();
   if (!status) return PA_ERR_DEVICE;
@@ -375,7 +412,10 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(log_decay) ||
       !aligned16(state_in) || !aligned16(state_out))
     return PA_ERR_ALIGN;
-  if (o == q || o == k || o == v) return PA_ERR_SHAPE;
+  const LinearAttnBytes n(sh, desc);
+  if (!apart({{o, n.x}, {state_out, n.state}}, {{q, n.x}, {k, n.x}, {v, n.x}, {log_decay, n.heads},
+                                                {state_in == state_out ? nullptr : state_in, n.state}}))
+    return PA_ERR_SHAPE;
   return pa::launch_linear_attn_step(sh, desc->dtype == PA_F32, q, k, v, log_decay, state_in, o,
                                      state_out, static_cast<cudaStream_t>(stream));
 }

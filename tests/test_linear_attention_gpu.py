@@ -462,3 +462,41 @@ def test_calls_after_a_recorded_error_end_at_once(dtype, D, B, L, H):
     call(*out)
     assert pa_capi.device_status() == 0
     assert all(torch.equal(x, w) for x, w in zip(out, want))
+
+
+@pytest.mark.gpu
+def test_tensors_side_by_side_in_one_buffer():
+    """Slices of one allocation that touch and do not overlap are separate tensors, the same tensor may be
+    several inputs, and a slice that overlaps another by one vector is refused."""
+    import pa_capi
+    B, L, H, D = 1, 4100, 2, 64
+    q, k, v, dO, ld, s, ds = _inputs(B, L, H, D, torch.bfloat16, 96, states=True)
+    n = q.numel()
+    buf = torch.empty(8 * n, dtype=q.dtype, device="cuda")
+    a = [buf[i * n:(i + 1) * n].view(q.shape) for i in range(8)]
+    for x, y in zip(a, (q, k, v, dO)):
+        x.copy_(y)
+    o, _ = _forward(q, k, v, ld)
+    pa_capi.linear_attn_fwd(*a[:3], ld, a[4])
+    assert torch.equal(a[4], o)
+    want = [torch.empty_like(q) for _ in range(3)]
+    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *want)
+    pa_capi.linear_attn_bwd(*a[:4], ld, *a[4:7])
+    assert all(torch.equal(x, w) for x, w in zip(a[4:7], want))
+    pa_capi.linear_attn_fwd(q, q, q, ld, o)
+    _close(o, *(mix(q, q, q, ld, absolute=m)[0] for m in (False, True)), REL[q.dtype], 2.0 ** -8)
+    off = buf[n * 3 - 8:n * 4 - 8].view(q.shape)
+    with pytest.raises(pa_capi.PaError):
+        pa_capi.linear_attn_fwd(*a[:3], ld, off)
+    with pytest.raises(pa_capi.PaError):
+        pa_capi.linear_attn_bwd(*a[:4], ld, a[4], a[5], buf[n * 6 - 8:n * 7 - 8].view(q.shape))
+    pos = torch.arange(L, dtype=torch.int32, device="cuda").view(1, 1, L)
+    desc = pa_capi.rope_desc(q, k)
+    turned = [torch.empty_like(q) for _ in range(2)]
+    pa_capi.rope_fwd(q, k, pos, *turned, desc)
+    a[0].copy_(q)
+    a[1].copy_(k)
+    pa_capi.rope_fwd(a[0], a[1], pos, a[0], a[2], desc)  # q in place, k beside itself
+    assert torch.equal(a[0], turned[0]) and torch.equal(a[2], turned[1])
+    with pytest.raises(pa_capi.PaError):
+        pa_capi.rope_fwd(a[0], a[1], pos, a[3], buf[n * 2 - 8:n * 3 - 8].view(q.shape), desc)

@@ -181,3 +181,77 @@ def test_binding_refuses_workspaces_that_the_kernel_must_not_write():
             with pytest.raises(ValueError, match="workspace must be contiguous"):
                 pa_capi._linear_attn_ws(size_of, d, ws, OnGpu(-1), None)
         assert pa_capi._linear_attn_ws(size_of, d, plain, OnGpu(-1), None) == (plain, 1 << 22)
+
+
+# 2 x 128 tokens of 2 heads of 64 in bf16 and 2 x 2 states of 64 x 64: 64 KB each, so addresses 64 KB apart
+# are tensors side by side
+K64 = 1 << 16
+
+
+def _spans(n):
+    return [(i + 1) * K64 for i in range(n)]
+
+
+@pytest.mark.parametrize("shift", [16, K64 - 16, 16 - K64, -16, 0])
+def test_linear_attention_refuses_tensors_that_share_bytes(shift):
+    """Each output over each input, each other output and the workspace, by 16 bytes, by all but 16, and whole."""
+    import pa_capi
+    lib = pa_capi.load()
+
+    def each(call, names, outputs, free=()):
+        at = dict(zip(names, _spans(len(names))))
+        for o in outputs:
+            for other in names:
+                if other != o and (o, other, shift) not in free:
+                    assert call(dict(at, **{o: at[other] + shift})) == SHAPE, (o, other)
+
+    names = ["q", "k", "v", "s", "o", "so", "ld", "n"]
+    small = ("ld", "n")  # shorter than the shift: only what lies over them meets them
+    skip = [(o, x, d) for o in ("o", "so", "dq", "dk", "dv", "dsi") for x in small for d in (16, K64 - 16)]
+    each(lambda a: lib.pa_linear_attn_fwd(_desc(), a["q"], a["k"], a["v"], a["ld"], a["n"], a["s"], a["o"], a["so"],
+                                          None, 0, None), names, ("o", "so"), [*skip, ("so", "s", 0)])
+    names = ["q", "k", "v", "dO", "s", "ds", "dq", "dk", "dv", "dsi", "ld", "n"]
+    each(lambda a: lib.pa_linear_attn_bwd(_desc(), a["q"], a["k"], a["v"], a["dO"], a["ld"], a["n"], a["s"], a["ds"],
+                                          a["dq"], a["dk"], a["dv"], a["dsi"], 0, None, 0, None),
+         names, ("dq", "dk", "dv", "dsi"), skip)
+    # one token: 256 sequences of 2 heads for tensors of 64 KB, 8 MB of states
+    names = ["q", "k", "v", "o", "ld"]
+    base = dict(zip(names, _spans(5)), s=1 << 24, so=1 << 25)
+    step = lambda a: lib.pa_linear_attn_step(_desc(B=256, L=1), a["q"], a["k"], a["v"], a["ld"], a["s"], a["o"],
+                                             a["so"], None)
+    for x in ("q", "k", "v"):
+        assert step(dict(base, o=base[x] + shift)) == SHAPE
+    assert step(dict(base, o=base["s"] + shift)) == SHAPE
+    if shift:
+        assert step(dict(base, so=base["s"] + shift)) == SHAPE
+    assert step(dict(base, so=base["o"] + shift)) == SHAPE
+
+
+def test_linear_attention_refuses_a_workspace_over_a_tensor():
+    """And takes one beside it: then a workspace that is too small is what is wrong."""
+    import pa_capi
+    lib = pa_capi.load()
+    desc = ctypes.byref(pa_capi.AttnDesc(1, 8192, 2, 64, pa_capi.PA_BF16, 0.0))  # tensors of 2 MB
+    need = lib.pa_linear_attn_fwd_workspace_size(desc)
+    assert need > 0
+    M2 = 2 << 20
+    fwd = lambda ws, nb: lib.pa_linear_attn_fwd(desc, M2, 2 * M2, 3 * M2, 64, None, None, 4 * M2, None, ws, nb, None)
+    for ws in (M2, 2 * M2 + 256, 4 * M2 - 256, 5 * M2 - 256):
+        assert fwd(ws, need) == SHAPE
+    assert fwd(5 * M2, need - 1) == WORKSPACE
+    assert fwd(None, 0) == WORKSPACE
+
+
+@pytest.mark.parametrize("shift", [16, 1024, -16])
+def test_rope_refuses_tensors_that_share_bytes(shift):
+    """8 tokens of 2 heads of 64 in bf16 (2 KB) and of 1 (1 KB); positions 64 bytes."""
+    import pa_capi
+    lib = pa_capi.load()
+    q, k, pos, qo, ko = 1 << 16, 2 << 16, 3 << 16, 4 << 16, 5 << 16
+    in_k = shift if abs(shift) < 1024 else 512
+    for a in ((q, k, pos, q + shift, ko), (q, k, pos, k + in_k, ko), (q, k, pos, k, ko), (q, k, pos, qo, q + shift),
+              (q, k, pos, qo, k + in_k), (q, k, pos, qo, qo + shift), (q, k, pos, pos - 16, ko),
+              (q, k, pos, q, q + shift), (q, k, pos, qo, pos - 1008)):
+        assert lib.pa_rope_fwd(_rope(), *a, None) == SHAPE, a
+        assert lib.pa_rope_bwd(_rope(), *a, 0, None) == SHAPE, a
+        assert lib.pa_rope_bwd(_rope(), *a, 1, None) == SHAPE, a
