@@ -382,7 +382,9 @@ def _linear_attn_ws(size_of, d, workspace, q, stream):
             return None, 0
         import torch
         # memory of the stream that will use it: the allocator orders its reuse there
-        with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
+        # (ExternalStream(0) would be a new stream, not the default one)
+        with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream) if stream
+                               else torch.cuda.default_stream()):
             workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif workspace.get_device() != q.get_device():
         raise ValueError(f"linear attention: workspace must be on {q.device}, not {workspace.device}")

@@ -500,3 +500,43 @@ def test_tensors_side_by_side_in_one_buffer():
     assert torch.equal(a[0], turned[0]) and torch.equal(a[2], turned[1])
     with pytest.raises(pa_capi.PaError):
         pa_capi.rope_fwd(a[0], a[1], pos, a[3], buf[n * 2 - 8:n * 3 - 8].view(q.shape), desc)
+
+
+@pytest.mark.gpu
+def test_the_bindings_workspace_is_allocated_on_the_stream_of_the_call(monkeypatch):
+    """Whatever stream is current: memory that the allocator may hand out again on another one while the
+    kernels still write it would change results now and then only, so the allocation itself is looked at; and
+    the same memory is then asked for and overwritten on the current stream."""
+    import pa_capi
+    q, k, v, dO, ld, _, _ = _inputs(1, 4100, 2, 64, torch.bfloat16, 97)
+    want = _forward(q, k, v, ld)[0], *(torch.empty_like(q) for _ in range(3))
+    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *want[1:])
+    d = pa_capi.attn_desc(q)
+    sizes = [pa_capi.linear_attn_fwd_workspace_size(d), pa_capi.linear_attn_bwd_workspace_size(d)]
+    assert min(sizes) > 0
+    empty, made = torch.empty, []
+
+    def watched(*a, **kw):
+        made.append((a[0], torch.cuda.current_stream().cuda_stream))
+        return empty(*a, **kw)
+
+    side = torch.cuda.Stream()
+    default = torch.cuda.default_stream()
+    for handle, expect, current in ((side.cuda_stream, side, default), (None, default, default), (None, side, side),
+                                    (0, default, side)):
+        outs = [[torch.zeros_like(q) for _ in range(4)] for _ in range(3)]
+        torch.cuda.synchronize()
+        with torch.cuda.stream(current):
+            for o in outs:
+                made.clear()
+                with monkeypatch.context() as m:
+                    m.setattr(torch, "empty", watched)
+                    pa_capi.linear_attn_fwd(q, k, v, ld, o[0], stream=handle)
+                    pa_capi.linear_attn_bwd(q, k, v, dO, ld, *o[1:], stream=handle)
+                assert made == [(n, expect.cuda_stream) for n in sizes]
+                if current is not expect:
+                    for n in sizes * 2:
+                        torch.full((n,), 255, dtype=torch.uint8, device="cuda")
+        torch.cuda.synchronize()
+        for o in outs:
+            assert all(torch.equal(x, w) for x, w in zip(o, want))
