@@ -280,3 +280,50 @@ def test_one_token_takes_the_single_token_kernel_without_a_graph(pa):
     for a, b, c in zip(plain, off, on):
         assert np.array_equal(_h(a), _h(b))
         assert rel_err(_h(c), _h(a)) < TOL
+
+
+@pytest.mark.gpu
+def test_replays_of_a_captured_step_follow_their_inputs(pa):
+    """Inputs and targets are rewritten between replays, and the gradients overwritten with the rewritten
+    step's: what a replay leaves is its own work. Each is then compared with an eager step on the same values."""
+    N, L, E, H = 2, 390, 128, 2
+    pos = np.broadcast_to(np.arange(L), (1, N, L)).astype(np.int32)
+    prev, s = pa.get_stream(), torch.cuda.Stream()
+    pa.set_stream(s.cuda_stream)
+    try:
+        with torch.cuda.stream(s):
+            layer = pa.LinearAttention(E, H, sections=[32])
+            X, T, P = _t(pa, seeded_normal(70, (N, L, E))), _t(pa, seeded_normal(71, (N, L, E))), _ints(pa, pos)
+            mse = pa.MSE()
+
+            def step():
+                for p in layer.parameters():
+                    p.zero_grad()
+                loss = mse(layer.forward(X, P), T)
+                loss.backward()
+                return loss
+
+            def put(seed):
+                X.to_device(seeded_normal(seed, (N, L, E)).ravel().tolist())
+                T.to_device(seeded_normal(seed + 1, (N, L, E)).ravel().tolist())
+
+            eager = step()  # stays alive
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=s):
+                step()
+            grads = []
+            for seed in (72, 74):
+                put(seed)
+                g.replay()
+                torch.cuda.synchronize()
+                grads.append([_g(p) for p in layer.parameters()])
+            for seed, got in zip((72, 74), grads):
+                put(seed)
+                loss = step()
+                for p, w in zip(layer.parameters(), got):
+                    assert np.array_equal(_g(p), w)
+            assert not any(np.array_equal(a, b) for a, b in zip(*grads))
+            del eager, loss, g
+    finally:
+        torch.cuda.synchronize()
+        pa.set_stream(prev)
