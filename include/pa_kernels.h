@@ -204,8 +204,11 @@ int pa_rope_bwd(const pa_rope_desc* desc, const void* dq_out, const void* dk_out
  * NULL starts from zero; state_out (NULL: not wanted) is the state after the
  * last valid token and may be state_in. Results do not depend on the run: each
  * sum has one order. The scale lies within 2^-64 .. 2^64 (PA_ERR_SHAPE otherwise).
- * Values of valid tokens and states are finite: an infinity or NaN there may
- * show in outputs of other tokens of its sequence and head, earlier ones too.
+ * Values of valid tokens and states should be finite: an infinity or NaN in a
+ * token shows in o and dq of its sequence and head from the chunk of 128 tokens
+ * that holds it on, so also a little before it, and in dk and dv up to that
+ * chunk's end; o and dq before the chunk, dk and dv after it, other heads and
+ * other sequences keep their values.
  * A workspace belongs to one call at a time: calls that may overlap on the GPU,
  * and graphs that may, need one each. An output or a workspace that shares bytes
  * with an input or with another of them is refused (PA_ERR_SHAPE), but for a

@@ -540,3 +540,71 @@ def test_the_bindings_workspace_is_allocated_on_the_stream_of_the_call(monkeypat
         torch.cuda.synchronize()
         for o in outs:
             assert all(torch.equal(x, w) for x, w in zip(o, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [32, 64])
+def test_bf16_math_of_fp32_tensors_cut_into_segments(D):
+    """As test_bf16_math_of_fp32_tensors, with sequences long enough for segment states, and lengths that end
+    inside and between segments."""
+    import pa_capi
+    B, L, H = 2, 4100, 2
+    q, k, v, dO, ld, s, ds = _inputs(B, L, H, D, torch.float32, 98, states=True)
+    q, k, v, dO = (x.bfloat16().float() for x in (q, k, v, dO))
+    assert pa_capi.linear_attn_fwd_workspace_size(pa_capi.attn_desc(q)) > 0
+    for lens in (None, torch.tensor([4001, 1290], dtype=torch.int32).cuda()):
+        pa_capi.set_f32_math("bf16")
+        try:
+            o, so = _forward(q, k, v, ld, seq_lens=lens, state_in=s)
+            g = [torch.empty_like(q) for _ in range(3)]
+            dsi = torch.empty_like(s)
+            pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, seq_lens=lens, state_in=s, d_state_out=ds, d_state_in=dsi)
+        finally:
+            pa_capi.set_f32_math("split3")
+        want, ws = mix(q, k, v, ld, lens, s)
+        mag, ms = mix(q, k, v, ld, lens, s, absolute=True)
+        _close(o, want, mag, 2.0 ** -8, 2.0 ** -24)
+        _close(so, ws, ms, 2.0 ** -15, 2.0 ** -24)
+        wg, mg = mix_grads(q, k, v, ld, dO, lens, s, ds), mix_grads_absolute(q, k, v, ld, dO, lens, s, ds)
+        for got, w, m in zip(g, wg, mg):
+            _close(got, w, m, 2.0 ** -8, 2.0 ** -24)
+        _close(dsi, wg[3], mg[3], 2.0 ** -15, 2.0 ** -24)
+        # one bf16 per operand, or these would not be the kernels of that mode: more than split products allow
+        assert rel_err(o.double().cpu(), want.cpu()) > NORM[torch.float32]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_how_far_a_value_that_is_not_finite_reaches(dtype, D, bad):
+    """One such value in one valid token: outputs and dq of the chunks of 128 tokens before its own, and dk and dv of
+    those after it, keep their bits, as do all other heads and sequences. Cut and uncut sequences."""
+    import pa_capi
+    for L, t in ((700, 300), (4100, 2050)):
+        x = list(_inputs(2, L, 2, D, dtype, 99, states=True))
+        ld, s, ds = x[4:]
+        for i in range(4):  # q, k, v, dO in turn
+            y = [z.clone() for z in x[:4]]
+            y[i][1, t, 1, D // 2] = bad
+            got = []
+            for q, k, v, dO in (x[:4], y):
+                o, so = _forward(q, k, v, ld, state_in=s)
+                g = [torch.empty_like(q) for _ in range(3)]
+                dsi = torch.empty_like(s)
+                pa_capi.linear_attn_bwd(q, k, v, dO, ld, *g, state_in=s, d_state_out=ds, d_state_in=dsi)
+                got.append((o, g[0], g[1], g[2], so, dsi))
+            first, after = t // 128 * 128, (t // 128 + 1) * 128
+            for n, (a, b) in enumerate(zip(*got)):
+                assert torch.equal(a[0], b[0])
+                if n >= 4:
+                    assert torch.equal(a[1, 0], b[1, 0])
+                    continue
+                assert torch.equal(a[1, :, 0], b[1, :, 0])
+                keep = slice(0, first) if n < 2 else slice(after, L)
+                assert torch.equal(a[1, keep, 1], b[1, keep, 1])
+            if i == 0:  # q alone: its own output, and no state
+                assert torch.equal(got[0][4], got[1][4])
+                clean = torch.ones(L, dtype=torch.bool)
+                clean[t] = False
+                assert torch.equal(got[0][0][1, clean], got[1][0][1, clean])
+                assert not torch.isfinite(got[1][0][1, t, 1]).all()
