@@ -67,13 +67,16 @@ __device__ __forceinline__ int valid_tokens(const int32_t* lens, int b, int L) {
 // product hi*hi + hi*lo + lo*hi (2^-16 in all).
 //
 // What bounds it. 8 x 4096 tokens of 16 heads of 64 in bf16 (268 MB: 41 us at the copy rate) take 58
-// us alone, 4.6 TB/s, 66 us back to back under the power limit. A chunk takes 2900 clocks, and by
+// us alone, 4.6 TB/s, 64-65 us back to back under the power limit. A chunk takes 2900 clocks, and by
 // count 270 KB of it pass the 128 bytes a clock of the SM's shared memory, 2200 clocks: tiles of
 // q, k and v land there, V' is made there in two parts, and the four products read their operands
 // there (but P, from TMEM); 128 of 148 SMs are busy. At head dim 128 a unit is half of V's columns,
 // and each half forms P anew: a state of 128 x 128 would need 128 registers of each of 128 threads.
 // Chunks of fp32 move 700 KB (three products, and tiles split into parts in place), 5400 of 6000
-// clocks. Short calls wait for their own code: the first chunk of a cold launch takes 5 us.
+// clocks, 3.7 us: 8 x 1024 tokens of 8 heads of 64 in one launch are 8 chunks a block and 5.5 us to
+// start, 35 us, and cut in two 34. Heads of 32 in fp32 take the instance of 64 columns, half of each
+// tile zeros: 33 us where heads of 64 take 34. Short calls wait for their own code: the first chunk of
+// a cold launch takes 5 us.
 //
 // TMEM columns: Q K^T and P 2 x 128 (P of 32 tokens over their 32 scores: hi in the
 // first 16 columns, lo in the others), Q S 64, P V 64, K^T [V' hi, V' lo] 128.
@@ -1084,7 +1087,10 @@ MixPlan mix_plan(const AttnShape& sh, bool f32, int n_dir) {
   // None where the second launch and the second reading of k and v cost more than the chunks that a
   // sequence no longer waits for. bf16: 8 heads in 2 segments 8 chunks 18.6 us whole and 19.3 cut, 12
   // chunks 24.5 and 23.6; 32 heads in 4, 6 chunks 16.5 and 17.2, 8 chunks 18.5 and 17.4. A chunk of
-  // fp32 takes twice as long: 32 heads in 2 segments 6 chunks 30 and 29, 8 chunks 37 and 34.
+  // fp32 takes twice as long: 32 heads in 2 segments 6 chunks 30 and 29, 8 chunks 37 and 34. With 64 heads
+  // in 2 segments a cut gains less (warm, back to back): fp32 6 chunks 27.6 whole and 27.5 cut, 8 chunks
+  // 35.1 and 34.0, 12 chunks 49.9 and 47.4; bf16 12 chunks 20.9 and 21.5, 16 chunks 26.1 and 24.7. From half
+  // as many units as SMs on nothing is cut, and some SMs idle.
   if (seg > 1 && chunks - (chunks + seg - 1) / seg < (f32 ? 3 : 6)) seg = 1;
   if (seg < 1) seg = 1;
   int seg_chunks = (chunks + seg - 1) / seg;

@@ -11,7 +11,8 @@
 // fp32 product is off by 2^-24 * 2e5 = 0.012 rad. The host passes w_i / 2 pi in
 // 64 bits; the kernel takes the fraction of position * w_i / 2 pi in 64 bits
 // (one multiply, one rounding to the nearest whole turn) and only then fp32
-// sine and cosine, exact to about 3e-7 for every 32-bit position.
+// sine and cosine: the angle is off by 1e-7 rad up to position 2^24 (the fp32
+// fraction) and by 4e-7 at 2^31 (the 64-bit product).
 //
 // Bound by HBM: q and k are read once and written once. A block computes the
 // cosines and sines of its tokens once into shared memory, and all heads of q
