@@ -150,10 +150,10 @@ def test_rope_past_2_31_values():
 @pytest.mark.gpu
 @pytest.mark.parametrize("layout", ["halves", "pairs"])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-@pytest.mark.parametrize("D,sections", [(64, [8, 16]), (128, [64]), (50, [3, 7]), (7, [2])])
+@pytest.mark.parametrize("D,sections", [(64, [8, 16]), (128, [64]), (50, [3, 7]), (7, [2]), (130, [9])])
 def test_rope_in_place_in_every_form(dtype, layout, D, sections):
     """Whole vectors and single values, forward and gradient: an output over its own input gives the bits
-    of one beside it. 19 heads in all: a thread takes several groups of them, one after another."""
+    of one beside it. With heads of 130 a thread takes several groups of four, one after another."""
     import pa_capi
     q, pos = _data(2, 290, 16, D, dtype, len(sections), 3000, 10)
     k, _ = _data(2, 290, 3, D, dtype, 1, 2, 11)
@@ -164,3 +164,22 @@ def test_rope_in_place_in_every_form(dtype, layout, D, sections):
         a, b = q.clone(), k.clone()
         turn_by(a, b, pos, a, b, desc)
         assert torch.equal(a, qo) and torch.equal(b, ko)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["halves", "pairs"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("Hq,Hk,D,sections", [(70, 9, 256, [60, 68]), (1, 11, 130, [9]), (40, 40, 90, [20, 25])])
+def test_rope_more_heads_than_a_block_takes_at_once(dtype, layout, Hq, Hk, D, sections):
+    """A thread then goes through several groups of four heads with the angles of the first, from q on into k."""
+    import pa_capi
+    q, pos = _data(2, 190, Hq, D, dtype, len(sections), 5000, 12)
+    k, _ = _data(2, 190, Hk, D, dtype, 1, 2, 13)
+    desc = pa_capi.rope_desc(q, k, sections, layout=layout)
+    qo, ko = torch.full_like(q, float("nan")), torch.full_like(k, float("nan"))
+    pa_capi.rope_fwd(q, k, pos, qo, ko, desc)
+    for x, y in ((q, qo), (k, ko)):
+        _check(y, x, turn(x, pos, sections, layout=layout), sections, layout)
+    pa_capi.rope_bwd(q, k, pos, qo, ko, desc)
+    for x, y in ((q, qo), (k, ko)):
+        _check(y, x, turn(x, pos, sections, layout=layout, inverse=True), sections, layout)
