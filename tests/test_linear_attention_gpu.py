@@ -608,3 +608,41 @@ def test_how_far_a_value_that_is_not_finite_reaches(dtype, D, bad):
                 clean[t] = False
                 assert torch.equal(got[0][0][1, clean], got[1][0][1, clean])
                 assert not torch.isfinite(got[1][0][1, t, 1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_replayed_steps_in_place_equal_a_loop(dtype, D):
+    """A captured single-token step that updates its state in place, its token's buffers refilled before each
+    replay, for more blocks than a wave holds."""
+    import pa_capi
+    B, H, n = 90, 16, 12
+    q, k, v, _, ld, s, _ = _inputs(B, n, H, D, dtype, 100, states=True)
+    token = [torch.empty_like(q[:, :1]).contiguous() for _ in range(4)]
+    want, state = [], s.clone()
+    for t in range(n):
+        o = torch.empty_like(token[3])
+        pa_capi.linear_attn_step(*(x[:, t:t + 1].contiguous() for x in (q, k, v)), ld, state, o, state)
+        want.append(o)
+    held = s.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pa_capi.linear_attn_step(*token[:3], ld, held, token[3], held)
+    for t in range(n):
+        for x, y in zip(token, (q, k, v)):
+            x.copy_(y[:, t:t + 1])
+        g.replay()
+        assert torch.equal(token[3], want[t])
+    assert torch.equal(held, state)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,D", TYPES)
+def test_many_sequences_of_one_token(dtype, D):
+    """Thousands of units of one token each through the chunks, and the gradients of both states."""
+    B, H = 1300, 3
+    q, k, v, dO, ld, s, ds = _inputs(B, 1, H, D, dtype, 101, states=True)
+    lens = torch.ones(B, dtype=torch.int32)
+    lens[::5] = 0
+    _check_forward(q, k, v, ld, lens.cuda(), s)
+    _check_backward(q, k, v, dO, ld, lens.cuda(), s, ds)

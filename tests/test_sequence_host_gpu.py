@@ -327,3 +327,42 @@ def test_replays_of_a_captured_step_follow_their_inputs(pa):
     finally:
         torch.cuda.synchronize()
         pa.set_stream(prev)
+
+
+@pytest.mark.gpu
+def test_the_graph_switched_off_changes_no_value_of_any_layer(pa):
+    """The other layers with the graph off give the bits that they give with it on; a graph recorded before
+    runs its backward while it is off, and recording goes on afterwards."""
+    N, L, E = 2, 70, 128
+    x, target = seeded_normal(80, (N, L, E)), _t(pa, seeded_normal(81, (N, L, E)))
+    ln, mha, lin, act, mix_layer, mse = (pa.LayerNorm(E), pa.MultiheadAttention(E, 2), pa.Linear(E, E), pa.ReLU(),
+                                         pa.LinearAttention(E, 2), pa.MSE())
+    layers = (ln, mha, lin, mix_layer)
+
+    def run():
+        X = _t(pa, x, True)
+        h = pa.add(X, mha.forward(ln.forward(X)))
+        h = pa.add(h, mix_layer.forward(ln.forward(h)))
+        y = act.forward(lin.forward(h))
+        return X, y, mse(y, target)
+
+    X0, y0, loss0 = run()
+    loss0.backward()
+    want = [_g(X0), *(_g(p) for m in layers for p in m.parameters())]
+    X1, y1, loss1 = run()
+    for m in layers:
+        for p in m.parameters():
+            p.zero_grad()
+    pa.set_grad_enabled(False)
+    try:
+        X2, y2, loss2 = run()
+        for t in (y2, loss2):
+            with pytest.raises(RuntimeError, match="does not require"):
+                t.backward()
+        loss1.backward()
+        got = [_g(X1), *(_g(p) for m in layers for p in m.parameters())]
+    finally:
+        pa.set_grad_enabled(True)
+    assert np.array_equal(_h(y2), _h(y0)) and np.array_equal(_h(loss2), _h(loss0))
+    assert all(np.array_equal(a, b) for a, b in zip(got, want))
+    assert not _g(X2).any()
