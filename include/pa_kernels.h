@@ -236,6 +236,131 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
                         const float* log_decay, const float* state_in, void* o, float* state_out,
                         pa_stream_t stream);
 
+/* ---------------------------------------------------------------- packed causal attention
+ * Causal softmax attention over sequences of different lengths laid end to end,
+ * with heads of k and v shared by groups of q's heads; not in the reference,
+ * whose attention sees every token and has one length. Tokens
+ * cu_seqlens[i] .. cu_seqlens[i + 1] - 1 are sequence i (device int32
+ * [num_seqs + 1], ascending from any start; a sequence may be empty). Head h of
+ * q goes with head h / (num_heads / num_kv_heads) of k and v; a token sees the
+ * tokens of its own sequence up to itself:
+ *   o_i = sum_{j <= i} softmax_j(scale q_i . k_j) v_j,  lse[h][i] = log sum_j exp(scale q_i . k_j).
+ * q, o, dO, dq are [tokens, num_heads, head_dim], k, v, dk, dv [tokens,
+ * num_kv_heads, head_dim], lse [num_heads, tokens] fp32. The heads of a token
+ * are contiguous; tokens of q, k, v and of dq, dk, dv may lie further apart
+ * (slices of one projection's output or gradient), o, dO and lse are contiguous.
+ * Tokens in no sequence (before the first, behind the last) are neither used
+ * nor written. Entries of cu_seqlens outside 0 .. tokens, or that descend, are
+ * taken as clamped to the entry before and to tokens: nothing is read or written out of
+ * bounds, but sequences that overlap give no defined result.
+ * bf16: head_dim 64 or 128. Results do not depend on the run: each sum has one order.
+ * An infinity or NaN in a token shows in the heads of its group and its sequence:
+ * in o, lse and dq from the block of 128 tokens that holds it on, so also a little
+ * before it, and in dk and dv anywhere; other sequences keep their values.
+ * A workspace (256-byte aligned) belongs to one call at a time: calls that may
+ * overlap on the GPU, and graphs that may, need one each. An output or workspace
+ * that shares bytes with another tensor of the call is refused (PA_ERR_SHAPE). */
+typedef struct pa_packed_attn_desc {
+  int32_t tokens;       /* rows of q, k, v: all sequences' tokens (and any in none) */
+  int32_t num_seqs;
+  int32_t num_heads;    /* heads of q and o */
+  int32_t num_kv_heads; /* heads of k and v; divides num_heads */
+  int32_t head_dim;
+  int32_t dtype;        /* pa_dtype of all but lse */
+  float softmax_scale;  /* <= 0 selects 1/sqrt(head_dim) */
+  /* values from one token to the next; 0: contiguous. Multiples of 16 bytes. */
+  int32_t q_stride, k_stride, v_stride;
+  int32_t dq_stride, dk_stride, dv_stride;
+} pa_packed_attn_desc;
+size_t pa_packed_attn_fwd_workspace_size(const pa_packed_attn_desc* desc);
+int pa_packed_attn_fwd(const pa_packed_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const int32_t* cu_seqlens, void* o, float* lse, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream);
+/* Gradients of q, k and v (overwritten, or added to when accumulate != 0) from
+ * dO and the forward's o and lse; dk and dv are sums over the group's heads. */
+size_t pa_packed_attn_bwd_workspace_size(const pa_packed_attn_desc* desc);
+int pa_packed_attn_bwd(const pa_packed_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const void* o, const void* dO, const float* lse, const int32_t* cu_seqlens,
+                       void* dq, void* dk, void* dv, int accumulate, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream);
+
+/* ---------------------------------------------------------------- attention over a paged cache
+ * One new token of each sequence against that sequence's cache of keys and
+ * values, the single-token form of pa_packed_attn_fwd; not in the reference.
+ * The caches are pools of pages, [num_pages, page_size, num_kv_heads, head_dim]
+ * each; token t of sequence b is row t % page_size of page
+ * page_table[b][t / page_size] (device int32 [batch, max_pages]). seq_lens
+ * (device int32 [batch], clamped to 0 .. max_pages * page_size) counts the
+ * cached tokens, the new one among them: its k and v are in the cache before
+ * the call (pa_qk_norm_rope_cache). What the cache holds behind a sequence's length is
+ * not used (NaN allowed). A page number outside 0 .. num_pages - 1 holds no
+ * tokens: those places are left out, as if masked. Where no token is left (a length
+ * of 0), o is 0 and lse -infinity.
+ * q and o [batch, num_heads, head_dim] (q_stride values from one sequence's q
+ * to the next), lse [batch, num_heads] fp32 or NULL. bf16: head_dim 64 or 128;
+ * fp32: 32 or 64, in fp32 arithmetic under either f32 math mode. Any page_size,
+ * any group num_heads / num_kv_heads. Results do not depend on the run.
+ * Workspace and outputs as for pa_packed_attn_fwd. */
+typedef struct pa_paged_attn_desc {
+  int32_t batch;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t dtype;
+  float softmax_scale; /* <= 0 selects 1/sqrt(head_dim) */
+  int32_t page_size;   /* tokens of a page */
+  int32_t num_pages;   /* pages of the pool */
+  int32_t max_pages;   /* entries of a row of page_table */
+  int32_t q_stride;    /* 0: contiguous */
+} pa_paged_attn_desc;
+size_t pa_paged_attn_step_workspace_size(const pa_paged_attn_desc* desc);
+int pa_paged_attn_step(const pa_paged_attn_desc* desc, const void* q, const void* k_cache,
+                       const void* v_cache, const int32_t* page_table, const int32_t* seq_lens,
+                       void* o, float* lse, void* workspace, size_t workspace_bytes,
+                       pa_stream_t stream);
+
+/* ---------------------------------------------------------------- head norms with rotary positions
+ * The root-mean-square norm of each head of q and k and their rotary positions
+ * in one pass; not in the reference. With x a head of a token,
+ *   n = x / sqrt(mean(x^2) + eps) * gamma,   y = turn(n)   (as pa_rope_fwd turns).
+ * gamma_q and gamma_k are device fp32 [head_dim], shared by all heads; NULL: that
+ * tensor is turned without a norm. desc->rope as for pa_rope_fwd, with head_dim a
+ * multiple of 16 bytes' values (8 in bf16, 4 in fp32); the strides count values from one
+ * token of an input to the next (0: contiguous), so that q, k and v may be slices of one
+ * projection's output. Outputs are contiguous [B, L, heads, D], but for dq and
+ * dk, which have strides of their own. An output that shares bytes with another tensor
+ * of the call is refused (PA_ERR_SHAPE), but q_out may be q and k_out k where
+ * those are contiguous. */
+typedef struct pa_qk_norm_desc {
+  pa_rope_desc rope;
+  float eps;            /* >= 0 */
+  int32_t q_stride, k_stride, v_stride;
+  int32_t dq_stride, dk_stride;
+} pa_qk_norm_desc;
+int pa_qk_norm_rope_fwd(const pa_qk_norm_desc* desc, const void* q, const void* k, const float* gamma_q,
+                        const float* gamma_k, const int32_t* positions, void* q_out, void* k_out,
+                        pa_stream_t stream);
+/* The same for tokens that go into a cache of pa_paged_attn_step: the turned k
+ * and v [B, L, num_kv_heads, D] of token t are written to row slots[t] (device
+ * int32 [B, L]: page * page_size + place) of k_cache and v_cache, taken as
+ * [num_slots, num_kv_heads, D]; a slot outside 0 .. num_slots - 1 is not
+ * written (padding tokens), and one that several tokens name holds values of any of them.
+ * k_out (NULL: not wanted) also receives the turned k, as the prompt's own attention needs it. */
+int pa_qk_norm_rope_cache(const pa_qk_norm_desc* desc, const void* q, const void* k, const void* v,
+                          const float* gamma_q, const float* gamma_k, const int32_t* positions,
+                          const int32_t* slots, void* q_out, void* k_out, void* k_cache, void* v_cache,
+                          int64_t num_slots, pa_stream_t stream);
+/* Gradients from those of q_out and k_out and the forward's inputs: dq, dk, and
+ * dgamma_q, dgamma_k (fp32 [head_dim], sums over all tokens and heads in one
+ * order; NULL goes with a NULL gamma, or: not wanted), overwritten, or added to
+ * when accumulate != 0. dq may be dq_out and dk dk_out (contiguous, accumulate 0). */
+size_t pa_qk_norm_rope_bwd_workspace_size(const pa_qk_norm_desc* desc);
+int pa_qk_norm_rope_bwd(const pa_qk_norm_desc* desc, const void* dq_out, const void* dk_out,
+                        const void* q, const void* k, const float* gamma_q, const float* gamma_k,
+                        const int32_t* positions, void* dq, void* dk, float* dgamma_q,
+                        float* dgamma_k, int accumulate, void* workspace, size_t workspace_bytes,
+                        pa_stream_t stream);
+
 /* ---------------------------------------------------------------- layer norm */
 
 /* y = gamma * (x - mean) * rstd + beta over rows of length N; saves mean, rstd.

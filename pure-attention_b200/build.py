@@ -32,6 +32,9 @@ KERNEL_SOURCES = [
     "training.cu",
     "rope.cu",
     "linear_attn.cu",
+    "packed_attn.cu",
+    "paged_attn.cu",
+    "qk_norm_rope.cu",
     "capi.cu",
     "attn_bwd_noalloc.cu",
 ]

@@ -236,9 +236,8 @@ bool apart(std::initializer_list<Span> out, std::initializer_list<Span> in) {
   return true;
 }
 
-// Validates a rope descriptor and the pointers of one call; fills `sh`.
-int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_t* positions,
-               const void* qo, const void* ko, pa::RopeShape* sh) {
+// Validates a rope descriptor; fills `sh`.
+int check_rope_desc(const pa_rope_desc* d, pa::RopeShape* sh) {
   if (!d) return PA_ERR_NULL;
   if (d->batch <= 0 || d->seq_len <= 0 || d->num_heads <= 0 || d->num_kv_heads < 0 ||
       d->head_dim <= 0 || d->axes < 1 || d->axes > PA_ROPE_MAX_AXES)
@@ -261,16 +260,6 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
   if (tokens > 0x7fffffffLL ||
       (static_cast<long long>(d->num_heads) + d->num_kv_heads) * d->head_dim * 8 > 0x7fffffffLL)
     return PA_ERR_SHAPE;
-  if (!q || !qo || !positions || (d->num_kv_heads > 0 && (!k || !ko))) return PA_ERR_NULL;
-  if (!aligned16(q) || !aligned16(qo) || (d->num_kv_heads > 0 && (!aligned16(k) || !aligned16(ko))))
-    return PA_ERR_ALIGN;
-  if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0) return PA_ERR_ALIGN;
-  // in place is one tensor's turn over the whole of itself
-  const size_t head = static_cast<size_t>(tokens) * d->head_dim * (d->dtype == PA_F32 ? 4 : 2);
-  const size_t nq = d->num_heads * head, nk = d->num_kv_heads * head;
-  if (!apart({{qo, nq}, {ko, nk}}, {{q == qo ? nullptr : q, nq}, {k == ko ? nullptr : k, nk},
-                                    {positions, static_cast<size_t>(d->axes) * tokens * sizeof(int32_t)}}))
-    return PA_ERR_SHAPE;
   sh->B = d->batch;
   sh->L = d->seq_len;
   sh->Hq = d->num_heads;
@@ -282,6 +271,25 @@ int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_
   sh->halves = d->layout == PA_ROPE_HALVES;
   sh->per_axis = d->freqs == PA_ROPE_PER_AXIS;
   sh->base = d->base;
+  return PA_OK;
+}
+
+// The same, and the pointers of one call.
+int check_rope(const pa_rope_desc* d, const void* q, const void* k, const int32_t* positions,
+               const void* qo, const void* ko, pa::RopeShape* sh) {
+  const int st = check_rope_desc(d, sh);
+  if (st != PA_OK) return st;
+  const long long tokens = static_cast<long long>(d->batch) * d->seq_len;
+  if (!q || !qo || !positions || (d->num_kv_heads > 0 && (!k || !ko))) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(qo) || (d->num_kv_heads > 0 && (!aligned16(k) || !aligned16(ko))))
+    return PA_ERR_ALIGN;
+  if ((reinterpret_cast<uintptr_t>(positions) & 3u) != 0) return PA_ERR_ALIGN;
+  // in place is one tensor's turn over the whole of itself
+  const size_t head = static_cast<size_t>(tokens) * d->head_dim * (d->dtype == PA_F32 ? 4 : 2);
+  const size_t nq = d->num_heads * head, nk = d->num_kv_heads * head;
+  if (!apart({{qo, nq}, {ko, nk}}, {{q == qo ? nullptr : q, nq}, {k == ko ? nullptr : k, nk},
+                                    {positions, static_cast<size_t>(d->axes) * tokens * sizeof(int32_t)}}))
+    return PA_ERR_SHAPE;
   return PA_OK;
 }
 
@@ -418,6 +426,301 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
     return PA_ERR_SHAPE;
   return pa::launch_linear_attn_step(sh, desc->dtype == PA_F32, q, k, v, log_decay, state_in, o,
                                      state_out, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+// ------------------------------------------------------------------ packed and paged attention, head norms
+namespace {
+// Rows of a tensor, `row` bytes every `step` bytes.
+struct Rows {
+  uintptr_t at;
+  size_t row, step, n;
+  Rows(const void* p, size_t rows, size_t row_bytes, size_t step_bytes)
+      : at(reinterpret_cast<uintptr_t>(p)), row(row_bytes), step(step_bytes), n(p ? rows : 0) {}
+  Rows(const void* p, size_t bytes) : Rows(p, bytes ? 1 : 0, bytes, bytes) {}
+  size_t end() const { return at + (n - 1) * step + row; }
+  // Whether a byte belongs to both: rows of the same pitch may interleave (slices of one tensor).
+  bool meets(const Rows& o) const {
+    if (!n || !o.n || at >= o.end() || o.at >= end()) return false;
+    if (step != o.step || n == 1 || o.n == 1) return true;
+    const size_t d = at < o.at ? (o.at - at) % step : (step - (at - o.at) % step) % step;
+    return d < row || step - d < o.row;
+  }
+};
+bool rows_apart(std::initializer_list<Rows> out, std::initializer_list<Rows> in) {
+  for (const Rows* a = out.begin(); a != out.end(); ++a) {
+    for (const Rows& b : in)
+      if (a->meets(b)) return false;
+    for (const Rows* b = a + 1; b != out.end(); ++b)
+      if (a->meets(*b)) return false;
+  }
+  return true;
+}
+
+// A stride of a descriptor: at least the heads' own values (0 stands for them), whole 16 bytes.
+int check_stride(int32_t given, long long own, int e, long long* stride) {
+  *stride = given == 0 ? own : given;
+  if (given < 0 || *stride < own) return PA_ERR_SHAPE;
+  return *stride * e % 16 == 0 ? PA_OK : PA_ERR_ALIGN;
+}
+
+int check_workspace(size_t need, const void* ws, size_t bytes) {
+  if (!ws || bytes < need) return PA_ERR_WORKSPACE;
+  return (reinterpret_cast<uintptr_t>(ws) & 255u) == 0 ? PA_OK : PA_ERR_ALIGN;
+}
+
+float scale_or_default(float given, int head_dim) {
+  return given > 0.f ? given : 1.0f / std::sqrt(static_cast<float>(head_dim));
+}
+
+int check_packed(const pa_packed_attn_desc* d, pa::PackedShape* sh) {
+  if (!d) return PA_ERR_NULL;
+  if (d->tokens <= 0 || d->num_seqs <= 0 || d->num_heads <= 0 || d->num_kv_heads <= 0 || d->head_dim <= 0 ||
+      d->num_heads % d->num_kv_heads != 0)
+    return PA_ERR_SHAPE;
+  if (d->dtype != PA_BF16) return PA_ERR_DTYPE;
+  if (d->head_dim != 64 && d->head_dim != 128) return PA_ERR_UNSUPPORTED;
+  // the kernels count tokens, and tiles of all heads, in ints
+  const long long tiles = static_cast<long long>(d->tokens) / 128 + d->num_seqs;
+  if (d->tokens > 0x7fffffff - 256 || tiles * d->num_heads > 0x7fffffffLL / 128) return PA_ERR_SHAPE;
+  if (!(d->softmax_scale <= 0x1p64f)) return PA_ERR_SHAPE;
+  sh->T = d->tokens;
+  sh->n = d->num_seqs;
+  sh->H = d->num_heads;
+  sh->Hk = d->num_kv_heads;
+  sh->D = d->head_dim;
+  sh->scale = scale_or_default(d->softmax_scale, d->head_dim);
+  if (!(sh->scale >= 0x1p-64f)) return PA_ERR_SHAPE;
+  const long long nq = static_cast<long long>(sh->H) * sh->D, nk = static_cast<long long>(sh->Hk) * sh->D;
+  const struct { int32_t given; long long own, *to; } strides[] = {
+      {d->q_stride, nq, &sh->q_stride},   {d->k_stride, nk, &sh->k_stride},   {d->v_stride, nk, &sh->v_stride},
+      {d->dq_stride, nq, &sh->dq_stride}, {d->dk_stride, nk, &sh->dk_stride}, {d->dv_stride, nk, &sh->dv_stride}};
+  for (const auto& x : strides)
+    if (const int st = check_stride(x.given, x.own, 2, x.to); st != PA_OK) return st;
+  return PA_OK;
+}
+
+int check_paged(const pa_paged_attn_desc* d, pa::PagedShape* sh) {
+  if (!d) return PA_ERR_NULL;
+  if (d->batch <= 0 || d->num_heads <= 0 || d->num_kv_heads <= 0 || d->head_dim <= 0 ||
+      d->num_heads % d->num_kv_heads != 0 || d->page_size <= 0 || d->num_pages <= 0 || d->max_pages <= 0)
+    return PA_ERR_SHAPE;
+  if (d->dtype != PA_BF16 && d->dtype != PA_F32) return PA_ERR_DTYPE;
+  const bool f32 = d->dtype == PA_F32;
+  if (d->head_dim != 64 && d->head_dim != (f32 ? 32 : 128)) return PA_ERR_UNSUPPORTED;
+  // places of a sequence, and of all sequences' key blocks and heads, are counted in ints
+  const long long places = static_cast<long long>(d->max_pages) * d->page_size;
+  if (places > 0x7fffffff - 256 || static_cast<long long>(d->batch) * d->num_heads > 0x7fffffffLL / 256 ||
+      (static_cast<long long>(d->num_pages) * d->page_size) > 0x7fffffffLL)
+    return PA_ERR_SHAPE;
+  if (!(d->softmax_scale <= 0x1p64f)) return PA_ERR_SHAPE;
+  sh->B = d->batch;
+  sh->H = d->num_heads;
+  sh->Hk = d->num_kv_heads;
+  sh->D = d->head_dim;
+  sh->f32 = f32;
+  sh->scale = scale_or_default(d->softmax_scale, d->head_dim);
+  if (!(sh->scale >= 0x1p-64f)) return PA_ERR_SHAPE;
+  sh->page_size = d->page_size;
+  sh->num_pages = d->num_pages;
+  sh->max_pages = d->max_pages;
+  return check_stride(d->q_stride, static_cast<long long>(sh->H) * sh->D, f32 ? 4 : 2, &sh->q_stride);
+}
+
+int check_norm(const pa_qk_norm_desc* d, pa::NormRope* sh) {
+  if (!d) return PA_ERR_NULL;
+  const int st = check_rope_desc(&d->rope, &sh->rope);
+  if (st != PA_OK) return st;
+  const int e = sh->rope.f32 ? 4 : 2;
+  if (sh->rope.D * e % 16 != 0) return PA_ERR_UNSUPPORTED;
+  if (!(d->eps >= 0.f) || !std::isfinite(d->eps)) return PA_ERR_SHAPE;
+  sh->eps = d->eps;
+  const long long nq = static_cast<long long>(sh->rope.Hq) * sh->rope.D,
+                  nk = static_cast<long long>(sh->rope.Hk) * sh->rope.D;
+  const struct { int32_t given; long long own, *to; } strides[] = {
+      {d->q_stride, nq, &sh->q_stride},   {d->k_stride, nk, &sh->k_stride},   {d->v_stride, nk, &sh->v_stride},
+      {d->dq_stride, nq, &sh->dq_stride}, {d->dk_stride, nk, &sh->dk_stride}};
+  for (const auto& x : strides)
+    if (const int t = check_stride(x.given, x.own, e, x.to); t != PA_OK) return t;
+  return PA_OK;
+}
+}  // namespace
+
+extern "C" {
+
+size_t pa_packed_attn_fwd_workspace_size(const pa_packed_attn_desc* desc) {
+  pa::PackedShape sh;
+  return check_packed(desc, &sh) == PA_OK ? pa::packed_attn_fwd_workspace_bytes(sh) : 0;
+}
+
+size_t pa_packed_attn_bwd_workspace_size(const pa_packed_attn_desc* desc) {
+  pa::PackedShape sh;
+  return check_packed(desc, &sh) == PA_OK ? pa::packed_attn_bwd_workspace_bytes(sh) : 0;
+}
+
+int pa_packed_attn_fwd(const pa_packed_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const int32_t* cu_seqlens, void* o, float* lse, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream) {
+  pa::PackedShape sh;
+  int st = check_packed(desc, &sh);
+  if (st != PA_OK) return st;
+  if (!q || !k || !v || !cu_seqlens || !o || !lse) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned4(cu_seqlens) || !aligned4(lse))
+    return PA_ERR_ALIGN;
+  const size_t need = pa::packed_attn_fwd_workspace_bytes(sh);
+  st = check_workspace(need, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  const size_t T = sh.T, q_row = 2ull * sh.H * sh.D, k_row = 2ull * sh.Hk * sh.D;
+  if (!rows_apart({{o, T * q_row}, {lse, 4 * T * sh.H}, {workspace, need}},
+                  {{q, T, q_row, 2ull * sh.q_stride}, {k, T, k_row, 2ull * sh.k_stride},
+                   {v, T, k_row, 2ull * sh.v_stride}, {cu_seqlens, 4ull * (sh.n + 1ull)}}))
+    return PA_ERR_SHAPE;
+  uint32_t* status = status_word();
+  if (!status) return PA_ERR_DEVICE;
+  return pa::launch_packed_attn_fwd(sh, q, k, v, cu_seqlens, o, lse, workspace, status,
+                                    static_cast<cudaStream_t>(stream));
+}
+
+int pa_packed_attn_bwd(const pa_packed_attn_desc* desc, const void* q, const void* k, const void* v,
+                       const void* o, const void* dO, const float* lse, const int32_t* cu_seqlens,
+                       void* dq, void* dk, void* dv, int accumulate, void* workspace,
+                       size_t workspace_bytes, pa_stream_t stream) {
+  pa::PackedShape sh;
+  int st = check_packed(desc, &sh);
+  if (st != PA_OK) return st;
+  if (!q || !k || !v || !o || !dO || !lse || !cu_seqlens || !dq || !dk || !dv) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(dO) || !aligned16(dq) ||
+      !aligned16(dk) || !aligned16(dv) || !aligned4(cu_seqlens) || !aligned4(lse))
+    return PA_ERR_ALIGN;
+  const size_t need = pa::packed_attn_bwd_workspace_bytes(sh);
+  st = check_workspace(need, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  const size_t T = sh.T, q_row = 2ull * sh.H * sh.D, k_row = 2ull * sh.Hk * sh.D;
+  if (!rows_apart({{dq, T, q_row, 2ull * sh.dq_stride}, {dk, T, k_row, 2ull * sh.dk_stride},
+                   {dv, T, k_row, 2ull * sh.dv_stride}, {workspace, need}},
+                  {{q, T, q_row, 2ull * sh.q_stride}, {k, T, k_row, 2ull * sh.k_stride},
+                   {v, T, k_row, 2ull * sh.v_stride}, {o, T * q_row}, {dO, T * q_row}, {lse, 4 * T * sh.H},
+                   {cu_seqlens, 4ull * (sh.n + 1ull)}}))
+    return PA_ERR_SHAPE;
+  uint32_t* status = status_word();
+  if (!status) return PA_ERR_DEVICE;
+  return pa::launch_packed_attn_bwd(sh, q, k, v, o, dO, lse, cu_seqlens, dq, dk, dv, accumulate != 0, workspace,
+                                    status, static_cast<cudaStream_t>(stream));
+}
+
+size_t pa_paged_attn_step_workspace_size(const pa_paged_attn_desc* desc) {
+  pa::PagedShape sh;
+  return check_paged(desc, &sh) == PA_OK ? pa::paged_attn_workspace_bytes(sh) : 0;
+}
+
+int pa_paged_attn_step(const pa_paged_attn_desc* desc, const void* q, const void* k_cache,
+                       const void* v_cache, const int32_t* page_table, const int32_t* seq_lens,
+                       void* o, float* lse, void* workspace, size_t workspace_bytes,
+                       pa_stream_t stream) {
+  pa::PagedShape sh;
+  int st = check_paged(desc, &sh);
+  if (st != PA_OK) return st;
+  if (!q || !k_cache || !v_cache || !page_table || !seq_lens || !o) return PA_ERR_NULL;
+  if (!aligned16(q) || !aligned16(k_cache) || !aligned16(v_cache) || !aligned16(o) || !aligned4(page_table) ||
+      !aligned4(seq_lens) || !aligned4(lse))
+    return PA_ERR_ALIGN;
+  const size_t need = pa::paged_attn_workspace_bytes(sh);
+  st = check_workspace(need, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  const size_t e = sh.f32 ? 4 : 2, q_row = e * sh.H * sh.D,
+               pool = e * sh.num_pages * sh.page_size * sh.Hk * sh.D;
+  if (!rows_apart({{o, sh.B * q_row}, {lse, 4ull * sh.B * sh.H}, {workspace, need}},
+                  {{q, static_cast<size_t>(sh.B), q_row, e * sh.q_stride}, {k_cache, pool}, {v_cache, pool},
+                   {page_table, 4ull * sh.B * sh.max_pages}, {seq_lens, 4ull * sh.B}}))
+    return PA_ERR_SHAPE;
+  return pa::launch_paged_attn(sh, q, k_cache, v_cache, page_table, seq_lens, o, lse, workspace,
+                               static_cast<cudaStream_t>(stream));
+}
+
+// k_out NULL with a cache: k goes into the cache alone.
+static int norm_rope_call(const pa_qk_norm_desc* desc, const void* q, const void* k, const float* gamma_q,
+                          const float* gamma_k, const int32_t* positions, void* q_out, void* k_out,
+                          const pa::NormRopeCache& cache, bool cached, pa_stream_t stream) {
+  pa::NormRope sh;
+  const int st = check_norm(desc, &sh);
+  if (st != PA_OK) return st;
+  const bool has_k = sh.rope.Hk > 0;
+  if (!q || !q_out || !positions || (has_k && !k) || (has_k && !cached && !k_out)) return PA_ERR_NULL;
+  if (cached) {
+    if (!has_k || cache.num_slots <= 0 || cache.num_slots > 0x7fffffffLL) return PA_ERR_SHAPE;
+    if (!cache.v || !cache.slots || !cache.k_cache || !cache.v_cache) return PA_ERR_NULL;
+  }
+  if (!has_k) k = k_out = nullptr;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(cache.v) || !aligned16(q_out) || !aligned16(k_out) ||
+      !aligned16(cache.k_cache) || !aligned16(cache.v_cache) || !aligned16(gamma_q) || !aligned16(gamma_k) ||
+      !aligned4(positions) || !aligned4(cache.slots))
+    return PA_ERR_ALIGN;
+  const size_t e = sh.rope.f32 ? 4 : 2, T = static_cast<size_t>(sh.rope.B) * sh.rope.L,
+               q_row = e * sh.rope.Hq * sh.rope.D, k_row = e * sh.rope.Hk * sh.rope.D, g = 4ull * sh.rope.D;
+  // in place is one contiguous tensor's turn over the whole of itself
+  const bool q_in_place = q == q_out && e * sh.q_stride == q_row, k_in_place = k == k_out && e * sh.k_stride == k_row;
+  if (!rows_apart({{q_out, T * q_row}, {k_out, T * k_row}, {cache.k_cache, cache.num_slots * k_row},
+                   {cache.v_cache, cache.num_slots * k_row}},
+                  {{q_in_place ? nullptr : q, T, q_row, e * sh.q_stride},
+                   {k_in_place ? nullptr : k, T, k_row, e * sh.k_stride},
+                   {cache.v, T, k_row, e * sh.v_stride}, {gamma_q, gamma_q ? g : 0}, {gamma_k, gamma_k ? g : 0},
+                   {positions, 4 * T * sh.rope.axes}, {cache.slots, cache.slots ? 4 * T : 0}}))
+    return PA_ERR_SHAPE;
+  return pa::launch_qk_norm_rope_fwd(sh, q, k, gamma_q, gamma_k, positions, q_out, k_out, cache,
+                                     static_cast<cudaStream_t>(stream));
+}
+
+int pa_qk_norm_rope_fwd(const pa_qk_norm_desc* desc, const void* q, const void* k, const float* gamma_q,
+                        const float* gamma_k, const int32_t* positions, void* q_out, void* k_out,
+                        pa_stream_t stream) {
+  return norm_rope_call(desc, q, k, gamma_q, gamma_k, positions, q_out, k_out, {}, false, stream);
+}
+
+int pa_qk_norm_rope_cache(const pa_qk_norm_desc* desc, const void* q, const void* k, const void* v,
+                          const float* gamma_q, const float* gamma_k, const int32_t* positions,
+                          const int32_t* slots, void* q_out, void* k_out, void* k_cache, void* v_cache,
+                          int64_t num_slots, pa_stream_t stream) {
+  return norm_rope_call(desc, q, k, gamma_q, gamma_k, positions, q_out, k_out,
+                        {v, slots, k_cache, v_cache, num_slots}, true, stream);
+}
+
+size_t pa_qk_norm_rope_bwd_workspace_size(const pa_qk_norm_desc* desc) {
+  pa::NormRope sh;
+  return check_norm(desc, &sh) == PA_OK ? pa::qk_norm_rope_bwd_workspace_bytes(sh) : 0;
+}
+
+int pa_qk_norm_rope_bwd(const pa_qk_norm_desc* desc, const void* dq_out, const void* dk_out,
+                        const void* q, const void* k, const float* gamma_q, const float* gamma_k,
+                        const int32_t* positions, void* dq, void* dk, float* dgamma_q,
+                        float* dgamma_k, int accumulate, void* workspace, size_t workspace_bytes,
+                        pa_stream_t stream) {
+  pa::NormRope sh;
+  int st = check_norm(desc, &sh);
+  if (st != PA_OK) return st;
+  const bool has_k = sh.rope.Hk > 0;
+  if (!dq_out || !q || !positions || !dq || (has_k && (!dk_out || !k || !dk))) return PA_ERR_NULL;
+  if ((dgamma_q && !gamma_q) || (dgamma_k && (!gamma_k || !has_k))) return PA_ERR_NULL;
+  if (!has_k) dk_out = k = dk = nullptr;
+  if (!aligned16(dq_out) || !aligned16(q) || !aligned16(dq) || !aligned16(dk_out) || !aligned16(k) ||
+      !aligned16(dk) || !aligned16(gamma_q) || !aligned16(gamma_k) || !aligned16(dgamma_q) ||
+      !aligned16(dgamma_k) || !aligned4(positions))
+    return PA_ERR_ALIGN;
+  const size_t need = pa::qk_norm_rope_bwd_workspace_bytes(sh);
+  st = check_workspace(need, workspace, workspace_bytes);
+  if (st != PA_OK) return st;
+  const size_t e = sh.rope.f32 ? 4 : 2, T = static_cast<size_t>(sh.rope.B) * sh.rope.L,
+               q_row = e * sh.rope.Hq * sh.rope.D, k_row = e * sh.rope.Hk * sh.rope.D, g = 4ull * sh.rope.D;
+  const bool q_in_place = !accumulate && dq == dq_out && e * sh.dq_stride == q_row,
+             k_in_place = !accumulate && dk == dk_out && e * sh.dk_stride == k_row;
+  if (!rows_apart({{dq, T, q_row, e * sh.dq_stride}, {dk, T, k_row, e * sh.dk_stride}, {dgamma_q, g}, {dgamma_k, g},
+                   {workspace, need}},
+                  {{q_in_place ? nullptr : dq_out, T * q_row}, {k_in_place ? nullptr : dk_out, T * k_row},
+                   {q, T, q_row, e * sh.q_stride}, {k, T, k_row, e * sh.k_stride}, {gamma_q, g}, {gamma_k, g},
+                   {positions, 4 * T * sh.rope.axes}}))
+    return PA_ERR_SHAPE;
+  return pa::launch_qk_norm_rope_bwd(sh, dq_out, dk_out, q, k, gamma_q, gamma_k, positions, dq, dk, dgamma_q,
+                                     dgamma_k, accumulate != 0, workspace, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

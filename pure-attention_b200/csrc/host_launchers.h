@@ -167,3 +167,57 @@ int launch_linear_attn_step(const AttnShape& sh, bool f32, const void* q, const 
                             cudaStream_t s);
 
 }  // namespace pa
+
+namespace pa {
+
+// packed_attn.cu, packed_attn_bwd.cu. Strides in values from one token to the next.
+struct PackedShape {
+  int T, n, H, Hk, D;  // tokens, sequences, heads of q, heads of k and v
+  float scale;
+  long long q_stride, k_stride, v_stride, dq_stride, dk_stride, dv_stride;
+};
+size_t packed_attn_fwd_workspace_bytes(const PackedShape& sh);
+size_t packed_attn_bwd_workspace_bytes(const PackedShape& sh);
+int launch_packed_attn_fwd(const PackedShape& sh, const void* q, const void* k, const void* v,
+                           const int32_t* cu, void* o, float* lse, void* ws, uint32_t* status,
+                           cudaStream_t s);
+int launch_packed_attn_bwd(const PackedShape& sh, const void* q, const void* k, const void* v,
+                           const void* o, const void* dO, const float* lse, const int32_t* cu,
+                           void* dq, void* dk, void* dv, bool accumulate, void* ws,
+                           uint32_t* status, cudaStream_t s);
+
+// paged_attn.cu
+struct PagedShape {
+  int B, H, Hk, D;
+  bool f32;
+  float scale;
+  int page_size, num_pages, max_pages;
+  long long q_stride;
+};
+size_t paged_attn_workspace_bytes(const PagedShape& sh);
+int launch_paged_attn(const PagedShape& sh, const void* q, const void* k_cache, const void* v_cache,
+                      const int32_t* table, const int32_t* lens, void* o, float* lse, void* ws,
+                      cudaStream_t s);
+
+// qk_norm_rope.cu. Null gamma: no norm.
+struct NormRope {
+  RopeShape rope;
+  float eps;
+  long long q_stride, k_stride, v_stride, dq_stride, dk_stride;
+};
+struct NormRopeCache {  // all null: no cache
+  const void* v;
+  const int32_t* slots;
+  void *k_cache, *v_cache;
+  long long num_slots;
+};
+int launch_qk_norm_rope_fwd(const NormRope& sh, const void* q, const void* k, const float* gq,
+                            const float* gk, const int32_t* positions, void* qo, void* ko,
+                            const NormRopeCache& cache, cudaStream_t s);
+size_t qk_norm_rope_bwd_workspace_bytes(const NormRope& sh);
+int launch_qk_norm_rope_bwd(const NormRope& sh, const void* dqo, const void* dko, const void* q,
+                            const void* k, const float* gq, const float* gk, const int32_t* positions,
+                            void* dq, void* dk, float* dgq, float* dgk, bool accumulate, void* ws,
+                            cudaStream_t s);
+
+}  // namespace pa

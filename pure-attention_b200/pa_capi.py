@@ -27,6 +27,9 @@ EXPORTS = [
     "pa_attn_delta",
     "pa_rope_fwd", "pa_rope_bwd", "pa_linear_attn_fwd_workspace_size", "pa_linear_attn_fwd",
     "pa_linear_attn_bwd_workspace_size", "pa_linear_attn_bwd", "pa_linear_attn_step",
+    "pa_packed_attn_fwd_workspace_size", "pa_packed_attn_fwd", "pa_packed_attn_bwd_workspace_size", "pa_packed_attn_bwd",
+    "pa_paged_attn_step_workspace_size", "pa_paged_attn_step",
+    "pa_qk_norm_rope_fwd", "pa_qk_norm_rope_cache", "pa_qk_norm_rope_bwd_workspace_size", "pa_qk_norm_rope_bwd",
     "pa_layer_norm_fwd", "pa_add_layer_norm_fwd", "pa_layer_norm_fwd_planes", "pa_layer_norm_bwd_workspace_size", "pa_layer_norm_bwd",
     "pa_layer_norm_bwd_accumulate", "pa_add_layer_norm_bwd",
     "pa_matmul_workspace_size", "pa_matmul", "pa_matmul_grad_x", "pa_matmul_grad_w",
@@ -59,6 +62,21 @@ class RopeDesc(ctypes.Structure):
                 ("sections", ctypes.c_int32 * 4), ("base", ctypes.c_double)]
 
 
+class PackedAttnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("tokens", "num_seqs", "num_heads", "num_kv_heads", "head_dim", "dtype")] + [
+        ("softmax_scale", ctypes.c_float)] + [(n + "_stride", ctypes.c_int32) for n in ("q", "k", "v", "dq", "dk", "dv")]
+
+
+class PagedAttnDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "num_heads", "num_kv_heads", "head_dim", "dtype")] + [
+        ("softmax_scale", ctypes.c_float)] + [(n, ctypes.c_int32) for n in ("page_size", "num_pages", "max_pages", "q_stride")]
+
+
+class QkNormDesc(ctypes.Structure):
+    _fields_ = [("rope", RopeDesc), ("eps", ctypes.c_float)] + [
+        (n + "_stride", ctypes.c_int32) for n in ("q", "k", "v", "dq", "dk")]
+
+
 _vp = ctypes.c_void_p
 _sz = ctypes.c_size_t
 _u32 = ctypes.c_uint32
@@ -86,6 +104,16 @@ _SIGS = {
     "pa_linear_attn_bwd_workspace_size": (_sz, [ctypes.POINTER(AttnDesc)]),
     "pa_linear_attn_bwd": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 12 + [_int, _vp, _sz, _vp]),
     "pa_linear_attn_step": (_int, [ctypes.POINTER(AttnDesc)] + [_vp] * 8),
+    "pa_packed_attn_fwd_workspace_size": (_sz, [ctypes.POINTER(PackedAttnDesc)]),
+    "pa_packed_attn_fwd": (_int, [ctypes.POINTER(PackedAttnDesc)] + [_vp] * 7 + [_sz, _vp]),
+    "pa_packed_attn_bwd_workspace_size": (_sz, [ctypes.POINTER(PackedAttnDesc)]),
+    "pa_packed_attn_bwd": (_int, [ctypes.POINTER(PackedAttnDesc)] + [_vp] * 10 + [_int, _vp, _sz, _vp]),
+    "pa_paged_attn_step_workspace_size": (_sz, [ctypes.POINTER(PagedAttnDesc)]),
+    "pa_paged_attn_step": (_int, [ctypes.POINTER(PagedAttnDesc)] + [_vp] * 8 + [_sz, _vp]),
+    "pa_qk_norm_rope_fwd": (_int, [ctypes.POINTER(QkNormDesc)] + [_vp] * 8),
+    "pa_qk_norm_rope_cache": (_int, [ctypes.POINTER(QkNormDesc)] + [_vp] * 11 + [ctypes.c_int64, _vp]),
+    "pa_qk_norm_rope_bwd_workspace_size": (_sz, [ctypes.POINTER(QkNormDesc)]),
+    "pa_qk_norm_rope_bwd": (_int, [ctypes.POINTER(QkNormDesc)] + [_vp] * 11 + [_int, _vp, _sz, _vp]),
     "pa_layer_norm_fwd": (_int, [_vp] * 6 + [_u32, _u32, _flt, _vp]),
     "pa_add_layer_norm_fwd": (_int, [_vp] * 8 + [_u32, _u32, _flt, _vp]),
     "pa_layer_norm_fwd_planes": (_int, [_vp] * 8 + [_u32, _u32, _flt, _vp, _sz, _vp]),
@@ -440,6 +468,215 @@ def linear_attn_step(q, k, v, log_decay, state_in, o, state_out, desc=None, stre
     _check("pa_linear_attn_step", load().pa_linear_attn_step(
         ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), log_decay.data_ptr(), state_in.data_ptr(),
         o.data_ptr(), state_out.data_ptr(), _stream() if stream is None else stream))
+
+
+# Descriptors and workspace sizes of the calls below by shape, as above.
+_packed_descs, _paged_descs, _norm_descs, _work_sizes = {}, {}, {}, {}
+
+
+def _token_stride(fn, name, t, heads, D, dev, dtype, tokens):
+    """Values from one token of t [..., heads, D] to the next: a tensor of its own, or a slice of
+    a wider one whose tokens are evenly spaced."""
+    if t.dtype is not dtype or t.dim() < 3 or t.shape[-2:] != (heads, D) or t.numel() != tokens * heads * D:
+        raise ValueError(f"{fn}: {name} must be {dtype} with {tokens} tokens of {heads} heads of {D}, "
+                         f"not {t.dtype} {tuple(t.shape)}")
+    if t.get_device() != dev:
+        raise ValueError(f"{fn}: {name} must be on the first tensor's device, not {t.device}")
+    if t.is_contiguous():
+        return heads * D
+    st, sh = t.stride(), t.shape
+    even = st[-1] == 1 and (heads == 1 or st[-2] == D)
+    step, rows = st[-3] if sh[-3] > 1 else None, sh[-3]
+    for n, d in zip(sh[-4::-1], st[-4::-1]):
+        if n > 1:
+            even = even and (step is None or d == step * rows)
+            step, rows = (d, n) if step is None else (step, rows * n)
+    if not even or (step is not None and step < heads * D):
+        raise ValueError(f"{fn}: {name} must have contiguous heads and evenly spaced tokens, not strides {st}")
+    return heads * D if step is None else step
+
+
+def _work(fn, need, workspace, like, stream):
+    """The call's workspace: the caller's, or one of the stream that will use it."""
+    if workspace is None:
+        import torch
+        if stream is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+        else:
+            with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()):
+                workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        raise ValueError(f"{fn}: workspace must be contiguous and on {like.device}")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def packed_attn_desc(q, k, v, cu_seqlens, dq=None, dk=None, dv=None, scale=0.0):
+    """Descriptor of causal attention over packed sequences: q [T, H, D], k and v [T, Hk, D]
+    (and their gradients), cu_seqlens [sequences + 1]."""
+    T, H, D = q.shape
+    Hk, fn, dev, t = k.shape[1], "packed_attn", q.get_device(), q.dtype
+    stride = lambda name, x, heads: 0 if x is None else _token_stride(fn, name, x, heads, D, dev, t, T)  # noqa: E731
+    strides = (stride("q", q, H), stride("k", k, Hk), stride("v", v, Hk), stride("dq", dq, H), stride("dk", dk, Hk),
+               stride("dv", dv, Hk))
+    key = (T, H, Hk, D, t, cu_seqlens.shape, scale, strides)
+    return _kept(_packed_descs, key, lambda: PackedAttnDesc(T, cu_seqlens.numel() - 1, H, Hk, D, _dtype_code(q),
+                                                            float(scale), *strides))
+
+
+def _size_of(name, d, q):
+    return _kept(_work_sizes, (name, bytes(d), q.get_device()), lambda: getattr(load(), name)(ctypes.byref(d)))
+
+
+def packed_attn_fwd_workspace_size(desc):
+    return load().pa_packed_attn_fwd_workspace_size(ctypes.byref(desc))
+
+
+def packed_attn_bwd_workspace_size(desc):
+    return load().pa_packed_attn_bwd_workspace_size(ctypes.byref(desc))
+
+
+def _check_packed(fn, q, cu_seqlens, lse, names, tensors):
+    import torch
+    dev = q.get_device()
+    T, H, D = q.shape
+    _check_tensors(fn, dev, q.dtype, (T, H, D), names, *tensors)
+    _check_tensors(fn, dev, torch.float32, (H, T), ("lse",), lse)
+    if cu_seqlens.dim() != 1:
+        raise ValueError(f"{fn}: cu_seqlens must have one dimension")
+    _check_tensors(fn, dev, torch.int32, cu_seqlens.shape, ("cu_seqlens",), cu_seqlens)
+    _check_device(fn, q, dev)
+
+
+def packed_attn_fwd(q, k, v, cu_seqlens, o, lse, scale=0.0, workspace=None, stream=None):
+    """o [T, H, D] and lse [H, T] of causal attention over the sequences cu_seqlens[i] ..
+    cu_seqlens[i + 1] - 1 (int32) of q [T, H, D] and k, v [T, Hk, D], whose tokens may be slices
+    of a wider tensor. A workspace is allocated with torch unless given."""
+    d = packed_attn_desc(q, k, v, cu_seqlens, scale=scale)
+    _check_packed("packed_attn_fwd", q, cu_seqlens, lse, ("o",), (o,))
+    ws, nb = _work("packed_attn_fwd", _size_of("pa_packed_attn_fwd_workspace_size", d, q), workspace, q, stream)
+    _check("pa_packed_attn_fwd", load().pa_packed_attn_fwd(
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), o.data_ptr(),
+        lse.data_ptr(), ws.data_ptr(), nb, _stream() if stream is None else stream))
+
+
+def packed_attn_bwd(q, k, v, o, dO, lse, cu_seqlens, dq, dk, dv, accumulate=False, scale=0.0, workspace=None,
+                    stream=None):
+    """Gradients dq, dk, dv (overwritten, or added to) of packed_attn_fwd from dO and its o and lse."""
+    d = packed_attn_desc(q, k, v, cu_seqlens, dq, dk, dv, scale)
+    _check_packed("packed_attn_bwd", q, cu_seqlens, lse, ("o", "dO"), (o, dO))
+    ws, nb = _work("packed_attn_bwd", _size_of("pa_packed_attn_bwd_workspace_size", d, q), workspace, q, stream)
+    _check("pa_packed_attn_bwd", load().pa_packed_attn_bwd(
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dO.data_ptr(), lse.data_ptr(),
+        cu_seqlens.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int(bool(accumulate)), ws.data_ptr(), nb,
+        _stream() if stream is None else stream))
+
+
+def paged_attn_desc(q, k_cache, page_table, scale=0.0):
+    """Descriptor of q [B, H, D] against caches [pages, page size, Hk, D] by page_table [B, pages a sequence]."""
+    B, H, D = q.shape
+    pages, size, Hk, _ = k_cache.shape
+    step = _token_stride("paged_attn_step", "q", q, H, D, q.get_device(), q.dtype, B)
+    key = (q.shape, q.dtype, k_cache.shape, page_table.shape, step, scale)
+    return _kept(_paged_descs, key, lambda: PagedAttnDesc(B, H, Hk, D, _dtype_code(q), float(scale), size, pages,
+                                                          page_table.shape[1], step))
+
+
+def paged_attn_step_workspace_size(desc):
+    return load().pa_paged_attn_step_workspace_size(ctypes.byref(desc))
+
+
+def paged_attn_step(q, k_cache, v_cache, page_table, seq_lens, o, lse=None, scale=0.0, workspace=None, stream=None):
+    """o [B, H, D] (and lse [B, H]) of one token's q of each sequence against its seq_lens (int32 [B])
+    cached tokens, found through page_table (int32 [B, pages a sequence]) in the pools k_cache and
+    v_cache [pages, page size, Hk, D]. A workspace is allocated with torch unless given."""
+    import torch
+    fn, dev = "paged_attn_step", q.get_device()
+    d = paged_attn_desc(q, k_cache, page_table, scale)
+    _check_tensors(fn, dev, q.dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
+    if k_cache.shape[3] != q.shape[2]:
+        raise ValueError(f"{fn}: the caches must have heads of {q.shape[2]}")
+    _check_tensors(fn, dev, torch.int32, (q.shape[0], d.max_pages), ("page_table",), page_table)
+    _check_tensors(fn, dev, torch.int32, q.shape[:1], ("seq_lens",), seq_lens)
+    _check_tensors(fn, dev, q.dtype, q.shape, ("o",), o)
+    if lse is not None:
+        _check_tensors(fn, dev, torch.float32, q.shape[:2], ("lse",), lse)
+    _check_device(fn, q, dev)
+    ws, nb = _work(fn, _size_of("pa_paged_attn_step_workspace_size", d, q), workspace, q, stream)
+    _check("pa_paged_attn_step", load().pa_paged_attn_step(
+        ctypes.byref(d), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
+        seq_lens.data_ptr(), o.data_ptr(), _ptr(lse), ws.data_ptr(), nb, _stream() if stream is None else stream))
+
+
+def _norm_desc(fn, rope, eps, q, k, v, dq, dk, positions, gammas):
+    """The descriptor of a call's tensors; checks those that may be slices, positions and gammas."""
+    import torch
+    B, L, H, Hk, D = rope.batch, rope.seq_len, rope.num_heads, rope.num_kv_heads, rope.head_dim
+    dtype, dev = torch.float32 if rope.dtype == PA_F32 else torch.bfloat16, q.get_device()
+    if (k is None) != (Hk == 0):
+        raise ValueError(f"{fn}: k goes with the descriptor's kv heads")
+    strides = tuple(0 if x is None else _token_stride(fn, name, x, heads, D, dev, dtype, B * L) for name, x, heads in
+                    (("q", q, H), ("k", k, Hk), ("v", v, Hk), ("dq", dq, H), ("dk", dk, Hk)))
+    _check_tensors(fn, dev, torch.int32, (rope.axes, B, L), ("positions",), positions)
+    _check_tensors(fn, dev, torch.float32, (D,), ("gamma_q", "gamma_k", "dgamma_q", "dgamma_k"), *gammas)
+    _check_device(fn, q, dev)
+    return _kept(_norm_descs, (bytes(rope), eps, strides), lambda: QkNormDesc(rope, eps, *strides)), dtype, dev
+
+
+def qk_norm_rope_fwd(q, k, gamma_q, gamma_k, positions, q_out, k_out, desc, eps=1e-6, stream=None):
+    """q_out and k_out: q and k (None: no k) with each head normed by its root mean square and scaled by
+    gamma [D] fp32 (None: not normed), then turned by positions (int32 [axes, B, L]) as desc, a
+    rope_desc, says. q and k [B, L, heads, D] may be slices of a wider tensor, or the outputs."""
+    fn = "qk_norm_rope_fwd"
+    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, None, None, None, positions, (gamma_q, gamma_k))
+    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_heads, desc.head_dim), ("q_out",), q_out)
+    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim), ("k_out",), k_out)
+    _check("pa_qk_norm_rope_fwd", load().pa_qk_norm_rope_fwd(
+        ctypes.byref(d), q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k), positions.data_ptr(), q_out.data_ptr(),
+        _ptr(k_out), _stream() if stream is None else stream))
+
+
+def qk_norm_rope_cache(q, k, v, gamma_q, gamma_k, positions, slots, q_out, k_cache, v_cache, desc, eps=1e-6,
+                       k_out=None, stream=None):
+    """qk_norm_rope_fwd whose k, and v as it is, go to rows slots (int32 [B, L]: page * page size + place;
+    outside the cache: not written) of k_cache and v_cache [pages, page size, Hk, D]; k_out (None: not
+    wanted) receives k too."""
+    import torch
+    fn = "qk_norm_rope_cache"
+    if k is None or v is None:
+        raise ValueError(f"{fn}: k and v are needed")
+    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, v, None, None, positions, (gamma_q, gamma_k))
+    B, L, Hk, D = desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim
+    _check_tensors(fn, dev, dtype, (B, L, desc.num_heads, D), ("q_out",), q_out)
+    _check_tensors(fn, dev, dtype, (B, L, Hk, D), ("k_out",), k_out)
+    _check_tensors(fn, dev, torch.int32, (B, L), ("slots",), slots)
+    if k_cache.dim() != 4 or k_cache.shape[2:] != (Hk, D):
+        raise ValueError(f"{fn}: the caches must be [pages, page size, {Hk}, {D}]")
+    _check_tensors(fn, dev, dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
+    _check("pa_qk_norm_rope_cache", load().pa_qk_norm_rope_cache(
+        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(gamma_q), _ptr(gamma_k),
+        positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.shape[0] * k_cache.shape[1], _stream() if stream is None else stream))
+
+
+def qk_norm_rope_bwd_workspace_size(desc):
+    return load().pa_qk_norm_rope_bwd_workspace_size(ctypes.byref(desc))
+
+
+def qk_norm_rope_bwd(dq_out, dk_out, q, k, gamma_q, gamma_k, positions, dq, dk, dgamma_q, dgamma_k, desc, eps=1e-6,
+                     accumulate=False, workspace=None, stream=None):
+    """Gradients dq, dk and dgamma_q, dgamma_k (None: not wanted) of qk_norm_rope_fwd's inputs from those
+    of its outputs, overwritten or added to. A workspace is allocated with torch unless given."""
+    fn = "qk_norm_rope_bwd"
+    if k is not None and dk is None:
+        raise ValueError(f"{fn}: dk goes with k")
+    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, None, dq, dk, positions, (gamma_q, gamma_k, dgamma_q, dgamma_k))
+    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_heads, desc.head_dim), ("dq_out",), dq_out)
+    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim), ("dk_out",), dk_out)
+    ws, nb = _work(fn, _size_of("pa_qk_norm_rope_bwd_workspace_size", d, q), workspace, q, stream)
+    _check("pa_qk_norm_rope_bwd", load().pa_qk_norm_rope_bwd(
+        ctypes.byref(d), dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k),
+        positions.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dgamma_q), _ptr(dgamma_k), int(bool(accumulate)),
+        ws.data_ptr(), nb, _stream() if stream is None else stream))
 
 
 def device_status(clear=True, stream=None):
