@@ -33,6 +33,7 @@ KERNEL_SOURCES = [
     "rope.cu",
     "linear_attn.cu",
     "packed_attn.cu",
+    "packed_attn_bwd.cu",
     "paged_attn.cu",
     "qk_norm_rope.cu",
     "capi.cu",

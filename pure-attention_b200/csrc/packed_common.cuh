@@ -1,0 +1,79 @@
+// What the kernels of packed causal attention share: the list of their work and
+// the maps of their tensors.
+//
+// A sequence of n tokens has ceil(n / unit) units of `unit` tokens (128 or 256,
+// counted from its own start). A causal unit's work grows with its place: unit i
+// of queries sees keys up to its own end, unit i of keys is seen by queries from
+// its own start. The list holds each sequence's units as (sequence, work), work =
+// 1 .. units, most work first, and a persistent kernel deals it out in turns
+// (snake): every CTA then ends within one unit's work of the others, with no
+// counter shared between CTAs and an order that does not depend on the run.
+#pragma once
+#include "host_launchers.h"
+
+namespace pa {
+
+// An entry: first token, length of the sequence, work (1 .. units of the sequence), sequence.
+struct PackedUnit {
+  int start, len, work, seq;
+};
+struct PackedList {
+  int count;  // entries
+  int pad[63];
+  // PackedUnit units[packed_units(...)], then scratch
+};
+// Most units that sequences of T tokens can have: each has less than one that is not full.
+inline size_t packed_units(const PackedShape& sh, int unit) { return static_cast<size_t>(sh.T) / unit + sh.n; }
+inline size_t packed_list_bytes(const PackedShape& sh, int unit) {
+  return (sizeof(PackedList) + 16 * packed_units(sh, unit) + 8 * static_cast<size_t>(sh.n) + 255) / 256 * 256;
+}
+// packed_attn.cu: writes the list into `list` (packed_list_bytes); the kernel after it may start beside it.
+int launch_packed_list(const PackedShape& sh, const int32_t* cu, int unit, void* list, cudaStream_t s);
+
+__device__ __forceinline__ PackedUnit packed_unit(const PackedList* list, int i) {
+  const int4 u = __ldg(reinterpret_cast<const int4*>(list + 1) + i);
+  return {u.x, u.y, u.z, u.w};
+}
+// Item of a CTA's turn.
+__device__ __forceinline__ long long packed_turn(int turn) {
+  const int c = (turn & 1) ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x);
+  return static_cast<long long>(turn) * gridDim.x + c;
+}
+
+// 3-D TMA map over [T, H, D] bf16 with `stride` values from token to token: box of 64 columns x 1
+// head x 128 tokens, 128-byte swizzle. Tokens past T read as zero.
+inline bool make_packed_map(CUtensorMap* m, const void* base, int T, int H, int D, long long stride) {
+  const uint64_t dims[3] = {static_cast<uint64_t>(D), static_cast<uint64_t>(H), static_cast<uint64_t>(T)};
+  const uint64_t strides[2] = {static_cast<uint64_t>(D) * 2, static_cast<uint64_t>(stride) * 2};
+  const uint32_t box[3] = {64, 1, 128};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// Launches `kernel` so that it may start beside the kernel before it in the stream
+// (it waits for that one's results where it needs them).
+template <typename K, typename... A>
+int launch_beside(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s, A... args) {
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
+// Zeroes rows [from, 128) of a swizzled tile of `chunks` 128-row x 128-byte boxes (one warp), and
+// orders the zeros before the tensor core's reads.
+__device__ __forceinline__ void zero_rows(uint8_t* tile, int chunks, int from) {
+  for (int c = 0; c < chunks; ++c)
+    for (int i = from * 8 + static_cast<int>(lane_id()); i < 128 * 8; i += 32)
+      *reinterpret_cast<uint4*>(tile + c * 16384 + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+}  // namespace pa
