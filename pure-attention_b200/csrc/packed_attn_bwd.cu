@@ -1,118 +1,828 @@
-// Gradients of causal attention over packed sequences with shared key-value heads.
+// Gradients of causal attention over packed sequences with shared key-value
+// heads, for sm_100a: bf16 in, fp32 accumulation in TMEM.
+//
+//   P = exp(S scale - lse),  dP = dO V^T,  Delta = rowsum(dO o),  dS = P (dP - Delta)
+//   dq = scale dS K,   dk = scale sum_heads dS^T Q,   dv = sum_heads P^T dO
+//
+// Two kernels compute S and dP twice (seven products where five would do) so
+// that each output is one accumulator in TMEM with one order of its sum: no fp32 dq
+// is added up in memory, results do not depend on the run, and neither
+// kernel's chain of products waits for the other's.
+//   packed_stats_kernel  Delta and lse log2(e) per (head, query row), laid out in
+//                        blocks of 128 rows of a sequence (rows behind its end: lse =
+//                        +inf, so that their P is 0)
+//   packed_dq_kernel     an item is (query tile, head), walking the key tiles up to
+//                        the diagonal; rows of the products are queries
+//   packed_dkv_kernel    an item is (key tile, kv head), walking the query tiles from
+//                        the diagonal on for each head of the group; rows are keys
+// Both keep P and dS in TMEM as the A operand of the products that use them.
 #include <cuda_bf16.h>
-#include "host_launchers.h"
+#include "packed_common.cuh"
 
 namespace pa {
 namespace {
 
 using bf16 = __nv_bfloat16;
 
-// First and one past the last token of the sequence that holds token t (first = last: none).
-__device__ __forceinline__ int2 sequence_of(const int32_t* cu, int n, int T, int t) {
-  int before = min(max(cu[0], 0), T);
-  for (int i = 0; i < n; ++i) {
-    const int end = min(max(cu[i + 1], before), T);
-    if (t >= before && t < end) return make_int2(before, end);
-    before = end;
-  }
-  return make_int2(0, 0);
+constexpr int kChunk = 128 * 128;  // bytes of one 128-row x 128-byte box
+
+// Rows of the statistics of one head: blocks of 128 rows, each sequence from a block of its own.
+// Sequence i starts at block start_i / 128 + i: every sequence before it has less than one block
+// that is not full.
+__host__ __device__ inline long long stat_blocks(int T, int n) { return static_cast<long long>(T) / 128 + n; }
+__device__ __forceinline__ size_t stat_row(const PackedUnit& u, int tile) {
+  return (static_cast<size_t>(u.start / 128) + u.seq + tile) * 128;
 }
 
-template <int N>
-__device__ __forceinline__ void row(const bf16* p, float (&x)[N]) {
-  for (int i = 0; i < N; ++i) x[i] = __bfloat162float(p[(threadIdx.x & 31) + 32 * i]);
-}
-template <int N>
-__device__ __forceinline__ float dot(const float (&x)[N], const float (&y)[N]) {
-  float s = 0.f;
-  for (int i = 0; i < N; ++i) s += x[i] * y[i];
-  for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-  return s;
-}
-template <int N>
-__device__ __forceinline__ void put(bf16* p, const float (&x)[N], bool add) {
-  for (int i = 0; i < N; ++i) {
-    bf16* at = p + (threadIdx.x & 31) + 32 * i;
-    *at = __float2bfloat16_rn(x[i] + (add ? __bfloat162float(*at) : 0.f));
-  }
-}
+// TMEM column of the k-th 16-column K-step of packed P / dS: each warpgroup packs its 64
+// columns (32 of bf16 pairs) at the start of the 64 fp32 columns that it read.
+__device__ __forceinline__ uint32_t step_col(int k) { return k < 4 ? k * 8 : 64 + (k - 4) * 8; }
 
+// ---------------------------------------------------------------- statistics
 template <int D>
-__global__ void packed_dq_kernel(const PackedShape sh, const bf16* q, const bf16* k, const bf16* v, const bf16* o,
-                                 const bf16* dO, const float* lse, const int32_t* cu, bf16* dq, float* delta, bool add) {
-  const int t = blockIdx.x * 4 + threadIdx.x / 32, h = blockIdx.y, kh = h / (sh.H / sh.Hk);
-  if (t >= sh.T) return;
-  const int2 seq = sequence_of(cu, sh.n, sh.T, t);
-  if (seq.x == seq.y) return;
-  constexpr int N = D / 32;
-  float x[N], y[N], g[N], acc[N] = {};
-  const size_t at = (static_cast<size_t>(t) * sh.H + h) * D;
-  row(o + at, y);
-  row(dO + at, g);
-  const float dl = dot(g, y), z = lse[static_cast<size_t>(h) * sh.T + t];
-  row(q + t * sh.q_stride + h * D, x);
-  for (int j = seq.x; j <= t; ++j) {
-    row(k + j * sh.k_stride + kh * D, y);
-    const float p = __expf(sh.scale * dot(x, y) - z);
-    float w[N];
-    row(v + j * sh.v_stride + kh * D, w);
-    const float ds = sh.scale * p * (dot(g, w) - dl);
-    for (int i = 0; i < N; ++i) acc[i] += ds * y[i];
-  }
-  put(dq + t * sh.dq_stride + h * D, acc, add);
-  if ((threadIdx.x & 31) == 0) delta[static_cast<size_t>(h) * sh.T + t] = dl;
-}
-
-template <int D>
-__global__ void packed_dkv_kernel(const PackedShape sh, const bf16* q, const bf16* k, const bf16* v, const bf16* dO,
-                                  const float* lse, const float* delta, const int32_t* cu, bf16* dk, bf16* dv, bool add) {
-  const int t = blockIdx.x * 4 + threadIdx.x / 32, kh = blockIdx.y, G = sh.H / sh.Hk;
-  if (t >= sh.T) return;
-  const int2 seq = sequence_of(cu, sh.n, sh.T, t);
-  if (seq.x == seq.y) return;
-  constexpr int N = D / 32;
-  float x[N], y[N], w[N], g[N], ak[N] = {}, av[N] = {};
-  row(k + t * sh.k_stride + kh * D, y);
-  row(v + t * sh.v_stride + kh * D, w);
-  for (int h = kh * G; h < kh * G + G; ++h)
-    for (int i = t; i < seq.y; ++i) {
-      row(q + i * sh.q_stride + h * D, x);
-      row(dO + (static_cast<size_t>(i) * sh.H + h) * D, g);
-      const size_t r = static_cast<size_t>(h) * sh.T + i;
-      const float p = __expf(sh.scale * dot(x, y) - lse[r]), ds = sh.scale * p * (dot(g, w) - delta[r]);
-      for (int e = 0; e < N; ++e) {
-        av[e] += p * g[e];
-        ak[e] += ds * x[e];
+__global__ void __launch_bounds__(256)
+    packed_stats_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O, const float* __restrict__ lse,
+                        const PackedList* __restrict__ list, int T, int H, long long rows, float* __restrict__ lse2,
+                        float* __restrict__ delta) {
+  constexpr int LANES = D / 8, STEP = 256 / LANES;  // lanes that share a row; rows of a pass
+  launch_dependents();
+  wait_prerequisites();
+  const long long n = static_cast<long long>(list->count) * H;
+  const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+  for (long long i = blockIdx.x; i < n; i += gridDim.x) {
+    const PackedUnit u = packed_unit(list, static_cast<int>(i / H));
+    const int h = static_cast<int>(i % H), tile = u.work - 1;
+    const size_t out = h * static_cast<size_t>(rows) + stat_row(u, tile);
+    uint4 a[128 / STEP], b[128 / STEP];
+#pragma unroll
+    for (int k = 0; k < 128 / STEP; ++k) {
+      const int row = tile * 128 + r0 + k * STEP;
+      if (row < u.len) {
+        const size_t at = ((static_cast<size_t>(u.start) + row) * H + h) * D + lane * 8;
+        a[k] = *reinterpret_cast<const uint4*>(dO + at);
+        b[k] = *reinterpret_cast<const uint4*>(O + at);
       }
     }
-  put(dk + t * sh.dk_stride + kh * D, ak, add);
-  put(dv + t * sh.dv_stride + kh * D, av, add);
+#pragma unroll
+    for (int k = 0; k < 128 / STEP; ++k) {
+      const int row = tile * 128 + r0 + k * STEP;
+      float s = 0.f;
+      if (row < u.len) {
+        const __nv_bfloat162 *x = reinterpret_cast<const __nv_bfloat162*>(&a[k]),
+                             *y = reinterpret_cast<const __nv_bfloat162*>(&b[k]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 p = __bfloat1622float2(x[e]), q = __bfloat1622float2(y[e]);
+          s = fmaf(p.x, q.x, fmaf(p.y, q.y, s));
+        }
+      }
+#pragma unroll
+      for (int m = LANES / 2; m > 0; m >>= 1) s += __shfl_xor_sync(0xffffffffu, s, m);
+      if (lane == 0) {
+        const int at = r0 + k * STEP;
+        delta[out + at] = s;
+        lse2[out + at] =
+            row < u.len ? lse[static_cast<size_t>(h) * T + u.start + row] * kLog2e : INFINITY;
+      }
+    }
+  }
+}
+
+// What the kernels' issuer knows of a tile of the stream it works through.
+struct StreamTile {
+  int it;  // item
+  bool valid, first, last, ragged;
+};
+
+// ---------------------------------------------------------------- dq
+// TMEM: S0 [0,128) S1 [128,256) dP [256,384) dq [384, 384 + D); dS over its S. Per tile g the
+// issuer runs dP(g+1) as soon as dP(g) is read, then dq(g), then S(g+2) over dS(g): the
+// exponentials of a tile never wait for its scores.
+template <int D>
+struct PackedDq {
+  static constexpr int KCH = D / 64;
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int QBUF = D == 64 ? 2 : 1;  // Q and dO of an item
+  static constexpr int KST = D == 64 ? 4 : 3, VST = D == 64 ? 4 : 2;
+  static constexpr int SMEM = (QBUF * 2 + KST + VST) * TILE + 1024;
+  static constexpr int THREADS = 384;
+  static constexpr uint32_t T_S = 0, T_DP = 256, T_DQ = 384;
+};
+
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    packed_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                     const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
+                     bf16* __restrict__ dq, long long dq_stride, const float* __restrict__ lse2,
+                     const float* __restrict__ delta, const PackedList* __restrict__ list, int H, int group,
+                     long long rows, float scale, float scale_log2, int accumulate, uint32_t* status) {
+  using C = PackedDq<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[32];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  launch_dependents();
+  if (cta_aborted(status, &abort_flag)) {
+    wait_prerequisites();
+    return;
+  }
+  uint8_t* smem = align1024(smem_raw);
+  uint8_t* sQ = smem;  // buffer u: Q, then dO
+  uint8_t* sK = sQ + C::QBUF * 2 * C::TILE;
+  uint8_t* sV = sK + C::KST * C::TILE;
+  auto q_full = [&](int u) { return smem_u32(&bars[0 + u]); };
+  auto q_empty = [&](int u) { return smem_u32(&bars[2 + u]); };
+  auto k_full = [&](int s) { return smem_u32(&bars[4 + s]); };
+  auto k_empty = [&](int s) { return smem_u32(&bars[8 + s]); };
+  auto v_full = [&](int s) { return smem_u32(&bars[12 + s]); };
+  auto v_empty = [&](int s) { return smem_u32(&bars[16 + s]); };
+  // By tile parity where the arriving side can be a tile ahead of the waiting one.
+  auto s_full = [&](int g) { return smem_u32(&bars[20 + (g & 1)]); };
+  auto ds_full = [&](int g) { return smem_u32(&bars[22 + (g & 1)]); };
+  const uint32_t dp_full = smem_u32(&bars[24]), dp_free = smem_u32(&bars[25]), dq_done = smem_u32(&bars[26]);
+  // the f-th ragged K tile has landed, and its rows behind the end are zero
+  auto k_ragged = [&](int f) { return smem_u32(&bars[27 + (f & 1)]); };
+  auto k_zeroed = [&](int f) { return smem_u32(&bars[29 + (f & 1)]); };
+
+  const int warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(q_full(u), 1);
+      mbar_init(q_empty(u), 1);
+      mbar_init(s_full(u), 1);
+      mbar_init(ds_full(u), 256);
+      mbar_init(k_ragged(u), 1);
+      mbar_init(k_zeroed(u), 1);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(k_full(s), 1);
+      mbar_init(k_empty(s), 1);
+      mbar_init(v_full(s), 1);
+      mbar_init(v_empty(s), 1);
+    }
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, 256);
+    mbar_init(dq_done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  wait_prerequisites();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const long long n_items = static_cast<long long>(list->count) * H;
+  auto unit_of = [&](int turn) {
+    const long long i = packed_turn(turn);
+    return i < n_items ? packed_unit(list, static_cast<int>(i / H)) : PackedUnit{0, 0, 0, 0};
+  };
+  auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % H); };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      tma_prefetch_desc(&mapQ);
+      tma_prefetch_desc(&mapK);
+      tma_prefetch_desc(&mapV);
+      tma_prefetch_desc(&mapdO);
+      bool ok = true;
+      PackedUnit next = unit_of(0);
+      int it = 0, g = 0, nv = 0;
+      for (; ok && next.work; ++it) {
+        const PackedUnit u = next;
+        const int h = head_of(it), kh = h / group, row = u.start + (u.work - 1) * 128;
+        next = unit_of(it + 1);
+        const int b = it % C::QBUF, k = it / C::QBUF;
+        if (k > 0 && !(ok = mbar_wait(q_empty(b), (k - 1) & 1, status))) break;
+        mbar_arrive_expect_tx(q_full(b), 2 * C::TILE);
+        for (int c = 0; c < C::KCH; ++c) {
+          tma_load_3d(smem_u32(sQ + b * 2 * C::TILE + c * kChunk), &mapQ, q_full(b), c * 64, h, row);
+          tma_load_3d(smem_u32(sQ + (b * 2 + 1) * C::TILE + c * kChunk), &mapdO, q_full(b), c * 64, h, row);
+        }
+        for (int j = 0; j < u.work; ++j) {
+          int s = g % C::KST;
+          if (g >= C::KST && !(ok = mbar_wait(k_empty(s), ((g / C::KST) - 1) & 1, status))) break;
+          mbar_arrive_expect_tx(k_full(s), C::TILE);
+          for (int c = 0; c < C::KCH; ++c)
+            tma_load_3d(smem_u32(sK + s * C::TILE + c * kChunk), &mapK, k_full(s), c * 64, kh, u.start + j * 128);
+          ++g;
+          s = nv % C::VST;
+          if (nv >= C::VST && !(ok = mbar_wait(v_empty(s), ((nv / C::VST) - 1) & 1, status))) break;
+          mbar_arrive_expect_tx(v_full(s), C::TILE);
+          for (int c = 0; c < C::KCH; ++c)
+            tma_load_3d(smem_u32(sV + s * C::TILE + c * kChunk), &mapV, v_full(s), c * 64, kh, u.start + j * 128);
+          ++nv;
+        }
+      }
+      if (!ok) {  // copies in flight land before the block ends
+        for (int i = max(0, it - C::QBUF + 1); i <= it; ++i) mbar_drain(q_full(i % C::QBUF), (i / C::QBUF) & 1);
+        for (int i = max(0, g - C::KST); i < g; ++i) mbar_drain(k_full(i % C::KST), (i / C::KST) & 1);
+        for (int i = max(0, nv - C::VST); i < nv; ++i) mbar_drain(v_full(i % C::VST), (i / C::VST) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idS = make_idesc(128, 128, 1, false, false);
+      constexpr uint32_t idQ = make_idesc(128, D, 1, false, true);
+      const uint64_t dQ0 = make_sdesc(smem_u32(sQ), 16, 1024);
+      const uint64_t dK0 = make_sdesc(smem_u32(sK), 16, 1024);
+      const uint64_t dV0 = make_sdesc(smem_u32(sV), 16, 1024);
+      const uint64_t dK_MN = make_sdesc(smem_u32(sK), kChunk, 1024);
+      auto product = [&](uint32_t to, uint64_t a, uint64_t b) {  // K-major x K-major over D
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k / 4) * kChunk + (k % 4) * 32) >> 4;
+          umma_f16_ss(to, a + off, b + off, idS, k > 0 ? 1u : 0u);
+        }
+      };
+      bool ok = true;
+      PackedUnit unit = unit_of(0);
+      int turn = 0, left = unit.work;  // tiles of the item still to come
+      auto next_tile = [&] {
+        StreamTile t = {turn, unit.work > 0, left == unit.work, left == 1,
+                        left == 1 && unit.work * 128 > unit.len};
+        if (t.valid && --left == 0) {
+          unit = unit_of(++turn);
+          left = unit.work;
+        }
+        return t;
+      };
+      int rg = 0, rz = 0;  // ragged tiles announced, waited for
+      auto issue_S = [&](const StreamTile& t, int g) {
+        if (t.first && !mbar_wait(q_full(t.it % C::QBUF), (t.it / C::QBUF) & 1, status)) return false;
+        if (!mbar_wait(k_full(g % C::KST), (g / C::KST) & 1, status)) return false;
+        if (t.ragged) mbar_arrive(k_ragged(rg++));
+        tc_fence_after();
+        product(tmem + C::T_S + (g & 1) * 128, dQ0 + (((t.it % C::QBUF) * 2 * C::TILE) >> 4),
+                dK0 + (((g % C::KST) * C::TILE) >> 4));
+        umma_commit(s_full(g));
+        return true;
+      };
+      auto issue_dP = [&](const StreamTile& t, int g) {
+        if (!mbar_wait(v_full(g % C::VST), (g / C::VST) & 1, status)) return false;
+        tc_fence_after();
+        product(tmem + C::T_DP, dQ0 + ((((t.it % C::QBUF) * 2 + 1) * C::TILE) >> 4),
+                dV0 + (((g % C::VST) * C::TILE) >> 4));
+        umma_commit(dp_full);
+        umma_commit(v_empty(g % C::VST));
+        if (t.last) umma_commit(q_empty(t.it % C::QBUF));  // (its last S was issued before)
+        return true;
+      };
+      StreamTile a = next_tile(), b = next_tile();
+      if (a.valid) ok = issue_S(a, 0) && issue_dP(a, 0) && (!b.valid || issue_S(b, 1));
+      for (int g = 0; ok && a.valid; ++g) {
+        if (b.valid && !(ok = mbar_wait(dp_free, g & 1, status) && issue_dP(b, g + 1))) break;
+        if (!(ok = mbar_wait(ds_full(g), (g >> 1) & 1, status))) break;
+        if (a.ragged) {
+          if (!(ok = mbar_wait(k_zeroed(rz), (rz >> 1) & 1, status))) break;
+          ++rz;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16_ts(tmem + C::T_DQ, tmem + C::T_S + (g & 1) * 128 + step_col(k),
+                      dK_MN + (((g % C::KST) * C::TILE + k * 2048) >> 4), idQ, (!a.first || k > 0) ? 1u : 0u);
+        umma_commit(k_empty(g % C::KST));
+        if (a.last) umma_commit(dq_done);
+        const StreamTile c = next_tile();
+        if (c.valid && !(ok = issue_S(c, g + 2))) break;
+        a = b;
+        b = c;
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ rows behind a sequence's end
+    PackedUnit next = unit_of(0);
+    int g = 0, f = 0;
+    for (int it = 0; next.work; ++it) {
+      const PackedUnit u = next;
+      next = unit_of(it + 1);
+      g += u.work;
+      if (u.work * 128 <= u.len) continue;
+      if (!mbar_wait_warp(k_ragged(f), (f >> 1) & 1, status)) break;
+      zero_rows(sK + ((g - 1) % C::KST) * C::TILE, C::KCH, u.len - (u.work - 1) * 128);
+      if (lane_id() == 0) mbar_arrive(k_zeroed(f));
+      ++f;
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ P and dS
+    // Warpgroup grp: keys [64 grp, 64 grp + 64) of each tile; thread = query row.
+    const int grp = (warp - 4) >> 2;
+    const int r = ((warp & 3) << 5) + static_cast<int>(lane_id());
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tdP = tmem + C::T_DP + lane_base + grp * 64;
+    bool ok = true;
+    PackedUnit next = unit_of(0);
+    auto stats = [&](const PackedUnit& u, int turn) {
+      if (!u.work) return make_float2(0.f, 0.f);
+      const size_t at = head_of(turn) * static_cast<size_t>(rows) + stat_row(u, u.work - 1) + r;
+      return make_float2(lse2[at], delta[at]);
+    };
+    float2 st_next = stats(next, 0);
+    int g = 0;
+    for (int it = 0; ok && next.work; ++it) {
+      const PackedUnit u = next;
+      const float neg_lse = -st_next.x, del = st_next.y;
+      next = unit_of(it + 1);
+      st_next = stats(next, it + 1);
+      for (int j = 0; j < u.work; ++j, ++g) {
+        const uint32_t tS = tmem + C::T_S + (g & 1) * 128 + lane_base + grp * 64;
+        if (!(ok = mbar_wait_warp(s_full(g), (g >> 1) & 1, status))) break;
+        tc_fence_after();
+        float p[64];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(p[i], scale_log2, neg_lse));
+        if (!(ok = mbar_wait_warp(dp_full, g & 1, status))) break;
+        tc_fence_after();
+        uint32_t ds[32];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_ld32_sync(tdP + c * 32, v);
+          if (c == 1) {
+            tc_fence_before();
+            mbar_arrive(dp_free);  // the next dP may overwrite it
+          }
+          if (j == u.work - 1) {  // the block on the diagonal
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float x = p[c * 32 + i] * (__uint_as_float(v[i]) - del);
+              v[i] = __float_as_uint(grp * 64 + c * 32 + i > r ? 0.f : x);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              v[i] = __float_as_uint(p[c * 32 + i] * (__uint_as_float(v[i]) - del));
+          }
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            ds[c * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+        }
+        tmem_st32(tS, ds);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(ds_full(g));
+      }
+      if (!ok || !(ok = mbar_wait_warp(dq_done, it & 1, status))) break;
+      // dq write-back: each warpgroup half of the columns. The loads complete before
+      // this thread's next ds_full, which the next item's first product into dq waits for.
+      tc_fence_after();
+      const int row = (u.work - 1) * 128 + r;
+      bf16* dst = dq + (static_cast<size_t>(u.start) + row) * dq_stride + static_cast<size_t>(head_of(it)) * D;
+#pragma unroll 1
+      for (int c = grp * (D / 64); c < (grp + 1) * (D / 64); ++c) {
+        uint32_t o[32];
+        tmem_ld32_sync(tmem + C::T_DQ + lane_base + c * 32, o);
+        if (row < u.len) {
+          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * scale;
+            if (accumulate) {
+              const uint4 old = d4[i];
+              const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 pf = __bfloat1622float2(p2[e]);
+                f[2 * e] += pf.x;
+                f[2 * e + 1] += pf.y;
+              }
+            }
+            d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                               pack_bf16x2(f[6], f[7]));
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ---------------------------------------------------------------- dk, dv
+// TMEM, d = 64: S0 [0,128) S1 [128,256) dP [256,384) dv [384,448) dk [448,512); d = 128: S [0,128)
+// dP [128,256) dv [256,384) dk [384,512). P^T over its S, dS^T over dP. Per tile g: dv(g) and the
+// next S into the same columns once P^T(g) is there, dk(g) and dP(g+1) once dS^T(g) is.
+template <int D>
+struct PackedDkv {
+  static constexpr int KCH = D / 64;
+  static constexpr int TILE = 128 * D * 2;
+  static constexpr int SBUF = D == 64 ? 2 : 1;
+  static constexpr int KVBUF = D == 64 ? 2 : 1;  // K and V of an item
+  static constexpr int QST = D == 64 ? 4 : 2, OST = D == 64 ? 3 : 2;
+  static constexpr int SMEM = (KVBUF * 2 + QST + OST) * TILE + QST * 1024 + 1024;
+  static constexpr int THREADS = 384;
+  static constexpr uint32_t T_S = 0, T_DP = 128 * SBUF, T_DV = T_DP + 128, T_DK = T_DV + D;
+};
+
+template <int D>
+__global__ void __launch_bounds__(384, 1)
+    packed_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
+                      const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
+                      bf16* __restrict__ dk, bf16* __restrict__ dv, long long dk_stride, long long dv_stride,
+                      const float* __restrict__ lse2, const float* __restrict__ delta,
+                      const PackedList* __restrict__ list, int Hk, int group, long long rows, float scale,
+                      float scale_log2, int accumulate, uint32_t* status) {
+  using C = PackedDkv<D>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[32];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  if (cta_aborted(status, &abort_flag)) {
+    wait_prerequisites();
+    return;
+  }
+  uint8_t* smem = align1024(smem_raw);
+  uint8_t* sKV = smem;  // buffer b: K, then V
+  uint8_t* sQ = sKV + C::KVBUF * 2 * C::TILE;
+  uint8_t* sO = sQ + C::QST * C::TILE;
+  uint8_t* sStat = sO + C::OST * C::TILE;  // stage s: lse2 and Delta of 128 queries
+  auto kv_full = [&](int b) { return smem_u32(&bars[0 + b]); };
+  auto kv_empty = [&](int b) { return smem_u32(&bars[2 + b]); };
+  auto q_full = [&](int s) { return smem_u32(&bars[4 + s]); };
+  auto q_empty = [&](int s) { return smem_u32(&bars[8 + s]); };
+  auto o_full = [&](int s) { return smem_u32(&bars[12 + s]); };
+  auto o_empty = [&](int s) { return smem_u32(&bars[15 + s]); };
+  auto ready = [&](int s) { return smem_u32(&bars[18 + s]); };  // Q and dO of a tile, rows behind the end zero
+  // By tile parity where the arriving side can be a tile ahead of the waiting one.
+  auto s_full = [&](int g) { return smem_u32(&bars[22 + (g & 1)]); };
+  auto p_full = [&](int g) { return smem_u32(&bars[24 + (g & 1)]); };
+  const uint32_t dp_full = smem_u32(&bars[26]), ds_full = smem_u32(&bars[27]), acc_done = smem_u32(&bars[28]);
+
+  const int warp = warp_id();
+  if (threadIdx.x == 0) {
+    for (int u = 0; u < 2; ++u) {
+      mbar_init(kv_full(u), 1);
+      mbar_init(kv_empty(u), 1);
+      mbar_init(s_full(u), 1);
+      mbar_init(p_full(u), 256);
+    }
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(q_full(s), 1);
+      mbar_init(q_empty(s), 1);
+      mbar_init(ready(s), 1);
+    }
+    for (int s = 0; s < 3; ++s) {
+      mbar_init(o_full(s), 1);
+      mbar_init(o_empty(s), 1);
+    }
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, 256);
+    mbar_init(acc_done, 1);
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(&tmem_slot), 512);
+    tmem_relinquish();
+  }
+  wait_prerequisites();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const long long n_items = static_cast<long long>(list->count) * Hk;
+  auto unit_of = [&](int turn) {
+    const long long i = packed_turn(turn);
+    return i < n_items ? packed_unit(list, static_cast<int>(i / Hk)) : PackedUnit{0, 0, 0, 0};
+  };
+  auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % Hk); };
+  // Unit of work w: key tile (tiles of the sequence) - w, seen by the w query tiles from its own on.
+  auto tiles_of = [](const PackedUnit& u) { return (u.len + 127) / 128; };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    if (elect_one()) {
+      tma_prefetch_desc(&mapQ);
+      tma_prefetch_desc(&mapK);
+      tma_prefetch_desc(&mapV);
+      tma_prefetch_desc(&mapdO);
+      bool ok = true;
+      PackedUnit next = unit_of(0);
+      int it = 0, g = 0, go = 0;
+      for (; ok && next.work; ++it) {
+        const PackedUnit u = next;
+        const int kh = head_of(it), first = tiles_of(u) - u.work;
+        next = unit_of(it + 1);
+        const int b = it % C::KVBUF, k = it / C::KVBUF;
+        if (k > 0 && !(ok = mbar_wait(kv_empty(b), (k - 1) & 1, status))) break;
+        mbar_arrive_expect_tx(kv_full(b), 2 * C::TILE);
+        for (int c = 0; c < C::KCH; ++c) {
+          tma_load_3d(smem_u32(sKV + b * 2 * C::TILE + c * kChunk), &mapK, kv_full(b), c * 64, kh,
+                      u.start + first * 128);
+          tma_load_3d(smem_u32(sKV + (b * 2 + 1) * C::TILE + c * kChunk), &mapV, kv_full(b), c * 64, kh,
+                      u.start + first * 128);
+        }
+        for (int h = kh * group; ok && h < (kh + 1) * group; ++h)
+          for (int j = first; j < first + u.work; ++j) {
+            int s = g % C::QST;
+            if (g >= C::QST && !(ok = mbar_wait(q_empty(s), ((g / C::QST) - 1) & 1, status))) break;
+            mbar_arrive_expect_tx(q_full(s), C::TILE + 1024);
+            for (int c = 0; c < C::KCH; ++c)
+              tma_load_3d(smem_u32(sQ + s * C::TILE + c * kChunk), &mapQ, q_full(s), c * 64, h, u.start + j * 128);
+            const size_t at = h * static_cast<size_t>(rows) + stat_row(u, j);
+            bulk_load(smem_u32(sStat + s * 1024), lse2 + at, 512, q_full(s));
+            bulk_load(smem_u32(sStat + s * 1024 + 512), delta + at, 512, q_full(s));
+            ++g;
+            s = go % C::OST;
+            if (go >= C::OST && !(ok = mbar_wait(o_empty(s), ((go / C::OST) - 1) & 1, status))) break;
+            mbar_arrive_expect_tx(o_full(s), C::TILE);
+            for (int c = 0; c < C::KCH; ++c)
+              tma_load_3d(smem_u32(sO + s * C::TILE + c * kChunk), &mapdO, o_full(s), c * 64, h, u.start + j * 128);
+            ++go;
+          }
+      }
+      if (!ok) {  // copies in flight land before the block ends
+        for (int i = max(0, it - C::KVBUF + 1); i <= it; ++i) mbar_drain(kv_full(i % C::KVBUF), (i / C::KVBUF) & 1);
+        for (int i = max(0, g - C::QST); i < g; ++i) mbar_drain(q_full(i % C::QST), (i / C::QST) & 1);
+        for (int i = max(0, go - C::OST); i < go; ++i) mbar_drain(o_full(i % C::OST), (i / C::OST) & 1);
+      }
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer
+    if (elect_one()) {
+      constexpr uint32_t idS = make_idesc(128, 128, 1, false, false);
+      constexpr uint32_t idG = make_idesc(128, D, 1, false, true);
+      const uint64_t dKV0 = make_sdesc(smem_u32(sKV), 16, 1024);
+      const uint64_t dQ0 = make_sdesc(smem_u32(sQ), 16, 1024);
+      const uint64_t dO0 = make_sdesc(smem_u32(sO), 16, 1024);
+      const uint64_t dQ_MN = make_sdesc(smem_u32(sQ), kChunk, 1024);
+      const uint64_t dO_MN = make_sdesc(smem_u32(sO), kChunk, 1024);
+      auto product = [&](uint32_t to, uint64_t a, uint64_t b) {  // K-major x K-major over D
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k / 4) * kChunk + (k % 4) * 32) >> 4;
+          umma_f16_ss(to, a + off, b + off, idS, k > 0 ? 1u : 0u);
+        }
+      };
+      auto add_to = [&](uint32_t to, uint32_t a, uint64_t b, bool fresh) {  // A from TMEM, over 128 queries
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          umma_f16_ts(to, a + step_col(k), b + ((k * 2048) >> 4), idG, (!fresh || k > 0) ? 1u : 0u);
+      };
+      bool ok = true;
+      PackedUnit unit = unit_of(0);
+      int turn = 0, left = unit.work * group;
+      auto next_tile = [&] {
+        StreamTile t = {turn, unit.work > 0, left == unit.work * group, left == 1, false};
+        if (t.valid && --left == 0) {
+          unit = unit_of(++turn);
+          left = unit.work * group;
+        }
+        return t;
+      };
+      auto issue_S = [&](const StreamTile& t, int g) {
+        const int b = t.it % C::KVBUF;
+        if (t.first && !mbar_wait(kv_full(b), (t.it / C::KVBUF) & 1, status)) return false;
+        if (!mbar_wait(ready(g % C::QST), (g / C::QST) & 1, status)) return false;
+        tc_fence_after();
+        product(tmem + C::T_S + (g % C::SBUF) * 128, dKV0 + ((b * 2 * C::TILE) >> 4),
+                dQ0 + (((g % C::QST) * C::TILE) >> 4));
+        umma_commit(s_full(g));
+        return true;
+      };
+      auto issue_dP = [&](const StreamTile& t, int g) {
+        const int b = t.it % C::KVBUF;
+        product(tmem + C::T_DP, dKV0 + (((b * 2 + 1) * C::TILE) >> 4), dO0 + (((g % C::OST) * C::TILE) >> 4));
+        umma_commit(dp_full);
+        if (t.last) umma_commit(kv_empty(b));  // (its last S was issued before)
+      };
+      StreamTile a = next_tile(), b = next_tile();
+      if (a.valid && (ok = issue_S(a, 0))) {
+        issue_dP(a, 0);
+        if (C::SBUF == 2 && b.valid) ok = issue_S(b, 1);
+      }
+      for (int g = 0; ok && a.valid; ++g) {
+        if (!(ok = mbar_wait(p_full(g), (g >> 1) & 1, status))) break;
+        tc_fence_after();
+        add_to(tmem + C::T_DV, tmem + C::T_S + (g % C::SBUF) * 128, dO_MN + (((g % C::OST) * C::TILE) >> 4), a.first);
+        umma_commit(o_empty(g % C::OST));
+        // the next S over P^T(g), in order behind dv(g); with one K / V buffer the first S of an
+        // item waits for its keys behind dk(g)
+        const StreamTile c = C::SBUF == 2 ? next_tile() : b;
+        const bool late = C::KVBUF == 1 && c.first;
+        if (c.valid && !late && !(ok = issue_S(c, g + C::SBUF))) break;
+        if (!(ok = mbar_wait(ds_full, g & 1, status))) break;
+        tc_fence_after();
+        add_to(tmem + C::T_DK, tmem + C::T_DP, dQ_MN + (((g % C::QST) * C::TILE) >> 4), a.first);
+        umma_commit(q_empty(g % C::QST));
+        if (a.last) umma_commit(acc_done);
+        if (c.valid && late && !(ok = issue_S(c, g + C::SBUF))) break;
+        if (b.valid) issue_dP(b, g + 1);  // (waited for with its S)
+        a = b;
+        b = C::SBUF == 2 ? c : next_tile();
+      }
+    }
+  } else if (warp == 2) {
+    // ------------------------------------------------------------ rows behind a sequence's end
+    // Queries there are zero, with lse = +inf: their P and dS are 0 whatever lies behind the sequence.
+    bool ok = true;
+    PackedUnit next = unit_of(0);
+    int g = 0;
+    for (int it = 0; ok && next.work; ++it) {
+      const PackedUnit u = next;
+      const int n = tiles_of(u), first = n - u.work;
+      next = unit_of(it + 1);
+      for (int h = 0; ok && h < group; ++h)
+        for (int j = first; j < n; ++j, ++g) {
+          if (!(ok = mbar_wait_warp(q_full(g % C::QST), (g / C::QST) & 1, status) &&
+                     mbar_wait_warp(o_full(g % C::OST), (g / C::OST) & 1, status)))
+            break;
+          if ((j + 1) * 128 > u.len) {
+            zero_rows(sQ + (g % C::QST) * C::TILE, C::KCH, u.len - j * 128);
+            zero_rows(sO + (g % C::OST) * C::TILE, C::KCH, u.len - j * 128);
+          }
+          if (lane_id() == 0) mbar_arrive(ready(g % C::QST));
+        }
+    }
+  } else if (warp >= 4) {
+    // ------------------------------------------------------------ P^T and dS^T
+    // Warpgroup grp: queries [64 grp, 64 grp + 64) of each tile; thread = key row.
+    const int grp = (warp - 4) >> 2;
+    const int r = ((warp & 3) << 5) + static_cast<int>(lane_id());
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t tdP = tmem + C::T_DP + lane_base + grp * 64;
+    bool ok = true;
+    PackedUnit next = unit_of(0);
+    int g = 0;
+    for (int it = 0; ok && next.work; ++it) {
+      const PackedUnit u = next;
+      next = unit_of(it + 1);
+      int j = 0;  // query tile of the head, from the diagonal on
+      for (int i = 0; i < u.work * group; ++i, ++g) {
+        const uint32_t tS = tmem + C::T_S + (g % C::SBUF) * 128 + lane_base + grp * 64;
+        const float* lse2s = reinterpret_cast<const float*>(sStat + (g % C::QST) * 1024) + grp * 64;
+        const float* dels = lse2s + 128;
+        if (!(ok = mbar_wait_warp(q_full(g % C::QST), (g / C::QST) & 1, status) &&
+                   mbar_wait_warp(s_full(g), (g >> 1) & 1, status)))
+          break;
+        tc_fence_after();
+        float p[64];
+        uint32_t pk[32];
+        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < 16; ++c) {
+          const float4 z = *reinterpret_cast<const float4*>(lse2s + 4 * c);
+          p[4 * c] = ex2(fmaf(p[4 * c], scale_log2, -z.x));
+          p[4 * c + 1] = ex2(fmaf(p[4 * c + 1], scale_log2, -z.y));
+          p[4 * c + 2] = ex2(fmaf(p[4 * c + 2], scale_log2, -z.z));
+          p[4 * c + 3] = ex2(fmaf(p[4 * c + 3], scale_log2, -z.w));
+        }
+        const bool diagonal = j == 0;
+        if (++j == u.work) j = 0;
+        if (diagonal) {
+#pragma unroll
+          for (int e = 0; e < 64; ++e)
+            if (grp * 64 + e < r) p[e] = 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e) pk[e] = pack_bf16x2(p[2 * e], p[2 * e + 1]);
+        tmem_st32(tS, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(p_full(g));
+        if (!(ok = mbar_wait_warp(dp_full, g & 1, status))) break;
+        tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          uint32_t v[32];
+          tmem_ld32_sync(tdP + c * 32, v);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float4 z = *reinterpret_cast<const float4*>(dels + c * 32 + 4 * e);
+            float x[4] = {__uint_as_float(v[4 * e]) - z.x, __uint_as_float(v[4 * e + 1]) - z.y,
+                          __uint_as_float(v[4 * e + 2]) - z.z, __uint_as_float(v[4 * e + 3]) - z.w};
+            if (diagonal) {
+#pragma unroll
+              for (int k = 0; k < 4; ++k)
+                if (grp * 64 + c * 32 + 4 * e + k < r) x[k] = 0.f;
+            }
+            pk[c * 16 + 2 * e] = pack_bf16x2(p[c * 32 + 4 * e] * x[0], p[c * 32 + 4 * e + 1] * x[1]);
+            pk[c * 16 + 2 * e + 1] = pack_bf16x2(p[c * 32 + 4 * e + 2] * x[2], p[c * 32 + 4 * e + 3] * x[3]);
+          }
+        }
+        tmem_st32(tdP, pk);
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(ds_full);
+      }
+      if (!ok || !(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
+      // Write-back: warpgroup 0 dv, warpgroup 1 dk. The loads complete before this thread's next
+      // p_full, which the next item's first products into dv and dk wait for.
+      tc_fence_after();
+      const int row = (tiles_of(u) - u.work) * 128 + r;
+      const size_t token = static_cast<size_t>(u.start) + row, col = static_cast<size_t>(head_of(it)) * D;
+      bf16* dst = grp == 0 ? dv + token * dv_stride + col : dk + token * dk_stride + col;
+      const uint32_t src = tmem + (grp == 0 ? C::T_DV : C::T_DK) + lane_base;
+      const float mul = grp == 0 ? 1.f : scale;
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t o[32];
+        tmem_ld32_sync(src + c * 32, o);
+        if (row < u.len) {
+          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float f[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * mul;
+            if (accumulate) {
+              const uint4 old = d4[i];
+              const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const float2 pf = __bfloat1622float2(p2[e]);
+                f[2 * e] += pf.x;
+                f[2 * e + 1] += pf.y;
+              }
+            }
+            d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                               pack_bf16x2(f[6], f[7]));
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+size_t stat_bytes(const PackedShape& sh) {
+  return (static_cast<size_t>(stat_blocks(sh.T, sh.n)) * 128 * sh.H * sizeof(float) + 255) / 256 * 256;
+}
+
+template <int D>
+int packed_bwd(const PackedShape& sh, const void* q, const void* k, const void* v, const void* o, const void* dO,
+               const float* lse, const int32_t* cu, void* dq, void* dk, void* dv, bool accumulate, void* ws,
+               uint32_t* status, cudaStream_t s) {
+  CUtensorMap mq, mk, mv, mo;
+  if (!make_packed_map(&mq, q, sh.T, sh.H, D, sh.q_stride) || !make_packed_map(&mk, k, sh.T, sh.Hk, D, sh.k_stride) ||
+      !make_packed_map(&mv, v, sh.T, sh.Hk, D, sh.v_stride) ||
+      !make_packed_map(&mo, dO, sh.T, sh.H, D, static_cast<long long>(sh.H) * D))
+    return PA_ERR_ALIGN;
+  static std::atomic<uint64_t> attr_dq{0}, attr_dkv{0};
+  if (!ensure_smem_attr(packed_dq_kernel<D>, PackedDq<D>::SMEM, attr_dq) ||
+      !ensure_smem_attr(packed_dkv_kernel<D>, PackedDkv<D>::SMEM, attr_dkv))
+    return PA_ERR_LAUNCH;
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  const PackedList* list = reinterpret_cast<const PackedList*>(w);
+  float* lse2 = reinterpret_cast<float*>(w + packed_list_bytes(sh, 128));
+  float* delta = reinterpret_cast<float*>(w + packed_list_bytes(sh, 128) + stat_bytes(sh));
+  const long long rows = stat_blocks(sh.T, sh.n) * 128;
+  const int group = sh.H / sh.Hk;
+  int st = launch_packed_list(sh, cu, 128, ws, s);
+  if (st != PA_OK) return st;
+  auto grid = [&](long long heads, long long most) {
+    const long long items = static_cast<long long>(packed_units(sh, 128)) * heads;
+    return dim3(static_cast<unsigned>(items < most ? items : most));
+  };
+  const int sms = device_sm_count();
+  st = launch_beside(packed_stats_kernel<D>, grid(sh.H, 8 * sms), 256, 0, s, static_cast<const bf16*>(dO),
+                     static_cast<const bf16*>(o), lse, list, sh.T, sh.H, rows, lse2, delta);
+  if (st != PA_OK) return st;
+  st = launch_beside(packed_dq_kernel<D>, grid(sh.H, sms), PackedDq<D>::THREADS, PackedDq<D>::SMEM, s, mq, mk, mv, mo,
+                     static_cast<bf16*>(dq), sh.dq_stride, static_cast<const float*>(lse2),
+                     static_cast<const float*>(delta), list, sh.H, group, rows, sh.scale, sh.scale * kLog2e,
+                     static_cast<int>(accumulate), status);
+  if (st != PA_OK) return st;
+  return launch_beside(packed_dkv_kernel<D>, grid(sh.Hk, sms), PackedDkv<D>::THREADS, PackedDkv<D>::SMEM, s, mq, mk, mv,
+                       mo, static_cast<bf16*>(dk), static_cast<bf16*>(dv), sh.dk_stride, sh.dv_stride,
+                       static_cast<const float*>(lse2), static_cast<const float*>(delta), list, sh.Hk, group, rows,
+                       sh.scale, sh.scale * kLog2e, static_cast<int>(accumulate), status);
 }
 
 }  // namespace
 
-size_t packed_attn_bwd_workspace_bytes(const PackedShape& sh) { return 4 * static_cast<size_t>(sh.T) * sh.H; }
-
-template <int D>
-static void packed_bwd(const PackedShape& sh, const bf16* q, const bf16* k, const bf16* v, const bf16* o,
-                       const bf16* dO, const float* lse, const int32_t* cu, bf16* dq, bf16* dk, bf16* dv, bool add,
-                       float* delta, cudaStream_t s) {
-  packed_dq_kernel<D><<<dim3((sh.T + 3) / 4, sh.H), 128, 0, s>>>(sh, q, k, v, o, dO, lse, cu, dq, delta, add);
-  packed_dkv_kernel<D><<<dim3((sh.T + 3) / 4, sh.Hk), 128, 0, s>>>(sh, q, k, v, dO, lse, delta, cu, dk, dv, add);
+size_t packed_attn_bwd_workspace_bytes(const PackedShape& sh) {
+  return packed_list_bytes(sh, 128) + 2 * stat_bytes(sh);
 }
 
 int launch_packed_attn_bwd(const PackedShape& sh, const void* q, const void* k, const void* v,
                            const void* o, const void* dO, const float* lse, const int32_t* cu,
                            void* dq, void* dk, void* dv, bool accumulate, void* ws,
-                           uint32_t*, cudaStream_t s) {
-  auto go = [&](auto bwd) {
-    bwd(sh, static_cast<const bf16*>(q), static_cast<const bf16*>(k), static_cast<const bf16*>(v),
-        static_cast<const bf16*>(o), static_cast<const bf16*>(dO), lse, cu, static_cast<bf16*>(dq),
-        static_cast<bf16*>(dk), static_cast<bf16*>(dv), accumulate, static_cast<float*>(ws), s);
-  };
-  if (sh.D == 64) go(packed_bwd<64>);
-  else go(packed_bwd<128>);
-  return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+                           uint32_t* status, cudaStream_t s) {
+  return sh.D == 64 ? packed_bwd<64>(sh, q, k, v, o, dO, lse, cu, dq, dk, dv, accumulate, ws, status, s)
+                    : packed_bwd<128>(sh, q, k, v, o, dO, lse, cu, dq, dk, dv, accumulate, ws, status, s);
 }
 
 }  // namespace pa
