@@ -1,63 +1,673 @@
 // Attention of one new token of each sequence over its paged cache.
+//
+//   o = sum_t exp(q.k_t scale - lse) v_t over the cached tokens t of the sequence
+//
+// Bound by HBM: every cached key and value is read once and used by the heads of one group.
+// A unit is (sequence, kv head, up to 16 heads of its group); all units' keys
+// are laid end to end in tiles of 64 and dealt out to the CTAs in equal runs, whatever the lengths
+// of the sequences: a CTA may hold several units, or a piece of a long one. A unit that lies in one
+// CTA is finished there; the pieces of the others (running maximum, sum, unnormalised o) go to
+// the workspace and a second kernel joins them in order. Nothing is counted in
+// memory, so a workspace may hold anything before the call and results do not depend on the run.
+//
+// Within a CTA a warp takes 16 keys of each tile through a ring of its own in shared memory
+// (cp.async, no barrier between warps) and keeps its own softmax statistics; the warps are merged
+// when the unit ends. bf16: the heads are the 16 rows of mma.m16n8k16 (the 5th-generation
+// tensor core wants 64 rows at least, and its rate is not needed: 32 products for
+// 16 keys of 128 values take a third of the time that HBM needs for them). fp32: plain FMA, exact
+// to fp32 rounding.
 #include <cuda_bf16.h>
-#include "host_launchers.h"
+#include "packed_common.cuh"
 
 namespace pa {
 namespace {
 
-__device__ __forceinline__ float to_f(float x) { return x; }
-__device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void put(float* p, float x) { *p = x; }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+using bf16 = __nv_bfloat16;
 
-// A warp takes a (sequence, head of q); its lanes share the head's values.
-template <typename T, int D>
-__global__ void paged_step_kernel(const PagedShape sh, const T* __restrict__ q, const T* __restrict__ kc,
-                                  const T* __restrict__ vc, const int32_t* __restrict__ table,
-                                  const int32_t* __restrict__ lens, T* __restrict__ o, float* __restrict__ lse) {
-  const int w = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, lane = threadIdx.x & 31;
-  if (w >= sh.B * sh.H) return;
-  const int b = w / sh.H, h = w % sh.H, kh = h / (sh.H / sh.Hk);
-  constexpr int N = D / 32;
-  float x[N], acc[N] = {}, m = -INFINITY, l = 0.f;
-  for (int i = 0; i < N; ++i) x[i] = to_f(q[b * sh.q_stride + static_cast<size_t>(h) * D + lane + 32 * i]) * sh.scale;
-  const int most = sh.max_pages * sh.page_size, n = max(0, min(lens[b], most));
-  for (int t = 0; t < n; ++t) {
-    const int page = table[static_cast<size_t>(b) * sh.max_pages + t / sh.page_size];
-    if (page < 0 || page >= sh.num_pages) continue;
-    const size_t row = ((static_cast<size_t>(page) * sh.page_size + t % sh.page_size) * sh.Hk + kh) * D + lane;
-    float s = 0.f;
-    for (int i = 0; i < N; ++i) s += x[i] * to_f(kc[row + 32 * i]);
-    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-    const float top = fmaxf(m, s), old = m == -INFINITY ? 0.f : __expf(m - top), p = s == -INFINITY ? 0.f : __expf(s - top);
-    l = l * old + p;
-    for (int i = 0; i < N; ++i) acc[i] = acc[i] * old + p * to_f(vc[row + 32 * i]);
-    m = top;
-  }
-  for (int i = 0; i < N; ++i) put(o + static_cast<size_t>(w) * D + lane + 32 * i, l == 0.f ? 0.f : acc[i] / l);
-  if (lse && lane == 0) lse[w] = l == 0.f ? -INFINITY : m + __logf(l);
+constexpr int kWarps = 4, kKeys = 16;         // keys of a warp and tile
+constexpr int kTileKeys = kWarps * kKeys;
+
+// A call's sizes, and the places of its units' pieces.
+struct PagedArgs {
+  PagedShape sh;
+  float scale_log2;
+  int chunks, chunk_heads;  // chunks of a group, heads of each
+  float* pieces;            // [2 * CTAs][piece_floats]
+  int2* spans;              // [units]: first and last CTA of each
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t at, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(at)
+               : "memory");
+}
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-template <typename T, int D>
-int paged_launch(const PagedShape& sh, const void* q, const void* kc, const void* vc, const int32_t* table,
-                 const int32_t* lens, void* o, float* lse, cudaStream_t s) {
-  paged_step_kernel<T, D><<<(sh.B * sh.H + 3) / 4, 128, 0, s>>>(sh, static_cast<const T*>(q), static_cast<const T*>(kc),
-                                                              static_cast<const T*>(vc), table, lens,
-                                                              static_cast<T*>(o), lse);
-  return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+// 16-byte piece c of row r of a warp's K or V block (rows of ROW bytes): swizzled, so that eight rows'
+// same piece lies in eight different groups of banks.
+template <int ROW>
+__device__ __forceinline__ uint32_t piece_at(int r, int c) {
+  return static_cast<uint32_t>(r * ROW + ((c ^ (r & 7)) << 4));
+}
+
+// ---------------------------------------------------------------- bf16: one warp's softmax over its keys
+// Thread (g = lane / 4, c = lane % 4) holds rows (heads) g and g + 8 of the products' fragments.
+template <int D>
+struct Bf16Core {
+  using T = bf16;
+  static constexpr int ROWS = 16, ROW = D * 2;
+  static constexpr int STATE = 32 * (D / 2) + 32;  // floats of a warp's state: o, then each row's m and sum
+  uint32_t q[D / 16][4];
+  float m[2], l[2], o[D / 8][4];
+
+  __device__ void start(const bf16* x, int heads) {  // x: the chunk's first head
+    const int g = lane_id() / 4, c = lane_id() % 4;
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = g + 8 * (i & 1), col = k * 16 + 2 * c + 8 * (i >> 1);
+        q[k][i] = row < heads ? *reinterpret_cast<const uint32_t*>(x + row * D + col) : 0u;
+      }
+    m[0] = m[1] = -INFINITY;
+    l[0] = l[1] = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+  }
+
+  // keys: bit t = key t of the block counts
+  __device__ void block(uint32_t sK, uint32_t sV, uint32_t keys, float scale_log2) {
+    const int lane = lane_id(), c = lane % 4;
+    // ldmatrix rows: lane's row of the 8x8 matrix lane / 8
+    const int r8 = lane & 7, mat = lane >> 3;
+    float s[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k) {
+      uint32_t b[4];  // keys 0-7: values 0-7, 8-15; keys 8-15: the same
+      ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), b);
+      mma_16816(s[0], q[k], b[0], b[1]);
+      mma_16816(s[1], q[k], b[2], b[3]);
+    }
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = n * 8 + 2 * c + (i & 1);
+        s[n][i] = (keys >> key) & 1 ? s[n][i] * scale_log2 : -INFINITY;
+      }
+    float top[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+    }
+    // m rises only by more than 8 (p <= 2^8 is exact in fp32 and bf16): o is seldom rescaled
+    const bool rise = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
+    if (__any_sync(0xffffffffu, rise)) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float to = fmaxf(m[h], top[h]), a = to == -INFINITY ? 1.f : ex2(m[h] - to);
+        m[h] = to;
+        l[h] *= a;
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n) {
+          o[n][2 * h] *= a;
+          o[n][2 * h + 1] *= a;
+        }
+      }
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+    uint32_t p[4];
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float x = ex2(s[n][2 * h] - base[h]), y = ex2(s[n][2 * h + 1] - base[h]);
+        l[h] += x + y;
+        p[2 * n + h] = pack_bf16x2(x, y);  // rounded once, for the product with v
+      }
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n) {
+      uint32_t b[4];  // values 0-7: keys 0-7, 8-15; values 8-15: the same
+      ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * n + (mat >> 1)), b);
+      mma_16816(o[2 * n], p, b[0], b[1]);
+      mma_16816(o[2 * n + 1], p, b[2], b[3]);
+    }
+  }
+
+  __device__ void dump(float* to) const {
+    const int lane = lane_id();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float sum = row_sum(h);
+      if (lane % 4 == 0) *reinterpret_cast<float2*>(to + 16 * D + 2 * (lane / 4 + 8 * h)) = make_float2(m[h], sum);
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) to[(4 * n + i) * 32 + lane] = o[n][i];
+  }
+  // A row's sum over the four threads that hold its keys.
+  __device__ float row_sum(int h) const {
+    float sum = l[h];
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    return sum + __shfl_xor_sync(0xffffffffu, sum, 2);
+  }
+  __device__ void merge(const float* from) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float2 other = *reinterpret_cast<const float2*>(from + 16 * D + 2 * (lane / 4 + 8 * h));
+      const float to = fmaxf(m[h], other.x);
+      const float a = to == -INFINITY ? 1.f : ex2(m[h] - to), b = to == -INFINITY ? 0.f : ex2(other.x - to);
+      m[h] = to;
+      l[h] = l[h] * a + (lane % 4 == 0 ? other.y * b : 0.f);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+        for (int i = 2 * h; i < 2 * h + 2; ++i) o[n][i] = o[n][i] * a + from[(4 * n + i) * 32 + lane] * b;
+    }
+  }
+  // f(row, m, l) once a row and f(row, column, two values) of the warp's state
+  template <typename F, typename G>
+  __device__ void each(int heads, F row_of, G pair_of) {
+    const int g = lane_id() / 4, c = lane_id() % 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float sum = row_sum(h);
+      const int row = g + 8 * h;
+      if (row >= heads) continue;
+      if (c == 0) row_of(row, m[h], sum);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) pair_of(row, n * 8 + 2 * c, o[n][2 * h], o[n][2 * h + 1], sum);
+    }
+  }
+};
+
+// ---------------------------------------------------------------- fp32
+// HC heads. Scores: lane = (key, half of its values); products with v: lane = D / 32 values.
+template <int D, int HC>
+struct F32Core {
+  using T = float;
+  static constexpr int ROWS = HC, ROW = D * 4;
+  static constexpr int N = D / 32, STATE = 32 * HC * (2 + N);
+  float m[HC], l[HC], o[HC][N];
+  float *q, *p;  // shared, of this warp: [HC][D] and [HC][16]
+
+  __device__ void start(const float* x, int heads) {
+    __syncwarp();
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      m[h] = -INFINITY;
+      l[h] = 0.f;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        o[h][i] = 0.f;
+        q[h * D + i * 32 + lane_id()] = h < heads ? x[h * D + i * 32 + lane_id()] : 0.f;
+      }
+    }
+    __syncwarp();
+  }
+
+  __device__ void block(const uint8_t* sK, const uint8_t* sV, uint32_t keys, float scale_log2) {
+    const int lane = lane_id(), key = lane & 15, half = lane >> 4;
+    float k[D / 2];
+#pragma unroll
+    for (int i = 0; i < D / 8; ++i)
+      *reinterpret_cast<float4*>(&k[4 * i]) =
+          *reinterpret_cast<const float4*>(sK + piece_at<ROW>(key, half * (D / 8) + i));
+    const bool on = (keys >> key) & 1;
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      float2 s2 = make_float2(0.f, 0.f), t2 = make_float2(0.f, 0.f);
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i) {
+        const float4 x = *reinterpret_cast<const float4*>(q + h * D + half * (D / 2) + 4 * i);
+        s2 = __ffma2_rn(make_float2(k[4 * i], k[4 * i + 1]), make_float2(x.x, x.y), s2);
+        t2 = __ffma2_rn(make_float2(k[4 * i + 2], k[4 * i + 3]), make_float2(x.z, x.w), t2);
+      }
+      float s = (s2.x + s2.y) + (t2.x + t2.y);
+      s += __shfl_xor_sync(0xffffffffu, s, 16);
+      s = on ? s * scale_log2 : -INFINITY;
+      float top = s;
+#pragma unroll
+      for (int d = 8; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+      if (top > m[h]) {  // the same in all lanes
+        const float a = ex2(m[h] - top);
+        m[h] = top;
+        l[h] *= a;
+#pragma unroll
+        for (int i = 0; i < N; ++i) o[h][i] *= a;
+      }
+      const float w = ex2(s - (m[h] == -INFINITY ? 0.f : m[h]));
+      if (half == 0) {
+        l[h] += w;  // this key's; summed over the lanes at the end
+        p[h * 16 + key] = w;
+      }
+    }
+    __syncwarp();
+#pragma unroll
+    for (int t = 0; t < 16; t += 4) {
+      float v[4][N];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint8_t* row = sV + piece_at<ROW>(t + j, lane * N / 4) + (lane * N % 4) * 4;
+        if constexpr (N == 2) {
+          const float2 x = *reinterpret_cast<const float2*>(row);
+          v[j][0] = x.x;
+          v[j][N - 1] = x.y;
+        } else {
+          v[j][0] = *reinterpret_cast<const float*>(row);
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < HC; ++h) {
+        const float4 w = *reinterpret_cast<const float4*>(p + h * 16 + t);
+        const float ws[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int i = 0; i < N; ++i) o[h][i] = fmaf(ws[j], v[j][i], o[h][i]);
+      }
+    }
+    __syncwarp();
+  }
+
+  __device__ void dump(float* to) const {
+    const int lane = lane_id();
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      to[h * 32 + lane] = m[h];
+      to[(HC + h) * 32 + lane] = l[h];
+#pragma unroll
+      for (int i = 0; i < N; ++i) to[(2 * HC + h * N + i) * 32 + lane] = o[h][i];
+    }
+  }
+  __device__ void merge(const float* from) {
+    const int lane = lane_id();
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      const float om = from[h * 32 + lane], to = fmaxf(m[h], om);
+      const float a = to == -INFINITY ? 1.f : ex2(m[h] - to), b = to == -INFINITY ? 0.f : ex2(om - to);
+      m[h] = to;
+      l[h] = l[h] * a + from[(HC + h) * 32 + lane] * b;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o[h][i] = o[h][i] * a + from[(2 * HC + h * N + i) * 32 + lane] * b;
+    }
+  }
+  template <typename F, typename G>
+  __device__ void each(int heads, F row_of, G pair_of) {
+#pragma unroll
+    for (int h = 0; h < HC; ++h) {
+      float sum = l[h];
+#pragma unroll
+      for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+      if (h >= heads) continue;
+      if (lane_id() == 0) row_of(h, m[h], sum);
+      if constexpr (N == 2) pair_of(h, 2 * static_cast<int>(lane_id()), o[h][0], o[h][N - 1], sum);
+      else pair_of(h, static_cast<int>(lane_id()), o[h][0], 0.f, sum);
+    }
+  }
+};
+
+template <typename Core>
+struct PagedSmem;
+template <int D>
+struct PagedSmem<Bf16Core<D>> {
+  static constexpr int STAGES = D == 128 ? 3 : 5, EXTRA = 0;
+};
+template <int D, int HC>
+struct PagedSmem<F32Core<D, HC>> {
+  static constexpr int STAGES = D == 64 ? 3 : 5, EXTRA = HC * (D + 16) * 4;  // q and p of a warp
+};
+template <typename Core>
+constexpr int paged_smem() {
+  return kWarps * (PagedSmem<Core>::STAGES * 2 * kKeys * Core::ROW + PagedSmem<Core>::EXTRA) +
+         2 * Core::STATE * 4;
+}
+// Floats of a unit's piece: o, then each row's m and sum; whole 16 bytes.
+template <int ROWS, int D>
+__host__ __device__ constexpr int piece_floats() {
+  return (ROWS * (D + 2) + 3) / 4 * 4;
+}
+
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, const int32_t* lens, int b) {
+  const int n = min(max(__ldg(lens + b), 0), a.sh.max_pages * a.sh.page_size);
+  return max(1, (n + kTileKeys - 1) / kTileKeys);  // an empty sequence has one tile without keys
+}
+
+// Where a tile of the whole run of tiles lies.
+struct TileAt {
+  int b, part, tile, n_tiles, len;  // sequence, (kv head, chunk), tile of the unit, its tiles, its keys
+  long long left;                   // tiles of the CTA's run still to come, this one too
+};
+
+template <typename Core, int D>
+__global__ void __launch_bounds__(kWarps * 32, 2)
+    paged_step_kernel(const __grid_constant__ PagedArgs a, const typename Core::T* __restrict__ q,
+                      const typename Core::T* __restrict__ kc, const typename Core::T* __restrict__ vc,
+                      const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
+                      typename Core::T* __restrict__ o, float* __restrict__ lse) {
+  using T = typename Core::T;
+  constexpr int STAGES = PagedSmem<Core>::STAGES, ROW = Core::ROW, BLOCK = kKeys * ROW;
+  constexpr int PIECES = ROW / 16, ROWS_A_GO = 32 / PIECES;  // 16-byte pieces of a row, rows a warp copies at once
+  extern __shared__ __align__(16) uint8_t smem[];
+  __shared__ long long s_scan[kWarps], s_total;
+  __shared__ TileAt s_first;
+  const int warp = warp_id(), lane = lane_id();
+  const int parts = a.sh.Hk * a.chunks, group = a.sh.H / a.sh.Hk;
+  launch_dependents();
+
+  // This CTA's run of tiles: every thread a run of sequences, their tiles' prefix sum, and the
+  // thread that holds the first tile finds its place.
+  const int per = (a.sh.B + kWarps * 32 - 1) / (kWarps * 32);
+  const int lo = min(a.sh.B, static_cast<int>(threadIdx.x) * per), hi = min(a.sh.B, lo + per);
+  long long mine = 0;
+  for (int b = lo; b < hi; ++b) mine += tiles_of(a, lens, b);
+  long long upto = mine;
+#pragma unroll
+  for (int d = 1; d < 32; d <<= 1) {
+    const long long x = __shfl_up_sync(0xffffffffu, upto, d);
+    if (lane >= d) upto += x;
+  }
+  if (lane == 31) s_scan[warp] = upto;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += s_scan[w];
+  if (threadIdx.x == kWarps * 32 - 1) s_total = upto;
+  __syncthreads();
+  const long long total = s_total * parts, run = (total + gridDim.x - 1) / gridDim.x;
+  const long long begin = blockIdx.x * run;
+  if (begin >= total) return;
+  if ((upto - mine) * parts <= begin && begin < upto * parts) {
+    long long at = (upto - mine) * parts;
+    int b = lo, n = tiles_of(a, lens, b);
+    while (at + static_cast<long long>(n) * parts <= begin) {
+      at += static_cast<long long>(n) * parts;
+      n = tiles_of(a, lens, ++b);
+    }
+    s_first = {b, static_cast<int>((begin - at) / n), static_cast<int>((begin - at) % n), n,
+               min(max(__ldg(lens + b), 0), a.sh.max_pages * a.sh.page_size), min(run, total - begin)};
+  }
+  __syncthreads();
+  TileAt use = s_first;
+  auto advance = [&](TileAt& t) {
+    --t.left;
+    if (++t.tile < t.n_tiles || t.left <= 0) return;
+    t.tile = 0;
+    if (++t.part < parts) return;
+    t.part = 0;
+    ++t.b;
+    t.n_tiles = tiles_of(a, lens, t.b);
+    t.len = min(max(__ldg(lens + t.b), 0), a.sh.max_pages * a.sh.page_size);
+  };
+
+  uint8_t* ring = smem + warp * STAGES * 2 * BLOCK;
+  float* scratch = reinterpret_cast<float*>(smem + kWarps * STAGES * 2 * BLOCK);
+  Core core;
+  if constexpr (sizeof(T) == 4) {
+    core.q = scratch + 2 * Core::STATE + warp * (Core::ROWS * (D + 16));
+    core.p = core.q + Core::ROWS * D;
+  }
+
+  // The place in the pools of lane's key of a tile (lanes 0-15), or -1; loaded a tile ahead.
+  auto slot_of = [&](const TileAt& t) {
+    const int key = t.tile * kTileKeys + warp * kKeys + (lane & 15);
+    if (t.left <= 0 || key >= t.len) return -1;
+    const int page = __ldg(table + static_cast<size_t>(t.b) * a.sh.max_pages + key / a.sh.page_size);
+    return page < 0 || page >= a.sh.num_pages ? -1 : page * a.sh.page_size + key % a.sh.page_size;
+  };
+  TileAt ahead = use;
+  int slot = slot_of(ahead), stage_in = 0;
+  uint32_t keys_of[STAGES];
+  // Copies the tile at `ahead` into stage `st`; rows that are no keys become zeros, so that what lies
+  // there cannot meet a weight of zero as NaN.
+  auto fetch = [&](int st, uint32_t& keys) {
+    keys = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
+    if (keys) {
+      const uint32_t dst = smem_u32(ring + st * 2 * BLOCK);
+      const size_t head = static_cast<size_t>(ahead.part / a.chunks) * D;
+#pragma unroll
+      for (int i = 0; i < kKeys / ROWS_A_GO; ++i) {
+        const int r = i * ROWS_A_GO + lane / PIECES, c = lane % PIECES;
+        const int s = __shfl_sync(0xffffffffu, slot, r);
+        const size_t at = static_cast<size_t>(s < 0 ? 0 : s) * a.sh.Hk * D + head + c * (16 / sizeof(T));
+        cp_async16(dst + piece_at<ROW>(r, c), kc + at, s >= 0);
+        cp_async16(dst + BLOCK + piece_at<ROW>(r, c), vc + at, s >= 0);
+      }
+    }
+    cp_async_commit();
+    advance(ahead);
+    slot = slot_of(ahead);
+  };
+#pragma unroll
+  for (int st = 0; st < STAGES - 1; ++st) fetch(st, keys_of[st]);
+  stage_in = STAGES - 1;
+
+  auto q_of = [&](const TileAt& t, int* heads, int* first) {
+    const int kh = t.part / a.chunks, c = t.part % a.chunks;
+    *heads = min(a.chunk_heads, group - c * a.chunk_heads);
+    *first = kh * group + c * a.chunk_heads;
+    return q + t.b * a.sh.q_stride + static_cast<size_t>(*first) * D;
+  };
+  int heads, first;
+  {
+    const T* x = q_of(use, &heads, &first);
+    core.start(x, heads);
+  }
+  bool from_before = use.tile > 0;  // the unit began in an earlier CTA
+  while (use.left > 0) {
+#pragma unroll
+    for (int st = 0; st < STAGES; ++st) {  // unrolled: the stage is a constant
+      if (use.left <= 0) break;
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();
+      {
+        const int to = (st + STAGES - 1) % STAGES;
+        fetch(to, keys_of[to]);
+      }
+      const uint32_t keys = keys_of[st];
+      if (keys) {
+        if constexpr (sizeof(T) == 2)
+          core.block(smem_u32(ring + st * 2 * BLOCK), smem_u32(ring + st * 2 * BLOCK + BLOCK), keys, a.scale_log2);
+        else
+          core.block(ring + st * 2 * BLOCK, ring + st * 2 * BLOCK + BLOCK, keys, a.scale_log2);
+      }
+      __syncwarp();
+      const TileAt was = use;
+      advance(use);
+      const bool ends = was.tile + 1 == was.n_tiles;
+      if (!ends && use.left > 0) continue;
+      // The unit, or this CTA's run, ends: merge the warps, 2 and 3 into 0 and 1, then 1 into 0.
+      if (warp >= 2) core.dump(scratch + (warp - 2) * Core::STATE);
+      __syncthreads();
+      if (warp < 2) core.merge(scratch + warp * Core::STATE);
+      __syncthreads();
+      if (warp == 1) core.dump(scratch);
+      __syncthreads();
+      if (warp == 0) {
+        core.merge(scratch);
+        if (ends && !from_before) {
+          const size_t out = static_cast<size_t>(was.b) * a.sh.H + first;
+          core.each(
+              heads,
+              [&](int row, float m, float l) {
+                if (lse) lse[out + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+              },
+              [&](int row, int col, float x, float y, float l) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                T* to = o + (out + row) * D + col;
+                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(x * inv, y * inv);
+                else if constexpr (D == 64) *reinterpret_cast<float2*>(to) = make_float2(x * inv, y * inv);
+                else *to = x * inv;
+              });
+        } else {
+          // slot 0 of a CTA: a unit from before; slot 1: one that goes on in the next
+          float* to = a.pieces + (2 * static_cast<size_t>(blockIdx.x) + (from_before ? 0 : 1)) * piece_floats<Core::ROWS, D>();
+          core.each(
+              heads,
+              [&](int row, float m, float l) {
+                *reinterpret_cast<float2*>(to + Core::ROWS * D + 2 * row) = make_float2(m, l);
+              },
+              [&](int row, int col, float x, float y, float) {
+                if constexpr (D / 32 >= 2) *reinterpret_cast<float2*>(to + row * D + col) = make_float2(x, y);
+                else to[row * D + col] = x;
+              });
+        }
+        if (!from_before && lane == 0) {  // the CTAs of a unit, told by the first
+          const int later = static_cast<int>((was.n_tiles - 1 - was.tile + run - 1) / run);
+          a.spans[static_cast<size_t>(was.b) * parts + was.part] = make_int2(blockIdx.x, blockIdx.x + (ends ? 0 : later));
+        }
+      }
+      __syncthreads();
+      if (use.left > 0) {
+        from_before = false;
+        const T* x = q_of(use, &heads, &first);
+        core.start(x, heads);
+      }
+    }
+  }
+  cp_async_wait<0>();
+}
+
+// Joins the pieces of the units that several CTAs hold: a block takes (sequence, head).
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(128)
+    paged_join_kernel(const __grid_constant__ PagedArgs a, T* __restrict__ o, float* __restrict__ lse) {
+  constexpr int LANES = D / 4, PARTS = 128 / LANES;  // threads that share a row, pieces at a time
+  __shared__ float s_m[128], s_l[PARTS], s_o[PARTS][D];
+  const int group = a.sh.H / a.sh.Hk, b = blockIdx.x / a.sh.H, h = blockIdx.x % a.sh.H, gh = h % group;
+  const int part = h / group * a.chunks + gh / a.chunk_heads, row = gh % a.chunk_heads;
+  wait_prerequisites();
+  const int2 span = a.spans[static_cast<size_t>(b) * a.sh.Hk * a.chunks + part];
+  if (span.x == span.y) return;
+  const int n = span.y - span.x + 1;
+  auto piece = [&](int i) {  // the first CTA's last unit, the others' first
+    return a.pieces + (2 * static_cast<size_t>(span.x + i) + (i == 0 ? 1 : 0)) * piece_floats<ROWS, D>();
+  };
+  float m = -INFINITY;
+  for (int i = threadIdx.x; i < n; i += 128) m = fmaxf(m, piece(i)[ROWS * D + 2 * row]);
+  s_m[threadIdx.x] = m;
+  __syncthreads();
+  for (int d = 64; d > 0; d >>= 1) {
+    if (threadIdx.x < d) s_m[threadIdx.x] = fmaxf(s_m[threadIdx.x], s_m[threadIdx.x + d]);
+    __syncthreads();
+  }
+  m = s_m[0];
+  const int lane = threadIdx.x % LANES, p = threadIdx.x / LANES;
+  float l = 0.f;
+  float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+  for (int i = p; i < n; i += PARTS) {
+    const float* from = piece(i);
+    const float2 ml = *reinterpret_cast<const float2*>(from + ROWS * D + 2 * row);
+    const float4 y = *reinterpret_cast<const float4*>(from + row * D + 4 * lane);
+    const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+    l = fmaf(ml.y, w, l);
+    x.x = fmaf(y.x, w, x.x), x.y = fmaf(y.y, w, x.y), x.z = fmaf(y.z, w, x.z), x.w = fmaf(y.w, w, x.w);
+  }
+  *reinterpret_cast<float4*>(&s_o[p][4 * lane]) = x;
+  if (lane == 0) s_l[p] = l;
+  __syncthreads();
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < PARTS; ++i) sum += s_l[i];
+  for (int d = threadIdx.x; d < D; d += 128) {
+    float y = 0.f;
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) y += s_o[i][d];
+    y = sum == 0.f ? 0.f : y / sum;
+    T* to = o + static_cast<size_t>(blockIdx.x) * D + d;
+    if constexpr (sizeof(T) == 2) *to = __float2bfloat16_rn(y);
+    else *to = y;
+  }
+  if (lse && threadIdx.x == 0) lse[blockIdx.x] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * kLn2;
+}
+
+// Heads of a chunk of a group, and the chunks: as even as they go.
+struct PagedPlan {
+  int chunks, chunk_heads, ctas;
+};
+PagedPlan paged_plan(const PagedShape& sh) {
+  const int group = sh.H / sh.Hk, most = sh.f32 ? 8 : 16;
+  PagedPlan p;
+  p.chunks = (group + most - 1) / most;
+  p.chunk_heads = (group + p.chunks - 1) / p.chunks;
+  p.ctas = 2 * device_sm_count();
+  return p;
+}
+
+template <typename Core, int D>
+int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const void* kc, const void* vc,
+                 const int32_t* table, const int32_t* lens, void* o, float* lse, void* ws, cudaStream_t s) {
+  using T = typename Core::T;
+  static std::atomic<uint64_t> attr{0};
+  if (!ensure_smem_attr(paged_step_kernel<Core, D>, paged_smem<Core>(), attr)) return PA_ERR_LAUNCH;
+  PagedArgs a;
+  a.sh = sh;
+  a.scale_log2 = sh.scale * kLog2e;
+  a.chunks = p.chunks;
+  a.chunk_heads = p.chunk_heads;
+  a.pieces = static_cast<float*>(ws);
+  a.spans = reinterpret_cast<int2*>(a.pieces + 2 * static_cast<size_t>(p.ctas) * 16 * (D + 2));
+  // as many CTAs as there can be tiles of keys
+  const long long unit_tiles = (static_cast<long long>(sh.max_pages) * sh.page_size + kTileKeys - 1) / kTileKeys;
+  const long long tiles = static_cast<long long>(sh.B) * sh.Hk * p.chunks * unit_tiles;
+  const int grid = static_cast<int>(tiles < p.ctas ? tiles : p.ctas);
+  paged_step_kernel<Core, D><<<grid, kWarps * 32, paged_smem<Core>(), s>>>(
+      a, static_cast<const T*>(q), static_cast<const T*>(kc), static_cast<const T*>(vc), table, lens,
+      static_cast<T*>(o), lse);
+  if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
+  if (unit_tiles == 1) return PA_OK;  // no unit is cut
+  return launch_beside(paged_join_kernel<T, D, Core::ROWS>, dim3(sh.B * sh.H), 128, 0, s, a, static_cast<T*>(o), lse);
+}
+
+template <int D>
+int paged_f32(const PagedShape& sh, const PagedPlan& p, const void* q, const void* kc, const void* vc,
+              const int32_t* table, const int32_t* lens, void* o, float* lse, void* ws, cudaStream_t s) {
+  if (p.chunk_heads <= 1) return paged_launch<F32Core<D, 1>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  if (p.chunk_heads <= 2) return paged_launch<F32Core<D, 2>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  if (p.chunk_heads <= 4) return paged_launch<F32Core<D, 4>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  return paged_launch<F32Core<D, 8>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedShape&) { return 256; }
+size_t paged_attn_workspace_bytes(const PagedShape& sh) {
+  const PagedPlan p = paged_plan(sh);
+  return 2 * static_cast<size_t>(p.ctas) * 16 * (sh.D + 2) * sizeof(float) +
+         (static_cast<size_t>(sh.B) * sh.Hk * p.chunks * sizeof(int2) + 255) / 256 * 256;
+}
 
 int launch_paged_attn(const PagedShape& sh, const void* q, const void* kc, const void* vc, const int32_t* table,
-                      const int32_t* lens, void* o, float* lse, void*, cudaStream_t s) {
+                      const int32_t* lens, void* o, float* lse, void* ws, cudaStream_t s) {
+  const PagedPlan p = paged_plan(sh);
   if (sh.f32)
-    return sh.D == 32 ? paged_launch<float, 32>(sh, q, kc, vc, table, lens, o, lse, s)
-                      : paged_launch<float, 64>(sh, q, kc, vc, table, lens, o, lse, s);
-  return sh.D == 64 ? paged_launch<__nv_bfloat16, 64>(sh, q, kc, vc, table, lens, o, lse, s)
-                    : paged_launch<__nv_bfloat16, 128>(sh, q, kc, vc, table, lens, o, lse, s);
+    return sh.D == 32 ? paged_f32<32>(sh, p, q, kc, vc, table, lens, o, lse, ws, s)
+                      : paged_f32<64>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  return sh.D == 64 ? paged_launch<Bf16Core<64>, 64>(sh, p, q, kc, vc, table, lens, o, lse, ws, s)
+                    : paged_launch<Bf16Core<128>, 128>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
 }
 
 }  // namespace pa
