@@ -27,9 +27,23 @@ using bf16 = __nv_bfloat16;
 constexpr int kWarps = 4, kKeys = 16;         // keys of a warp and tile
 constexpr int kTileKeys = kWarps * kKeys;
 
+// n / d for 0 <= n < 2^31 as a multiplication: m = floor(2^(31 + s) / d) + 1 with 2^s >= d.
+struct Divisor {
+  uint32_t m, shift;
+  explicit Divisor(int d = 1) {
+    uint32_t s = 0;
+    while ((1ll << s) < d) ++s;
+    shift = 31 + s;
+    m = static_cast<uint32_t>((1ull << shift) / d + 1);
+  }
+  __device__ int of(int n) const { return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(n)) * m >> shift); }
+};
+
 // A call's sizes, and the places of its units' pieces.
 struct PagedArgs {
   PagedShape sh;
+  Divisor page;
+  int end_tiles;            // 1, or 0 where a unit has one tile at most
   float scale_log2;
   int chunks, chunk_heads;  // chunks of a group, heads of each
   float* pieces;            // [2 * CTAs][piece_floats]
@@ -57,8 +71,7 @@ __device__ __forceinline__ void ldmatrix4_trans(uint32_t at, uint32_t (&r)[4]) {
                : "memory");
 }
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -101,21 +114,30 @@ struct Bf16Core {
     const int lane = lane_id(), c = lane % 4;
     // ldmatrix rows: lane's row of the 8x8 matrix lane / 8
     const int r8 = lane & 7, mat = lane >> 3;
-    float s[2][4] = {};
+    uint32_t kb[D / 16][4], vb[D / 16][4];
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)  // keys 0-7: values 0-7, 8-15; keys 8-15: the same
+      ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), kb[k]);
+#pragma unroll
+    for (int n = 0; n < D / 16; ++n)  // values 0-7: keys 0-7, 8-15; values 8-15: the same
+      ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * n + (mat >> 1)), vb[n]);
+    float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: four chains of products
 #pragma unroll
     for (int k = 0; k < D / 16; ++k) {
-      uint32_t b[4];  // keys 0-7: values 0-7, 8-15; keys 8-15: the same
-      ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), b);
-      mma_16816(s[0], q[k], b[0], b[1]);
-      mma_16816(s[1], q[k], b[2], b[3]);
+      mma_16816(k & 1 ? s2[0] : s[0], q[k], kb[k][0], kb[k][1]);
+      mma_16816(k & 1 ? s2[1] : s[1], q[k], kb[k][2], kb[k][3]);
     }
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = n * 8 + 2 * c + (i & 1);
-        s[n][i] = (keys >> key) & 1 ? s[n][i] * scale_log2 : -INFINITY;
-      }
+      for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * scale_log2;
+    if (keys != 0xffffu) {
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!((keys >> (n * 8 + 2 * c + (i & 1))) & 1)) s[n][i] = -INFINITY;
+    }
     float top[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -150,10 +172,8 @@ struct Bf16Core {
       }
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) {
-      uint32_t b[4];  // values 0-7: keys 0-7, 8-15; values 8-15: the same
-      ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * n + (mat >> 1)), b);
-      mma_16816(o[2 * n], p, b[0], b[1]);
-      mma_16816(o[2 * n + 1], p, b[2], b[3]);
+      mma_16816(o[2 * n], p, vb[n][0], vb[n][1]);
+      mma_16816(o[2 * n + 1], p, vb[n][2], vb[n][3]);
     }
   }
 
@@ -353,15 +373,19 @@ __host__ __device__ constexpr int piece_floats() {
   return (ROWS * (D + 2) + 3) / 4 * 4;
 }
 
-__device__ __forceinline__ int tiles_of(const PagedArgs& a, const int32_t* lens, int b) {
-  const int n = min(max(__ldg(lens + b), 0), a.sh.max_pages * a.sh.page_size);
-  return max(1, (n + kTileKeys - 1) / kTileKeys);  // an empty sequence has one tile without keys
+__device__ __forceinline__ int keys_of(const PagedArgs& a, const int32_t* lens, int b) {
+  return min(max(__ldg(lens + b), 0), a.sh.max_pages * a.sh.page_size);
+}
+// Tiles of a sequence, and one without keys: the end of a unit takes about as long as a tile, so that
+// many short sequences make no CTA late. Without it (a cache of one tile) no unit is cut.
+__device__ __forceinline__ int tiles_of(const PagedArgs& a, int keys) {
+  return max(1 - a.end_tiles, (keys + kTileKeys - 1) / kTileKeys) + a.end_tiles;
 }
 
 // Where a tile of the whole run of tiles lies.
 struct TileAt {
-  int b, part, tile, n_tiles, len;  // sequence, (kv head, chunk), tile of the unit, its tiles, its keys
-  long long left;                   // tiles of the CTA's run still to come, this one too
+  int b, kh, chunk, tile, n_tiles, len;  // sequence, kv head, chunk; tile of the unit, its tiles, its keys
+  long long left;                        // tiles of the CTA's run still to come, this one too
 };
 
 template <typename Core, int D>
@@ -385,7 +409,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   const int per = (a.sh.B + kWarps * 32 - 1) / (kWarps * 32);
   const int lo = min(a.sh.B, static_cast<int>(threadIdx.x) * per), hi = min(a.sh.B, lo + per);
   long long mine = 0;
-  for (int b = lo; b < hi; ++b) mine += tiles_of(a, lens, b);
+  for (int b = lo; b < hi; ++b) mine += tiles_of(a, keys_of(a, lens, b));
   long long upto = mine;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
@@ -402,13 +426,14 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   if (begin >= total) return;
   if ((upto - mine) * parts <= begin && begin < upto * parts) {
     long long at = (upto - mine) * parts;
-    int b = lo, n = tiles_of(a, lens, b);
-    while (at + static_cast<long long>(n) * parts <= begin) {
-      at += static_cast<long long>(n) * parts;
-      n = tiles_of(a, lens, ++b);
+    int b = lo, len = keys_of(a, lens, b);
+    while (at + static_cast<long long>(tiles_of(a, len)) * parts <= begin) {
+      at += static_cast<long long>(tiles_of(a, len)) * parts;
+      len = keys_of(a, lens, ++b);
     }
-    s_first = {b, static_cast<int>((begin - at) / n), static_cast<int>((begin - at) % n), n,
-               min(max(__ldg(lens + b), 0), a.sh.max_pages * a.sh.page_size), min(run, total - begin)};
+    const int n = tiles_of(a, len), part = static_cast<int>((begin - at) / n);
+    s_first = {b, part / a.chunks, part % a.chunks, static_cast<int>((begin - at) % n), n, len,
+               min(run, total - begin)};
   }
   __syncthreads();
   TileAt use = s_first;
@@ -416,11 +441,12 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     --t.left;
     if (++t.tile < t.n_tiles || t.left <= 0) return;
     t.tile = 0;
-    if (++t.part < parts) return;
-    t.part = 0;
-    ++t.b;
-    t.n_tiles = tiles_of(a, lens, t.b);
-    t.len = min(max(__ldg(lens + t.b), 0), a.sh.max_pages * a.sh.page_size);
+    if (++t.chunk < a.chunks) return;
+    t.chunk = 0;
+    if (++t.kh < a.sh.Hk) return;
+    t.kh = 0;
+    t.len = keys_of(a, lens, ++t.b);
+    t.n_tiles = tiles_of(a, t.len);
   };
 
   uint8_t* ring = smem + warp * STAGES * 2 * BLOCK;
@@ -435,26 +461,29 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
   auto slot_of = [&](const TileAt& t) {
     const int key = t.tile * kTileKeys + warp * kKeys + (lane & 15);
     if (t.left <= 0 || key >= t.len) return -1;
-    const int page = __ldg(table + static_cast<size_t>(t.b) * a.sh.max_pages + key / a.sh.page_size);
-    return page < 0 || page >= a.sh.num_pages ? -1 : page * a.sh.page_size + key % a.sh.page_size;
+    const int i = a.page.of(key), page = __ldg(table + static_cast<size_t>(t.b) * a.sh.max_pages + i);
+    return page < 0 || page >= a.sh.num_pages ? -1 : (page - i) * a.sh.page_size + key;
   };
   TileAt ahead = use;
-  int slot = slot_of(ahead), stage_in = 0;
-  uint32_t keys_of[STAGES];
+  int slot = slot_of(ahead);
+  uint32_t keys_in[STAGES];
   // Copies the tile at `ahead` into stage `st`; rows that are no keys become zeros, so that what lies
   // there cannot meet a weight of zero as NaN.
+  const int my_row = lane / PIECES, my_col = lane % PIECES;
+  const size_t pitch = static_cast<size_t>(a.sh.Hk) * D;
   auto fetch = [&](int st, uint32_t& keys) {
     keys = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
     if (keys) {
       const uint32_t dst = smem_u32(ring + st * 2 * BLOCK);
-      const size_t head = static_cast<size_t>(ahead.part / a.chunks) * D;
+      const int head = ahead.kh * D + my_col * (16 / static_cast<int>(sizeof(T)));
+      const T *k0 = kc + head, *v0 = vc + head;
 #pragma unroll
       for (int i = 0; i < kKeys / ROWS_A_GO; ++i) {
-        const int r = i * ROWS_A_GO + lane / PIECES, c = lane % PIECES;
+        const int r = i * ROWS_A_GO + my_row;
         const int s = __shfl_sync(0xffffffffu, slot, r);
-        const size_t at = static_cast<size_t>(s < 0 ? 0 : s) * a.sh.Hk * D + head + c * (16 / sizeof(T));
-        cp_async16(dst + piece_at<ROW>(r, c), kc + at, s >= 0);
-        cp_async16(dst + BLOCK + piece_at<ROW>(r, c), vc + at, s >= 0);
+        const size_t at = static_cast<uint32_t>(max(s, 0)) * pitch;
+        cp_async16(dst + piece_at<ROW>(r, my_col), k0 + at, s >= 0);
+        cp_async16(dst + BLOCK + piece_at<ROW>(r, my_col), v0 + at, s >= 0);
       }
     }
     cp_async_commit();
@@ -462,13 +491,11 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
     slot = slot_of(ahead);
   };
 #pragma unroll
-  for (int st = 0; st < STAGES - 1; ++st) fetch(st, keys_of[st]);
-  stage_in = STAGES - 1;
+  for (int st = 0; st < STAGES - 1; ++st) fetch(st, keys_in[st]);
 
   auto q_of = [&](const TileAt& t, int* heads, int* first) {
-    const int kh = t.part / a.chunks, c = t.part % a.chunks;
-    *heads = min(a.chunk_heads, group - c * a.chunk_heads);
-    *first = kh * group + c * a.chunk_heads;
+    *heads = min(a.chunk_heads, group - t.chunk * a.chunk_heads);
+    *first = t.kh * group + t.chunk * a.chunk_heads;
     return q + t.b * a.sh.q_stride + static_cast<size_t>(*first) * D;
   };
   int heads, first;
@@ -485,9 +512,9 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
       __syncwarp();
       {
         const int to = (st + STAGES - 1) % STAGES;
-        fetch(to, keys_of[to]);
+        fetch(to, keys_in[to]);
       }
-      const uint32_t keys = keys_of[st];
+      const uint32_t keys = keys_in[st];
       if (keys) {
         if constexpr (sizeof(T) == 2)
           core.block(smem_u32(ring + st * 2 * BLOCK), smem_u32(ring + st * 2 * BLOCK + BLOCK), keys, a.scale_log2);
@@ -537,7 +564,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
         }
         if (!from_before && lane == 0) {  // the CTAs of a unit, told by the first
           const int later = static_cast<int>((was.n_tiles - 1 - was.tile + run - 1) / run);
-          a.spans[static_cast<size_t>(was.b) * parts + was.part] = make_int2(blockIdx.x, blockIdx.x + (ends ? 0 : later));
+          a.spans[static_cast<size_t>(was.b) * parts + was.kh * a.chunks + was.chunk] = make_int2(blockIdx.x, blockIdx.x + (ends ? 0 : later));
         }
       }
       __syncthreads();
@@ -626,6 +653,7 @@ int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const 
   if (!ensure_smem_attr(paged_step_kernel<Core, D>, paged_smem<Core>(), attr)) return PA_ERR_LAUNCH;
   PagedArgs a;
   a.sh = sh;
+  a.page = Divisor(sh.page_size);
   a.scale_log2 = sh.scale * kLog2e;
   a.chunks = p.chunks;
   a.chunk_heads = p.chunk_heads;
@@ -633,7 +661,8 @@ int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const 
   a.spans = reinterpret_cast<int2*>(a.pieces + 2 * static_cast<size_t>(p.ctas) * 16 * (D + 2));
   // as many CTAs as there can be tiles of keys
   const long long unit_tiles = (static_cast<long long>(sh.max_pages) * sh.page_size + kTileKeys - 1) / kTileKeys;
-  const long long tiles = static_cast<long long>(sh.B) * sh.Hk * p.chunks * unit_tiles;
+  a.end_tiles = unit_tiles > 1;
+  const long long tiles = static_cast<long long>(sh.B) * sh.Hk * p.chunks * (unit_tiles + a.end_tiles);
   const int grid = static_cast<int>(tiles < p.ctas ? tiles : p.ctas);
   paged_step_kernel<Core, D><<<grid, kWarps * 32, paged_smem<Core>(), s>>>(
       a, static_cast<const T*>(q), static_cast<const T*>(kc), static_cast<const T*>(vc), table, lens,
