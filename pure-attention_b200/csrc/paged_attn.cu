@@ -85,144 +85,153 @@ __device__ __forceinline__ uint32_t piece_at(int r, int c) {
 }
 
 // ---------------------------------------------------------------- bf16: one warp's softmax over its keys
-// Thread (g = lane / 4, c = lane % 4) holds rows (heads) g and g + 8 of the products' fragments.
-template <int D>
+// Both products are taken transposed, S^T = K Q^T and o^T = V^T P^T: keys, then values, are the 16 rows
+// of mma.m16n8k16 and up to 8 heads (NB times 8) its columns, so that few heads waste little of it. Thread
+// (g = lane / 4, c = lane % 4) holds heads 2 c and 2 c + 1 of each 8 in both results.
+template <int D, int NB>
 struct Bf16Core {
   using T = bf16;
-  static constexpr int ROWS = 16, ROW = D * 2;
-  static constexpr int STATE = 32 * (D / 2) + 32;  // floats of a warp's state: o, then each row's m and sum
-  uint32_t q[D / 16][4];
-  float m[2], l[2], o[D / 8][4];
+  static constexpr int ROWS = 8 * NB, ROW = D * 2;
+  static constexpr int STATE = NB * (8 * D + 16);  // floats of a warp's state: o, then each head's m and sum
+  uint32_t q[NB][D / 16][2];
+  float m[NB][2], l[NB][2], o[NB][D / 16][4];
 
   __device__ void start(const bf16* x, int heads) {  // x: the chunk's first head
     const int g = lane_id() / 4, c = lane_id() % 4;
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k)
+    for (int n = 0; n < NB; ++n) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = g + 8 * (i & 1), col = k * 16 + 2 * c + 8 * (i >> 1);
-        q[k][i] = row < heads ? *reinterpret_cast<const uint32_t*>(x + row * D + col) : 0u;
-      }
-    m[0] = m[1] = -INFINITY;
-    l[0] = l[1] = 0.f;
+      for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        for (int i = 0; i < 2; ++i)
+          q[n][k][i] = 8 * n + g < heads
+                           ? *reinterpret_cast<const uint32_t*>(x + (8 * n + g) * D + k * 16 + 2 * c + 8 * i)
+                           : 0u;
+      m[n][0] = m[n][1] = -INFINITY;
+      l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) o[n][k][0] = o[n][k][1] = o[n][k][2] = o[n][k][3] = 0.f;
+    }
   }
 
   // keys: bit t = key t of the block counts
   __device__ void block(uint32_t sK, uint32_t sV, uint32_t keys, float scale_log2) {
-    const int lane = lane_id(), c = lane % 4;
+    const int lane = lane_id(), g = lane / 4;
     // ldmatrix rows: lane's row of the 8x8 matrix lane / 8
     const int r8 = lane & 7, mat = lane >> 3;
     uint32_t kb[D / 16][4], vb[D / 16][4];
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k)  // keys 0-7: values 0-7, 8-15; keys 8-15: the same
-      ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), kb[k]);
+    for (int k = 0; k < D / 16; ++k)  // keys 0-7, 8-15 of values 0-7, then of values 8-15
+      ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), kb[k]);
 #pragma unroll
-    for (int n = 0; n < D / 16; ++n)  // values 0-7: keys 0-7, 8-15; values 8-15: the same
-      ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * n + (mat >> 1)), vb[n]);
-    float s[2][4] = {}, s2[2][4] = {};  // even and odd steps: four chains of products
+    for (int k = 0; k < D / 16; ++k)  // values 0-7, 8-15 of keys 0-7, then of keys 8-15
+      ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), vb[k]);
+    uint32_t p[NB][2];
 #pragma unroll
-    for (int k = 0; k < D / 16; ++k) {
-      mma_16816(k & 1 ? s2[0] : s[0], q[k], kb[k][0], kb[k][1]);
-      mma_16816(k & 1 ? s2[1] : s[1], q[k], kb[k][2], kb[k][3]);
-    }
+    for (int n = 0; n < NB; ++n) {
+      float s[4] = {}, s2[4] = {};  // even and odd steps: two chains of products
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
+      for (int k = 0; k < D / 16; ++k) mma_16816(k & 1 ? s2 : s, kb[k], q[n][k][0], q[n][k][1]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[n][i] = (s[n][i] + s2[n][i]) * scale_log2;
-    if (keys != 0xffffu) {
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
+      for (int i = 0; i < 4; ++i) s[i] = (s[i] + s2[i]) * scale_log2;
+      if (keys != 0xffffu) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-          if (!((keys >> (n * 8 + 2 * c + (i & 1))) & 1)) s[n][i] = -INFINITY;
-    }
-    float top[2];
+          if (!((keys >> (g + 8 * (i >> 1))) & 1)) s[i] = -INFINITY;
+      }
+      float top[2] = {fmaxf(s[0], s[2]), fmaxf(s[1], s[3])};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      top[h] = fmaxf(fmaxf(s[0][2 * h], s[0][2 * h + 1]), fmaxf(s[1][2 * h], s[1][2 * h + 1]));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
-      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-    }
-    // m rises only by more than 8 (p <= 2^8 is exact in fp32 and bf16): o is seldom rescaled
-    const bool rise = top[0] > m[0] + 8.f || top[1] > m[1] + 8.f;
-    if (__any_sync(0xffffffffu, rise)) {
+      for (int d = 4; d < 32; d <<= 1)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float to = fmaxf(m[h], top[h]), a = to == -INFINITY ? 1.f : ex2(m[h] - to);
-        m[h] = to;
-        l[h] *= a;
+        for (int h = 0; h < 2; ++h) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], d));
+      // m rises only by more than 8 (p <= 2^8 is exact in fp32 and bf16): o is seldom rescaled
+      if (__any_sync(0xffffffffu, top[0] > m[n][0] + 8.f || top[1] > m[n][1] + 8.f)) {
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          o[n][2 * h] *= a;
-          o[n][2 * h + 1] *= a;
+        for (int h = 0; h < 2; ++h) {
+          const float to = fmaxf(m[n][h], top[h]), a = to == -INFINITY ? 1.f : ex2(m[n][h] - to);
+          m[n][h] = to;
+          l[n][h] *= a;
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k) {
+            o[n][k][h] *= a;
+            o[n][k][2 + h] *= a;
+          }
         }
       }
-    }
-    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
-    uint32_t p[4];
+      const float base[2] = {m[n][0] == -INFINITY ? 0.f : m[n][0], m[n][1] == -INFINITY ? 0.f : m[n][1]};
 #pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float x = ex2(s[n][2 * h] - base[h]), y = ex2(s[n][2 * h + 1] - base[h]);
-        l[h] += x + y;
-        p[2 * n + h] = pack_bf16x2(x, y);  // rounded once, for the product with v
+      for (int i = 0; i < 2; ++i) {
+        const float x = ex2(s[2 * i] - base[0]), y = ex2(s[2 * i + 1] - base[1]);
+        l[n][0] += x;
+        l[n][1] += y;
+        // rounded once, for the product with v; key rows become head rows
+        asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(p[n][i]) : "r"(pack_bf16x2(x, y)));
       }
-#pragma unroll
-    for (int n = 0; n < D / 16; ++n) {
-      mma_16816(o[2 * n], p, vb[n][0], vb[n][1]);
-      mma_16816(o[2 * n + 1], p, vb[n][2], vb[n][3]);
     }
+#pragma unroll
+    for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) mma_16816(o[n][k], vb[k], p[n][0], p[n][1]);
   }
 
+  // A head's sum over the eight threads that hold its keys.
+  __device__ float row_sum(int n, int h) const {
+    float sum = l[n][h];
+#pragma unroll
+    for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    return sum;
+  }
   __device__ void dump(float* to) const {
     const int lane = lane_id();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float sum = row_sum(h);
-      if (lane % 4 == 0) *reinterpret_cast<float2*>(to + 16 * D + 2 * (lane / 4 + 8 * h)) = make_float2(m[h], sum);
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float sum = row_sum(n, h);
+        if (lane < 4) *reinterpret_cast<float2*>(to + NB * 8 * D + 2 * (8 * n + 2 * lane + h)) = make_float2(m[n][h], sum);
+      }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[((n * (D / 16) + k) * 4 + i) * 32 + lane] = o[n][k][i];
     }
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) to[(4 * n + i) * 32 + lane] = o[n][i];
-  }
-  // A row's sum over the four threads that hold its keys.
-  __device__ float row_sum(int h) const {
-    float sum = l[h];
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    return sum + __shfl_xor_sync(0xffffffffu, sum, 2);
   }
   __device__ void merge(const float* from) {
     const int lane = lane_id();
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float2 other = *reinterpret_cast<const float2*>(from + 16 * D + 2 * (lane / 4 + 8 * h));
-      const float to = fmaxf(m[h], other.x);
-      const float a = to == -INFINITY ? 1.f : ex2(m[h] - to), b = to == -INFINITY ? 0.f : ex2(other.x - to);
-      m[h] = to;
-      l[h] = l[h] * a + (lane % 4 == 0 ? other.y * b : 0.f);
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n)
+      for (int h = 0; h < 2; ++h) {
+        const float2 other = *reinterpret_cast<const float2*>(from + NB * 8 * D + 2 * (8 * n + 2 * (lane % 4) + h));
+        const float to = fmaxf(m[n][h], other.x);
+        const float a = to == -INFINITY ? 1.f : ex2(m[n][h] - to), b = to == -INFINITY ? 0.f : ex2(other.x - to);
+        m[n][h] = to;
+        l[n][h] = l[n][h] * a + (lane < 4 ? other.y * b : 0.f);
 #pragma unroll
-        for (int i = 2 * h; i < 2 * h + 2; ++i) o[n][i] = o[n][i] * a + from[(4 * n + i) * 32 + lane] * b;
-    }
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int i = h; i < 4; i += 2)
+            o[n][k][i] = o[n][k][i] * a + from[((n * (D / 16) + k) * 4 + i) * 32 + lane] * b;
+      }
   }
-  // f(row, m, l) once a row and f(row, column, two values) of the warp's state
+  // f(row, m, l) once a head and f(row, column, value, l) for the warp's state
   template <typename F, typename G>
-  __device__ void each(int heads, F row_of, G pair_of) {
+  __device__ void each(int heads, F row_of, G value_of) {
     const int g = lane_id() / 4, c = lane_id() % 4;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float sum = row_sum(h);
-      const int row = g + 8 * h;
-      if (row >= heads) continue;
-      if (c == 0) row_of(row, m[h], sum);
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) pair_of(row, n * 8 + 2 * c, o[n][2 * h], o[n][2 * h + 1], sum);
-    }
+      for (int h = 0; h < 2; ++h) {
+        const float sum = row_sum(n, h);
+        const int row = 8 * n + 2 * c + h;
+        if (row >= heads) continue;
+        if (g == 0) row_of(row, m[n][h], sum);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          value_of(row, k * 16 + g, o[n][k][h], sum);
+          value_of(row, k * 16 + g + 8, o[n][k][2 + h], sum);
+        }
+      }
   }
 };
 
@@ -338,7 +347,7 @@ struct F32Core {
     }
   }
   template <typename F, typename G>
-  __device__ void each(int heads, F row_of, G pair_of) {
+  __device__ void each(int heads, F row_of, G value_of) {
 #pragma unroll
     for (int h = 0; h < HC; ++h) {
       float sum = l[h];
@@ -346,20 +355,22 @@ struct F32Core {
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
       if (h >= heads) continue;
       if (lane_id() == 0) row_of(h, m[h], sum);
-      if constexpr (N == 2) pair_of(h, 2 * static_cast<int>(lane_id()), o[h][0], o[h][N - 1], sum);
-      else pair_of(h, static_cast<int>(lane_id()), o[h][0], 0.f, sum);
+#pragma unroll
+      for (int i = 0; i < N; ++i) value_of(h, N * static_cast<int>(lane_id()) + i, o[h][i], sum);
     }
   }
 };
 
 template <typename Core>
 struct PagedSmem;
-template <int D>
-struct PagedSmem<Bf16Core<D>> {
-  static constexpr int STAGES = D == 128 ? 3 : 5, EXTRA = 0;
+template <int D, int NB>
+struct PagedSmem<Bf16Core<D, NB>> {
+  static constexpr int CTAS = NB == 1 ? 3 : 2;  // that share an SM
+  static constexpr int STAGES = (NB == 1 ? 2 : 3) * (128 / D), EXTRA = 0;
 };
 template <int D, int HC>
 struct PagedSmem<F32Core<D, HC>> {
+  static constexpr int CTAS = 2;
   static constexpr int STAGES = D == 64 ? 3 : 5, EXTRA = HC * (D + 16) * 4;  // q and p of a warp
 };
 template <typename Core>
@@ -389,7 +400,7 @@ struct TileAt {
 };
 
 template <typename Core, int D>
-__global__ void __launch_bounds__(kWarps * 32, 2)
+__global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
     paged_step_kernel(const __grid_constant__ PagedArgs a, const typename Core::T* __restrict__ q,
                       const typename Core::T* __restrict__ kc, const typename Core::T* __restrict__ vc,
                       const int32_t* __restrict__ table, const int32_t* __restrict__ lens,
@@ -542,12 +553,10 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
               [&](int row, float m, float l) {
                 if (lse) lse[out + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
               },
-              [&](int row, int col, float x, float y, float l) {
-                const float inv = l == 0.f ? 0.f : 1.f / l;
-                T* to = o + (out + row) * D + col;
-                if constexpr (sizeof(T) == 2) *reinterpret_cast<uint32_t*>(to) = pack_bf16x2(x * inv, y * inv);
-                else if constexpr (D == 64) *reinterpret_cast<float2*>(to) = make_float2(x * inv, y * inv);
-                else *to = x * inv;
+              [&](int row, int col, float x, float l) {
+                const float y = l == 0.f ? 0.f : x / l;
+                if constexpr (sizeof(T) == 2) o[(out + row) * D + col] = __float2bfloat16_rn(y);
+                else o[(out + row) * D + col] = y;
               });
         } else {
           // slot 0 of a CTA: a unit from before; slot 1: one that goes on in the next
@@ -557,10 +566,7 @@ __global__ void __launch_bounds__(kWarps * 32, 2)
               [&](int row, float m, float l) {
                 *reinterpret_cast<float2*>(to + Core::ROWS * D + 2 * row) = make_float2(m, l);
               },
-              [&](int row, int col, float x, float y, float) {
-                if constexpr (D / 32 >= 2) *reinterpret_cast<float2*>(to + row * D + col) = make_float2(x, y);
-                else to[row * D + col] = x;
-              });
+              [&](int row, int col, float x, float) { to[row * D + col] = x; });
         }
         if (!from_before && lane == 0) {  // the CTAs of a unit, told by the first
           const int later = static_cast<int>((was.n_tiles - 1 - was.tile + run - 1) / run);
@@ -641,7 +647,7 @@ PagedPlan paged_plan(const PagedShape& sh) {
   PagedPlan p;
   p.chunks = (group + most - 1) / most;
   p.chunk_heads = (group + p.chunks - 1) / p.chunks;
-  p.ctas = 2 * device_sm_count();
+  p.ctas = (!sh.f32 && p.chunk_heads <= 8 ? 3 : 2) * device_sm_count();
   return p;
 }
 
@@ -673,6 +679,13 @@ int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const 
 }
 
 template <int D>
+int paged_bf16(const PagedShape& sh, const PagedPlan& p, const void* q, const void* kc, const void* vc,
+               const int32_t* table, const int32_t* lens, void* o, float* lse, void* ws, cudaStream_t s) {
+  if (p.chunk_heads <= 8) return paged_launch<Bf16Core<D, 1>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  return paged_launch<Bf16Core<D, 2>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+}
+
+template <int D>
 int paged_f32(const PagedShape& sh, const PagedPlan& p, const void* q, const void* kc, const void* vc,
               const int32_t* table, const int32_t* lens, void* o, float* lse, void* ws, cudaStream_t s) {
   if (p.chunk_heads <= 1) return paged_launch<F32Core<D, 1>, D>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
@@ -695,8 +708,8 @@ int launch_paged_attn(const PagedShape& sh, const void* q, const void* kc, const
   if (sh.f32)
     return sh.D == 32 ? paged_f32<32>(sh, p, q, kc, vc, table, lens, o, lse, ws, s)
                       : paged_f32<64>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
-  return sh.D == 64 ? paged_launch<Bf16Core<64>, 64>(sh, p, q, kc, vc, table, lens, o, lse, ws, s)
-                    : paged_launch<Bf16Core<128>, 128>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
+  return sh.D == 64 ? paged_bf16<64>(sh, p, q, kc, vc, table, lens, o, lse, ws, s)
+                    : paged_bf16<128>(sh, p, q, kc, vc, table, lens, o, lse, ws, s);
 }
 
 }  // namespace pa
