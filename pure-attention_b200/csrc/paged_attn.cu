@@ -17,6 +17,7 @@
 // 16 keys of 128 values take a third of the time that HBM needs for them). fp32: plain FMA, exact
 // to fp32 rounding.
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "packed_common.cuh"
 
 namespace pa {
@@ -47,7 +48,10 @@ struct PagedArgs {
   float scale_log2;
   int chunks, chunk_heads;  // chunks of a group, heads of each
   float* pieces;            // [2 * CTAs][piece_floats]
-  int2* spans;              // [units]: first and last CTA of each
+  // Unit, first and last CTA of what the join takes: of each unit, or (cuts_by_cta) of the unit that begins
+  // in a CTA and goes on in the next, of which a CTA has one at most, whichever is fewer.
+  int4* cuts;
+  int cuts_by_cta;
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool real) {
@@ -92,14 +96,14 @@ template <int D, int NB>
 struct Bf16Core {
   using T = bf16;
   static constexpr int ROWS = 8 * NB, ROW = D * 2;
-  static constexpr int STATE = NB * (8 * D + 16);  // floats of a warp's state: o, then each head's m and sum
+  static constexpr int TURN = NB == 1 ? 64 : 32;  // values of a head that are merged at a time
   uint32_t q[NB][D / 16][2];
   float m[NB][2], l[NB][2], o[NB][D / 16][4];
 
-  __device__ void start(const bf16* x, int heads) {  // x: the chunk's first head
+  __device__ void load_q(const bf16* x, int heads) {  // x: the chunk's first head
     const int g = lane_id() / 4, c = lane_id() % 4;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
+    for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
 #pragma unroll
@@ -107,6 +111,10 @@ struct Bf16Core {
           q[n][k][i] = 8 * n + g < heads
                            ? *reinterpret_cast<const uint32_t*>(x + (8 * n + g) * D + k * 16 + 2 * c + 8 * i)
                            : 0u;
+  }
+  __device__ void start() {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
       m[n][0] = m[n][1] = -INFINITY;
       l[n][0] = l[n][1] = 0.f;
 #pragma unroll
@@ -114,18 +122,23 @@ struct Bf16Core {
     }
   }
 
-  // keys: bit t = key t of the block counts
-  __device__ void block(uint32_t sK, uint32_t sV, uint32_t keys, float scale_log2) {
-    const int lane = lane_id(), g = lane / 4;
+  // A block's K and V into registers, so that the ring can be filled again at once.
+  uint32_t kb[D / 16][4], vb[D / 16][4];
+  __device__ void load(const uint8_t* k_block, const uint8_t* v_block) {
     // ldmatrix rows: lane's row of the 8x8 matrix lane / 8
-    const int r8 = lane & 7, mat = lane >> 3;
-    uint32_t kb[D / 16][4], vb[D / 16][4];
+    const int r8 = lane_id() & 7, mat = lane_id() >> 3;
+    const uint32_t sK = smem_u32(k_block), sV = smem_u32(v_block);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)  // keys 0-7, 8-15 of values 0-7, then of values 8-15
       ldmatrix4(sK + piece_at<ROW>(r8 + 8 * (mat & 1), 2 * k + (mat >> 1)), kb[k]);
 #pragma unroll
     for (int k = 0; k < D / 16; ++k)  // values 0-7, 8-15 of keys 0-7, then of keys 8-15
       ldmatrix4_trans(sV + piece_at<ROW>(r8 + 8 * (mat >> 1), 2 * k + (mat & 1)), vb[k]);
+  }
+
+  // keys: bit t = key t of the block counts
+  __device__ void block(uint32_t keys, float scale_log2) {
+    const int g = lane_id() / 4;
     uint32_t p[NB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -174,64 +187,29 @@ struct Bf16Core {
       for (int n = 0; n < NB; ++n) mma_16816(o[n][k], vb[k], p[n][0], p[n][1]);
   }
 
-  // A head's sum over the eight threads that hold its keys.
-  __device__ float row_sum(int n, int h) const {
-    float sum = l[n][h];
-#pragma unroll
-    for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    return sum;
-  }
-  __device__ void dump(float* to) const {
-    const int lane = lane_id();
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float sum = row_sum(n, h);
-        if (lane < 4) *reinterpret_cast<float2*>(to + NB * 8 * D + 2 * (8 * n + 2 * lane + h)) = make_float2(m[n][h], sum);
-      }
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) to[((n * (D / 16) + k) * 4 + i) * 32 + lane] = o[n][k][i];
-    }
-  }
-  __device__ void merge(const float* from) {
-    const int lane = lane_id();
+  // A head's maximum and sum, and TURN of its values from TURN * turn on, into the warp's part of the
+  // scratch memory (rows of TURN + 4 floats: no two lanes meet in a bank).
+  __device__ void dump_ml(float2* to) const {
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float2 other = *reinterpret_cast<const float2*>(from + NB * 8 * D + 2 * (8 * n + 2 * (lane % 4) + h));
-        const float to = fmaxf(m[n][h], other.x);
-        const float a = to == -INFINITY ? 1.f : ex2(m[n][h] - to), b = to == -INFINITY ? 0.f : ex2(other.x - to);
-        m[n][h] = to;
-        l[n][h] = l[n][h] * a + (lane < 4 ? other.y * b : 0.f);
+        float sum = l[n][h];
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-#pragma unroll
-          for (int i = h; i < 4; i += 2)
-            o[n][k][i] = o[n][k][i] * a + from[((n * (D / 16) + k) * 4 + i) * 32 + lane] * b;
+        for (int d = 4; d < 32; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (lane_id() < 4) to[8 * n + 2 * lane_id() + h] = make_float2(m[n][h], sum);
       }
   }
-  // f(row, m, l) once a head and f(row, column, value, l) for the warp's state
-  template <typename F, typename G>
-  __device__ void each(int heads, F row_of, G value_of) {
+  template <int TURN_NO>
+  __device__ void dump(float* to) const {
     const int g = lane_id() / 4, c = lane_id() % 4;
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float sum = row_sum(n, h);
-        const int row = 8 * n + 2 * c + h;
-        if (row >= heads) continue;
-        if (g == 0) row_of(row, m[n][h], sum);
+      for (int k = 0; k < TURN / 16; ++k)
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          value_of(row, k * 16 + g, o[n][k][h], sum);
-          value_of(row, k * 16 + g + 8, o[n][k][2 + h], sum);
-        }
-      }
+        for (int i = 0; i < 4; ++i)
+          to[(8 * n + 2 * c + (i & 1)) * (TURN + 4) + k * 16 + g + 8 * (i >> 1)] = o[n][TURN_NO * (TURN / 16) + k][i];
   }
 };
 
@@ -241,23 +219,27 @@ template <int D, int HC>
 struct F32Core {
   using T = float;
   static constexpr int ROWS = HC, ROW = D * 4;
-  static constexpr int N = D / 32, STATE = 32 * HC * (2 + N);
+  static constexpr int N = D / 32, TURN = D;
   float m[HC], l[HC], o[HC][N];
   float *q, *p;  // shared, of this warp: [HC][D] and [HC][16]
 
-  __device__ void start(const float* x, int heads) {
+  __device__ void load_q(const float* x, int heads) {
     __syncwarp();
+#pragma unroll
+    for (int h = 0; h < HC; ++h)
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        q[h * D + i * 32 + lane_id()] = h < heads ? x[h * D + i * 32 + lane_id()] : 0.f;
+    __syncwarp();
+  }
+  __device__ void start() {
 #pragma unroll
     for (int h = 0; h < HC; ++h) {
       m[h] = -INFINITY;
       l[h] = 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        o[h][i] = 0.f;
-        q[h * D + i * 32 + lane_id()] = h < heads ? x[h * D + i * 32 + lane_id()] : 0.f;
-      }
+      for (int i = 0; i < N; ++i) o[h][i] = 0.f;
     }
-    __syncwarp();
   }
 
   __device__ void block(const uint8_t* sK, const uint8_t* sV, uint32_t keys, float scale_log2) {
@@ -324,40 +306,21 @@ struct F32Core {
     __syncwarp();
   }
 
-  __device__ void dump(float* to) const {
-    const int lane = lane_id();
-#pragma unroll
-    for (int h = 0; h < HC; ++h) {
-      to[h * 32 + lane] = m[h];
-      to[(HC + h) * 32 + lane] = l[h];
-#pragma unroll
-      for (int i = 0; i < N; ++i) to[(2 * HC + h * N + i) * 32 + lane] = o[h][i];
-    }
-  }
-  __device__ void merge(const float* from) {
-    const int lane = lane_id();
-#pragma unroll
-    for (int h = 0; h < HC; ++h) {
-      const float om = from[h * 32 + lane], to = fmaxf(m[h], om);
-      const float a = to == -INFINITY ? 1.f : ex2(m[h] - to), b = to == -INFINITY ? 0.f : ex2(om - to);
-      m[h] = to;
-      l[h] = l[h] * a + from[(HC + h) * 32 + lane] * b;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o[h][i] = o[h][i] * a + from[(2 * HC + h * N + i) * 32 + lane] * b;
-    }
-  }
-  template <typename F, typename G>
-  __device__ void each(int heads, F row_of, G value_of) {
+  __device__ void dump_ml(float2* to) const {
 #pragma unroll
     for (int h = 0; h < HC; ++h) {
       float sum = l[h];
 #pragma unroll
       for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-      if (h >= heads) continue;
-      if (lane_id() == 0) row_of(h, m[h], sum);
-#pragma unroll
-      for (int i = 0; i < N; ++i) value_of(h, N * static_cast<int>(lane_id()) + i, o[h][i], sum);
+      if (lane_id() == 0) to[h] = make_float2(m[h], sum);
     }
+  }
+  template <int>
+  __device__ void dump(float* to) const {
+#pragma unroll
+    for (int h = 0; h < HC; ++h)
+#pragma unroll
+      for (int i = 0; i < N; ++i) to[h * (D + 4) + N * lane_id() + i] = o[h][i];
   }
 };
 
@@ -376,7 +339,7 @@ struct PagedSmem<F32Core<D, HC>> {
 template <typename Core>
 constexpr int paged_smem() {
   return kWarps * (PagedSmem<Core>::STAGES * 2 * kKeys * Core::ROW + PagedSmem<Core>::EXTRA) +
-         2 * Core::STATE * 4;
+         kWarps * Core::ROWS * (Core::TURN + 4) * 4;
 }
 // Floats of a unit's piece: o, then each row's m and sum; whole 16 bytes.
 template <int ROWS, int D>
@@ -408,9 +371,11 @@ __global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
   using T = typename Core::T;
   constexpr int STAGES = PagedSmem<Core>::STAGES, ROW = Core::ROW, BLOCK = kKeys * ROW;
   constexpr int PIECES = ROW / 16, ROWS_A_GO = 32 / PIECES;  // 16-byte pieces of a row, rows a warp copies at once
-  extern __shared__ __align__(16) uint8_t smem[];
+  // whole lines: cp.async takes a line of memory in one request only where it lands in one line here
+  extern __shared__ __align__(128) uint8_t smem[];
   __shared__ long long s_scan[kWarps], s_total;
   __shared__ TileAt s_first;
+  __shared__ float2 s_ml[kWarps][Core::ROWS];
   const int warp = warp_id(), lane = lane_id();
   const int parts = a.sh.Hk * a.chunks, group = a.sh.H / a.sh.Hk;
   launch_dependents();
@@ -434,7 +399,10 @@ __global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
   __syncthreads();
   const long long total = s_total * parts, run = (total + gridDim.x - 1) / gridDim.x;
   const long long begin = blockIdx.x * run;
-  if (begin >= total) return;
+  if (begin >= total) {
+    if (a.cuts_by_cta && threadIdx.x == 0) a.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   if ((upto - mine) * parts <= begin && begin < upto * parts) {
     long long at = (upto - mine) * parts;
     int b = lo, len = keys_of(a, lens, b);
@@ -464,25 +432,30 @@ __global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
   float* scratch = reinterpret_cast<float*>(smem + kWarps * STAGES * 2 * BLOCK);
   Core core;
   if constexpr (sizeof(T) == 4) {
-    core.q = scratch + 2 * Core::STATE + warp * (Core::ROWS * (D + 16));
+    core.q = scratch + kWarps * Core::ROWS * (Core::TURN + 4) + warp * (Core::ROWS * (D + 16));
     core.p = core.q + Core::ROWS * D;
   }
 
-  // The place in the pools of lane's key of a tile (lanes 0-15), or -1; loaded a tile ahead.
-  auto slot_of = [&](const TileAt& t) {
+  // The page of lane's key of a tile (lanes 0-15) is loaded a tile ahead, and looked at only when that
+  // tile is copied: an instruction that uses it any sooner would stop the warp until it is there.
+  auto key_of = [&](const TileAt& t) {
     const int key = t.tile * kTileKeys + warp * kKeys + (lane & 15);
-    if (t.left <= 0 || key >= t.len) return -1;
-    const int i = a.page.of(key), page = __ldg(table + static_cast<size_t>(t.b) * a.sh.max_pages + i);
-    return page < 0 || page >= a.sh.num_pages ? -1 : (page - i) * a.sh.page_size + key;
+    return t.left > 0 && key < t.len ? key : -1;
+  };
+  auto page_of = [&](const TileAt& t) {
+    const int key = key_of(t);
+    return key < 0 ? -1 : __ldg(table + static_cast<size_t>(t.b) * a.sh.max_pages + a.page.of(key));
   };
   TileAt ahead = use;
-  int slot = slot_of(ahead);
+  int page = page_of(ahead);
   uint32_t keys_in[STAGES];
   // Copies the tile at `ahead` into stage `st`; rows that are no keys become zeros, so that what lies
   // there cannot meet a weight of zero as NaN.
   const int my_row = lane / PIECES, my_col = lane % PIECES;
   const size_t pitch = static_cast<size_t>(a.sh.Hk) * D;
   auto fetch = [&](int st, uint32_t& keys) {
+    const int key = key_of(ahead);  // -1 with page -1
+    const int slot = page < 0 || page >= a.sh.num_pages ? -1 : (page - a.page.of(key)) * a.sh.page_size + key;
     keys = __ballot_sync(0xffffffffu, slot >= 0) & 0xffffu;
     if (keys) {
       const uint32_t dst = smem_u32(ring + st * 2 * BLOCK);
@@ -499,10 +472,10 @@ __global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
     }
     cp_async_commit();
     advance(ahead);
-    slot = slot_of(ahead);
+    page = page_of(ahead);
   };
 #pragma unroll
-  for (int st = 0; st < STAGES - 1; ++st) fetch(st, keys_in[st]);
+  for (int st = 0; st < STAGES; ++st) fetch(st, keys_in[st]);
 
   auto q_of = [&](const TileAt& t, int* heads, int* first) {
     *heads = min(a.chunk_heads, group - t.chunk * a.chunk_heads);
@@ -512,130 +485,160 @@ __global__ void __launch_bounds__(kWarps * 32, PagedSmem<Core>::CTAS)
   int heads, first;
   {
     const T* x = q_of(use, &heads, &first);
-    core.start(x, heads);
+    core.load_q(x, heads);
+    core.start();
   }
   bool from_before = use.tile > 0;  // the unit began in an earlier CTA
   while (use.left > 0) {
 #pragma unroll
     for (int st = 0; st < STAGES; ++st) {  // unrolled: the stage is a constant
       if (use.left <= 0) break;
-      cp_async_wait<STAGES - 2>();
+      cp_async_wait<STAGES - 1>();
       __syncwarp();
-      {
-        const int to = (st + STAGES - 1) % STAGES;
-        fetch(to, keys_in[to]);
-      }
       const uint32_t keys = keys_in[st];
-      if (keys) {
-        if constexpr (sizeof(T) == 2)
-          core.block(smem_u32(ring + st * 2 * BLOCK), smem_u32(ring + st * 2 * BLOCK + BLOCK), keys, a.scale_log2);
-        else
-          core.block(ring + st * 2 * BLOCK, ring + st * 2 * BLOCK + BLOCK, keys, a.scale_log2);
+      const uint8_t *k_block = ring + st * 2 * BLOCK, *v_block = k_block + BLOCK;
+      if constexpr (sizeof(T) == 2) {
+        if (keys) core.load(k_block, v_block);
+        __syncwarp();
+        fetch(st, keys_in[st]);
+        if (keys) core.block(keys, a.scale_log2);
+      } else {
+        if (keys) core.block(k_block, v_block, keys, a.scale_log2);
+        __syncwarp();
+        fetch(st, keys_in[st]);
       }
-      __syncwarp();
       const TileAt was = use;
       advance(use);
       const bool ends = was.tile + 1 == was.n_tiles;
       if (!ends && use.left > 0) continue;
-      // The unit, or this CTA's run, ends: merge the warps, 2 and 3 into 0 and 1, then 1 into 0.
-      if (warp >= 2) core.dump(scratch + (warp - 2) * Core::STATE);
-      __syncthreads();
-      if (warp < 2) core.merge(scratch + warp * Core::STATE);
-      __syncthreads();
-      if (warp == 1) core.dump(scratch);
-      __syncthreads();
-      if (warp == 0) {
-        core.merge(scratch);
-        if (ends && !from_before) {
-          const size_t out = static_cast<size_t>(was.b) * a.sh.H + first;
-          core.each(
-              heads,
-              [&](int row, float m, float l) {
-                if (lse) lse[out + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
-              },
-              [&](int row, int col, float x, float l) {
-                const float y = l == 0.f ? 0.f : x / l;
-                if constexpr (sizeof(T) == 2) o[(out + row) * D + col] = __float2bfloat16_rn(y);
-                else o[(out + row) * D + col] = y;
-              });
-        } else {
-          // slot 0 of a CTA: a unit from before; slot 1: one that goes on in the next
-          float* to = a.pieces + (2 * static_cast<size_t>(blockIdx.x) + (from_before ? 0 : 1)) * piece_floats<Core::ROWS, D>();
-          core.each(
-              heads,
-              [&](int row, float m, float l) {
-                *reinterpret_cast<float2*>(to + Core::ROWS * D + 2 * row) = make_float2(m, l);
-              },
-              [&](int row, int col, float x, float) { to[row * D + col] = x; });
-        }
-        if (!from_before && lane == 0) {  // the CTAs of a unit, told by the first
-          const int later = static_cast<int>((was.n_tiles - 1 - was.tile + run - 1) / run);
-          a.spans[static_cast<size_t>(was.b) * parts + was.kh * a.chunks + was.chunk] = make_int2(blockIdx.x, blockIdx.x + (ends ? 0 : later));
-        }
-      }
-      __syncthreads();
+      // The unit, or this CTA's run, ends. The next unit's q is loaded while the warps' states are merged
+      // through the scratch memory, TURN values of each head at a time, by all threads.
+      const int was_heads = heads, was_first = first;
       if (use.left > 0) {
-        from_before = false;
         const T* x = q_of(use, &heads, &first);
-        core.start(x, heads);
+        core.load_q(x, heads);
       }
+      const bool whole = ends && !from_before;
+      // slot 0 of a CTA: a unit from before; slot 1: one that goes on in the next
+      float* piece = a.pieces + (2 * static_cast<size_t>(blockIdx.x) + (from_before ? 0 : 1)) * piece_floats<Core::ROWS, D>();
+      const size_t out = static_cast<size_t>(was.b) * a.sh.H + was_first;
+      constexpr int TURN = Core::TURN, FOURS = TURN / 4;
+      auto merge = [&](auto turn) {
+        constexpr int AT = decltype(turn)::value * TURN;
+        __syncthreads();  // the scratch memory is free
+        if (AT == 0) core.dump_ml(s_ml[warp]);
+        core.template dump<decltype(turn)::value>(scratch + warp * Core::ROWS * (TURN + 4));
+        __syncthreads();
+        for (int i = threadIdx.x; i < was_heads * FOURS; i += kWarps * 32) {
+          const int row = i / FOURS, col = i % FOURS * 4;
+          float m = -INFINITY, l = 0.f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) m = fmaxf(m, s_ml[w][row].x);
+          float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 ml = s_ml[w][row];
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
+            const float4 y = *reinterpret_cast<const float4*>(scratch + (w * Core::ROWS + row) * (TURN + 4) + col);
+            l = fmaf(ml.y, f, l);
+            x.x = fmaf(y.x, f, x.x), x.y = fmaf(y.y, f, x.y), x.z = fmaf(y.z, f, x.z), x.w = fmaf(y.w, f, x.w);
+          }
+          if (!whole) {
+            *reinterpret_cast<float4*>(piece + row * D + AT + col) = x;
+            if (AT == 0 && col == 0) *reinterpret_cast<float2*>(piece + Core::ROWS * D + 2 * row) = make_float2(m, l);
+            continue;
+          }
+          const float inv = l == 0.f ? 0.f : 1.f / l;
+          T* to = o + (out + row) * D + AT + col;
+          if constexpr (sizeof(T) == 2)
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+          else
+            *reinterpret_cast<float4*>(to) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+          if (lse && AT == 0 && col == 0) lse[out + row] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
+        }
+      };
+      merge(std::integral_constant<int, 0>());
+      if constexpr (D / TURN > 1) merge(std::integral_constant<int, 1>());
+      if constexpr (D / TURN > 2) {
+        merge(std::integral_constant<int, 2>());
+        merge(std::integral_constant<int, 3>());
+      }
+      if (warp == 0) {
+        if (!from_before && lane == 0 && (!a.cuts_by_cta || !ends)) {  // told by the first of a unit's CTAs
+          const int unit = (was.b * a.sh.Hk + was.kh) * a.chunks + was.chunk;
+          const int later = ends ? 0 : static_cast<int>((was.n_tiles - 1 - was.tile + run - 1) / run);
+          a.cuts[a.cuts_by_cta ? blockIdx.x : unit] = make_int4(unit, blockIdx.x, blockIdx.x + later, 0);
+        }
+        if (a.cuts_by_cta && lane == 0 && use.left <= 0 && (from_before || ends))
+          a.cuts[blockIdx.x] = make_int4(0, 0, 0, 0);  // nothing that begins here goes on
+      }
+      from_before = false;
+      core.start();
     }
   }
   cp_async_wait<0>();
 }
 
-// Joins the pieces of the units that several CTAs hold: a block takes (sequence, head).
+// Joins the pieces of the units that several CTAs hold: a block takes (cut unit, head). Its threads share
+// the pieces out, each with a running maximum, so that the loads of all pieces are on their way at once.
+constexpr int kJoinThreads = 256;
 template <typename T, int D, int ROWS>
-__global__ void __launch_bounds__(128)
+__global__ void __launch_bounds__(kJoinThreads)
     paged_join_kernel(const __grid_constant__ PagedArgs a, T* __restrict__ o, float* __restrict__ lse) {
-  constexpr int LANES = D / 4, PARTS = 128 / LANES;  // threads that share a row, pieces at a time
-  __shared__ float s_m[128], s_l[PARTS], s_o[PARTS][D];
-  const int group = a.sh.H / a.sh.Hk, b = blockIdx.x / a.sh.H, h = blockIdx.x % a.sh.H, gh = h % group;
-  const int part = h / group * a.chunks + gh / a.chunk_heads, row = gh % a.chunk_heads;
+  constexpr int LANES = D / 4, PARTS = kJoinThreads / LANES;  // threads that share a row, pieces at a time
+  __shared__ float2 s_ml[PARTS];
+  __shared__ __align__(16) float s_o[PARTS][D];
+  const int row = blockIdx.x % a.chunk_heads;
   wait_prerequisites();
-  const int2 span = a.spans[static_cast<size_t>(b) * a.sh.Hk * a.chunks + part];
-  if (span.x == span.y) return;
-  const int n = span.y - span.x + 1;
+  const int4 cut = a.cuts[blockIdx.x / a.chunk_heads];  // unit, first and last CTA
+  const int group = a.sh.H / a.sh.Hk, chunk = cut.x % a.chunks, n = cut.z - cut.y + 1;
+  if (n <= 1 || chunk * a.chunk_heads + row >= group) return;
   auto piece = [&](int i) {  // the first CTA's last unit, the others' first
-    return a.pieces + (2 * static_cast<size_t>(span.x + i) + (i == 0 ? 1 : 0)) * piece_floats<ROWS, D>();
+    return a.pieces + (2 * static_cast<size_t>(cut.y + i) + (i == 0 ? 1 : 0)) * piece_floats<ROWS, D>();
   };
-  float m = -INFINITY;
-  for (int i = threadIdx.x; i < n; i += 128) m = fmaxf(m, piece(i)[ROWS * D + 2 * row]);
-  s_m[threadIdx.x] = m;
-  __syncthreads();
-  for (int d = 64; d > 0; d >>= 1) {
-    if (threadIdx.x < d) s_m[threadIdx.x] = fmaxf(s_m[threadIdx.x], s_m[threadIdx.x + d]);
-    __syncthreads();
-  }
-  m = s_m[0];
   const int lane = threadIdx.x % LANES, p = threadIdx.x / LANES;
-  float l = 0.f;
+  float m = -INFINITY, l = 0.f;
   float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-  for (int i = p; i < n; i += PARTS) {
-    const float* from = piece(i);
-    const float2 ml = *reinterpret_cast<const float2*>(from + ROWS * D + 2 * row);
-    const float4 y = *reinterpret_cast<const float4*>(from + row * D + 4 * lane);
-    const float w = ml.x == -INFINITY ? 0.f : ex2(ml.x - m);
-    l = fmaf(ml.y, w, l);
-    x.x = fmaf(y.x, w, x.x), x.y = fmaf(y.y, w, x.y), x.z = fmaf(y.z, w, x.z), x.w = fmaf(y.w, w, x.w);
+  auto add = [&](float2 ml, float4 y) {
+    const float to = fmaxf(m, ml.x);
+    const float u = to == -INFINITY ? 1.f : ex2(m - to), w = ml.x == -INFINITY ? 0.f : ex2(ml.x - to);
+    m = to;
+    l = l * u + ml.y * w;
+    x.x = x.x * u + y.x * w, x.y = x.y * u + y.y * w, x.z = x.z * u + y.z * w, x.w = x.w * u + y.w * w;
+  };
+  constexpr int GO = 8;
+#pragma unroll 1
+  for (int i0 = p; i0 < n; i0 += GO * PARTS) {
+    float2 ml[GO];
+    float4 y[GO];
+#pragma unroll
+    for (int k = 0; k < GO; ++k) {
+      const int i = i0 + k * PARTS;
+      if (i < n) {
+        const float* from = piece(i);
+        ml[k] = *reinterpret_cast<const float2*>(from + ROWS * D + 2 * row);
+        y[k] = *reinterpret_cast<const float4*>(from + row * D + 4 * lane);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < GO; ++k)
+      if (i0 + k * PARTS < n) add(ml[k], y[k]);
   }
   *reinterpret_cast<float4*>(&s_o[p][4 * lane]) = x;
-  if (lane == 0) s_l[p] = l;
+  if (lane == 0) s_ml[p] = make_float2(m, l);
   __syncthreads();
-  float sum = 0.f;
+  if (p > 0) return;
 #pragma unroll
-  for (int i = 0; i < PARTS; ++i) sum += s_l[i];
-  for (int d = threadIdx.x; d < D; d += 128) {
-    float y = 0.f;
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) y += s_o[i][d];
-    y = sum == 0.f ? 0.f : y / sum;
-    T* to = o + static_cast<size_t>(blockIdx.x) * D + d;
-    if constexpr (sizeof(T) == 2) *to = __float2bfloat16_rn(y);
-    else *to = y;
-  }
-  if (lse && threadIdx.x == 0) lse[blockIdx.x] = sum == 0.f ? -INFINITY : (m + __log2f(sum)) * kLn2;
+  for (int i = 1; i < PARTS; ++i) add(s_ml[i], *reinterpret_cast<const float4*>(&s_o[i][4 * lane]));
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int unit = cut.x / a.chunks;  // (sequence, kv head)
+  const size_t out = static_cast<size_t>(unit / a.sh.Hk) * a.sh.H + (unit % a.sh.Hk) * group + chunk * a.chunk_heads + row;
+  T* to = o + out * D + 4 * lane;
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(x.x * inv, x.y * inv), pack_bf16x2(x.z * inv, x.w * inv));
+  else
+    *reinterpret_cast<float4*>(to) = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+  if (lse && lane == 0) lse[out] = l == 0.f ? -INFINITY : (m + __log2f(l)) * kLn2;
 }
 
 // Heads of a chunk of a group, and the chunks: as even as they go.
@@ -664,18 +667,21 @@ int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const 
   a.chunks = p.chunks;
   a.chunk_heads = p.chunk_heads;
   a.pieces = static_cast<float*>(ws);
-  a.spans = reinterpret_cast<int2*>(a.pieces + 2 * static_cast<size_t>(p.ctas) * 16 * (D + 2));
+  a.cuts = reinterpret_cast<int4*>(a.pieces + 2 * static_cast<size_t>(p.ctas) * 16 * (D + 2));
   // as many CTAs as there can be tiles of keys
   const long long unit_tiles = (static_cast<long long>(sh.max_pages) * sh.page_size + kTileKeys - 1) / kTileKeys;
   a.end_tiles = unit_tiles > 1;
   const long long tiles = static_cast<long long>(sh.B) * sh.Hk * p.chunks * (unit_tiles + a.end_tiles);
   const int grid = static_cast<int>(tiles < p.ctas ? tiles : p.ctas);
+  a.cuts_by_cta = static_cast<long long>(sh.B) * sh.Hk * p.chunks > grid;
   paged_step_kernel<Core, D><<<grid, kWarps * 32, paged_smem<Core>(), s>>>(
       a, static_cast<const T*>(q), static_cast<const T*>(kc), static_cast<const T*>(vc), table, lens,
       static_cast<T*>(o), lse);
   if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
   if (unit_tiles == 1) return PA_OK;  // no unit is cut
-  return launch_beside(paged_join_kernel<T, D, Core::ROWS>, dim3(sh.B * sh.H), 128, 0, s, a, static_cast<T*>(o), lse);
+  const int cuts = a.cuts_by_cta ? grid : sh.B * sh.Hk * p.chunks;
+  return launch_beside(paged_join_kernel<T, D, Core::ROWS>, dim3(cuts * p.chunk_heads), kJoinThreads, 0, s, a,
+                       static_cast<T*>(o), lse);
 }
 
 template <int D>
@@ -699,7 +705,7 @@ int paged_f32(const PagedShape& sh, const PagedPlan& p, const void* q, const voi
 size_t paged_attn_workspace_bytes(const PagedShape& sh) {
   const PagedPlan p = paged_plan(sh);
   return 2 * static_cast<size_t>(p.ctas) * 16 * (sh.D + 2) * sizeof(float) +
-         (static_cast<size_t>(sh.B) * sh.Hk * p.chunks * sizeof(int2) + 255) / 256 * 256;
+         p.ctas * sizeof(int4);
 }
 
 int launch_paged_attn(const PagedShape& sh, const void* q, const void* kc, const void* vc, const int32_t* table,
