@@ -470,8 +470,13 @@ def linear_attn_step(q, k, v, log_decay, state_in, o, state_out, desc=None, stre
         o.data_ptr(), state_out.data_ptr(), _stream() if stream is None else stream))
 
 
-# Descriptors and workspace sizes of the calls below by shape, as above.
-_packed_descs, _paged_descs, _norm_descs, _work_sizes = {}, {}, {}, {}
+# The calls below by the layouts of their tensors: the checks, descriptors and workspace sizes of a call are
+# those of any other with the same layouts, and making them costs a short call more than its launch.
+_calls = {}
+
+
+def _layouts(*tensors):
+    return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
 def _token_stride(fn, name, t, heads, D, dev, dtype, tokens):
@@ -497,7 +502,7 @@ def _token_stride(fn, name, t, heads, D, dev, dtype, tokens):
 
 
 def _work(fn, need, workspace, like, stream):
-    """The call's workspace: the caller's, or one of the stream that will use it."""
+    """The call's workspace, as pointer, bytes and owner: the caller's, or one of the stream that will use it."""
     if workspace is None:
         import torch
         if stream is None:
@@ -505,9 +510,24 @@ def _work(fn, need, workspace, like, stream):
         else:
             with torch.cuda.stream(torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()):
                 workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
-    elif workspace.get_device() != like.get_device() or not workspace.is_contiguous():
+        return workspace.data_ptr(), need, workspace
+    if workspace.get_device() != like.get_device() or not workspace.is_contiguous():
         raise ValueError(f"{fn}: workspace must be contiguous and on {like.device}")
-    return workspace, workspace.numel() * workspace.element_size()
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size(), workspace
+
+
+def _on_stream(fn, t, stream):
+    """The stream of a call whose tensors have to be on the current device."""
+    import torch
+    dev = t.get_device()
+    if dev < 0 or dev != torch._C._cuda_getDevice():
+        raise ValueError(f"{fn}: tensors must be on the current CUDA device, not {t.device}")
+    return _stream() if stream is None else stream
+
+
+def _prepared(d, size_of=None):
+    """A descriptor, ready to be passed, and its workspace's bytes."""
+    return ctypes.byref(d), d, 0 if size_of is None else size_of(d)
 
 
 def packed_attn_desc(q, k, v, cu_seqlens, dq=None, dk=None, dv=None, scale=0.0):
@@ -516,15 +536,9 @@ def packed_attn_desc(q, k, v, cu_seqlens, dq=None, dk=None, dv=None, scale=0.0):
     T, H, D = q.shape
     Hk, fn, dev, t = k.shape[1], "packed_attn", q.get_device(), q.dtype
     stride = lambda name, x, heads: 0 if x is None else _token_stride(fn, name, x, heads, D, dev, t, T)  # noqa: E731
-    strides = (stride("q", q, H), stride("k", k, Hk), stride("v", v, Hk), stride("dq", dq, H), stride("dk", dk, Hk),
-               stride("dv", dv, Hk))
-    key = (T, H, Hk, D, t, cu_seqlens.shape, scale, strides)
-    return _kept(_packed_descs, key, lambda: PackedAttnDesc(T, cu_seqlens.numel() - 1, H, Hk, D, _dtype_code(q),
-                                                            float(scale), *strides))
-
-
-def _size_of(name, d, q):
-    return _kept(_work_sizes, (name, bytes(d), q.get_device()), lambda: getattr(load(), name)(ctypes.byref(d)))
+    return PackedAttnDesc(T, cu_seqlens.numel() - 1, H, Hk, D, _dtype_code(q), float(scale), stride("q", q, H),
+                          stride("k", k, Hk), stride("v", v, Hk), stride("dq", dq, H), stride("dk", dk, Hk),
+                          stride("dv", dv, Hk))
 
 
 def packed_attn_fwd_workspace_size(desc):
@@ -544,31 +558,39 @@ def _check_packed(fn, q, cu_seqlens, lse, names, tensors):
     if cu_seqlens.dim() != 1:
         raise ValueError(f"{fn}: cu_seqlens must have one dimension")
     _check_tensors(fn, dev, torch.int32, cu_seqlens.shape, ("cu_seqlens",), cu_seqlens)
-    _check_device(fn, q, dev)
 
 
 def packed_attn_fwd(q, k, v, cu_seqlens, o, lse, scale=0.0, workspace=None, stream=None):
     """o [T, H, D] and lse [H, T] of causal attention over the sequences cu_seqlens[i] ..
     cu_seqlens[i + 1] - 1 (int32) of q [T, H, D] and k, v [T, Hk, D], whose tokens may be slices
     of a wider tensor. A workspace is allocated with torch unless given."""
-    d = packed_attn_desc(q, k, v, cu_seqlens, scale=scale)
-    _check_packed("packed_attn_fwd", q, cu_seqlens, lse, ("o",), (o,))
-    ws, nb = _work("packed_attn_fwd", _size_of("pa_packed_attn_fwd_workspace_size", d, q), workspace, q, stream)
+    def make():
+        d = packed_attn_desc(q, k, v, cu_seqlens, scale=scale)
+        _check_packed("packed_attn_fwd", q, cu_seqlens, lse, ("o",), (o,))
+        return _prepared(d, packed_attn_fwd_workspace_size)
+
+    ref, _, need = _kept(_calls, ("packed_attn_fwd", scale, _layouts(q, k, v, cu_seqlens, o, lse)), make)
+    stream_ = _on_stream("packed_attn_fwd", q, stream)
+    ws, nb, _owner = _work("packed_attn_fwd", need, workspace, q, stream)
     _check("pa_packed_attn_fwd", load().pa_packed_attn_fwd(
-        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), o.data_ptr(),
-        lse.data_ptr(), ws.data_ptr(), nb, _stream() if stream is None else stream))
+        ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), cu_seqlens.data_ptr(), o.data_ptr(), lse.data_ptr(), ws, nb,
+        stream_))
 
 
 def packed_attn_bwd(q, k, v, o, dO, lse, cu_seqlens, dq, dk, dv, accumulate=False, scale=0.0, workspace=None,
                     stream=None):
     """Gradients dq, dk, dv (overwritten, or added to) of packed_attn_fwd from dO and its o and lse."""
-    d = packed_attn_desc(q, k, v, cu_seqlens, dq, dk, dv, scale)
-    _check_packed("packed_attn_bwd", q, cu_seqlens, lse, ("o", "dO"), (o, dO))
-    ws, nb = _work("packed_attn_bwd", _size_of("pa_packed_attn_bwd_workspace_size", d, q), workspace, q, stream)
+    def make():
+        d = packed_attn_desc(q, k, v, cu_seqlens, dq, dk, dv, scale)
+        _check_packed("packed_attn_bwd", q, cu_seqlens, lse, ("o", "dO"), (o, dO))
+        return _prepared(d, packed_attn_bwd_workspace_size)
+
+    ref, _, need = _kept(_calls, ("packed_attn_bwd", scale, _layouts(q, k, v, o, dO, lse, cu_seqlens, dq, dk, dv)), make)
+    stream_ = _on_stream("packed_attn_bwd", q, stream)
+    ws, nb, _owner = _work("packed_attn_bwd", need, workspace, q, stream)
     _check("pa_packed_attn_bwd", load().pa_packed_attn_bwd(
-        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dO.data_ptr(), lse.data_ptr(),
-        cu_seqlens.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int(bool(accumulate)), ws.data_ptr(), nb,
-        _stream() if stream is None else stream))
+        ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), dO.data_ptr(), lse.data_ptr(),
+        cu_seqlens.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), int(bool(accumulate)), ws, nb, stream_))
 
 
 def paged_attn_desc(q, k_cache, page_table, scale=0.0):
@@ -576,9 +598,7 @@ def paged_attn_desc(q, k_cache, page_table, scale=0.0):
     B, H, D = q.shape
     pages, size, Hk, _ = k_cache.shape
     step = _token_stride("paged_attn_step", "q", q, H, D, q.get_device(), q.dtype, B)
-    key = (q.shape, q.dtype, k_cache.shape, page_table.shape, step, scale)
-    return _kept(_paged_descs, key, lambda: PagedAttnDesc(B, H, Hk, D, _dtype_code(q), float(scale), size, pages,
-                                                          page_table.shape[1], step))
+    return PagedAttnDesc(B, H, Hk, D, _dtype_code(q), float(scale), size, pages, page_table.shape[1], step)
 
 
 def paged_attn_step_workspace_size(desc):
@@ -589,26 +609,30 @@ def paged_attn_step(q, k_cache, v_cache, page_table, seq_lens, o, lse=None, scal
     """o [B, H, D] (and lse [B, H]) of one token's q of each sequence against its seq_lens (int32 [B])
     cached tokens, found through page_table (int32 [B, pages a sequence]) in the pools k_cache and
     v_cache [pages, page size, Hk, D]. A workspace is allocated with torch unless given."""
-    import torch
-    fn, dev = "paged_attn_step", q.get_device()
-    d = paged_attn_desc(q, k_cache, page_table, scale)
-    _check_tensors(fn, dev, q.dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
-    if k_cache.shape[3] != q.shape[2]:
-        raise ValueError(f"{fn}: the caches must have heads of {q.shape[2]}")
-    _check_tensors(fn, dev, torch.int32, (q.shape[0], d.max_pages), ("page_table",), page_table)
-    _check_tensors(fn, dev, torch.int32, q.shape[:1], ("seq_lens",), seq_lens)
-    _check_tensors(fn, dev, q.dtype, q.shape, ("o",), o)
-    if lse is not None:
+    fn = "paged_attn_step"
+
+    def make():
+        import torch
+        d, dev = paged_attn_desc(q, k_cache, page_table, scale), q.get_device()
+        _check_tensors(fn, dev, q.dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
+        if k_cache.shape[3] != q.shape[2]:
+            raise ValueError(f"{fn}: the caches must have heads of {q.shape[2]}")
+        _check_tensors(fn, dev, torch.int32, (q.shape[0], d.max_pages), ("page_table",), page_table)
+        _check_tensors(fn, dev, torch.int32, q.shape[:1], ("seq_lens",), seq_lens)
+        _check_tensors(fn, dev, q.dtype, q.shape, ("o",), o)
         _check_tensors(fn, dev, torch.float32, q.shape[:2], ("lse",), lse)
-    _check_device(fn, q, dev)
-    ws, nb = _work(fn, _size_of("pa_paged_attn_step_workspace_size", d, q), workspace, q, stream)
+        return _prepared(d, paged_attn_step_workspace_size)
+
+    ref, _, need = _kept(_calls, (fn, scale, _layouts(q, k_cache, v_cache, page_table, seq_lens, o, lse)), make)
+    stream_ = _on_stream(fn, q, stream)
+    ws, nb, _owner = _work(fn, need, workspace, q, stream)
     _check("pa_paged_attn_step", load().pa_paged_attn_step(
-        ctypes.byref(d), q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(),
-        seq_lens.data_ptr(), o.data_ptr(), _ptr(lse), ws.data_ptr(), nb, _stream() if stream is None else stream))
+        ref, q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), page_table.data_ptr(), seq_lens.data_ptr(),
+        o.data_ptr(), _ptr(lse), ws, nb, stream_))
 
 
-def _norm_desc(fn, rope, eps, q, k, v, dq, dk, positions, gammas):
-    """The descriptor of a call's tensors; checks those that may be slices, positions and gammas."""
+def _norm_desc(fn, rope, eps, q, k, v, dq, dk, positions, gammas, outs, size_of=None):
+    """Checks a call's tensors against its rope_desc and makes its descriptor. outs: (name, tensor, heads)."""
     import torch
     B, L, H, Hk, D = rope.batch, rope.seq_len, rope.num_heads, rope.num_kv_heads, rope.head_dim
     dtype, dev = torch.float32 if rope.dtype == PA_F32 else torch.bfloat16, q.get_device()
@@ -618,8 +642,10 @@ def _norm_desc(fn, rope, eps, q, k, v, dq, dk, positions, gammas):
                     (("q", q, H), ("k", k, Hk), ("v", v, Hk), ("dq", dq, H), ("dk", dk, Hk)))
     _check_tensors(fn, dev, torch.int32, (rope.axes, B, L), ("positions",), positions)
     _check_tensors(fn, dev, torch.float32, (D,), ("gamma_q", "gamma_k", "dgamma_q", "dgamma_k"), *gammas)
-    _check_device(fn, q, dev)
-    return _kept(_norm_descs, (bytes(rope), eps, strides), lambda: QkNormDesc(rope, eps, *strides)), dtype, dev
+    for name, x, heads in outs:
+        _check_tensors(fn, dev, dtype, (B, L, heads, D), (name,), x)
+    # (a copy: the caller's may be changed after this call)
+    return _prepared(QkNormDesc(RopeDesc.from_buffer_copy(rope), eps, *strides), size_of)
 
 
 def qk_norm_rope_fwd(q, k, gamma_q, gamma_k, positions, q_out, k_out, desc, eps=1e-6, stream=None):
@@ -627,12 +653,13 @@ def qk_norm_rope_fwd(q, k, gamma_q, gamma_k, positions, q_out, k_out, desc, eps=
     gamma [D] fp32 (None: not normed), then turned by positions (int32 [axes, B, L]) as desc, a
     rope_desc, says. q and k [B, L, heads, D] may be slices of a wider tensor, or the outputs."""
     fn = "qk_norm_rope_fwd"
-    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, None, None, None, positions, (gamma_q, gamma_k))
-    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_heads, desc.head_dim), ("q_out",), q_out)
-    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim), ("k_out",), k_out)
+    ref, _, _ = _kept(
+        _calls, (fn, eps, bytes(desc), _layouts(q, k, gamma_q, gamma_k, positions, q_out, k_out)),
+        lambda: _norm_desc(fn, desc, eps, q, k, None, None, None, positions, (gamma_q, gamma_k),
+                           (("q_out", q_out, desc.num_heads), ("k_out", k_out, desc.num_kv_heads))))
     _check("pa_qk_norm_rope_fwd", load().pa_qk_norm_rope_fwd(
-        ctypes.byref(d), q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k), positions.data_ptr(), q_out.data_ptr(),
-        _ptr(k_out), _stream() if stream is None else stream))
+        ref, q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k), positions.data_ptr(), q_out.data_ptr(), _ptr(k_out),
+        _on_stream(fn, q, stream)))
 
 
 def qk_norm_rope_cache(q, k, v, gamma_q, gamma_k, positions, slots, q_out, k_cache, v_cache, desc, eps=1e-6,
@@ -640,22 +667,27 @@ def qk_norm_rope_cache(q, k, v, gamma_q, gamma_k, positions, slots, q_out, k_cac
     """qk_norm_rope_fwd whose k, and v as it is, go to rows slots (int32 [B, L]: page * page size + place;
     outside the cache: not written) of k_cache and v_cache [pages, page size, Hk, D]; k_out (None: not
     wanted) receives k too."""
-    import torch
     fn = "qk_norm_rope_cache"
-    if k is None or v is None:
-        raise ValueError(f"{fn}: k and v are needed")
-    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, v, None, None, positions, (gamma_q, gamma_k))
-    B, L, Hk, D = desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim
-    _check_tensors(fn, dev, dtype, (B, L, desc.num_heads, D), ("q_out",), q_out)
-    _check_tensors(fn, dev, dtype, (B, L, Hk, D), ("k_out",), k_out)
-    _check_tensors(fn, dev, torch.int32, (B, L), ("slots",), slots)
-    if k_cache.dim() != 4 or k_cache.shape[2:] != (Hk, D):
-        raise ValueError(f"{fn}: the caches must be [pages, page size, {Hk}, {D}]")
-    _check_tensors(fn, dev, dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
+
+    def make():
+        import torch
+        if k is None or v is None:
+            raise ValueError(f"{fn}: k and v are needed")
+        Hk, D = desc.num_kv_heads, desc.head_dim
+        got = _norm_desc(fn, desc, eps, q, k, v, None, None, positions, (gamma_q, gamma_k),
+                         (("q_out", q_out, desc.num_heads), ("k_out", k_out, Hk)))
+        _check_tensors(fn, q.get_device(), torch.int32, (desc.batch, desc.seq_len), ("slots",), slots)
+        if k_cache.dim() != 4 or k_cache.shape[2:] != (Hk, D):
+            raise ValueError(f"{fn}: the caches must be [pages, page size, {Hk}, {D}]")
+        _check_tensors(fn, q.get_device(), q.dtype, k_cache.shape, ("k_cache", "v_cache"), k_cache, v_cache)
+        return got
+
+    ref, _, _ = _kept(_calls, (fn, eps, bytes(desc), _layouts(q, k, v, gamma_q, gamma_k, positions, slots, q_out,
+                                                              k_cache, v_cache, k_out)), make)
     _check("pa_qk_norm_rope_cache", load().pa_qk_norm_rope_cache(
-        ctypes.byref(d), q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(gamma_q), _ptr(gamma_k),
-        positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(),
-        k_cache.shape[0] * k_cache.shape[1], _stream() if stream is None else stream))
+        ref, q.data_ptr(), k.data_ptr(), v.data_ptr(), _ptr(gamma_q), _ptr(gamma_k), positions.data_ptr(),
+        slots.data_ptr(), q_out.data_ptr(), _ptr(k_out), k_cache.data_ptr(), v_cache.data_ptr(),
+        k_cache.shape[0] * k_cache.shape[1], _on_stream(fn, q, stream)))
 
 
 def qk_norm_rope_bwd_workspace_size(desc):
@@ -667,16 +699,22 @@ def qk_norm_rope_bwd(dq_out, dk_out, q, k, gamma_q, gamma_k, positions, dq, dk, 
     """Gradients dq, dk and dgamma_q, dgamma_k (None: not wanted) of qk_norm_rope_fwd's inputs from those
     of its outputs, overwritten or added to. A workspace is allocated with torch unless given."""
     fn = "qk_norm_rope_bwd"
-    if k is not None and dk is None:
-        raise ValueError(f"{fn}: dk goes with k")
-    d, dtype, dev = _norm_desc(fn, desc, eps, q, k, None, dq, dk, positions, (gamma_q, gamma_k, dgamma_q, dgamma_k))
-    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_heads, desc.head_dim), ("dq_out",), dq_out)
-    _check_tensors(fn, dev, dtype, (desc.batch, desc.seq_len, desc.num_kv_heads, desc.head_dim), ("dk_out",), dk_out)
-    ws, nb = _work(fn, _size_of("pa_qk_norm_rope_bwd_workspace_size", d, q), workspace, q, stream)
+
+    def make():
+        if k is not None and dk is None:
+            raise ValueError(f"{fn}: dk goes with k")
+        return _norm_desc(fn, desc, eps, q, k, None, dq, dk, positions, (gamma_q, gamma_k, dgamma_q, dgamma_k),
+                          (("dq_out", dq_out, desc.num_heads), ("dk_out", dk_out, desc.num_kv_heads)),
+                          qk_norm_rope_bwd_workspace_size)
+
+    ref, _, need = _kept(_calls, (fn, eps, bytes(desc), _layouts(dq_out, dk_out, q, k, gamma_q, gamma_k, positions, dq,
+                                                                 dk, dgamma_q, dgamma_k)), make)
+    stream_ = _on_stream(fn, q, stream)
+    ws, nb, _owner = _work(fn, need, workspace, q, stream)
     _check("pa_qk_norm_rope_bwd", load().pa_qk_norm_rope_bwd(
-        ctypes.byref(d), dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k),
-        positions.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dgamma_q), _ptr(dgamma_k), int(bool(accumulate)),
-        ws.data_ptr(), nb, _stream() if stream is None else stream))
+        ref, dq_out.data_ptr(), _ptr(dk_out), q.data_ptr(), _ptr(k), _ptr(gamma_q), _ptr(gamma_k),
+        positions.data_ptr(), dq.data_ptr(), _ptr(dk), _ptr(dgamma_q), _ptr(dgamma_k), int(bool(accumulate)), ws, nb,
+        stream_))
 
 
 def device_status(clear=True, stream=None):
