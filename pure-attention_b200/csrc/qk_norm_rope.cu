@@ -10,6 +10,8 @@
 // The statistics are sums in fp32 over the lanes that share a head; r is computed
 // again in the backward, which reads x anyway, rather than stored.
 #include <cmath>
+#include <cstring>
+#include <type_traits>
 #include <cuda_bf16.h>
 #include "host_launchers.h"
 
@@ -18,11 +20,16 @@ namespace {
 
 constexpr int kNormThreads = 256;
 constexpr int kNormMaxPairs = 128;  // head_dim <= 256
+// Heads that a thread loads before it works on the first.
+__host__ __device__ constexpr int norm_at_once(int U, bool bwd) { return U > 1 ? 1 : bwd ? 2 : 4; }
 
+// w_i / 2 pi as a fraction of 2^64: position * turns modulo 2^64 is the fraction of a turn, exact but for the
+// table's own rounding (2^-33 of a turn at position 2^31), in integers.
 struct NormTable {
-  double turns[kNormMaxPairs];  // w_i / 2 pi
+  uint64_t turns[kNormMaxPairs];
   uint8_t axis[kNormMaxPairs];
 };
+constexpr int kNormAngles = 4;  // of a tile that a thread computes, at most
 
 // One tensor of the call: heads of D values, tokens `stride` values apart.
 template <typename T>
@@ -46,49 +53,13 @@ struct NormArgs {
   const int32_t* pos;
   float* partial;  // backward: [block][2][D] sums of dgamma
   long long n_tok;
-  int P, D, lanes, tile;  // lanes that share a head (a power of two); tokens of a tile
+  int P, D, lanes, tile, G;  // lanes that share a head (a power of two); tokens of a tile, head slots of a token
   float eps;
 };
 
 __device__ __forceinline__ float to_f(float x) { return x; }
 __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// V values at p (16 bytes of them, or one) as floats, and back.
-template <int V>
-__device__ __forceinline__ void load_run(const float* p, float (&f)[V]) {
-  if constexpr (V == 4) {
-    const float4 x = *reinterpret_cast<const float4*>(p);
-    f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
-  } else {
-    f[0] = *p;
-  }
-}
-template <int V>
-__device__ __forceinline__ void load_run(const __nv_bfloat16* p, float (&f)[V]) {
-  if constexpr (V == 8) {
-    const uint4 x = *reinterpret_cast<const uint4*>(p);
-    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      f[2 * j] = __uint_as_float(w[j] << 16);
-      f[2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
-    }
-  } else {
-    f[0] = __bfloat162float(*p);
-  }
-}
-template <int V>
-__device__ __forceinline__ void store_run(float* p, const float (&f)[V]) {
-  if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
-  else *p = f[0];
-}
-template <int V>
-__device__ __forceinline__ void store_run(__nv_bfloat16* p, const float (&f)[V]) {
-  if constexpr (V == 8)
-    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
-                                              pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
-  else *p = __float2bfloat16_rn(f[0]);
-}
 template <int N>
 __device__ __forceinline__ void load_f32(const float* p, float (&f)[N]) {
   if constexpr (N % 4 == 0) {
@@ -108,7 +79,6 @@ __device__ __forceinline__ void load_f32(const float* p, float (&f)[N]) {
 template <int V, bool HALVES>
 struct UnitAt {
   static constexpr bool TWO = HALVES || V == 1;
-  static constexpr int N = TWO ? V : V / 2;  // angles of a unit
   int e, second, angle;
   bool on, turns;
   __device__ UnitAt(int c, int P, int D) {
@@ -122,189 +92,326 @@ struct UnitAt {
   }
 };
 
-template <int V, bool HALVES>
-__device__ __forceinline__ void turn_unit(float (&a)[V], float (&b)[V], const float* co, const float* si, float sign) {
-  constexpr int N = UnitAt<V, HALVES>::N;
-  float c[N], s[N];
-  load_f32<N>(co, c);
-  load_f32<N>(si, s);
-  if constexpr (UnitAt<V, HALVES>::TWO) {
+// The unit's values in memory, as they are, and as floats: two runs of V.
+template <typename T, int V>
+struct Raw {
+  using R = std::conditional_t<V == 1, T, uint4>;
+  R r[2];
+};
+template <typename T, int V>
+__device__ __forceinline__ void read_raw(Raw<T, V>& x, const T* p, int second, bool two) {
+  using R = typename Raw<T, V>::R;
+  x.r[0] = *reinterpret_cast<const R*>(p);
+  if (two) x.r[1] = *reinterpret_cast<const R*>(p + second);
+  else memset(&x.r[1], 0, sizeof(R));
+}
+template <int V>
+struct Unit {
+  float v[2][V];
+};
+template <typename T, int V>
+__device__ __forceinline__ Unit<V> floats_of(const Raw<T, V>& x) {
+  Unit<V> f;
 #pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const float x = a[j], y = b[j], t = sign * s[j];
-      a[j] = x * c[j] - y * t;
-      b[j] = y * c[j] + x * t;
-    }
-  } else {
+  for (int z = 0; z < 2; ++z) {
+    if constexpr (V == 1) {
+      f.v[z][0] = to_f(x.r[z]);
+    } else {
+      const uint32_t w[4] = {x.r[z].x, x.r[z].y, x.r[z].z, x.r[z].w};
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float x = a[2 * j], y = a[2 * j + 1], t = sign * s[j];
-      a[2 * j] = x * c[j] - y * t;
-      a[2 * j + 1] = y * c[j] + x * t;
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (sizeof(T) == 2) {
+          f.v[z][2 * j] = __uint_as_float(w[j] << 16);
+          f.v[z][2 * j + 1] = __uint_as_float(w[j] & 0xffff0000u);
+        } else {
+          f.v[z][j] = __uint_as_float(w[j]);
+        }
+      }
     }
   }
+  return f;
+}
+template <typename T, int V>
+__device__ __forceinline__ void write_run(T* p, const float (&f)[V]) {
+  if constexpr (V == 8)
+    *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]),
+                                              pack_bf16x2(f[4], f[5]), pack_bf16x2(f[6], f[7]));
+  else if constexpr (V == 4) *reinterpret_cast<float4*>(p) = make_float4(f[0], f[1], f[2], f[3]);
+  else if constexpr (sizeof(T) == 2) *p = __float2bfloat16_rn(f[0]);
+  else *p = f[0];
 }
 
-// T: value type; V: values of a run (16 bytes of them; 1 where the runs are no whole
-// vectors); U: units of a lane; BWD: gradients; ACC: added to what dx holds.
-// A tile is `tile` tokens; `lanes` lanes share a head, and the block's groups of lanes
-// take the tile's heads one after the other.
+// What a unit's turn multiplies by, N of each: with (a, b) a pair, a' = a ca - b sb, b' = b cb + a sa, where ca
+// and sa are the cosine and the sine times gamma of a, cb and sb times gamma of b. A unit that passes
+// through has ca = gamma alone. Kept from head to head of a token (of the backward: without gamma).
+template <int V, bool HALVES>
+struct Turn {
+  static constexpr int N = UnitAt<V, HALVES>::TWO ? V : V / 2;
+  float ca[N], cb[N], sa[N], sb[N];
+  __device__ __forceinline__ void set(const float* co, const float* si, const Unit<V>& gm, bool turns) {
+    float c[N], s[N];
+    if (turns) {
+      load_f32<N>(co, c);
+      load_f32<N>(si, s);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      if (!turns) c[j] = 1.f, s[j] = 0.f;
+      const float ga = UnitAt<V, HALVES>::TWO ? gm.v[0][j] : gm.v[0][(2 * j) % V],
+                  gb = UnitAt<V, HALVES>::TWO ? gm.v[1][j] : gm.v[0][(2 * j + 1) % V];
+      ca[j] = c[j] * ga;
+      sa[j] = s[j] * ga;
+      cb[j] = c[j] * gb;
+      sb[j] = s[j] * gb;
+    }
+  }
+  // f (times r) turned; BACK: by the negative angles
+  template <bool BACK>
+  __device__ __forceinline__ void apply(Unit<V>& f, float r) const {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      float& a = UnitAt<V, HALVES>::TWO ? f.v[0][j] : f.v[0][(2 * j) % V];
+      float& b = UnitAt<V, HALVES>::TWO ? f.v[1][j] : f.v[0][(2 * j + 1) % V];
+      const float x = a, y = b;
+      if (BACK) {
+        a = fmaf(x, ca[j], y * sa[j]);
+        b = fmaf(y, cb[j], -(x * sb[j]));
+      } else {
+        a = r * fmaf(x, ca[j], -(y * sb[j]));
+        b = r * fmaf(y, cb[j], x * sa[j]);
+      }
+    }
+  }
+};
+
+// T: value type; V: values of a run (16 bytes of them; 1 where the runs are no whole vectors); U: units of a
+// lane; BWD: gradients; ACC: added to what dx holds. Thread = (token of a tile, head slot of G, lane of a
+// head): a slot takes heads slot, slot + G, ... of q and then of k, so a thread keeps its token's angles and
+// its part of gamma from head to head. The loads of AT_ONCE heads are in flight.
 template <typename T, int V, int U, bool HALVES, bool BWD, bool ACC>
-__global__ void __launch_bounds__(kNormThreads)
+__global__ void __launch_bounds__(kNormThreads, U > 1 ? 1 : 2)
     qk_norm_rope_kernel(const __grid_constant__ NormArgs<T> g, const __grid_constant__ NormTable tab) {
   using At = UnitAt<V, HALVES>;
+  constexpr int AT_ONCE = norm_at_once(U, BWD), RUNS = At::TWO ? 2 : 1;
   extern __shared__ __align__(16) float tables[];  // 2 x (cos [tile][P], sin [tile][P])
-  const int lane = threadIdx.x & (g.lanes - 1), group = threadIdx.x / g.lanes, groups = kNormThreads / g.lanes;
+  // the parameter's table: lanes that index it differently there would be served one by one
+  __shared__ uint64_t s_turns[kNormMaxPairs];
+  __shared__ int s_axis[kNormMaxPairs];
   const int P = g.P, D = g.D;
-  const float inv_d = 1.f / D;
-  float dg[2][U][2][V];
-  if (BWD) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < V; ++j) dg[i][u][0][j] = dg[i][u][1][j] = 0.f;
+  for (int i = threadIdx.x; i < P; i += kNormThreads) {
+    s_turns[i] = tab.turns[i];
+    s_axis[i] = tab.axis[i];
   }
+  __syncthreads();
+  const int lane = threadIdx.x & (g.lanes - 1), slot = threadIdx.x / g.lanes % g.G, t = threadIdx.x / (g.lanes * g.G);
+  const float inv_d = 1.f / D;
+  const int first_ta = threadIdx.x / P, first_p = threadIdx.x - first_ta * P;
+  const int step_ta = kNormThreads / P, step_p = kNormThreads - step_ta * P;
   const long long n_tiles = (g.n_tok + g.tile - 1) / g.tile;
+  auto tokens_of = [&](long long tile) {
+    const long long left = g.n_tok - tile * g.tile;
+    return static_cast<int>(left < g.tile ? left : g.tile);
+  };
+  // The angles of a tile in two parts: the positions of a thread's are loaded before the tile before it is
+  // worked on, their cosines and sines computed after it.
+  int pos[kNormAngles];
+  auto positions = [&](long long tile) {
+    const int nt = tokens_of(tile);
+    int ta = first_ta, p = first_p;
+#pragma unroll
+    for (int k = 0; k < kNormAngles; ++k) {
+      if (ta < nt) pos[k] = g.pos[s_axis[p] * g.n_tok + tile * g.tile + ta];
+      ta += step_ta;
+      p += step_p;
+      if (p >= P) p -= P, ++ta;
+    }
+  };
+  auto angles = [&](long long tile, int half) {
+    const int nt = tokens_of(tile);
+    float* to = tables + half * 2 * g.tile * P + threadIdx.x;
+    int ta = first_ta, p = first_p;
+#pragma unroll
+    for (int k = 0; k < kNormAngles; ++k) {
+      if (ta < nt) {
+        const uint64_t turn = static_cast<uint64_t>(static_cast<int64_t>(pos[k])) * s_turns[p];
+        float sn, cs;
+        sincospif(static_cast<float>(static_cast<int32_t>(turn >> 32)) * 0x1p-31f, &sn, &cs);
+        to[k * kNormThreads] = cs;
+        to[k * kNormThreads + g.tile * P] = sn;
+      }
+      ta += step_ta;
+      p += step_p;
+      if (p >= P) p -= P, ++ta;
+    }
+  };
+
+  Unit<V> dg[2][U];
+  if (BWD) memset(dg, 0, sizeof(dg));
+  positions(blockIdx.x);
+  angles(blockIdx.x, 0);
   int parity = 0;
 #pragma unroll 1
   for (long long tile = blockIdx.x; tile < n_tiles; tile += gridDim.x, parity ^= 1) {
-    float *cosines = tables + parity * 2 * g.tile * P, *sines = cosines + g.tile * P;
-    const long long t0 = tile * g.tile;
-    const int nt = static_cast<int>(g.n_tok - t0 < g.tile ? g.n_tok - t0 : g.tile);
-    for (int i = threadIdx.x; i < nt * P; i += kNormThreads) {
-      const int ti = i / P, p = i - ti * P;
-      const double u = static_cast<double>(g.pos[tab.axis[p] * g.n_tok + t0 + ti]) * tab.turns[p];
-      float s, c;
-      sincospif(2.f * static_cast<float>(u - rint(u)), &s, &c);
-      cosines[i] = c;
-      sines[i] = s;
-    }
-    __syncthreads();
+    const float *cosines = tables + parity * 2 * g.tile * P, *sines = cosines + g.tile * P;
+    const long long tok = tile * g.tile + t;
+    const bool live = t < tokens_of(tile), more = tile + gridDim.x < n_tiles;
+    if (more) positions(tile + gridDim.x);
+    bool first = true;  // the tile's angles have not been waited for
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
       const NormSide<T>& sd = g.side[w];
       if (!sd.x) continue;
-      // all lanes of a warp take the same number of turns: the sums are over whole warps
-      const int items = nt * sd.heads, turns = (items + groups - 1) / groups;
+      const bool normed = sd.gamma != nullptr;
+      const T* src = sd.x + tok * sd.x_stride + static_cast<long long>(slot) * D;
+      const T* src_dy = BWD ? sd.dy + (tok * sd.heads + slot) * D : nullptr;
+      T* dst = sd.y ? sd.y + tok * sd.y_stride + static_cast<long long>(slot) * D : nullptr;
+      T* row = nullptr;
+      if (!BWD && w == 1 && g.slots && live) {
+        const long long s = g.slots[tok];
+        if (s >= 0 && s < g.num_slots) row = g.k_cache + (s * sd.heads + slot) * D;
+      }
+      Turn<V, HALVES> turn[U];
+      Unit<V> gm[U];
+      // (all lanes of a warp take the same number of turns: the sums are over whole warps)
 #pragma unroll 1
-      for (int k = 0; k < turns; ++k) {
-        const int i = group + k * groups;
-        const bool live = i < items;
-        const int t = live ? i / sd.heads : 0, h = live ? i - t * sd.heads : 0;
-        const long long tok = t0 + t;
-        const T* src = sd.x + tok * sd.x_stride + static_cast<long long>(h) * D;
-        float a[U][2][V], y[U][2][V];
-        float s1 = 0.f, s2 = 0.f;
+      for (int h0 = 0; h0 < sd.heads; h0 += AT_ONCE * g.G) {
+        Raw<T, V> rx[AT_ONCE][U], ry[AT_ONCE][U];
+        auto any = [&](int n) { return n == 0 || h0 + n * g.G < sd.heads; };  // in the whole block
+        auto has = [&](int n) { return live && slot + h0 + n * g.G < sd.heads; };
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const At at(lane + u * g.lanes, P, D);
+        for (int n = 0; n < AT_ONCE; ++n) {
+          if (!any(n)) continue;
 #pragma unroll
-          for (int j = 0; j < V; ++j) a[u][0][j] = a[u][1][j] = y[u][0][j] = y[u][1][j] = 0.f;
-          if (!live || !at.on) continue;
-          load_run<V>(src + at.e, a[u][0]);
-          if (At::TWO && at.turns) load_run<V>(src + at.e + at.second, a[u][1]);
-          if (BWD) {
-            const T* dy = sd.dy + (tok * sd.heads + h) * D;
-            load_run<V>(dy + at.e, y[u][0]);
-            if (At::TWO && at.turns) load_run<V>(dy + at.e + at.second, y[u][1]);
+          for (int u = 0; u < U; ++u) {
+            const At at(lane + u * g.lanes, P, D);
+            if (has(n) && at.on) {
+              const int off = (h0 + n * g.G) * D + at.e;
+              read_raw<T, V>(rx[n][u], src + off, at.second, At::TWO && at.turns);
+              if (BWD) read_raw<T, V>(ry[n][u], src_dy + off, at.second, At::TWO && at.turns);
+            } else {
+              memset(&rx[n][u], 0, sizeof(rx[n][u]));
+              if (BWD) memset(&ry[n][u], 0, sizeof(ry[n][u]));
+            }
           }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const At at(lane + u * g.lanes, P, D);
-          if (BWD && live && at.on && at.turns)
-            turn_unit<V, HALVES>(y[u][0], y[u][1], cosines + t * P + at.angle, sines + t * P + at.angle, -1.f);
-#pragma unroll
-          for (int j = 0; j < V; ++j) s1 += a[u][0][j] * a[u][0][j] + a[u][1][j] * a[u][1][j];
-        }
-        float r = 1.f;
-        if (sd.gamma) {
-          float gm[U][2][V];
+        if (h0 == 0) {
+          if (first) __syncthreads();  // the angles are there
+          first = false;
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const At at(lane + u * g.lanes, P, D);
 #pragma unroll
-            for (int j = 0; j < V; ++j) gm[u][0][j] = gm[u][1][j] = 0.f;
-            if (!at.on) continue;
-            load_f32<V>(sd.gamma + at.e, gm[u][0]);
-            if (At::TWO && at.turns) load_f32<V>(sd.gamma + at.e + at.second, gm[u][1]);
-            if (BWD) {
-#pragma unroll
-              for (int z = 0; z < 2; ++z)
-#pragma unroll
-                for (int j = 0; j < V; ++j) s2 += y[u][z][j] * gm[u][z][j] * a[u][z][j];
-            }
-          }
-          for (int m = g.lanes / 2; m > 0; m >>= 1) {
-            s1 += __shfl_xor_sync(0xffffffffu, s1, m);
-            if (BWD) s2 += __shfl_xor_sync(0xffffffffu, s2, m);
-          }
-          r = rsqrtf(s1 * inv_d + g.eps);
-          const float back = r * r * s2 * inv_d;
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
             for (int z = 0; z < 2; ++z)
 #pragma unroll
-              for (int j = 0; j < V; ++j) {
-                if (BWD) {
-                  if (live) dg[w][u][z][j] += y[u][z][j] * (a[u][z][j] * r);
-                  a[u][z][j] = r * (y[u][z][j] * gm[u][z][j] - a[u][z][j] * back);
-                } else {
-                  a[u][z][j] = a[u][z][j] * r * gm[u][z][j];
-                }
-              }
-        } else if (BWD) {
-#pragma unroll
-          for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < V; ++j) a[u][0][j] = y[u][0][j], a[u][1][j] = y[u][1][j];
-        }
-        if (!live) continue;
-        T* dst = sd.y ? sd.y + tok * sd.y_stride + static_cast<long long>(h) * D : nullptr;
-        T* row = nullptr;
-        if (!BWD && w == 1 && g.slots) {
-          const long long slot = g.slots[tok];
-          if (slot >= 0 && slot < g.num_slots) row = g.k_cache + (slot * sd.heads + h) * D;
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const At at(lane + u * g.lanes, P, D);
-          if (!at.on) continue;
-          if (!BWD && at.turns)
-            turn_unit<V, HALVES>(a[u][0], a[u][1], cosines + t * P + at.angle, sines + t * P + at.angle, 1.f);
-#pragma unroll
-          for (int z = 0; z < 2; ++z) {
-            if (z == 1 && !(At::TWO && at.turns)) continue;
-            const int e = at.e + z * at.second;
-            if (ACC) {
-              float old[V];
-              load_run<V>(dst + e, old);
-#pragma unroll
-              for (int j = 0; j < V; ++j) a[u][z][j] += old[j];
+              for (int j = 0; j < V; ++j) gm[u].v[z][j] = z == 0 || (At::TWO && at.turns) ? 1.f : 0.f;
+            if (normed && at.on) {
+              load_f32<V>(sd.gamma + at.e, gm[u].v[0]);
+              if (At::TWO && at.turns) load_f32<V>(sd.gamma + at.e + at.second, gm[u].v[1]);
             }
-            if (dst) store_run<V>(dst + e, a[u][z]);
-            if (row) store_run<V>(row + e, a[u][z]);
+            Unit<V> one;
+#pragma unroll
+            for (int j = 0; j < V; ++j) one.v[0][j] = one.v[1][j] = 1.f;
+            const int angle = live && at.on && at.turns ? t * P + at.angle : 0;
+            turn[u].set(cosines + angle, sines + angle, BWD ? one : gm[u], at.on && at.turns);
+          }
+        }
+        // A unit's values are unpacked for the sums, and again for the results: packed they take half the
+        // registers, and twice the heads are in flight.
+        float s1[AT_ONCE], s2[AT_ONCE];
+        if (normed) {
+#pragma unroll
+          for (int n = 0; n < AT_ONCE; ++n) {
+            if (!any(n)) continue;
+            s1[n] = s2[n] = 0.f;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              const Unit<V> x = floats_of<T, V>(rx[n][u]);
+              Unit<V> y;
+              if (BWD) {
+                y = floats_of<T, V>(ry[n][u]);
+                turn[u].template apply<true>(y, 1.f);
+              }
+#pragma unroll
+              for (int z = 0; z < RUNS; ++z)
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                  s1[n] = fmaf(x.v[z][j], x.v[z][j], s1[n]);
+                  if (BWD) s2[n] = fmaf(y.v[z][j] * gm[u].v[z][j], x.v[z][j], s2[n]);
+                }
+            }
+          }
+          for (int m = g.lanes / 2; m > 0; m >>= 1)
+#pragma unroll
+            for (int n = 0; n < AT_ONCE; ++n) {
+              if (!any(n)) continue;
+              s1[n] += __shfl_xor_sync(0xffffffffu, s1[n], m);
+              if (BWD) s2[n] += __shfl_xor_sync(0xffffffffu, s2[n], m);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+          if (!any(n) || !has(n)) continue;
+          const float r = normed ? rsqrtf(s1[n] * inv_d + g.eps) : 1.f, back = BWD && normed ? r * r * s2[n] * inv_d : 0.f;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const At at(lane + u * g.lanes, P, D);
+            if (!at.on) continue;
+            const int off = (h0 + n * g.G) * D + at.e;
+            Unit<V> x;
+            if (!BWD || normed) x = floats_of<T, V>(rx[n][u]);
+            if (BWD) {
+              Unit<V> y = floats_of<T, V>(ry[n][u]);
+              turn[u].template apply<true>(y, 1.f);
+              if (normed) {
+#pragma unroll
+                for (int z = 0; z < RUNS; ++z)
+#pragma unroll
+                  for (int j = 0; j < V; ++j) {
+                    const float f = x.v[z][j];
+                    dg[w][u].v[z][j] = fmaf(y.v[z][j] * f, r, dg[w][u].v[z][j]);
+                    x.v[z][j] = r * fmaf(f, -back, y.v[z][j] * gm[u].v[z][j]);
+                  }
+              } else {
+                x = y;
+              }
+            } else {
+              turn[u].template apply<false>(x, r);
+            }
+            if (ACC) {
+              Raw<T, V> old;
+              read_raw<T, V>(old, dst + off, at.second, At::TWO && at.turns);
+              const Unit<V> f = floats_of<T, V>(old);
+#pragma unroll
+              for (int z = 0; z < RUNS; ++z)
+#pragma unroll
+                for (int j = 0; j < V; ++j) x.v[z][j] += f.v[z][j];
+            }
+#pragma unroll
+            for (int z = 0; z < RUNS; ++z) {
+              if (z == 1 && !at.turns) continue;
+              if (dst) write_run<T, V>(dst + off + z * at.second, x.v[z]);
+              if (row) write_run<T, V>(row + off + z * at.second, x.v[z]);
+            }
           }
         }
       }
     }
     if (!BWD && g.slots) {  // v as it is, 16 bytes at a time
       constexpr int W = 16 / sizeof(T);
-      const int per = g.side[1].heads * D / W;
+      const int per = g.side[1].heads * D / W, nt = tokens_of(tile);
       for (int i = threadIdx.x; i < nt * per; i += kNormThreads) {
-        const int t = i / per, e = (i - t * per) * W;
-        const long long slot = g.slots[t0 + t];
-        if (slot >= 0 && slot < g.num_slots)
-          *reinterpret_cast<uint4*>(g.v_cache + slot * g.side[1].heads * D + e) =
-              *reinterpret_cast<const uint4*>(g.v + (t0 + t) * g.v_stride + e);
+        const int tv = i / per, e = (i - tv * per) * W;
+        const long long s = g.slots[tile * g.tile + tv];
+        if (s >= 0 && s < g.num_slots)
+          *reinterpret_cast<uint4*>(g.v_cache + s * g.side[1].heads * D + e) =
+              *reinterpret_cast<const uint4*>(g.v + (tile * g.tile + tv) * g.v_stride + e);
       }
     }
+    if (more) angles(tile + gridDim.x, parity ^ 1);
   }
   if (BWD) {
-    // this block's sums of dgamma: the groups' one after the other
+    // this block's sums of dgamma: the threads' that share a lane, one after the other
+    const int groups = kNormThreads / g.lanes, group = threadIdx.x / g.lanes;
     __syncthreads();
     float* sums = tables;  // [groups][D]
 #pragma unroll
@@ -314,9 +421,10 @@ __global__ void __launch_bounds__(kNormThreads)
         const At at(lane + u * g.lanes, P, D);
         if (!at.on) continue;
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-          sums[group * D + at.e + j] = dg[w][u][0][j];
-          if (At::TWO && at.turns) sums[group * D + at.e + at.second + j] = dg[w][u][1][j];
+        for (int z = 0; z < RUNS; ++z) {
+          if (z == 1 && !at.turns) continue;
+#pragma unroll
+          for (int j = 0; j < V; ++j) sums[group * D + at.e + z * at.second + j] = dg[w][u].v[z][j];
         }
       }
       __syncthreads();
@@ -351,12 +459,13 @@ __global__ void __launch_bounds__(1024)
   }
 }
 
-int norm_blocks() { return 4 * device_sm_count(); }
+// Blocks of a call at most: of the backward as many as there are sums of dgamma.
+int norm_blocks(bool bwd) { return (bwd ? 2 : 16) * device_sm_count(); }
 
 struct NormPlan {
-  int V, U, lanes, tile;
+  int V, U, lanes, tile, G;
   unsigned grid;
-  size_t smem;
+  int smem;
 };
 
 NormPlan norm_plan(const RopeShape& r, bool bwd) {
@@ -367,47 +476,59 @@ NormPlan norm_plan(const RopeShape& r, bool bwd) {
   const int units = (r.halves ? r.pairs : 2 * r.pairs) / run + (r.D - 2 * r.pairs) / p.V;
   p.lanes = 1;
   while (p.lanes < units && p.lanes < 32) p.lanes *= 2;
-  p.U = (units + p.lanes - 1) / p.lanes;
-  const int groups = kNormThreads / p.lanes, heads = r.Hq + r.Hk;
-  const long long n_tok = static_cast<long long>(r.B) * r.L;
-  // a few heads a group and tile; with few tokens one token a block, so that more blocks share them
-  p.tile = (4 * groups + heads - 1) / heads;
-  const long long spread = n_tok / device_sm_count();
+  p.U = p.V == 1 ? 8 : (units + p.lanes - 1) / p.lanes;  // V == 1: at most 255 units of 32 lanes
+  // Head slots so that a thread has two turns of q's heads, and no more than there are heads of k; the rest of
+  // the block for tokens; with few tokens one token a block, so that more blocks share them. 8 x 4096 tokens of
+  // 16 + 2 heads of 128 in bf16: one turn 90 us, two 78; 16 + 16 heads 117 and 111, of 64 64 and 62.
+  const int fit = kNormThreads / p.lanes, at_once = norm_at_once(p.U, bwd);
+  p.G = (r.Hq + 2 * at_once - 1) / (2 * at_once);
+  if (r.Hk > 0 && p.G > r.Hk) p.G = r.Hk;
+  if (p.G > fit) p.G = fit;
+  p.tile = fit / p.G;
+  const long long n_tok = static_cast<long long>(r.B) * r.L, spread = n_tok / device_sm_count();
   if (p.tile > spread) p.tile = spread < 1 ? 1 : static_cast<int>(spread);
-  if (p.tile > 16) p.tile = 16;  // 2 x 2 x 16 x 128 fp32 of angles at most: 32 KB
-  const long long tiles = (n_tok + p.tile - 1) / p.tile;
-  p.grid = static_cast<unsigned>(tiles < norm_blocks() ? tiles : norm_blocks());
-  p.smem = 4 * static_cast<size_t>(p.tile) * r.pairs * sizeof(float);
-  const size_t sums = static_cast<size_t>(groups) * r.D * sizeof(float);  // <= 32 KB (groups * D <= 8192)
+  if (p.tile > kNormAngles * kNormThreads / r.pairs) p.tile = kNormAngles * kNormThreads / r.pairs;
+  if (p.tile == 1) {  // the block is one token's
+    p.G = r.Hq > r.Hk ? r.Hq : r.Hk;
+    if (p.G > fit) p.G = fit;
+  }
+  const long long tiles = (n_tok + p.tile - 1) / p.tile, blocks = norm_blocks(bwd);
+  p.grid = static_cast<unsigned>(tiles < blocks ? tiles : blocks);
+  p.smem = 4 * p.tile * r.pairs * 4;
+  const int sums = fit * r.D * 4;  // <= 32 KB: a lane has 8 U values of a head at most
   if (bwd && sums > p.smem) p.smem = sums;
   return p;
 }
 
 NormTable norm_table(const RopeShape& r) {
   NormTable tab;
-  const double turn = 1.0 / 6.283185307179586476925286766559, log2_base = std::log2(r.base);
+  const long double turn = 1.0L / 6.28318530717958647692528676655900577L;
   int i = 0;
   for (int a = 0; a < r.axes; ++a)
     for (int j = 0; j < r.sections[a]; ++j, ++i) {
-      const double f = r.per_axis ? static_cast<double>(j) / r.sections[a] : static_cast<double>(i) / r.pairs;
-      tab.turns[i] = turn * std::exp2(-f * log2_base);
+      const long double f = r.per_axis ? static_cast<long double>(j) / r.sections[a] : static_cast<long double>(i) / r.pairs;
+      tab.turns[i] = static_cast<uint64_t>(turn * std::pow(static_cast<long double>(r.base), -f) * 0x1p64L + 0.5L);
       tab.axis[i] = static_cast<uint8_t>(a);
     }
   return tab;
 }
 
+template <typename T, int V, int U, bool HALVES, bool BWD, bool ACC>
+int norm_go(const NormPlan& p, const NormArgs<T>& g, const NormTable& tab, cudaStream_t s) {
+  qk_norm_rope_kernel<T, V, U, HALVES, BWD, ACC><<<p.grid, kNormThreads, p.smem, s>>>(g, tab);
+  return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
 template <typename T, int V, int U, bool HALVES>
-void norm_go(const NormPlan& p, const NormArgs<T>& g, const NormTable& tab, bool bwd, bool acc, cudaStream_t s) {
-  if (!bwd) qk_norm_rope_kernel<T, V, U, HALVES, false, false><<<p.grid, kNormThreads, p.smem, s>>>(g, tab);
-  else if (!acc) qk_norm_rope_kernel<T, V, U, HALVES, true, false><<<p.grid, kNormThreads, p.smem, s>>>(g, tab);
-  else qk_norm_rope_kernel<T, V, U, HALVES, true, true><<<p.grid, kNormThreads, p.smem, s>>>(g, tab);
+int norm_go(const NormPlan& p, const NormArgs<T>& g, const NormTable& tab, bool bwd, bool acc, cudaStream_t s) {
+  if (!bwd) return norm_go<T, V, U, HALVES, false, false>(p, g, tab, s);
+  return acc ? norm_go<T, V, U, HALVES, true, true>(p, g, tab, s) : norm_go<T, V, U, HALVES, true, false>(p, g, tab, s);
 }
 
 template <typename T, int V, int U>
-void norm_go(const NormPlan& p, const NormArgs<T>& g, const NormTable& tab, bool halves, bool bwd, bool acc,
-             cudaStream_t s) {
-  if (halves) norm_go<T, V, U, true>(p, g, tab, bwd, acc, s);
-  else norm_go<T, V, U, false>(p, g, tab, bwd, acc, s);
+int norm_go(const NormPlan& p, const NormArgs<T>& g, const NormTable& tab, bool halves, bool bwd, bool acc,
+            cudaStream_t s) {
+  return halves ? norm_go<T, V, U, true>(p, g, tab, bwd, acc, s) : norm_go<T, V, U, false>(p, g, tab, bwd, acc, s);
 }
 
 template <typename T>
@@ -419,12 +540,12 @@ int norm_launch(const NormRope& sh, const NormPlan& p, NormArgs<T>& g, bool bwd,
   g.D = r.D;
   g.lanes = p.lanes;
   g.tile = p.tile;
+  g.G = p.G;
   g.eps = sh.eps;
   const NormTable tab = norm_table(r);
-  if (p.V == 1) norm_go<T, 1, 8>(p, g, tab, r.halves, bwd, acc, s);  // at most 255 units of 32 lanes
-  else if (p.U == 1) norm_go<T, V, 1>(p, g, tab, r.halves, bwd, acc, s);
-  else norm_go<T, V, 2>(p, g, tab, r.halves, bwd, acc, s);
-  return cudaGetLastError() == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+  if (p.V == 1) return norm_go<T, 1, 8>(p, g, tab, r.halves, bwd, acc, s);
+  if (p.U == 1) return norm_go<T, V, 1>(p, g, tab, r.halves, bwd, acc, s);
+  return norm_go<T, V, 2>(p, g, tab, r.halves, bwd, acc, s);
 }
 
 template <typename T>
@@ -475,7 +596,7 @@ int launch_qk_norm_rope_fwd(const NormRope& sh, const void* q, const void* k, co
 }
 
 size_t qk_norm_rope_bwd_workspace_bytes(const NormRope& sh) {
-  return static_cast<size_t>(norm_blocks()) * 2 * sh.rope.D * sizeof(float);
+  return static_cast<size_t>(norm_blocks(true)) * 2 * sh.rope.D * sizeof(float);
 }
 
 int launch_qk_norm_rope_bwd(const NormRope& sh, const void* dqo, const void* dko, const void* q,
