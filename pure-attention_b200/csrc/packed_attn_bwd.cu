@@ -17,6 +17,7 @@
 //                        the diagonal on for each head of the group; rows are keys
 // Both keep P and dS in TMEM as the A operand of the products that use them.
 #include <cuda_bf16.h>
+#include <type_traits>
 #include "packed_common.cuh"
 
 namespace pa {
@@ -39,29 +40,43 @@ __device__ __forceinline__ size_t stat_row(const PackedUnit& u, int tile) {
 __device__ __forceinline__ uint32_t step_col(int k) { return k < 4 ? k * 8 : 64 + (k - 4) * 8; }
 
 // ---------------------------------------------------------------- statistics
+constexpr int kStatBlocks = 3;  // per SM; a thread has its piece of 4 or 8 rows of o and dO in flight
 template <int D>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, kStatBlocks)
     packed_stats_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O, const float* __restrict__ lse,
                         const PackedList* __restrict__ list, int T, int H, long long rows, float* __restrict__ lse2,
                         float* __restrict__ delta) {
   constexpr int LANES = D / 8, STEP = 256 / LANES;  // lanes that share a row; rows of a pass
   launch_dependents();
   wait_prerequisites();
-  const long long n = static_cast<long long>(list->count) * H;
-  const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
-  for (long long i = blockIdx.x; i < n; i += gridDim.x) {
-    const PackedUnit u = packed_unit(list, static_cast<int>(i / H));
-    const int h = static_cast<int>(i % H), tile = u.work - 1;
-    const size_t out = h * static_cast<size_t>(rows) + stat_row(u, tile);
+  // item = (unit, head), stepped through without divisions
+  const int count = list->count, lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+  const int du = static_cast<int>(gridDim.x) / H, dh = static_cast<int>(gridDim.x) % H;
+  int at_unit = static_cast<int>(blockIdx.x) / H, h = static_cast<int>(blockIdx.x) % H;
+  auto unit_of = [&](int i) { return i < count ? packed_unit(list, i) : PackedUnit{0, 0, 0, 0}; };
+  PackedUnit next = unit_of(at_unit);
+  while (next.work) {
+    const PackedUnit u = next;
+    const int tile = u.work - 1, head = h;
+    at_unit += du;
+    h += dh;
+    if (h >= H) {
+      h -= H;
+      ++at_unit;
+    }
+    next = unit_of(at_unit);
+    const size_t out = head * static_cast<size_t>(rows) + stat_row(u, tile);
     uint4 a[128 / STEP], b[128 / STEP];
+    float l[128 / STEP];
 #pragma unroll
     for (int k = 0; k < 128 / STEP; ++k) {
       const int row = tile * 128 + r0 + k * STEP;
       if (row < u.len) {
-        const size_t at = ((static_cast<size_t>(u.start) + row) * H + h) * D + lane * 8;
+        const size_t at = ((static_cast<size_t>(u.start) + row) * H + head) * D + lane * 8;
         a[k] = *reinterpret_cast<const uint4*>(dO + at);
         b[k] = *reinterpret_cast<const uint4*>(O + at);
       }
+      l[k] = row < u.len ? lse[static_cast<size_t>(head) * T + u.start + row] * kLog2e : INFINITY;
     }
 #pragma unroll
     for (int k = 0; k < 128 / STEP; ++k) {
@@ -81,11 +96,68 @@ __global__ void __launch_bounds__(256)
       if (lane == 0) {
         const int at = r0 + k * STEP;
         delta[out + at] = s;
-        lse2[out + at] =
-            row < u.len ? lse[static_cast<size_t>(h) * T + u.start + row] * kLog2e : INFINITY;
+        lse2[out + at] = l[k];
       }
     }
   }
+}
+
+// 32 values of a row, scaled: to[i] (=|+=) o[i] * mul.
+__device__ __forceinline__ void write_row(bf16* to, const uint32_t (&o)[32], float mul, int accumulate) {
+  uint4* d4 = reinterpret_cast<uint4*>(to);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float f[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * mul;
+    if (accumulate) {
+      const uint4 old = d4[i];
+      const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float2 pf = __bfloat1622float2(p2[e]);
+        f[2 * e] += pf.x;
+        f[2 * e + 1] += pf.y;
+      }
+    }
+    d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                       pack_bf16x2(f[6], f[7]));
+  }
+}
+
+// Who computes P and dS: warps 0 to 2 load, issue and clear ragged rows; from warp 4 on, pairs of
+// warpgroups compute, a thread half a row of a tile. At 64 head dimensions the products of a tile are short, and
+// two pairs take the tiles in turn, so that one's exponentials run beside the other's dS (sequences of up to 4096
+// tokens, 12800 in all, 16 heads: dq 169 to 153 us, dk and dv 235 to 178 us). They need more than the
+// 96 registers that 640 threads leave each, and the first four warps give theirs. At 128 the products take longer
+// than the exponentials and TMEM has no room for another tile in flight: there one pair with 168
+// registers a thread is faster (8192 tokens, 16 + 4 heads: dq 299 us, two pairs 330; dk and dv 463 us, 479).
+template <int D>
+struct BwdWarps {
+  static constexpr int PAIRS = D == 64 ? 2 : 1;
+  static constexpr int ROLES = 4, PAIR = 256, THREADS = ROLES * 32 + PAIRS * PAIR;
+  static constexpr int CHUNK = PAIRS == 2 ? 16 : 32;  // columns of dP that a thread holds at a time
+  static constexpr int FEW = 64, MANY = 104;
+  static_assert(FEW * 128 + MANY * 512 <= 640 * 96, "an increase would wait forever");
+  static __device__ __forceinline__ void roles_regs() {
+    if constexpr (PAIRS == 2) regs_dec<FEW>();
+  }
+  static __device__ __forceinline__ void pairs_regs() {
+    if constexpr (PAIRS == 2) regs_inc<MANY>();
+  }
+  // The first tile of `pair` from tile g on.
+  static __device__ __forceinline__ int first(int g, int pair) { return PAIRS == 2 ? g + ((g ^ pair) & 1) : g; }
+};
+
+template <int N>
+__device__ __forceinline__ void load_columns(uint32_t at, uint32_t (&v)[N]) {
+  if constexpr (N == 32) tmem_ld32_sync(at, v);
+  else tmem_ld16_sync(at, v);
+}
+template <int N>
+__device__ __forceinline__ void store_columns(uint32_t at, const uint32_t (&v)[N]) {
+  if constexpr (N == 16) tmem_st16(at, v);
+  else PA_TMEM_ST_X8(at, v);
 }
 
 // What the kernels' issuer knows of a tile of the stream it works through.
@@ -105,20 +177,20 @@ struct PackedDq {
   static constexpr int QBUF = D == 64 ? 2 : 1;  // Q and dO of an item
   static constexpr int KST = D == 64 ? 4 : 3, VST = D == 64 ? 4 : 2;
   static constexpr int SMEM = (QBUF * 2 + KST + VST) * TILE + 1024;
-  static constexpr int THREADS = 384;
   static constexpr uint32_t T_S = 0, T_DP = 256, T_DQ = 384;
 };
 
 template <int D>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                      const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
                      bf16* __restrict__ dq, long long dq_stride, const float* __restrict__ lse2,
                      const float* __restrict__ delta, const PackedList* __restrict__ list, int H, int group,
                      long long rows, float scale, float scale_log2, int accumulate, uint32_t* status) {
   using C = PackedDq<D>;
+  using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[32];
+  __shared__ uint64_t bars[34];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   launch_dependents();
@@ -136,13 +208,15 @@ __global__ void __launch_bounds__(384, 1)
   auto k_empty = [&](int s) { return smem_u32(&bars[8 + s]); };
   auto v_full = [&](int s) { return smem_u32(&bars[12 + s]); };
   auto v_empty = [&](int s) { return smem_u32(&bars[16 + s]); };
-  // By tile parity where the arriving side can be a tile ahead of the waiting one.
+  // By tile parity: each pair waits for its own tiles only, and an arriving side can be a tile ahead.
   auto s_full = [&](int g) { return smem_u32(&bars[20 + (g & 1)]); };
   auto ds_full = [&](int g) { return smem_u32(&bars[22 + (g & 1)]); };
-  const uint32_t dp_full = smem_u32(&bars[24]), dp_free = smem_u32(&bars[25]), dq_done = smem_u32(&bars[26]);
-  // the f-th ragged K tile has landed, and its rows behind the end are zero
-  auto k_ragged = [&](int f) { return smem_u32(&bars[27 + (f & 1)]); };
-  auto k_zeroed = [&](int f) { return smem_u32(&bars[29 + (f & 1)]); };
+  auto dp_full = [&](int g) { return smem_u32(&bars[24 + (g & 1)]); };
+  auto dp_free = [&](int g) { return smem_u32(&bars[26 + (g & 1)]); };
+  const uint32_t acc_done = smem_u32(&bars[28]), acc_free = smem_u32(&bars[29]);  // an item's dq is there; was read
+  // the f-th ragged K tile has landed, and its rows behind the end are zero; two are on the way at most
+  auto k_ragged = [&](int f) { return smem_u32(&bars[30 + (f & 1)]); };
+  auto k_zeroed = [&](int f) { return smem_u32(&bars[32 + (f & 1)]); };
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -150,7 +224,9 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(q_full(u), 1);
       mbar_init(q_empty(u), 1);
       mbar_init(s_full(u), 1);
-      mbar_init(ds_full(u), 256);
+      mbar_init(ds_full(u), W::PAIR);
+      mbar_init(dp_full(u), 1);
+      mbar_init(dp_free(u), W::PAIR);
       mbar_init(k_ragged(u), 1);
       mbar_init(k_zeroed(u), 1);
     }
@@ -160,9 +236,8 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(v_full(s), 1);
       mbar_init(v_empty(s), 1);
     }
-    mbar_init(dp_full, 1);
-    mbar_init(dp_free, 256);
-    mbar_init(dq_done, 1);
+    mbar_init(acc_done, 1);
+    mbar_init(acc_free, W::PAIR);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -180,6 +255,7 @@ __global__ void __launch_bounds__(384, 1)
     return i < n_items ? packed_unit(list, static_cast<int>(i / H)) : PackedUnit{0, 0, 0, 0};
   };
   auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % H); };
+  if (warp < W::ROLES) W::roles_regs();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -267,7 +343,7 @@ __global__ void __launch_bounds__(384, 1)
         tc_fence_after();
         product(tmem + C::T_DP, dQ0 + ((((t.it % C::QBUF) * 2 + 1) * C::TILE) >> 4),
                 dV0 + (((g % C::VST) * C::TILE) >> 4));
-        umma_commit(dp_full);
+        umma_commit(dp_full(g));
         umma_commit(v_empty(g % C::VST));
         if (t.last) umma_commit(q_empty(t.it % C::QBUF));  // (its last S was issued before)
         return true;
@@ -275,19 +351,21 @@ __global__ void __launch_bounds__(384, 1)
       StreamTile a = next_tile(), b = next_tile();
       if (a.valid) ok = issue_S(a, 0) && issue_dP(a, 0) && (!b.valid || issue_S(b, 1));
       for (int g = 0; ok && a.valid; ++g) {
-        if (b.valid && !(ok = mbar_wait(dp_free, g & 1, status) && issue_dP(b, g + 1))) break;
+        if (b.valid && !(ok = mbar_wait(dp_free(g), (g >> 1) & 1, status) && issue_dP(b, g + 1))) break;
         if (!(ok = mbar_wait(ds_full(g), (g >> 1) & 1, status))) break;
         if (a.ragged) {
           if (!(ok = mbar_wait(k_zeroed(rz), (rz >> 1) & 1, status))) break;
           ++rz;
         }
+        // dq restarts from zero: the item before has been read
+        if (a.first && a.it > 0 && !(ok = mbar_wait(acc_free, (a.it - 1) & 1, status))) break;
         tc_fence_after();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
           umma_f16_ts(tmem + C::T_DQ, tmem + C::T_S + (g & 1) * 128 + step_col(k),
                       dK_MN + (((g % C::KST) * C::TILE + k * 2048) >> 4), idQ, (!a.first || k > 0) ? 1u : 0u);
         umma_commit(k_empty(g % C::KST));
-        if (a.last) umma_commit(dq_done);
+        if (a.last) umma_commit(acc_done);
         const StreamTile c = next_tile();
         if (c.valid && !(ok = issue_S(c, g + 2))) break;
         a = b;
@@ -308,13 +386,14 @@ __global__ void __launch_bounds__(384, 1)
       if (lane_id() == 0) mbar_arrive(k_zeroed(f));
       ++f;
     }
-  } else if (warp >= 4) {
+  } else if (warp >= W::ROLES) {
     // ------------------------------------------------------------ P and dS
-    // Warpgroup grp: keys [64 grp, 64 grp + 64) of each tile; thread = query row.
-    const int grp = (warp - 4) >> 2;
+    // A pair takes every other tile, its warpgroup `half` the keys [64 half, 64 half + 64); thread = query row.
+    W::pairs_regs();
+    const int pair = (warp - W::ROLES) >> 3, half = ((warp - W::ROLES) >> 2) & 1;
     const int r = ((warp & 3) << 5) + static_cast<int>(lane_id());
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tdP = tmem + C::T_DP + lane_base + grp * 64;
+    const uint32_t tdP = tmem + C::T_DP + lane_base + half * 64;
     bool ok = true;
     PackedUnit next = unit_of(0);
     auto stats = [&](const PackedUnit& u, int turn) {
@@ -323,85 +402,70 @@ __global__ void __launch_bounds__(384, 1)
       return make_float2(lse2[at], delta[at]);
     };
     float2 st_next = stats(next, 0);
-    int g = 0;
+    int g0 = 0;  // the item's first tile
     for (int it = 0; ok && next.work; ++it) {
       const PackedUnit u = next;
       const float neg_lse = -st_next.x, del = st_next.y;
       next = unit_of(it + 1);
       st_next = stats(next, it + 1);
-      for (int j = 0; j < u.work; ++j, ++g) {
-        const uint32_t tS = tmem + C::T_S + (g & 1) * 128 + lane_base + grp * 64;
+      const int last = g0 + u.work - 1;
+      for (int g = W::first(g0, pair); g <= last; g += W::PAIRS) {
+        const uint32_t tS = tmem + C::T_S + (g & 1) * 128 + lane_base + half * 64;
         if (!(ok = mbar_wait_warp(s_full(g), (g >> 1) & 1, status))) break;
         tc_fence_after();
         float p[64];
-        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
-        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
-        tmem_ld_wait();
+        tmem_ld32_sync(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld32_sync(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
 #pragma unroll
         for (int i = 0; i < 64; ++i) p[i] = ex2(fmaf(p[i], scale_log2, neg_lse));
-        if (!(ok = mbar_wait_warp(dp_full, g & 1, status))) break;
+        if (!(ok = mbar_wait_warp(dp_full(g), (g >> 1) & 1, status))) break;
         tc_fence_after();
-        uint32_t ds[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
-          tmem_ld32_sync(tdP + c * 32, v);
-          if (c == 1) {
+        for (int c = 0; c < 64 / W::CHUNK; ++c) {
+          constexpr int N = W::CHUNK;
+          uint32_t v[N], ds[N / 2];
+          load_columns(tdP + c * N, v);
+          if (c == 64 / N - 1) {
             tc_fence_before();
-            mbar_arrive(dp_free);  // the next dP may overwrite it
+            mbar_arrive(dp_free(g));  // the next dP may overwrite it
           }
-          if (j == u.work - 1) {  // the block on the diagonal
+          if (g == last) {  // the block on the diagonal
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const float x = p[c * 32 + i] * (__uint_as_float(v[i]) - del);
-              v[i] = __float_as_uint(grp * 64 + c * 32 + i > r ? 0.f : x);
+            for (int i = 0; i < N; ++i) {
+              const float x = p[c * N + i] * (__uint_as_float(v[i]) - del);
+              v[i] = __float_as_uint(half * 64 + c * N + i > r ? 0.f : x);
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              v[i] = __float_as_uint(p[c * 32 + i] * (__uint_as_float(v[i]) - del));
+            for (int i = 0; i < N; ++i)
+              v[i] = __float_as_uint(p[c * N + i] * (__uint_as_float(v[i]) - del));
           }
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            ds[c * 16 + i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          for (int i = 0; i < N / 2; ++i)
+            ds[i] = pack_bf16x2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1]));
+          store_columns(tS + c * (N / 2), ds);
         }
-        tmem_st32(tS, ds);
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(ds_full(g));
       }
-      if (!ok || !(ok = mbar_wait_warp(dq_done, it & 1, status))) break;
-      // dq write-back: each warpgroup half of the columns. The loads complete before
-      // this thread's next ds_full, which the next item's first product into dq waits for.
+      if (!ok) break;
+      g0 = last + 1;
+      if (W::PAIRS == 2 && (last & 1) != pair) continue;
+      // dq write-back by the pair of the last tile, each warpgroup half of the columns, while
+      // the other pair begins the next item
+      if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
       tc_fence_after();
       const int row = (u.work - 1) * 128 + r;
       bf16* dst = dq + (static_cast<size_t>(u.start) + row) * dq_stride + static_cast<size_t>(head_of(it)) * D;
 #pragma unroll 1
-      for (int c = grp * (D / 64); c < (grp + 1) * (D / 64); ++c) {
+      for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
         uint32_t o[32];
         tmem_ld32_sync(tmem + C::T_DQ + lane_base + c * 32, o);
-        if (row < u.len) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * scale;
-            if (accumulate) {
-              const uint4 old = d4[i];
-              const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 pf = __bfloat1622float2(p2[e]);
-                f[2 * e] += pf.x;
-                f[2 * e + 1] += pf.y;
-              }
-            }
-            d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                               pack_bf16x2(f[6], f[7]));
-          }
-        }
+        if (row < u.len) write_row(dst + c * 32, o, scale, accumulate);
       }
+      tc_fence_before();
+      mbar_arrive(acc_free);
     }
   }
 
@@ -425,12 +489,11 @@ struct PackedDkv {
   static constexpr int KVBUF = D == 64 ? 2 : 1;  // K and V of an item
   static constexpr int QST = D == 64 ? 4 : 2, OST = D == 64 ? 3 : 2;
   static constexpr int SMEM = (KVBUF * 2 + QST + OST) * TILE + QST * 1024 + 1024;
-  static constexpr int THREADS = 384;
   static constexpr uint32_t T_S = 0, T_DP = 128 * SBUF, T_DV = T_DP + 128, T_DK = T_DV + D;
 };
 
 template <int D>
-__global__ void __launch_bounds__(384, 1)
+__global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     packed_dkv_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                       const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
                       bf16* __restrict__ dk, bf16* __restrict__ dv, long long dk_stride, long long dv_stride,
@@ -438,6 +501,7 @@ __global__ void __launch_bounds__(384, 1)
                       const PackedList* __restrict__ list, int Hk, int group, long long rows, float scale,
                       float scale_log2, int accumulate, uint32_t* status) {
   using C = PackedDkv<D>;
+  using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[32];
   __shared__ uint32_t tmem_slot;
@@ -458,10 +522,12 @@ __global__ void __launch_bounds__(384, 1)
   auto o_full = [&](int s) { return smem_u32(&bars[12 + s]); };
   auto o_empty = [&](int s) { return smem_u32(&bars[15 + s]); };
   auto ready = [&](int s) { return smem_u32(&bars[18 + s]); };  // Q and dO of a tile, rows behind the end zero
-  // By tile parity where the arriving side can be a tile ahead of the waiting one.
+  // By tile parity: each pair waits for its own tiles only, and an arriving side can be a tile ahead.
   auto s_full = [&](int g) { return smem_u32(&bars[22 + (g & 1)]); };
   auto p_full = [&](int g) { return smem_u32(&bars[24 + (g & 1)]); };
-  const uint32_t dp_full = smem_u32(&bars[26]), ds_full = smem_u32(&bars[27]), acc_done = smem_u32(&bars[28]);
+  auto dp_full = [&](int g) { return smem_u32(&bars[26 + (g & 1)]); };
+  auto ds_full = [&](int g) { return smem_u32(&bars[28 + (g & 1)]); };
+  const uint32_t acc_done = smem_u32(&bars[30]), acc_free = smem_u32(&bars[31]);  // dv and dk are there; were read
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -469,7 +535,9 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(kv_full(u), 1);
       mbar_init(kv_empty(u), 1);
       mbar_init(s_full(u), 1);
-      mbar_init(p_full(u), 256);
+      mbar_init(p_full(u), W::PAIR);
+      mbar_init(dp_full(u), 1);
+      mbar_init(ds_full(u), W::PAIR);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(q_full(s), 1);
@@ -480,9 +548,8 @@ __global__ void __launch_bounds__(384, 1)
       mbar_init(o_full(s), 1);
       mbar_init(o_empty(s), 1);
     }
-    mbar_init(dp_full, 1);
-    mbar_init(ds_full, 256);
     mbar_init(acc_done, 1);
+    mbar_init(acc_free, W::PAIR);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -502,6 +569,7 @@ __global__ void __launch_bounds__(384, 1)
   auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % Hk); };
   // Unit of work w: key tile (tiles of the sequence) - w, seen by the w query tiles from its own on.
   auto tiles_of = [](const PackedUnit& u) { return (u.len + 127) / 128; };
+  if (warp < W::ROLES) W::roles_regs();
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -597,7 +665,7 @@ __global__ void __launch_bounds__(384, 1)
       auto issue_dP = [&](const StreamTile& t, int g) {
         const int b = t.it % C::KVBUF;
         product(tmem + C::T_DP, dKV0 + (((b * 2 + 1) * C::TILE) >> 4), dO0 + (((g % C::OST) * C::TILE) >> 4));
-        umma_commit(dp_full);
+        umma_commit(dp_full(g));
         if (t.last) umma_commit(kv_empty(b));  // (its last S was issued before)
       };
       StreamTile a = next_tile(), b = next_tile();
@@ -607,6 +675,8 @@ __global__ void __launch_bounds__(384, 1)
       }
       for (int g = 0; ok && a.valid; ++g) {
         if (!(ok = mbar_wait(p_full(g), (g >> 1) & 1, status))) break;
+        // dv and dk restart from zero: the item before has been read
+        if (a.first && a.it > 0 && !(ok = mbar_wait(acc_free, (a.it - 1) & 1, status))) break;
         tc_fence_after();
         add_to(tmem + C::T_DV, tmem + C::T_S + (g % C::SBUF) * 128, dO_MN + (((g % C::OST) * C::TILE) >> 4), a.first);
         umma_commit(o_empty(g % C::OST));
@@ -615,7 +685,7 @@ __global__ void __launch_bounds__(384, 1)
         const StreamTile c = C::SBUF == 2 ? next_tile() : b;
         const bool late = C::KVBUF == 1 && c.first;
         if (c.valid && !late && !(ok = issue_S(c, g + C::SBUF))) break;
-        if (!(ok = mbar_wait(ds_full, g & 1, status))) break;
+        if (!(ok = mbar_wait(ds_full(g), (g >> 1) & 1, status))) break;
         tc_fence_after();
         add_to(tmem + C::T_DK, tmem + C::T_DP, dQ_MN + (((g % C::QST) * C::TILE) >> 4), a.first);
         umma_commit(q_empty(g % C::QST));
@@ -648,114 +718,106 @@ __global__ void __launch_bounds__(384, 1)
           if (lane_id() == 0) mbar_arrive(ready(g % C::QST));
         }
     }
-  } else if (warp >= 4) {
+  } else if (warp >= W::ROLES) {
     // ------------------------------------------------------------ P^T and dS^T
-    // Warpgroup grp: queries [64 grp, 64 grp + 64) of each tile; thread = key row.
-    const int grp = (warp - 4) >> 2;
+    // A pair takes every other tile, its warpgroup `half` the queries [64 half, 64 half + 64); thread = key row.
+    W::pairs_regs();
+    const int pair = (warp - W::ROLES) >> 3, half = ((warp - W::ROLES) >> 2) & 1;
     const int r = ((warp & 3) << 5) + static_cast<int>(lane_id());
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t tdP = tmem + C::T_DP + lane_base + grp * 64;
+    const uint32_t tdP = tmem + C::T_DP + lane_base + half * 64;
     bool ok = true;
     PackedUnit next = unit_of(0);
-    int g = 0;
+    int g0 = 0;  // the item's first tile
     for (int it = 0; ok && next.work; ++it) {
       const PackedUnit u = next;
       next = unit_of(it + 1);
-      int j = 0;  // query tile of the head, from the diagonal on
-      for (int i = 0; i < u.work * group; ++i, ++g) {
-        const uint32_t tS = tmem + C::T_S + (g % C::SBUF) * 128 + lane_base + grp * 64;
-        const float* lse2s = reinterpret_cast<const float*>(sStat + (g % C::QST) * 1024) + grp * 64;
+      const int last = g0 + u.work * group - 1;
+      int j = (W::first(g0, pair) - g0) % u.work;  // query tile of the head, from the diagonal on
+      for (int g = W::first(g0, pair); g <= last; g += W::PAIRS) {
+        const uint32_t tS = tmem + C::T_S + (g % C::SBUF) * 128 + lane_base + half * 64;
+        const float* lse2s = reinterpret_cast<const float*>(sStat + (g % C::QST) * 1024) + half * 64;
         const float* dels = lse2s + 128;
         if (!(ok = mbar_wait_warp(q_full(g % C::QST), (g / C::QST) & 1, status) &&
                    mbar_wait_warp(s_full(g), (g >> 1) & 1, status)))
           break;
         tc_fence_after();
         float p[64];
-        uint32_t pk[32];
-        tmem_ld32(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
-        tmem_ld32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
-        tmem_ld_wait();
-#pragma unroll
-        for (int c = 0; c < 16; ++c) {
-          const float4 z = *reinterpret_cast<const float4*>(lse2s + 4 * c);
-          p[4 * c] = ex2(fmaf(p[4 * c], scale_log2, -z.x));
-          p[4 * c + 1] = ex2(fmaf(p[4 * c + 1], scale_log2, -z.y));
-          p[4 * c + 2] = ex2(fmaf(p[4 * c + 2], scale_log2, -z.z));
-          p[4 * c + 3] = ex2(fmaf(p[4 * c + 3], scale_log2, -z.w));
-        }
+        tmem_ld32_sync(tS, *reinterpret_cast<uint32_t(*)[32]>(&p[0]));
+        tmem_ld32_sync(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&p[32]));
         const bool diagonal = j == 0;
-        if (++j == u.work) j = 0;
-        if (diagonal) {
+        j += W::PAIRS;
+        if (j >= u.work) j -= u.work;
+        if (j >= u.work) j -= u.work;  // (two tiles on in a head of one)
+        // Queries before the key. (dS needs no mask of its own: there P is 0 and dP - Delta finite.)
+        auto exponentials = [&](auto masked) {
 #pragma unroll
-          for (int e = 0; e < 64; ++e)
-            if (grp * 64 + e < r) p[e] = 0.f;
-        }
+          for (int c = 0; c < 4; ++c) {
+            uint32_t pk[8];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) pk[e] = pack_bf16x2(p[2 * e], p[2 * e + 1]);
-        tmem_st32(tS, pk);
+            for (int e = 0; e < 4; ++e) {
+              const float4 z = *reinterpret_cast<const float4*>(lse2s + 16 * c + 4 * e);
+              float* x = &p[16 * c + 4 * e];
+              x[0] = ex2(fmaf(x[0], scale_log2, -z.x));
+              x[1] = ex2(fmaf(x[1], scale_log2, -z.y));
+              x[2] = ex2(fmaf(x[2], scale_log2, -z.z));
+              x[3] = ex2(fmaf(x[3], scale_log2, -z.w));
+            }
+            if constexpr (decltype(masked)::value) {
+#pragma unroll
+              for (int e = 0; e < 16; ++e)
+                if (half * 64 + 16 * c + e < r) p[16 * c + e] = 0.f;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e) pk[e] = pack_bf16x2(p[16 * c + 2 * e], p[16 * c + 2 * e + 1]);
+            PA_TMEM_ST_X8(tS + c * 8, pk);
+          }
+        };
+        if (diagonal) exponentials(std::true_type{});
+        else exponentials(std::false_type{});
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(p_full(g));
-        if (!(ok = mbar_wait_warp(dp_full, g & 1, status))) break;
+        if (!(ok = mbar_wait_warp(dp_full(g), (g >> 1) & 1, status))) break;
         tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t v[32];
-          tmem_ld32_sync(tdP + c * 32, v);
+        for (int c = 0; c < 64 / W::CHUNK; ++c) {
+          constexpr int N = W::CHUNK;
+          uint32_t v[N], pk[N / 2];
+          load_columns(tdP + c * N, v);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float4 z = *reinterpret_cast<const float4*>(dels + c * 32 + 4 * e);
-            float x[4] = {__uint_as_float(v[4 * e]) - z.x, __uint_as_float(v[4 * e + 1]) - z.y,
-                          __uint_as_float(v[4 * e + 2]) - z.z, __uint_as_float(v[4 * e + 3]) - z.w};
-            if (diagonal) {
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (grp * 64 + c * 32 + 4 * e + k < r) x[k] = 0.f;
-            }
-            pk[c * 16 + 2 * e] = pack_bf16x2(p[c * 32 + 4 * e] * x[0], p[c * 32 + 4 * e + 1] * x[1]);
-            pk[c * 16 + 2 * e + 1] = pack_bf16x2(p[c * 32 + 4 * e + 2] * x[2], p[c * 32 + 4 * e + 3] * x[3]);
+          for (int e = 0; e < N / 4; ++e) {
+            const float4 z = *reinterpret_cast<const float4*>(dels + c * N + 4 * e);
+            const float x[4] = {__uint_as_float(v[4 * e]) - z.x, __uint_as_float(v[4 * e + 1]) - z.y,
+                                __uint_as_float(v[4 * e + 2]) - z.z, __uint_as_float(v[4 * e + 3]) - z.w};
+            pk[2 * e] = pack_bf16x2(p[c * N + 4 * e] * x[0], p[c * N + 4 * e + 1] * x[1]);
+            pk[2 * e + 1] = pack_bf16x2(p[c * N + 4 * e + 2] * x[2], p[c * N + 4 * e + 3] * x[3]);
           }
+          store_columns(tdP + c * (N / 2), pk);  // over columns that have been read
         }
-        tmem_st32(tdP, pk);
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(ds_full);
+        mbar_arrive(ds_full(g));
       }
-      if (!ok || !(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
-      // Write-back: warpgroup 0 dv, warpgroup 1 dk. The loads complete before this thread's next
-      // p_full, which the next item's first products into dv and dk wait for.
+      if (!ok) break;
+      g0 = last + 1;
+      if (W::PAIRS == 2 && (last & 1) != pair) continue;
+      // Write-back by the pair of the last tile, half 0 dv and half 1 dk, while the other pair begins
+      // the next item.
+      if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
       tc_fence_after();
       const int row = (tiles_of(u) - u.work) * 128 + r;
       const size_t token = static_cast<size_t>(u.start) + row, col = static_cast<size_t>(head_of(it)) * D;
-      bf16* dst = grp == 0 ? dv + token * dv_stride + col : dk + token * dk_stride + col;
-      const uint32_t src = tmem + (grp == 0 ? C::T_DV : C::T_DK) + lane_base;
-      const float mul = grp == 0 ? 1.f : scale;
+      bf16* dst = half == 0 ? dv + token * dv_stride + col : dk + token * dk_stride + col;
+      const uint32_t src = tmem + (half == 0 ? C::T_DV : C::T_DK) + lane_base;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32_sync(src + c * 32, o);
-        if (row < u.len) {
-          uint4* d4 = reinterpret_cast<uint4*>(dst + c * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float f[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * mul;
-            if (accumulate) {
-              const uint4 old = d4[i];
-              const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const float2 pf = __bfloat1622float2(p2[e]);
-                f[2 * e] += pf.x;
-                f[2 * e + 1] += pf.y;
-              }
-            }
-            d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                               pack_bf16x2(f[6], f[7]));
-          }
-        }
+        if (row < u.len) write_row(dst + c * 32, o, half == 0 ? 1.f : scale, accumulate);
       }
+      tc_fence_before();
+      mbar_arrive(acc_free);
     }
   }
 
@@ -797,15 +859,15 @@ int packed_bwd(const PackedShape& sh, const void* q, const void* k, const void* 
     return dim3(static_cast<unsigned>(items < most ? items : most));
   };
   const int sms = device_sm_count();
-  st = launch_beside(packed_stats_kernel<D>, grid(sh.H, 8 * sms), 256, 0, s, static_cast<const bf16*>(dO),
+  st = launch_beside(packed_stats_kernel<D>, grid(sh.H, kStatBlocks * sms), 256, 0, s, static_cast<const bf16*>(dO),
                      static_cast<const bf16*>(o), lse, list, sh.T, sh.H, rows, lse2, delta);
   if (st != PA_OK) return st;
-  st = launch_beside(packed_dq_kernel<D>, grid(sh.H, sms), PackedDq<D>::THREADS, PackedDq<D>::SMEM, s, mq, mk, mv, mo,
+  st = launch_beside(packed_dq_kernel<D>, grid(sh.H, sms), BwdWarps<D>::THREADS, PackedDq<D>::SMEM, s, mq, mk, mv, mo,
                      static_cast<bf16*>(dq), sh.dq_stride, static_cast<const float*>(lse2),
                      static_cast<const float*>(delta), list, sh.H, group, rows, sh.scale, sh.scale * kLog2e,
                      static_cast<int>(accumulate), status);
   if (st != PA_OK) return st;
-  return launch_beside(packed_dkv_kernel<D>, grid(sh.Hk, sms), PackedDkv<D>::THREADS, PackedDkv<D>::SMEM, s, mq, mk, mv,
+  return launch_beside(packed_dkv_kernel<D>, grid(sh.Hk, sms), BwdWarps<D>::THREADS, PackedDkv<D>::SMEM, s, mq, mk, mv,
                        mo, static_cast<bf16*>(dk), static_cast<bf16*>(dv), sh.dk_stride, sh.dv_stride,
                        static_cast<const float*>(lse2), static_cast<const float*>(delta), list, sh.Hk, group, rows,
                        sh.scale, sh.scale * kLog2e, static_cast<int>(accumulate), status);
