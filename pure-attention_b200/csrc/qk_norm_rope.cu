@@ -500,17 +500,33 @@ NormPlan norm_plan(const RopeShape& r, bool bwd) {
   return p;
 }
 
-NormTable norm_table(const RopeShape& r) {
-  NormTable tab;
+// The table of a call's rotation, kept per thread for the calls that follow with the same one: 64 powers
+// in long double are 8 us of host time, more than a launch.
+const NormTable& norm_table(const RopeShape& r) {
+  struct Kept {
+    RopeShape of;
+    bool valid = false;
+    NormTable tab;
+  };
+  static thread_local Kept kept;
+  const auto same = [&r](const RopeShape& o) {
+    if (o.axes != r.axes || o.pairs != r.pairs || o.per_axis != r.per_axis || o.base != r.base) return false;
+    for (int a = 0; a < r.axes; ++a)
+      if (o.sections[a] != r.sections[a]) return false;
+    return true;
+  };
+  if (kept.valid && same(kept.of)) return kept.tab;
   const long double turn = 1.0L / 6.28318530717958647692528676655900577L;
   int i = 0;
   for (int a = 0; a < r.axes; ++a)
     for (int j = 0; j < r.sections[a]; ++j, ++i) {
       const long double f = r.per_axis ? static_cast<long double>(j) / r.sections[a] : static_cast<long double>(i) / r.pairs;
-      tab.turns[i] = static_cast<uint64_t>(turn * std::pow(static_cast<long double>(r.base), -f) * 0x1p64L + 0.5L);
-      tab.axis[i] = static_cast<uint8_t>(a);
+      kept.tab.turns[i] = static_cast<uint64_t>(turn * std::pow(static_cast<long double>(r.base), -f) * 0x1p64L + 0.5L);
+      kept.tab.axis[i] = static_cast<uint8_t>(a);
     }
-  return tab;
+  kept.of = r;
+  kept.valid = true;
+  return kept.tab;
 }
 
 template <typename T, int V, int U, bool HALVES, bool BWD, bool ACC>
@@ -542,7 +558,7 @@ int norm_launch(const NormRope& sh, const NormPlan& p, NormArgs<T>& g, bool bwd,
   g.tile = p.tile;
   g.G = p.G;
   g.eps = sh.eps;
-  const NormTable tab = norm_table(r);
+  const NormTable& tab = norm_table(r);
   if (p.V == 1) return norm_go<T, 1, 8>(p, g, tab, r.halves, bwd, acc, s);
   if (p.U == 1) return norm_go<T, V, 1>(p, g, tab, r.halves, bwd, acc, s);
   return norm_go<T, V, 2>(p, g, tab, r.halves, bwd, acc, s);

@@ -522,7 +522,10 @@ def _on_stream(fn, t, stream):
     dev = t.get_device()
     if dev < 0 or dev != torch._C._cuda_getDevice():
         raise ValueError(f"{fn}: tensors must be on the current CUDA device, not {t.device}")
-    return _stream() if stream is None else stream
+    if stream is not None:
+        return stream
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return _stream() if raw is None else raw(dev)
 
 
 def _prepared(d, size_of=None):
