@@ -127,6 +127,10 @@ struct PackedFwd {
   static constexpr int QBUF = 2 * Q_ITEM + KV_RING + 1024 <= 227 * 1024 ? 2 : 1;
   static constexpr int SMEM = QBUF * Q_ITEM + KV_RING + 1024;
   static constexpr int THREADS = 384;
+  // Registers of a thread: a softmax thread holds a row of S (128 values), and the first four warps give
+  // theirs; the shares add up to the 384 x 168 of the launch.
+  static constexpr int FEW = 88, MANY = 208;
+  static_assert((FEW + 2 * MANY) * 128 <= THREADS * 168, "an increase would wait forever");
   static constexpr bool SEP_P = D == 64;  // P in its own TMEM columns
   static constexpr uint32_t T_S = 0, T_O = 256;
   static constexpr uint32_t T_P = SEP_P ? 384 : 0;
@@ -233,6 +237,7 @@ __global__ void __launch_bounds__(384, 1)
 
   // Counters that run over all items: it, items; g, key tiles (ring slot and its
   // phase); gt, key tiles of query tile t; f, ragged tiles.
+  if (warp < 4) regs_dec<C::FEW>();
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (elect_one()) {
@@ -373,6 +378,7 @@ __global__ void __launch_bounds__(384, 1)
     }
   } else if (warp >= 4) {
     // ------------------------------------------------------------ softmax
+    regs_inc<C::MANY>();
     const int t = (warp - 4) / 4;               // query tile of this warpgroup
     const int r = threadIdx.x - 128 * (t + 1);  // row within the tile == TMEM lane
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -393,9 +399,7 @@ __global__ void __launch_bounds__(384, 1)
         if (!(ok = mbar_wait_warp(s_full(t), gt & 1, status))) break;
         tc_fence_after();
         float s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(tS + c * 32, *reinterpret_cast<uint32_t(*)[32]>(&s[c * 32]));
-        tmem_ld_wait();
+        tmem_ld128_sync(tS, reinterpret_cast<uint32_t(&)[128]>(s));
         if (C::SEP_P) {
           tc_fence_before();
           mbar_arrive(s_free(t));  // S may now be overwritten by the next tile's product
@@ -446,8 +450,7 @@ __global__ void __launch_bounds__(384, 1)
 #pragma unroll 1
           for (int c = 0; c < D / 32; ++c) {
             uint32_t o[32];
-            tmem_ld32(tO + c * 32, o);
-            tmem_ld_wait();
+            tmem_ld32_sync(tO + c * 32, o);
 #pragma unroll
             for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
             tmem_st32(tO + c * 32, o);
@@ -466,20 +469,21 @@ __global__ void __launch_bounds__(384, 1)
       const bool live = row < w.len;
       const float inv_l = 1.f / l;
       const size_t token = static_cast<size_t>(w.start) + row;
-      bf16* orow = O + (token * H + head) * D;
+      bf16* oquad = O + ((token - (r & 3)) * H + head) * D;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32], pkd[16];
-        tmem_ld32(tO + c * 32, o);
-        tmem_ld_wait();
+        uint32_t o[32];
+        uint4 u[4];
+        tmem_ld32_sync(tO + c * 32, o);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-          pkd[i] = pack_bf16x2(__uint_as_float(o[2 * i]) * inv_l, __uint_as_float(o[2 * i + 1]) * inv_l);
-        if (live) {
-          uint4* dst = reinterpret_cast<uint4*>(orow + c * 32);
+        for (int i = 0; i < 4; ++i) {
+          uint32_t w4[4];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) dst[i] = make_uint4(pkd[4 * i], pkd[4 * i + 1], pkd[4 * i + 2], pkd[4 * i + 3]);
+          for (int e = 0; e < 4; ++e)
+            w4[e] = pack_bf16x2(__uint_as_float(o[8 * i + 2 * e]) * inv_l, __uint_as_float(o[8 * i + 2 * e + 1]) * inv_l);
+          u[i] = make_uint4(w4[0], w4[1], w4[2], w4[3]);
         }
+        store_rows(oquad + c * 32, static_cast<long long>(H) * D, w.len - (row & ~3), u);
       }
       if (live) lse[static_cast<size_t>(head) * T + token] = (m + __log2f(l)) * kLn2;
     }

@@ -102,16 +102,18 @@ __global__ void __launch_bounds__(256, kStatBlocks)
   }
 }
 
-// 32 values of a row, scaled: to[i] (=|+=) o[i] * mul.
-__device__ __forceinline__ void write_row(bf16* to, const uint32_t (&o)[32], float mul, int accumulate) {
-  uint4* d4 = reinterpret_cast<uint4*>(to);
+// 32 values of a lane's row `row`, scaled: to[i] (=|+=) o[i] * mul. to: the columns in row 0 of the sequence. All lanes of
+// the warp take part.
+__device__ __forceinline__ void write_row(bf16* to, long long stride, int row, int len, const uint32_t (&o)[32],
+                                          float mul, int accumulate) {
+  uint4 u[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     float f[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(o[8 * i + e]) * mul;
-    if (accumulate) {
-      const uint4 old = d4[i];
+    if (accumulate && row < len) {
+      const uint4 old = reinterpret_cast<const uint4*>(to + row * stride)[i];
       const __nv_bfloat162* p2 = reinterpret_cast<const __nv_bfloat162*>(&old);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -120,9 +122,11 @@ __device__ __forceinline__ void write_row(bf16* to, const uint32_t (&o)[32], flo
         f[2 * e + 1] += pf.y;
       }
     }
-    d4[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
-                       pack_bf16x2(f[6], f[7]));
+    u[i] = make_uint4(pack_bf16x2(f[0], f[1]), pack_bf16x2(f[2], f[3]), pack_bf16x2(f[4], f[5]),
+                      pack_bf16x2(f[6], f[7]));
   }
+  const int quad = row & ~3;
+  store_rows(to + quad * stride, stride, len - quad, u);
 }
 
 // Who computes P and dS: warps 0 to 2 load, issue and clear ragged rows; from warp 4 on, pairs of
@@ -457,12 +461,12 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
       tc_fence_after();
       const int row = (u.work - 1) * 128 + r;
-      bf16* dst = dq + (static_cast<size_t>(u.start) + row) * dq_stride + static_cast<size_t>(head_of(it)) * D;
+      bf16* dst = dq + static_cast<size_t>(u.start) * dq_stride + static_cast<size_t>(head_of(it)) * D;
 #pragma unroll 1
       for (int c = half * (D / 64); c < (half + 1) * (D / 64); ++c) {
         uint32_t o[32];
         tmem_ld32_sync(tmem + C::T_DQ + lane_base + c * 32, o);
-        if (row < u.len) write_row(dst + c * 32, o, scale, accumulate);
+        write_row(dst + c * 32, dq_stride, row, u.len, o, scale, accumulate);
       }
       tc_fence_before();
       mbar_arrive(acc_free);
@@ -807,14 +811,15 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
       tc_fence_after();
       const int row = (tiles_of(u) - u.work) * 128 + r;
-      const size_t token = static_cast<size_t>(u.start) + row, col = static_cast<size_t>(head_of(it)) * D;
-      bf16* dst = half == 0 ? dv + token * dv_stride + col : dk + token * dk_stride + col;
+      const size_t start = static_cast<size_t>(u.start), col = static_cast<size_t>(head_of(it)) * D;
+      const long long stride = half == 0 ? dv_stride : dk_stride;
+      bf16* dst = (half == 0 ? dv : dk) + start * stride + col;
       const uint32_t src = tmem + (half == 0 ? C::T_DV : C::T_DK) + lane_base;
 #pragma unroll 1
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
         tmem_ld32_sync(src + c * 32, o);
-        if (row < u.len) write_row(dst + c * 32, o, half == 0 ? 1.f : scale, accumulate);
+        write_row(dst + c * 32, stride, row, u.len, o, half == 0 ? 1.f : scale, accumulate);
       }
       tc_fence_before();
       mbar_arrive(acc_free);

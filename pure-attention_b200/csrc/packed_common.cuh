@@ -66,6 +66,31 @@ int launch_beside(K kernel, dim3 grid, int threads, size_t smem, cudaStream_t s,
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
+// Stores 32 columns of bf16 of a warp's 32 consecutive rows, a lane's row as four 16-byte pieces in u.
+// The lanes of a quad exchange pieces first, so that a store covers 64 bytes of 8 rows and not 16
+// of 32: the write-back of an item is bound by the lines that its stores touch. to: the columns in the
+// quad's first row; rows: rows that exist from there on. All lanes of the warp take part.
+__device__ __forceinline__ void store_rows(__nv_bfloat16* to, long long stride, int rows, uint4 (&u)[4]) {
+  const int q = static_cast<int>(lane_id() & 3);
+#pragma unroll
+  for (int b = 1; b < 4; b <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & b) continue;
+      const bool up = q & b;
+      uint4 v = up ? u[j] : u[j | b];
+      v.x = __shfl_xor_sync(0xffffffffu, v.x, b);
+      v.y = __shfl_xor_sync(0xffffffffu, v.y, b);
+      v.z = __shfl_xor_sync(0xffffffffu, v.z, b);
+      v.w = __shfl_xor_sync(0xffffffffu, v.w, b);
+      if (up) u[j] = v;
+      else u[j | b] = v;
+    }
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (j < rows) *reinterpret_cast<uint4*>(to + j * stride + q * 8) = u[j];
+}
+
 // Zeroes rows [from, 128) of a swizzled tile of `chunks` 128-row x 128-byte boxes (one warp), and
 // orders the zeros before the tensor core's reads.
 __device__ __forceinline__ void zero_rows(uint8_t* tile, int chunks, int from) {
