@@ -9,6 +9,12 @@
 //   dx = r (u - x r^2 mean(u x)).
 // The statistics are sums in fp32 over the lanes that share a head; r is computed
 // again in the backward, which reads x anyway, rather than stored.
+//
+// Bound by HBM in bytes (x once, y once; the backward x, dy and dx), and next to that by instructions: some 300 for
+// 16 bytes of a head a lane (conversions, squares, shuffles, two products a value), 53% of the issue slots. 8 x
+// 4096 tokens of 16 + 2 heads of 128 in bf16: 76 us (4.0 TB/s of 6.55 a plain copy; the rotation alone 66), the
+// gradient 148 us (3.1 TB/s), in fp32 168 us (5.4). Slower, 89 to 122 us: inputs through a ring of bulk copies or of
+// cp.async, packed pairs of fp32, vectors of 8 bytes, fewer heads in flight with more blocks.
 #include <cmath>
 #include <cstring>
 #include <type_traits>
