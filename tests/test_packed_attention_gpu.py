@@ -257,3 +257,36 @@ def test_lengths_out_of_bounds_stay_in_bounds():
         assert (o[:a] == 7).all() and (o[b:] == 7).all()
         if b > a:
             _near(o[a:b], want[a:b], bound[a:b])
+
+
+@pytest.mark.parametrize("H, Hk, D", [(16, 16, 64), (16, 16, 128), (24, 8, 64)])
+def test_more_work_than_the_gpu_holds_at_once(H, Hk, D):
+    """Several items for each CTA, of long and short sequences, full and ragged."""
+    lens = [300, 0, 77, 640, 129, 512, 33, 255, 1, 128]
+    q, k, v, cu = _inputs(lens, H, Hk, D, 20, fused=True)
+    dO = _normal(torch.Generator(device="cuda").manual_seed(21), *q.shape)
+    o, lse = _fwd(q, k, v, cu)
+    (want, bound), (wl, bl) = ref.packed(q, k, v, lens, 0)
+    _near(o, want, bound)
+    _near(lse, wl, bl, 2.0 ** -22)
+    for x, (w, b) in zip(_bwd(q, k, v, cu, dO, o=o, lse=lse), ref.packed(q, k, v, lens, 0, dO, o)):
+        _near(x, w, b)
+
+
+def test_calls_after_a_failed_wait_leave_their_outputs():
+    """While the device's status word is set, the kernels skip their work; cleared, they run."""
+    import pa_capi
+    q, k, v, cu = _inputs([200, 77], 4, 2, 64, 22)
+    dO = _normal(torch.Generator(device="cuda").manual_seed(23), *q.shape)
+    want = _fwd(q, k, v, cu)
+    grads = _bwd(q, k, v, cu, dO, o=want[0], lse=want[1])
+    assert pa_capi.device_status() == 0
+    pa_capi.wait_selftest(100_000_000, arrive=False)
+    skipped = [*_fwd(q, k, v, cu), *_bwd(q, k, v, cu, dO, o=want[0], lse=want[1])]
+    assert pa_capi.device_status(clear=True) == 6  # PA_ERR_TIMEOUT
+    for x in skipped:
+        assert (x == 7).all()
+    again = [*_fwd(q, k, v, cu), *_bwd(q, k, v, cu, dO, o=want[0], lse=want[1])]
+    assert pa_capi.device_status() == 0
+    for x, y in zip(again, [*want, *grads]):
+        assert torch.equal(x, y)
