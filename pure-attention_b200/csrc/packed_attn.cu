@@ -88,8 +88,7 @@ __global__ void __launch_bounds__(kListThreads)
   if ((tid & 31) == 0) before = tid ? warps[(tid >> 5) - 1] : 0;
   int top = 0;
   for (int i = lo; i < hi; ++i) {
-    before = max(before, min(max(cu[i], 0), T));
-    const int len = max(before, min(cu[i + 1], T)) - before;
+    const int len = packed_seq(cu, i, T, before);
     seqs[i] = make_int2(before, len);
     top = max(top, units_of(len, unit));
   }
@@ -173,11 +172,12 @@ template <int D>
 __global__ void __launch_bounds__(384, 1)
     packed_fwd_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                       const __grid_constant__ CUtensorMap mapV, bf16* __restrict__ O, float* __restrict__ lse,
-                      const PackedList* __restrict__ list, int T, int H, int group, int pair_heads,
+                      const __grid_constant__ PackedWork work, int T, int H, int group, int pair_heads,
                       float scale_log2, uint32_t* status) {
   using C = PackedFwd<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[24];
+  __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   if (cta_aborted(status, &abort_flag)) {
@@ -227,17 +227,19 @@ __global__ void __launch_bounds__(384, 1)
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
+  const int n_hh = pair_heads ? H / 2 : H;
   wait_prerequisites();  // the list
+  if (threadIdx.x == 64 && !work.list) own = work.direct(static_cast<int>(blockIdx.x) / n_hh);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int n_hh = pair_heads ? H / 2 : H;
-  const long long n_items = static_cast<long long>(list->count) * n_hh;
+  const long long n_items = work.items(n_hh);
   // Items in turn; the next one's unit is fetched while the current one runs.
   auto unit_of = [&](int turn) {
     const long long i = packed_turn(turn);
-    return i < n_items ? packed_unit(list, static_cast<int>(i / n_hh)) : PackedUnit{0, 0, 0, 0};
+    if (!work.list) return turn == 0 ? own : PackedUnit{0, 0, 0, 0};
+    return i < n_items ? work.listed(static_cast<int>(i / n_hh)) : PackedUnit{0, 0, 0, 0};
   };
   auto item_of = [&](int turn, const PackedUnit& u) {
     return packed_item(u, static_cast<int>(packed_turn(turn) % n_hh), pair_heads, group);
@@ -517,13 +519,15 @@ int packed_fwd(const PackedShape& sh, const void* q, const void* k, const void* 
   if (!ensure_smem_attr(packed_fwd_kernel<D>, C::SMEM, attr)) return PA_ERR_LAUNCH;
   const int group = sh.H / sh.Hk;
   const bool pair_heads = group % 2 == 0;
-  const int st = launch_packed_list(sh, cu, pair_heads ? 128 : 256, ws, s);
+  const int unit = pair_heads ? 128 : 256, heads = pair_heads ? sh.H / 2 : sh.H;
+  const size_t items = packed_units(sh, unit) * heads, sms = device_sm_count();
+  PackedWork work;
+  const int st = packed_work(&work, sh, cu, unit, heads, static_cast<int>(sms), ws, s);
   if (st != PA_OK) return st;
-  const size_t items = packed_units(sh, pair_heads ? 128 : 256) * (pair_heads ? sh.H / 2 : sh.H);
-  const size_t sms = device_sm_count();
-  return launch_beside(packed_fwd_kernel<D>, dim3(static_cast<unsigned>(items < sms ? items : sms)), C::THREADS,
-                       C::SMEM, s, mq, mk, mv, static_cast<bf16*>(o), lse, static_cast<const PackedList*>(ws), sh.T,
-                       sh.H, group, static_cast<int>(pair_heads), sh.scale * kLog2e, status);
+  const dim3 grid(static_cast<unsigned>(items < sms ? items : sms));
+  return launch_beside(work.list != nullptr, packed_fwd_kernel<D>, grid, C::THREADS, C::SMEM, s, mq, mk, mv,
+                       static_cast<bf16*>(o), lse, work, sh.T, sh.H, group, static_cast<int>(pair_heads),
+                       sh.scale * kLog2e, status);
 }
 
 }  // namespace

@@ -52,16 +52,17 @@ constexpr int kStatBlocks = 3;  // per SM; a thread has its piece of 4 or 8 rows
 template <int D>
 __global__ void __launch_bounds__(256, kStatBlocks)
     packed_stats_kernel(const bf16* __restrict__ dO, const bf16* __restrict__ O, const float* __restrict__ lse,
-                        const PackedList* __restrict__ list, int T, int H, long long rows, float* __restrict__ lse2,
+                        const __grid_constant__ PackedWork work, int T, int H, long long rows, float* __restrict__ lse2,
                         float* __restrict__ delta) {
   constexpr int LANES = D / 8, STEP = 256 / LANES;  // lanes that share a row; rows of a pass
   launch_dependents();
   wait_prerequisites();
   // item = (unit, head), stepped through without divisions
-  const int count = list->count, lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
+  const int count = work.list ? work.list->count : static_cast<int>(gridDim.x) / H;
+  const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
   const int du = static_cast<int>(gridDim.x) / H, dh = static_cast<int>(gridDim.x) % H;
   int at_unit = static_cast<int>(blockIdx.x) / H, h = static_cast<int>(blockIdx.x) % H;
-  auto unit_of = [&](int i) { return i < count ? packed_unit(list, i) : PackedUnit{0, 0, 0, 0}; };
+  auto unit_of = [&](int i) { return i >= count ? PackedUnit{0, 0, 0, 0} : work.list ? work.listed(i) : work.direct(i); };
   PackedUnit next = unit_of(at_unit);
   while (next.work) {
     const PackedUnit u = next;
@@ -197,12 +198,13 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     packed_dq_kernel(const __grid_constant__ CUtensorMap mapQ, const __grid_constant__ CUtensorMap mapK,
                      const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
                      bf16* __restrict__ dq, long long dq_stride, const float* __restrict__ lse2,
-                     const float* __restrict__ delta, const PackedList* __restrict__ list, int H, int group,
+                     const float* __restrict__ delta, const __grid_constant__ PackedWork work, int H, int group,
                      long long rows, float scale, float scale_log2, int accumulate, uint32_t* status) {
   using C = PackedDq<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[34];
+  __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   launch_dependents();
@@ -257,14 +259,16 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     tmem_relinquish();
   }
   wait_prerequisites();
+  if (threadIdx.x == 64 && !work.list) own = work.direct(static_cast<int>(blockIdx.x) / H);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const long long n_items = static_cast<long long>(list->count) * H;
+  const long long n_items = work.items(H);
   auto unit_of = [&](int turn) {
     const long long i = packed_turn(turn);
-    return i < n_items ? packed_unit(list, static_cast<int>(i / H)) : PackedUnit{0, 0, 0, 0};
+    if (!work.list) return turn == 0 ? own : PackedUnit{0, 0, 0, 0};
+    return i < n_items ? work.listed(static_cast<int>(i / H)) : PackedUnit{0, 0, 0, 0};
   };
   auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % H); };
   if (warp < W::ROLES) W::roles_regs();
@@ -510,12 +514,13 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
                       const __grid_constant__ CUtensorMap mapV, const __grid_constant__ CUtensorMap mapdO,
                       bf16* __restrict__ dk, bf16* __restrict__ dv, long long dk_stride, long long dv_stride,
                       const float* __restrict__ lse2, const float* __restrict__ delta,
-                      const PackedList* __restrict__ list, int Hk, int group, long long rows, float scale,
+                      const __grid_constant__ PackedWork work, int Hk, int group, long long rows, float scale,
                       float scale_log2, int accumulate, uint32_t* status) {
   using C = PackedDkv<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[32];
+  __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
   if (cta_aborted(status, &abort_flag)) {
@@ -569,14 +574,16 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     tmem_relinquish();
   }
   wait_prerequisites();
+  if (threadIdx.x == 64 && !work.list) own = work.direct(static_cast<int>(blockIdx.x) / Hk);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const long long n_items = static_cast<long long>(list->count) * Hk;
+  const long long n_items = work.items(Hk);
   auto unit_of = [&](int turn) {
     const long long i = packed_turn(turn);
-    return i < n_items ? packed_unit(list, static_cast<int>(i / Hk)) : PackedUnit{0, 0, 0, 0};
+    if (!work.list) return turn == 0 ? own : PackedUnit{0, 0, 0, 0};
+    return i < n_items ? work.listed(static_cast<int>(i / Hk)) : PackedUnit{0, 0, 0, 0};
   };
   auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % Hk); };
   // Unit of work w: key tile (tiles of the sequence) - w, seen by the w query tiles from its own on.
@@ -860,29 +867,29 @@ int packed_bwd(const PackedShape& sh, const void* q, const void* k, const void* 
       !ensure_smem_attr(packed_dkv_kernel<D>, PackedDkv<D>::SMEM, attr_dkv))
     return PA_ERR_LAUNCH;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  const PackedList* list = reinterpret_cast<const PackedList*>(w);
   float* lse2 = reinterpret_cast<float*>(w + packed_list_bytes(sh, 128));
   float* delta = reinterpret_cast<float*>(w + packed_list_bytes(sh, 128) + stat_bytes(sh));
   const long long rows = stat_blocks(sh.T, sh.n) * 128;
   const int group = sh.H / sh.Hk;
-  int st = launch_packed_list(sh, cu, 128, ws, s);
-  if (st != PA_OK) return st;
   auto grid = [&](long long heads, long long most) {
     const long long items = static_cast<long long>(packed_units(sh, 128)) * heads;
     return dim3(static_cast<unsigned>(items < most ? items : most));
   };
   const int sms = device_sm_count();
-  st = launch_beside(packed_stats_kernel<D>, grid(sh.H, kStatBlocks * sms), 256, 0, s, static_cast<const bf16*>(dO),
-                     static_cast<const bf16*>(o), lse, list, sh.T, sh.H, rows, lse2, delta);
+  PackedWork work;
+  int st = packed_work(&work, sh, cu, 128, sh.H, sms, ws, s);
   if (st != PA_OK) return st;
-  st = launch_beside(packed_dq_kernel<D>, grid(sh.H, sms), BwdWarps<D>::THREADS, PackedDq<D>::SMEM, s, mq, mk, mv, mo,
-                     static_cast<bf16*>(dq), sh.dq_stride, static_cast<const float*>(lse2),
-                     static_cast<const float*>(delta), list, sh.H, group, rows, sh.scale, sh.scale * kLog2e,
+  st = launch_beside(work.list != nullptr, packed_stats_kernel<D>, grid(sh.H, kStatBlocks * sms), 256, 0, s,
+                     static_cast<const bf16*>(dO), static_cast<const bf16*>(o), lse, work, sh.T, sh.H, rows, lse2, delta);
+  if (st != PA_OK) return st;
+  st = launch_beside(true, packed_dq_kernel<D>, grid(sh.H, sms), BwdWarps<D>::THREADS, PackedDq<D>::SMEM, s, mq, mk, mv,
+                     mo, static_cast<bf16*>(dq), sh.dq_stride, static_cast<const float*>(lse2),
+                     static_cast<const float*>(delta), work, sh.H, group, rows, sh.scale, sh.scale * kLog2e,
                      static_cast<int>(accumulate), status);
   if (st != PA_OK) return st;
-  return launch_beside(packed_dkv_kernel<D>, grid(sh.Hk, sms), BwdWarps<D>::THREADS, PackedDkv<D>::SMEM, s, mq, mk, mv,
-                       mo, static_cast<bf16*>(dk), static_cast<bf16*>(dv), sh.dk_stride, sh.dv_stride,
-                       static_cast<const float*>(lse2), static_cast<const float*>(delta), list, sh.Hk, group, rows,
+  return launch_beside(true, packed_dkv_kernel<D>, grid(sh.Hk, sms), BwdWarps<D>::THREADS, PackedDkv<D>::SMEM, s, mq, mk,
+                       mv, mo, static_cast<bf16*>(dk), static_cast<bf16*>(dv), sh.dk_stride, sh.dv_stride,
+                       static_cast<const float*>(lse2), static_cast<const float*>(delta), work, sh.Hk, group, rows,
                        sh.scale, sh.scale * kLog2e, static_cast<int>(accumulate), status);
 }
 

@@ -686,7 +686,7 @@ int paged_launch(const PagedShape& sh, const PagedPlan& p, const void* q, const 
   if (cudaGetLastError() != cudaSuccess) return PA_ERR_LAUNCH;
   if (unit_tiles == 1) return PA_OK;  // no unit is cut
   const int cuts = a.cuts_by_cta ? grid : sh.B * sh.Hk * p.chunks;
-  return launch_beside(paged_join_kernel<T, D, Core::ROWS>, dim3(cuts * p.chunk_heads), kJoinThreads, 0, s, a,
+  return launch_beside(true, paged_join_kernel<T, D, Core::ROWS>, dim3(cuts * p.chunk_heads), kJoinThreads, 0, s, a,
                        static_cast<T*>(o), lse);
 }
 

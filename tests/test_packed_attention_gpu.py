@@ -290,3 +290,24 @@ def test_calls_after_a_failed_wait_leave_their_outputs():
     assert pa_capi.device_status() == 0
     for x, y in zip(again, [*want, *grads]):
         assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("lens, T, H, Hk, D", [
+    ([5, 0, 130, 1], 140, 8, 2, 64),              # as many units as the GPU has SMs at most: no list
+    ([0] * 15 + [200], 200, 4, 4, 128),
+    ([0] * 16 + [200], 200, 4, 4, 128),           # one sequence more: a list
+    ([16, 0, 3, 128, 129], 276, 16, 16, 64),      # (units and heads on both sides of 148)
+    ([16, 0, 3, 128, 129], 276, 24, 8, 64),
+    ([1] * 9, 9, 12, 3, 128),
+])
+def test_few_units_and_many_sequences(lens, T, H, Hk, D):
+    """Small calls, which find their work without a list, and the same sizes with one."""
+    q, k, v, cu = _inputs(lens, H, Hk, D, 24)
+    assert q.shape[0] == sum(lens) <= T
+    dO = _normal(torch.Generator(device="cuda").manual_seed(25), *q.shape)
+    o, lse = _fwd(q, k, v, cu)
+    (want, bound), (wl, bl) = ref.packed(q, k, v, lens, 0)
+    _near(o, want, bound)
+    _near(lse, wl, bl, 2.0 ** -22)
+    for x, (w, b) in zip(_bwd(q, k, v, cu, dO, o=o, lse=lse), ref.packed(q, k, v, lens, 0, dO, o)):
+        _near(x, w, b)
