@@ -158,6 +158,7 @@ struct BwdWarps {
   static __device__ __forceinline__ void pairs_regs() {
     if constexpr (PAIRS == 2) regs_inc<MANY>();
   }
+  static __device__ __forceinline__ int pair_of(int g) { return PAIRS == 2 ? g & 1 : 0; }
   // The first tile of `pair` from tile g on.
   static __device__ __forceinline__ int first(int g, int pair) { return PAIRS == 2 ? g + ((g ^ pair) & 1) : g; }
 };
@@ -203,7 +204,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   using C = PackedDq<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[34];
+  __shared__ uint64_t bars[35];
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -227,7 +228,10 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   auto ds_full = [&](int g) { return smem_u32(&bars[22 + (g & 1)]); };
   auto dp_full = [&](int g) { return smem_u32(&bars[24 + (g & 1)]); };
   auto dp_free = [&](int g) { return smem_u32(&bars[26 + (g & 1)]); };
-  const uint32_t acc_done = smem_u32(&bars[28]), acc_free = smem_u32(&bars[29]);  // an item's dq is there; was read
+  // An item's dq is there, for the pair of its last tile (which may wait for it before the item before is
+  // done, so each pair has a barrier of its own); it has been read.
+  auto acc_done = [&](int pair) { return smem_u32(&bars[28 + pair]); };
+  const uint32_t acc_free = smem_u32(&bars[34]);
   // the f-th ragged K tile has landed, and its rows behind the end are zero; two are on the way at most
   auto k_ragged = [&](int f) { return smem_u32(&bars[30 + (f & 1)]); };
   auto k_zeroed = [&](int f) { return smem_u32(&bars[32 + (f & 1)]); };
@@ -250,7 +254,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       mbar_init(v_full(s), 1);
       mbar_init(v_empty(s), 1);
     }
-    mbar_init(acc_done, 1);
+    for (int u = 0; u < 2; ++u) mbar_init(acc_done(u), 1);
     mbar_init(acc_free, W::PAIR);
     fence_mbar_init();
   }
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
           umma_f16_ts(tmem + C::T_DQ, tmem + C::T_S + (g & 1) * 128 + step_col(k),
                       dK_MN + (((g % C::KST) * C::TILE + k * 2048) >> 4), idQ, (!a.first || k > 0) ? 1u : 0u);
         umma_commit(k_empty(g % C::KST));
-        if (a.last) umma_commit(acc_done);
+        if (a.last) umma_commit(acc_done(W::pair_of(g)));
         const StreamTile c = next_tile();
         if (c.valid && !(ok = issue_S(c, g + 2))) break;
         a = b;
@@ -418,7 +422,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       return make_float2(lse2[at], delta[at]);
     };
     float2 st_next = stats(next, 0);
-    int g0 = 0;  // the item's first tile
+    int g0 = 0, done = 0;  // the item's first tile; items that this pair wrote
     for (int it = 0; ok && next.work; ++it) {
       const PackedUnit u = next;
       const float neg_lse = -st_next.x, del = st_next.y;
@@ -467,10 +471,11 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       }
       if (!ok) break;
       g0 = last + 1;
-      if (W::PAIRS == 2 && (last & 1) != pair) continue;
+      if (W::pair_of(last) != pair) continue;
       // dq write-back by the pair of the last tile, each warpgroup half of the columns, while
       // the other pair begins the next item
-      if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
+      if (!(ok = mbar_wait_warp(acc_done(pair), done & 1, status))) break;
+      ++done;
       tc_fence_after();
       const int row = (u.work - 1) * 128 + r;
       bf16* dst = dq + static_cast<size_t>(u.start) * dq_stride + static_cast<size_t>(head_of(it)) * D;
@@ -519,7 +524,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   using C = PackedDkv<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[32];
+  __shared__ uint64_t bars[33];
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -544,7 +549,8 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   auto p_full = [&](int g) { return smem_u32(&bars[24 + (g & 1)]); };
   auto dp_full = [&](int g) { return smem_u32(&bars[26 + (g & 1)]); };
   auto ds_full = [&](int g) { return smem_u32(&bars[28 + (g & 1)]); };
-  const uint32_t acc_done = smem_u32(&bars[30]), acc_free = smem_u32(&bars[31]);  // dv and dk are there; were read
+  auto acc_done = [&](int pair) { return smem_u32(&bars[30 + pair]); };  // dv and dk are there, as for dq; were read
+  const uint32_t acc_free = smem_u32(&bars[32]);
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -565,7 +571,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       mbar_init(o_full(s), 1);
       mbar_init(o_empty(s), 1);
     }
-    mbar_init(acc_done, 1);
+    for (int u = 0; u < 2; ++u) mbar_init(acc_done(u), 1);
     mbar_init(acc_free, W::PAIR);
     fence_mbar_init();
   }
@@ -708,7 +714,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
         tc_fence_after();
         add_to(tmem + C::T_DK, tmem + C::T_DP, dQ_MN + (((g % C::QST) * C::TILE) >> 4), a.first);
         umma_commit(q_empty(g % C::QST));
-        if (a.last) umma_commit(acc_done);
+        if (a.last) umma_commit(acc_done(W::pair_of(g)));
         if (c.valid && late && !(ok = issue_S(c, g + C::SBUF))) break;
         if (b.valid) issue_dP(b, g + 1);  // (waited for with its S)
         a = b;
@@ -747,7 +753,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     const uint32_t tdP = tmem + C::T_DP + lane_base + half * 64;
     bool ok = true;
     PackedUnit next = unit_of(0);
-    int g0 = 0;  // the item's first tile
+    int g0 = 0, done = 0;  // the item's first tile; items that this pair wrote
     for (int it = 0; ok && next.work; ++it) {
       const PackedUnit u = next;
       next = unit_of(it + 1);
@@ -820,10 +826,11 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       }
       if (!ok) break;
       g0 = last + 1;
-      if (W::PAIRS == 2 && (last & 1) != pair) continue;
+      if (W::pair_of(last) != pair) continue;
       // Write-back by the pair of the last tile, half 0 dv and half 1 dk, while the other pair begins
       // the next item.
-      if (!(ok = mbar_wait_warp(acc_done, it & 1, status))) break;
+      if (!(ok = mbar_wait_warp(acc_done(pair), done & 1, status))) break;
+      ++done;
       tc_fence_after();
       const int row = (tiles_of(u) - u.work) * 128 + r;
       const size_t start = static_cast<size_t>(u.start), col = static_cast<size_t>(head_of(it)) * D;

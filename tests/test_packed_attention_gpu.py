@@ -311,3 +311,18 @@ def test_few_units_and_many_sequences(lens, T, H, Hk, D):
     _near(lse, wl, bl, 2.0 ** -22)
     for x, (w, b) in zip(_bwd(q, k, v, cu, dO, o=o, lse=lse), ref.packed(q, k, v, lens, 0, dO, o)):
         _near(x, w, b)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_sequences_of_one_tile(D):
+    """Items of one tile, several to a CTA: an item's sums are read while the next one's are computed."""
+    lens, H = [700] + [90, 128, 1, 33] * 25, 12
+    q, k, v, cu = _inputs(lens, H, H, D, 26)
+    dO = _normal(torch.Generator(device="cuda").manual_seed(27), *q.shape)
+    o, lse = _fwd(q, k, v, cu)
+    (want, bound), _ = ref.packed(q, k, v, lens, 0)
+    _near(o, want, bound)
+    want = ref.packed(q, k, v, lens, 0, dO, o)
+    for _ in range(10):
+        for x, (w, b) in zip(_bwd(q, k, v, cu, dO, o=o, lse=lse), want):
+            _near(x, w, b)
