@@ -17,7 +17,7 @@
 //                        the diagonal on for each head of the group; rows are keys
 // Both keep P and dS in TMEM as the A operand of the products that use them.
 //
-// Measured, lists and statistics included: 12800 tokens in 8 sequences of up to 4096, 16 heads of 64, 336 us (546
+// Measured, lists and statistics included: 12800 tokens in 8 sequences of up to 4096, 16 heads of 64, 331 us (556
 // TFLOP/s of the five products under the mask); 8192 tokens, 16 + 4 heads of 128, 765 us (900). At 128 the tensor
 // pipe is 70% busy. At 64 it is 37% (dq) and 45% (dk, dv), the exponential unit 50%: a tile's products are
 // short (one of 128 x 128 x 64 takes 362 clocks in a row of them, 768 with its barrier waited for), and what is left
@@ -208,7 +208,6 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  launch_dependents();
   if (cta_aborted(status, &abort_flag)) {
     wait_prerequisites();
     return;
@@ -263,6 +262,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     tmem_relinquish();
   }
   wait_prerequisites();
+  launch_dependents();  // from here on the statistics are there, and dk and dv need no more
   if (threadIdx.x == 64 && !work.list) own = work.direct(static_cast<int>(blockIdx.x) / H);
   tc_fence_before();
   __syncthreads();
@@ -579,7 +579,8 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     tmem_alloc(smem_u32(&tmem_slot), 512);
     tmem_relinquish();
   }
-  wait_prerequisites();
+  // Its blocks start as those of dq end, and not when all have: what they read was complete before any block of dq
+  // let them start. They wait for dq at their own end, so that the call ends with both (336 to 331 us).
   if (threadIdx.x == 64 && !work.list) own = work.direct(static_cast<int>(blockIdx.x) / Hk);
   tc_fence_before();
   __syncthreads();
@@ -854,6 +855,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  wait_prerequisites();
 }
 
 size_t stat_bytes(const PackedShape& sh) {
