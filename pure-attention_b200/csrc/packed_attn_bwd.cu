@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256, kStatBlocks)
   launch_dependents();
   wait_prerequisites();
   // item = (unit, head), stepped through without divisions
-  const int count = work.list ? work.list->count : static_cast<int>(gridDim.x) / H;
+  const int count = work.list ? __ldcg(&work.list->count) : static_cast<int>(gridDim.x) / H;
   const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
   const int du = static_cast<int>(gridDim.x) / H, dh = static_cast<int>(gridDim.x) % H;
   int at_unit = static_cast<int>(blockIdx.x) / H, h = static_cast<int>(blockIdx.x) % H;
@@ -590,7 +590,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   auto unit_of = [&](int turn) {
     const long long i = packed_turn(turn);
     if (!work.list) return turn == 0 ? own : PackedUnit{0, 0, 0, 0};
-    return i < n_items ? work.listed(static_cast<int>(i / Hk)) : PackedUnit{0, 0, 0, 0};
+    return i < n_items ? work.listed<false>(static_cast<int>(i / Hk)) : PackedUnit{0, 0, 0, 0};
   };
   auto head_of = [&](int turn) { return static_cast<int>(packed_turn(turn) % Hk); };
   // Unit of work w: key tile (tiles of the sequence) - w, seen by the w query tiles from its own on.

@@ -35,11 +35,13 @@ int launch_packed_list(const PackedShape& sh, const int32_t* cu, int unit, void*
 // Sequence i of the tokens: starts are a running maximum, clamped to the tokens. `before` is the start of the
 // sequence before it (0 at first), and its own afterwards.
 __device__ __forceinline__ int packed_seq(const int32_t* cu, int i, int T, int& before) {
-  before = max(before, min(max(cu[i], 0), T));
-  return max(before, min(cu[i + 1], T)) - before;
+  before = max(before, min(max(__ldcg(cu + i), 0), T));
+  return max(before, min(__ldcg(cu + i + 1), T)) - before;
 }
 
-// Where a kernel has its units from: the list, or (NULL) the lengths.
+// Where a kernel has its units from: the list, or (NULL) the lengths. The kernel of dk and dv, which does not wait for
+// the kernel before it, reads past its SM's own cache, where an older list may still be (in all kernels that cost up
+// to 1%).
 constexpr int kDirectSeqs = 16;
 struct PackedWork {
   const PackedList* list;
@@ -48,10 +50,13 @@ struct PackedWork {
 
   // Items of `heads` heads a unit in the list.
   __device__ __forceinline__ long long items(int heads) const {
-    return list ? static_cast<long long>(list->count) * heads : 0;
+    return list ? static_cast<long long>(__ldcg(&list->count)) * heads : 0;
   }
+  // WAITED: the kernel waits for the one before it.
+  template <bool WAITED = true>
   __device__ __forceinline__ PackedUnit listed(int i) const {
-    const int4 u = __ldg(reinterpret_cast<const int4*>(list + 1) + i);
+    const int4* at = reinterpret_cast<const int4*>(list + 1) + i;
+    const int4 u = WAITED ? __ldg(at) : __ldcg(at);
     return {u.x, u.y, u.z, u.w};
   }
   __device__ __forceinline__ PackedUnit direct(int i) const {
