@@ -18,7 +18,7 @@
 // Both keep P and dS in TMEM as the A operand of the products that use them.
 //
 // Measured, lists and statistics included: 12800 tokens in 8 sequences of up to 4096, 16 heads of 64, 331 us (556
-// TFLOP/s of the five products under the mask); 8192 tokens, 16 + 4 heads of 128, 765 us (900). At 128 the tensor
+// TFLOP/s of the five products under the mask); 8192 tokens, 16 + 4 heads of 128, 750 us (916). At 128 the tensor
 // pipe is 70% busy. At 64 it is 37% (dq) and 45% (dk, dv), the exponential unit 50%: a tile's products are
 // short (one of 128 x 128 x 64 takes 362 clocks in a row of them, 768 with its barrier waited for), and what is left
 // is the way from issue to barrier, 450 clocks each, which tiles in turn hide in part. dP in two buffers, dS in columns of its own and a
