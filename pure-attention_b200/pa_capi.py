@@ -479,6 +479,13 @@ def _layouts(*tensors):
     return tuple([None if t is None else (t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors])
 
 
+def _int32(fn, name, n):
+    """A descriptor's field is an int32, and ctypes would drop what lies above."""
+    if n > 0x7fffffff:
+        raise ValueError(f"{fn}: {name} is {n}, past the 2^31 - 1 that a descriptor holds")
+    return n
+
+
 def _token_stride(fn, name, t, heads, D, dev, dtype, tokens):
     """Values from one token of t [..., heads, D] to the next: a tensor of its own, or a slice of
     a wider one whose tokens are evenly spaced."""
@@ -498,7 +505,7 @@ def _token_stride(fn, name, t, heads, D, dev, dtype, tokens):
             step, rows = (d, n) if step is None else (step, rows * n)
     if not even or (step is not None and step < heads * D):
         raise ValueError(f"{fn}: {name} must have contiguous heads and evenly spaced tokens, not strides {st}")
-    return heads * D if step is None else step
+    return heads * D if step is None else _int32(fn, f"{name}'s stride", step)
 
 
 def _work(fn, need, workspace, like, stream):
@@ -539,9 +546,9 @@ def packed_attn_desc(q, k, v, cu_seqlens, dq=None, dk=None, dv=None, scale=0.0):
     T, H, D = q.shape
     Hk, fn, dev, t = k.shape[1], "packed_attn", q.get_device(), q.dtype
     stride = lambda name, x, heads: 0 if x is None else _token_stride(fn, name, x, heads, D, dev, t, T)  # noqa: E731
-    return PackedAttnDesc(T, cu_seqlens.numel() - 1, H, Hk, D, _dtype_code(q), float(scale), stride("q", q, H),
-                          stride("k", k, Hk), stride("v", v, Hk), stride("dq", dq, H), stride("dk", dk, Hk),
-                          stride("dv", dv, Hk))
+    return PackedAttnDesc(T, _int32(fn, "cu_seqlens' count", cu_seqlens.numel() - 1), H, Hk, D, _dtype_code(q),
+                          float(scale), stride("q", q, H), stride("k", k, Hk), stride("v", v, Hk), stride("dq", dq, H),
+                          stride("dk", dk, Hk), stride("dv", dv, Hk))
 
 
 def packed_attn_fwd_workspace_size(desc):
@@ -601,7 +608,8 @@ def paged_attn_desc(q, k_cache, page_table, scale=0.0):
     B, H, D = q.shape
     pages, size, Hk, _ = k_cache.shape
     step = _token_stride("paged_attn_step", "q", q, H, D, q.get_device(), q.dtype, B)
-    return PagedAttnDesc(B, H, Hk, D, _dtype_code(q), float(scale), size, pages, page_table.shape[1], step)
+    return PagedAttnDesc(B, H, Hk, D, _dtype_code(q), float(scale), size, pages,
+                         _int32("paged_attn_step", "page_table's width", page_table.shape[1]), step)
 
 
 def paged_attn_step_workspace_size(desc):
