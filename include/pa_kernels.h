@@ -257,6 +257,8 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
  * An infinity or NaN in a token shows in the heads of its group and its sequence:
  * in o, lse and dq from the block of 128 tokens that holds it on, so also a little
  * before it, and in dk and dv anywhere; other sequences keep their values.
+ * A score of -infinity (not NaN) counts as masked in o and lse, as in pa_paged_attn_step: a
+ * token that sees no others has o 0 and lse -infinity. The gradients of such a sequence may hold NaN.
  * A workspace (256-byte aligned) belongs to one call at a time: calls that may
  * overlap on the GPU, and graphs that may, need one each. An output or workspace
  * that shares bytes with another tensor of the call is refused (PA_ERR_SHAPE). */

@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(384, 1)
           if (!(ok = mbar_wait_warp(pv_done(t), (gt - 1) & 1, status))) break;
           tc_fence_after();
         }
-        const float neg_m = -m;
+        const float neg_m = m == -INFINITY ? 0.f : -m;  // no key so far: P is 0, not exp(-inf + inf)
         float sum = 0.f;
 #pragma unroll
         for (int c = 0; c < 8; ++c) {
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(384, 1)
       tc_fence_after();
       const int row = (t ? w.row[1] : w.row[0]) + r, head = t ? w.head[1] : w.head[0];
       const bool live = row < w.len;
-      const float inv_l = 1.f / l;
+      const float inv_l = l == 0.f ? 0.f : 1.f / l;  // (0: all its scores are -infinity)
       const size_t token = static_cast<size_t>(w.start) + row;
       bf16* oquad = O + ((token - (r & 3)) * H + head) * D;
 #pragma unroll
