@@ -1,12 +1,14 @@
 """Causal attention and head norms where they can go wrong beyond their own files' cases: scores of
--infinity."""
+-infinity, more items than SMs in every form, thousands of sequences, workspaces that are used again at once,
+streams given by handle, gradients of a whole training batch."""
 import math
 
 import pytest
 
 torch = pytest.importorskip("torch")
 import causal_ref as ref  # noqa: E402
-from test_packed_attention_gpu import _fwd, _inputs, _near  # noqa: E402
+from seq_ref import turn  # noqa: E402
+from test_packed_attention_gpu import _bwd, _fwd, _inputs, _near, _normal  # noqa: E402
 from test_paged_attention_gpu import _cache, _query, _step  # noqa: E402
 
 BF16, F32 = torch.bfloat16, torch.float32
@@ -111,3 +113,147 @@ def test_paged_scores_of_minus_infinity_are_as_if_masked(dtype):
             assert ((lse[b].double() - wl).abs() <= 2.0 ** -16 * (1 + wl.abs())).all()
         else:
             assert (o[b] == 0).all() and (lse[b] == -torch.inf).all()
+
+
+def _check_all(q, k, v, cu, lens, seed):
+    dO = _normal(torch.Generator(device="cuda").manual_seed(seed), *q.shape)
+    o, lse = _fwd(q, k, v, cu)
+    (want, bound), (wl, bl) = ref.packed(q, k, v, lens, 0)
+    _near(o, want, bound)
+    _near(lse, wl, bl, 2.0 ** -22)
+    for x, (w, b) in zip(_bwd(q, k, v, cu, dO, o=o, lse=lse), ref.packed(q, k, v, lens, 0, dO, o)):
+        _near(x, w, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H, Hk, D", [(32, 4, 64), (32, 4, 128), (64, 16, 64), (64, 16, 128), (48, 24, 128), (36, 12, 128)])
+def test_several_items_a_block_in_groups(H, Hk, D):
+    """Items of two heads of a group (even groups) and of one, forward and gradients, more than the SMs: at
+    4 heads of k in forward and dq only, at 12 to 24 in dk and dv too."""
+    lens = [300, 0, 77, 640, 129, 512, 33, 255, 1, 128]
+    q, k, v, cu = _inputs(lens, H, Hk, D, 34, fused=True)
+    _check_all(q, k, v, cu, lens, 35)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_thousands_of_sequences(D):
+    """More than the threads that lay out the list of work: each takes a run of them, some empty."""
+    lens = [3, 0, 1, 7, 2] * 250 + [300, 0, 130] + [0] * 900 + [5, 1] * 40
+    assert len(lens) > 2048
+    q, k, v, cu = _inputs(lens, 2, 1, D, 36)
+    _check_all(q, k, v, cu, lens, 37)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_a_workspace_used_again_at_once(D):
+    """Calls of other lengths follow each other on one stream with the same workspaces: each sees its own list of
+    work and its own statistics."""
+    import pa_capi
+    T, H, Hk = 2400, 8, 4
+    sets = []
+    for i, lens in enumerate(([2400], [100] * 24, [1, 2399], [700, 0, 1000, 700], [5] * 480, [0] * 20 + [1200, 1200])):
+        q, k, v, cu = _inputs(lens, H, Hk, D, 38 + i)
+        dO = _normal(torch.Generator(device="cuda").manual_seed(50 + i), *q.shape)
+        cu = torch.nn.functional.pad(cu, (0, 481 - cu.numel()), value=T)  # empty sequences behind: one size of workspace
+        o, lse = _fwd(q, k, v, cu)
+        sets.append((q, k, v, cu, dO, o, lse, _bwd(q, k, v, cu, dO, o=o, lse=lse)))
+    d = pa_capi.packed_attn_desc(*sets[0][:4])
+    wf, wb = (torch.empty(f(d), dtype=torch.uint8, device="cuda") for f in
+              (pa_capi.packed_attn_fwd_workspace_size, pa_capi.packed_attn_bwd_workspace_size))
+    got = [[torch.empty_like(x) for x in (s[5], s[6], *s[7])] for s in sets * 4]
+    torch.cuda.synchronize()
+    for (q, k, v, cu, dO, o, lse, _), out in zip(sets * 4, got):
+        pa_capi.packed_attn_fwd(q, k, v, cu, out[0], out[1], workspace=wf)
+        pa_capi.packed_attn_bwd(q, k, v, o, dO, lse, cu, *out[2:], workspace=wb)
+    for s, out in zip(sets * 4, got):
+        for x, w in zip(out, (s[5], s[6], *s[7])):
+            assert torch.equal(x, w)
+
+
+@pytest.mark.gpu
+def test_calls_on_a_stream_given_by_its_handle():
+    """Each operator with the handle of another stream than the current one, and with the default stream's: what it
+    reads was written there, and its result is that of the current stream."""
+    import pa_capi as pa
+    q, k, v, cu = _inputs([500, 31], 8, 2, 64, 60)
+    T, g = q.shape[0], torch.Generator(device="cuda").manual_seed(61)
+    dO = _normal(g, *q.shape)
+    kc, vc, table = _cache([300, 900], 16, 2, 64, BF16, 62)
+    q1, lens = _query(2, 8, 64, BF16, 63), torch.tensor([300, 900], dtype=torch.int32, device="cuda")
+    x, y, z = (t.view(1, T, -1, 64) for t in (q, k, v))
+    pos, gamma = torch.arange(T, device="cuda", dtype=torch.int32).view(1, 1, T), torch.rand(64, generator=g, device="cuda")
+    slots = torch.randperm(600, generator=g, device="cuda")[:T].to(torch.int32).view(1, T)
+    desc = pa.rope_desc(x, y)
+    ins = {n: t.contiguous() for n, t in dict(q=q, k=k, v=v, dO=dO, kc=kc, vc=vc, q1=q1).items()}
+    o, lse = _fwd(q, k, v, cu)
+
+    def calls(i, **kw):
+        x, y, z = (i[n].view(1, T, -1, 64) for n in "qkv")
+        return {
+            "packed": ((o, lse), lambda a, b: pa.packed_attn_fwd(i["q"], i["k"], i["v"], cu, a, b, **kw)),
+            "packed gradient": ((q, k, v), lambda *a: pa.packed_attn_bwd(i["q"], i["k"], i["v"], o, i["dO"], lse, cu, *a,
+                                                                        **kw)),
+            "paged": ((q1, lse[:, :2].t().contiguous()), lambda a, b: pa.paged_attn_step(
+                i["q1"], i["kc"], i["vc"], table, lens, a, b, **kw)),
+            "norm": ((x, y), lambda a, b: pa.qk_norm_rope_fwd(x, y, gamma, gamma, pos, a, b, desc, **kw)),
+            "norm to cache": ((x, kc, vc), lambda a, b, c: pa.qk_norm_rope_cache(x, y, z, gamma, gamma, pos, slots, a, b, c,
+                                                                                desc, **kw)),
+            "norm gradient": ((x, y, gamma, gamma), lambda *a: pa.qk_norm_rope_bwd(
+                i["dO"].view(1, T, -1, 64), y, x, y, gamma, gamma, pos, *a, desc, **kw)),
+        }
+
+    side = torch.cuda.Stream()
+    for name, (like, call) in calls(ins).items():
+        want = [torch.zeros_like(t) for t in like]
+        call(*want)
+        for handle in (side, torch.cuda.default_stream()):
+            late = {n: torch.zeros_like(t) for n, t in ins.items()}
+            got = [torch.zeros_like(t) for t in like]
+            other = torch.cuda.Stream()  # the current stream of the call, on which nothing is waited for
+            torch.cuda.synchronize()
+            with torch.cuda.stream(handle):
+                torch.cuda._sleep(2_000_000)  # about a millisecond
+                for n, t in ins.items():
+                    late[n].copy_(t)
+            with torch.cuda.stream(other):
+                calls(late, stream=handle.cuda_stream)[name][1](*got)
+            torch.cuda.synchronize()
+            for a, b in zip(got, want):
+                assert torch.equal(a, b), (name, handle)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, B, L", [(BF16, 8, 4096), (F32, 4, 4096)])
+def test_norm_gradients_of_a_training_batch(dtype, B, L):
+    """32768 tokens of 16 + 2 heads of 128. dgamma: a thread adds at most 16 tiles x 8 heads, a block 32 threads, a sum
+    10 blocks and 32 parts: chains of 202 terms, 202 2^-24 < 2^-16 of the magnitudes, with 2^-18 of each term
+    as for dx; together below the 2^-15 of the smaller cases."""
+    import pa_capi
+    H, Hk, D, eps = 16, 2, 128, 1e-6
+    g = torch.Generator(device="cuda").manual_seed(70)
+    normal = lambda *s: torch.randn(*s, generator=g, device="cuda")  # noqa: E731
+    q, k, _ = (p.unflatten(-1, (n, D)) for p, n in zip(
+        normal(B, L, (H + 2 * Hk) * D).to(dtype).split([H * D, Hk * D, Hk * D], -1), (H, Hk, Hk)))
+    gq, gk = 1 + 0.3 * normal(D), 1 + 0.3 * normal(D)
+    dqo, dko = normal(B, L, H, D).to(dtype), normal(B, L, Hk, D).to(dtype)
+    pos = torch.randint(0, 100000, (1, B, L), generator=g, device="cuda", dtype=torch.int32)
+    dq, dk, dgq, dgk = (torch.empty(x.shape, dtype=x.dtype, device="cuda") for x in (q, k, gq, gk))
+    pa_capi.qk_norm_rope_bwd(dqo, dko, q, k, gq, gk, pos, dq, dk, dgq, dgk, pa_capi.rope_desc(q, k), eps)
+    step = {BF16: 2.0 ** -8, F32: 2.0 ** -24}[dtype]
+    for x, gamma, dy, dx, dg in ((q, gq, dqo, dq, dgq), (k, gk, dko, dk, dgk)):
+        wg, mg = torch.zeros(D, dtype=torch.float64, device="cuda"), torch.zeros(D, dtype=torch.float64, device="cuda")
+        for b in range(B):
+            xb, db, gd = x[b:b + 1].double(), dy[b:b + 1].double(), gamma.double()
+            dn = turn(db, pos[:, b:b + 1], [D // 2], inverse=True)
+            m = db.abs()
+            mag = (m[..., :D // 2] + m[..., D // 2:]).repeat(1, 1, 1, 2)
+            r = (xb.square().mean(-1, keepdim=True) + eps).rsqrt()
+            u, mu = dn * gd, mag * gd.abs()
+            want = r * (u - xb * r ** 2 * (u * xb).mean(-1, keepdim=True))
+            bound = r * (mu + xb.abs() * r ** 2 * (mu * xb.abs()).mean(-1, keepdim=True))
+            _near(dx[b:b + 1], want, 2.0 ** -18 * bound, step)
+            wg += (dn * xb * r).sum((0, 1, 2))
+            mg += (mag * xb.abs() * r).sum((0, 1, 2))
+        _near(dg, wg, 2.0 ** -15 * mg, 2.0 ** -22)
