@@ -256,8 +256,8 @@ __global__ void __launch_bounds__(384, 1)
       tma_prefetch_desc(&mapV);
       bool ok = true;
       PackedUnit unit = unit_of(0);
-      int it = 0, g = 0;
-      for (; ok && unit.work; ++it) {
+      int it = 0, g = 0;  // items, key tiles sent for
+      while (ok && unit.work) {
         const PackedItem w = item_of(it, unit);
         unit = unit_of(it + 1);
         const int u = it % C::QBUF, k = it / C::QBUF;
@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(384, 1)
             for (int c = 0; c < C::KCH; ++c)
               tma_load_3d(smem_u32(sQ + u * C::Q_ITEM + t * C::TILE + c * C::CHUNK), &mapQ, q_full(u), c * 64,
                           w.head[t], w.start + w.row[t]);
+        ++it;
         for (int j = 0; j < w.n_kv; ++j, ++g) {
           const int s = g % C::STAGES;
           if (g >= C::STAGES && !(ok = mbar_wait(kv_empty(s), ((g / C::STAGES) - 1) & 1, status))) break;
@@ -280,10 +281,8 @@ __global__ void __launch_bounds__(384, 1)
           }
         }
       }
-      if (!ok) {  // copies in flight land before the block ends
-        for (int i = max(0, it - C::QBUF + 1); i <= it; ++i) mbar_drain(q_full(i % C::QBUF), (i / C::QBUF) & 1);
-        for (int i = max(0, g - C::STAGES); i < g; ++i) mbar_drain(kv_full(i % C::STAGES), (i / C::STAGES) & 1);
-      }
+      drain_ring<C::QBUF>(it, q_full);
+      drain_ring<C::STAGES>(g, kv_full);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer

@@ -286,8 +286,8 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       tma_prefetch_desc(&mapdO);
       bool ok = true;
       PackedUnit next = unit_of(0);
-      int it = 0, g = 0, nv = 0;
-      for (; ok && next.work; ++it) {
+      int it = 0, g = 0, nv = 0;  // items, tiles of K and of V sent for
+      while (ok && next.work) {
         const PackedUnit u = next;
         const int h = head_of(it), kh = h / group, row = u.start + (u.work - 1) * 128;
         next = unit_of(it + 1);
@@ -298,6 +298,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
           tma_load_3d(smem_u32(sQ + b * 2 * C::TILE + c * kChunk), &mapQ, q_full(b), c * 64, h, row);
           tma_load_3d(smem_u32(sQ + (b * 2 + 1) * C::TILE + c * kChunk), &mapdO, q_full(b), c * 64, h, row);
         }
+        ++it;
         for (int j = 0; j < u.work; ++j) {
           int s = g % C::KST;
           if (g >= C::KST && !(ok = mbar_wait(k_empty(s), ((g / C::KST) - 1) & 1, status))) break;
@@ -313,11 +314,9 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
           ++nv;
         }
       }
-      if (!ok) {  // copies in flight land before the block ends
-        for (int i = max(0, it - C::QBUF + 1); i <= it; ++i) mbar_drain(q_full(i % C::QBUF), (i / C::QBUF) & 1);
-        for (int i = max(0, g - C::KST); i < g; ++i) mbar_drain(k_full(i % C::KST), (i / C::KST) & 1);
-        for (int i = max(0, nv - C::VST); i < nv; ++i) mbar_drain(v_full(i % C::VST), (i / C::VST) & 1);
-      }
+      drain_ring<C::QBUF>(it, q_full);
+      drain_ring<C::KST>(g, k_full);
+      drain_ring<C::VST>(nv, v_full);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer
@@ -606,8 +605,8 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
       tma_prefetch_desc(&mapdO);
       bool ok = true;
       PackedUnit next = unit_of(0);
-      int it = 0, g = 0, go = 0;
-      for (; ok && next.work; ++it) {
+      int it = 0, g = 0, go = 0;  // items, tiles of Q (with their statistics) and of dO sent for
+      while (ok && next.work) {
         const PackedUnit u = next;
         const int kh = head_of(it), first = tiles_of(u) - u.work;
         next = unit_of(it + 1);
@@ -620,6 +619,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
           tma_load_3d(smem_u32(sKV + (b * 2 + 1) * C::TILE + c * kChunk), &mapV, kv_full(b), c * 64, kh,
                       u.start + first * 128);
         }
+        ++it;
         for (int h = kh * group; ok && h < (kh + 1) * group; ++h)
           for (int j = first; j < first + u.work; ++j) {
             int s = g % C::QST;
@@ -639,11 +639,9 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
             ++go;
           }
       }
-      if (!ok) {  // copies in flight land before the block ends
-        for (int i = max(0, it - C::KVBUF + 1); i <= it; ++i) mbar_drain(kv_full(i % C::KVBUF), (i / C::KVBUF) & 1);
-        for (int i = max(0, g - C::QST); i < g; ++i) mbar_drain(q_full(i % C::QST), (i / C::QST) & 1);
-        for (int i = max(0, go - C::OST); i < go; ++i) mbar_drain(o_full(i % C::OST), (i / C::OST) & 1);
-      }
+      drain_ring<C::KVBUF>(it, kv_full);
+      drain_ring<C::QST>(g, q_full);
+      drain_ring<C::OST>(go, o_full);
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer

@@ -108,6 +108,14 @@ int launch_beside(bool beside, K kernel, dim3 grid, int threads, size_t smem, cu
   return cudaLaunchKernelEx(&cfg, kernel, args...) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
+// Waits for the copies of a ring of SLOTS buffers that may still be on their way when `sent` fills were sent
+// for: the last SLOTS of them, and none that was not. full(slot) is the barrier of a slot. A block does so whatever
+// was recorded: a failure, in it or in another block and at any moment, lets the roles that would have waited leave.
+template <int SLOTS, typename F>
+__device__ __forceinline__ void drain_ring(int sent, F full) {
+  for (int i = max(0, sent - SLOTS); i < sent; ++i) mbar_drain(full(i % SLOTS), (i / SLOTS) & 1);
+}
+
 // Stores 32 columns of bf16 of a warp's 32 consecutive rows, a lane's row as four 16-byte pieces in u.
 // The lanes of a quad exchange pieces first, so that a store covers 64 bytes of 8 rows and not 16
 // of 32: the write-back of an item is bound by the lines that its stores touch. to: the columns in the
