@@ -176,7 +176,7 @@ __global__ void __launch_bounds__(384, 1)
                       float scale_log2, uint32_t* status) {
   using C = PackedFwd<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[24];
+  __shared__ uint64_t bars[23];
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(384, 1)
   auto pv_done = [&](int t) { return smem_u32(&bars[18 + t]); };
   const uint32_t v_ragged = smem_u32(&bars[20]);  // a ragged V tile has landed
   const uint32_t v_zeroed = smem_u32(&bars[21]);  // and its rows behind the end are zero
+  const uint32_t mma_done = smem_u32(&bars[22]);  // all products have ended
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -221,6 +222,7 @@ __global__ void __launch_bounds__(384, 1)
     }
     mbar_init(v_ragged, 1);
     mbar_init(v_zeroed, 1);
+    mbar_init(mma_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -371,6 +373,7 @@ __global__ void __launch_bounds__(384, 1)
           if (j + 2 == w.n_kv) umma_commit(q_empty(u));  // the item's last S products are issued
         }
       }
+      drain_products(mma_done);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ rows behind a sequence's end

@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   using C = PackedDq<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[35];
+  __shared__ uint64_t bars[36];
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -231,6 +231,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   // done, so each pair has a barrier of its own); it has been read.
   auto acc_done = [&](int pair) { return smem_u32(&bars[28 + pair]); };
   const uint32_t acc_free = smem_u32(&bars[34]);
+  const uint32_t mma_done = smem_u32(&bars[35]);  // all products have ended
   // the f-th ragged K tile has landed, and its rows behind the end are zero; two are on the way at most
   auto k_ragged = [&](int f) { return smem_u32(&bars[30 + (f & 1)]); };
   auto k_zeroed = [&](int f) { return smem_u32(&bars[32 + (f & 1)]); };
@@ -255,6 +256,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     }
     for (int u = 0; u < 2; ++u) mbar_init(acc_done(u), 1);
     mbar_init(acc_free, W::PAIR);
+    mbar_init(mma_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -390,6 +392,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
         a = b;
         b = c;
       }
+      drain_products(mma_done);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ rows behind a sequence's end
@@ -523,7 +526,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   using C = PackedDkv<D>;
   using W = BwdWarps<D>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t bars[33];
+  __shared__ uint64_t bars[34];
   __shared__ PackedUnit own;  // without a list: the CTA's only unit
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
@@ -550,6 +553,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
   auto ds_full = [&](int g) { return smem_u32(&bars[28 + (g & 1)]); };
   auto acc_done = [&](int pair) { return smem_u32(&bars[30 + pair]); };  // dv and dk are there, as for dq; were read
   const uint32_t acc_free = smem_u32(&bars[32]);
+  const uint32_t mma_done = smem_u32(&bars[33]);  // all products have ended
 
   const int warp = warp_id();
   if (threadIdx.x == 0) {
@@ -572,6 +576,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     }
     for (int u = 0; u < 2; ++u) mbar_init(acc_done(u), 1);
     mbar_init(acc_free, W::PAIR);
+    mbar_init(mma_done, 1);
     fence_mbar_init();
   }
   if (warp == 1) {
@@ -719,6 +724,7 @@ __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
         a = b;
         b = C::SBUF == 2 ? c : next_tile();
       }
+      drain_products(mma_done);
     }
   } else if (warp == 2) {
     // ------------------------------------------------------------ rows behind a sequence's end

@@ -116,6 +116,13 @@ __device__ __forceinline__ void drain_ring(int sent, F full) {
   for (int i = max(0, sent - SLOTS); i < sent; ++i) mbar_drain(full(i % SLOTS), (i / SLOTS) & 1);
 }
 
+// The same for the tensor products of the issuing thread, which read shared memory and write TMEM that the block
+// gives up at its end: `done` is a barrier for this alone.
+__device__ __forceinline__ void drain_products(uint32_t done) {
+  umma_commit(done);
+  mbar_drain(done, 0);
+}
+
 // Stores 32 columns of bf16 of a warp's 32 consecutive rows, a lane's row as four 16-byte pieces in u.
 // The lanes of a quad exchange pieces first, so that a store covers 64 bytes of 8 rows and not 16
 // of 32: the write-back of an item is bound by the lines that its stores touch. to: the columns in the

@@ -1,6 +1,6 @@
 """Causal attention and head norms where they can go wrong beyond their own files' cases: scores of
 -infinity, more items than SMs in every form, thousands of sequences, workspaces that are used again at once,
-streams given by handle, gradients of a whole training batch."""
+streams given by handle, errors recorded while kernels run, gradients of a whole training batch."""
 import math
 
 import pytest
@@ -257,3 +257,50 @@ def test_norm_gradients_of_a_training_batch(dtype, B, L):
             wg += (dn * xb * r).sum((0, 1, 2))
             mg += (mag * xb.abs() * r).sum((0, 1, 2))
         _near(dg, wg, 2.0 ** -15 * mg, 2.0 ** -22)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("backward", [False, True])
+@pytest.mark.parametrize("lens, H, Hk, D", [([12000, 1, 4000], 16, 4, 64), ([12000, 1, 4000], 16, 16, 64),
+                                            ([9000, 77, 300], 16, 4, 128), ([9000, 77, 300], 9, 9, 128)])
+def test_calls_that_a_recorded_error_interrupts(lens, H, Hk, D, backward):
+    """An error that another kernel records in the middle of a row of calls: the one that runs then ends within a
+    few milliseconds (a wait for a copy that was never sent takes 20), those behind it leave their outputs, and once
+    the error is cleared the same calls give the same bits: no copy or product of an ended block is still on its way."""
+    import pa_capi
+    q, k, v, cu = _inputs(lens, H, Hk, D, 80)
+    dO = _normal(torch.Generator(device="cuda").manual_seed(81), *q.shape)
+    o, lse = _fwd(q, k, v, cu)
+    want = _bwd(q, k, v, cu, dO, o=o, lse=lse) if backward else (o, lse)
+    outs = [[torch.full_like(x, 7.0) for x in want] for _ in range(16)]
+    assert pa_capi.device_status() == 0
+
+    def call(out):
+        if backward:
+            pa_capi.packed_attn_bwd(q, k, v, o, dO, lse, cu, *out)
+        else:
+            pa_capi.packed_attn_fwd(q, k, v, cu, *out)
+
+    call(outs[-1])  # (memory and launches are ready)
+    outs[-1] = [torch.full_like(x, 7.0) for x in want]
+    a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    side, limit = torch.cuda.Stream(), 2_000_000
+    torch.cuda.synchronize()
+    pa_capi.wait_selftest(limit, arrive=False, stream=side.cuda_stream)
+    try:
+        a.record()
+        for out in outs:
+            call(out)
+        b.record()
+        torch.cuda.synchronize()
+        assert pa_capi.device_status(clear=False) == 6  # PA_ERR_TIMEOUT
+        assert a.elapsed_time(b) < limit * 1e-6 + 12, a.elapsed_time(b)
+        assert all(torch.equal(x, y) for x, y in zip(outs[0], want))  # before it
+        assert all((x == 7).all() for x in outs[-1])                  # behind it
+    finally:
+        pa_capi.device_status(clear=True)
+    for out in outs[:4]:
+        call(out)
+    for out in outs[:4]:
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+    assert pa_capi.device_status() == 0
