@@ -237,14 +237,15 @@ __global__ void __launch_bounds__(384, 1)
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const long long n_items = work.items(n_hh);
+  const int block = static_cast<int>(blockIdx.x), blocks = static_cast<int>(gridDim.x);
   // Items in turn; the next one's unit is fetched while the current one runs.
   auto unit_of = [&](int turn) {
-    const long long i = packed_turn(turn);
+    const long long i = packed_turn(turn, block, blocks);
     if (!work.list) return turn == 0 ? own : PackedUnit{0, 0, 0, 0};
     return i < n_items ? work.listed(static_cast<int>(i / n_hh)) : PackedUnit{0, 0, 0, 0};
   };
   auto item_of = [&](int turn, const PackedUnit& u) {
-    return packed_item(u, static_cast<int>(packed_turn(turn) % n_hh), pair_heads, group);
+    return packed_item(u, static_cast<int>(packed_turn(turn, block, blocks) % n_hh), pair_heads, group);
   };
 
   // Counters that run over all items: it, items; g, key tiles (ring slot and its

@@ -39,9 +39,7 @@ __device__ __forceinline__ int packed_seq(const int32_t* cu, int i, int T, int& 
   return max(before, min(__ldcg(cu + i + 1), T)) - before;
 }
 
-// Where a kernel has its units from: the list, or (NULL) the lengths. The kernel of dk and dv, which does not wait for
-// the kernel before it, reads past its SM's own cache, where an older list may still be (in all kernels that cost up
-// to 1%).
+// Where a kernel has its units from: the list, or (NULL) the lengths.
 constexpr int kDirectSeqs = 16;
 struct PackedWork {
   const PackedList* list;
@@ -50,13 +48,10 @@ struct PackedWork {
 
   // Items of `heads` heads a unit in the list.
   __device__ __forceinline__ long long items(int heads) const {
-    return list ? static_cast<long long>(__ldcg(&list->count)) * heads : 0;
+    return list ? static_cast<long long>(load_written(&list->count)) * heads : 0;
   }
-  // WAITED: the kernel waits for the one before it.
-  template <bool WAITED = true>
   __device__ __forceinline__ PackedUnit listed(int i) const {
-    const int4* at = reinterpret_cast<const int4*>(list + 1) + i;
-    const int4 u = WAITED ? __ldg(at) : __ldcg(at);
+    const int4 u = load_written(reinterpret_cast<const int4*>(list + 1) + i);
     return {u.x, u.y, u.z, u.w};
   }
   __device__ __forceinline__ PackedUnit direct(int i) const {
@@ -76,10 +71,9 @@ inline int packed_work(PackedWork* w, const PackedShape& sh, const int32_t* cu, 
   *w = {direct ? nullptr : static_cast<const PackedList*>(ws), cu, sh.n, sh.T, unit};
   return direct ? PA_OK : launch_packed_list(sh, cu, unit, ws, s);
 }
-// Item of a CTA's turn.
-__device__ __forceinline__ long long packed_turn(int turn) {
-  const int c = (turn & 1) ? static_cast<int>(gridDim.x - 1 - blockIdx.x) : static_cast<int>(blockIdx.x);
-  return static_cast<long long>(turn) * gridDim.x + c;
+// Item of a CTA's turn, CTA `block` of the `blocks` that share the work out.
+__device__ __forceinline__ long long packed_turn(int turn, int block, int blocks) {
+  return static_cast<long long>(turn) * blocks + ((turn & 1) ? blocks - 1 - block : block);
 }
 
 // 3-D TMA map over [T, H, D] bf16 with `stride` values from token to token: box of 64 columns x 1

@@ -231,6 +231,22 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 // one waits where it needs the first one's results (at once, if it was launched without).
 __device__ __forceinline__ void launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void wait_prerequisites() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Loads of what a kernel before this one may write while this one already runs, behind wait_prerequisites: coherent
+// loads, not those for memory that stays as it is for a kernel's whole life, and volatile, so that the compiler moves none
+// before that wait.
+__device__ __forceinline__ int load_written(const int* p) {
+  int v;
+  asm volatile("ld.global.s32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
+  return v;
+}
+__device__ __forceinline__ int4 load_written(const int4* p) {
+  int4 v;
+  asm volatile("ld.global.v4.s32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
 
 // ---------------------------------------------------------------- TMA
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
