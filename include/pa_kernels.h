@@ -253,7 +253,8 @@ int pa_linear_attn_step(const pa_attn_desc* desc, const void* q, const void* k, 
  * nor written. Entries of cu_seqlens outside 0 .. tokens, or that descend, are
  * taken as clamped to the entry before and to tokens: nothing is read or written out of
  * bounds, but sequences that overlap give no defined result.
- * bf16: head_dim 64 or 128. Results do not depend on the run: each sum has one order.
+ * bf16: head_dim 64 or 128. Sums are fp32; the weights P, up to 2^8 times their row's largest before the division,
+ * and dS are rounded to bf16 as operands of their products. Results do not depend on the run: each sum has one order.
  * An infinity or NaN in a token shows in the heads of its group and its sequence:
  * in o, lse and dq from the block of 128 tokens that holds it on, so also a little
  * before it, and in dk and dv anywhere; other sequences keep their values.
@@ -300,7 +301,7 @@ int pa_packed_attn_bwd(const pa_packed_attn_desc* desc, const void* q, const voi
  * of 0), o is 0 and lse -infinity.
  * q and o [batch, num_heads, head_dim] (q_stride values from one sequence's q
  * to the next), lse [batch, num_heads] fp32 or NULL. bf16: head_dim 64 or 128;
- * fp32: 32 or 64, in fp32 arithmetic under either f32 math mode. Any page_size,
+ * fp32: 32 or 64, in fp32 arithmetic under either f32 math mode; in bf16 P is rounded as in pa_packed_attn_fwd. Any page_size,
  * any group num_heads / num_kv_heads. Results do not depend on the run.
  * Workspace and outputs as for pa_packed_attn_fwd. */
 typedef struct pa_paged_attn_desc {
@@ -332,7 +333,9 @@ int pa_paged_attn_step(const pa_paged_attn_desc* desc, const void* q, const void
  * projection's output. Outputs are contiguous [B, L, heads, D], but for dq and
  * dk, which have strides of their own. An output that shares bytes with another tensor
  * of the call is refused (PA_ERR_SHAPE), but q_out may be q and k_out k where
- * those are contiguous. */
+ * those are contiguous. Squares are summed in fp32: a head whose sum passes fp32's range is normed to zeros. Turned
+ * pairs that are no whole vectors of 16 bytes (halves: not a multiple of 8 of them, pairs: of 4; fp32: of 4, of 2) move
+ * value by value, some 10 times slower. */
 typedef struct pa_qk_norm_desc {
   pa_rope_desc rope;
   float eps;            /* >= 0 */

@@ -17,13 +17,15 @@
 //                        the diagonal on for each head of the group; rows are keys
 // Both keep P and dS in TMEM as the A operand of the products that use them.
 //
-// Measured, lists and statistics included: 12800 tokens in 8 sequences of up to 4096, 16 heads of 64, 331 us (556
-// TFLOP/s of the five products under the mask); 8192 tokens, 16 + 4 heads of 128, 750 us (916). At 128 the tensor
+// Measured, lists and statistics included: 12800 tokens in 8 sequences of up to 4096, 16 heads of 64, 332 us (553
+// TFLOP/s of the five products under the mask); 8192 tokens, 16 + 4 heads of 128, 739 us (930). At 128 the tensor
 // pipe is 70% busy. At 64 it is 37% (dq) and 45% (dk, dv), the exponential unit 50%: a tile's products are
-// short (one of 128 x 128 x 64 takes 362 clocks in a row of them, 768 with its barrier waited for), and what is left
-// is the way from issue to barrier, 450 clocks each, which tiles in turn hide in part. dP in two buffers, dS in columns of its own and a
+// short (one of 128 x 128 x 64 takes 362 clocks in a row of them, 768 with its barrier waited for), and each waits 450
+// clocks from issue to barrier, which tiles in turn hide in part. dP in two buffers, dS in columns of its own and a
 // second issuing warp, which take those waits out of the chain one by one, were not faster (dq 153 to 155 us; dk
-// and dv with P^T in shared memory for the room 178 to 236 us).
+// and dv with P^T in shared memory for the room 178 to 236 us; dq and dk / dv measured as launches of their own). One pass
+// over the keys with five products, as attn_bwd.cu has for lengths that are all alike (905 TFLOP/s without a mask), was
+// not tried: it adds dq up in memory, in an order that would have to be fixed for results that do not depend on the run.
 #include <cuda_bf16.h>
 #include <type_traits>
 #include "packed_common.cuh"

@@ -39,7 +39,10 @@ __device__ __forceinline__ int packed_seq(const int32_t* cu, int i, int T, int& 
   return max(before, min(__ldcg(cu + i + 1), T)) - before;
 }
 
-// Where a kernel has its units from: the list, or (NULL) the lengths.
+// Where a kernel has its units from: the list, or (NULL) the lengths, which every kernel then walks by itself. Sequences of
+// 10 tokens, 2 + 1 heads of 64, us on the GPU without and with the list: 4 of them 7.7 and 9.6 forward, 11.4 and 14.6
+// gradients; 8 8.4 and 9.8, 13.1 and 14.7; 16 10.0 and 9.9, 16.5 and 14.6; 32 13.5 and 10.2, 23.1 and 15.4. So the list
+// pays from 16 on forward, and for gradients a few sequences sooner.
 constexpr int kDirectSeqs = 16;
 struct PackedWork {
   const PackedList* list;

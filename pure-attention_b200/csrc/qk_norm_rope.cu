@@ -14,7 +14,9 @@
 // 16 bytes of a head a lane (conversions, squares, shuffles, two products a value), 53% of the issue slots. 8 x
 // 4096 tokens of 16 + 2 heads of 128 in bf16: 76 us (4.0 TB/s of 6.55 a plain copy; the rotation alone 66), the
 // gradient 148 us (3.1 TB/s), in fp32 168 us (5.4). Slower, 89 to 122 us: inputs through a ring of bulk copies or of
-// cp.async, packed pairs of fp32, vectors of 8 bytes, fewer heads in flight with more blocks.
+// cp.async, packed pairs of fp32, vectors of 8 bytes, fewer heads in flight with more blocks. Where the turned pairs are
+// no whole vectors of 16 bytes (halves: a number of pairs that 8, in fp32 4, does not divide) values move one by one: the
+// same batch with heads of 80, 24 pairs turned 71 us and the gradient 136, 20 pairs 836 and 966.
 #include <cmath>
 #include <cstring>
 #include <type_traits>
