@@ -301,7 +301,8 @@ int pa_packed_attn_bwd(const pa_packed_attn_desc* desc, const void* q, const voi
  * of 0), o is 0 and lse -infinity.
  * q and o [batch, num_heads, head_dim] (q_stride values from one sequence's q
  * to the next), lse [batch, num_heads] fp32 or NULL. bf16: head_dim 64 or 128;
- * fp32: 32 or 64, in fp32 arithmetic under either f32 math mode; in bf16 P is rounded as in pa_packed_attn_fwd. Any page_size,
+ * fp32: 32 or 64, in fp32 arithmetic under either f32 math mode; in bf16 P is rounded
+ * as in pa_packed_attn_fwd. Any page_size,
  * any group num_heads / num_kv_heads. Results do not depend on the run.
  * Workspace and outputs as for pa_packed_attn_fwd. */
 typedef struct pa_paged_attn_desc {

@@ -863,9 +863,9 @@ __device__ __forceinline__ void packed_dkv(const BwdMaps& maps, bf16* __restrict
 }
 
 // One launch for both: an SM takes a block of dk and dv as soon as its block of dq ends, and each waits for the
-// statistics by itself. As two launches, the second waiting for all of the first, 100 tokens of 8 + 2 heads of 64 take 19.3 us on the
-// GPU instead of 13.4, 8192 tokens of 16 + 4 heads of 128 878 instead of 842 as called, 12800 tokens of 16 heads of 64 355 instead of
-// 350.
+// statistics by itself. As two launches, the second waiting for all of the first: 100 tokens of 8 + 2 heads of 64 19.3 us
+// on the GPU instead of 13.4; as called 8192 tokens of 16 + 4 heads of 128 878 instead of 842, 12800 tokens of 16
+// heads of 64 355 instead of 350.
 template <int D>
 __global__ void __launch_bounds__(BwdWarps<D>::THREADS, 1)
     packed_bwd_kernel(const __grid_constant__ BwdMaps maps, bf16* __restrict__ dq, bf16* __restrict__ dk,
